@@ -31,6 +31,8 @@ from .functional import (  # noqa: F401
 )
 from . import planes  # noqa: F401
 from .ssimulacra2 import SSIMULACRA2, ssimulacra2  # noqa: F401
+from .attention import qk_norm_rotary  # noqa: F401
+from .optim import Muon, muon_step, orthogonalize  # noqa: F401
 from .modules import (GMSD, L1, MSE, MSSSIM, PSNR, SSIM, Charbonnier, Huber,  # noqa: F401
                       StreamingMetrics)
 
@@ -42,6 +44,7 @@ __all__ = [
     "set_fused_loss_grad", "metrics", "StreamingMetrics",
     "MSE", "PSNR", "SSIM", "MSSSIM", "GMSD", "L1", "Charbonnier", "Huber",
     "ssimulacra2", "SSIMULACRA2", "backend_status",
+    "qk_norm_rotary", "orthogonalize", "muon_step", "Muon",
 ]
 
 

@@ -22,7 +22,7 @@ LIBDIR = HERE / "_lib"
 LIB = LIBDIR / "libfa_b200.so"
 SOURCES = ["abi.cu", "pixel.cu", "ssim_fwd.cu", "ssim_bwd.cu", "gmsd.cu", "pool.cu", "grad_scale.cu",
            "ssim_compat.cu", "f64.cu",
-           "ssimulacra2.cu"]
+           "ssimulacra2.cu", "qk_rotary.cu", "orthogonalize.cu", "abi_train.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

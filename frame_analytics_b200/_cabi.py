@@ -60,12 +60,61 @@ class fa_view(ctypes.Structure):
     ]
 
 
+class fa_heads(ctypes.Structure):
+    """Mirror of ``struct fa_heads`` in include/fa_b200.h."""
+
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("heads", ctypes.c_int32),
+        ("pad_", ctypes.c_int32),
+        ("stride_b", ctypes.c_int64),
+        ("stride_l", ctypes.c_int64),
+        ("stride_h", ctypes.c_int64),
+    ]
+
+
+class fa_qk_params(ctypes.Structure):
+    """Mirror of ``struct fa_qk_params`` in include/fa_b200.h."""
+
+    _fields_ = [
+        *[(name, ctypes.c_int32) for name in
+          ("dtype", "weight_dtype", "batch", "length", "dim", "rotary", "interleaved",
+           "weight_per_head", "table", "positions_64")],
+        ("cos_table", ctypes.c_void_p),
+        ("sin_table", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("pos_stride_b", ctypes.c_int64),
+        ("pos_stride_l", ctypes.c_int64),
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("eps", ctypes.c_double),
+    ]
+
+
+class fa_matrix(ctypes.Structure):
+    """Mirror of ``struct fa_matrix`` in include/fa_b200.h."""
+
+    _fields_ = [
+        ("src", ctypes.c_void_p),
+        ("dst", ctypes.c_void_p),
+        ("momentum", ctypes.c_void_p),
+        ("rows", ctypes.c_int32),
+        ("cols", ctypes.c_int32),
+        ("src_row_stride", ctypes.c_int64),
+        ("dst_row_stride", ctypes.c_int64),
+        ("step", ctypes.c_double),
+    ]
+
+
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _d = ctypes.c_double
 _sz = ctypes.c_size_t
 _pview = ctypes.POINTER(fa_view)
+_ph = ctypes.POINTER(fa_heads)
+_pq = ctypes.POINTER(fa_qk_params)
+_pm = ctypes.POINTER(fa_matrix)
 
 # name -> argtypes (restype int unless listed in _RESTYPE)
 PROTOTYPES = {
@@ -134,6 +183,13 @@ PROTOTYPES = {
     "fa_b200_gmsd64": [_pview, _pview, _vp, _d, _d, _i, _vp, _sz, _vp, _vp, _vp, _i, _vp],
     "fa_b200_gmsd64_backward": [_vp, _vp, _i, _i, _i, _i, _i, _d, _d, _vp, _vp, _vp, _vp, _vp,
                                 _vp, _vp, _i, _vp],
+    "fa_b200_qk_norm_rotary": [_ph, _ph, _ph, _ph, _pq, _i, _vp],
+    "fa_b200_qk_norm_rotary_backward_workspace_bytes": [_i, _i, _i, _i, _i, _vp],
+    "fa_b200_qk_norm_rotary_backward": [_ph, _ph, _ph, _ph, _ph, _ph, _pq, _vp, _vp, _vp, _sz,
+                                        _i, _vp],
+    "fa_b200_orthogonalize_workspace_bytes": [_pm, _i, _i, _vp],
+    "fa_b200_orthogonalize": [_pm, _i, _i, _vp, _i, _vp, _sz, _i, _vp],
+    "fa_b200_muon_step": [_pm, _i, _i, _vp, _i, _d, _i, _d, _vp, _sz, _i, _vp],
     "fa_b200_ssim_gmsd": [_pview, _pview, _vp, _i, _d, _d, _d, _d, _d, _d, _vp, _sz,
                           _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp],
 }

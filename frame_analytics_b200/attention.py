@@ -1,0 +1,199 @@
+"""Attention operands: the norm of query and key heads with the rotation by
+position, in one pass (no counterpart in the reference; ``csrc/qk_rotary.cu``).
+
+A network trained against the package's losses normalises its queries and keys
+so that attention logits stay bounded under orthogonalised updates
+(:class:`frame_analytics_b200.Muon`), and rotates them by token position.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import backend
+from ._cabi import fa_heads, fa_qk_params
+from .functional import _reject_double_backward
+
+__all__ = ["qk_norm_rotary"]
+
+_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+_MAX_DIM = 512
+
+
+def _heads(t: torch.Tensor) -> fa_heads:
+    b, l, h, _ = t.stride()
+    return fa_heads(t.data_ptr(), t.shape[2], 0, b, l, h)
+
+
+def _params(q, cos, sin, q_weight, k_weight, eps, positions, interleaved) -> fa_qk_params:
+    w = q_weight if q_weight is not None else k_weight
+    code = backend.DTYPE_CODE[q.dtype]
+    p = fa_qk_params(code, code if w is None else backend.DTYPE_CODE[w.dtype],
+                     q.shape[0], q.shape[1], q.shape[3], 0, interleaved,
+                     w is not None and w.dim() == 2)
+    if cos is not None:
+        p.rotary, p.table = 2 * cos.shape[1], cos.shape[0]
+        p.cos_table, p.sin_table = cos.data_ptr(), sin.data_ptr()
+    if positions is not None:
+        p.positions, p.positions_64 = positions.data_ptr(), positions.dtype == torch.int64
+        p.pos_stride_l = positions.stride(-1)
+        p.pos_stride_b = positions.stride(0) if positions.dim() == 2 else 0
+    p.q_weight, p.k_weight = backend._ptr(q_weight), backend._ptr(k_weight)
+    p.eps = eps
+    return p
+
+
+def _forward(q, k, q_out, k_out, *rest):
+    p = _params(q, *rest)
+    backend._call(q, backend.lib().fa_b200_qk_norm_rotary, _heads(q), _heads(k), _heads(q_out),
+                  _heads(k_out), p, backend._dev(q), backend._stream(q))
+
+
+class _QkNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, eps, positions, interleaved):
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        _forward(q, k, q_out, k_out, cos, sin, q_weight, k_weight, eps, positions, interleaved)
+        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
+        ctx.eps, ctx.interleaved = eps, interleaved
+        return q_out, k_out
+
+    @staticmethod
+    def backward(ctx, gq, gk):
+        _reject_double_backward()
+        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
+        p = _params(q, cos, sin, q_weight, k_weight, ctx.eps, positions, ctx.interleaved)
+        gq = gq if gq.stride(-1) == 1 else gq.contiguous()
+        gk = gk if gk.stride(-1) == 1 else gk.contiguous()
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        need = ctx.needs_input_grad
+        dqw = torch.empty_like(q_weight) if q_weight is not None and need[2] else None
+        dkw = torch.empty_like(k_weight) if k_weight is not None and need[3] else None
+        L = backend.lib()
+        nb = backend._cached_ws("qk", L.fa_b200_qk_norm_rotary_backward_workspace_bytes,
+                                q.shape[0], q.shape[1], q.shape[2], k.shape[2], q.shape[3])
+        ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
+        backend._call(q, L.fa_b200_qk_norm_rotary_backward, _heads(q), _heads(k), _heads(gq),
+                      _heads(gk), _heads(dq), _heads(dk), p, backend._ptr(dqw),
+                      backend._ptr(dkw), ws.data_ptr(), nb, backend._dev(q), backend._stream(q))
+        return dq, dk, dqw, dkw, None, None, None, None, None
+
+
+def _check_weight(name, w, x, other):
+    if w is None:
+        return
+    if w.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"{name} must be {x.dtype} or float32, got {w.dtype}")
+    if tuple(w.shape) not in ((x.shape[3],), (x.shape[2], x.shape[3])):
+        raise ValueError(f"{name} must have shape ({x.shape[3]},) or "
+                         f"({x.shape[2]}, {x.shape[3]}), got {tuple(w.shape)}")
+    if other is not None and (other.dtype != w.dtype or other.dim() != w.dim()):
+        raise ValueError("q_weight and k_weight must have one dtype and one number of dimensions")
+
+
+def _check_out(name, o, x):
+    if not torch.is_tensor(o) or o.shape != x.shape or o.dtype != x.dtype or o.device != x.device:
+        raise ValueError(f"{name} must be a {x.dtype} tensor of shape {tuple(x.shape)} on {x.device}")
+    if o.stride(-1) != 1 and o.shape[-1] != 1:
+        raise ValueError(f"{name} must have unit stride in its last dimension")
+    if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())):
+        raise ValueError(f"{name} has elements that share memory")
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] = None,
+                   sin: Optional[torch.Tensor] = None, *,
+                   q_weight: Optional[torch.Tensor] = None,
+                   k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                   positions: Optional[torch.Tensor] = None, interleaved: bool = False,
+                   out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+                   ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Normalise every query and key head and rotate it by its token's position:
+    ``y = R_p (w * x / sqrt(mean(x**2) + eps))``.  Differentiable in the
+    operands and the weights.
+
+    ``q`` (B, L, Hq, D) and ``k`` (B, L, Hk, D), float16 / bfloat16 / float32,
+    may be views of a packed projection (any strides with unit stride in D; D
+    at most 512).  ``cos`` / ``sin``: float32 (P, R/2) tables; the first
+    ``R <= D`` components turn, in pairs (i, i + R/2), or (2i, 2i + 1) with
+    ``interleaved``.  ``positions``: int32 / int64 (L,) or (B, L) rows of the
+    tables, by default 0..L-1; a position outside the tables gives NaN for its
+    token.  Weights: (D,) shared by the heads, or (heads, D); in the operands'
+    dtype or float32.
+
+    Returns contiguous (B, L, Hq, D) and (B, L, Hk, D).  ``out=(q_out, k_out)``
+    writes there instead (any strides with unit stride in D: a slice of a cache,
+    or the inputs themselves); it takes no part in autograd."""
+    for name, t in (("q", q), ("k", k)):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be (B, L, heads, D), got shape {tuple(t.shape)}")
+        if t.dtype not in _DTYPES:
+            raise TypeError(f"{name} must be float16, bfloat16 or float32, got {t.dtype}")
+    if q.dtype != k.dtype or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} differ in "
+                         "batch, length, head size or dtype")
+    dim = q.shape[3]
+    if dim > _MAX_DIM or dim < 1:
+        raise ValueError(f"the head size must be 1..{_MAX_DIM}, got {dim}")
+    if q.shape[2] < 1 or k.shape[2] < 1:
+        raise ValueError("q and k need at least one head each")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 \
+                or sin.dtype != torch.float32:
+            raise ValueError("cos and sin must be float32 tables of one shape (P, R/2)")
+        if not 2 <= 2 * cos.shape[1] <= dim:
+            raise ValueError(f"the tables rotate {2 * cos.shape[1]} of {dim} components")
+    if positions is not None:
+        if cos is None:
+            raise ValueError("positions need cos and sin")
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+        if tuple(positions.shape) not in ((q.shape[1],), (q.shape[0], q.shape[1])):
+            raise ValueError(f"positions must be ({q.shape[1]},) or ({q.shape[0]}, {q.shape[1]}), "
+                             f"got {tuple(positions.shape)}")
+    elif cos is not None and q.shape[1] > cos.shape[0]:
+        raise ValueError(f"{q.shape[1]} tokens for tables of {cos.shape[0]} positions")
+    if not (eps >= 0.0):
+        raise ValueError(f"eps must not be negative, got {eps}")
+    _check_weight("q_weight", q_weight, q, k_weight)
+    _check_weight("k_weight", k_weight, k, q_weight)
+    given = [t for t in (q, k, cos, sin, q_weight, k_weight, positions) if t is not None]
+    backend.require_cuda(*given)
+    if any(t.device != q.device for t in given):
+        raise ValueError("all tensors must be on one device")
+    grad = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
+    if out is not None:
+        if grad:
+            raise ValueError("out= takes no part in autograd; call under torch.no_grad()")
+        if not isinstance(out, (tuple, list)) or len(out) != 2:
+            raise ValueError("out must be a pair (q_out, k_out)")
+        _check_out("out[0]", out[0], q)
+        _check_out("out[1]", out[1], k)
+    q = q if q.stride(-1) == 1 else q.contiguous()
+    k = k if k.stride(-1) == 1 else k.contiguous()
+    if cos is not None:
+        cos, sin = cos.contiguous(), sin.contiguous()
+    q_weight = None if q_weight is None else q_weight.contiguous()
+    k_weight = None if k_weight is None else k_weight.contiguous()
+    rest = (cos, sin, q_weight, k_weight, float(eps), positions, bool(interleaved))
+    if q.shape[0] == 0 or q.shape[1] == 0:
+        if out is not None:
+            return out[0], out[1]
+        # connected to the graph, so that a backward gives zero gradients
+        zero = sum(w.sum() * 0 for w in (q_weight, k_weight) if w is not None)
+        return ((q * 1.0 + zero).to(q.dtype).contiguous(),
+                (k * 1.0 + zero).to(k.dtype).contiguous())
+    if grad:
+        return _QkNormRotary.apply(q, k, q_weight, k_weight, cos, sin, float(eps), positions,
+                                   bool(interleaved))
+    if out is None:
+        out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
+               torch.empty(k.shape, dtype=k.dtype, device=k.device))
+    _forward(q, k, out[0], out[1], *rest)
+    return out[0], out[1]

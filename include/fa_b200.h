@@ -532,6 +532,91 @@ FA_B200_API int fa_b200_ssimulacra2(const fa_view* x, const fa_view* y, double d
                                     size_t workspace_bytes, double* out_per_image,
                                     double* out_total, int device, void* stream);
 
+/* ---- operators of a training step around the losses (no counterpart in the
+ * reference) ------------------------------------------------------------- */
+
+/* Heads of one attention operand: [B, L, heads, dim] with unit stride in dim;
+ * strides in elements. */
+typedef struct fa_heads {
+  void* data;
+  int32_t heads;
+  int32_t pad_;
+  int64_t stride_b, stride_l, stride_h;
+} fa_heads;
+
+/* What queries and keys share.  cos_table, sin_table: float32 [table,
+ * rotary / 2] contiguous; positions: int32, or int64 when positions_64, with
+ * element strides for batch and token (0 broadcasts), or null for the token's
+ * index.  A position outside [0, table) makes its token's outputs NaN.
+ * Weights: null, [dim], or [heads, dim] when weight_per_head; weight_dtype is
+ * `dtype` or FA_F32.  rotary is even and at most dim; dim at most 512. */
+typedef struct fa_qk_params {
+  int32_t dtype, weight_dtype;
+  int32_t batch, length, dim, rotary;
+  int32_t interleaved, weight_per_head;
+  int32_t table, positions_64;
+  const float* cos_table;
+  const float* sin_table;
+  const void* positions;
+  int64_t pos_stride_b, pos_stride_l;
+  const void* q_weight;
+  const void* k_weight;
+  double eps;
+} fa_qk_params;
+
+/* Norm of every query and key head and rotation by position:
+ *   y = R_p (w o x / sqrt(mean(x^2) + eps)).
+ * dtype FA_F16, FA_BF16 or FA_F32.  An output may be its own input; otherwise
+ * the buffers do not overlap. */
+FA_B200_API int fa_b200_qk_norm_rotary(const fa_heads* q, const fa_heads* k,
+                                       const fa_heads* q_out, const fa_heads* k_out,
+                                       const fa_qk_params* params, int device, void* stream);
+
+/* Its gradient: dq, dk, and the weights' gradients in weight_dtype (null to
+ * skip one).  The workspace needs no zeroing. */
+FA_B200_API int fa_b200_qk_norm_rotary_backward_workspace_bytes(int batch, int length,
+                                                                int q_heads, int k_heads,
+                                                                int dim, size_t* out_bytes);
+FA_B200_API int fa_b200_qk_norm_rotary_backward(const fa_heads* q, const fa_heads* k,
+                                                const fa_heads* gq, const fa_heads* gk,
+                                                const fa_heads* dq, const fa_heads* dk,
+                                                const fa_qk_params* params, void* dq_weight,
+                                                void* dk_weight, void* workspace,
+                                                size_t workspace_bytes, int device,
+                                                void* stream);
+
+/* One matrix of an orthogonalised update; rows contiguous, row strides in
+ * elements.  src: the matrix, or the gradient; dst: the result, or the weight
+ * (updated in place); momentum: float32 contiguous (updates only); step: the
+ * factor of the orthogonalised matrix in the weight's update. */
+typedef struct fa_matrix {
+  const void* src;
+  void* dst;
+  float* momentum;
+  int32_t rows, cols;
+  int64_t src_row_stride, dst_row_stride;
+  double step;
+} fa_matrix;
+
+/* Newton-Schulz orthogonalisation of `count` matrices:
+ *   X <- X / |X|_F,  then for each of `steps` triples (a, b, c) in HOST memory
+ *   X <- a X + (b A + c A^2) X,  A = X X^T  (on the shorter side),
+ * written in dtype (FA_F16, FA_BF16, FA_F32).  A zero matrix gives zeros, one
+ * that holds an infinity or a NaN gives NaN.  Every matrix of a call has the
+ * same dtype; the sizes may differ.  The workspace needs no zeroing. */
+FA_B200_API int fa_b200_orthogonalize_workspace_bytes(const fa_matrix* matrices, int count,
+                                                      int dtype, size_t* out_bytes);
+FA_B200_API int fa_b200_orthogonalize(const fa_matrix* matrices, int count, int dtype,
+                                      const double* coefficients, int steps, void* workspace,
+                                      size_t workspace_bytes, int device, void* stream);
+
+/* The optimiser step: momentum <- mu momentum + src; U = src + mu momentum
+ * (nesterov) or momentum; dst <- decay dst - step O(U).  Same workspace. */
+FA_B200_API int fa_b200_muon_step(const fa_matrix* matrices, int count, int dtype,
+                                  const double* coefficients, int steps, double mu,
+                                  int nesterov, double decay, void* workspace,
+                                  size_t workspace_bytes, int device, void* stream);
+
 /* No counterpart in the reference: test hook of the bounded device-side
  * waits.  Launches one thread that waits `limit_ns` (at most 1 s) for an
  * mbarrier phase that nothing completes and then records FA_E_TIMEOUT the

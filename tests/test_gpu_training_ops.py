@@ -1,0 +1,509 @@
+"""The training-step operators on the GPU, against plain float64 formulas.
+
+Tolerances: u is the unit roundoff of the output's type (2^-24, 2^-11, 2^-8
+for float32, float16, bfloat16).  Each output is rounded once (u relative per
+value); the sums behind it are float32 over n terms, whose error stays below
+n 2^-24 of the sum of magnitudes.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import frame_analytics_b200 as fa
+from frame_analytics_b200.optim import NEWTON_SCHULZ
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+# --------------------------------------------------------------------------- #
+# query / key norm and rotation
+# --------------------------------------------------------------------------- #
+
+def tables(positions, rotary, device="cuda"):
+    half = rotary // 2
+    a = (torch.arange(positions, dtype=torch.float64, device=device)[:, None]
+         * 10000.0 ** (-torch.arange(half, dtype=torch.float64, device=device) / half))
+    return a.cos().float(), a.sin().float()
+
+
+def plain_qk(x, cos, sin, w, eps, positions, interleaved):
+    """float64, differentiable."""
+    y = x / (x.square().mean(-1, keepdim=True) + eps).sqrt()
+    if w is not None:
+        y = y * w
+    if cos is None:
+        return y
+    if positions is None:
+        positions = torch.arange(x.shape[1], device=x.device)
+    c, s = (t.double()[positions.long()] for t in (cos, sin))
+    if c.dim() == 2:
+        c, s = c[None], s[None]
+    c, s = c[:, :, None], s[:, :, None]
+    r = 2 * cos.shape[1]
+    i1 = slice(0, r, 2) if interleaved else slice(0, r // 2)
+    i2 = slice(1, r, 2) if interleaved else slice(r // 2, r)
+    out = y.clone()
+    out[..., i1] = y[..., i1] * c - y[..., i2] * s
+    out[..., i2] = y[..., i2] * c + y[..., i1] * s
+    return out
+
+
+def close(got, want, u, terms):
+    """|got - want| within one rounding plus float32 sums of `terms` terms, on the
+    scale of the output (its largest value: sums may cancel)."""
+    want = want.double()
+    err = (got.double() - want).abs()
+    tol = u * want.abs() + (8 + terms) * 2.0 ** -24 * want.abs().max().clamp_min(1e-30)
+    if u == 2.0 ** -11:
+        tol = tol + 2.0 ** -25  # float16's subnormal spacing
+    assert bool((err <= tol).all()), (err / tol).max().item()
+
+
+# batch, length, q heads, k heads, dim, rotary, interleaved, weights
+QK = [
+    (1, 1, 1, 1, 64, 64, False, "dim"),
+    (4, 1, 8, 2, 128, 128, False, "dim"),
+    (2, 33, 4, 4, 64, 64, True, "dim"),
+    (3, 17, 3, 1, 80, 80, False, "head"),
+    (2, 9, 4, 2, 96, 48, True, "head"),
+    (2, 40, 5, 5, 48, 24, False, "none"),
+    (1, 301, 2, 1, 256, 256, False, "dim"),
+    (2, 5, 2, 3, 7, 6, False, "dim"),      # odd head size: two components pass or turn alone
+    (1, 6, 1, 2, 1, 0, False, "dim"),
+    (2, 3, 2, 2, 33, 20, True, "head"),
+    (1, 4, 2, 1, 512, 512, False, "dim"),
+    (1, 4, 2, 1, 130, 130, True, "dim"),
+    (2, 65, 6, 2, 128, 0, False, "dim"),
+    (70, 2, 2, 2, 32, 32, False, "head"),
+]
+
+
+def qk_case(case, dtype, seed=0, w_dtype=None):
+    b, n, hq, hk, d, r, inter, weights = case
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    packed = torch.randn(b, n, hq + 2 * hk, d, generator=g, device="cuda").to(dtype)
+    q, k = packed[:, :, :hq], packed[:, :, hq:hq + hk]
+    cos, sin = tables(n + 11, r) if r else (None, None)
+    pos = torch.randint(0, n + 11, (b, n), generator=g, device="cuda") if r else None
+    ws = [None, None]
+    if weights != "none":
+        ws = [(1 + 0.3 * torch.randn((h, d) if weights == "head" else (d,), generator=g,
+                                     device="cuda")).to(w_dtype or dtype) for h in (hq, hk)]
+    gs = [torch.randn(b, n, h, d, generator=g, device="cuda").to(dtype) for h in (hq, hk)]
+    return q, k, cos, sin, pos, ws, gs, inter
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", QK)
+def test_qk_forward(case, dtype):
+    q, k, cos, sin, pos, (qw, kw), _, inter = qk_case(case, dtype)
+    got = fa.qk_norm_rotary(q, k, cos, sin, q_weight=qw, k_weight=kw, positions=pos,
+                            interleaved=inter, eps=1e-5)
+    for x, w, y in ((q, qw, got[0]), (k, kw, got[1])):
+        want = plain_qk(x.double(), cos, sin, None if w is None else w.double(), 1e-5, pos, inter)
+        assert y.shape == x.shape and y.dtype == dtype and y.is_contiguous()
+        close(y, want, U[dtype], 8)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", QK)
+def test_qk_backward(case, dtype):
+    q, k, cos, sin, pos, ws, gs, inter = qk_case(case, dtype, seed=1)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, *ws) if t is not None]
+    qw, kw = leaves[2:] if len(leaves) == 4 else (None, None)
+    out = fa.qk_norm_rotary(leaves[0], leaves[1], cos, sin, q_weight=qw, k_weight=kw,
+                            positions=pos, interleaved=inter, eps=1e-5)
+    got = torch.autograd.grad(out, leaves, gs)
+    wide = [t.detach().double().requires_grad_(True) for t in leaves]
+    wqw, wkw = wide[2:] if len(wide) == 4 else (None, None)
+    ref = (plain_qk(wide[0], cos, sin, wqw, 1e-5, pos, inter),
+           plain_qk(wide[1], cos, sin, wkw, 1e-5, pos, inter))
+    want = torch.autograd.grad(ref, wide, [g.double() for g in gs])
+    tokens = q.shape[0] * q.shape[1]
+    for i, (a, b) in enumerate(zip(got, want)):
+        assert a.shape == b.shape and a.dtype == leaves[i].dtype
+        if i < 2:
+            close(a, b, U[dtype], 16)
+        else:  # sums over tokens (and heads) of terms of order 1, with either sign
+            n = tokens * (1 if b.dim() == 2 else (q, k)[i - 2].shape[2])
+            err = (a.double() - b).abs()
+            tol = U[dtype] * b.abs() + 2.0 ** -24 * (8 + n) * 4 * math.sqrt(n)
+            assert bool((err <= tol).all()), (err / tol).max().item()
+
+
+def test_qk_gradient_against_differences():
+    """Central differences of the float64 plain form's scalar, with the kernel's
+    own float32 gradient: the difference quotient is good to h^2."""
+    q, k, cos, sin, pos, ws, gs, inter = qk_case((1, 3, 2, 1, 16, 8, True, "head"),
+                                                 torch.float32, seed=5)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, *ws)]
+    out = fa.qk_norm_rotary(leaves[0], leaves[1], cos, sin, q_weight=leaves[2],
+                            k_weight=leaves[3], positions=pos, interleaved=inter)
+    grads = torch.autograd.grad(out, leaves, gs)
+
+    def value(ts):
+        t = [u.double() for u in ts]
+        return float((plain_qk(t[0], cos, sin, t[2], 1e-6, pos, inter) * gs[0]).sum()
+                     + (plain_qk(t[1], cos, sin, t[3], 1e-6, pos, inter) * gs[1]).sum())
+
+    h = 1e-4
+    for i, leaf in enumerate(leaves):
+        flat = leaf.detach().double().flatten()
+        for j in range(0, flat.numel(), 5):
+            vals = []
+            for sgn in (1, -1):
+                moved = flat.clone()
+                moved[j] += sgn * h
+                ts = [t.detach().double() for t in leaves]
+                ts[i] = moved.view(leaf.shape)
+                vals.append(value(ts))
+            fd = (vals[0] - vals[1]) / (2 * h)
+            assert abs(fd - float(grads[i].flatten()[j])) < 2e-5 * (1 + abs(fd))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_qk_float32_weights_and_their_gradient(dtype):
+    q, k, cos, sin, pos, ws, gs, inter = qk_case(QK[2], dtype, w_dtype=torch.float32)
+    ws = [w.requires_grad_(True) for w in ws]
+    out = fa.qk_norm_rotary(q, k, cos, sin, q_weight=ws[0], k_weight=ws[1], positions=pos,
+                            interleaved=inter)
+    got = torch.autograd.grad(out, ws, gs)
+    wide = [w.detach().double().requires_grad_(True) for w in ws]
+    ref = [plain_qk(x.double(), cos, sin, w, 1e-6, pos, inter) for x, w in zip((q, k), wide)]
+    want = torch.autograd.grad(ref, wide, [g.double() for g in gs])
+    for a, b in zip(got, want):
+        assert a.dtype == torch.float32
+        assert float((a.double() - b).abs().max()) < 2.0 ** -24 * 400 * float(b.abs().max())
+
+
+def test_qk_default_positions_int32_and_broadcast_agree():
+    q, k, cos, sin, _, ws, _, _ = qk_case(QK[2], torch.bfloat16)
+    n = q.shape[1]
+    a = fa.qk_norm_rotary(q, k, cos, sin, q_weight=ws[0], k_weight=ws[1])
+    row = torch.arange(n, device="cuda")
+    for p in (row, row.int(), row.expand(2, n), row.repeat(2, 1).int()):
+        b = fa.qk_norm_rotary(q, k, cos, sin, q_weight=ws[0], k_weight=ws[1], positions=p)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("dim,rotary", [(64, 64), (33, 20)])
+def test_qk_positions_outside_the_tables_give_nan_rows(dim, rotary):
+    q, k, cos, sin, _, ws, gs, _ = qk_case((2, 4, 2, 1, dim, rotary, False, "dim"), torch.float32)
+    P = cos.shape[0]
+    pos = torch.tensor([[0, P, 1, -1], [P - 1, 2, 1 << 40, -(1 << 40)]], device="cuda")
+    bad = (pos < 0) | (pos >= P)
+    qg = q.detach().requires_grad_(True)
+    y = fa.qk_norm_rotary(qg, k, cos, sin, q_weight=ws[0], k_weight=ws[1], positions=pos)
+    (dq,) = torch.autograd.grad(y[0], qg, gs[0])
+    for t in (*y, dq):
+        assert bool(t[bad].isnan().all()) and bool(t[~bad].isfinite().all())
+
+
+def test_qk_out_in_place_strided_and_cache_slice():
+    q, k, cos, sin, pos, ws, _, _ = qk_case((3, 1, 4, 2, 64, 64, False, "dim"), torch.bfloat16)
+    want = fa.qk_norm_rotary(q, k, cos, sin, q_weight=ws[0], k_weight=ws[1], positions=pos)
+    cache = torch.zeros(3, 2, 50, 64, dtype=torch.bfloat16, device="cuda")  # (B, Hk, L, D)
+    slot = cache[:, :, 7:8].transpose(1, 2)
+    q_in = q.clone()
+    got = fa.qk_norm_rotary(q_in, k, cos, sin, q_weight=ws[0], k_weight=ws[1], positions=pos,
+                            out=(q_in, slot))
+    assert got[0] is q_in and torch.equal(q_in, want[0])
+    assert torch.equal(cache[:, :, 7], want[1][:, 0]) and int(cache.count_nonzero()) == \
+        int(want[1].count_nonzero())
+    for dim, rot in ((512, 512), (33, 20)):
+        q, k, cos, sin, pos, ws, _, _ = qk_case((2, 3, 2, 1, dim, rot, False, "dim"), torch.float32)
+        want = fa.qk_norm_rotary(q, k, cos, sin, positions=pos)
+        q, k = q.clone(), k.clone()
+        fa.qk_norm_rotary(q, k, cos, sin, positions=pos, out=(q, k))
+        assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+def test_qk_misaligned_and_non_unit_stride_inputs_agree():
+    q, k, cos, sin, pos, ws, _, _ = qk_case((2, 6, 2, 2, 64, 64, False, "dim"), torch.bfloat16)
+    want = fa.qk_norm_rotary(q, k, cos, sin, q_weight=ws[0], k_weight=ws[1], positions=pos)
+    store = torch.empty(2 * 6 * 2 * 65 + 1, dtype=torch.bfloat16, device="cuda")
+    odd = store[1:].view(2, 6, 2, 65)[..., :64].copy_(q)
+    swapped = k.transpose(1, 3).contiguous().transpose(1, 3)
+    got = fa.qk_norm_rotary(odd, swapped, cos, sin, q_weight=ws[0], k_weight=ws[1], positions=pos)
+    for a, b in zip(got, want):  # other kernels may sum in another order: one rounding
+        assert float((a.float() - b.float()).abs().max()) <= 2.0 ** -7 * float(b.abs().max())
+
+
+def test_qk_extreme_rows():
+    """A zero row stays zero (eps keeps it finite), an infinite one gives NaN
+    there alone, and its neighbours are untouched."""
+    q, k, cos, sin, pos, _, _, _ = qk_case((1, 4, 2, 1, 64, 64, False, "none"), torch.float32)
+    q = q.clone()
+    q[0, 1, 0] = 0
+    q[0, 2, 1, 5] = float("inf")
+    y, _ = fa.qk_norm_rotary(q, k, cos, sin, positions=pos)
+    assert bool((y[0, 1, 0] == 0).all())
+    assert bool(y[0, 2, 1].isnan().any())
+    ok = torch.ones(4, 2, dtype=torch.bool, device="cuda")
+    ok[2, 1] = False
+    assert bool(y[0][ok].isfinite().all())
+
+
+def test_qk_empty_and_graph_capture_and_streams():
+    q = torch.empty(2, 0, 4, 64, device="cuda", requires_grad=True)
+    w = torch.ones(64, device="cuda", requires_grad=True)
+    cos, sin = tables(8, 64)
+    y, z = fa.qk_norm_rotary(q, q[:, :, :2], cos, sin, q_weight=w, k_weight=w)
+    assert y.shape == (2, 0, 4, 64) and z.shape == (2, 0, 2, 64)
+    (y.sum() + z.sum()).backward()
+    assert bool((w.grad == 0).all())
+    q, k, cos, sin, pos, ws, _, _ = qk_case(QK[1], torch.bfloat16)
+    want = fa.qk_norm_rotary(q, k, cos, sin, q_weight=ws[0], k_weight=ws[1], positions=pos)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fa.qk_norm_rotary(q, k, cos, sin, q_weight=ws[0], k_weight=ws[1], positions=pos)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = fa.qk_norm_rotary(q, k, cos, sin, q_weight=ws[0], k_weight=ws[1], positions=pos)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_qk_weight_gradient_is_the_same_bits_every_time():
+    q, k, cos, sin, pos, ws, gs, inter = qk_case((2, 701, 4, 2, 64, 64, False, "dim"),
+                                                 torch.float32)
+    ws = [w.requires_grad_(True) for w in ws]
+    runs = []
+    for _ in range(3):
+        out = fa.qk_norm_rotary(q, k, cos, sin, q_weight=ws[0], k_weight=ws[1], positions=pos)
+        runs.append(torch.autograd.grad(out, ws, gs))
+    for r in runs[1:]:
+        assert torch.equal(r[0], runs[0][0]) and torch.equal(r[1], runs[0][1])
+
+
+# --------------------------------------------------------------------------- #
+# orthogonalised updates
+# --------------------------------------------------------------------------- #
+
+def plain_ns(x, steps=5, coefficients=NEWTON_SCHULZ):
+    """float64; (..., m, n)."""
+    x = x.double()
+    norm = x.square().sum((-2, -1), keepdim=True).sqrt()
+    x = torch.where(norm > 0, x / norm, torch.zeros_like(x))
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    cs = coefficients if hasattr(coefficients[0], "__len__") else [coefficients] * steps
+    for a, b, c in cs:
+        g = x @ x.mT
+        x = a * x + (b * g + c * g @ g) @ x
+    return x.mT if tall else x
+
+
+def gradient(shape, kind, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(shape, generator=g, device="cuda")
+    m, n = shape[-2:]
+    if kind == "spiky":
+        r = max(1, min(m, n) // 16)
+        x = x + 30 * (torch.randn(*shape[:-1], r, generator=g, device="cuda")
+                      @ torch.randn(*shape[:-2], r, n, generator=g, device="cuda"))
+    return 1e-3 * x
+
+
+# relative 2-norm error allowed: the products' error (bfloat16: float16 operands,
+# 2^-12 each with the identity and diagonals kept apart, times the slope of five
+# steps; the others: float32-like) and the output's rounding
+NS_TOL = {torch.float32: 2e-5, torch.float16: 3e-4, torch.bfloat16: 2.5e-3}
+
+NS_SHAPES = [(1, 1), (1, 7), (5, 1), (16, 16), (33, 20), (64, 64), (65, 130), (127, 129),
+             (128, 128), (200, 72), (257, 300), (384, 1000), (1000, 384), (640, 640)]
+
+
+def rel(got, want):
+    d = torch.linalg.vector_norm(got.double() - want)
+    return float(d / torch.linalg.vector_norm(want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", ["noise", "spiky"])
+@pytest.mark.parametrize("shape", NS_SHAPES)
+def test_orthogonalize(shape, kind, dtype):
+    x = gradient(shape, kind).to(dtype)
+    y = fa.orthogonalize(x)
+    assert y.shape == x.shape and y.dtype == dtype and y.is_contiguous()
+    assert rel(y, plain_ns(x)) < NS_TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_orthogonalize_singular_values_follow_the_polynomial(dtype):
+    u = torch.linalg.qr(torch.randn(48, 48, dtype=torch.float64, device="cuda"))[0]
+    v = torch.linalg.qr(torch.randn(90, 48, dtype=torch.float64, device="cuda"))[0]
+    s = torch.logspace(0, -2, 48, dtype=torch.float64, device="cuda")
+    x = ((u * s) @ v.mT).to(dtype)
+    got = torch.linalg.svdvals(fa.orthogonalize(x).double())
+    assert float(got.max()) < 1.25 and float(got.min()) > 0.6
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(3, 40, 56), (2, 3, 130, 70), (150, 12, 20), (5, 200, 333)])
+def test_orthogonalize_stacks(shape, dtype):
+    x = gradient(shape, "noise", seed=2).to(dtype)
+    y = fa.orthogonalize(x)
+    want = plain_ns(x)
+    assert y.shape == x.shape
+    worst = max(rel(a, b) for a, b in zip(y.flatten(0, -3), want.flatten(0, -3)))
+    assert worst < NS_TOL[dtype]
+    # a matrix of a stack is what it is alone
+    one = fa.orthogonalize(x.flatten(0, -3)[1])
+    assert rel(one, y.flatten(0, -3)[1].double()) < NS_TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_orthogonalize_scale_does_not_matter(dtype):
+    x = gradient((72, 100), "noise", seed=3)
+    want = fa.orthogonalize(x.to(dtype))
+    for e in ((-20, 10) if dtype == torch.float16 else (-100, 60)):
+        # powers of two scale float16 exactly only above its subnormals
+        got = fa.orthogonalize((x * 2.0 ** (10 + e if dtype == torch.float16 and e < 0 else e)).to(dtype))
+        if dtype != torch.float16:
+            assert torch.equal(got, want)
+        else:
+            assert bool(got.isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [(24, 40), (300, 260)])
+def test_orthogonalize_zero_nan_and_inf(size, dtype):
+    x = gradient((4, *size), "noise", seed=4).to(dtype)
+    clean = fa.orthogonalize(x)
+    x[0] = 0
+    x[1, 3, 5] = float("nan")
+    x[2, size[0] - 1, 0] = -float("inf")
+    y = fa.orthogonalize(x)
+    assert bool((y[0] == 0).all())
+    assert bool(y[1].isnan().all()) and bool(y[2].isnan().all())
+    assert torch.equal(y[3], clean[3])
+
+
+def test_orthogonalize_views_strides_steps_and_coefficients():
+    base = gradient((6, 90, 70), "noise", seed=5)
+    want = plain_ns(base[::2, 5:75, 3:53].contiguous())
+    for dtype in (torch.float32, torch.bfloat16):
+        b = base.to(dtype)
+        v = b[::2, 5:75, 3:53]
+        assert rel(fa.orthogonalize(v), plain_ns(v)) < NS_TOL[dtype]
+        assert rel(fa.orthogonalize(v.mT), plain_ns(v).mT) < NS_TOL[dtype]
+        e = v[0].expand(3, 70, 50)
+        assert rel(fa.orthogonalize(e), plain_ns(e)) < NS_TOL[dtype]
+    x = base[0]
+    for steps in (1, 2, 3, 8):
+        assert rel(fa.orthogonalize(x, steps=steps), plain_ns(x, steps)) < NS_TOL[torch.float32]
+    many = [(4.0, -6.0, 2.5), (3.0, -4.0, 1.8), (1.875, -1.25, 0.375)]
+    assert rel(fa.orthogonalize(x, steps=3, coefficients=many), plain_ns(x, 3, many)) < 2e-5
+    cubic = (1.5, -0.5, 0.0)
+    assert rel(fa.orthogonalize(x, steps=10, coefficients=cubic), plain_ns(x, 10, cubic)) < 2e-5
+    assert want.shape == (3, 70, 50)
+
+
+def test_orthogonalize_empty():
+    for shape in ((0, 5, 5), (3, 0, 4), (4, 0)):
+        assert fa.orthogonalize(torch.empty(shape, device="cuda")).shape == shape
+
+
+def test_orthogonalize_same_bits_every_time_and_in_a_graph():
+    x = gradient((2, 300, 500), "spiky", seed=6).to(torch.bfloat16)
+    a = fa.orthogonalize(x)
+    for _ in range(3):
+        assert torch.equal(fa.orthogonalize(x), a)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        b = fa.orthogonalize(x)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(a, b)
+
+
+def plain_muon(w, g, m, lr, mu, nesterov, wd, scale):
+    w, g, m = w.double(), g.double(), m.double()
+    m = mu * m + g
+    u = g + mu * m if nesterov else m
+    rows, cols = w.shape[0], w[0].numel()
+    s = {"aspect": math.sqrt(max(1, rows / cols)), "rms": 0.2 * math.sqrt(max(rows, cols)),
+         "none": 1.0}[scale]
+    return (1 - lr * wd) * w - lr * s * plain_ns(u.reshape(rows, cols)).view(w.shape), m
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nesterov,wd,scale", [(True, 0.0, "aspect"), (False, 0.1, "rms"),
+                                               (True, 0.01, "none")])
+def test_muon_step(dtype, nesterov, wd, scale):
+    shapes = [(64, 96), (96, 64), (64, 96), (16, 3, 3, 3), (130, 50), (1, 9), (300, 280)]
+    g = torch.Generator(device="cuda").manual_seed(7)
+    W = [(torch.randn(s, generator=g, device="cuda") / 8).to(dtype) for s in shapes]
+    G = [(1e-2 * torch.randn(s, generator=g, device="cuda")).to(dtype) for s in shapes]
+    M = [1e-2 * torch.randn(s, generator=g, device="cuda") for s in shapes]
+    want = [plain_muon(w, gr, m, 0.02, 0.9, nesterov, wd, scale) for w, gr, m in zip(W, G, M)]
+    fa.muon_step(W, G, M, lr=0.02, momentum=0.9, nesterov=nesterov, weight_decay=wd, scale=scale)
+    for w, m, (ww, wm) in zip(W, M, want):
+        assert rel(m, wm) < 2.0 ** -22
+        # one rounding of the weight, and the update's own error times its share of the weight
+        tol = 2 * U[dtype] + NS_TOL[dtype] * 0.02 * 0.2 * 20 / float(ww.square().mean().sqrt()) / 8
+        assert rel(w, ww) < tol
+
+
+def test_muon_optimizer_matches_the_functional_step_and_survives_checkpoints():
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.Conv2d(3, 24, 3), torch.nn.Conv2d(24, 8, 3)).cuda()
+    net = net.to(memory_format=torch.channels_last)
+    ps = [p for p in net.parameters() if p.dim() > 1]
+    opt = fa.Muon(ps, lr=0.05, weight_decay=0.1)
+    twins = [p.detach().clone(memory_format=torch.preserve_format) for p in ps]
+    moms = [torch.zeros_like(t) for t in twins]
+    x = torch.randn(2, 3, 20, 20, device="cuda").to(memory_format=torch.channels_last)
+    for _ in range(3):
+        opt.zero_grad()
+        net(x).square().mean().backward()
+        grads = [p.grad.clone(memory_format=torch.preserve_format) for p in ps]
+        opt.step()
+        fa.muon_step(twins, grads, moms, lr=0.05, weight_decay=0.1)
+    for p, t, g in zip(ps, twins, grads):
+        assert torch.equal(p.detach(), t)
+    half = [torch.nn.Parameter(t.to(torch.bfloat16)) for t in twins]
+    o1 = fa.Muon(half, lr=0.01)
+    for h in half:
+        h.grad = torch.randn_like(h)
+    o1.step()
+    copies = [torch.nn.Parameter(h.detach().clone(memory_format=torch.preserve_format)) for h in half]
+    o2 = fa.Muon(copies, lr=0.01)
+    o2.load_state_dict(o1.state_dict())
+    for h, c in zip(half, copies):
+        assert o2.state[c]["momentum_buffer"].dtype == torch.float32
+        h.grad = torch.randn_like(h)
+        c.grad = h.grad.clone(memory_format=torch.preserve_format)
+    o1.step()
+    o2.step()
+    for h, c in zip(half, copies):
+        assert torch.equal(h, c)
+
+
+def test_muon_orders_of_memory():
+    """A channels-last kernel is updated as its contiguous twin is, whatever the
+    gradient's layout."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    w = torch.randn(12, 5, 3, 3, generator=g, device="cuda")
+    gr = torch.randn(12, 5, 3, 3, generator=g, device="cuda")
+    m = torch.zeros_like(w)
+    want, _ = plain_muon(w, gr, m, 0.1, 0.95, True, 0.0, "aspect")
+    cl = torch.channels_last
+    for wf in (torch.contiguous_format, cl):
+        for gf in (torch.contiguous_format, cl):
+            w1 = w.clone().contiguous(memory_format=wf)
+            m1 = torch.zeros_like(w1)
+            fa.muon_step([w1], [gr.contiguous(memory_format=gf)], [m1], lr=0.1)
+            assert rel(w1, want) < 2e-6
+            assert torch.equal(m1, gr)
