@@ -9,46 +9,108 @@
 // The optimiser step on a weight W with gradient G and momentum M:
 //   M <- mu M + G,  U = G + mu M (Nesterov) or M,
 //   W <- (1 - lr wd) W - lr scale O(U).
-#include "train.cuh"
+//
+// Three launches serve a whole list of matrices: momentum and norms, packing,
+// and one persistent kernel for all products of all steps.
+//
+// Number formats.  The products run on the tensor cores with float16 operands
+// and float32 accumulators; float16 has three more bits than bfloat16 at the
+// same rate, and powers of two per step (from a bound on the singular values)
+// keep every value inside its range.  A rounding of relative size e in the
+// term a X grows with the small singular values (by a per step), while one in
+// B X does not: B vanishes on small singular directions.  So X travels as a
+// pair of float16 (hi, lo: 22 bits); only hi enters the products and the term
+// a X uses both.  The diagonals of A and B, which hold most of their mass near
+// convergence, travel in float32 beside the float16 off-diagonal parts O:
+//   A = D + O:  A^2 = D^2 + D O + O D + O O,   B X = diag(B) X + offdiag(B) X.
+// Together: 5e-4 to 1.2e-3 relative for bfloat16 matrices (bfloat16 products:
+// 1e-2 to 1e-1).  float32 and float16 matrices run every product three times
+// (hi hi + hi lo + lo hi), which is float32-like (about 1e-6).
+#include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
+
+#include "mbar.cuh"
+#include "train.cuh"
 
 namespace fab {
 
-constexpr int kMats = 64;          // matrices of one launch sequence
-constexpr int kNormBlocks = 32;    // partial sums of squares of one matrix
+constexpr int kMats = 128;         // matrices of one launch sequence
+constexpr int kGroups = 8;         // shapes of one launch sequence
+constexpr int kMaxSteps = 32;
+constexpr int kNormBlocks = 64;    // partial sums of squares of one matrix, at most
+
+constexpr int BM = 128;            // tile rows: the lanes of tensor memory
+constexpr int BK = 64;             // 128 bytes of float16: one swizzle row
+constexpr int kBox = 64 * 128;     // bytes of a 64 x 64 box
+constexpr int kEpilogue = 256;     // 8 epilogue warps: 4 quarters of the rows x 2 column halves
+constexpr int kThreads = 128 + kEpilogue;  // producer, issuer, allocator, spare before them
+// The tensor cores add into an accumulator with truncation, a relative loss of
+// about 2^-25 for each 16 columns of K, always towards zero.  float32-like
+// products therefore move their sums to registers (rounded adds) every
+// kChunk K blocks, and keep the small products hi lo + lo hi in an accumulator
+// of their own: 2304 x 768 float32 is 2e-5 off without, see the tests.
+constexpr int kChunk = 4;
+
+// Tensor maps of one shape: X twice (it alternates), O and offdiag(B); hi, lo.
+enum { MAP_X0, MAP_X1, MAP_A, MAP_B, kMaps };
+
+struct NsGroup {
+  CUtensorMap map[kMaps][2];
+  int rows, cols, s, l;            // s = shorter side, l = longer
+  int tall, batch, first;          // matrices [first, first + batch)
+  int px, pa;                      // row pitches of X and of A, B in elements
+  int bn_sym, bn_app;              // tile columns of the symmetric products and of B X
+  int tiles_sym, tiles_app;        // tiles of one matrix
+  __half *x[2][2], *a[2], *b[2];   // [alternation][hi, lo]
+  float *da, *db;                  // diagonals, [batch][pa]
+};
 
 struct NsMat {
-  const void* src;   // x, or the gradient
-  void* dst;         // out, or the weight
-  float* mom;        // momentum, or null
-  long long x_off, a_off;  // offsets of X[2] and of A, B in floats
-  long long src_row, dst_row;  // row strides
-  int rows, cols;
-  float step;                  // W <- decay W - step O
+  const void* src;                 // x, or the gradient
+  void* dst;                       // out, or the weight
+  float* mom;                      // momentum, or null
+  long long src_row, dst_row;
+  float step;                      // W <- decay W - step O
+  int group;
+};
+
+struct NsStep {
+  float a, b, c;
+  int ex, ea, eb, ex2;             // stored value = true value x 2^e: X, A, B, next X
 };
 
 struct NsArgs {
+  NsGroup g[kGroups];
   NsMat m[kMats];
-  float* ws;
-  double* part;      // [kMats][kNormBlocks]
-  float mu;
+  NsStep k[kMaxSteps];
+  int groups, mats, steps;
+  int tiles_sym, tiles_app;        // over all matrices
+  unsigned* done;                  // [3][kMats] finished tiles of the three products
+  unsigned* failed;                // set when a wait of this call gave up
+  double* part;                    // [kMats][kNormBlocks]
+  unsigned* err;
+  float mu, decay;
   int nesterov;
-  float decay;
 };
 
-__device__ __forceinline__ float nan_f() { return __int_as_float(0x7fffffff); }
+// ---------------------------------------------------------------------------
+// momentum, norm, packing
+// ---------------------------------------------------------------------------
 
-// Updates the momentum and sums the squares of the update.
+// Updates the momentum and sums the squares of the update, in double: float32
+// squares of a float32 matrix could leave its range.
 template <typename T>
 __global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ NsArgs a) {
   __shared__ double sm[32];
   const NsMat& m = a.m[blockIdx.y];
-  const long long n = (long long)m.rows * m.cols;
+  const NsGroup& g = a.g[m.group];
+  const long long n = (long long)g.rows * g.cols;
   const T* src = reinterpret_cast<const T*>(m.src);
   double ss = 0;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += 256ll * gridDim.x) {
-    const long long r = i / m.cols, c = i - r * m.cols;
+    const long long r = i / g.cols, c = i - r * g.cols;
     float u = Ld<T>::f(src[r * m.src_row + c]);
     if (m.mom) {
       const float v = fmaf(a.mu, m.mom[i], u);
@@ -59,142 +121,720 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ Ns
   }
   ss = block_sum(ss, sm);
   if (threadIdx.x == 0) a.part[blockIdx.y * kNormBlocks + blockIdx.x] = ss;
+  // the product kernel's counters, for this call
+  if (blockIdx.x == 0 && threadIdx.x < 3) a.done[threadIdx.x * kMats + blockIdx.y] = 0u;
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 3) *a.failed = 0u;
 }
 
+__device__ __forceinline__ void split_half(float v, __half* hi, __half* lo) {
+  *hi = __float2half_rn(v);
+  *lo = __float2half_rn(v - __half2float(*hi));
+}
+
+// X = update / norm as (hi, lo) at the pitch px; the pitch's tail is zeroed.
 template <typename T>
-__global__ void __launch_bounds__(256) ns_pack_kernel(const __grid_constant__ NsArgs a) {
+__global__ void __launch_bounds__(256) ns_pack_kernel(const __grid_constant__ NsArgs a,
+                                                      int norm_blocks) {
   const NsMat& m = a.m[blockIdx.y];
-  const long long n = (long long)m.rows * m.cols;
+  const NsGroup& g = a.g[m.group];
   const T* src = reinterpret_cast<const T*>(m.src);
   double ss = 0;
-  for (int i = 0; i < kNormBlocks; ++i) ss += a.part[blockIdx.y * kNormBlocks + i];
+  for (int i = 0; i < norm_blocks; ++i) ss += a.part[blockIdx.y * kNormBlocks + i];
   const bool finite = ss <= 1.7e308;
-  const double inv = ss > 0 ? 1.0 / sqrt(ss) : 0.0;
+  const double inv = ss > 0 ? ldexp(1.0, a.k[0].ex) / sqrt(ss) : 0.0;
+  const long long n = (long long)g.rows * g.px;
+  const long long base = (long long)(blockIdx.y - g.first) * n;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += 256ll * gridDim.x) {
-    const long long r = i / m.cols, c = i - r * m.cols;
-    float u = Ld<T>::f(src[r * m.src_row + c]);
-    if (m.mom) {
-      const float v = m.mom[i];
-      u = a.nesterov ? fmaf(a.mu, v, u) : v;
+    const long long r = i / g.px, c = i - r * g.px;
+    float u = 0.f;
+    if (c < g.cols) {
+      u = Ld<T>::f(src[r * m.src_row + c]);
+      if (m.mom) {
+        const float v = m.mom[r * g.cols + c];
+        u = a.nesterov ? fmaf(a.mu, v, u) : v;
+      }
+      u = finite ? (float)(u * inv) : __int_as_float(0x7fffffff);
     }
-    a.ws[m.x_off + i] = finite ? (float)(u * inv) : nan_f();
+    __half hi, lo;
+    split_half(u, &hi, &lo);
+    g.x[0][0][base + i] = hi;
+    g.x[0][1][base + i] = lo;
   }
 }
 
-enum { NS_GRAM, NS_SQUARE, NS_APPLY, NS_FINAL };
+// ---------------------------------------------------------------------------
+// the products: tcgen05, TMA
+// ---------------------------------------------------------------------------
 
-// 64 x 64 outputs of one matrix; D[i][j] = sum_k P(i, k) Q(k, j).
-template <int MODE, typename T>
-__global__ void __launch_bounds__(256) ns_product_kernel(const __grid_constant__ NsArgs a, int cur,
-                                                         float ca, float cb, float cc) {
-  __shared__ float sp[16][65], sq[16][65];
-  const NsMat& m = a.m[blockIdx.y];
-  const bool tall = m.rows > m.cols;
-  const int s = min(m.rows, m.cols);
-  const long long n = (long long)m.rows * m.cols;
-  const float* X = a.ws + m.x_off + cur * n;
-  float* X2 = a.ws + m.x_off + (1 - cur) * n;
-  float* A = a.ws + m.a_off;
-  float* B = A + (long long)s * s;
-  const int M = MODE <= NS_SQUARE ? s : m.rows, N = MODE <= NS_SQUARE ? s : m.cols;
-  const int K = MODE == NS_GRAM ? max(m.rows, m.cols) : s;
-  const int tn = (N + 63) / 64, tiles = ((M + 63) / 64) * tn;
-  const float *P, *Q;
-  long long pi, pk, qk, qj;  // strides
-  if (MODE == NS_GRAM) {
-    P = Q = X;
-    pi = qj = tall ? 1 : m.cols;
-    pk = qk = tall ? m.cols : 1;
-  } else if (MODE == NS_SQUARE) {
-    P = Q = A;
-    pi = qk = s;
-    pk = qj = 1;
-  } else {
-    P = tall ? X : B;
-    Q = tall ? B : X;
-    pi = tall ? m.cols : s;
-    qk = tall ? s : m.cols;
-    pk = qj = 1;
-  }
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-    const int i0 = t / tn * 64, j0 = t % tn * 64;
-    float acc[4][4] = {};
-    for (int k0 = 0; k0 < K; k0 += 16) {
-      for (int e = threadIdx.x; e < 1024; e += 256) {
-        const int kk = e & 15, ii = e >> 4;
-        sp[kk][ii] = i0 + ii < M && k0 + kk < K ? P[(i0 + ii) * pi + (k0 + kk) * pk] : 0.f;
-        sq[kk][ii] = j0 + ii < N && k0 + kk < K ? Q[(j0 + ii) * qj + (k0 + kk) * qk] : 0.f;
+__device__ __forceinline__ unsigned ld_acquire(const unsigned* p) {
+  unsigned v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];\n" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
+// Bounded wait on an mbarrier phase, or on a counter of finished tiles, that
+// tells whether it was reached.  On giving up (two seconds, or another wait of
+// the launch already has) it records FA_E_TIMEOUT and the caller leaves its
+// loop.  The launch's own word tells the other waits: the host-mapped word is
+// across the bus and is only written.
+__device__ __noinline__ bool wait_slow(unsigned bar, unsigned parity, const unsigned* flag,
+                                       unsigned want, const NsArgs& a) {
+  const unsigned long long t0 = globaltimer_ns();
+  for (unsigned i = 1;; ++i) {
+    if (flag ? ld_acquire(flag) >= want : mbar_try(bar, parity)) return true;
+    if ((i & 255u) == 0u) {
+      const bool failed = *reinterpret_cast<volatile unsigned*>(a.failed) != 0u;
+      if (failed || globaltimer_ns() - t0 > kWaitLimitNs) {
+        if (!failed) {
+          *reinterpret_cast<volatile unsigned*>(a.failed) = 1u;
+          *reinterpret_cast<volatile unsigned*>(a.err) = (unsigned)FA_E_TIMEOUT;
+          __threadfence_system();
+        }
+        return false;
       }
-      __syncthreads();
-#pragma unroll
-      for (int kk = 0; kk < 16; ++kk)
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            acc[u][v] = fmaf(sp[kk][ty + 16 * u], sq[kk][tx + 16 * v], acc[u][v]);
-      __syncthreads();
     }
+  }
+}
+__device__ __forceinline__ bool wait_bar(unsigned long long* bar, unsigned parity,
+                                         const NsArgs& a) {
+  const unsigned b = smem_u32(bar);
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i)
+    if (mbar_try(b, parity)) return true;
+  return wait_slow(b, parity, nullptr, 0, a);
+}
+__device__ __forceinline__ bool wait_flag(const unsigned* flag, unsigned want, const NsArgs& a) {
+  if (ld_acquire(flag) >= want) return true;
+  return wait_slow(0, 0, flag, want, a);
+}
+
+__device__ __forceinline__ void tma_box(unsigned dst, const CUtensorMap* map, int x, int y, int z,
+                                        unsigned bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
+      "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+// Shared-memory operand descriptor, 128-byte swizzle.  Rows along K (K-major):
+// 128-byte rows, 8-row groups 1024 bytes apart.  Rows along the other axis
+// (MN-major): 64-element blocks kBox apart, groups of 8 K rows 1024 bytes apart.
+__device__ __forceinline__ unsigned long long operand(unsigned addr) {
+  return (unsigned long long)((addr & 0x3ffffu) >> 4) |
+         ((unsigned long long)(kBox >> 4) << 16) | ((unsigned long long)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ void mma_f16(unsigned d, unsigned long long a, unsigned long long b,
+                                        unsigned idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((unsigned)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(unsigned long long* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(
+          smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(unsigned long long* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// 32 accumulator columns of this thread's row.
+__device__ __forceinline__ void tmem_load32(unsigned addr, float (&v)[32]) {
+  unsigned* u = reinterpret_cast<unsigned*>(v);
+  __syncwarp();
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+      "%30, %31}, [%32];\n"
+      "tcgen05.wait::ld.sync.aligned;\n"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]),
+        "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]),
+        "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]),
+        "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]),
+        "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+      : "r"(addr)
+      : "memory");
+}
+
+// Where a tile is.  Tiles are numbered phase by phase (A, A^2, B X of step 0,
+// of step 1, ...), inside a phase matrix by matrix; CTA c takes numbers c,
+// c + gridDim.x, ...  A tile waits only for tiles of earlier phases, and every
+// CTA is resident, so the lowest unfinished tile can always proceed.
+struct Tile {
+  int phase, step;                 // phase 0: A, 1: A^2, 2: B X
+  int group, mat;                  // mat counts over the whole call
+  int i0, j0, bn, kblocks;
+};
+
+struct Walk {
+  int step = 0, phase = 0;
+  long long t;
+  __device__ explicit Walk(long long first) : t(first) {}
+  __device__ bool next(const NsArgs& a, Tile* o) {
+    for (;;) {
+      const int n = phase == 2 ? a.tiles_app : a.tiles_sym;
+      if (t < n) break;
+      t -= n;
+      if (++phase == 3) {
+        phase = 0;
+        if (++step == a.steps) return false;
+      }
+    }
+    int r = (int)t, gi = 0;
+    for (;; ++gi) {
+      const NsGroup& g = a.g[gi];
+      const int n = g.batch * (phase == 2 ? g.tiles_app : g.tiles_sym);
+      if (r < n) break;
+      r -= n;
+    }
+    const NsGroup& g = a.g[gi];
+    o->phase = phase;
+    o->step = step;
+    o->group = gi;
+    if (phase == 2) {
+      const int b = r / g.tiles_app;
+      r -= b * g.tiles_app;
+      o->mat = g.first + b;
+      o->bn = g.bn_app;
+      const int tn = (g.cols + o->bn - 1) / o->bn;
+      o->i0 = r / tn * BM;
+      o->j0 = r % tn * o->bn;
+      o->kblocks = (g.s + BK - 1) / BK;
+    } else {
+      const int b = r / g.tiles_sym;
+      r -= b * g.tiles_sym;
+      o->mat = g.first + b;
+      o->bn = g.bn_sym;
+      // lower triangle by 128-row blocks; see sym_tiles
+      int ti, tj;
+      if (o->bn == 128) {
+        int u = (int)((sqrtf(8.f * r + 1.f) - 1.f) * 0.5f);
+        while (u * (u + 1) / 2 > r) --u;
+        while ((u + 1) * (u + 2) / 2 <= r) ++u;
+        ti = u;
+        tj = r - u * (u + 1) / 2;
+      } else {
+        int u = (int)((sqrtf(4.f * r + 1.f) - 1.f) * 0.5f);
+        while (u * (u + 1) > r) --u;
+        while ((u + 1) * (u + 2) <= r) ++u;
+        r -= u * (u + 1);
+        ti = o->bn == 256 ? 2 * u + r / (u + 1) : u;
+        tj = o->bn == 256 ? r % (u + 1) : r;
+      }
+      o->i0 = ti * BM;
+      o->j0 = tj * o->bn;
+      o->kblocks = ((phase == 0 ? g.l : g.s) + BK - 1) / BK;
+    }
+    t += gridDim.x;
+    return true;
+  }
+};
+
+// Tiles of the lower triangle of an s x s product: row block ti (128 rows)
+// takes the tiles that start at or left of its own last column.
+static int sym_tiles(int s, int bn) {
+  const int T = (s + 127) / 128, u = T / 2;
+  if (bn == 128) return T * (T + 1) / 2;
+  if (bn == 256) return T % 2 ? (u + 1) * (u + 1) : u * (u + 1);
+  return T * (T + 1);
+}
+
+template <bool SPLIT>
+struct Stage {
+  static constexpr int kParts = SPLIT ? 2 : 1;
+  static constexpr int kBytes = kParts * (BM / 64 + 256 / 64) * kBox;  // 48 or 96 KB
+  static constexpr int kCount = SPLIT ? 2 : 4;
+  static constexpr int kSmem = kCount * kBytes + 1024 + 256;
+};
+
+__device__ __forceinline__ void load_half32(const __half* p, float (&v)[32]) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+  for (int q = 0; q < 4; ++q) {
+    const int4 w = __ldcg(reinterpret_cast<const int4*>(p) + q);
+    const unsigned* u = reinterpret_cast<const unsigned*>(&w);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int i = i0 + ty + 16 * u, j = j0 + tx + 16 * v;
-        if (i >= M || j >= N) continue;
-        const long long o = (long long)i * N + j;
-        const float d = acc[u][v];
-        if (MODE == NS_GRAM) A[o] = d;
-        else if (MODE == NS_SQUARE) B[o] = fmaf(cb, A[o], cc * d);
-        else if (MODE == NS_APPLY) X2[o] = fmaf(ca, X[o], d);
-        else {
-          const float y = fmaf(ca, X[o], d);
-          T* w = reinterpret_cast<T*>(m.dst) + i * m.dst_row + j;
-          *w = St<T>::v(m.mom ? fmaf(a.decay, Ld<T>::f(*w), -m.step * y) : y);
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(u + e));
+      v[8 * q + 2 * e] = f.x;
+      v[8 * q + 2 * e + 1] = f.y;
+    }
+  }
+}
+__device__ __forceinline__ void add_half32(const __half* p, float (&v)[32]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int4 w = __ldcg(reinterpret_cast<const int4*>(p) + q);
+    const unsigned* u = reinterpret_cast<const unsigned*>(&w);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(u + e));
+      v[8 * q + 2 * e] += f.x;
+      v[8 * q + 2 * e + 1] += f.y;
+    }
+  }
+}
+__device__ __forceinline__ void store_half32(__half* p, const __half (&h)[32]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    reinterpret_cast<int4*>(p)[q] = reinterpret_cast<const int4*>(h)[q];
+}
+__device__ __forceinline__ float exp2i(int e) { return __int_as_float((127 + e) << 23); }
+
+// Epilogue of 32 columns [j0, j0 + 32) of row i of a tile; v holds the raw sums.
+template <bool SPLIT, typename T>
+__device__ __forceinline__ void ns_emit(const NsArgs& a, const Tile& t, int i, int j0,
+                                        float (&v)[32]) {
+  const NsGroup& g = a.g[t.group];
+  const NsMat& m = a.m[t.mat];
+  const NsStep& k = a.k[t.step];
+  const int b = t.mat - g.first;
+  if (t.phase < 2) {
+    if (i >= g.s || j0 >= g.s || j0 / BM > t.i0 / BM) return;
+    const long long plane = (long long)b * g.s * g.pa;
+    const float alpha = t.phase == 0 ? exp2i(-2 * k.ex) : exp2i(-2 * k.ea);
+    const float up = exp2i(t.phase == 0 ? k.ea : k.eb);
+    __half* const out0 = t.phase == 0 ? g.a[0] : g.b[0];
+    __half* const out1 = t.phase == 0 ? g.a[1] : g.b[1];
+    float* diag = (t.phase == 0 ? g.da : g.db) + (long long)b * g.pa;
+    if (t.phase == 1) {
+      const float* da = g.da + (long long)b * g.pa;
+      const float di = __ldcg(da + i), down = exp2i(-k.ea);
+      __align__(16) float o[32], dj[32];
+      load_half32(g.a[0] + plane + (long long)i * g.pa + j0, o);
+      if (SPLIT) add_half32(g.a[1] + plane + (long long)i * g.pa + j0, o);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        reinterpret_cast<float4*>(dj)[q] = __ldcg(reinterpret_cast<const float4*>(da + j0) + q);
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        const float ov = o[c] * down, p2 = v[c] * alpha;
+        v[c] = j0 + c == i ? fmaf(k.c, fmaf(di, di, p2), k.b * di)
+                           : fmaf(k.c, fmaf(di + dj[c], ov, p2), k.b * ov);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) v[c] *= alpha;
+    }
+    __align__(16) __half hi[32], lo[32];
+#pragma unroll
+    for (int c = 0; c < 32; ++c) {
+      if (j0 + c == i) {
+        diag[i] = v[c];
+        v[c] = 0.f;
+      }
+      split_half(v[c] * up, &hi[c], &lo[c]);
+    }
+    store_half32(out0 + plane + (long long)i * g.pa + j0, hi);
+    if (SPLIT) store_half32(out1 + plane + (long long)i * g.pa + j0, lo);
+    if (j0 / BM < t.i0 / BM) {  // the mirror image, above the diagonal
+#pragma unroll
+      for (int c = 0; c < 32; ++c) {
+        if (j0 + c < g.s) {
+          const long long o = plane + (long long)(j0 + c) * g.pa + i;
+          out0[o] = hi[c];
+          if (SPLIT) out1[o] = lo[c];
         }
       }
+    }
+  } else {
+    if (i >= g.rows || j0 >= g.cols) return;
+    const int from = t.step & 1;
+    const long long at = ((long long)b * g.rows + i) * g.px + j0;
+    const float* db = g.db + (long long)b * g.pa;
+    const float alpha = exp2i(-k.eb - k.ex), xs = exp2i(-k.ex);
+    float x[32];
+    load_half32(g.x[from][0] + at, x);
+    add_half32(g.x[from][1] + at, x);
+    if (g.tall) {
+      __align__(16) float f[32];
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        reinterpret_cast<float4*>(f)[q] = __ldcg(reinterpret_cast<const float4*>(db + j0) + q);
+#pragma unroll
+      for (int c = 0; c < 32; ++c) v[c] = fmaf(k.a + f[c], x[c] * xs, v[c] * alpha);
+    } else {
+      const float f = k.a + __ldcg(db + i);
+#pragma unroll
+      for (int c = 0; c < 32; ++c) v[c] = fmaf(f, x[c] * xs, v[c] * alpha);
+    }
+    if (t.step + 1 < a.steps) {
+      const float up = exp2i(k.ex2);
+      __align__(16) __half hi[32], lo[32];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) split_half(v[c] * up, &hi[c], &lo[c]);
+      store_half32(g.x[1 - from][0] + at, hi);
+      store_half32(g.x[1 - from][1] + at, lo);
+    } else {
+      T* w = reinterpret_cast<T*>(m.dst) + i * m.dst_row + j0;
+#pragma unroll
+      for (int c = 0; c < 32; ++c)
+        if (j0 + c < g.cols)
+          w[c] = St<T>::v(m.mom ? fmaf(a.decay, Ld<T>::f(w[c]), -m.step * v[c]) : v[c]);
+    }
   }
 }
 
-static long long ns_floats(int rows, int cols) {
-  const long long s = std::min(rows, cols);
-  return 2ll * rows * cols + 2 * s * s;
+// Products of the current matrices.  Warp 0 copies operand tiles into shared
+// memory (TMA), warp 1 issues the products (one thread), warps 4-11 read the
+// accumulators (two, so that a tile's epilogue overlaps the next tile's
+// products).
+template <bool SPLIT, typename T>
+__global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_constant__ NsArgs a) {
+  using St_ = Stage<SPLIT>;
+  constexpr int S = St_::kCount, PARTS = St_::kParts;
+  extern __shared__ char smem_raw[];
+  const unsigned smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  __shared__ unsigned long long full[4], empty[4], tm_full[2], tm_empty[2], sm_empty[2],
+      drain;
+  __shared__ unsigned tmem_base;
+  __shared__ volatile int dead;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tm_full[i], 1);
+      mbar_init(&tm_empty[i], kEpilogue);
+      mbar_init(&sm_empty[i], kEpilogue);
+    }
+    mbar_init(&drain, 1);
+    dead = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    fence_async_smem();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(
+                     smem_u32(&tmem_base))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  const unsigned tmem = tmem_base;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      Walk walk(blockIdx.x);
+      Tile t;
+      unsigned n = 0;  // stages issued
+      bool ok = true;
+      while (ok && walk.next(a, &t)) {
+        const NsGroup& g = a.g[t.group];
+        // what this tile reads: X of the last step, O, or offdiag(B)
+        const int from = t.phase == 0 ? 2 : t.phase - 1;
+        const int rounds = t.phase == 0 ? t.step : t.step + 1;
+        const unsigned want = (unsigned)rounds * (t.phase == 0 ? g.tiles_app : g.tiles_sym);
+        if (!wait_flag(a.done + from * kMats + t.mat, want, a)) break;
+        asm volatile("fence.proxy.async;\n" ::: "memory");
+        const int xi = MAP_X0 + (t.step & 1);
+        const int mp = t.phase == 0 ? xi : t.phase == 1 ? MAP_A : g.tall ? xi : MAP_B;
+        const int mq = t.phase == 0 ? xi : t.phase == 1 ? MAP_A : g.tall ? MAP_B : xi;
+        const bool p_mn = t.phase == 0 && g.tall;
+        const bool q_mn = t.phase == 0 ? g.tall : t.phase == 2 && !g.tall;
+        const int z = t.mat - g.first, qb = t.bn / 64;
+        for (int kb = 0; kb < t.kblocks; ++kb, ++n) {
+          const int s = n % S;
+          if (n >= (unsigned)S && !wait_bar(&empty[s], (n / S - 1) & 1, a)) {
+            ok = false;
+            break;
+          }
+          const unsigned bar = smem_u32(&full[s]);
+          const unsigned base = smem0 + s * St_::kBytes;
+          mbar_expect_tx(&full[s], PARTS * (BM / 64 + qb) * kBox);
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) {
+            const unsigned bp = base + part * (BM / 64) * kBox;
+            const unsigned bq = base + (PARTS * (BM / 64) + part * 4) * kBox;
+            for (int i = 0; i < BM / 64; ++i)
+              tma_box(bp + i * kBox, &g.map[mp][part], p_mn ? t.i0 + 64 * i : kb * BK,
+                      p_mn ? kb * BK : t.i0 + 64 * i, z, bar);
+            for (int i = 0; i < qb; ++i)
+              tma_box(bq + i * kBox, &g.map[mq][part], q_mn ? t.j0 + 64 * i : kb * BK,
+                      q_mn ? kb * BK : t.j0 + 64 * i, z, bar);
+          }
+        }
+      }
+      // copies still in flight land before the block ends
+      for (unsigned i = n > (unsigned)S ? n - S : 0; i < n; ++i)
+        wait_bar(&full[i % S], (i / S) & 1, a);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      Walk walk(blockIdx.x);
+      Tile t;
+      unsigned n = 0, tile = 0, sums = 0;
+      bool ok = true;
+      for (; ok && walk.next(a, &t); ++tile) {
+        const NsGroup& g = a.g[t.group];
+        const bool p_mn = t.phase == 0 && g.tall;
+        const bool q_mn = t.phase == 0 ? g.tall : t.phase == 2 && !g.tall;
+        // float32 accumulators, float16 operands, M = 128
+        const unsigned idesc = (1u << 4) | ((unsigned)p_mn << 15) | ((unsigned)q_mn << 16) |
+                               ((unsigned)(t.bn / 8) << 17) | ((unsigned)(BM / 16) << 24);
+        const int chunk = SPLIT ? kChunk : t.kblocks;
+        const unsigned ps = (p_mn ? 2048u : 32u) >> 4, qs = (q_mn ? 2048u : 32u) >> 4;
+        if (SPLIT && tile >= 2 && !wait_bar(&sm_empty[tile & 1], (tile / 2 - 1) & 1, a)) break;
+        const unsigned dsmall = tmem + 256 + (tile & 1) * 128;
+        for (int kb0 = 0; ok && kb0 < t.kblocks; kb0 += chunk, ++sums) {
+          const int buf = sums & 1;
+          if (sums >= 2 && !wait_bar(&tm_empty[buf], (sums / 2 - 1) & 1, a)) {
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          const unsigned d = tmem + buf * (SPLIT ? 128 : 256);
+          const int kb1 = min(t.kblocks, kb0 + chunk);
+          for (int kb = kb0; kb < kb1; ++kb, ++n) {
+            const int s = n % S;
+            if (!wait_bar(&full[s], (n / S) & 1, a)) {
+              ok = false;
+              break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            const unsigned base = smem0 + s * St_::kBytes;
+            const unsigned long long p0 = operand(base);
+            const unsigned long long q0 = operand(base + PARTS * (BM / 64) * kBox);
+            const unsigned long long p1 = p0 + ((BM / 64) * kBox >> 4), q1 = q0 + (4 * kBox >> 4);
+#pragma unroll
+            for (int k = 0; k < BK / 16; ++k) {
+              const unsigned long long po = k * ps, qo = k * qs;
+              if (SPLIT) {
+                mma_f16(dsmall, p0 + po, q1 + qo, idesc, kb > 0 || k > 0);
+                mma_f16(dsmall, p1 + po, q0 + qo, idesc, true);
+              }
+              mma_f16(d, p0 + po, q0 + qo, idesc, kb > kb0 || k > 0);
+            }
+            mma_commit(&empty[s]);
+          }
+          mma_commit(&tm_full[buf]);
+        }
+      }
+      // products still in flight end before tensor memory is given back
+      mma_commit(&drain);
+      wait_bar(&drain, 0, a);
+    }
+  } else if (warp >= 4) {
+    Walk walk(blockIdx.x);
+    Tile t;
+    const int w = warp & 3, h = (warp - 4) >> 2;
+    unsigned sums = 0;
+    for (unsigned tile = 0; walk.next(a, &t); ++tile) {
+      const NsGroup& g = a.g[t.group];
+      const int half = t.bn / 2;
+      const unsigned lanes = (unsigned)(32 * w) << 16;
+      // this thread's row, columns t.j0 + h * half + [0, half)
+      const int i = t.i0 + 32 * w + lane, jh = t.j0 + h * half;
+      const int chunks = SPLIT ? (t.kblocks + kChunk - 1) / kChunk : 1;
+      __align__(16) float sum[SPLIT ? 2 : 1][32];
+      bool ok = true;
+      for (int ch = 0; ch < chunks; ++ch, ++sums) {
+        const int buf = sums & 1;
+        if (lane == 0) ok = ok && wait_bar(&tm_full[buf], (sums / 2) & 1, a);
+        __syncwarp();
+        if constexpr (SPLIT) {
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            if (q * 32 >= half) break;
+            float v[32];
+            tmem_load32(tmem + buf * 128 + h * half + q * 32 + lanes, v);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) sum[q][c] = ch ? sum[q][c] + v[c] : v[c];
+          }
+          __syncwarp();
+          asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+          mbar_arrive(&tm_empty[buf]);
+        }
+      }
+      if (!ok) dead = 1;
+      asm volatile("bar.sync 1, 256;\n" ::: "memory");
+      if (dead) break;
+      // the producer waited for what the products read; order this thread's loads too
+      ld_acquire(a.done + (t.phase == 0 ? 2 : t.phase - 1) * kMats + t.mat);
+      if constexpr (SPLIT) {
+        // the small products of the whole tile are complete with its last chunk
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          if (q * 32 >= half) break;
+          float v[32];
+          tmem_load32(tmem + 256 + (tile & 1) * 128 + h * half + q * 32 + lanes, v);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) sum[q][c] += v[c];
+        }
+        __syncwarp();
+        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+        mbar_arrive(&sm_empty[tile & 1]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          if (q * 32 < half) ns_emit<SPLIT, T>(a, t, i, jh + q * 32, sum[q]);
+      } else {
+        const int buf = (sums - 1) & 1;
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        for (int c0 = 0; c0 < half; c0 += 32) {
+          tmem_load32(tmem + buf * 256 + h * half + c0 + lanes, sum[0]);
+          if (c0 + 32 >= half) {
+            __syncwarp();
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+            mbar_arrive(&tm_empty[buf]);
+          }
+          ns_emit<SPLIT, T>(a, t, i, jh + c0, sum[0]);
+        }
+      }
+      // other blocks read these values through TMA: order them before the count
+      asm volatile("fence.proxy.async;\n" ::: "memory");
+      asm volatile("bar.sync 1, 256;\n" ::: "memory");
+      if (threadIdx.x == 128) {
+        __threadfence();
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;\n" ::"l"(a.done + t.phase * kMats +
+                                                                       t.mat)
+                     : "memory");
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  if (warp == 2) {
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
+  }
 }
 
-static constexpr size_t kNsHead = sizeof(double) * kMats * kNormBlocks;
+// ---------------------------------------------------------------------------
+// host
+// ---------------------------------------------------------------------------
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiledFn encode_tiled() {
+  static const EncodeTiledFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) !=
+            cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<EncodeTiledFn>(f);
+  }();
+  return fn;
+}
+
+// [batch][rows][pitch] float16 with `cols` live columns; boxes of 64 x 64.
+// Elements outside arrive as zeros.
+static bool half_map(CUtensorMap* map, __half* p, int batch, int rows, int cols, int pitch) {
+  EncodeTiledFn fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t dim[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch};
+  const cuuint64_t stride[2] = {(cuuint64_t)pitch * 2, (cuuint64_t)pitch * 2 * rows};
+  const cuuint32_t box[3] = {64, 64, 1}, one[3] = {1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p, dim, stride, box, one,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static constexpr size_t kNsHead = sizeof(double) * kMats * kNormBlocks + 4 * (3 * kMats + 1);
+
+static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+static int pitch64(int n) { return (n + 63) / 64 * 64; }
+
+// The next matrices that share a launch sequence: at most kMats, of at most
+// kGroups shapes.  Members of one shape are numbered together.
+struct Batch {
+  int n = 0, groups = 0;
+  int member[kMats];               // call index of matrix i
+  int group[kMats];                // its shape
+  int rows[kGroups], cols[kGroups], count[kGroups], first[kGroups];
+};
+
+static int take_batch(const fa_matrix* m, int from, int count, Batch* o) {
+  int raw_group[kMats];
+  int n = 0;
+  o->groups = 0;
+  for (; n < kMats && from + n < count; ++n) {
+    int g = 0;
+    while (g < o->groups && (o->rows[g] != m[from + n].rows || o->cols[g] != m[from + n].cols)) ++g;
+    if (g == o->groups) {
+      if (g == kGroups) break;
+      o->rows[g] = m[from + n].rows;
+      o->cols[g] = m[from + n].cols;
+      o->count[g] = 0;
+      ++o->groups;
+    }
+    ++o->count[g];
+    raw_group[n] = g;
+  }
+  int at[kGroups], sum = 0;
+  for (int g = 0; g < o->groups; ++g) {
+    o->first[g] = at[g] = sum;
+    sum += o->count[g];
+  }
+  for (int i = 0; i < n; ++i) {
+    const int k = at[raw_group[i]]++;
+    o->member[k] = from + i;
+    o->group[k] = raw_group[i];
+  }
+  o->n = n;
+  return n;
+}
+
+// Workspace of one shape, and its pointers when `base` is given.
+static size_t group_layout(NsGroup* g, bool split, char* base) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    char* p = base ? base + off : nullptr;
+    off += up256(bytes);
+    return p;
+  };
+  const size_t x = (size_t)2 * g->batch * g->rows * g->px, q = (size_t)2 * g->batch * g->s * g->pa;
+  for (int i = 0; i < 2; ++i)
+    for (int h = 0; h < 2; ++h) g->x[i][h] = reinterpret_cast<__half*>(take(x));
+  for (int h = 0; h < (split ? 2 : 1); ++h) {
+    g->a[h] = reinterpret_cast<__half*>(take(q));
+    g->b[h] = reinterpret_cast<__half*>(take(q));
+  }
+  g->da = reinterpret_cast<float*>(take((size_t)4 * g->batch * g->pa));
+  g->db = reinterpret_cast<float*>(take((size_t)4 * g->batch * g->pa));
+  return off;
+}
+
+static void group_shape(NsGroup* g, int rows, int cols, int batch, int first) {
+  g->rows = rows;
+  g->cols = cols;
+  g->s = std::min(rows, cols);
+  g->l = std::max(rows, cols);
+  g->tall = rows > cols;
+  g->batch = batch;
+  g->first = first;
+  g->px = pitch64(cols);
+  g->pa = pitch64(g->s);
+}
 
 size_t ns_ws_bytes(const fa_matrix* m, int count, int dtype) {
-  (void)dtype;
-  long long most = 0;
-  for (int i = 0; i < count; i += kMats) {
-    long long f = 0;
-    for (int j = i; j < std::min(count, i + kMats); ++j) f += ns_floats(m[j].rows, m[j].cols);
-    most = std::max(most, f);
+  size_t most = 0;
+  Batch b;
+  for (int i = 0; i < count; i += take_batch(m, i, count, &b)) {
+    take_batch(m, i, count, &b);
+    size_t sum = 0;
+    for (int g = 0; g < b.groups; ++g) {
+      NsGroup gr{};
+      group_shape(&gr, b.rows[g], b.cols[g], b.count[g], 0);
+      sum += group_layout(&gr, dtype != FA_BF16, nullptr);
+    }
+    most = std::max(most, sum);
   }
-  return kNsHead + 4 * (size_t)most;
-}
-
-template <typename T>
-static int ns_run(NsArgs& a, int count, const double* coef, int steps, int device,
-                  cudaStream_t st) {
-  const unsigned y = (unsigned)count;
-  int tiles = 1;
-  for (int i = 0; i < count; ++i)
-    tiles = std::max(tiles, ((a.m[i].rows + 63) / 64) * ((a.m[i].cols + 63) / 64));
-  const unsigned gx = (unsigned)std::min(tiles, std::max(1, sm_count(device) * 8 / count));
-  ns_norm_kernel<T><<<dim3(kNormBlocks, y), 256, 0, st>>>(a);
-  ns_pack_kernel<T><<<dim3(kNormBlocks, y), 256, 0, st>>>(a);
-  for (int k = 0; k < steps; ++k) {
-    const float ca = (float)coef[3 * k], cb = (float)coef[3 * k + 1], cc = (float)coef[3 * k + 2];
-    ns_product_kernel<NS_GRAM, T><<<dim3(gx, y), 256, 0, st>>>(a, k & 1, ca, cb, cc);
-    ns_product_kernel<NS_SQUARE, T><<<dim3(gx, y), 256, 0, st>>>(a, k & 1, ca, cb, cc);
-    if (k + 1 < steps)
-      ns_product_kernel<NS_APPLY, T><<<dim3(gx, y), 256, 0, st>>>(a, k & 1, ca, cb, cc);
-    else
-      ns_product_kernel<NS_FINAL, T><<<dim3(gx, y), 256, 0, st>>>(a, k & 1, ca, cb, cc);
-  }
-  FAB_LAUNCH_CHECK();
-  return FA_OK;
+  return up256(kNsHead) + most;
 }
 
 // Everything about a call that can be refused before the device is touched.
@@ -204,8 +844,66 @@ int ns_check(const fa_matrix* m, int count, int dtype, bool update) {
   for (int i = 0; i < count; ++i) {
     if (!m[i].src || !m[i].dst || (update && !m[i].momentum)) return FA_E_ARG;
     if (m[i].rows <= 0 || m[i].cols <= 0) return FA_E_SHAPE;
+    if (std::min(m[i].rows, m[i].cols) > 32768 || std::max(m[i].rows, m[i].cols) > (1 << 22))
+      return FA_E_SHAPE;
     if (m[i].src_row_stride < m[i].cols || m[i].dst_row_stride < m[i].cols) return FA_E_SHAPE;
   }
+  return FA_OK;
+}
+
+// Exponents that keep the stored float16 values below 2^15: the largest
+// singular value after each step follows from the polynomial on [0, the last
+// bound], and every entry of X, A, B is at most the matrix's largest singular
+// value.  False where the iteration may grow beyond what they can hold.
+static bool plan_steps(NsStep* k, const double* coef, int steps) {
+  double top = 1.0;
+  auto exponent = [](double bound) { return 14 - (int)std::ceil(std::log2(std::max(bound, 1.0))); };
+  for (int i = 0; i < steps; ++i) {
+    const double a = coef[3 * i], b = coef[3 * i + 1], c = coef[3 * i + 2];
+    if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
+    k[i].a = (float)a;
+    k[i].b = (float)b;
+    k[i].c = (float)c;
+    const double edge = top * 1.02;
+    double next = 0, inner = 0;
+    for (int j = 0; j <= 2048; ++j) {
+      const double s = edge * j / 2048, q = s * s * (b + c * s * s);
+      inner = std::max(inner, std::fabs(q));
+      next = std::max(next, std::fabs(s * (a + q)));
+    }
+    k[i].ex = exponent(edge);
+    k[i].ea = exponent(edge * edge);
+    k[i].eb = exponent(inner);
+    k[i].ex2 = exponent(next * 1.02);
+    if (!(next <= 128.0) || !(inner <= 8192.0)) return false;
+    top = next;
+  }
+  return true;
+}
+
+template <bool SPLIT, typename T>
+static int ns_run(const NsArgs& a, int device, cudaStream_t st) {
+  const int sms = sm_count(device);
+  long long most = 0;
+  for (int g = 0; g < a.groups; ++g)
+    most = std::max<long long>(most, (long long)a.g[g].rows * a.g[g].px);
+  const int nb = (int)std::max<long long>(
+      1, std::min<long long>(std::min<long long>(kNormBlocks, (most + 4095) / 4096),
+                             std::max(1, sms * 8 / a.mats)));
+  ns_norm_kernel<T><<<dim3(nb, a.mats), 256, 0, st>>>(a);
+  FAB_LAUNCH_CHECK();
+  const int pb = (int)std::max<long long>(
+      1, std::min<long long>((most + 2047) / 2048, std::max(1, sms * 8 / a.mats)));
+  ns_pack_kernel<T><<<dim3(pb, a.mats), 256, 0, st>>>(a, nb);
+  FAB_LAUNCH_CHECK();
+  constexpr int smem = Stage<SPLIT>::kSmem;
+  FAB_TRY(cudaFuncSetAttribute(ns_product_kernel<SPLIT, T>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // every block waits for other blocks' tiles: a cooperative launch makes them resident
+  const unsigned grid = (unsigned)std::min(sms, std::max(a.tiles_sym, a.tiles_app));
+  void* args[] = {const_cast<NsArgs*>(&a)};
+  FAB_TRY(cudaLaunchCooperativeKernel(reinterpret_cast<void*>(ns_product_kernel<SPLIT, T>),
+                                      dim3(grid), dim3(kThreads), args, smem, st));
   return FA_OK;
 }
 
@@ -213,37 +911,63 @@ int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int
             bool update, double mu, int nesterov, double decay, void* ws, size_t ws_bytes,
             int device, cudaStream_t st) {
   if (!coef || !ws) return FA_E_ARG;
-  if (steps < 1) return FA_E_SHAPE;
-  for (int i0 = 0; i0 < count; i0 += kMats) {
-    const int n = std::min(kMats, count - i0);
-    NsArgs a{};
-    a.part = reinterpret_cast<double*>(ws);
-    a.ws = reinterpret_cast<float*>(static_cast<char*>(ws) + kNsHead);
-    a.mu = (float)mu;
-    a.nesterov = nesterov;
-    a.decay = (float)decay;
-    long long off = 0;
-    for (int i = 0; i < n; ++i) {
-      const fa_matrix& f = mats[i0 + i];
+  if (steps < 1 || steps > kMaxSteps) return FA_E_SHAPE;
+  const bool split = dtype != FA_BF16;
+  NsArgs a;
+  a.steps = steps;
+  if (!plan_steps(a.k, coef, steps)) return FA_E_ARG;
+  a.err = wait_error_word();
+  if (!a.err) return FA_E_INTERNAL;
+  a.mu = (float)mu;
+  a.decay = (float)decay;
+  a.nesterov = nesterov;
+  const uintptr_t base = reinterpret_cast<uintptr_t>(ws);
+  if (base & 255) return FA_E_ARG;
+  a.part = reinterpret_cast<double*>(ws);
+  a.done = reinterpret_cast<unsigned*>(a.part + kMats * kNormBlocks);
+  a.failed = a.done + 3 * kMats;
+  Batch bt;
+  for (int i0 = 0; i0 < count; i0 += bt.n) {
+    take_batch(mats, i0, count, &bt);
+    size_t off = up256(kNsHead);
+    a.groups = bt.groups;
+    a.mats = bt.n;
+    a.tiles_sym = a.tiles_app = 0;
+    for (int gi = 0; gi < bt.groups; ++gi) {
+      NsGroup& g = a.g[gi];
+      group_shape(&g, bt.rows[gi], bt.cols[gi], bt.count[gi], bt.first[gi]);
+      off += group_layout(&g, split, static_cast<char*>(ws) + off);
+      if (off > ws_bytes) return FA_E_ARG;
+      g.bn_sym = 128;
+      g.bn_app = 128;
+      g.tiles_sym = sym_tiles(g.s, g.bn_sym);
+      g.tiles_app = (g.rows + BM - 1) / BM * ((g.cols + g.bn_app - 1) / g.bn_app);
+      a.tiles_sym += g.batch * g.tiles_sym;
+      a.tiles_app += g.batch * g.tiles_app;
+      for (int h = 0; h < (split ? 2 : 1); ++h) {
+        if (!half_map(&g.map[MAP_X0][h], g.x[0][h], g.batch, g.rows, g.cols, g.px) ||
+            !half_map(&g.map[MAP_X1][h], g.x[1][h], g.batch, g.rows, g.cols, g.px) ||
+            !half_map(&g.map[MAP_A][h], g.a[h], g.batch, g.s, g.s, g.pa) ||
+            !half_map(&g.map[MAP_B][h], g.b[h], g.batch, g.s, g.s, g.pa))
+          return FA_E_INTERNAL;
+      }
+    }
+    for (int i = 0; i < bt.n; ++i) {
+      const fa_matrix& f = mats[bt.member[i]];
       NsMat& m = a.m[i];
       m.src = f.src;
       m.dst = f.dst;
       m.mom = update ? f.momentum : nullptr;
-      m.rows = f.rows;
-      m.cols = f.cols;
       m.src_row = f.src_row_stride;
       m.dst_row = f.dst_row_stride;
       m.step = (float)f.step;
-      m.x_off = off;
-      m.a_off = off + 2ll * f.rows * f.cols;
-      off += ns_floats(f.rows, f.cols);
+      m.group = bt.group[i];
     }
-    if (ws_bytes < kNsHead + 4 * (size_t)off) return FA_E_ARG;
     int rc;
     switch (dtype) {
-      case FA_F16: rc = ns_run<f16_t>(a, n, coef, steps, device, st); break;
-      case FA_BF16: rc = ns_run<bf16_t>(a, n, coef, steps, device, st); break;
-      default: rc = ns_run<float>(a, n, coef, steps, device, st); break;
+      case FA_F16: rc = ns_run<true, f16_t>(a, device, st); break;
+      case FA_BF16: rc = ns_run<false, bf16_t>(a, device, st); break;
+      default: rc = ns_run<true, float>(a, device, st); break;
     }
     if (rc) return rc;
   }
