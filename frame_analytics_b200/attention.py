@@ -76,10 +76,10 @@ class _QkNormRotary(torch.autograd.Function):
         L = backend.lib()
         nb = backend._cached_ws("qk", L.fa_b200_qk_norm_rotary_backward_workspace_bytes,
                                 q.shape[0], q.shape[1], q.shape[2], k.shape[2], q.shape[3])
-        ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
+        ws = backend.workspace(q, nb)
         backend._call(q, L.fa_b200_qk_norm_rotary_backward, _heads(q), _heads(k), _heads(gq),
                       _heads(gk), _heads(dq), _heads(dk), p, backend._ptr(dqw),
-                      backend._ptr(dkw), ws.data_ptr(), nb, backend._dev(q), backend._stream(q))
+                      backend._ptr(dkw), ws.data_ptr(), ws.numel(), backend._dev(q), backend._stream(q))
         return dq, dk, dqw, dkw, None, None, None, None, None
 
 

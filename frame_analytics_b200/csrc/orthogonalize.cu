@@ -39,7 +39,7 @@ namespace fab {
 constexpr int kMats = 128;         // matrices of one launch sequence
 constexpr int kGroups = 8;         // shapes of one launch sequence
 constexpr int kMaxSteps = 32;
-constexpr int kNormBlocks = 64;    // partial sums of squares of one matrix, at most
+constexpr int kNormBlocks = 512;   // partial sums of squares of one matrix, at most
 
 constexpr int BM = 128;            // tile rows: the lanes of tensor memory
 constexpr int BK = 64;             // 128 bytes of float16: one swizzle row
@@ -74,6 +74,7 @@ struct NsMat {
   long long src_row, dst_row;
   float step;                      // W <- decay W - step O
   int group;
+  int vec;                         // rows are whole aligned 16-byte vectors
 };
 
 struct NsStep {
@@ -99,6 +100,54 @@ struct NsArgs {
 // momentum, norm, packing
 // ---------------------------------------------------------------------------
 
+// Both passes read the gradient and the momentum once each: a warp takes 512
+// columns of a row at a time, 8 to a lane and load.
+constexpr int kSpan = 512;
+
+// Update values u[8] of columns [c, c + 8) of row r (zeros past the last
+// column).  STORE writes the new momentum; otherwise it was written before.
+template <typename T, bool STORE>
+__device__ __forceinline__ void ns_update(const NsArgs& a, const NsMat& m, int r, int c, int cols,
+                                          float (&u)[8]) {
+  const T* src = reinterpret_cast<const T*>(m.src) + r * m.src_row + c;
+  const int n = min(8, cols - c);
+  if (m.vec) {  // n is 8
+    __align__(16) T e[8];
+#pragma unroll
+    for (int q = 0; q < (int)sizeof(T) / 2; ++q)
+      reinterpret_cast<uint4*>(e)[q] = __ldg(reinterpret_cast<const uint4*>(src) + q);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = Ld<T>::f(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = i < n ? Ld<T>::f(src[i]) : 0.f;
+  }
+  if (!m.mom) return;
+  float* mom = m.mom + (long long)r * cols + c;
+  __align__(16) float v[8];
+  if (m.vec) {
+    reinterpret_cast<float4*>(v)[0] = reinterpret_cast<const float4*>(mom)[0];
+    reinterpret_cast<float4*>(v)[1] = reinterpret_cast<const float4*>(mom)[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? mom[i] : 0.f;
+  }
+  if constexpr (STORE) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = fmaf(a.mu, v[i], u[i]);
+    if (m.vec) {
+      reinterpret_cast<float4*>(mom)[0] = reinterpret_cast<const float4*>(v)[0];
+      reinterpret_cast<float4*>(mom)[1] = reinterpret_cast<const float4*>(v)[1];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) mom[i] = v[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) u[i] = a.nesterov ? fmaf(a.mu, v[i], u[i]) : v[i];
+}
+
 // Updates the momentum and sums the squares of the update, in double: float32
 // squares of a float32 matrix could leave its range.
 template <typename T>
@@ -106,18 +155,20 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ Ns
   __shared__ double sm[32];
   const NsMat& m = a.m[blockIdx.y];
   const NsGroup& g = a.g[m.group];
-  const long long n = (long long)g.rows * g.cols;
-  const T* src = reinterpret_cast<const T*>(m.src);
+  const int spans = (g.cols + kSpan - 1) / kSpan, lane = threadIdx.x & 31;
+  const long long items = (long long)g.rows * spans;
   double ss = 0;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += 256ll * gridDim.x) {
-    const long long r = i / g.cols, c = i - r * g.cols;
-    float u = Ld<T>::f(src[r * m.src_row + c]);
-    if (m.mom) {
-      const float v = fmaf(a.mu, m.mom[i], u);
-      m.mom[i] = v;
-      u = a.nesterov ? fmaf(a.mu, v, u) : v;
+  for (long long it = blockIdx.x * 8ll + (threadIdx.x >> 5); it < items; it += 8ll * gridDim.x) {
+    const int r = (int)(it / spans), c0 = (int)(it - (long long)r * spans) * kSpan + 8 * lane;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = c0 + 256 * h;
+      if (c >= g.cols) continue;
+      float u[8];
+      ns_update<T, true>(a, m, r, c, g.cols, u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss += (double)u[i] * u[i];
     }
-    ss += (double)u * u;
   }
   ss = block_sum(ss, sm);
   if (threadIdx.x == 0) a.part[blockIdx.y * kNormBlocks + blockIdx.x] = ss;
@@ -135,30 +186,41 @@ __device__ __forceinline__ void split_half(float v, __half* hi, __half* lo) {
 template <typename T>
 __global__ void __launch_bounds__(256) ns_pack_kernel(const __grid_constant__ NsArgs a,
                                                       int norm_blocks) {
+  __shared__ double sm[32];
   const NsMat& m = a.m[blockIdx.y];
   const NsGroup& g = a.g[m.group];
-  const T* src = reinterpret_cast<const T*>(m.src);
   double ss = 0;
-  for (int i = 0; i < norm_blocks; ++i) ss += a.part[blockIdx.y * kNormBlocks + i];
+  for (int i = threadIdx.x; i < norm_blocks; i += 256)
+    ss += __ldg(a.part + blockIdx.y * kNormBlocks + i);
+  ss = block_sum(ss, sm);
   const bool finite = ss <= 1.7e308;
   const double inv = ss > 0 ? ldexp(1.0, a.k[0].ex) / sqrt(ss) : 0.0;
-  const long long n = (long long)g.rows * g.px;
-  const long long base = (long long)(blockIdx.y - g.first) * n;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += 256ll * gridDim.x) {
-    const long long r = i / g.px, c = i - r * g.px;
-    float u = 0.f;
-    if (c < g.cols) {
-      u = Ld<T>::f(src[r * m.src_row + c]);
-      if (m.mom) {
-        const float v = m.mom[r * g.cols + c];
-        u = a.nesterov ? fmaf(a.mu, v, u) : v;
+  // inv = f 2^e, the power in two exact steps: no product leaves float's range
+  int e;
+  const float f = (float)frexp(inv, &e);
+  const float e1 = ldexpf(1.f, e / 2), e2 = ldexpf(1.f, e - e / 2);
+  const int spans = (g.px + kSpan - 1) / kSpan, lane = threadIdx.x & 31;
+  const long long items = (long long)g.rows * spans;
+  const long long base = (long long)(blockIdx.y - g.first) * g.rows * g.px;
+  for (long long it = blockIdx.x * 8ll + (threadIdx.x >> 5); it < items; it += 8ll * gridDim.x) {
+    const int r = (int)(it / spans), c0 = (int)(it - (long long)r * spans) * kSpan + 8 * lane;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = c0 + 256 * h;
+      if (c >= g.px) continue;
+      float u[8] = {};
+      if (c < g.cols) ns_update<T, false>(a, m, r, c, g.cols, u);
+      __align__(16) __half hi[8], lo[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float x = u[i] * e1 * e2 * f;
+        if (!finite && c + i < g.cols) x = __int_as_float(0x7fffffff);
+        split_half(x, &hi[i], &lo[i]);
       }
-      u = finite ? (float)(u * inv) : __int_as_float(0x7fffffff);
+      const long long o = base + (long long)r * g.px + c;
+      *reinterpret_cast<uint4*>(g.x[0][0] + o) = *reinterpret_cast<const uint4*>(hi);
+      *reinterpret_cast<uint4*>(g.x[0][1] + o) = *reinterpret_cast<const uint4*>(lo);
     }
-    __half hi, lo;
-    split_half(u, &hi, &lo);
-    g.x[0][0][base + i] = hi;
-    g.x[0][1][base + i] = lo;
   }
 }
 
@@ -821,6 +883,31 @@ static void group_shape(NsGroup* g, int rows, int cols, int batch, int first) {
   g->pa = pitch64(g->s);
 }
 
+static int tile_count(const NsGroup& g, bool sym, int bn) {
+  return sym ? sym_tiles(g.s, bn) : (g.rows + BM - 1) / BM * ((g.cols + bn - 1) / bn);
+}
+
+// Columns of a tile.  Wider tiles reuse the row operand more (measured on
+// 4096 x 8192: a tile of 64, 128, 256 columns takes 0.57, 0.71, 1 of the time
+// of the last), narrower ones fill more multiprocessors: the fewest waves
+// times the time of one.  Three products (split) hold their sums in registers
+// and two accumulators each, which leaves room for 128 columns.
+static int pick_bn(const NsGroup& g, bool sym, bool split, int sms) {
+  static const int width[3] = {64, 128, 256};
+  static const double cost[3] = {0.57, 0.71, 1.0};
+  int best = 64;
+  double least = 1e300;
+  for (int i = 0; i < (split ? 2 : 3); ++i) {
+    const long long tiles = (long long)g.batch * tile_count(g, sym, width[i]);
+    const double c = (double)((tiles + sms - 1) / sms) * cost[i];
+    if (c < least) {
+      least = c;
+      best = width[i];
+    }
+  }
+  return best;
+}
+
 size_t ns_ws_bytes(const fa_matrix* m, int count, int dtype) {
   size_t most = 0;
   Batch b;
@@ -889,11 +976,11 @@ static int ns_run(const NsArgs& a, int device, cudaStream_t st) {
     most = std::max<long long>(most, (long long)a.g[g].rows * a.g[g].px);
   const int nb = (int)std::max<long long>(
       1, std::min<long long>(std::min<long long>(kNormBlocks, (most + 4095) / 4096),
-                             std::max(1, sms * 8 / a.mats)));
+                             std::max(1, sms * 8 / a.mats)));  // 8 warps of 512 columns
   ns_norm_kernel<T><<<dim3(nb, a.mats), 256, 0, st>>>(a);
   FAB_LAUNCH_CHECK();
   const int pb = (int)std::max<long long>(
-      1, std::min<long long>((most + 2047) / 2048, std::max(1, sms * 8 / a.mats)));
+      1, std::min<long long>((most + 4095) / 4096, std::max(1, sms * 8 / a.mats)));
   ns_pack_kernel<T><<<dim3(pb, a.mats), 256, 0, st>>>(a, nb);
   FAB_LAUNCH_CHECK();
   constexpr int smem = Stage<SPLIT>::kSmem;
@@ -938,10 +1025,10 @@ int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int
       group_shape(&g, bt.rows[gi], bt.cols[gi], bt.count[gi], bt.first[gi]);
       off += group_layout(&g, split, static_cast<char*>(ws) + off);
       if (off > ws_bytes) return FA_E_ARG;
-      g.bn_sym = 128;
-      g.bn_app = 128;
-      g.tiles_sym = sym_tiles(g.s, g.bn_sym);
-      g.tiles_app = (g.rows + BM - 1) / BM * ((g.cols + g.bn_app - 1) / g.bn_app);
+      g.bn_sym = pick_bn(g, true, split, sm_count(device));
+      g.bn_app = pick_bn(g, false, split, sm_count(device));
+      g.tiles_sym = tile_count(g, true, g.bn_sym);
+      g.tiles_app = tile_count(g, false, g.bn_app);
       a.tiles_sym += g.batch * g.tiles_sym;
       a.tiles_app += g.batch * g.tiles_app;
       for (int h = 0; h < (split ? 2 : 1); ++h) {
@@ -962,6 +1049,10 @@ int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int
       m.dst_row = f.dst_row_stride;
       m.step = (float)f.step;
       m.group = bt.group[i];
+      const int item = dtype == FA_F32 ? 4 : 2;
+      m.vec = f.cols % 8 == 0 && reinterpret_cast<uintptr_t>(f.src) % 16 == 0 &&
+              (f.rows == 1 || f.src_row_stride * item % 16 == 0) &&
+              (!m.mom || reinterpret_cast<uintptr_t>(m.mom) % 16 == 0);
     }
     int rc;
     switch (dtype) {

@@ -241,19 +241,468 @@ __global__ void __launch_bounds__(128) qk_dw_sum_kernel(const float* part, int c
   else reinterpret_cast<T*>(out)[i] = St<T>::v(sum);
 }
 
+// ---------------------------------------------------------------------------
+// Vector kernels: head sizes and alignments that whole vectors cover.
+//
+// A head vector is held by a group of G lanes (a power of two); a lane owns two
+// chunks of V components, A and B.  Adjacent halves rotate (A with B), so
+// chunk A lies in the first half of the rotated part and B V-for-V in the
+// second; lanes past the rotated part own two chunks of the rest.  Interleaved
+// pairs lie inside a chunk, and A and B are chunks of the two halves of the
+// head.  So no component changes lanes and a row costs two vector loads and
+// stores a lane and log2(G) shuffles.  The angles of a token are loaded once
+// and serve a lane's chunk in `hpi` heads.
+//
+// Both kernels are bound by HBM: the work per component is about 10 (backward:
+// 25) float operations for 4 to 12 bytes.
+// ---------------------------------------------------------------------------
+template <int BYTES> struct RawOf;
+template <> struct RawOf<16> { typedef uint4 type; };
+template <> struct RawOf<8> { typedef uint2 type; };
+// V components as they lie in memory: rows in flight wait unconverted.
+template <typename T, int V> using Raw = typename RawOf<sizeof(T) * V>::type;
+
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> qk_raw(const T* p, bool live) {
+  Raw<T, V> u{};
+  if (live) u = *reinterpret_cast<const Raw<T, V>*>(p);
+  return u;
+}
+template <typename T, int V>
+__device__ __forceinline__ void qk_wide(const Raw<T, V>& u, float (&v)[V]) {
+  const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = Ld<T>::f(e[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void qk_store(T* p, const float (&v)[V]) {
+  Raw<T, V> u;
+  T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+  for (int i = 0; i < V; ++i) e[i] = St<T>::v(v[i]);
+  *reinterpret_cast<Raw<T, V>*>(p) = u;
+}
+
+// What a lane owns: the offsets of its chunks and whether they turn.
+struct QkLane {
+  int a0, b0, t0;     // chunk offsets; first table column (of A when interleaved)
+  int t1;             // interleaved: first table column of B
+  bool live, turn, turn_b;
+};
+template <int V>
+__device__ __forceinline__ QkLane qk_lane(const QkArgs& a, int j) {
+  QkLane q;
+  const int pairs = a.D / (2 * V);
+  q.live = j < pairs;
+  if (!q.live) j = 0;
+  if (a.interleaved) {
+    q.a0 = j * V;
+    q.b0 = a.D / 2 + j * V;
+    q.t0 = q.a0 / 2;
+    q.t1 = q.b0 / 2;
+    q.turn = q.a0 < 2 * a.half;
+    q.turn_b = q.b0 < 2 * a.half;
+  } else {
+    const int rot = a.half / V;
+    q.turn = q.turn_b = j < rot;
+    q.t0 = q.t1 = j * V;
+    const int rest = j - rot, r = 2 * a.half;
+    q.a0 = q.turn ? j * V : r + rest * V;
+    q.b0 = q.turn ? a.half + j * V : r + (a.D - r) / 2 + rest * V;
+  }
+  return q;
+}
+
+// cos and sin of the lane's V pairs: (A[i], B[i]), or interleaved the V/2 pairs
+// of A and then those of B.
+template <int V>
+__device__ __forceinline__ void qk_angles(const QkArgs& a, const QkLane& q, int p, float (&c)[V],
+                                          float (&s)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    c[i] = 1.f;
+    s[i] = 0.f;
+  }
+  const long long o = (long long)max(p, 0) * a.half;
+  if (a.interleaved) {
+    if constexpr (V == 8) {
+      if (q.turn) {
+        *reinterpret_cast<float4*>(c) = __ldg(reinterpret_cast<const float4*>(a.cos_ + o + q.t0));
+        *reinterpret_cast<float4*>(s) = __ldg(reinterpret_cast<const float4*>(a.sin_ + o + q.t0));
+      }
+      if (q.turn_b) {
+        *reinterpret_cast<float4*>(c + 4) = __ldg(reinterpret_cast<const float4*>(a.cos_ + o + q.t1));
+        *reinterpret_cast<float4*>(s + 4) = __ldg(reinterpret_cast<const float4*>(a.sin_ + o + q.t1));
+      }
+    } else {
+      if (q.turn) {
+        *reinterpret_cast<float2*>(c) = __ldg(reinterpret_cast<const float2*>(a.cos_ + o + q.t0));
+        *reinterpret_cast<float2*>(s) = __ldg(reinterpret_cast<const float2*>(a.sin_ + o + q.t0));
+      }
+      if (q.turn_b) {
+        *reinterpret_cast<float2*>(c + 2) = __ldg(reinterpret_cast<const float2*>(a.cos_ + o + q.t1));
+        *reinterpret_cast<float2*>(s + 2) = __ldg(reinterpret_cast<const float2*>(a.sin_ + o + q.t1));
+      }
+    }
+  } else if (q.turn) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      *reinterpret_cast<float4*>(c + i) = __ldg(reinterpret_cast<const float4*>(a.cos_ + o + q.t0 + i));
+      *reinterpret_cast<float4*>(s + i) = __ldg(reinterpret_cast<const float4*>(a.sin_ + o + q.t0 + i));
+    }
+  }
+}
+
+// Turns the chunks that turn by the angles (sign -1: back).  The others are not
+// multiplied by an identity: 0 times an infinity would be NaN.
+template <int V>
+__device__ __forceinline__ void qk_turn(const QkArgs& a, const QkLane& q, float (&x)[V],
+                                        float (&y)[V], const float (&c)[V], const float (&s)[V],
+                                        float sign) {
+  if (a.interleaved) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      const float x0 = x[2 * i], x1 = x[2 * i + 1], y0 = y[2 * i], y1 = y[2 * i + 1];
+      const float sx = sign * s[i], sy = sign * s[V / 2 + i];
+      if (q.turn) {
+        x[2 * i] = fmaf(x0, c[i], -x1 * sx);
+        x[2 * i + 1] = fmaf(x1, c[i], x0 * sx);
+      }
+      if (q.turn_b) {
+        y[2 * i] = fmaf(y0, c[V / 2 + i], -y1 * sy);
+        y[2 * i + 1] = fmaf(y1, c[V / 2 + i], y0 * sy);
+      }
+    }
+  } else if (q.turn) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float x0 = x[i], y0 = y[i], si = sign * s[i];
+      x[i] = fmaf(x0, c[i], -y0 * si);
+      y[i] = fmaf(y0, c[i], x0 * si);
+    }
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void qk_weights(const QkArgs& a, const QkSide& s, const QkLane& q,
+                                           int head, float (&wa)[V], float (&wb)[V]) {
+  if (!s.w) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) wa[i] = wb[i] = 1.f;
+    return;
+  }
+  const long long o = a.per_head ? (long long)head * a.D : 0;
+  if (a.w32) {
+    const float* w = reinterpret_cast<const float*>(s.w) + o;
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+      *reinterpret_cast<float4*>(wa + i) = __ldg(reinterpret_cast<const float4*>(w + q.a0 + i));
+      *reinterpret_cast<float4*>(wb + i) = __ldg(reinterpret_cast<const float4*>(w + q.b0 + i));
+    }
+  } else {
+    const T* w = reinterpret_cast<const T*>(s.w) + o;
+    qk_wide<T, V>(qk_raw<T, V>(w + q.a0, true), wa);
+    qk_wide<T, V>(qk_raw<T, V>(w + q.b0, true), wb);
+  }
+}
+
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Items of `hpi` heads of one side of one token, the items of a token side by
+// side; U rows of a lane are in flight.
+template <typename T, int V, int G, int U>
+__global__ void __launch_bounds__(256, 2) qk_fwd_kernel(const __grid_constant__ QkArgs a, int hpi,
+                                                     int items_q, int items, long long total) {
+  const QkLane q = qk_lane<V>(a, threadIdx.x & (G - 1));
+  const long long item = ((long long)blockIdx.x * 256 + threadIdx.x) / G;
+  // lanes of idle groups stay: the shuffles name the whole warp
+  const bool busy = item < total && q.live;
+  const int t = item < total ? (int)(item / items) : 0;
+  const int it = item < total ? (int)(item - (long long)t * items) : 0;
+  const int b = t / a.L, l = t - b * a.L;
+  const QkSide& s = a.s[it >= items_q];
+  const int h0 = (it >= items_q ? it - items_q : it) * hpi, h1 = min(s.heads, h0 + hpi);
+  __align__(16) float c[V], sn[V], wa[V], wb[V];
+  const int p = qk_position(a, b, l);
+  qk_angles<V>(a, q, p, c, sn);
+  if (!a.per_head) qk_weights<T, V>(a, s, q, 0, wa, wb);
+  const T* x = reinterpret_cast<const T*>(s.x) + b * s.xb + l * s.xl;
+  T* y = reinterpret_cast<T*>(s.out) + b * s.ob + l * s.ol;
+  for (int r = 0; r < hpi; r += U) {
+    Raw<T, V> ra[U], rb[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = h0 + r + u;
+      ra[u] = qk_raw<T, V>(x + h * s.xh + q.a0, busy && h < h1);
+      rb[u] = qk_raw<T, V>(x + h * s.xh + q.b0, busy && h < h1);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float xa[V], xb[V], ss = 0.f;
+      qk_wide<T, V>(ra[u], xa);
+      qk_wide<T, V>(rb[u], xb);
+#pragma unroll
+      for (int i = 0; i < V; ++i) ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
+      float rs = rsqrtf(fmaf(group_sum<G>(ss), a.inv_d, a.eps));
+      if (p < 0) rs = __int_as_float(0x7fffffff);
+      const int h = h0 + r + u;
+      if (busy && h < h1) {
+        if (a.per_head) qk_weights<T, V>(a, s, q, h, wa, wb);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          xa[i] *= rs * wa[i];
+          xb[i] *= rs * wb[i];
+        }
+        qk_turn<V>(a, q, xa, xb, c, sn, 1.f);
+        qk_store<T, V>(y + h * s.oh + q.a0, xa);
+        qk_store<T, V>(y + h * s.oh + q.b0, xb);
+      }
+    }
+  }
+}
+
+// Sums the blocks' partial weight gradients part[block][D] in a fixed order.
+// Blocks whose number is `it` modulo `items` hold item `it`.
+template <typename T>
+__device__ __forceinline__ void qk_dw_finish(const QkArgs& a, const float* part, int rounds,
+                                             int items, int first, int count, int heads, void* out,
+                                             float* sm) {
+  const int n = a.per_head ? heads * a.D : a.D;
+  int w = 32;
+  while (w < 256 && w < n) w *= 2;
+  const int sub = 256 / w, o0 = threadIdx.x % w, sb = threadIdx.x / w;
+  for (int base = 0; base < n; base += w) {
+    const int o = base + o0;
+    float sum = 0.f;
+    if (o < n) {
+      const int d = a.per_head ? o % a.D : o;
+      const int lo = a.per_head ? first + o / a.D : first, nit = a.per_head ? 1 : count;
+      const int terms = rounds * nit;
+#pragma unroll 8
+      for (int k = sb; k < terms; k += sub) {
+        const int blk = (k / nit) * items + lo + k % nit;
+        sum += __ldcg(part + (long long)blk * a.D + d);
+      }
+    }
+    __syncthreads();
+    sm[threadIdx.x] = sum;
+    __syncthreads();
+    if (sb == 0 && o < n) {
+      for (int i = 1; i < sub; ++i) sum += sm[i * w + o0];
+      if (a.w32) reinterpret_cast<float*>(out)[o] = sum;
+      else reinterpret_cast<T*>(out)[o] = St<T>::v(sum);
+    }
+  }
+}
+
+// A block keeps one item (one side, `hpi` heads; one head when the weights are
+// per head) and walks over tokens, so that each lane sums the weight gradient
+// of its chunks in registers; the block's sums go to `part`, and the last block
+// adds the blocks up.
+template <typename T, int V, int G, int U>
+__global__ void __launch_bounds__(256, 2) qk_bwd_kernel(const __grid_constant__ QkArgs a, int hpi,
+                                                     int items_q, int items, unsigned* counter,
+                                                     float* part, void* dqw, void* dkw) {
+  __shared__ float sm[8 * kMaxDim];
+  __shared__ int flag;
+  const QkLane q = qk_lane<V>(a, threadIdx.x & (G - 1));
+  const int it = blockIdx.x % items, round = blockIdx.x / items, rounds = gridDim.x / items;
+  const QkSide& s = a.s[it >= items_q];
+  const int h0 = (it >= items_q ? it - items_q : it) * hpi, h1 = min(s.heads, h0 + hpi);
+  const int tokens = a.B * a.L;
+  constexpr int GPB = 256 / G;
+  __align__(16) float c[V], sn[V], wa[V], wb[V];
+  float da[V], db[V];
+  qk_weights<T, V>(a, s, q, h0, wa, wb);  // per head: hpi is 1
+#pragma unroll
+  for (int i = 0; i < V; ++i) da[i] = db[i] = 0.f;
+  for (int t0 = round * GPB; t0 < tokens; t0 += rounds * GPB) {
+    const int t = t0 + threadIdx.x / G;
+    const bool busy = t < tokens && q.live;
+    const int b = t < tokens ? t / a.L : 0, l = t < tokens ? t - b * a.L : 0;
+    const int p = qk_position(a, b, l);
+    qk_angles<V>(a, q, p, c, sn);
+    const T* x = reinterpret_cast<const T*>(s.x) + b * s.xb + l * s.xl;
+    const T* g = reinterpret_cast<const T*>(s.g) + b * s.gb + l * s.gl;
+    T* dx = reinterpret_cast<T*>(s.out) + b * s.ob + l * s.ol;
+    for (int r = 0; r < hpi; r += U) {
+      Raw<T, V> ra[U], rb[U], sa[U], sb[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = h0 + r + u;
+        const bool live = busy && h < h1;
+        ra[u] = qk_raw<T, V>(x + h * s.xh + q.a0, live);
+        rb[u] = qk_raw<T, V>(x + h * s.xh + q.b0, live);
+        sa[u] = qk_raw<T, V>(g + h * s.gh + q.a0, live);
+        sb[u] = qk_raw<T, V>(g + h * s.gh + q.b0, live);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int h = h0 + r + u;
+        float xa[V], xb[V], ga[V], gb[V];
+        qk_wide<T, V>(ra[u], xa);
+        qk_wide<T, V>(rb[u], xb);
+        qk_wide<T, V>(sa[u], ga);
+        qk_wide<T, V>(sb[u], gb);
+        qk_turn<V>(a, q, ga, gb, c, sn, -1.f);
+        float ss = 0.f, dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
+          dot = fmaf(xa[i] * wa[i], ga[i], fmaf(xb[i] * wb[i], gb[i], dot));
+        }
+        float rs = rsqrtf(fmaf(group_sum<G>(ss), a.inv_d, a.eps));
+        if (p < 0) rs = __int_as_float(0x7fffffff);
+        const float m = group_sum<G>(dot) * rs * a.inv_d;
+        if (busy && h < h1) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float ha = xa[i] * rs, hb = xb[i] * rs;
+            da[i] = fmaf(ga[i], ha, da[i]);
+            db[i] = fmaf(gb[i], hb, db[i]);
+            xa[i] = rs * fmaf(-ha, m, wa[i] * ga[i]);
+            xb[i] = rs * fmaf(-hb, m, wb[i] * gb[i]);
+          }
+          qk_store<T, V>(dx + h * s.oh + q.a0, xa);
+          qk_store<T, V>(dx + h * s.oh + q.b0, xb);
+        }
+      }
+    }
+  }
+  if (!dqw && !dkw) return;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+#pragma unroll
+    for (int o = G; o < 32; o <<= 1) {
+      da[i] += __shfl_xor_sync(0xffffffffu, da[i], o);
+      db[i] += __shfl_xor_sync(0xffffffffu, db[i], o);
+    }
+  }
+  if (q.live && (threadIdx.x & 31) < G) {
+    float* w = sm + (threadIdx.x >> 5) * a.D;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[q.a0 + i] = da[i];
+      w[q.b0 + i] = db[i];
+    }
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < a.D; d += 256) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += sm[i * a.D + d];
+    part[(long long)blockIdx.x * a.D + d] = sum;
+  }
+  if (!last_block_arrived(counter, gridDim.x, &flag)) return;
+  if (dqw) qk_dw_finish<T>(a, part, rounds, items, 0, items_q, a.s[0].heads, dqw, sm);
+  if (dkw)
+    qk_dw_finish<T>(a, part, rounds, items, items_q, items - items_q, a.s[1].heads, dkw, sm);
+}
+
 static int qk_dw_chunks(long long tokens) {
   return (int)std::max<long long>(1, std::min<long long>(tokens / 16, 256));
+}
+
+// Blocks of the vector backward: as many as run at once (two a multiprocessor
+// at its registers), a whole number of rounds over the items.
+static int qk_bwd_rounds(long long tokens, int items, int groups, int sms) {
+  const long long need = (tokens + groups - 1) / groups;
+  return (int)std::max<long long>(1, std::min<long long>(need, std::max(1, 2 * sms / items)));
 }
 
 size_t qk_backward_ws_bytes(int batch, int length, int q_heads, int k_heads, int dim) {
   const long long tokens = (long long)batch * length;
   const long long per = q_heads + k_heads;
-  return (size_t)(4 * (tokens * per + (long long)qk_dw_chunks(tokens) * per * dim));
+  const size_t any = (size_t)(4 * (tokens * per + (long long)qk_dw_chunks(tokens) * per * dim));
+  const size_t vec = (size_t)4 * dim * std::max<long long>(512, 2 * per);
+  return FAB_COUNTER_BYTES + std::max(any, vec);
+}
+
+// Whether the vector kernels with V components a chunk serve this call.
+static bool qk_vector(const QkArgs& a, int V, int item, bool backward) {
+  if (a.D < 16 || a.D % (2 * V) || a.D / (2 * V) > 32 || a.half % 4) return false;
+  if (a.interleaved ? (2 * a.half) % V : a.half % V || ((a.D - 2 * a.half) / 2) % V) return false;
+  if ((long long)a.B * a.L > 0x7fff0000LL) return false;
+  uintptr_t bits = 0;
+  auto side = [&](const void* p, long long sb, long long sl, long long sh, int heads) {
+    bits |= reinterpret_cast<uintptr_t>(p);
+    if (a.B > 1) bits |= (uintptr_t)(sb * item);
+    if (a.L > 1) bits |= (uintptr_t)(sl * item);
+    if (heads > 1) bits |= (uintptr_t)(sh * item);
+  };
+  for (const QkSide& s : a.s) {
+    side(s.x, s.xb, s.xl, s.xh, s.heads);
+    side(s.out, s.ob, s.ol, s.oh, s.heads);
+    if (backward) side(s.g, s.gb, s.gl, s.gh, s.heads);
+    if (s.w && !a.w32) bits |= reinterpret_cast<uintptr_t>(s.w);
+  }
+  uintptr_t wide = 0;
+  for (const QkSide& s : a.s)
+    if (s.w && a.w32) wide |= reinterpret_cast<uintptr_t>(s.w);
+  wide |= reinterpret_cast<uintptr_t>(a.cos_) | reinterpret_cast<uintptr_t>(a.sin_);
+  return bits % (V * item) == 0 && wide % 16 == 0;
+}
+
+template <typename T, int V, int G>
+static int qk_launch(const QkArgs& a, bool backward, char* ws, void* dqw, void* dkw, int device,
+                     cudaStream_t st) {
+  const long long tokens = (long long)a.B * a.L;
+  const int hq = a.s[0].heads, hk = a.s[1].heads, sms = sm_count(device);
+  // Heads an item: the angles serve more of them, but every multiprocessor gets
+  // its 1024 lanes first.
+  auto lanes = [&](int hpi) { return tokens * ((hq + hpi - 1) / hpi + (hk + hpi - 1) / hpi) * G; };
+  const int hpi = backward && a.per_head ? 1
+                  : lanes(8) >= 1024ll * sms ? 8 : lanes(4) >= 1024ll * sms ? 4 : 1;
+  const int items_q = (hq + hpi - 1) / hpi, items = items_q + (hk + hpi - 1) / hpi;
+  if (!backward) {
+    const long long total = tokens * items;
+    const long long blocks = (total * G + 255) / 256;
+    if (blocks > 0x7fffffffLL) return FA_E_SHAPE;
+    if (hpi == 1)
+      qk_fwd_kernel<T, V, G, 1><<<(unsigned)blocks, 256, 0, st>>>(a, hpi, items_q, items, total);
+    else
+      qk_fwd_kernel<T, V, G, 4><<<(unsigned)blocks, 256, 0, st>>>(a, hpi, items_q, items, total);
+  } else {
+    const int rounds = qk_bwd_rounds(tokens, items, 256 / G, sms);
+    unsigned* counter = reinterpret_cast<unsigned*>(ws);
+    float* part = reinterpret_cast<float*>(ws + FAB_COUNTER_BYTES);
+    const unsigned blocks = (unsigned)(rounds * items);
+    if (hpi == 1)
+      qk_bwd_kernel<T, V, G, 1><<<blocks, 256, 0, st>>>(a, hpi, items_q, items, counter, part, dqw,
+                                                       dkw);
+    else
+      qk_bwd_kernel<T, V, G, 2><<<blocks, 256, 0, st>>>(a, hpi, items_q, items, counter, part, dqw,
+                                                       dkw);
+  }
+  FAB_LAUNCH_CHECK();
+  return FA_OK;
+}
+
+template <typename T, int V>
+static int qk_group(const QkArgs& a, bool backward, char* ws, void* dqw, void* dkw, int device,
+                    cudaStream_t st) {
+  const int pairs = a.D / (2 * V);
+  if (pairs <= 4) return qk_launch<T, V, 4>(a, backward, ws, dqw, dkw, device, st);
+  if (pairs <= 8) return qk_launch<T, V, 8>(a, backward, ws, dqw, dkw, device, st);
+  if (pairs <= 16) return qk_launch<T, V, 16>(a, backward, ws, dqw, dkw, device, st);
+  return qk_launch<T, V, 32>(a, backward, ws, dqw, dkw, device, st);
 }
 
 template <typename T>
-static int qk_run(const QkArgs& a, bool backward, void* ws, void* dqw, void* dkw, int device,
+static int qk_run(const QkArgs& a, bool backward, void* wsv, void* dqw, void* dkw, int device,
                   cudaStream_t st) {
+  char* ws = static_cast<char*>(wsv);
+  if constexpr (sizeof(T) == 2) {
+    if (qk_vector(a, 8, 2, backward)) return qk_group<T, 8>(a, backward, ws, dqw, dkw, device, st);
+    if (qk_vector(a, 4, 2, backward)) return qk_group<T, 4>(a, backward, ws, dqw, dkw, device, st);
+  } else {
+    if (qk_vector(a, 4, 4, backward)) return qk_group<T, 4>(a, backward, ws, dqw, dkw, device, st);
+  }
   const long long tokens = (long long)a.B * a.L;
   const int per = a.s[0].heads + a.s[1].heads;
   const long long rows = tokens * per;
@@ -265,7 +714,7 @@ static int qk_run(const QkArgs& a, bool backward, void* ws, void* dqw, void* dkw
     return FA_OK;
   }
   QkArgs b = a;
-  b.rstd = reinterpret_cast<float*>(ws);
+  b.rstd = reinterpret_cast<float*>(ws + FAB_COUNTER_BYTES);
   qk_bwd_any_kernel<T><<<grid, 256, 0, st>>>(b, rows);
   FAB_LAUNCH_CHECK();
   if (dqw || dkw) {

@@ -573,7 +573,7 @@ FA_B200_API int fa_b200_qk_norm_rotary(const fa_heads* q, const fa_heads* k,
                                        const fa_qk_params* params, int device, void* stream);
 
 /* Its gradient: dq, dk, and the weights' gradients in weight_dtype (null to
- * skip one).  The workspace needs no zeroing. */
+ * skip one). */
 FA_B200_API int fa_b200_qk_norm_rotary_backward_workspace_bytes(int batch, int length,
                                                                 int q_heads, int k_heads,
                                                                 int dim, size_t* out_bytes);
