@@ -75,6 +75,7 @@ struct NsMat {
   float step;                      // W <- decay W - step O
   int group;
   int vec;                         // rows are whole aligned 16-byte vectors
+  int vec_dst;                     // the result's rows are whole aligned vectors of four
 };
 
 struct NsStep {
@@ -407,139 +408,277 @@ static int sym_tiles(int s, int bn) {
   return T * (T + 1);
 }
 
+// Shared memory: operand stages, then a 32 x 32 float buffer for each epilogue
+// warp.  A stage holds 64 K columns of the row operand (128 rows) and of the
+// column operand (256 rows; split: 128, twice).
 template <bool SPLIT>
 struct Stage {
   static constexpr int kParts = SPLIT ? 2 : 1;
-  static constexpr int kBytes = kParts * (BM / 64 + 256 / 64) * kBox;  // 48 or 96 KB
-  static constexpr int kCount = SPLIT ? 2 : 4;
-  static constexpr int kSmem = kCount * kBytes + 1024 + 256;
+  static constexpr int kWide = SPLIT ? 128 : 256;                      // widest tile
+  static constexpr int kBytes = kParts * (BM / 64 + kWide / 64) * kBox;  // 48 or 64 KB
+  static constexpr int kCount = SPLIT ? 3 : 4;
+  static constexpr int kTurn = (kEpilogue / 32) * 4096;
+  static constexpr int kSmem = kCount * kBytes + kTurn + 1024;
 };
 
-__device__ __forceinline__ void load_half32(const __half* p, float (&v)[32]) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int4 w = __ldcg(reinterpret_cast<const int4*>(p) + q);
-    const unsigned* u = reinterpret_cast<const unsigned*>(&w);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(u + e));
-      v[8 * q + 2 * e] = f.x;
-      v[8 * q + 2 * e + 1] = f.y;
-    }
-  }
-}
-__device__ __forceinline__ void add_half32(const __half* p, float (&v)[32]) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int4 w = __ldcg(reinterpret_cast<const int4*>(p) + q);
-    const unsigned* u = reinterpret_cast<const unsigned*>(&w);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(u + e));
-      v[8 * q + 2 * e] += f.x;
-      v[8 * q + 2 * e + 1] += f.y;
-    }
-  }
-}
-__device__ __forceinline__ void store_half32(__half* p, const __half (&h)[32]) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    reinterpret_cast<int4*>(p)[q] = reinterpret_cast<const int4*>(h)[q];
-}
 __device__ __forceinline__ float exp2i(int e) { return __int_as_float((127 + e) << 23); }
 
-// Epilogue of 32 columns [j0, j0 + 32) of row i of a tile; v holds the raw sums.
-template <bool SPLIT, typename T>
-__device__ __forceinline__ void ns_emit(const NsArgs& a, const Tile& t, int i, int j0,
-                                        float (&v)[32]) {
+// Four float16 (8 bytes) to float, and to the pair hi + lo.
+__device__ __forceinline__ float4 half4_float(uint2 u) {
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+template <bool LO>
+__device__ __forceinline__ void put_half4(float4 v, __half* hi, __half* lo) {
+  const __half2 h0 = __floats2half2_rn(v.x, v.y), h1 = __floats2half2_rn(v.z, v.w);
+  uint2 u;
+  u.x = *reinterpret_cast<const unsigned*>(&h0);
+  u.y = *reinterpret_cast<const unsigned*>(&h1);
+  *reinterpret_cast<uint2*>(hi) = u;
+  if (LO) {
+    const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+    const __half2 l0 = __floats2half2_rn(v.x - f0.x, v.y - f0.y);
+    const __half2 l1 = __floats2half2_rn(v.z - f1.x, v.w - f1.y);
+    u.x = *reinterpret_cast<const unsigned*>(&l0);
+    u.y = *reinterpret_cast<const unsigned*>(&l1);
+    *reinterpret_cast<uint2*>(lo) = u;
+  }
+}
+
+// What the epilogue of a tile needs, gathered while its products run.  Every
+// output is  v = p * sum + q * (e + f (d_i + d_j)),  q the stored value at the
+// same place (O for the square, X for the last product, nothing for A), d the
+// diagonals that apply, and the powers of two of the formats folded into p, e, f.
+struct Out {
+  int rows, cols, pitch;
+  float p, e, f;
+  const __half *q0, *q1;           // null: no such part
+  const float *di, *dj;            // diagonals by row and by column, or null
+  __half *o0, *o1;                 // null o0: the result itself
+  float *diag;                     // where the diagonal goes (symmetric products)
+  float ds, dp, dq;                // on it: dp * (sum * ds + d^2) + dq * d
+};
+
+template <bool SPLIT>
+__device__ __forceinline__ void ns_out(const NsArgs& a, const Tile& t, Out* o) {
   const NsGroup& g = a.g[t.group];
-  const NsMat& m = a.m[t.mat];
   const NsStep& k = a.k[t.step];
-  const int b = t.mat - g.first;
+  const long long b = t.mat - g.first;
   if (t.phase < 2) {
-    if (i >= g.s || j0 >= g.s || j0 / BM > t.i0 / BM) return;
-    const long long plane = (long long)b * g.s * g.pa;
-    const float alpha = t.phase == 0 ? exp2i(-2 * k.ex) : exp2i(-2 * k.ea);
-    const float up = exp2i(t.phase == 0 ? k.ea : k.eb);
-    __half* const out0 = t.phase == 0 ? g.a[0] : g.b[0];
-    __half* const out1 = t.phase == 0 ? g.a[1] : g.b[1];
-    float* diag = (t.phase == 0 ? g.da : g.db) + (long long)b * g.pa;
-    if (t.phase == 1) {
-      const float* da = g.da + (long long)b * g.pa;
-      const float di = __ldcg(da + i), down = exp2i(-k.ea);
-      __align__(16) float o[32], dj[32];
-      load_half32(g.a[0] + plane + (long long)i * g.pa + j0, o);
-      if (SPLIT) add_half32(g.a[1] + plane + (long long)i * g.pa + j0, o);
-#pragma unroll
-      for (int q = 0; q < 8; ++q)
-        reinterpret_cast<float4*>(dj)[q] = __ldcg(reinterpret_cast<const float4*>(da + j0) + q);
-#pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        const float ov = o[c] * down, p2 = v[c] * alpha;
-        v[c] = j0 + c == i ? fmaf(k.c, fmaf(di, di, p2), k.b * di)
-                           : fmaf(k.c, fmaf(di + dj[c], ov, p2), k.b * ov);
-      }
+    const long long plane = b * g.s * g.pa;
+    o->rows = o->cols = g.s;
+    o->pitch = g.pa;
+    o->di = o->dj = nullptr;
+    o->q0 = o->q1 = nullptr;
+    o->e = o->f = 0.f;
+    if (t.phase == 0) {
+      o->p = exp2i(k.ea - 2 * k.ex);
+      o->o0 = g.a[0] + plane;
+      o->o1 = SPLIT ? g.a[1] + plane : nullptr;
+      o->diag = g.da + b * g.pa;
+      o->ds = exp2i(-2 * k.ex);
+      o->dp = 1.f;
+      o->dq = 0.f;
     } else {
-#pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] *= alpha;
+      o->p = k.c * exp2i(k.eb - 2 * k.ea);
+      o->e = k.b * exp2i(k.eb - k.ea);
+      o->f = k.c * exp2i(k.eb - k.ea);
+      o->q0 = g.a[0] + plane;
+      o->q1 = SPLIT ? g.a[1] + plane : nullptr;
+      o->di = o->dj = g.da + b * g.pa;
+      o->o0 = g.b[0] + plane;
+      o->o1 = SPLIT ? g.b[1] + plane : nullptr;
+      o->diag = g.db + b * g.pa;
+      o->ds = exp2i(-2 * k.ea);
+      o->dp = k.c;
+      o->dq = k.b;
     }
-    __align__(16) __half hi[32], lo[32];
+  } else {
+    const int from = t.step & 1;
+    const long long plane = b * g.rows * g.px;
+    const bool last = t.step + 1 == a.steps;
+    const float up = last ? 1.f : exp2i(k.ex2);
+    o->rows = g.rows;
+    o->cols = g.cols;
+    o->pitch = g.px;
+    o->p = exp2i(-k.eb - k.ex) * up;
+    o->f = exp2i(-k.ex) * up;
+    o->e = k.a * o->f;
+    o->q0 = g.x[from][0] + plane;
+    o->q1 = g.x[from][1] + plane;
+    o->di = g.tall ? nullptr : g.db + b * g.pa;
+    o->dj = g.tall ? g.db + b * g.pa : nullptr;
+    o->o0 = last ? nullptr : g.x[1 - from][0] + plane;
+    o->o1 = g.x[1 - from][1] + plane;
+    o->diag = nullptr;
+  }
+}
+
+// A warp's 32 x 32 buffer, in units of four columns: unit q of row r lies at
+// q ^ (r mod 8) ^ (r / 8).  Eight rows at one unit (turning in), a row's eight
+// units (reading rows) and rows 0, 4, 8, ... at one column (reading columns)
+// are in different banks.
+__device__ __forceinline__ int turn_unit(int r, int q) { return r * 8 + (q ^ (r & 7) ^ (r >> 3)); }
+
+// The last step's output: rows i + 4 it, four columns from j, as the result or
+// into the weight.
+template <typename T>
+__device__ __forceinline__ void ns_result(const NsArgs& a, const Tile& t, const Out& o, int i,
+                                          int j, int left, const float4 (&v)[8]) {
+  const NsMat& m = a.m[t.mat];
+  T* w = reinterpret_cast<T*>(m.dst) + i * m.dst_row + j;
+  const float step = m.step;
+  const bool update = m.mom != nullptr;
+  if (m.vec_dst) {  // whole vectors of four
+    typedef typename RawOf<4 * sizeof(T)>::type V4;
+    if (j >= o.cols) return;
+    V4 old[8];
+    if (update) {
 #pragma unroll
-    for (int c = 0; c < 32; ++c) {
-      if (j0 + c == i) {
-        diag[i] = v[c];
-        v[c] = 0.f;
+      for (int it = 0; it < 8; ++it)
+        if (4 * it < left) old[it] = *reinterpret_cast<const V4*>(w + 4 * it * m.dst_row);
+    }
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {
+      if (4 * it >= left) break;
+      const float vs[4] = {v[it].x, v[it].y, v[it].z, v[it].w};
+      V4 u;
+      T* e4 = reinterpret_cast<T*>(&u);
+      const T* o4 = reinterpret_cast<const T*>(&old[it]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        e4[e] = St<T>::v(update ? fmaf(a.decay, Ld<T>::f(o4[e]), -step * vs[e]) : vs[e]);
+      *reinterpret_cast<V4*>(w + 4 * it * m.dst_row) = u;
+    }
+  } else {
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {
+      if (4 * it >= left) break;
+      T* x = w + 4 * it * m.dst_row;
+      const float vs[4] = {v[it].x, v[it].y, v[it].z, v[it].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j + e < o.cols)
+          x[e] = St<T>::v(update ? fmaf(a.decay, Ld<T>::f(x[e]), -step * vs[e]) : vs[e]);
+    }
+  }
+}
+
+// Epilogue of a 32 x 32 block of a tile, rows [i0, i0 + 32), columns
+// [j0, j0 + 32).  `sums` of row i0 + lane are turned in shared memory so that
+// eight lanes share a row's 64 bytes of float16, four columns to a lane.
+template <bool SPLIT, typename T>
+__device__ __forceinline__ void ns_emit(const NsArgs& a, const Tile& t, const Out& o, int i0,
+                                        int j0, float4* turn, const float (&sums)[32]) {
+  const bool sym = t.phase < 2;
+  // warp-uniform: outside the matrix, or above the diagonal blocks
+  if (i0 >= o.rows || j0 >= o.cols || (sym && j0 / BM > t.i0 / BM)) return;
+  const int lane = threadIdx.x & 31, r0 = lane >> 3, q4 = lane & 7, j = j0 + 4 * q4;
+  const long long at0 = (long long)(i0 + r0) * o.pitch + j, four = 4ll * o.pitch;
+  const int left = o.rows - i0 - r0;  // rows 4 it + r0 are inside for 4 it < left
+  // Each loop below is a batch of independent accesses: a scheduler has two of
+  // these warps, so latency is hidden inside a warp or not at all.
+  uint2 hi[8], lo[8];
+#pragma unroll
+  for (int it = 0; it < 8; ++it) hi[it] = lo[it] = make_uint2(0u, 0u);
+  if (o.q0) {
+    const __half* p = o.q0 + at0;
+#pragma unroll
+    for (int it = 0; it < 8; ++it, p += four)
+      if (4 * it < left) hi[it] = __ldcg(reinterpret_cast<const uint2*>(p));
+  }
+  if (o.q1) {
+    const __half* p = o.q1 + at0;
+#pragma unroll
+    for (int it = 0; it < 8; ++it, p += four)
+      if (4 * it < left) lo[it] = __ldcg(reinterpret_cast<const uint2*>(p));
+  }
+  const float row_d = o.di && i0 + lane < o.rows ? __ldcg(o.di + i0 + lane) : 0.f;
+  float4 cd = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (o.dj) cd = __ldcg(reinterpret_cast<const float4*>(o.dj + j));  // inside the pitch of 64
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    turn[turn_unit(lane, q)] =
+        make_float4(sums[4 * q], sums[4 * q + 1], sums[4 * q + 2], sums[4 * q + 3]);
+  __syncwarp();
+  if (sym && i0 == j0) {  // the diagonal stays in float32, and zero in its place
+    if (lane < o.rows - i0) {
+      float* d = reinterpret_cast<float*>(turn) + 4 * turn_unit(lane, lane >> 2) + (lane & 3);
+      o.diag[i0 + lane] = fmaf(o.dp, fmaf(*d, o.ds, row_d * row_d), o.dq * row_d);
+      *d = 0.f;
+    }
+    __syncwarp();
+  }
+  float4 v[8];
+#pragma unroll
+  for (int it = 0; it < 8; ++it) v[it] = turn[turn_unit(4 * it + r0, q4)];
+  cd.x = fmaf(o.f, cd.x, o.e);
+  cd.y = fmaf(o.f, cd.y, o.e);
+  cd.z = fmaf(o.f, cd.z, o.e);
+  cd.w = fmaf(o.f, cd.w, o.e);
+  if (o.q0) {
+    const float fd_row = o.f * row_d;
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {
+      const float fd = __shfl_sync(0xffffffffu, fd_row, 4 * it + r0);
+      float4 x = half4_float(hi[it]);
+      if (SPLIT || !sym) {
+        const float4 l = half4_float(lo[it]);
+        x.x += l.x;
+        x.y += l.y;
+        x.z += l.z;
+        x.w += l.w;
       }
-      split_half(v[c] * up, &hi[c], &lo[c]);
+      v[it].x = fmaf(x.x, cd.x + fd, v[it].x * o.p);
+      v[it].y = fmaf(x.y, cd.y + fd, v[it].y * o.p);
+      v[it].z = fmaf(x.z, cd.z + fd, v[it].z * o.p);
+      v[it].w = fmaf(x.w, cd.w + fd, v[it].w * o.p);
     }
-    store_half32(out0 + plane + (long long)i * g.pa + j0, hi);
-    if (SPLIT) store_half32(out1 + plane + (long long)i * g.pa + j0, lo);
-    if (j0 / BM < t.i0 / BM) {  // the mirror image, above the diagonal
+  } else {
 #pragma unroll
-      for (int c = 0; c < 32; ++c) {
-        if (j0 + c < g.s) {
-          const long long o = plane + (long long)(j0 + c) * g.pa + i;
-          out0[o] = hi[c];
-          if (SPLIT) out1[o] = lo[c];
-        }
+    for (int it = 0; it < 8; ++it) {
+      v[it].x *= o.p;
+      v[it].y *= o.p;
+      v[it].z *= o.p;
+      v[it].w *= o.p;
+    }
+  }
+  const bool mirror = sym && j0 / BM < t.i0 / BM;
+  if (mirror) {
+#pragma unroll
+    for (int it = 0; it < 8; ++it) turn[turn_unit(4 * it + r0, q4)] = v[it];
+  }
+  if (o.o0) {
+    __half *p0 = o.o0 + at0, *p1 = o.o1 + at0;
+#pragma unroll
+    for (int it = 0; it < 8; ++it, p0 += four, p1 += four) {
+      if (4 * it < left) {
+        if (SPLIT || !sym) put_half4<true>(v[it], p0, p1);
+        else put_half4<false>(v[it], p0, nullptr);
       }
     }
   } else {
-    if (i >= g.rows || j0 >= g.cols) return;
-    const int from = t.step & 1;
-    const long long at = ((long long)b * g.rows + i) * g.px + j0;
-    const float* db = g.db + (long long)b * g.pa;
-    const float alpha = exp2i(-k.eb - k.ex), xs = exp2i(-k.ex);
-    float x[32];
-    load_half32(g.x[from][0] + at, x);
-    add_half32(g.x[from][1] + at, x);
-    if (g.tall) {
-      __align__(16) float f[32];
+    ns_result<T>(a, t, o, i0 + r0, j, left, v);
+  }
+  if (mirror) {  // the same values above the diagonal: four rows to a lane
+    __syncwarp();
+    const float* f = reinterpret_cast<const float*>(turn) + r0;
+    const long long to = (long long)(j0 + r0) * o.pitch + i0 + 4 * q4;
+    __half *p0 = o.o0 + to, *p1 = o.o1 + to;
 #pragma unroll
-      for (int q = 0; q < 8; ++q)
-        reinterpret_cast<float4*>(f)[q] = __ldcg(reinterpret_cast<const float4*>(db + j0) + q);
+    for (int it = 0; it < 8; ++it)  // column 4 it + r0: unit it, place r0
+      v[it] = make_float4(f[4 * turn_unit(4 * q4, it)], f[4 * turn_unit(4 * q4 + 1, it)],
+                          f[4 * turn_unit(4 * q4 + 2, it)], f[4 * turn_unit(4 * q4 + 3, it)]);
 #pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = fmaf(k.a + f[c], x[c] * xs, v[c] * alpha);
-    } else {
-      const float f = k.a + __ldcg(db + i);
-#pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = fmaf(f, x[c] * xs, v[c] * alpha);
-    }
-    if (t.step + 1 < a.steps) {
-      const float up = exp2i(k.ex2);
-      __align__(16) __half hi[32], lo[32];
-#pragma unroll
-      for (int c = 0; c < 32; ++c) split_half(v[c] * up, &hi[c], &lo[c]);
-      store_half32(g.x[1 - from][0] + at, hi);
-      store_half32(g.x[1 - from][1] + at, lo);
-    } else {
-      T* w = reinterpret_cast<T*>(m.dst) + i * m.dst_row + j0;
-#pragma unroll
-      for (int c = 0; c < 32; ++c)
-        if (j0 + c < g.cols)
-          w[c] = St<T>::v(m.mom ? fmaf(a.decay, Ld<T>::f(w[c]), -m.step * v[c]) : v[c]);
+    for (int it = 0; it < 8; ++it, p0 += four, p1 += four) {
+      if (j0 + 4 * it + r0 < o.cols) {
+        if (SPLIT) put_half4<true>(v[it], p0, p1);
+        else put_half4<false>(v[it], p0, nullptr);
+      }
     }
   }
+  __syncwarp();  // the buffer is free for the next block
 }
 
 // Products of the current matrices.  Warp 0 copies operand tiles into shared
@@ -616,7 +755,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
 #pragma unroll
           for (int part = 0; part < PARTS; ++part) {
             const unsigned bp = base + part * (BM / 64) * kBox;
-            const unsigned bq = base + (PARTS * (BM / 64) + part * 4) * kBox;
+            const unsigned bq = base + (PARTS * (BM / 64) + part * (St_::kWide / 64)) * kBox;
             for (int i = 0; i < BM / 64; ++i)
               tma_box(bp + i * kBox, &g.map[mp][part], p_mn ? t.i0 + 64 * i : kb * BK,
                       p_mn ? kb * BK : t.i0 + 64 * i, z, bar);
@@ -666,7 +805,8 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
             const unsigned base = smem0 + s * St_::kBytes;
             const unsigned long long p0 = operand(base);
             const unsigned long long q0 = operand(base + PARTS * (BM / 64) * kBox);
-            const unsigned long long p1 = p0 + ((BM / 64) * kBox >> 4), q1 = q0 + (4 * kBox >> 4);
+            const unsigned long long p1 = p0 + ((BM / 64) * kBox >> 4);
+            const unsigned long long q1 = q0 + ((St_::kWide / 64) * kBox >> 4);
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k) {
               const unsigned long long po = k * ps, qo = k * qs;
@@ -689,13 +829,16 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
     Walk walk(blockIdx.x);
     Tile t;
     const int w = warp & 3, h = (warp - 4) >> 2;
+    float4* const turn = reinterpret_cast<float4*>(smem_raw + (smem0 - smem_u32(smem_raw)) +
+                                                 S * St_::kBytes + (warp - 4) * 4096);
     unsigned sums = 0;
     for (unsigned tile = 0; walk.next(a, &t); ++tile) {
-      const NsGroup& g = a.g[t.group];
       const int half = t.bn / 2;
       const unsigned lanes = (unsigned)(32 * w) << 16;
-      // this thread's row, columns t.j0 + h * half + [0, half)
-      const int i = t.i0 + 32 * w + lane, jh = t.j0 + h * half;
+      // this warp's rows, columns t.j0 + h * half + [0, half)
+      const int i = t.i0 + 32 * w, jh = t.j0 + h * half;
+      Out out;
+      ns_out<SPLIT>(a, t, &out);
       const int chunks = SPLIT ? (t.kblocks + kChunk - 1) / kChunk : 1;
       __align__(16) float sum[SPLIT ? 2 : 1][32];
       bool ok = true;
@@ -738,7 +881,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
         mbar_arrive(&sm_empty[tile & 1]);
 #pragma unroll
         for (int q = 0; q < 2; ++q)
-          if (q * 32 < half) ns_emit<SPLIT, T>(a, t, i, jh + q * 32, sum[q]);
+          if (q * 32 < half) ns_emit<SPLIT, T>(a, t, out, i, jh + q * 32, turn, sum[q]);
       } else {
         const int buf = (sums - 1) & 1;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
@@ -749,7 +892,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             mbar_arrive(&tm_empty[buf]);
           }
-          ns_emit<SPLIT, T>(a, t, i, jh + c0, sum[0]);
+          ns_emit<SPLIT, T>(a, t, out, i, jh + c0, turn, sum[0]);
         }
       }
       // other blocks read these values through TMA: order them before the count
@@ -1053,6 +1196,8 @@ int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int
       m.vec = f.cols % 8 == 0 && reinterpret_cast<uintptr_t>(f.src) % 16 == 0 &&
               (f.rows == 1 || f.src_row_stride * item % 16 == 0) &&
               (!m.mom || reinterpret_cast<uintptr_t>(m.mom) % 16 == 0);
+      m.vec_dst = f.cols % 4 == 0 && reinterpret_cast<uintptr_t>(f.dst) % (4 * item) == 0 &&
+                  (f.rows == 1 || f.dst_row_stride % 4 == 0);
     }
     int rc;
     switch (dtype) {

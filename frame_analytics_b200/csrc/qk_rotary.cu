@@ -256,9 +256,6 @@ __global__ void __launch_bounds__(128) qk_dw_sum_kernel(const float* part, int c
 // Both kernels are bound by HBM: the work per component is about 10 (backward:
 // 25) float operations for 4 to 12 bytes.
 // ---------------------------------------------------------------------------
-template <int BYTES> struct RawOf;
-template <> struct RawOf<16> { typedef uint4 type; };
-template <> struct RawOf<8> { typedef uint2 type; };
 // V components as they lie in memory: rows in flight wait unconverted.
 template <typename T, int V> using Raw = typename RawOf<sizeof(T) * V>::type;
 

@@ -28,4 +28,9 @@ template <> struct St<bf16_t> {
   }
 };
 
+// A vector register type of so many bytes.
+template <int BYTES> struct RawOf;
+template <> struct RawOf<16> { typedef uint4 type; };
+template <> struct RawOf<8> { typedef uint2 type; };
+
 }  // namespace fab
