@@ -112,9 +112,6 @@ _i64 = ctypes.c_int64
 _d = ctypes.c_double
 _sz = ctypes.c_size_t
 _pview = ctypes.POINTER(fa_view)
-_ph = ctypes.POINTER(fa_heads)
-_pq = ctypes.POINTER(fa_qk_params)
-_pm = ctypes.POINTER(fa_matrix)
 
 # name -> argtypes (restype int unless listed in _RESTYPE)
 PROTOTYPES = {
@@ -183,13 +180,13 @@ PROTOTYPES = {
     "fa_b200_gmsd64": [_pview, _pview, _vp, _d, _d, _i, _vp, _sz, _vp, _vp, _vp, _i, _vp],
     "fa_b200_gmsd64_backward": [_vp, _vp, _i, _i, _i, _i, _i, _d, _d, _vp, _vp, _vp, _vp, _vp,
                                 _vp, _vp, _i, _vp],
-    "fa_b200_qk_norm_rotary": [_ph, _ph, _ph, _ph, _pq, _i, _vp],
+    "fa_b200_qk_norm_rotary": [_vp, _vp, _vp, _vp, _vp, _i, _vp],
     "fa_b200_qk_norm_rotary_backward_workspace_bytes": [_i, _i, _i, _i, _i, _vp],
-    "fa_b200_qk_norm_rotary_backward": [_ph, _ph, _ph, _ph, _ph, _ph, _pq, _vp, _vp, _vp, _sz,
+    "fa_b200_qk_norm_rotary_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
                                         _i, _vp],
-    "fa_b200_orthogonalize_workspace_bytes": [_pm, _i, _i, _vp],
-    "fa_b200_orthogonalize": [_pm, _i, _i, _vp, _i, _vp, _sz, _i, _vp],
-    "fa_b200_muon_step": [_pm, _i, _i, _vp, _i, _d, _i, _d, _vp, _sz, _i, _vp],
+    "fa_b200_orthogonalize_workspace_bytes": [_vp, _i, _i, _vp],
+    "fa_b200_orthogonalize": [_vp, _i, _i, _vp, _i, _vp, _sz, _i, _vp],
+    "fa_b200_muon_step": [_vp, _i, _i, _vp, _i, _d, _i, _d, _vp, _sz, _i, _vp],
     "fa_b200_ssim_gmsd": [_pview, _pview, _vp, _i, _d, _d, _d, _d, _d, _d, _vp, _sz,
                           _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp],
 }

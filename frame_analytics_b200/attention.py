@@ -8,12 +8,12 @@ so that attention logits stay bounded under orthogonalised updates
 
 from __future__ import annotations
 
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import backend
-from ._cabi import fa_heads, fa_qk_params
 from .functional import _reject_double_backward
 
 __all__ = ["qk_norm_rotary"]
@@ -22,33 +22,43 @@ _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 _MAX_DIM = 512
 
 
-def _heads(t: torch.Tensor) -> fa_heads:
+# struct fa_heads and struct fa_qk_params of include/fa_b200.h as bytes: a call
+# on one token takes a few microseconds on the GPU, so the host side counts
+_HEADS = struct.Struct("@Pii3q").pack
+_PARAMS = struct.Struct("@10i3P2q2Pd").pack
+
+
+def _heads(t: torch.Tensor) -> bytes:
     b, l, h, _ = t.stride()
-    return fa_heads(t.data_ptr(), t.shape[2], 0, b, l, h)
+    return _HEADS(t.data_ptr(), t.shape[2], 0, b, l, h)
 
 
-def _params(q, cos, sin, q_weight, k_weight, eps, positions, interleaved) -> fa_qk_params:
-    w = q_weight if q_weight is not None else k_weight
+def _params(q, cos, sin, q_weight, k_weight, eps, positions, interleaved) -> bytes:
     code = backend.DTYPE_CODE[q.dtype]
-    p = fa_qk_params(code, code if w is None else backend.DTYPE_CODE[w.dtype],
-                     q.shape[0], q.shape[1], q.shape[3], 0, interleaved,
-                     w is not None and w.dim() == 2)
+    w = q_weight if q_weight is not None else k_weight
+    if w is None:
+        w_code, per_head = code, 0
+    else:
+        w_code, per_head = backend.DTYPE_CODE[w.dtype], w.dim() == 2
+    b, l, _, d = q.shape
+    rotary = table = cp = sp = pp = wide = pos_b = pos_l = 0
     if cos is not None:
-        p.rotary, p.table = 2 * cos.shape[1], cos.shape[0]
-        p.cos_table, p.sin_table = cos.data_ptr(), sin.data_ptr()
+        table, rotary = cos.shape
+        rotary *= 2
+        cp, sp = cos.data_ptr(), sin.data_ptr()
     if positions is not None:
-        p.positions, p.positions_64 = positions.data_ptr(), positions.dtype == torch.int64
-        p.pos_stride_l = positions.stride(-1)
-        p.pos_stride_b = positions.stride(0) if positions.dim() == 2 else 0
-    p.q_weight, p.k_weight = backend._ptr(q_weight), backend._ptr(k_weight)
-    p.eps = eps
-    return p
+        pp, wide = positions.data_ptr(), positions.dtype == torch.int64
+        stride = positions.stride()
+        pos_l = stride[-1]
+        pos_b = stride[0] if len(stride) == 2 else 0
+    return _PARAMS(code, w_code, b, l, d, rotary, interleaved, per_head, table, wide, cp, sp, pp,
+                   pos_b, pos_l, 0 if q_weight is None else q_weight.data_ptr(),
+                   0 if k_weight is None else k_weight.data_ptr(), eps)
 
 
 def _forward(q, k, q_out, k_out, *rest):
-    p = _params(q, *rest)
     backend._call(q, backend.lib().fa_b200_qk_norm_rotary, _heads(q), _heads(k), _heads(q_out),
-                  _heads(k_out), p, backend._dev(q), backend._stream(q))
+                  _heads(k_out), _params(q, *rest), backend._dev(q), backend._stream(q))
 
 
 class _QkNormRotary(torch.autograd.Function):
@@ -104,29 +114,11 @@ def _check_out(name, o, x):
         raise ValueError(f"{name} has elements that share memory")
 
 
-def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] = None,
-                   sin: Optional[torch.Tensor] = None, *,
-                   q_weight: Optional[torch.Tensor] = None,
-                   k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
-                   positions: Optional[torch.Tensor] = None, interleaved: bool = False,
-                   out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
-                   ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Normalise every query and key head and rotate it by its token's position:
-    ``y = R_p (w * x / sqrt(mean(x**2) + eps))``.  Differentiable in the
-    operands and the weights.
+# Shapes and dtypes that passed _check: metadata, no tensor is kept.
+_checked: set = set()
 
-    ``q`` (B, L, Hq, D) and ``k`` (B, L, Hk, D), float16 / bfloat16 / float32,
-    may be views of a packed projection (any strides with unit stride in D; D
-    at most 512).  ``cos`` / ``sin``: float32 (P, R/2) tables; the first
-    ``R <= D`` components turn, in pairs (i, i + R/2), or (2i, 2i + 1) with
-    ``interleaved``.  ``positions``: int32 / int64 (L,) or (B, L) rows of the
-    tables, by default 0..L-1; a position outside the tables gives NaN for its
-    token.  Weights: (D,) shared by the heads, or (heads, D); in the operands'
-    dtype or float32.
 
-    Returns contiguous (B, L, Hq, D) and (B, L, Hk, D).  ``out=(q_out, k_out)``
-    writes there instead (any strides with unit stride in D: a slice of a cache,
-    or the inputs themselves); it takes no part in autograd."""
+def _check(q, k, cos, sin, q_weight, k_weight, eps, positions) -> None:
     for name, t in (("q", q), ("k", k)):
         if t.dim() != 4:
             raise ValueError(f"{name} must be (B, L, heads, D), got shape {tuple(t.shape)}")
@@ -162,10 +154,45 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor]
         raise ValueError(f"eps must not be negative, got {eps}")
     _check_weight("q_weight", q_weight, q, k_weight)
     _check_weight("k_weight", k_weight, k, q_weight)
-    given = [t for t in (q, k, cos, sin, q_weight, k_weight, positions) if t is not None]
-    backend.require_cuda(*given)
-    if any(t.device != q.device for t in given):
-        raise ValueError("all tensors must be on one device")
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor] = None,
+                   sin: Optional[torch.Tensor] = None, *,
+                   q_weight: Optional[torch.Tensor] = None,
+                   k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                   positions: Optional[torch.Tensor] = None, interleaved: bool = False,
+                   out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+                   ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Normalise every query and key head and rotate it by its token's position:
+    ``y = R_p (w * x / sqrt(mean(x**2) + eps))``.  Differentiable in the
+    operands and the weights.
+
+    ``q`` (B, L, Hq, D) and ``k`` (B, L, Hk, D), float16 / bfloat16 / float32,
+    may be views of a packed projection (any strides with unit stride in D; D
+    at most 512).  ``cos`` / ``sin``: float32 (P, R/2) tables; the first
+    ``R <= D`` components turn, in pairs (i, i + R/2), or (2i, 2i + 1) with
+    ``interleaved``.  ``positions``: int32 / int64 (L,) or (B, L) rows of the
+    tables, by default 0..L-1; a position outside the tables gives NaN for its
+    token.  Weights: (D,) shared by the heads, or (heads, D); in the operands'
+    dtype or float32.
+
+    Returns contiguous (B, L, Hq, D) and (B, L, Hk, D).  ``out=(q_out, k_out)``
+    writes there instead (any strides with unit stride in D: a slice of a cache,
+    or the inputs themselves); it takes no part in autograd."""
+    key = (q.shape, q.dtype, k.shape, k.dtype, eps, *[
+        None if t is None else (t.shape, t.dtype)
+        for t in (cos, sin, positions, q_weight, k_weight)])
+    if key not in _checked:
+        _check(q, k, cos, sin, q_weight, k_weight, eps, positions)
+        if len(_checked) > 4096:
+            _checked.clear()
+        _checked.add(key)
+    index = q.get_device()
+    for t in (q, k, cos, sin, q_weight, k_weight, positions):
+        if t is not None and t.get_device() != index or index < 0:
+            backend.require_cuda(*[u for u in (q, k, cos, sin, q_weight, k_weight, positions)
+                                   if u is not None])
+            raise ValueError("all tensors must be on one device")
     grad = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
     if out is not None:

@@ -103,7 +103,8 @@ def _dev(t: torch.Tensor) -> int:
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the raw handle: torch.cuda.current_stream builds a Stream object each call
+    return torch._C._cuda_getCurrentRawStream(_dev(t))
 
 
 def _ptr(t: Optional[torch.Tensor]):

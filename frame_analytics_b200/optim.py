@@ -10,12 +10,12 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Iterable, Optional, Sequence
 
 import torch
 
 from . import backend
-from ._cabi import fa_matrix
 
 __all__ = ["orthogonalize", "muon_step", "Muon", "NEWTON_SCHULZ"]
 
@@ -26,6 +26,8 @@ NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 _MAX_STEPS = 32
 _coef_cache: dict = {}
+# struct fa_matrix of include/fa_b200.h as bytes
+_MATRIX = struct.Struct("@3P2i2qd").pack
 
 
 def _coefficients(coefficients, steps: int):
@@ -102,8 +104,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5,
     count, item = x3.shape[0], x.element_size()
     sb, sr = x3.stride(0) * item, x3.stride(1) if m > 1 else n
     src, dst = x3.data_ptr(), out.data_ptr()
-    mats = (fa_matrix * count)(*[(src + i * sb, dst + i * m * n * item, None, m, n, sr, n, 0.0)
-                                 for i in range(count)])
+    mats = b"".join([_MATRIX(src + i * sb, dst + i * m * n * item, 0, m, n, sr, n, 0.0)
+                     for i in range(count)])
     _run(backend.lib().fa_b200_orthogonalize, mats, count, x, coef, steps)
     return out
 
@@ -167,44 +169,48 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                          f"momentum {momentum} in [0, 1)")
     if not weights:
         return
-    first, rows, keep, seen = weights[0], [], [], set()
+    first, rows, keep = weights[0], [], []
+    dtype, index, scales = first.dtype, first.get_device(), {}
     for i, (w, g, m) in enumerate(zip(weights, grads, momenta)):
-        if w.dtype not in _DTYPES or w.dtype != first.dtype:
+        shape = w.shape
+        if w.dtype != dtype or dtype not in _DTYPES:
             raise TypeError(f"weights must share one of float16, bfloat16, float32; weight {i} is {w.dtype}")
-        if w.dim() < 2:
-            raise ValueError(f"weight {i} of shape {tuple(w.shape)} is not a matrix")
-        if g.shape != w.shape or g.dtype != w.dtype:
-            raise ValueError(f"gradient {i} must be {w.dtype} of shape {tuple(w.shape)}, got "
+        if len(shape) < 2:
+            raise ValueError(f"weight {i} of shape {tuple(shape)} is not a matrix")
+        if g.shape != shape or g.dtype != dtype:
+            raise ValueError(f"gradient {i} must be {w.dtype} of shape {tuple(shape)}, got "
                              f"{g.dtype} {tuple(g.shape)}")
-        if m.shape != w.shape or m.dtype != torch.float32:
-            raise ValueError(f"momentum {i} must be float32 of shape {tuple(w.shape)}, got "
+        if m.shape != shape or m.dtype != torch.float32:
+            raise ValueError(f"momentum {i} must be float32 of shape {tuple(shape)}, got "
                              f"{m.dtype} {tuple(m.shape)}")
-        backend.require_cuda(w, g, m)
-        if not w.device == g.device == m.device == first.device:
+        if not (w.get_device() == g.get_device() == m.get_device() == index) or index < 0:
+            backend.require_cuda(w, g, m)
             raise ValueError("weights, gradients and momenta must be on one device")
-        if w.numel() == 0:
+        n = w.numel()
+        if n == 0:
             continue
-        wm = _rows_layout(w.detach())
-        if wm is None:
-            raise ValueError(f"weight {i} must be contiguous (or a channels-last kernel)")
-        mm = _like_layout(m, w)
-        if mm is None:
-            raise ValueError(f"momentum {i} must have its weight's memory layout")
-        gm = _like_layout(g.detach(), w)
-        if gm is None:
-            # the weight's order of elements: a copy
-            gm = _rows_layout(torch.empty_like(w).copy_(g.detach()))
-            keep.append(gm)
-        for p in (wm.data_ptr(), mm.data_ptr()):
-            if p in seen:
-                raise ValueError(f"weight {i} or its momentum is given twice")
-            seen.add(p)
-        r, c = wm.shape
-        rows.append((gm.data_ptr(), wm.data_ptr(), mm.data_ptr(), r, c, c, c,
-                     lr * _scale(scale, r, c)))
+        wm, gm, mm = w, g, m
+        if not (w.is_contiguous() and g.is_contiguous() and m.is_contiguous()):
+            wm, mm, gm = _rows_layout(w.detach()), _like_layout(m, w), _like_layout(g.detach(), w)
+            if wm is None:
+                raise ValueError(f"weight {i} must be contiguous (or a channels-last kernel)")
+            if mm is None:
+                raise ValueError(f"momentum {i} must have its weight's memory layout")
+            if gm is None:
+                # the weight's order of elements: a copy
+                gm = _rows_layout(torch.empty_like(w).copy_(g.detach()))
+                keep.append(gm)
+        step = scales.get(shape)
+        if step is None:
+            step = scales[shape] = lr * _scale(scale, shape[0], n // shape[0])
+        r = shape[0]
+        c = n // r
+        rows.append((gm.data_ptr(), wm.data_ptr(), mm.data_ptr(), r, c, c, c, step))
+    if len({p for row in rows for p in row[1:3]}) < 2 * len(rows):
+        raise ValueError("a weight or a momentum is given twice")
     if not rows:
         return
-    mats = (fa_matrix * len(rows))(*rows)
+    mats = b"".join([_MATRIX(*row) for row in rows])
     _run(backend.lib().fa_b200_muon_step, mats, len(rows), first, coef, steps, momentum,
          int(nesterov), 1.0 - lr * weight_decay)
 
