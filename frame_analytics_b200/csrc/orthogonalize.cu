@@ -29,6 +29,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "mbar.cuh"
@@ -62,7 +63,7 @@ struct NsGroup {
   int tall, batch, first;          // matrices [first, first + batch)
   int px, pa;                      // row pitches of X and of A, B in elements
   int bn_sym, bn_app;              // tile columns of the symmetric products and of B X
-  int tiles_sym, tiles_app;        // tiles of one matrix
+  int tiles_sym, tiles_app;        // tiles of one matrix (of pairs, where blocks pair up)
   __half *x[2][2], *a[2], *b[2];   // [alternation][hi, lo]
   float *da, *db;                  // diagonals, [batch][pa]
 };
@@ -271,13 +272,22 @@ __device__ __forceinline__ bool wait_flag(const unsigned* flag, unsigned want, c
   return wait_slow(0, 0, flag, want, a);
 }
 
+// PAIR: `bar` may be the other block's of the pair.
+template <bool PAIR>
 __device__ __forceinline__ void tma_box(unsigned dst, const CUtensorMap* map, int x, int y, int z,
                                         unsigned bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
-      "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::"
+        "bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
+        "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(dst),
+        "l"(reinterpret_cast<unsigned long long>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
 }
 
 // Shared-memory operand descriptor, 128-byte swizzle.  Rows along K (K-major):
@@ -289,22 +299,54 @@ __device__ __forceinline__ unsigned long long operand(unsigned addr) {
          (1ull << 46) | (2ull << 61);
 }
 
+template <bool PAIR>
 __device__ __forceinline__ void mma_f16(unsigned d, unsigned long long a, unsigned long long b,
                                         unsigned idesc, bool add) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"((unsigned)add)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((unsigned)add)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((unsigned)add)
+        : "memory");
 }
+// Arrives when the products issued so far are complete; PAIR: in both blocks.
+template <bool PAIR>
 __device__ __forceinline__ void mma_commit(unsigned long long* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(
-          smem_u32(bar))
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
+        "[%0], %1;\n" ::"r"(smem_u32(bar)), "h"((unsigned short)3)
+        : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(
+            smem_u32(bar))
+        : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(unsigned long long* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+// The same shared address in the pair's first block, which issues the products.
+__device__ __forceinline__ unsigned in_leader(unsigned addr) {
+  unsigned r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;\n" : "=r"(r) : "r"(addr));
+  return r;
+}
+template <bool PAIR>
+__device__ __forceinline__ void arrive_leader(unsigned long long* bar) {
+  if constexpr (PAIR)
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(
+                     in_leader(smem_u32(bar)))
+                 : "memory");
+  else
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::
+                   : "memory");
 }
 
 // 32 accumulator columns of this thread's row.
@@ -326,19 +368,32 @@ __device__ __forceinline__ void tmem_load32(unsigned addr, float (&v)[32]) {
 }
 
 // Where a tile is.  Tiles are numbered phase by phase (A, A^2, B X of step 0,
-// of step 1, ...), inside a phase matrix by matrix; CTA c takes numbers c,
-// c + gridDim.x, ...  A tile waits only for tiles of earlier phases, and every
-// CTA is resident, so the lowest unfinished tile can always proceed.
+// of step 1, ...), inside a phase matrix by matrix; block (or pair) c takes
+// numbers c, c + units, ...  A tile waits only for tiles of earlier phases, and
+// every block is resident, so the lowest unfinished tile can always proceed.
 struct Tile {
   int phase, step;                 // phase 0: A, 1: A^2, 2: B X
   int group, mat;                  // mat counts over the whole call
-  int i0, j0, bn, kblocks;
+  int i0, j0, bn, kblocks;         // i0: this block's 128 rows
 };
 
+// Tiles of the lower triangle of an s x s product, bm rows by bn columns: row
+// block ti takes the tiles that start at or left of its own last column.
+__host__ __device__ __forceinline__ int sym_tiles(int s, int bm, int bn) {
+  const int T = (s + bm - 1) / bm, u = T / 2;
+  if (bm == bn) return T * (T + 1) / 2;
+  if (bm < bn) return T % 2 ? (u + 1) * (u + 1) : u * (u + 1);  // bn = 2 bm
+  return T * (T + 1);                                            // bm = 2 bn
+}
+
+template <bool PAIR>
 struct Walk {
+  static constexpr int kRows = PAIR ? 2 * BM : BM;
   int step = 0, phase = 0;
+  const int units, rank;
   long long t;
-  __device__ explicit Walk(long long first) : t(first) {}
+  __device__ Walk() : units(PAIR ? gridDim.x / 2 : gridDim.x), rank(PAIR ? blockIdx.x & 1 : 0),
+                      t(PAIR ? blockIdx.x / 2 : blockIdx.x) {}
   __device__ bool next(const NsArgs& a, Tile* o) {
     for (;;) {
       const int n = phase == 2 ? a.tiles_app : a.tiles_sym;
@@ -360,23 +415,22 @@ struct Walk {
     o->phase = phase;
     o->step = step;
     o->group = gi;
+    int ti, tj;
     if (phase == 2) {
       const int b = r / g.tiles_app;
       r -= b * g.tiles_app;
       o->mat = g.first + b;
       o->bn = g.bn_app;
       const int tn = (g.cols + o->bn - 1) / o->bn;
-      o->i0 = r / tn * BM;
-      o->j0 = r % tn * o->bn;
+      ti = r / tn;
+      tj = r - ti * tn;
       o->kblocks = (g.s + BK - 1) / BK;
     } else {
       const int b = r / g.tiles_sym;
       r -= b * g.tiles_sym;
       o->mat = g.first + b;
       o->bn = g.bn_sym;
-      // lower triangle by 128-row blocks; see sym_tiles
-      int ti, tj;
-      if (o->bn == 128) {
+      if (o->bn == kRows) {
         int u = (int)((sqrtf(8.f * r + 1.f) - 1.f) * 0.5f);
         while (u * (u + 1) / 2 > r) --u;
         while ((u + 1) * (u + 2) / 2 <= r) ++u;
@@ -387,36 +441,30 @@ struct Walk {
         while (u * (u + 1) > r) --u;
         while ((u + 1) * (u + 2) <= r) ++u;
         r -= u * (u + 1);
-        ti = o->bn == 256 ? 2 * u + r / (u + 1) : u;
-        tj = o->bn == 256 ? r % (u + 1) : r;
+        ti = o->bn > kRows ? 2 * u + r / (u + 1) : u;
+        tj = o->bn > kRows ? r % (u + 1) : r;
       }
-      o->i0 = ti * BM;
-      o->j0 = tj * o->bn;
       o->kblocks = ((phase == 0 ? g.l : g.s) + BK - 1) / BK;
     }
-    t += gridDim.x;
+    o->i0 = ti * kRows + rank * BM;
+    o->j0 = tj * o->bn;
+    t += units;
     return true;
   }
 };
 
-// Tiles of the lower triangle of an s x s product: row block ti (128 rows)
-// takes the tiles that start at or left of its own last column.
-static int sym_tiles(int s, int bn) {
-  const int T = (s + 127) / 128, u = T / 2;
-  if (bn == 128) return T * (T + 1) / 2;
-  if (bn == 256) return T % 2 ? (u + 1) * (u + 1) : u * (u + 1);
-  return T * (T + 1);
-}
-
 // Shared memory: operand stages, then a 32 x 32 float buffer for each epilogue
 // warp.  A stage holds 64 K columns of the row operand (128 rows) and of the
 // column operand (256 rows; split: 128, twice).
-template <bool SPLIT>
+// A pair of blocks shares a tile of 256 rows: each block keeps its own 128 rows
+// of the row operand and half of the column operand.
+template <bool SPLIT, bool PAIR>
 struct Stage {
   static constexpr int kParts = SPLIT ? 2 : 1;
-  static constexpr int kWide = SPLIT ? 128 : 256;                      // widest tile
-  static constexpr int kBytes = kParts * (BM / 64 + kWide / 64) * kBox;  // 48 or 64 KB
-  static constexpr int kCount = SPLIT ? 3 : 4;
+  static constexpr int kWidest = SPLIT ? 128 : 256;                    // tile columns
+  static constexpr int kWide = PAIR ? kWidest / 2 : kWidest;           // column operand here
+  static constexpr int kBytes = kParts * (BM / 64 + kWide / 64) * kBox;  // 32 to 64 KB
+  static constexpr int kCount = PAIR ? (SPLIT ? 4 : 6) : (SPLIT ? 3 : 4);  // 192 KB
   static constexpr int kTurn = (kEpilogue / 32) * 4096;
   static constexpr int kSmem = kCount * kBytes + kTurn + 1024;
 };
@@ -685,13 +733,13 @@ __device__ __forceinline__ void ns_emit(const NsArgs& a, const Tile& t, const Ou
 // memory (TMA), warp 1 issues the products (one thread), warps 4-11 read the
 // accumulators (two, so that a tile's epilogue overlaps the next tile's
 // products).
-template <bool SPLIT, typename T>
+template <bool SPLIT, bool PAIR, typename T>
 __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_constant__ NsArgs a) {
-  using St_ = Stage<SPLIT>;
+  using St_ = Stage<SPLIT, PAIR>;
   constexpr int S = St_::kCount, PARTS = St_::kParts;
   extern __shared__ char smem_raw[];
   const unsigned smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  __shared__ unsigned long long full[4], empty[4], tm_full[2], tm_empty[2], sm_empty[2],
+  __shared__ unsigned long long full[6], empty[6], tm_full[2], tm_empty[2], sm_empty[2],
       drain;
   __shared__ unsigned tmem_base;
   __shared__ volatile int dead;
@@ -704,8 +752,8 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tm_full[i], 1);
-      mbar_init(&tm_empty[i], kEpilogue);
-      mbar_init(&sm_empty[i], kEpilogue);
+      mbar_init(&tm_empty[i], (kEpilogue / 32) * (PAIR ? 2 : 1));  // a warp each
+      mbar_init(&sm_empty[i], (kEpilogue / 32) * (PAIR ? 2 : 1));
     }
     mbar_init(&drain, 1);
     dead = 0;
@@ -713,19 +761,28 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
     fence_async_smem();
   }
   if (warp == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(
-                     smem_u32(&tmem_base))
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(
+                       smem_u32(&tmem_base))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(
+                       smem_u32(&tmem_base))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the other block's barriers are ready
   asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
   const unsigned tmem = tmem_base;
+  const int rank = PAIR ? blockIdx.x & 1 : 0;
 
   if (warp == 0) {
     if (lane == 0) {
-      Walk walk(blockIdx.x);
+      Walk<PAIR> walk;
       Tile t;
       unsigned n = 0;  // stages issued
       bool ok = true;
@@ -734,7 +791,8 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
         // what this tile reads: X of the last step, O, or offdiag(B)
         const int from = t.phase == 0 ? 2 : t.phase - 1;
         const int rounds = t.phase == 0 ? t.step : t.step + 1;
-        const unsigned want = (unsigned)rounds * (t.phase == 0 ? g.tiles_app : g.tiles_sym);
+        const unsigned want =
+            (unsigned)rounds * (t.phase == 0 ? g.tiles_app : g.tiles_sym) * (PAIR ? 2u : 1u);
         if (!wait_flag(a.done + from * kMats + t.mat, want, a)) break;
         asm volatile("fence.proxy.async;\n" ::: "memory");
         const int xi = MAP_X0 + (t.step & 1);
@@ -742,36 +800,39 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
         const int mq = t.phase == 0 ? xi : t.phase == 1 ? MAP_A : g.tall ? MAP_B : xi;
         const bool p_mn = t.phase == 0 && g.tall;
         const bool q_mn = t.phase == 0 ? g.tall : t.phase == 2 && !g.tall;
-        const int z = t.mat - g.first, qb = t.bn / 64;
+        const int z = t.mat - g.first, qw = t.bn / (PAIR ? 2 : 1), qb = qw / 64;
+        const int jq = t.j0 + rank * qw;
         for (int kb = 0; kb < t.kblocks; ++kb, ++n) {
           const int s = n % S;
           if (n >= (unsigned)S && !wait_bar(&empty[s], (n / S - 1) & 1, a)) {
             ok = false;
             break;
           }
-          const unsigned bar = smem_u32(&full[s]);
+          // both blocks' copies count on the first block's barrier
+          const unsigned bar = PAIR ? in_leader(smem_u32(&full[s])) : smem_u32(&full[s]);
           const unsigned base = smem0 + s * St_::kBytes;
-          mbar_expect_tx(&full[s], PARTS * (BM / 64 + qb) * kBox);
+          if (rank == 0)
+            mbar_expect_tx(&full[s], (PAIR ? 2 : 1) * PARTS * (BM / 64 + qb) * kBox);
 #pragma unroll
           for (int part = 0; part < PARTS; ++part) {
             const unsigned bp = base + part * (BM / 64) * kBox;
             const unsigned bq = base + (PARTS * (BM / 64) + part * (St_::kWide / 64)) * kBox;
             for (int i = 0; i < BM / 64; ++i)
-              tma_box(bp + i * kBox, &g.map[mp][part], p_mn ? t.i0 + 64 * i : kb * BK,
+              tma_box<PAIR>(bp + i * kBox, &g.map[mp][part], p_mn ? t.i0 + 64 * i : kb * BK,
                       p_mn ? kb * BK : t.i0 + 64 * i, z, bar);
             for (int i = 0; i < qb; ++i)
-              tma_box(bq + i * kBox, &g.map[mq][part], q_mn ? t.j0 + 64 * i : kb * BK,
-                      q_mn ? kb * BK : t.j0 + 64 * i, z, bar);
+              tma_box<PAIR>(bq + i * kBox, &g.map[mq][part], q_mn ? jq + 64 * i : kb * BK,
+                      q_mn ? kb * BK : jq + 64 * i, z, bar);
           }
         }
       }
       // copies still in flight land before the block ends
-      for (unsigned i = n > (unsigned)S ? n - S : 0; i < n; ++i)
+      for (unsigned i = n > (unsigned)S ? n - S : 0; rank == 0 && i < n; ++i)
         wait_bar(&full[i % S], (i / S) & 1, a);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      Walk walk(blockIdx.x);
+    if (lane == 0 && rank == 0) {
+      Walk<PAIR> walk;
       Tile t;
       unsigned n = 0, tile = 0, sums = 0;
       bool ok = true;
@@ -779,9 +840,9 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
         const NsGroup& g = a.g[t.group];
         const bool p_mn = t.phase == 0 && g.tall;
         const bool q_mn = t.phase == 0 ? g.tall : t.phase == 2 && !g.tall;
-        // float32 accumulators, float16 operands, M = 128
+        // float32 accumulators, float16 operands, M = 128 (256 over a pair)
         const unsigned idesc = (1u << 4) | ((unsigned)p_mn << 15) | ((unsigned)q_mn << 16) |
-                               ((unsigned)(t.bn / 8) << 17) | ((unsigned)(BM / 16) << 24);
+                               ((unsigned)(t.bn / 8) << 17) | ((unsigned)((PAIR ? 2 : 1) * BM / 16) << 24);
         const int chunk = SPLIT ? kChunk : t.kblocks;
         const unsigned ps = (p_mn ? 2048u : 32u) >> 4, qs = (q_mn ? 2048u : 32u) >> 4;
         if (SPLIT && tile >= 2 && !wait_bar(&sm_empty[tile & 1], (tile / 2 - 1) & 1, a)) break;
@@ -811,22 +872,24 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
             for (int k = 0; k < BK / 16; ++k) {
               const unsigned long long po = k * ps, qo = k * qs;
               if (SPLIT) {
-                mma_f16(dsmall, p0 + po, q1 + qo, idesc, kb > 0 || k > 0);
-                mma_f16(dsmall, p1 + po, q0 + qo, idesc, true);
+                mma_f16<PAIR>(dsmall, p0 + po, q1 + qo, idesc, kb > 0 || k > 0);
+                mma_f16<PAIR>(dsmall, p1 + po, q0 + qo, idesc, true);
               }
-              mma_f16(d, p0 + po, q0 + qo, idesc, kb > kb0 || k > 0);
+              mma_f16<PAIR>(d, p0 + po, q0 + qo, idesc, kb > kb0 || k > 0);
             }
-            mma_commit(&empty[s]);
+            mma_commit<PAIR>(&empty[s]);
           }
-          mma_commit(&tm_full[buf]);
+          mma_commit<PAIR>(&tm_full[buf]);
         }
       }
       // products still in flight end before tensor memory is given back
-      mma_commit(&drain);
+      mma_commit<PAIR>(&drain);
       wait_bar(&drain, 0, a);
     }
+    // the second block's barriers hear of it too, and it stays until they have
+    if (PAIR && lane == 0 && rank == 1) wait_bar(&drain, 0, a);
   } else if (warp >= 4) {
-    Walk walk(blockIdx.x);
+    Walk<PAIR> walk;
     Tile t;
     const int w = warp & 3, h = (warp - 4) >> 2;
     float4* const turn = reinterpret_cast<float4*>(smem_raw + (smem0 - smem_u32(smem_raw)) +
@@ -858,7 +921,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
           }
           __syncwarp();
           asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-          mbar_arrive(&tm_empty[buf]);
+          if (lane == 0) arrive_leader<PAIR>(&tm_empty[buf]);
         }
       }
       if (!ok) dead = 1;
@@ -878,7 +941,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
         }
         __syncwarp();
         asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-        mbar_arrive(&sm_empty[tile & 1]);
+        if (lane == 0) arrive_leader<PAIR>(&sm_empty[tile & 1]);
 #pragma unroll
         for (int q = 0; q < 2; ++q)
           if (q * 32 < half) ns_emit<SPLIT, T>(a, t, out, i, jh + q * 32, turn, sum[q]);
@@ -890,7 +953,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
           if (c0 + 32 >= half) {
             __syncwarp();
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-            mbar_arrive(&tm_empty[buf]);
+            if (lane == 0) arrive_leader<PAIR>(&tm_empty[buf]);
           }
           ns_emit<SPLIT, T>(a, t, out, i, jh + c0, turn, sum[0]);
         }
@@ -908,9 +971,13 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // neither block's memory is in use any more
   if (warp == 2) {
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
+    if constexpr (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
   }
 }
 
@@ -1026,29 +1093,37 @@ static void group_shape(NsGroup* g, int rows, int cols, int batch, int first) {
   g->pa = pitch64(g->s);
 }
 
-static int tile_count(const NsGroup& g, bool sym, int bn) {
-  return sym ? sym_tiles(g.s, bn) : (g.rows + BM - 1) / BM * ((g.cols + bn - 1) / bn);
+static int tile_count(const NsGroup& g, bool sym, int bm, int bn) {
+  return sym ? sym_tiles(g.s, bm, bn)
+             : ((g.rows + bm - 1) / bm) * ((g.cols + bn - 1) / bn);
 }
 
-// Columns of a tile.  Wider tiles reuse the row operand more (measured on
-// 4096 x 8192: a tile of 64, 128, 256 columns takes 0.57, 0.71, 1 of the time
-// of the last), narrower ones fill more multiprocessors: the fewest waves
-// times the time of one.  Three products (split) hold their sums in registers
-// and two accumulators each, which leaves room for 128 columns.
-static int pick_bn(const NsGroup& g, bool sym, bool split, int sms) {
-  static const int width[3] = {64, 128, 256};
-  static const double cost[3] = {0.57, 0.71, 1.0};
-  int best = 64;
+// Microseconds of 64 K columns of a tile on one multiprocessor, by its columns
+// (64, 128, 256) and with both blocks of a pair on one tile.  The products
+// themselves take a third to a half of it: the operands come out of the second
+// level cache at about 65 GB/s a multiprocessor, so what counts is bytes a
+// tile.  Split tiles hold their sums in registers and two accumulators, which
+// leaves room for 128 columns.
+static const double kTileUs[2][2][3] = {{{0.41, 0.50, 0.69}, {9.9, 9.9, 0.47}},
+                                        {{0.62, 0.80, 9.9}, {9.9, 0.70, 9.9}}};
+static const int kTileCols[3] = {64, 128, 256};
+
+// Tile columns with the least time: waves of tiles, one wave more in effect for
+// the epilogue that nothing hides.
+static double pick_bn(const NsGroup& g, bool sym, bool split, bool pair, int units, int* bn) {
   double least = 1e300;
-  for (int i = 0; i < (split ? 2 : 3); ++i) {
-    const long long tiles = (long long)g.batch * tile_count(g, sym, width[i]);
-    const double c = (double)((tiles + sms - 1) / sms) * cost[i];
+  for (int i = 0; i < 3; ++i) {
+    const double us = kTileUs[split][pair][i];
+    if (us > 9) continue;
+    const long long tiles =
+        (long long)g.batch * tile_count(g, sym, pair ? 2 * BM : BM, kTileCols[i]);
+    const double c = (double)((tiles + units - 1) / units) * us;
     if (c < least) {
       least = c;
-      best = width[i];
+      *bn = kTileCols[i];
     }
   }
-  return best;
+  return least;
 }
 
 size_t ns_ws_bytes(const fa_matrix* m, int count, int dtype) {
@@ -1111,8 +1186,62 @@ static bool plan_steps(NsStep* k, const double* coef, int steps) {
   return true;
 }
 
+// Pairs of blocks that are resident together, at most one block on a
+// multiprocessor; asked once for each device.
 template <bool SPLIT, typename T>
-static int ns_run(const NsArgs& a, int device, cudaStream_t st) {
+static int pairs_resident(int device) {
+  constexpr int MAXD = 64;
+  static std::atomic<int> known[MAXD];
+  if (device < 0 && cudaGetDevice(&device) != cudaSuccess) return 0;
+  if (device < MAXD && known[device].load() > 0) return known[device].load() - 1;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 2;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)(sm_count(device) / 2 * 2));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Stage<SPLIT, true>::kSmem;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaFuncSetAttribute(ns_product_kernel<SPLIT, true, T>,
+                           cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           Stage<SPLIT, true>::kSmem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, ns_product_kernel<SPLIT, true, T>, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  if (device < MAXD) known[device].store(n + 1);
+  return n;
+}
+
+template <bool SPLIT, bool PAIR, typename T>
+static int ns_products(const NsArgs& a, int units, cudaStream_t st) {
+  constexpr int smem = Stage<SPLIT, PAIR>::kSmem;
+  FAB_TRY(cudaFuncSetAttribute(ns_product_kernel<SPLIT, PAIR, T>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  // every block waits for other blocks' tiles: a cooperative launch makes them resident
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeCooperative;
+  at[0].val.cooperative = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 2;
+  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  cfg.gridDim = dim3((unsigned)std::min(units, std::max(a.tiles_sym, a.tiles_app)) *
+                     (PAIR ? 2u : 1u));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = PAIR ? 2 : 1;
+  FAB_TRY(cudaLaunchKernelEx(&cfg, ns_product_kernel<SPLIT, PAIR, T>, a));
+  return FA_OK;
+}
+
+template <bool SPLIT, typename T>
+static int ns_run(NsArgs& a, int device, cudaStream_t st) {
   const int sms = sm_count(device);
   long long most = 0;
   for (int g = 0; g < a.groups; ++g)
@@ -1126,15 +1255,31 @@ static int ns_run(const NsArgs& a, int device, cudaStream_t st) {
       1, std::min<long long>((most + 4095) / 4096, std::max(1, sms * 8 / a.mats)));
   ns_pack_kernel<T><<<dim3(pb, a.mats), 256, 0, st>>>(a, nb);
   FAB_LAUNCH_CHECK();
-  constexpr int smem = Stage<SPLIT>::kSmem;
-  FAB_TRY(cudaFuncSetAttribute(ns_product_kernel<SPLIT, T>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  // every block waits for other blocks' tiles: a cooperative launch makes them resident
-  const unsigned grid = (unsigned)std::min(sms, std::max(a.tiles_sym, a.tiles_app));
-  void* args[] = {const_cast<NsArgs*>(&a)};
-  FAB_TRY(cudaLaunchCooperativeKernel(reinterpret_cast<void*>(ns_product_kernel<SPLIT, T>),
-                                      dim3(grid), dim3(kThreads), args, smem, st));
-  return FA_OK;
+  // tile shapes: single blocks or pairs for the whole launch, the faster by estimate
+  const int pairs = pairs_resident<SPLIT, T>(device);
+  int bn[2][kGroups][2];
+  double cost[2] = {0, 0};
+  for (int pair = 0; pair < 2; ++pair)
+    for (int g = 0; g < a.groups; ++g)
+      for (int sym = 0; sym < 2; ++sym) {
+        const NsGroup& gr = a.g[g];
+        const double c = pick_bn(gr, sym, SPLIT, pair, pair ? std::max(pairs, 1) : sms,
+                                 &bn[pair][g][sym]);
+        cost[pair] += c * (sym ? gr.l + gr.s : gr.s);  // K of A and A^2, of B X
+      }
+  const bool pair = pairs > 0 && cost[1] < cost[0];
+  a.tiles_sym = a.tiles_app = 0;
+  for (int i = 0; i < a.groups; ++i) {
+    NsGroup& g = a.g[i];
+    g.bn_app = bn[pair][i][0];
+    g.bn_sym = bn[pair][i][1];
+    g.tiles_sym = tile_count(g, true, pair ? 2 * BM : BM, g.bn_sym);
+    g.tiles_app = tile_count(g, false, pair ? 2 * BM : BM, g.bn_app);
+    a.tiles_sym += g.batch * g.tiles_sym;
+    a.tiles_app += g.batch * g.tiles_app;
+  }
+  return pair ? ns_products<SPLIT, true, T>(a, pairs, st)
+              : ns_products<SPLIT, false, T>(a, sms, st);
 }
 
 int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int steps,
@@ -1162,18 +1307,11 @@ int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int
     size_t off = up256(kNsHead);
     a.groups = bt.groups;
     a.mats = bt.n;
-    a.tiles_sym = a.tiles_app = 0;
     for (int gi = 0; gi < bt.groups; ++gi) {
       NsGroup& g = a.g[gi];
       group_shape(&g, bt.rows[gi], bt.cols[gi], bt.count[gi], bt.first[gi]);
       off += group_layout(&g, split, static_cast<char*>(ws) + off);
       if (off > ws_bytes) return FA_E_ARG;
-      g.bn_sym = pick_bn(g, true, split, sm_count(device));
-      g.bn_app = pick_bn(g, false, split, sm_count(device));
-      g.tiles_sym = tile_count(g, true, g.bn_sym);
-      g.tiles_app = tile_count(g, false, g.bn_app);
-      a.tiles_sym += g.batch * g.tiles_sym;
-      a.tiles_app += g.batch * g.tiles_app;
       for (int h = 0; h < (split ? 2 : 1); ++h) {
         if (!half_map(&g.map[MAP_X0][h], g.x[0][h], g.batch, g.rows, g.cols, g.px) ||
             !half_map(&g.map[MAP_X1][h], g.x[1][h], g.batch, g.rows, g.cols, g.px) ||
