@@ -46,6 +46,10 @@ constexpr int BM = 128;            // tile rows: the lanes of tensor memory
 constexpr int BK = 64;             // 128 bytes of float16: one swizzle row
 constexpr int kBox = 64 * 128;     // bytes of a 64 x 64 box
 constexpr int kEpilogue = 256;     // 8 epilogue warps: 4 quarters of the rows x 2 column halves
+constexpr int kSplitUnits = 148;   // parts of split tiles at most: one a multiprocessor
+constexpr int kSplitTiles = kSplitUnits / 2;
+constexpr int kMaxParts = 16;
+constexpr int kPart = BM * 64;     // floats of a part: split tiles have 64 columns
 constexpr int kThreads = 128 + kEpilogue;  // producer, issuer, allocator, spare before them
 // The tensor cores add into an accumulator with truncation, a relative loss of
 // about 2^-25 for each 16 columns of K, always towards zero.  float32-like
@@ -64,6 +68,8 @@ struct NsGroup {
   int px, pa;                      // row pitches of X and of A, B in elements
   int bn_sym, bn_app;              // tile columns of the symmetric products and of B X
   int tiles_sym, tiles_app;        // tiles of one matrix (of pairs, where blocks pair up)
+  int ks[2];                       // parts of K that A's and A^2's tiles are split into
+  int slot;                        // the first of this shape's tiles among those split
   __half *x[2][2], *a[2], *b[2];   // [alternation][hi, lo]
   float *da, *db;                  // diagonals, [batch][pa]
 };
@@ -89,11 +95,15 @@ struct NsArgs {
   NsMat m[kMats];
   NsStep k[kMaxSteps];
   int groups, mats, steps;
-  int tiles_sym, tiles_app;        // over all matrices
+  int tiles[3];                    // of the three products, over all matrices
   unsigned* done;                  // [3][kMats] finished tiles of the three products
+  unsigned* joins;                 // [2][kSplitTiles] finished parts of the split tiles
+  float* parts;                    // [kSplitUnits] sums of a part of a tile
   unsigned* failed;                // set when a wait of this call gave up
   double* part;                    // [kMats][kNormBlocks]
   unsigned* err;
+  int pair;                        // two blocks a tile
+  int ks;                          // parts of a tile at most
   float mu, decay;
   int nesterov;
 };
@@ -176,7 +186,10 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ Ns
   if (threadIdx.x == 0) a.part[blockIdx.y * kNormBlocks + blockIdx.x] = ss;
   // the product kernel's counters, for this call
   if (blockIdx.x == 0 && threadIdx.x < 3) a.done[threadIdx.x * kMats + blockIdx.y] = 0u;
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 3) *a.failed = 0u;
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
+    if (threadIdx.x == 3) *a.failed = 0u;
+    if (threadIdx.x < 2 * kSplitTiles) a.joins[threadIdx.x] = 0u;
+  }
 }
 
 __device__ __forceinline__ void split_half(float v, __half* hi, __half* lo) {
@@ -374,7 +387,8 @@ __device__ __forceinline__ void tmem_load32(unsigned addr, float (&v)[32]) {
 struct Tile {
   int phase, step;                 // phase 0: A, 1: A^2, 2: B X
   int group, mat;                  // mat counts over the whole call
-  int i0, j0, bn, kblocks;         // i0: this block's 128 rows
+  int i0, j0, bn, kb0, kb1;        // i0: this block's 128 rows; K blocks [kb0, kb1)
+  int ks, part, slot, region;      // parts of K, which one, the tile and its first part's place
 };
 
 // Tiles of the lower triangle of an s x s product, bm rows by bn columns: row
@@ -396,7 +410,7 @@ struct Walk {
                       t(PAIR ? blockIdx.x / 2 : blockIdx.x) {}
   __device__ bool next(const NsArgs& a, Tile* o) {
     for (;;) {
-      const int n = phase == 2 ? a.tiles_app : a.tiles_sym;
+      const int n = a.tiles[phase];
       if (t < n) break;
       t -= n;
       if (++phase == 3) {
@@ -407,7 +421,7 @@ struct Walk {
     int r = (int)t, gi = 0;
     for (;; ++gi) {
       const NsGroup& g = a.g[gi];
-      const int n = g.batch * (phase == 2 ? g.tiles_app : g.tiles_sym);
+      const int n = g.batch * (phase == 2 ? g.tiles_app : g.tiles_sym * g.ks[phase]);
       if (r < n) break;
       r -= n;
     }
@@ -415,6 +429,9 @@ struct Walk {
     o->phase = phase;
     o->step = step;
     o->group = gi;
+    o->ks = 1;
+    o->part = 0;
+    o->kb0 = 0;
     int ti, tj;
     if (phase == 2) {
       const int b = r / g.tiles_app;
@@ -424,10 +441,17 @@ struct Walk {
       const int tn = (g.cols + o->bn - 1) / o->bn;
       ti = r / tn;
       tj = r - ti * tn;
-      o->kblocks = (g.s + BK - 1) / BK;
+      o->kb1 = (g.s + BK - 1) / BK;
     } else {
-      const int b = r / g.tiles_sym;
-      r -= b * g.tiles_sym;
+      const int ks = g.ks[phase];
+      const int tile = r / ks;
+      o->ks = ks;
+      o->part = r - tile * ks;
+      o->slot = g.slot + tile;
+      // a place of its own for both products: matrices are in different phases
+      o->region = o->slot * a.ks;
+      const int b = tile / g.tiles_sym;
+      r = tile - b * g.tiles_sym;
       o->mat = g.first + b;
       o->bn = g.bn_sym;
       if (o->bn == kRows) {
@@ -444,7 +468,9 @@ struct Walk {
         ti = o->bn > kRows ? 2 * u + r / (u + 1) : u;
         tj = o->bn > kRows ? r % (u + 1) : r;
       }
-      o->kblocks = ((phase == 0 ? g.l : g.s) + BK - 1) / BK;
+      const int kb = ((phase == 0 ? g.l : g.s) + BK - 1) / BK;
+      o->kb0 = (int)((long long)kb * o->part / ks);
+      o->kb1 = (int)((long long)kb * (o->part + 1) / ks);
     }
     o->i0 = ti * kRows + rank * BM;
     o->j0 = tj * o->bn;
@@ -463,8 +489,8 @@ struct Stage {
   static constexpr int kParts = SPLIT ? 2 : 1;
   static constexpr int kWidest = SPLIT ? 128 : 256;                    // tile columns
   static constexpr int kWide = PAIR ? kWidest / 2 : kWidest;           // column operand here
-  static constexpr int kBytes = kParts * (BM / 64 + kWide / 64) * kBox;  // 32 to 64 KB
-  static constexpr int kCount = PAIR ? (SPLIT ? 4 : 6) : (SPLIT ? 3 : 4);  // 192 KB
+  static constexpr int kBytes = kParts * (BM / 64 + kWide / 64) * kBox;  // 48, 32, 64 KB
+  static constexpr int kCount = PAIR ? 6 : SPLIT ? 3 : 4;              // 192 KB
   static constexpr int kTurn = (kEpilogue / 32) * 4096;
   static constexpr int kSmem = kCount * kBytes + kTurn + 1024;
 };
@@ -729,6 +755,44 @@ __device__ __forceinline__ void ns_emit(const NsArgs& a, const Tile& t, const Ou
   __syncwarp();  // the buffer is free for the next block
 }
 
+// A part of a split tile: its sums go to memory, and the block that finishes the
+// last part adds all of them in their order (so the result does not depend on
+// which block that is) and goes on with the tile.
+__device__ __forceinline__ bool ns_join(const NsArgs& a, const Tile& t, int w, int h,
+                                        float (&sums)[32], volatile int* joined) {
+  const int lane = threadIdx.x & 31;
+  // four columns of 32 rows are 512 contiguous bytes
+  const long long at = (long long)(8 * h) * BM + 32 * w + lane;
+  float4* const tile = reinterpret_cast<float4*>(a.parts) + (long long)t.region * (kPart / 4);
+  float4* p = tile + t.part * (kPart / 4) + at;
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    __stcg(p + q * BM, make_float4(sums[4 * q], sums[4 * q + 1], sums[4 * q + 2], sums[4 * q + 3]));
+  __threadfence();
+  asm volatile("bar.sync 1, 256;\n" ::: "memory");
+  if (threadIdx.x == 128) {
+    const unsigned old = atomicAdd(a.joins + t.phase * kSplitTiles + t.slot, 1u);
+    *joined = old % (unsigned)t.ks == (unsigned)t.ks - 1u;
+    __threadfence();
+  }
+  asm volatile("bar.sync 1, 256;\n" ::: "memory");
+  if (!*joined) return false;
+#pragma unroll
+  for (int c = 0; c < 32; ++c) sums[c] = 0.f;
+  const float4* from = tile + at;
+  for (int k = 0; k < t.ks; ++k, from += kPart / 4) {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float4 v = __ldcg(from + q * BM);
+      sums[4 * q] += v.x;
+      sums[4 * q + 1] += v.y;
+      sums[4 * q + 2] += v.z;
+      sums[4 * q + 3] += v.w;
+    }
+  }
+  return true;
+}
+
 // Products of the current matrices.  Warp 0 copies operand tiles into shared
 // memory (TMA), warp 1 issues the products (one thread), warps 4-11 read the
 // accumulators (two, so that a tile's epilogue overlaps the next tile's
@@ -742,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
   __shared__ unsigned long long full[6], empty[6], tm_full[2], tm_empty[2], sm_empty[2],
       drain;
   __shared__ unsigned tmem_base;
-  __shared__ volatile int dead;
+  __shared__ volatile int dead, joined;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -802,7 +866,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
         const bool q_mn = t.phase == 0 ? g.tall : t.phase == 2 && !g.tall;
         const int z = t.mat - g.first, qw = t.bn / (PAIR ? 2 : 1), qb = qw / 64;
         const int jq = t.j0 + rank * qw;
-        for (int kb = 0; kb < t.kblocks; ++kb, ++n) {
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
           const int s = n % S;
           if (n >= (unsigned)S && !wait_bar(&empty[s], (n / S - 1) & 1, a)) {
             ok = false;
@@ -843,11 +907,11 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
         // float32 accumulators, float16 operands, M = 128 (256 over a pair)
         const unsigned idesc = (1u << 4) | ((unsigned)p_mn << 15) | ((unsigned)q_mn << 16) |
                                ((unsigned)(t.bn / 8) << 17) | ((unsigned)((PAIR ? 2 : 1) * BM / 16) << 24);
-        const int chunk = SPLIT ? kChunk : t.kblocks;
+        const int chunk = SPLIT ? kChunk : t.kb1 - t.kb0;
         const unsigned ps = (p_mn ? 2048u : 32u) >> 4, qs = (q_mn ? 2048u : 32u) >> 4;
         if (SPLIT && tile >= 2 && !wait_bar(&sm_empty[tile & 1], (tile / 2 - 1) & 1, a)) break;
         const unsigned dsmall = tmem + 256 + (tile & 1) * 128;
-        for (int kb0 = 0; ok && kb0 < t.kblocks; kb0 += chunk, ++sums) {
+        for (int kb0 = t.kb0; ok && kb0 < t.kb1; kb0 += chunk, ++sums) {
           const int buf = sums & 1;
           if (sums >= 2 && !wait_bar(&tm_empty[buf], (sums / 2 - 1) & 1, a)) {
             ok = false;
@@ -855,7 +919,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
           }
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
           const unsigned d = tmem + buf * (SPLIT ? 128 : 256);
-          const int kb1 = min(t.kblocks, kb0 + chunk);
+          const int kb1 = min(t.kb1, kb0 + chunk);
           for (int kb = kb0; kb < kb1; ++kb, ++n) {
             const int s = n % S;
             if (!wait_bar(&full[s], (n / S) & 1, a)) {
@@ -872,7 +936,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
             for (int k = 0; k < BK / 16; ++k) {
               const unsigned long long po = k * ps, qo = k * qs;
               if (SPLIT) {
-                mma_f16<PAIR>(dsmall, p0 + po, q1 + qo, idesc, kb > 0 || k > 0);
+                mma_f16<PAIR>(dsmall, p0 + po, q1 + qo, idesc, kb > t.kb0 || k > 0);
                 mma_f16<PAIR>(dsmall, p1 + po, q0 + qo, idesc, true);
               }
               mma_f16<PAIR>(d, p0 + po, q0 + qo, idesc, kb > kb0 || k > 0);
@@ -902,7 +966,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
       const int i = t.i0 + 32 * w, jh = t.j0 + h * half;
       Out out;
       ns_out<SPLIT>(a, t, &out);
-      const int chunks = SPLIT ? (t.kblocks + kChunk - 1) / kChunk : 1;
+      const int chunks = SPLIT ? (t.kb1 - t.kb0 + kChunk - 1) / kChunk : 1;
       __align__(16) float sum[SPLIT ? 2 : 1][32];
       bool ok = true;
       for (int ch = 0; ch < chunks; ++ch, ++sums) {
@@ -942,12 +1006,17 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
         __syncwarp();
         asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
         if (lane == 0) arrive_leader<PAIR>(&sm_empty[tile & 1]);
+        if (PAIR || t.ks == 1 || ns_join(a, t, w, h, sum[0], &joined)) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
-          if (q * 32 < half) ns_emit<SPLIT, T>(a, t, out, i, jh + q * 32, turn, sum[q]);
+          for (int q = 0; q < 2; ++q)
+            if (q * 32 < half) ns_emit<SPLIT, T>(a, t, out, i, jh + q * 32, turn, sum[q]);
+        } else {
+          continue;
+        }
       } else {
         const int buf = (sums - 1) & 1;
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        bool mine = true;
         for (int c0 = 0; c0 < half; c0 += 32) {
           tmem_load32(tmem + buf * 256 + h * half + c0 + lanes, sum[0]);
           if (c0 + 32 >= half) {
@@ -955,8 +1024,10 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             if (lane == 0) arrive_leader<PAIR>(&tm_empty[buf]);
           }
-          ns_emit<SPLIT, T>(a, t, out, i, jh + c0, turn, sum[0]);
+          mine = PAIR || t.ks == 1 || ns_join(a, t, w, h, sum[0], &joined);
+          if (mine) ns_emit<SPLIT, T>(a, t, out, i, jh + c0, turn, sum[0]);
         }
+        if (!mine) continue;
       }
       // other blocks read these values through TMA: order them before the count
       asm volatile("fence.proxy.async;\n" ::: "memory");
@@ -1016,7 +1087,7 @@ static bool half_map(CUtensorMap* map, __half* p, int batch, int rows, int cols,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static constexpr size_t kNsHead = sizeof(double) * kMats * kNormBlocks + 4 * (3 * kMats + 1);
+static constexpr size_t kNsHead = sizeof(double) * kMats * kNormBlocks + 4 * (3 * kMats + 1 + 2 * kSplitTiles);
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static int pitch64(int n) { return (n + 63) / 64 * 64; }
@@ -1098,29 +1169,32 @@ static int tile_count(const NsGroup& g, bool sym, int bm, int bn) {
              : ((g.rows + bm - 1) / bm) * ((g.cols + bn - 1) / bn);
 }
 
-// Microseconds of 64 K columns of a tile on one multiprocessor, by its columns
-// (64, 128, 256) and with both blocks of a pair on one tile.  The products
-// themselves take a third to a half of it: the operands come out of the second
-// level cache at about 65 GB/s a multiprocessor, so what counts is bytes a
-// tile.  Split tiles hold their sums in registers and two accumulators, which
-// leaves room for 128 columns.
-static const double kTileUs[2][2][3] = {{{0.41, 0.50, 0.69}, {9.9, 9.9, 0.47}},
-                                        {{0.62, 0.80, 9.9}, {9.9, 0.70, 9.9}}};
-static const int kTileCols[3] = {64, 128, 256};
+// Time of a tile on one multiprocessor in microseconds: us for each 64 columns
+// of K, tail for the part of the epilogue that nothing hides.  Tile columns 64,
+// 128, 256, and 256 with both blocks of a pair on one tile.  Measured on
+// 4096 x 8192, 12 x 768 x 768 and 2048 x 2048 (bfloat16) and 2304 x 768
+// (float32).  The products themselves take a third to a half of it: copying a
+// tile's operands in and reading them out of shared memory take the rest, so
+// what counts is bytes a tile.  float32 tiles hold their sums in registers and
+// two accumulators, which leaves room for 128 columns; a pair gained nothing
+// there (2048 x 2048: 794 against 781 us).
+struct TileTime { int bn; bool pair; double us, tail; };
+static const TileTime kTimes[2][4] = {
+    {{64, false, 0.41, 3.0}, {128, false, 0.50, 6.0}, {256, false, 0.69, 12.0}, {256, true, 0.47, 15.0}},
+    {{64, false, 0.95, 3.5}, {128, false, 1.03, 6.5}, {0, false, 0, 0}, {0, true, 0, 0}}};
 
-// Tile columns with the least time: waves of tiles, one wave more in effect for
-// the epilogue that nothing hides.
+// Tile columns with the least time, and that time: waves of tiles times a
+// tile's.  kb: 64-column blocks of K, over both products where sym.
 static double pick_bn(const NsGroup& g, bool sym, bool split, bool pair, int units, int* bn) {
   double least = 1e300;
-  for (int i = 0; i < 3; ++i) {
-    const double us = kTileUs[split][pair][i];
-    if (us > 9) continue;
-    const long long tiles =
-        (long long)g.batch * tile_count(g, sym, pair ? 2 * BM : BM, kTileCols[i]);
-    const double c = (double)((tiles + units - 1) / units) * us;
-    if (c < least) {
-      least = c;
-      *bn = kTileCols[i];
+  const int kb = ((sym ? g.l + g.s : g.s) + BK - 1) / BK;
+  for (const TileTime& c : kTimes[split]) {
+    if (c.bn == 0 || c.pair != pair) continue;
+    const long long tiles = (long long)g.batch * tile_count(g, sym, pair ? 2 * BM : BM, c.bn);
+    const double t = (double)((tiles + units - 1) / units) * kb * c.us + (sym ? 2 : 1) * c.tail;
+    if (t < least) {
+      least = t;
+      *bn = c.bn;
     }
   }
   return least;
@@ -1129,6 +1203,7 @@ static double pick_bn(const NsGroup& g, bool sym, bool split, bool pair, int uni
 size_t ns_ws_bytes(const fa_matrix* m, int count, int dtype) {
   size_t most = 0;
   Batch b;
+  const size_t parts = sizeof(float) * kPart * kSplitUnits;
   for (int i = 0; i < count; i += take_batch(m, i, count, &b)) {
     take_batch(m, i, count, &b);
     size_t sum = 0;
@@ -1139,7 +1214,7 @@ size_t ns_ws_bytes(const fa_matrix* m, int count, int dtype) {
     }
     most = std::max(most, sum);
   }
-  return up256(kNsHead) + most;
+  return up256(kNsHead) + parts + most;
 }
 
 // Everything about a call that can be refused before the device is touched.
@@ -1186,9 +1261,54 @@ static bool plan_steps(NsStep* k, const double* coef, int steps) {
   return true;
 }
 
+// Tile shapes of a launch: single blocks or pairs for all of it, the faster by
+// estimate.  Where the symmetric products have so few tiles that half of the
+// multiprocessors would idle, their tiles take 64 columns and K is split as
+// well, at most one part a multiprocessor and at least six blocks a part
+// (joining the parts costs about 4 us: 64 x 5000 bfloat16 236 -> 138 us, but
+// 512 x 512 with parts of three blocks 153 -> 169 us).
+static void plan_tiles(NsArgs& a, bool split, int sms, int pairs) {
+  constexpr int kLeast = 6;
+  int few = 0;
+  for (int i = 0; i < a.groups; ++i)
+    few += a.g[i].batch * std::min(1 << 12, sym_tiles(a.g[i].s, BM, 64));
+  const int units = std::min(sms, kSplitUnits);
+  a.ks = few * 2 <= units ? std::min(units / few, kMaxParts) : 1;
+  bool parts = false;
+  for (int i = 0; i < a.groups; ++i)
+    for (int p = 0; p < 2; ++p) {
+      const int kb = ((p == 0 ? a.g[i].l : a.g[i].s) + BK - 1) / BK;
+      a.g[i].ks[p] = std::max(1, std::min(a.ks, kb / kLeast));
+      parts |= a.g[i].ks[p] > 1;
+    }
+  int bn[2][kGroups][2];
+  double time[2] = {0, 0};
+  for (int pair = 0; pair < (split ? 1 : 2); ++pair)
+    for (int g = 0; g < a.groups; ++g)
+      for (int sym = 0; sym < 2; ++sym)
+        time[pair] += pick_bn(a.g[g], sym, split, pair, pair ? std::max(pairs, 1) : sms,
+                              &bn[pair][g][sym]);
+  a.pair = !split && !parts && pairs > 0 && time[1] < time[0];
+  const int bm = a.pair ? 2 * BM : BM;
+  a.tiles[0] = a.tiles[1] = a.tiles[2] = 0;
+  int slot = 0;
+  for (int i = 0; i < a.groups; ++i) {
+    NsGroup& g = a.g[i];
+    const bool in_parts = g.ks[0] > 1 || g.ks[1] > 1;
+    g.bn_app = bn[a.pair][i][0];
+    g.bn_sym = in_parts ? 64 : bn[a.pair][i][1];
+    g.tiles_sym = tile_count(g, true, bm, g.bn_sym);
+    g.tiles_app = tile_count(g, false, bm, g.bn_app);
+    g.slot = slot;
+    if (in_parts) slot += g.batch * g.tiles_sym;
+    for (int p = 0; p < 2; ++p) a.tiles[p] += g.batch * g.tiles_sym * g.ks[p];
+    a.tiles[2] += g.batch * g.tiles_app;
+  }
+}
+
 // Pairs of blocks that are resident together, at most one block on a
 // multiprocessor; asked once for each device.
-template <bool SPLIT, typename T>
+template <typename T>
 static int pairs_resident(int device) {
   constexpr int MAXD = 64;
   static std::atomic<int> known[MAXD];
@@ -1201,14 +1321,14 @@ static int pairs_resident(int device) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)(sm_count(device) / 2 * 2));
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Stage<SPLIT, true>::kSmem;
+  cfg.dynamicSmemBytes = Stage<false, true>::kSmem;
   cfg.attrs = at;
   cfg.numAttrs = 1;
   int n = 0;
-  if (cudaFuncSetAttribute(ns_product_kernel<SPLIT, true, T>,
+  if (cudaFuncSetAttribute(ns_product_kernel<false, true, T>,
                            cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           Stage<SPLIT, true>::kSmem) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, ns_product_kernel<SPLIT, true, T>, &cfg) != cudaSuccess) {
+                           Stage<false, true>::kSmem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, ns_product_kernel<false, true, T>, &cfg) != cudaSuccess) {
     cudaGetLastError();
     n = 0;
   }
@@ -1229,7 +1349,7 @@ static int ns_products(const NsArgs& a, int units, cudaStream_t st) {
   at[1].id = cudaLaunchAttributeClusterDimension;
   at[1].val.clusterDim.x = 2;
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)std::min(units, std::max(a.tiles_sym, a.tiles_app)) *
+  cfg.gridDim = dim3((unsigned)std::min(units, std::max(a.tiles[0], std::max(a.tiles[1], a.tiles[2]))) *
                      (PAIR ? 2u : 1u));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
@@ -1255,31 +1375,14 @@ static int ns_run(NsArgs& a, int device, cudaStream_t st) {
       1, std::min<long long>((most + 4095) / 4096, std::max(1, sms * 8 / a.mats)));
   ns_pack_kernel<T><<<dim3(pb, a.mats), 256, 0, st>>>(a, nb);
   FAB_LAUNCH_CHECK();
-  // tile shapes: single blocks or pairs for the whole launch, the faster by estimate
-  const int pairs = pairs_resident<SPLIT, T>(device);
-  int bn[2][kGroups][2];
-  double cost[2] = {0, 0};
-  for (int pair = 0; pair < 2; ++pair)
-    for (int g = 0; g < a.groups; ++g)
-      for (int sym = 0; sym < 2; ++sym) {
-        const NsGroup& gr = a.g[g];
-        const double c = pick_bn(gr, sym, SPLIT, pair, pair ? std::max(pairs, 1) : sms,
-                                 &bn[pair][g][sym]);
-        cost[pair] += c * (sym ? gr.l + gr.s : gr.s);  // K of A and A^2, of B X
-      }
-  const bool pair = pairs > 0 && cost[1] < cost[0];
-  a.tiles_sym = a.tiles_app = 0;
-  for (int i = 0; i < a.groups; ++i) {
-    NsGroup& g = a.g[i];
-    g.bn_app = bn[pair][i][0];
-    g.bn_sym = bn[pair][i][1];
-    g.tiles_sym = tile_count(g, true, pair ? 2 * BM : BM, g.bn_sym);
-    g.tiles_app = tile_count(g, false, pair ? 2 * BM : BM, g.bn_app);
-    a.tiles_sym += g.batch * g.tiles_sym;
-    a.tiles_app += g.batch * g.tiles_app;
+  if constexpr (SPLIT) {
+    plan_tiles(a, SPLIT, sms, 0);
+  } else {
+    const int pairs = pairs_resident<T>(device);
+    plan_tiles(a, SPLIT, sms, pairs);
+    if (a.pair) return ns_products<SPLIT, true, T>(a, pairs, st);
   }
-  return pair ? ns_products<SPLIT, true, T>(a, pairs, st)
-              : ns_products<SPLIT, false, T>(a, sms, st);
+  return ns_products<SPLIT, false, T>(a, sms, st);
 }
 
 int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int steps,
@@ -1301,10 +1404,12 @@ int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int
   a.part = reinterpret_cast<double*>(ws);
   a.done = reinterpret_cast<unsigned*>(a.part + kMats * kNormBlocks);
   a.failed = a.done + 3 * kMats;
+  a.joins = a.failed + 1;
+  a.parts = reinterpret_cast<float*>(static_cast<char*>(ws) + up256(kNsHead));
   Batch bt;
   for (int i0 = 0; i0 < count; i0 += bt.n) {
     take_batch(mats, i0, count, &bt);
-    size_t off = up256(kNsHead);
+    size_t off = up256(kNsHead) + sizeof(float) * kPart * kSplitUnits;
     a.groups = bt.groups;
     a.mats = bt.n;
     for (int gi = 0; gi < bt.groups; ++gi) {
