@@ -597,9 +597,9 @@ __device__ __forceinline__ int turn_unit(int r, int q) { return r * 8 + (q ^ (r 
 
 // The last step's output: rows i + 4 it, four columns from j, as the result or
 // into the weight.
-template <typename T>
+template <typename T, int NB>
 __device__ __forceinline__ void ns_result(const NsArgs& a, const Tile& t, const Out& o, int i,
-                                          int j, int left, const float4 (&v)[8]) {
+                                          int j, int left, const float4 (&v)[NB]) {
   const NsMat& m = a.m[t.mat];
   T* w = reinterpret_cast<T*>(m.dst) + i * m.dst_row + j;
   const float step = m.step;
@@ -607,14 +607,14 @@ __device__ __forceinline__ void ns_result(const NsArgs& a, const Tile& t, const 
   if (m.vec_dst) {  // whole vectors of four
     typedef typename RawOf<4 * sizeof(T)>::type V4;
     if (j >= o.cols) return;
-    V4 old[8];
+    V4 old[NB];
     if (update) {
 #pragma unroll
-      for (int it = 0; it < 8; ++it)
+      for (int it = 0; it < NB; ++it)
         if (4 * it < left) old[it] = *reinterpret_cast<const V4*>(w + 4 * it * m.dst_row);
     }
 #pragma unroll
-    for (int it = 0; it < 8; ++it) {
+    for (int it = 0; it < NB; ++it) {
       if (4 * it >= left) break;
       const float vs[4] = {v[it].x, v[it].y, v[it].z, v[it].w};
       V4 u;
@@ -627,7 +627,7 @@ __device__ __forceinline__ void ns_result(const NsArgs& a, const Tile& t, const 
     }
   } else {
 #pragma unroll
-    for (int it = 0; it < 8; ++it) {
+    for (int it = 0; it < NB; ++it) {
       if (4 * it >= left) break;
       T* x = w + 4 * it * m.dst_row;
       const float vs[4] = {v[it].x, v[it].y, v[it].z, v[it].w};
@@ -649,25 +649,11 @@ __device__ __forceinline__ void ns_emit(const NsArgs& a, const Tile& t, const Ou
   // warp-uniform: outside the matrix, or above the diagonal blocks
   if (i0 >= o.rows || j0 >= o.cols || (sym && j0 / BM > t.i0 / BM)) return;
   const int lane = threadIdx.x & 31, r0 = lane >> 3, q4 = lane & 7, j = j0 + 4 * q4;
-  const long long at0 = (long long)(i0 + r0) * o.pitch + j, four = 4ll * o.pitch;
-  const int left = o.rows - i0 - r0;  // rows 4 it + r0 are inside for 4 it < left
   // Each loop below is a batch of independent accesses: a scheduler has two of
-  // these warps, so latency is hidden inside a warp or not at all.
-  uint2 hi[8], lo[8];
-#pragma unroll
-  for (int it = 0; it < 8; ++it) hi[it] = lo[it] = make_uint2(0u, 0u);
-  if (o.q0) {
-    const __half* p = o.q0 + at0;
-#pragma unroll
-    for (int it = 0; it < 8; ++it, p += four)
-      if (4 * it < left) hi[it] = __ldcg(reinterpret_cast<const uint2*>(p));
-  }
-  if (o.q1) {
-    const __half* p = o.q1 + at0;
-#pragma unroll
-    for (int it = 0; it < 8; ++it, p += four)
-      if (4 * it < left) lo[it] = __ldcg(reinterpret_cast<const uint2*>(p));
-  }
+  // these warps, so latency is hidden inside a warp or not at all.  Split tiles
+  // hold another 32 sums in registers meanwhile: half the rows at a time.
+  constexpr int NB = SPLIT ? 4 : 8;
+  const long long four = 4ll * o.pitch;
   const float row_d = o.di && i0 + lane < o.rows ? __ldcg(o.di + i0 + lane) : 0.f;
   float4 cd = make_float4(0.f, 0.f, 0.f, 0.f);
   if (o.dj) cd = __ldcg(reinterpret_cast<const float4*>(o.dj + j));  // inside the pitch of 64
@@ -675,6 +661,12 @@ __device__ __forceinline__ void ns_emit(const NsArgs& a, const Tile& t, const Ou
   for (int q = 0; q < 8; ++q)
     turn[turn_unit(lane, q)] =
         make_float4(sums[4 * q], sums[4 * q + 1], sums[4 * q + 2], sums[4 * q + 3]);
+  const bool mirror = sym && j0 / BM < t.i0 / BM;
+  const float fd_row = o.f * row_d;
+  cd.x = fmaf(o.f, cd.x, o.e);
+  cd.y = fmaf(o.f, cd.y, o.e);
+  cd.z = fmaf(o.f, cd.z, o.e);
+  cd.w = fmaf(o.f, cd.w, o.e);
   __syncwarp();
   if (sym && i0 == j0) {  // the diagonal stays in float32, and zero in its place
     if (lane < o.rows - i0) {
@@ -684,71 +676,91 @@ __device__ __forceinline__ void ns_emit(const NsArgs& a, const Tile& t, const Ou
     }
     __syncwarp();
   }
-  float4 v[8];
+#pragma unroll 1
+  for (int rb = r0; rb < 32; rb += 4 * NB) {
+    const long long at0 = (long long)(i0 + rb) * o.pitch + j;
+    const int left = o.rows - i0 - rb;  // rows rb + 4 it are inside for 4 it < left
+    uint2 hi[NB], lo[NB];
 #pragma unroll
-  for (int it = 0; it < 8; ++it) v[it] = turn[turn_unit(4 * it + r0, q4)];
-  cd.x = fmaf(o.f, cd.x, o.e);
-  cd.y = fmaf(o.f, cd.y, o.e);
-  cd.z = fmaf(o.f, cd.z, o.e);
-  cd.w = fmaf(o.f, cd.w, o.e);
-  if (o.q0) {
-    const float fd_row = o.f * row_d;
+    for (int it = 0; it < NB; ++it) hi[it] = lo[it] = make_uint2(0u, 0u);
+    if (o.q0) {
+      const __half* p = o.q0 + at0;
 #pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      const float fd = __shfl_sync(0xffffffffu, fd_row, 4 * it + r0);
-      float4 x = half4_float(hi[it]);
-      if (SPLIT || !sym) {
-        const float4 l = half4_float(lo[it]);
-        x.x += l.x;
-        x.y += l.y;
-        x.z += l.z;
-        x.w += l.w;
+      for (int it = 0; it < NB; ++it, p += four)
+        if (4 * it < left) hi[it] = __ldcg(reinterpret_cast<const uint2*>(p));
+    }
+    if (o.q1) {
+      const __half* p = o.q1 + at0;
+#pragma unroll
+      for (int it = 0; it < NB; ++it, p += four)
+        if (4 * it < left) lo[it] = __ldcg(reinterpret_cast<const uint2*>(p));
+    }
+    float4 v[NB];
+#pragma unroll
+    for (int it = 0; it < NB; ++it) v[it] = turn[turn_unit(rb + 4 * it, q4)];
+    if (o.q0) {
+#pragma unroll
+      for (int it = 0; it < NB; ++it) {
+        const float fd = __shfl_sync(0xffffffffu, fd_row, rb + 4 * it);
+        float4 x = half4_float(hi[it]);
+        if (SPLIT || !sym) {
+          const float4 l = half4_float(lo[it]);
+          x.x += l.x;
+          x.y += l.y;
+          x.z += l.z;
+          x.w += l.w;
+        }
+        v[it].x = fmaf(x.x, cd.x + fd, v[it].x * o.p);
+        v[it].y = fmaf(x.y, cd.y + fd, v[it].y * o.p);
+        v[it].z = fmaf(x.z, cd.z + fd, v[it].z * o.p);
+        v[it].w = fmaf(x.w, cd.w + fd, v[it].w * o.p);
       }
-      v[it].x = fmaf(x.x, cd.x + fd, v[it].x * o.p);
-      v[it].y = fmaf(x.y, cd.y + fd, v[it].y * o.p);
-      v[it].z = fmaf(x.z, cd.z + fd, v[it].z * o.p);
-      v[it].w = fmaf(x.w, cd.w + fd, v[it].w * o.p);
-    }
-  } else {
+    } else {
 #pragma unroll
-    for (int it = 0; it < 8; ++it) {
-      v[it].x *= o.p;
-      v[it].y *= o.p;
-      v[it].z *= o.p;
-      v[it].w *= o.p;
-    }
-  }
-  const bool mirror = sym && j0 / BM < t.i0 / BM;
-  if (mirror) {
-#pragma unroll
-    for (int it = 0; it < 8; ++it) turn[turn_unit(4 * it + r0, q4)] = v[it];
-  }
-  if (o.o0) {
-    __half *p0 = o.o0 + at0, *p1 = o.o1 + at0;
-#pragma unroll
-    for (int it = 0; it < 8; ++it, p0 += four, p1 += four) {
-      if (4 * it < left) {
-        if (SPLIT || !sym) put_half4<true>(v[it], p0, p1);
-        else put_half4<false>(v[it], p0, nullptr);
+      for (int it = 0; it < NB; ++it) {
+        v[it].x *= o.p;
+        v[it].y *= o.p;
+        v[it].z *= o.p;
+        v[it].w *= o.p;
       }
     }
-  } else {
-    ns_result<T>(a, t, o, i0 + r0, j, left, v);
+    if (mirror) {
+#pragma unroll
+      for (int it = 0; it < NB; ++it) turn[turn_unit(rb + 4 * it, q4)] = v[it];
+    }
+    if (o.o0) {
+      __half *p0 = o.o0 + at0, *p1 = o.o1 + at0;
+#pragma unroll
+      for (int it = 0; it < NB; ++it, p0 += four, p1 += four) {
+        if (4 * it < left) {
+          if (SPLIT || !sym) put_half4<true>(v[it], p0, p1);
+          else put_half4<false>(v[it], p0, nullptr);
+        }
+      }
+    } else {
+      ns_result<T, NB>(a, t, o, i0 + rb, j, left, v);
+    }
   }
   if (mirror) {  // the same values above the diagonal: four rows to a lane
     __syncwarp();
     const float* f = reinterpret_cast<const float*>(turn) + r0;
-    const long long to = (long long)(j0 + r0) * o.pitch + i0 + 4 * q4;
-    __half *p0 = o.o0 + to, *p1 = o.o1 + to;
+#pragma unroll 1
+    for (int cb = 0; cb < 8; cb += NB) {
+      // column 4 (cb + it) + r0: unit cb + it, place r0
+      const long long to = (long long)(j0 + 4 * cb + r0) * o.pitch + i0 + 4 * q4;
+      __half *p0 = o.o0 + to, *p1 = o.o1 + to;
+      float4 v[NB];
 #pragma unroll
-    for (int it = 0; it < 8; ++it)  // column 4 it + r0: unit it, place r0
-      v[it] = make_float4(f[4 * turn_unit(4 * q4, it)], f[4 * turn_unit(4 * q4 + 1, it)],
-                          f[4 * turn_unit(4 * q4 + 2, it)], f[4 * turn_unit(4 * q4 + 3, it)]);
+      for (int it = 0; it < NB; ++it)
+        v[it] = make_float4(
+            f[4 * turn_unit(4 * q4, cb + it)], f[4 * turn_unit(4 * q4 + 1, cb + it)],
+            f[4 * turn_unit(4 * q4 + 2, cb + it)], f[4 * turn_unit(4 * q4 + 3, cb + it)]);
 #pragma unroll
-    for (int it = 0; it < 8; ++it, p0 += four, p1 += four) {
-      if (j0 + 4 * it + r0 < o.cols) {
-        if (SPLIT) put_half4<true>(v[it], p0, p1);
-        else put_half4<false>(v[it], p0, nullptr);
+      for (int it = 0; it < NB; ++it, p0 += four, p1 += four) {
+        if (j0 + 4 * (cb + it) + r0 < o.cols) {
+          if (SPLIT) put_half4<true>(v[it], p0, p1);
+          else put_half4<false>(v[it], p0, nullptr);
+        }
       }
     }
   }
