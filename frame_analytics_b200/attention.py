@@ -222,5 +222,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor]
     if out is None:
         out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),
                torch.empty(k.shape, dtype=k.dtype, device=k.device))
-    _forward(q, k, out[0], out[1], *rest)
+        _forward(q, k, out[0], out[1], *rest)
+    else:
+        _forward(q, k, out[0], out[1], *rest)
+        torch.autograd.graph.increment_version(out)
     return out[0], out[1]

@@ -213,6 +213,8 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     mats = b"".join([_MATRIX(*row) for row in rows])
     _run(backend.lib().fa_b200_muon_step, mats, len(rows), first, coef, steps, momentum,
          int(nesterov), 1.0 - lr * weight_decay)
+    # autograd notices weights that a graph still needs, as for torch's own updates
+    torch.autograd.graph.increment_version(weights + momenta)
 
 
 class Muon(torch.optim.Optimizer):

@@ -507,3 +507,83 @@ def test_muon_orders_of_memory():
             fa.muon_step([w1], [gr.contiguous(memory_format=gf)], [m1], lr=0.1)
             assert rel(w1, want) < 2e-6
             assert torch.equal(m1, gr)
+
+
+# --------------------------------------------------------------------------- #
+# the product kernel's other shapes: K in parts, pairs of blocks, many shapes
+# --------------------------------------------------------------------------- #
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(64, 5000), (5000, 64), (100, 3501), (2, 130, 2050),
+                                   (2050, 190), (3, 20, 1999)])
+def test_orthogonalize_long_and_narrow(shape, dtype):
+    """Few tiles: K is split over blocks and joined."""
+    x = gradient(shape, "noise", seed=11).to(dtype)
+    y = fa.orthogonalize(x)
+    assert rel(y, plain_ns(x)) < NS_TOL[dtype]
+    assert torch.equal(fa.orthogonalize(x), y)  # joined in one order
+
+
+@pytest.mark.parametrize("shape", [(20, 1030, 1100), (5, 2100, 1500), (4100, 4200)])
+def test_orthogonalize_large(shape):
+    """Many tiles: pairs of blocks share them; sizes that leave a block of the
+    last pair without rows."""
+    x = gradient(shape, "spiky", seed=12).to(torch.bfloat16)
+    y = fa.orthogonalize(x)
+    want = plain_ns(x)
+    worst = max(rel(a, b) for a, b in zip(y.view(-1, *shape[-2:]), want.view(-1, *shape[-2:])))
+    assert worst < NS_TOL[torch.bfloat16]
+    assert torch.equal(fa.orthogonalize(x), y)
+
+
+def test_orthogonalize_float32_large():
+    x = gradient((2, 1100, 1290), "spiky", seed=13)
+    assert max(rel(a, b) for a, b in zip(fa.orthogonalize(x), plain_ns(x))) < NS_TOL[torch.float32]
+
+
+def test_muon_step_with_more_shapes_than_a_launch_holds():
+    g = torch.Generator(device="cuda").manual_seed(14)
+    shapes = [(8 + 7 * i, 90 - 5 * i) for i in range(13)] * 2 + [(33, 20)] * 120
+    W = [torch.randn(s, generator=g, device="cuda") for s in shapes]
+    G = [torch.randn(s, generator=g, device="cuda") for s in shapes]
+    M = [torch.randn(s, generator=g, device="cuda") for s in shapes]
+    want = [plain_muon(w, gr, m, 0.1, 0.95, True, 0.0, "none") for w, gr, m in zip(W, G, M)]
+    fa.muon_step(W, G, M, lr=0.1, scale="none")
+    for w, m, (ww, wm) in zip(W, M, want):
+        assert rel(w, ww) < 2e-6 and rel(m, wm) < 2.0 ** -22
+
+
+def test_orthogonalize_on_two_streams_at_once():
+    xs = [gradient((3, 300, 420), "noise", seed=20 + i).to(torch.bfloat16) for i in range(2)]
+    want = [fa.orthogonalize(x) for x in xs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(fa.orthogonalize(xs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, want[i]) for y in got[i])
+
+
+def test_in_place_outputs_count_as_modified():
+    w = torch.randn(8, 8, device="cuda", requires_grad=True)
+    loss = (w * w).sum()
+    with torch.no_grad():
+        fa.muon_step([w], [torch.randn_like(w)], [torch.zeros_like(w)], lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_training_example_learns():
+    import sys
+
+    from conftest import REPO
+    sys.path.insert(0, str(REPO / "examples"))
+    import train_restoration
+
+    losses = train_restoration.train(steps=40, size=64, frames=4)
+    assert all(math.isfinite(v) for v in losses)
+    assert sum(losses[-5:]) < 0.8 * sum(losses[:5]), (losses[:5], losses[-5:])
