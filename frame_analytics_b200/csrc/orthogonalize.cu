@@ -870,7 +870,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
         const unsigned want =
             (unsigned)rounds * (t.phase == 0 ? g.tiles_app : g.tiles_sym) * (PAIR ? 2u : 1u);
         if (!wait_flag(a.done + from * kMats + t.mat, want, a)) break;
-        asm volatile("fence.proxy.async;\n" ::: "memory");
+        asm volatile("fence.proxy.async.global;\n" ::: "memory");
         const int xi = MAP_X0 + (t.step & 1);
         const int mp = t.phase == 0 ? xi : t.phase == 1 ? MAP_A : g.tall ? xi : MAP_B;
         const int mq = t.phase == 0 ? xi : t.phase == 1 ? MAP_A : g.tall ? MAP_B : xi;
@@ -1003,8 +1003,9 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
       if (!ok) dead = 1;
       asm volatile("bar.sync 1, 256;\n" ::: "memory");
       if (dead) break;
-      // the producer waited for what the products read; order this thread's loads too
-      ld_acquire(a.done + (t.phase == 0 ? 2 : t.phase - 1) * kMats + t.mat);
+      // What this tile's epilogue loads was finished before the producer's wait
+      // for it, and the chain of barriers from there to here orders it; the loads
+      // bypass the first-level cache, which may hold an older step's lines.
       if constexpr (SPLIT) {
         // the small products of the whole tile are complete with its last chunk
 #pragma unroll
@@ -1041,11 +1042,11 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
         }
         if (!mine) continue;
       }
-      // other blocks read these values through TMA: order them before the count
-      asm volatile("fence.proxy.async;\n" ::: "memory");
+      // other blocks read these values through TMA: order them before the count,
+      // whose release covers the whole block's stores after the barrier
+      asm volatile("fence.proxy.async.global;\n" ::: "memory");
       asm volatile("bar.sync 1, 256;\n" ::: "memory");
       if (threadIdx.x == 128) {
-        __threadfence();
         asm volatile("red.release.gpu.global.add.u32 [%0], 1;\n" ::"l"(a.done + t.phase * kMats +
                                                                        t.mat)
                      : "memory");

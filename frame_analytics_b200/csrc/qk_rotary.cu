@@ -254,7 +254,11 @@ __global__ void __launch_bounds__(128) qk_dw_sum_kernel(const float* part, int c
 // and serve a lane's chunk in `hpi` heads.
 //
 // Both kernels are bound by HBM: the work per component is about 10 (backward:
-// 25) float operations for 4 to 12 bytes.
+// 25) float operations for 4 to 12 bytes.  Measured on one B200: forward, 1 x
+// 32761 tokens of 32 + 8 heads of 128, float16: 132 us, 5.1 TB/s of the bytes
+// it cannot do without (0.79 of the measured copy rate); backward, 2 x 8160
+// tokens of 16 + 16 heads of 64, bfloat16: 62 us, 3.2 TB/s (0.50), held back by
+// load latency at the 16 warps a multiprocessor that its registers leave.
 // ---------------------------------------------------------------------------
 // V components as they lie in memory: rows in flight wait unconverted.
 template <typename T, int V> using Raw = typename RawOf<sizeof(T) * V>::type;
@@ -500,8 +504,11 @@ __device__ __forceinline__ void qk_dw_finish(const QkArgs& a, const float* part,
 // A block keeps one item (one side, `hpi` heads; one head when the weights are
 // per head) and walks over tokens, so that each lane sums the weight gradient
 // of its chunks in registers; the block's sums go to `part`, and the last block
-// adds the blocks up.
-template <typename T, int V, int G, int U>
+// adds the blocks up.  One head vector of a lane in flight: a second one costs
+// the registers of a load batch and measured slower (62 against 68 us on
+// 2 x 8160 tokens of 16 + 16 heads of 64, bfloat16), as did three blocks a
+// multiprocessor.
+template <typename T, int V, int G>
 __global__ void __launch_bounds__(256, 2) qk_bwd_kernel(const __grid_constant__ QkArgs a, int hpi,
                                                      int items_q, int items, unsigned* counter,
                                                      float* part, void* dqw, void* dkw) {
@@ -527,47 +534,39 @@ __global__ void __launch_bounds__(256, 2) qk_bwd_kernel(const __grid_constant__ 
     const T* x = reinterpret_cast<const T*>(s.x) + b * s.xb + l * s.xl;
     const T* g = reinterpret_cast<const T*>(s.g) + b * s.gb + l * s.gl;
     T* dx = reinterpret_cast<T*>(s.out) + b * s.ob + l * s.ol;
-    for (int r = 0; r < hpi; r += U) {
-      Raw<T, V> ra[U], rb[U], sa[U], sb[U];
+    for (int r = 0; r < hpi; ++r) {
+      const int h = h0 + r;
+      const bool live = busy && h < h1;
+      const Raw<T, V> ra = qk_raw<T, V>(x + h * s.xh + q.a0, live);
+      const Raw<T, V> rb = qk_raw<T, V>(x + h * s.xh + q.b0, live);
+      const Raw<T, V> sa = qk_raw<T, V>(g + h * s.gh + q.a0, live);
+      const Raw<T, V> sb = qk_raw<T, V>(g + h * s.gh + q.b0, live);
+      float xa[V], xb[V], ga[V], gb[V];
+      qk_wide<T, V>(ra, xa);
+      qk_wide<T, V>(rb, xb);
+      qk_wide<T, V>(sa, ga);
+      qk_wide<T, V>(sb, gb);
+      qk_turn<V>(a, q, ga, gb, c, sn, -1.f);
+      float ss = 0.f, dot = 0.f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int h = h0 + r + u;
-        const bool live = busy && h < h1;
-        ra[u] = qk_raw<T, V>(x + h * s.xh + q.a0, live);
-        rb[u] = qk_raw<T, V>(x + h * s.xh + q.b0, live);
-        sa[u] = qk_raw<T, V>(g + h * s.gh + q.a0, live);
-        sb[u] = qk_raw<T, V>(g + h * s.gh + q.b0, live);
+      for (int i = 0; i < V; ++i) {
+        ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
+        dot = fmaf(xa[i] * wa[i], ga[i], fmaf(xb[i] * wb[i], gb[i], dot));
       }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int h = h0 + r + u;
-        float xa[V], xb[V], ga[V], gb[V];
-        qk_wide<T, V>(ra[u], xa);
-        qk_wide<T, V>(rb[u], xb);
-        qk_wide<T, V>(sa[u], ga);
-        qk_wide<T, V>(sb[u], gb);
-        qk_turn<V>(a, q, ga, gb, c, sn, -1.f);
-        float ss = 0.f, dot = 0.f;
+      float rs = rsqrtf(fmaf(group_sum<G>(ss), a.inv_d, a.eps));
+      if (p < 0) rs = __int_as_float(0x7fffffff);
+      const float m = group_sum<G>(dot) * rs * a.inv_d;
+      if (live) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          ss = fmaf(xa[i], xa[i], fmaf(xb[i], xb[i], ss));
-          dot = fmaf(xa[i] * wa[i], ga[i], fmaf(xb[i] * wb[i], gb[i], dot));
+          const float ha = xa[i] * rs, hb = xb[i] * rs;
+          da[i] = fmaf(ga[i], ha, da[i]);
+          db[i] = fmaf(gb[i], hb, db[i]);
+          xa[i] = rs * fmaf(-ha, m, wa[i] * ga[i]);
+          xb[i] = rs * fmaf(-hb, m, wb[i] * gb[i]);
         }
-        float rs = rsqrtf(fmaf(group_sum<G>(ss), a.inv_d, a.eps));
-        if (p < 0) rs = __int_as_float(0x7fffffff);
-        const float m = group_sum<G>(dot) * rs * a.inv_d;
-        if (busy && h < h1) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float ha = xa[i] * rs, hb = xb[i] * rs;
-            da[i] = fmaf(ga[i], ha, da[i]);
-            db[i] = fmaf(gb[i], hb, db[i]);
-            xa[i] = rs * fmaf(-ha, m, wa[i] * ga[i]);
-            xb[i] = rs * fmaf(-hb, m, wb[i] * gb[i]);
-          }
-          qk_store<T, V>(dx + h * s.oh + q.a0, xa);
-          qk_store<T, V>(dx + h * s.oh + q.b0, xb);
-        }
+        qk_store<T, V>(dx + h * s.oh + q.a0, xa);
+        qk_store<T, V>(dx + h * s.oh + q.b0, xb);
       }
     }
   }
@@ -669,12 +668,7 @@ static int qk_launch(const QkArgs& a, bool backward, char* ws, void* dqw, void* 
     unsigned* counter = reinterpret_cast<unsigned*>(ws);
     float* part = reinterpret_cast<float*>(ws + FAB_COUNTER_BYTES);
     const unsigned blocks = (unsigned)(rounds * items);
-    if (hpi == 1)
-      qk_bwd_kernel<T, V, G, 1><<<blocks, 256, 0, st>>>(a, hpi, items_q, items, counter, part, dqw,
-                                                       dkw);
-    else
-      qk_bwd_kernel<T, V, G, 2><<<blocks, 256, 0, st>>>(a, hpi, items_q, items, counter, part, dqw,
-                                                       dkw);
+    qk_bwd_kernel<T, V, G><<<blocks, 256, 0, st>>>(a, hpi, items_q, items, counter, part, dqw, dkw);
   }
   FAB_LAUNCH_CHECK();
   return FA_OK;
