@@ -5,6 +5,9 @@ A drop-in for the metric path of frame_analytics: ``psnr``, ``mse``, ``l1``,
 ``ms_ssim``, ``gmsd`` / ``gms``, ``ssimulacra2``, with the same arguments and results,
 computed by hand-written CUDA kernels behind a C ABI (``include/fa_b200.h``).
 
+Around the losses, for networks trained against them: ``qk_norm_rotary``
+(attention operands), ``orthogonalize``, ``muon_step`` and ``Muon`` (weight updates).
+
 >>> import torch, frame_analytics_b200 as fa
 >>> a = torch.randint(0, 256, (8, 3, 1080, 1920), dtype=torch.uint8, device="cuda")
 >>> b = (a.float() + 4 * torch.randn(a.shape, device="cuda")).clamp(0, 255).byte()

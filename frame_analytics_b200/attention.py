@@ -173,7 +173,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor]
     ``R <= D`` components turn, in pairs (i, i + R/2), or (2i, 2i + 1) with
     ``interleaved``.  ``positions``: int32 / int64 (L,) or (B, L) rows of the
     tables, by default 0..L-1; a position outside the tables gives NaN for its
-    token.  Weights: (D,) shared by the heads, or (heads, D); in the operands'
+    token (and then for the weights' gradients).  Weights: (D,) shared by the heads, or (heads, D); in the operands'
     dtype or float32.
 
     Returns contiguous (B, L, Hq, D) and (B, L, Hk, D).  ``out=(q_out, k_out)``

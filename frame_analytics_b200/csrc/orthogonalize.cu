@@ -13,6 +13,14 @@
 // Three launches serve a whole list of matrices: momentum and norms, packing,
 // and one persistent kernel for all products of all steps.
 //
+// Measured on one B200, a call: 4096 x 8192 bfloat16 2.5 ms (0.98 PFLOP/s of
+// the products it cannot do without), 12 x 768 x 768 bfloat16 0.27 ms (0.41),
+// 2304 x 768 float32 0.27 ms (0.085, three times that in products run).  Large
+// matrices are bound by the products (0.45 us for 256 x 256 x 64 on a pair of
+// blocks), middle ones by operand bytes out of the second-level cache and the
+// ends of the phases, small ones by the latency of 15 dependent products (about
+// 4 us each).
+//
 // Number formats.  The products run on the tensor cores with float16 operands
 // and float32 accumulators; float16 has three more bits than bfloat16 at the
 // same rate, and powers of two per step (from a bound on the singular values)
