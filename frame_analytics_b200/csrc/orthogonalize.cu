@@ -18,8 +18,8 @@
 // 2304 x 768 float32 0.27 ms (0.085, three times that in products run).  Large
 // matrices are bound by the products (0.45 us for 256 x 256 x 64 on a pair of
 // blocks), middle ones by operand bytes out of the second-level cache and the
-// ends of the phases, small ones by the latency of 15 dependent products (about
-// 4 us each).
+// ends of the phases, small ones by the latency of 15 dependent products (at
+// least 4 us each; matrices up to 64 x 128 have a kernel of their own).
 //
 // Number formats.  The products run on the tensor cores with float16 operands
 // and float32 accumulators; float16 has three more bits than bfloat16 at the
@@ -110,6 +110,7 @@ struct NsArgs {
   unsigned* failed;                // set when a wait of this call gave up
   double* part;                    // [kMats][kNormBlocks]
   unsigned* err;
+  int small;                       // every matrix fits one block
   int pair;                        // two blocks a tile
   int ks;                          // parts of a tile at most
   float mu, decay;
@@ -1074,6 +1075,154 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
 }
 
 // ---------------------------------------------------------------------------
+// small matrices: one block each, one launch
+// ---------------------------------------------------------------------------
+
+// Up to 64 x 128 (or 128 x 64) a matrix and its products fit one block's shared
+// memory in float32, and the 15 dependent products cost float32 FMAs and block
+// barriers (2.5 us each at 64 x 64) in place of trips through memory:
+// 64 x 64 bfloat16 42 us on the GPU against 77 with the three launches of the tiled
+// kernel, 64 x 128 about 60 against 80.  At twice
+// the longer side the products alone take as long as the tiled kernel.
+constexpr int kSmallS = 64, kSmallL = 128;
+constexpr int kLdX = kSmallL + 4, kLdA = kSmallS + 4;  // 8 rows' vectors in 8 bank groups
+constexpr int kSmallSmem = (int)sizeof(float) * (kSmallS * kLdX + 2 * kSmallS * kLdA);
+
+// acc[u][v] = sum over k < n of P[ty + 16 u][k] P[tx + 16 v][k]
+__device__ __forceinline__ void rows_product(const float* P, int ld, int n, int ty, int tx,
+                                             float (&acc)[4][4]) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) acc[u][v] = 0.f;
+  for (int k = 0; k < n; k += 4) {
+    float4 p[4], q[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      p[u] = *reinterpret_cast<const float4*>(P + (ty + 16 * u) * ld + k);
+      q[u] = *reinterpret_cast<const float4*>(P + (tx + 16 * u) * ld + k);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        acc[u][v] = fmaf(p[u].x, q[v].x, acc[u][v]);
+        acc[u][v] = fmaf(p[u].y, q[v].y, acc[u][v]);
+        acc[u][v] = fmaf(p[u].z, q[v].z, acc[u][v]);
+        acc[u][v] = fmaf(p[u].w, q[v].w, acc[u][v]);
+      }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) ns_small_kernel(const __grid_constant__ NsArgs a) {
+  extern __shared__ char smem_raw[];
+  float* const X = reinterpret_cast<float*>(smem_raw);  // [64][kLdX]: the shorter side in rows
+  float* const A = X + kSmallS * kLdX;
+  float* const B = A + kSmallS * kLdA;
+  __shared__ double sm[32];
+  const NsMat& m = a.m[blockIdx.x];
+  const NsGroup& g = a.g[m.group];
+  const int s = g.s, l = g.l, n = g.rows * g.cols;
+  for (int i = threadIdx.x; i < kSmallS * kLdX; i += 256) X[i] = 0.f;  // beyond s and l too
+  __syncthreads();
+  const T* src = reinterpret_cast<const T*>(m.src);
+  double ss = 0;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int r = i / g.cols, c = i - r * g.cols;
+    float u = Ld<T>::f(src[r * m.src_row + c]);
+    if (m.mom) {
+      const float v = fmaf(a.mu, m.mom[i], u);
+      m.mom[i] = v;
+      u = a.nesterov ? fmaf(a.mu, v, u) : v;
+    }
+    ss += (double)u * u;
+    X[g.tall ? c * kLdX + r : r * kLdX + c] = u;
+  }
+  ss = block_sum(ss, sm);
+  const bool finite = ss <= 1.7e308;
+  const double inv = ss > 0 ? 1.0 / sqrt(ss) : 0.0;
+  int e;
+  const float f = (float)frexp(inv, &e);
+  const float e1 = ldexpf(1.f, e / 2), e2 = ldexpf(1.f, e - e / 2);
+  __syncthreads();
+  for (int i = threadIdx.x; i < s * l; i += 256) {
+    const int r = i / l, at = r * kLdX + (i - r * l);
+    X[at] = finite ? X[at] * e1 * e2 * f : __int_as_float(0x7fffffff);
+  }
+  __syncthreads();
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int s4 = (s + 3) & ~3, l4 = (l + 3) & ~3;
+  for (int st = 0; st < a.steps; ++st) {
+    const NsStep& k = a.k[st];
+    float acc[4][4];
+    rows_product(X, kLdX, l4, ty, tx, acc);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) A[(ty + 16 * u) * kLdA + tx + 16 * v] = acc[u][v];
+    __syncthreads();
+    rows_product(A, kLdA, s4, ty, tx, acc);  // A is symmetric
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int at = (ty + 16 * u) * kLdA + tx + 16 * v;
+        B[at] = fmaf(k.b, A[at], k.c * acc[u][v]);
+      }
+    __syncthreads();
+    // rows ty + 16 u, columns 4 tx + 64 w + [0, 4)
+    float4 y[2][4];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      if (64 * w >= l) break;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        y[w][u] = *reinterpret_cast<const float4*>(X + (ty + 16 * u) * kLdX + 4 * tx + 64 * w);
+        y[w][u].x *= k.a;
+        y[w][u].y *= k.a;
+        y[w][u].z *= k.a;
+        y[w][u].w *= k.a;
+      }
+      for (int q = 0; q < s4; q += 4) {
+        float4 b4[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          b4[u] = *reinterpret_cast<const float4*>(B + (ty + 16 * u) * kLdA + q);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const float4 x = *reinterpret_cast<const float4*>(X + (q + d) * kLdX + 4 * tx + 64 * w);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const float bv = d == 0 ? b4[u].x : d == 1 ? b4[u].y : d == 2 ? b4[u].z : b4[u].w;
+            y[w][u].x = fmaf(bv, x.x, y[w][u].x);
+            y[w][u].y = fmaf(bv, x.y, y[w][u].y);
+            y[w][u].z = fmaf(bv, x.z, y[w][u].z);
+            y[w][u].w = fmaf(bv, x.w, y[w][u].w);
+          }
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      if (64 * w >= l) break;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<float4*>(X + (ty + 16 * u) * kLdX + 4 * tx + 64 * w) = y[w][u];
+    }
+    __syncthreads();
+  }
+  T* dst = reinterpret_cast<T*>(m.dst);
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int r = i / g.cols, c = i - r * g.cols;
+    const float v = X[g.tall ? c * kLdX + r : r * kLdX + c];
+    T* w = dst + r * m.dst_row + c;
+    *w = St<T>::v(m.mom ? fmaf(a.decay, Ld<T>::f(*w), -m.step * v) : v);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
 
@@ -1385,6 +1534,13 @@ template <bool SPLIT, typename T>
 static int ns_run(NsArgs& a, int device, cudaStream_t st) {
   const int sms = sm_count(device);
   long long most = 0;
+  if (a.small) {
+    FAB_TRY(cudaFuncSetAttribute(ns_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kSmallSmem));
+    ns_small_kernel<T><<<a.mats, 256, kSmallSmem, st>>>(a);
+    FAB_LAUNCH_CHECK();
+    return FA_OK;
+  }
   for (int g = 0; g < a.groups; ++g)
     most = std::max<long long>(most, (long long)a.g[g].rows * a.g[g].px);
   const int nb = (int)std::max<long long>(
@@ -1433,12 +1589,16 @@ int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int
     size_t off = up256(kNsHead) + sizeof(float) * kPart * kSplitUnits;
     a.groups = bt.groups;
     a.mats = bt.n;
+    a.small = 1;
+    for (int gi = 0; gi < bt.groups; ++gi)
+      a.small &= std::min(bt.rows[gi], bt.cols[gi]) <= kSmallS &&
+                 std::max(bt.rows[gi], bt.cols[gi]) <= kSmallL;
     for (int gi = 0; gi < bt.groups; ++gi) {
       NsGroup& g = a.g[gi];
       group_shape(&g, bt.rows[gi], bt.cols[gi], bt.count[gi], bt.first[gi]);
       off += group_layout(&g, split, static_cast<char*>(ws) + off);
       if (off > ws_bytes) return FA_E_ARG;
-      for (int h = 0; h < (split ? 2 : 1); ++h) {
+      for (int h = 0; !a.small && h < (split ? 2 : 1); ++h) {
         if (!half_map(&g.map[MAP_X0][h], g.x[0][h], g.batch, g.rows, g.cols, g.px) ||
             !half_map(&g.map[MAP_X1][h], g.x[1][h], g.batch, g.rows, g.cols, g.px) ||
             !half_map(&g.map[MAP_A][h], g.a[h], g.batch, g.s, g.s, g.pa) ||

@@ -83,7 +83,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5,
 
     float16, bfloat16 or float32 in and out; the result is contiguous.  bfloat16
     runs one tensor-core product per matrix product (about 1e-3 relative before
-    the output is rounded); float16 and float32 run three (about 1e-6).
+    the output is rounded); float16 and float32 run three (about 1e-6), and
+    matrices up to 64 x 128 run in float32.  The shorter side is at most 32768.
     ``coefficients``: a triple (a, b, c), or one for each step.  A zero matrix
     gives zeros; one that holds an infinity or a NaN gives NaN.  The result
     takes no part in autograd."""

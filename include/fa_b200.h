@@ -603,7 +603,9 @@ typedef struct fa_matrix {
  *   X <- a X + (b A + c A^2) X,  A = X X^T  (on the shorter side),
  * written in dtype (FA_F16, FA_BF16, FA_F32).  A zero matrix gives zeros, one
  * that holds an infinity or a NaN gives NaN.  Every matrix of a call has the
- * same dtype; the sizes may differ.  The workspace needs no zeroing. */
+ * same dtype; the sizes may differ: the shorter side at most 32768, the longer
+ * 4194304 (FA_E_SHAPE).  The workspace is 256-byte aligned and needs no
+ * zeroing. */
 FA_B200_API int fa_b200_orthogonalize_workspace_bytes(const fa_matrix* matrices, int count,
                                                       int dtype, size_t* out_bytes);
 FA_B200_API int fa_b200_orthogonalize(const fa_matrix* matrices, int count, int dtype,
