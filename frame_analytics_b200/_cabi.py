@@ -187,6 +187,7 @@ PROTOTYPES = {
     "fa_b200_orthogonalize_workspace_bytes": [_vp, _i, _i, _vp],
     "fa_b200_orthogonalize": [_vp, _i, _i, _vp, _i, _vp, _sz, _i, _vp],
     "fa_b200_muon_step": [_vp, _i, _i, _vp, _i, _d, _i, _d, _vp, _sz, _i, _vp],
+    "fa_b200_orthogonalize_wait_limit": [ctypes.c_ulonglong],
     "fa_b200_ssim_gmsd": [_pview, _pview, _vp, _i, _d, _d, _d, _d, _d, _d, _vp, _sz,
                           _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp],
 }

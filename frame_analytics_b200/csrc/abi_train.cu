@@ -13,6 +13,7 @@ int ns_check(const fa_matrix* m, int count, int dtype, bool update);
 int ns_impl(const fa_matrix* m, int count, int dtype, const double* coef, int steps, bool update,
             double mu, int nesterov, double decay, void* ws, size_t ws_bytes, int device,
             cudaStream_t st);
+int ns_wait_limit(unsigned long long limit_ns);
 
 }  // namespace fab
 
@@ -80,6 +81,10 @@ FA_B200_API int fa_b200_muon_step(const fa_matrix* matrices, int count, int dtyp
   FAB_DEVICE_SCOPE(device);
   return ns_impl(matrices, count, dtype, coefficients, steps, true, mu, nesterov, decay,
                  workspace, workspace_bytes, device, static_cast<cudaStream_t>(stream));
+}
+
+FA_B200_API int fa_b200_orthogonalize_wait_limit(unsigned long long limit_ns) {
+  return ns_wait_limit(limit_ns);
 }
 
 }  // extern "C"

@@ -110,6 +110,7 @@ struct NsArgs {
   unsigned* failed;                // set when a wait of this call gave up
   double* part;                    // [kMats][kNormBlocks]
   unsigned* err;
+  unsigned long long limit_ns;     // of a wait
   int small;                       // every matrix fits one block
   int pair;                        // two blocks a tile
   int ks;                          // parts of a tile at most
@@ -259,10 +260,12 @@ __device__ __forceinline__ unsigned ld_acquire(const unsigned* p) {
 }
 
 // Bounded wait on an mbarrier phase, or on a counter of finished tiles, that
-// tells whether it was reached.  On giving up (two seconds, or another wait of
-// the launch already has) it records FA_E_TIMEOUT and the caller leaves its
-// loop.  The launch's own word tells the other waits: the host-mapped word is
-// across the bus and is only written.
+// tells whether it was reached.  On giving up (after the launch's limit, or when
+// another wait of the launch already has) it records FA_E_TIMEOUT and the caller
+// leaves its loop.  The launch's own word tells the other waits: the host-mapped
+// word is across the bus and is only written.  No wait spans more than the few
+// tiles that it is for, the longest about 0.1 s (65536 blocks of K): a launch may
+// last longer than the limit.
 __device__ __noinline__ bool wait_slow(unsigned bar, unsigned parity, const unsigned* flag,
                                        unsigned want, const NsArgs& a) {
   const unsigned long long t0 = globaltimer_ns();
@@ -270,7 +273,7 @@ __device__ __noinline__ bool wait_slow(unsigned bar, unsigned parity, const unsi
     if (flag ? ld_acquire(flag) >= want : mbar_try(bar, parity)) return true;
     if ((i & 255u) == 0u) {
       const bool failed = *reinterpret_cast<volatile unsigned*>(a.failed) != 0u;
-      if (failed || globaltimer_ns() - t0 > kWaitLimitNs) {
+      if (failed || globaltimer_ns() - t0 > a.limit_ns) {
         if (!failed) {
           *reinterpret_cast<volatile unsigned*>(a.failed) = 1u;
           *reinterpret_cast<volatile unsigned*>(a.err) = (unsigned)FA_E_TIMEOUT;
@@ -971,8 +974,6 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
       mma_commit<PAIR>(&drain);
       wait_bar(&drain, 0, a);
     }
-    // the second block's barriers hear of it too, and it stays until they have
-    if (PAIR && lane == 0 && rank == 1) wait_bar(&drain, 0, a);
   } else if (warp >= 4) {
     Walk<PAIR> walk;
     Tile t;
@@ -1064,7 +1065,12 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
-  if constexpr (PAIR) cluster_sync();  // neither block's memory is in use any more
+  if constexpr (PAIR) {
+    cluster_sync();  // neither block's memory is in use any more
+    // The first block has issued its last commit, which arrives at the second
+    // block's barriers too: that block stays until it has.
+    if (rank == 1 && threadIdx.x == 32) wait_bar(&drain, 0, a);
+  }
   if (warp == 2) {
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     if constexpr (PAIR)
@@ -1258,6 +1264,15 @@ static bool half_map(CUtensorMap* map, __half* p, int batch, int rows, int cols,
 }
 
 static constexpr size_t kNsHead = sizeof(double) * kMats * kNormBlocks + 4 * (3 * kMats + 1 + 2 * kSplitTiles);
+
+// Limit of the device-side waits of the launches to come.
+static std::atomic<unsigned long long> g_wait_limit{kWaitLimitNs};
+
+int ns_wait_limit(unsigned long long limit_ns) {
+  if (limit_ns > kWaitLimitNs) return FA_E_ARG;
+  g_wait_limit.store(limit_ns ? limit_ns : kWaitLimitNs);
+  return FA_OK;
+}
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static int pitch64(int n) { return (n + 63) / 64 * 64; }
@@ -1573,6 +1588,7 @@ int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int
   if (!plan_steps(a.k, coef, steps)) return FA_E_ARG;
   a.err = wait_error_word();
   if (!a.err) return FA_E_INTERNAL;
+  a.limit_ns = g_wait_limit.load();
   a.mu = (float)mu;
   a.decay = (float)decay;
   a.nesterov = nesterov;

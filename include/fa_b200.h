@@ -619,6 +619,11 @@ FA_B200_API int fa_b200_muon_step(const fa_matrix* matrices, int count, int dtyp
                                   int nesterov, double decay, void* workspace,
                                   size_t workspace_bytes, int device, void* stream);
 
+/* Test hook: the limit of each device-side wait of the two calls above, from
+ * the next launch of this process on; 0 gives the default, 2 s, which is also
+ * the most (FA_E_ARG).  A launch may last longer than the limit of its waits. */
+FA_B200_API int fa_b200_orthogonalize_wait_limit(unsigned long long limit_ns);
+
 /* No counterpart in the reference: test hook of the bounded device-side
  * waits.  Launches one thread that waits `limit_ns` (at most 1 s) for an
  * mbarrier phase that nothing completes and then records FA_E_TIMEOUT the

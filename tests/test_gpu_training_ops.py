@@ -587,3 +587,27 @@ def test_training_example_learns():
     losses = train_restoration.train(steps=40, size=64, frames=4)
     assert all(math.isfinite(v) for v in losses)
     assert sum(losses[-5:]) < 0.8 * sum(losses[:5]), (losses[:5], losses[-5:])
+
+
+@pytest.mark.parametrize("shape,dtype", [((4100, 4200), torch.bfloat16), ((1500, 1400), torch.float32)])
+def test_a_launch_may_last_longer_than_the_limit_of_its_waits(shape, dtype):
+    """32 steps on 4100 x 4200 take about 10 ms, a tile below 0.1 ms: a limit of
+    3 ms for each wait is never reached.  (That shape runs in pairs of blocks.)"""
+    from frame_analytics_b200 import _cabi
+    L = _cabi.load()
+    x = gradient(shape, "noise", seed=15).to(dtype)
+    cubic = (1.5, -0.5, 0.0)
+    want = fa.orthogonalize(x, steps=32, coefficients=cubic)
+    t = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    assert L.fa_b200_orthogonalize_wait_limit(3_000_000) == 0
+    try:
+        t[0].record()
+        got = fa.orthogonalize(x, steps=32, coefficients=cubic)
+        t[1].record()
+        torch.cuda.synchronize()
+        fa.orthogonalize(x[:8, :8])  # a wait that gave up would be reported here
+    finally:
+        assert L.fa_b200_orthogonalize_wait_limit(0) == 0
+    if dtype == torch.bfloat16:
+        assert t[0].elapsed_time(t[1]) > 2 * 3
+    assert torch.equal(got, want)

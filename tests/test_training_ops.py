@@ -134,3 +134,10 @@ def test_structures_match_the_header():
     assert ctypes.sizeof(fa_heads) == 40
     assert ctypes.sizeof(fa_matrix) == 56
     assert ctypes.sizeof(fa_qk_params) == 40 + 24 + 16 + 16 + 8
+
+
+def test_the_wait_limit_is_at_most_the_default():
+    L = _cabi.load()
+    assert L.fa_b200_orthogonalize_wait_limit(2_000_000_001) == 5
+    assert L.fa_b200_orthogonalize_wait_limit(1_000_000) == 0
+    assert L.fa_b200_orthogonalize_wait_limit(0) == 0
