@@ -1277,46 +1277,6 @@ int ns_wait_limit(unsigned long long limit_ns) {
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static int pitch64(int n) { return (n + 63) / 64 * 64; }
 
-// The next matrices that share a launch sequence: at most kMats, of at most
-// kGroups shapes.  Members of one shape are numbered together.
-struct Batch {
-  int n = 0, groups = 0;
-  int member[kMats];               // call index of matrix i
-  int group[kMats];                // its shape
-  int rows[kGroups], cols[kGroups], count[kGroups], first[kGroups];
-};
-
-static int take_batch(const fa_matrix* m, int from, int count, Batch* o) {
-  int raw_group[kMats];
-  int n = 0;
-  o->groups = 0;
-  for (; n < kMats && from + n < count; ++n) {
-    int g = 0;
-    while (g < o->groups && (o->rows[g] != m[from + n].rows || o->cols[g] != m[from + n].cols)) ++g;
-    if (g == o->groups) {
-      if (g == kGroups) break;
-      o->rows[g] = m[from + n].rows;
-      o->cols[g] = m[from + n].cols;
-      o->count[g] = 0;
-      ++o->groups;
-    }
-    ++o->count[g];
-    raw_group[n] = g;
-  }
-  int at[kGroups], sum = 0;
-  for (int g = 0; g < o->groups; ++g) {
-    o->first[g] = at[g] = sum;
-    sum += o->count[g];
-  }
-  for (int i = 0; i < n; ++i) {
-    const int k = at[raw_group[i]]++;
-    o->member[k] = from + i;
-    o->group[k] = raw_group[i];
-  }
-  o->n = n;
-  return n;
-}
-
 // Workspace of one shape, and its pointers when `base` is given.
 static size_t group_layout(NsGroup* g, bool split, char* base) {
   size_t off = 0;
@@ -1347,6 +1307,58 @@ static void group_shape(NsGroup* g, int rows, int cols, int batch, int first) {
   g->first = first;
   g->px = pitch64(cols);
   g->pa = pitch64(g->s);
+}
+
+// The next matrices that share a launch sequence: at most kMats, of at most
+// kGroups shapes, and of at most kMostBytes of workspace (but at least one).
+// Members of one shape are numbered together.
+struct Batch {
+  int n = 0, groups = 0;
+  int member[kMats];               // call index of matrix i
+  int group[kMats];                // its shape
+  int rows[kGroups], cols[kGroups], count[kGroups], first[kGroups];
+};
+
+// A matrix needs 8 to 16 bytes an element of workspace, a hundred large ones
+// more than the model they belong to.  A few gigabytes of matrices fill the
+// machine: in sequences of 4, 2, 1 and 0.4 GB, 20 x 4096 x 4096 bfloat16 takes
+// 31.1, 30.1, 29.7 and 29.9 ms; in 2.3, 1.1 and 0.6 GB, 60 x 1024 x 4096 takes
+// 6.9, 7.4 and 7.9 ms.
+constexpr size_t kMostBytes = (size_t)2 << 30;
+
+static void take_batch(const fa_matrix* m, int from, int count, bool split, Batch* o) {
+  int raw_group[kMats];
+  int n = 0;
+  size_t bytes = 0;
+  o->groups = 0;
+  for (; n < kMats && from + n < count; ++n) {
+    NsGroup one{};
+    group_shape(&one, m[from + n].rows, m[from + n].cols, 1, 0);
+    bytes += group_layout(&one, split, nullptr);  // of n in one group: not more
+    if (n > 0 && bytes > kMostBytes) break;
+    int g = 0;
+    while (g < o->groups && (o->rows[g] != m[from + n].rows || o->cols[g] != m[from + n].cols)) ++g;
+    if (g == o->groups) {
+      if (g == kGroups) break;
+      o->rows[g] = m[from + n].rows;
+      o->cols[g] = m[from + n].cols;
+      o->count[g] = 0;
+      ++o->groups;
+    }
+    ++o->count[g];
+    raw_group[n] = g;
+  }
+  int at[kGroups], sum = 0;
+  for (int g = 0; g < o->groups; ++g) {
+    o->first[g] = at[g] = sum;
+    sum += o->count[g];
+  }
+  for (int i = 0; i < n; ++i) {
+    const int k = at[raw_group[i]]++;
+    o->member[k] = from + i;
+    o->group[k] = raw_group[i];
+  }
+  o->n = n;
 }
 
 static int tile_count(const NsGroup& g, bool sym, int bm, int bn) {
@@ -1389,8 +1401,8 @@ size_t ns_ws_bytes(const fa_matrix* m, int count, int dtype) {
   size_t most = 0;
   Batch b;
   const size_t parts = sizeof(float) * kPart * kSplitUnits;
-  for (int i = 0; i < count; i += take_batch(m, i, count, &b)) {
-    take_batch(m, i, count, &b);
+  for (int i = 0; i < count; i += b.n) {
+    take_batch(m, i, count, dtype != FA_BF16, &b);
     size_t sum = 0;
     for (int g = 0; g < b.groups; ++g) {
       NsGroup gr{};
@@ -1601,7 +1613,7 @@ int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int
   a.parts = reinterpret_cast<float*>(static_cast<char*>(ws) + up256(kNsHead));
   Batch bt;
   for (int i0 = 0; i0 < count; i0 += bt.n) {
-    take_batch(mats, i0, count, &bt);
+    take_batch(mats, i0, count, split, &bt);
     size_t off = up256(kNsHead) + sizeof(float) * kPart * kSplitUnits;
     a.groups = bt.groups;
     a.mats = bt.n;

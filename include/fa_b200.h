@@ -605,7 +605,9 @@ typedef struct fa_matrix {
  * that holds an infinity or a NaN gives NaN.  Every matrix of a call has the
  * same dtype; the sizes may differ: the shorter side at most 32768, the longer
  * 4194304 (FA_E_SHAPE).  The workspace is 256-byte aligned and needs no
- * zeroing. */
+ * zeroing; it is at most 2 GiB and a few MB, or what the largest matrix takes
+ * (8 to 16 bytes an element, sides rounded up to 64): longer lists run in
+ * parts, one after the other. */
 FA_B200_API int fa_b200_orthogonalize_workspace_bytes(const fa_matrix* matrices, int count,
                                                       int dtype, size_t* out_bytes);
 FA_B200_API int fa_b200_orthogonalize(const fa_matrix* matrices, int count, int dtype,

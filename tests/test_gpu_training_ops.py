@@ -611,3 +611,28 @@ def test_a_launch_may_last_longer_than_the_limit_of_its_waits(shape, dtype):
     if dtype == torch.bfloat16:
         assert t[0].elapsed_time(t[1]) > 2 * 3
     assert torch.equal(got, want)
+
+
+def test_lists_that_one_workspace_does_not_hold():
+    """45 x 2048 x 2048 would take 2.3 GB, 12 x (2048 x 4096 and 4096 x 4096)
+    3.4 GB: they run in parts that share 2 GiB.  Matrices on either side of a
+    cut against float64."""
+    x = gradient((45, 2048, 2048), "noise", seed=16).to(torch.bfloat16)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    y = fa.orthogonalize(x)
+    extra = torch.cuda.max_memory_allocated() - before - y.numel() * y.element_size()
+    assert extra <= (2 << 30) + (64 << 20)
+    for i in (0, 1, 21, 41, 42, 43, 44):
+        assert rel(y[i], plain_ns(x[i])) < NS_TOL[torch.bfloat16]
+    del x, y
+    shapes = [(2048, 4096), (4096, 4096)] * 12
+    g = torch.Generator(device="cuda").manual_seed(17)
+    W = [torch.zeros(s, dtype=torch.bfloat16, device="cuda") for s in shapes]
+    G = [torch.randn(s, generator=g, device="cuda").to(torch.bfloat16) for s in shapes]
+    M = [torch.zeros(s, device="cuda") for s in shapes]
+    fa.muon_step(W, G, M, lr=1.0, scale="none", nesterov=False)
+    for i in (0, 1, 13, 14, 15, 16, 23):
+        assert torch.equal(M[i], G[i].float())
+        assert rel(W[i], -plain_ns(G[i])) < NS_TOL[torch.bfloat16]

@@ -141,3 +141,22 @@ def test_the_wait_limit_is_at_most_the_default():
     assert L.fa_b200_orthogonalize_wait_limit(2_000_000_001) == 5
     assert L.fa_b200_orthogonalize_wait_limit(1_000_000) == 0
     assert L.fa_b200_orthogonalize_wait_limit(0) == 0
+
+
+def workspace(shapes, dtype):
+    L = _cabi.load()
+    m = (fa_matrix * len(shapes))(*[(16, 16, None, r, c, c, c, 0.1) for r, c in shapes])
+    size = ctypes.c_size_t(0)
+    assert L.fa_b200_orthogonalize_workspace_bytes(m, len(shapes), dtype, ctypes.byref(size)) == 0
+    return size.value
+
+
+@pytest.mark.parametrize("code", [1, 2, 3], ids=["f16", "bf16", "f32"])
+@pytest.mark.parametrize("shapes", [
+    [(4096, 4096)] * 128,
+    [(4096, 11008), (11008, 4096), (4096, 4096)] * 32,
+    [(16, 16)] + [(2048, 2048)] * 200 + [(8192, 8192)],
+])
+def test_workspace_does_not_grow_with_the_list(shapes, code):
+    one = max(workspace([s], code) for s in set(shapes))
+    assert one <= workspace(shapes, code) <= max(one, (2 << 30) + (16 << 20))
