@@ -39,6 +39,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <new>
 
 #include "mbar.cuh"
 #include "train.cuh"
@@ -88,6 +89,7 @@ struct NsMat {
   float* mom;                      // momentum, or null
   long long src_row, dst_row;
   float step;                      // W <- decay W - step O
+  int cols, s, l, tall;            // s, l: its shorter and its longer side
   int group;
   int vec;                         // rows are whole aligned 16-byte vectors
   int vec_dst;                     // the result's rows are whole aligned vectors of four
@@ -111,7 +113,6 @@ struct NsArgs {
   double* part;                    // [kMats][kNormBlocks]
   unsigned* err;
   unsigned long long limit_ns;     // of a wait
-  int small;                       // every matrix fits one block
   int pair;                        // two blocks a tile
   int ks;                          // parts of a tile at most
   float mu, decay;
@@ -1088,8 +1089,9 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
 // memory in float32, and the 15 dependent products cost float32 FMAs and block
 // barriers (2.5 us each at 64 x 64) in place of trips through memory:
 // 64 x 64 bfloat16 42 us on the GPU against 77 with the three launches of the tiled
-// kernel, 64 x 128 about 60 against 80.  At twice
-// the longer side the products alone take as long as the tiled kernel.
+// kernel, 64 x 128 about 60 against 80.  At twice the longer side the products
+// alone take as long as the tiled kernel.  A matrix's own shape decides, so that
+// it is updated alike whatever else a list holds.
 constexpr int kSmallS = 64, kSmallL = 128;
 constexpr int kLdX = kSmallL + 4, kLdA = kSmallS + 4;  // 8 rows' vectors in 8 bank groups
 constexpr int kSmallSmem = (int)sizeof(float) * (kSmallS * kLdX + 2 * kSmallS * kLdA);
@@ -1128,14 +1130,13 @@ __global__ void __launch_bounds__(256) ns_small_kernel(const __grid_constant__ N
   float* const B = A + kSmallS * kLdA;
   __shared__ double sm[32];
   const NsMat& m = a.m[blockIdx.x];
-  const NsGroup& g = a.g[m.group];
-  const int s = g.s, l = g.l, n = g.rows * g.cols;
+  const int s = m.s, l = m.l, n = s * l;
   for (int i = threadIdx.x; i < kSmallS * kLdX; i += 256) X[i] = 0.f;  // beyond s and l too
   __syncthreads();
   const T* src = reinterpret_cast<const T*>(m.src);
   double ss = 0;
   for (int i = threadIdx.x; i < n; i += 256) {
-    const int r = i / g.cols, c = i - r * g.cols;
+    const int r = i / m.cols, c = i - r * m.cols;
     float u = Ld<T>::f(src[r * m.src_row + c]);
     if (m.mom) {
       const float v = fmaf(a.mu, m.mom[i], u);
@@ -1143,7 +1144,7 @@ __global__ void __launch_bounds__(256) ns_small_kernel(const __grid_constant__ N
       u = a.nesterov ? fmaf(a.mu, v, u) : v;
     }
     ss += (double)u * u;
-    X[g.tall ? c * kLdX + r : r * kLdX + c] = u;
+    X[m.tall ? c * kLdX + r : r * kLdX + c] = u;
   }
   ss = block_sum(ss, sm);
   const bool finite = ss <= 1.7e308;
@@ -1221,8 +1222,8 @@ __global__ void __launch_bounds__(256) ns_small_kernel(const __grid_constant__ N
   }
   T* dst = reinterpret_cast<T*>(m.dst);
   for (int i = threadIdx.x; i < n; i += 256) {
-    const int r = i / g.cols, c = i - r * g.cols;
-    const float v = X[g.tall ? c * kLdX + r : r * kLdX + c];
+    const int r = i / m.cols, c = i - r * m.cols;
+    const float v = X[m.tall ? c * kLdX + r : r * kLdX + c];
     T* w = dst + r * m.dst_row + c;
     *w = St<T>::v(m.mom ? fmaf(a.decay, Ld<T>::f(*w), -m.step * v) : v);
   }
@@ -1264,6 +1265,9 @@ static bool half_map(CUtensorMap* map, __half* p, int batch, int rows, int cols,
 }
 
 static constexpr size_t kNsHead = sizeof(double) * kMats * kNormBlocks + 4 * (3 * kMats + 1 + 2 * kSplitTiles);
+
+// Workspace of a list whose matrices fit a block each: none, but not null.
+static constexpr size_t kNsNoWs = 256;
 
 // Limit of the device-side waits of the launches to come.
 static std::atomic<unsigned long long> g_wait_limit{kWaitLimitNs};
@@ -1311,7 +1315,8 @@ static void group_shape(NsGroup* g, int rows, int cols, int batch, int first) {
 
 // The next matrices that share a launch sequence: at most kMats, of at most
 // kGroups shapes, and of at most kMostBytes of workspace (but at least one).
-// Members of one shape are numbered together.
+// Members of one shape are numbered together.  Matrices that fit one block are
+// passed over: they have launches of their own.
 struct Batch {
   int n = 0, groups = 0;
   int member[kMats];               // call index of matrix i
@@ -1326,39 +1331,48 @@ struct Batch {
 // 6.9, 7.4 and 7.9 ms.
 constexpr size_t kMostBytes = (size_t)2 << 30;
 
-static void take_batch(const fa_matrix* m, int from, int count, bool split, Batch* o) {
-  int raw_group[kMats];
-  int n = 0;
+static bool fits_block(const fa_matrix& m) {
+  return std::min(m.rows, m.cols) <= kSmallS && std::max(m.rows, m.cols) <= kSmallL;
+}
+
+// False when none is left from *next on.
+static bool take_batch(const fa_matrix* m, int* next, int count, bool split, Batch* o) {
+  int raw_group[kMats], raw_member[kMats];
+  int n = 0, i = *next;
   size_t bytes = 0;
   o->groups = 0;
-  for (; n < kMats && from + n < count; ++n) {
+  for (; n < kMats && i < count; ++i) {
+    if (fits_block(m[i])) continue;
     NsGroup one{};
-    group_shape(&one, m[from + n].rows, m[from + n].cols, 1, 0);
+    group_shape(&one, m[i].rows, m[i].cols, 1, 0);
     bytes += group_layout(&one, split, nullptr);  // of n in one group: not more
     if (n > 0 && bytes > kMostBytes) break;
     int g = 0;
-    while (g < o->groups && (o->rows[g] != m[from + n].rows || o->cols[g] != m[from + n].cols)) ++g;
+    while (g < o->groups && (o->rows[g] != m[i].rows || o->cols[g] != m[i].cols)) ++g;
     if (g == o->groups) {
       if (g == kGroups) break;
-      o->rows[g] = m[from + n].rows;
-      o->cols[g] = m[from + n].cols;
+      o->rows[g] = m[i].rows;
+      o->cols[g] = m[i].cols;
       o->count[g] = 0;
       ++o->groups;
     }
     ++o->count[g];
-    raw_group[n] = g;
+    raw_member[n] = i;
+    raw_group[n++] = g;
   }
+  *next = i;
   int at[kGroups], sum = 0;
   for (int g = 0; g < o->groups; ++g) {
     o->first[g] = at[g] = sum;
     sum += o->count[g];
   }
-  for (int i = 0; i < n; ++i) {
-    const int k = at[raw_group[i]]++;
-    o->member[k] = from + i;
-    o->group[k] = raw_group[i];
+  for (int k = 0; k < n; ++k) {
+    const int to = at[raw_group[k]]++;
+    o->member[to] = raw_member[k];
+    o->group[to] = raw_group[k];
   }
   o->n = n;
+  return n > 0;
 }
 
 static int tile_count(const NsGroup& g, bool sym, int bm, int bn) {
@@ -1401,8 +1415,7 @@ size_t ns_ws_bytes(const fa_matrix* m, int count, int dtype) {
   size_t most = 0;
   Batch b;
   const size_t parts = sizeof(float) * kPart * kSplitUnits;
-  for (int i = 0; i < count; i += b.n) {
-    take_batch(m, i, count, dtype != FA_BF16, &b);
+  for (int next = 0; take_batch(m, &next, count, dtype != FA_BF16, &b);) {
     size_t sum = 0;
     for (int g = 0; g < b.groups; ++g) {
       NsGroup gr{};
@@ -1411,7 +1424,7 @@ size_t ns_ws_bytes(const fa_matrix* m, int count, int dtype) {
     }
     most = std::max(most, sum);
   }
-  return up256(kNsHead) + parts + most;
+  return most ? up256(kNsHead) + parts + most : kNsNoWs;
 }
 
 // Everything about a call that can be refused before the device is touched.
@@ -1557,17 +1570,39 @@ static int ns_products(const NsArgs& a, int units, cudaStream_t st) {
   return FA_OK;
 }
 
+template <typename T>
+static int ns_run_small(const NsArgs& a, cudaStream_t st) {
+  FAB_TRY(cudaFuncSetAttribute(ns_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kSmallSmem));
+  ns_small_kernel<T><<<a.mats, 256, kSmallSmem, st>>>(a);
+  FAB_LAUNCH_CHECK();
+  return FA_OK;
+}
+
+static void ns_fill(NsMat* o, const fa_matrix& f, int group, bool update, int dtype) {
+  o->src = f.src;
+  o->dst = f.dst;
+  o->mom = update ? f.momentum : nullptr;
+  o->src_row = f.src_row_stride;
+  o->dst_row = f.dst_row_stride;
+  o->step = (float)f.step;
+  o->cols = f.cols;
+  o->s = std::min(f.rows, f.cols);
+  o->l = std::max(f.rows, f.cols);
+  o->tall = f.rows > f.cols;
+  o->group = group;
+  const int item = dtype == FA_F32 ? 4 : 2;
+  o->vec = f.cols % 8 == 0 && reinterpret_cast<uintptr_t>(f.src) % 16 == 0 &&
+           (f.rows == 1 || f.src_row_stride * item % 16 == 0) &&
+           (!o->mom || reinterpret_cast<uintptr_t>(o->mom) % 16 == 0);
+  o->vec_dst = f.cols % 4 == 0 && reinterpret_cast<uintptr_t>(f.dst) % (4 * item) == 0 &&
+               (f.rows == 1 || f.dst_row_stride % 4 == 0);
+}
+
 template <bool SPLIT, typename T>
 static int ns_run(NsArgs& a, int device, cudaStream_t st) {
   const int sms = sm_count(device);
   long long most = 0;
-  if (a.small) {
-    FAB_TRY(cudaFuncSetAttribute(ns_small_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 kSmallSmem));
-    ns_small_kernel<T><<<a.mats, 256, kSmallSmem, st>>>(a);
-    FAB_LAUNCH_CHECK();
-    return FA_OK;
-  }
   for (int g = 0; g < a.groups; ++g)
     most = std::max<long long>(most, (long long)a.g[g].rows * a.g[g].px);
   const int nb = (int)std::max<long long>(
@@ -1589,12 +1624,114 @@ static int ns_run(NsArgs& a, int device, cudaStream_t st) {
   return ns_products<SPLIT, false, T>(a, sms, st);
 }
 
+// Where a list holds both kinds, its one-block matrices run on a stream of their
+// own beside the tiled ones: 3 x 64 x 64 with 6 x 64 x 576 and 4 x 180 x 180,
+// bfloat16, take 105 us so, and 157 us one kind after the other.  A stream serves
+// one call at a time; one is kept for each device.
+struct Side {
+  cudaStream_t stream = nullptr;
+  cudaEvent_t begin = nullptr, end = nullptr;
+};
+static std::atomic<Side*> g_side[64];
+
+static void side_free(Side* s) {
+  if (!s) return;
+  if (s->begin) cudaEventDestroy(s->begin);
+  if (s->end) cudaEventDestroy(s->end);
+  if (s->stream) cudaStreamDestroy(s->stream);
+  delete s;
+}
+
+// A stream that follows `st`; null where one is not to be had, or where `st` is
+// being captured (a kept stream would join the capture).
+static Side* side_fork(int device, cudaStream_t st) {
+  if (device < 0 && cudaGetDevice(&device) != cudaSuccess) device = 64;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (device >= 64 || cudaStreamIsCapturing(st, &cap) != cudaSuccess ||
+      cap != cudaStreamCaptureStatusNone) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  Side* s = g_side[device].exchange(nullptr);
+  if (!s) {
+    s = new (std::nothrow) Side;
+    if (!s) return nullptr;
+    if (cudaStreamCreateWithFlags(&s->stream, cudaStreamNonBlocking) != cudaSuccess ||
+        cudaEventCreateWithFlags(&s->begin, cudaEventDisableTiming) != cudaSuccess ||
+        cudaEventCreateWithFlags(&s->end, cudaEventDisableTiming) != cudaSuccess) {
+      cudaGetLastError();
+      side_free(s);
+      return nullptr;
+    }
+  }
+  if (cudaEventRecord(s->begin, st) != cudaSuccess ||
+      cudaStreamWaitEvent(s->stream, s->begin, 0) != cudaSuccess) {
+    cudaGetLastError();
+    side_free(s);
+    return nullptr;
+  }
+  return s;
+}
+
+static int side_join(Side* s, int device, cudaStream_t st) {
+  if (device < 0 && cudaGetDevice(&device) != cudaSuccess) device = 0;
+  int rc = status_of(cudaEventRecord(s->end, s->stream));
+  if (!rc) rc = status_of(cudaStreamWaitEvent(st, s->end, 0));
+  side_free(g_side[device].exchange(s));
+  return rc;
+}
+
+// The matrices that fit one block, each.
+static int ns_blocks(NsArgs& a, const fa_matrix* mats, int count, int dtype, bool update,
+                     cudaStream_t st) {
+  a.mats = 0;
+  for (int i = 0; i < count; ++i) {
+    if (fits_block(mats[i])) ns_fill(&a.m[a.mats++], mats[i], 0, update, dtype);
+    if (a.mats == 0 || (a.mats < kMats && i + 1 < count)) continue;
+    const int rc = dtype == FA_F16    ? ns_run_small<f16_t>(a, st)
+                   : dtype == FA_BF16 ? ns_run_small<bf16_t>(a, st)
+                                      : ns_run_small<float>(a, st);
+    if (rc) return rc;
+    a.mats = 0;
+  }
+  return FA_OK;
+}
+
+// The others.
+static int ns_tiles(NsArgs& a, const fa_matrix* mats, int count, int dtype, bool update, char* ws,
+                    int device, cudaStream_t st) {
+  const bool split = dtype != FA_BF16;
+  Batch bt;
+  for (int next = 0; take_batch(mats, &next, count, split, &bt);) {
+    size_t off = up256(kNsHead) + sizeof(float) * kPart * kSplitUnits;
+    a.groups = bt.groups;
+    a.mats = bt.n;
+    for (int gi = 0; gi < bt.groups; ++gi) {
+      NsGroup& g = a.g[gi];
+      group_shape(&g, bt.rows[gi], bt.cols[gi], bt.count[gi], bt.first[gi]);
+      off += group_layout(&g, split, ws + off);
+      for (int h = 0; h < (split ? 2 : 1); ++h) {
+        if (!half_map(&g.map[MAP_X0][h], g.x[0][h], g.batch, g.rows, g.cols, g.px) ||
+            !half_map(&g.map[MAP_X1][h], g.x[1][h], g.batch, g.rows, g.cols, g.px) ||
+            !half_map(&g.map[MAP_A][h], g.a[h], g.batch, g.s, g.s, g.pa) ||
+            !half_map(&g.map[MAP_B][h], g.b[h], g.batch, g.s, g.s, g.pa))
+          return FA_E_INTERNAL;
+      }
+    }
+    for (int i = 0; i < bt.n; ++i) ns_fill(&a.m[i], mats[bt.member[i]], bt.group[i], update, dtype);
+    const int rc = dtype == FA_F16    ? ns_run<true, f16_t>(a, device, st)
+                   : dtype == FA_BF16 ? ns_run<false, bf16_t>(a, device, st)
+                                      : ns_run<true, float>(a, device, st);
+    if (rc) return rc;
+  }
+  return FA_OK;
+}
+
 int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int steps,
             bool update, double mu, int nesterov, double decay, void* ws, size_t ws_bytes,
             int device, cudaStream_t st) {
   if (!coef || !ws) return FA_E_ARG;
   if (steps < 1 || steps > kMaxSteps) return FA_E_SHAPE;
-  const bool split = dtype != FA_BF16;
   NsArgs a;
   a.steps = steps;
   if (!plan_steps(a.k, coef, steps)) return FA_E_ARG;
@@ -1605,61 +1742,24 @@ int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int
   a.decay = (float)decay;
   a.nesterov = nesterov;
   const uintptr_t base = reinterpret_cast<uintptr_t>(ws);
-  if (base & 255) return FA_E_ARG;
+  const size_t need = ns_ws_bytes(mats, count, dtype);
+  if ((base & 255) || ws_bytes < need) return FA_E_ARG;
+  bool small = false;
+  for (int i = 0; i < count && !small; ++i) small = fits_block(mats[i]);
   a.part = reinterpret_cast<double*>(ws);
   a.done = reinterpret_cast<unsigned*>(a.part + kMats * kNormBlocks);
   a.failed = a.done + 3 * kMats;
   a.joins = a.failed + 1;
   a.parts = reinterpret_cast<float*>(static_cast<char*>(ws) + up256(kNsHead));
-  Batch bt;
-  for (int i0 = 0; i0 < count; i0 += bt.n) {
-    take_batch(mats, i0, count, split, &bt);
-    size_t off = up256(kNsHead) + sizeof(float) * kPart * kSplitUnits;
-    a.groups = bt.groups;
-    a.mats = bt.n;
-    a.small = 1;
-    for (int gi = 0; gi < bt.groups; ++gi)
-      a.small &= std::min(bt.rows[gi], bt.cols[gi]) <= kSmallS &&
-                 std::max(bt.rows[gi], bt.cols[gi]) <= kSmallL;
-    for (int gi = 0; gi < bt.groups; ++gi) {
-      NsGroup& g = a.g[gi];
-      group_shape(&g, bt.rows[gi], bt.cols[gi], bt.count[gi], bt.first[gi]);
-      off += group_layout(&g, split, static_cast<char*>(ws) + off);
-      if (off > ws_bytes) return FA_E_ARG;
-      for (int h = 0; !a.small && h < (split ? 2 : 1); ++h) {
-        if (!half_map(&g.map[MAP_X0][h], g.x[0][h], g.batch, g.rows, g.cols, g.px) ||
-            !half_map(&g.map[MAP_X1][h], g.x[1][h], g.batch, g.rows, g.cols, g.px) ||
-            !half_map(&g.map[MAP_A][h], g.a[h], g.batch, g.s, g.s, g.pa) ||
-            !half_map(&g.map[MAP_B][h], g.b[h], g.batch, g.s, g.s, g.pa))
-          return FA_E_INTERNAL;
-      }
-    }
-    for (int i = 0; i < bt.n; ++i) {
-      const fa_matrix& f = mats[bt.member[i]];
-      NsMat& m = a.m[i];
-      m.src = f.src;
-      m.dst = f.dst;
-      m.mom = update ? f.momentum : nullptr;
-      m.src_row = f.src_row_stride;
-      m.dst_row = f.dst_row_stride;
-      m.step = (float)f.step;
-      m.group = bt.group[i];
-      const int item = dtype == FA_F32 ? 4 : 2;
-      m.vec = f.cols % 8 == 0 && reinterpret_cast<uintptr_t>(f.src) % 16 == 0 &&
-              (f.rows == 1 || f.src_row_stride * item % 16 == 0) &&
-              (!m.mom || reinterpret_cast<uintptr_t>(m.mom) % 16 == 0);
-      m.vec_dst = f.cols % 4 == 0 && reinterpret_cast<uintptr_t>(f.dst) % (4 * item) == 0 &&
-                  (f.rows == 1 || f.dst_row_stride % 4 == 0);
-    }
-    int rc;
-    switch (dtype) {
-      case FA_F16: rc = ns_run<true, f16_t>(a, device, st); break;
-      case FA_BF16: rc = ns_run<false, bf16_t>(a, device, st); break;
-      default: rc = ns_run<true, float>(a, device, st); break;
-    }
-    if (rc) return rc;
+  // tiled matrices need a workspace: both kinds are in the list
+  Side* side = need > kNsNoWs && small ? side_fork(device, st) : nullptr;
+  int rc = ns_blocks(a, mats, count, dtype, update, side ? side->stream : st);
+  if (!rc) rc = ns_tiles(a, mats, count, dtype, update, static_cast<char*>(ws), device, st);
+  if (side) {
+    const int joined = side_join(side, device, st);
+    if (!rc) rc = joined;
   }
-  return FA_OK;
+  return rc;
 }
 
 }  // namespace fab

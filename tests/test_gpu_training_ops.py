@@ -636,3 +636,65 @@ def test_lists_that_one_workspace_does_not_hold():
     for i in (0, 1, 13, 14, 15, 16, 23):
         assert torch.equal(M[i], G[i].float())
         assert rel(W[i], -plain_ns(G[i])) < NS_TOL[torch.bfloat16]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_small_matrix_is_updated_alike_whatever_the_list_holds(dtype):
+    """Matrices up to 64 x 128 run in float32, alone, beside larger ones, and on
+    either side of a cut at 128 matrices or 8 shapes."""
+    g = torch.Generator(device="cuda").manual_seed(18)
+
+    def step(shapes, at):
+        G = [grads[s] for s in shapes]
+        W = [torch.zeros(s, dtype=dtype, device="cuda") for s in shapes]
+        M = [torch.zeros(s, device="cuda") for s in shapes]
+        fa.muon_step(W, G, M, lr=1.0, scale="none", nesterov=False)
+        for s, w in zip(shapes, W):
+            assert rel(w, -plain_ns(grads[s])) < NS_TOL[dtype]
+        return [W[i] for i in at]
+
+    small = [(64, 64), (16, 27), (128, 64), (1, 5), (64, 128), (9, 100), (33, 20), (40, 40), (7, 7),
+             (12, 80)]
+    large = [(300, 280), (65, 64), (64, 129)]
+    grads = {s: torch.randn(s, generator=g, device="cuda").to(dtype) for s in small + large}
+    alone = {s: step([s], [0])[0] for s in small}
+    for s in small:  # float32 and one rounding of the output
+        assert rel(alone[s], -plain_ns(grads[s])) < 2 * U[dtype] + 2e-5
+    mixed = [large[0]] + small + large[1:] + small[::-1]
+    at = [i for i, s in enumerate(mixed) if s in small]
+    for i, w in zip(at, step(mixed, at)):
+        assert torch.equal(w, alone[mixed[i]])
+    many = [small[i % 10] for i in range(150)] + [large[0]]
+    for i, w in enumerate(step(many, range(150))):
+        assert torch.equal(w, alone[many[i]])
+
+
+def test_mixed_lists_in_a_graph_and_on_two_streams():
+    """Small matrices run beside the larger ones: what follows on the caller's
+    stream waits for both."""
+    g = torch.Generator(device="cuda").manual_seed(19)
+    shapes = [(64, 64), (300, 280), (16, 27), (128, 64), (65, 200)]
+    G = [torch.randn(s, generator=g, device="cuda") for s in shapes]
+
+    def step(x):
+        W = [torch.zeros_like(t) for t in x]
+        fa.muon_step(W, x, [torch.zeros_like(t) for t in x], lr=1.0, nesterov=False)
+        return [2 * w for w in W]
+
+    want = step(G)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(8):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(step([t.clone() for t in G]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got.append(step(G))
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for run in got:
+        assert all(torch.equal(a, b) for a, b in zip(run, want))
