@@ -246,12 +246,17 @@ class Muon(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         super().load_state_dict(state_dict)
         # the base class casts state to its parameter's dtype; momentum stays float32
+        # and takes its parameter's memory layout
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             for p, key in zip(group["params"], saved["params"]):
                 buf = state_dict["state"].get(key, {}).get("momentum_buffer")
-                if buf is not None:
-                    self.state[p]["momentum_buffer"] = buf.detach().to(
-                        device=p.device, dtype=torch.float32, copy=True)
+                if buf is None:
+                    continue
+                if buf.shape != p.shape:
+                    raise ValueError(f"momentum of shape {tuple(buf.shape)} for a parameter of "
+                                     f"shape {tuple(p.shape)}")
+                self.state[p]["momentum_buffer"] = torch.empty_like(
+                    p, dtype=torch.float32, requires_grad=False).copy_(buf.detach())
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -265,8 +270,11 @@ class Muon(torch.optim.Optimizer):
                 if p.grad is None:
                     continue
                 state = self.state[p]
-                if "momentum_buffer" not in state:
+                buf = state.get("momentum_buffer")
+                if buf is None:
                     state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32)
+                elif buf.stride() != p.stride():  # the parameter was laid out anew
+                    state["momentum_buffer"] = torch.empty_like(p, dtype=torch.float32).copy_(buf)
                 ws, gs, ms = sets.setdefault((p.device, p.dtype), ([], [], []))
                 ws.append(p)
                 gs.append(p.grad)

@@ -698,3 +698,53 @@ def test_mixed_lists_in_a_graph_and_on_two_streams():
     torch.cuda.synchronize()
     for run in got:
         assert all(torch.equal(a, b) for a, b in zip(run, want))
+
+
+@pytest.mark.parametrize("relaid", ["checkpoint", "in place"])
+@pytest.mark.parametrize("frm,to", [(torch.contiguous_format, torch.channels_last),
+                                    (torch.channels_last, torch.contiguous_format)])
+def test_muon_momentum_follows_its_parameters_layout(frm, to, relaid):
+    """Against a run that keeps its layout: the momenta are the same numbers, the
+    weights differ by what two sums in other orders may (each within NS_TOL of
+    the update, whose norm is at most 1.3 sqrt(cols) lr)."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    w = torch.randn(24, 12, 3, 3, generator=g, device="cuda") / 8
+    grads = [torch.randn(w.shape, generator=g, device="cuda") for _ in range(3)]
+
+    def optimizer(start, fmt):
+        p = torch.nn.Parameter(start.detach().clone().contiguous(memory_format=fmt))
+        return p, fa.Muon([p], lr=0.05)
+
+    def advance(p, opt, gr):
+        p.grad = gr.contiguous(memory_format=torch.contiguous_format).clone()
+        opt.step()
+
+    keep, kept = optimizer(w, frm)
+    p, opt = optimizer(w, frm)
+    advance(keep, kept, grads[0])
+    advance(p, opt, grads[0])
+    assert torch.equal(p, keep)
+    if relaid == "checkpoint":
+        saved = opt.state_dict()
+        p, opt = optimizer(p, to)
+        opt.load_state_dict(saved)
+    else:
+        p.data = p.data.contiguous(memory_format=to)
+    for gr in grads[1:]:
+        advance(keep, kept, gr)
+        advance(p, opt, gr)
+    assert p.is_contiguous(memory_format=to)
+    m = opt.state[p]["momentum_buffer"]
+    assert m.stride() == p.stride() and torch.equal(m, kept.state[keep]["momentum_buffer"])
+    update = 2 * 1.3 * math.sqrt(24) * 0.05
+    tol = 2 * NS_TOL[torch.float32] * update + 2 * 2 * U[torch.float32] * float(w.norm())
+    assert float((p - keep).detach().norm()) < tol
+
+
+def test_muon_refuses_a_checkpoint_of_another_shape():
+    a, b = (torch.nn.Parameter(torch.zeros(s, device="cuda")) for s in ((4, 6), (1, 6)))
+    one, two = fa.Muon([a]), fa.Muon([b])
+    b.grad = torch.ones_like(b)
+    two.step()
+    with pytest.raises(ValueError, match="shape"):
+        one.load_state_dict(two.state_dict())
