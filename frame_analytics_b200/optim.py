@@ -131,6 +131,15 @@ def _like_layout(t: torch.Tensor, w: torch.Tensor) -> Optional[torch.Tensor]:
     return None
 
 
+def _copied(t: torch.Tensor, like: torch.Tensor, name: str, back: list) -> torch.Tensor:
+    """A copy of `t` with `like`'s order of elements, to be written back."""
+    if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        raise ValueError(f"{name} has elements that share memory")
+    c = torch.empty_like(like, dtype=t.dtype).copy_(t.detach())
+    back.append((t.detach(), c))
+    return c
+
+
 _SCALES = ("aspect", "rms", "none")
 
 
@@ -155,7 +164,8 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     more, rows = the first, the others flattened) and ``momenta`` (float32, the
     weights' shapes) are updated; ``grads`` have the weights' dtype.  ``scale``
     s: ``"aspect"`` sqrt(max(1, rows / cols)), ``"rms"`` 0.2 sqrt(max(rows,
-    cols)), ``"none"`` 1.  All matrices run through one sequence of launches,
+    cols)), ``"none"`` 1.  Contiguous tensors and channels-last kernels are used
+    where they lie, others through copies.  All matrices run through one sequence of launches,
     whatever their shapes."""
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     if not len(weights) == len(grads) == len(momenta):
@@ -170,7 +180,7 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
                          f"momentum {momentum} in [0, 1)")
     if not weights:
         return
-    first, rows, keep = weights[0], [], []
+    first, rows, keep, back = weights[0], [], [], []
     dtype, index, scales = first.dtype, first.get_device(), {}
     for i, (w, g, m) in enumerate(zip(weights, grads, momenta)):
         shape = w.shape
@@ -192,14 +202,16 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
             continue
         wm, gm, mm = w, g, m
         if not (w.is_contiguous() and g.is_contiguous() and m.is_contiguous()):
-            wm, mm, gm = _rows_layout(w.detach()), _like_layout(m, w), _like_layout(g.detach(), w)
+            w_ = w.detach()
+            wm = _rows_layout(w_)
             if wm is None:
-                raise ValueError(f"weight {i} must be contiguous (or a channels-last kernel)")
+                w_ = _copied(w, torch.empty(shape, dtype=dtype, device=w.device), f"weight {i}", back)
+                wm = _rows_layout(w_)
+            mm, gm = _like_layout(m.detach(), w_), _like_layout(g.detach(), w_)
             if mm is None:
-                raise ValueError(f"momentum {i} must have its weight's memory layout")
+                mm = _rows_layout(_copied(m, w_, f"momentum {i}", back))
             if gm is None:
-                # the weight's order of elements: a copy
-                gm = _rows_layout(torch.empty_like(w).copy_(g.detach()))
+                gm = _rows_layout(torch.empty_like(w_).copy_(g.detach()))
                 keep.append(gm)
         step = scales.get(shape)
         if step is None:
@@ -214,6 +226,8 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     mats = b"".join([_MATRIX(*row) for row in rows])
     _run(backend.lib().fa_b200_muon_step, mats, len(rows), first, coef, steps, momentum,
          int(nesterov), 1.0 - lr * weight_decay)
+    for t, c in back:
+        t.copy_(c)
     # autograd notices weights that a graph still needs, as for torch's own updates
     torch.autograd.graph.increment_version(weights + momenta)
 

@@ -741,6 +741,44 @@ def test_muon_momentum_follows_its_parameters_layout(frm, to, relaid):
     assert float((p - keep).detach().norm()) < tol
 
 
+def test_muon_takes_any_layout():
+    g = torch.Generator(device="cuda").manual_seed(22)
+    w = torch.randn(40, 72, generator=g, device="cuda") / 8
+    gr = torch.randn(40, 72, generator=g, device="cuda")
+    m = torch.randn(40, 72, generator=g, device="cuda")
+
+    def layouts(t):
+        wide = [torch.full((40, 150), 7.0, device="cuda") for _ in range(2)]
+        return [t.clone(), t.t().contiguous().t(), wide[0][:, 3:147:2].copy_(t),
+                wide[1][:, 150 - 72:].copy_(t)]
+
+    want_w, want_m = w.clone(), m.clone()
+    fa.muon_step([want_w], [gr], [want_m], lr=0.1)
+    for i in range(3):
+        for j in range(3):
+            for k in range(3):
+                wl, gl, ml = layouts(w)[i], layouts(gr)[j], layouts(m)[k]
+                fa.muon_step([wl], [gl], [ml], lr=0.1)
+                assert torch.equal(wl, want_w) and torch.equal(ml, want_m) and torch.equal(gl, gr)
+    sliced = layouts(w)[3]
+    base = sliced._base
+    fa.muon_step([sliced], [gr], [m.clone()], lr=0.1)
+    assert torch.equal(sliced, want_w) and bool((base[:, :3] == 7).all())
+    # 3-D kernels, channels last
+    w5, g5 = (torch.randn(8, 4, 3, 2, 2, generator=g, device="cuda") for _ in range(2))
+    last = w5.contiguous(memory_format=torch.channels_last_3d)
+    m5 = torch.zeros_like(last)
+    fa.muon_step([w5], [g5], [torch.zeros_like(w5)], lr=0.1)
+    fa.muon_step([last], [g5], [m5], lr=0.1)
+    assert torch.equal(last, w5) and torch.equal(m5, g5)
+    # one row, spread over the list's rows
+    shared = torch.zeros(1, 72, device="cuda").expand(40, 72)
+    for args in (([shared], [gr], [m]), ([w], [gr], [shared])):
+        with pytest.raises(ValueError, match="share memory"):
+            fa.muon_step(*args, lr=0.1)
+    fa.muon_step([w.clone()], [gr[:1].expand(40, 72)], [m], lr=0.1)
+
+
 def test_muon_refuses_a_checkpoint_of_another_shape():
     a, b = (torch.nn.Parameter(torch.zeros(s, device="cuda")) for s in ((4, 6), (1, 6)))
     one, two = fa.Muon([a]), fa.Muon([b])
