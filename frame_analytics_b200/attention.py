@@ -12,6 +12,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import backend
 from .functional import _reject_double_backward
@@ -114,6 +115,11 @@ def _check_out(name, o, x):
         raise ValueError(f"{name} has elements that share memory")
 
 
+def _reject_tangents(*tensors) -> None:
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("qk_norm_rotary has no forward-mode derivative")
+
+
 # Shapes and dtypes that passed _check: metadata, no tensor is kept.
 _checked: set = set()
 
@@ -164,8 +170,9 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor]
                    out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
                    ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Normalise every query and key head and rotate it by its token's position:
-    ``y = R_p (w * x / sqrt(mean(x**2) + eps))``.  Differentiable in the
-    operands and the weights.
+    ``y = R_p (w * x / sqrt(mean(x**2) + eps))``.  Differentiable once, in
+    reverse mode, in the operands and the weights; ``cos`` and ``sin`` that want
+    a gradient are refused.
 
     ``q`` (B, L, Hq, D) and ``k`` (B, L, Hk, D), float16 / bfloat16 / float32,
     may be views of a packed projection (any strides with unit stride in D; D
@@ -173,8 +180,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor]
     ``R <= D`` components turn, in pairs (i, i + R/2), or (2i, 2i + 1) with
     ``interleaved``.  ``positions``: int32 / int64 (L,) or (B, L) rows of the
     tables, by default 0..L-1; a position outside the tables gives NaN for its
-    token (and then for the weights' gradients).  Weights: (D,) shared by the heads, or (heads, D); in the operands'
-    dtype or float32.
+    token (and then for the weights' gradients).  Weights: (D,) shared by the
+    heads, or (heads, D); in the operands' dtype or float32.
 
     Returns contiguous (B, L, Hq, D) and (B, L, Hk, D).  ``out=(q_out, k_out)``
     writes there instead (any strides with unit stride in D: a slice of a cache,
@@ -187,13 +194,18 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor]
         if len(_checked) > 4096:
             _checked.clear()
         _checked.add(key)
+    tracked = torch.is_grad_enabled()
+    if tracked and cos is not None and (cos.requires_grad or sin.requires_grad):
+        raise ValueError("qk_norm_rotary gives cos and sin no gradient: detach them")
+    if forward_ad._current_level >= 0:
+        _reject_tangents(q, k, cos, sin, q_weight, k_weight)
     index = q.get_device()
     for t in (q, k, cos, sin, q_weight, k_weight, positions):
         if t is not None and t.get_device() != index or index < 0:
             backend.require_cuda(*[u for u in (q, k, cos, sin, q_weight, k_weight, positions)
                                    if u is not None])
             raise ValueError("all tensors must be on one device")
-    grad = torch.is_grad_enabled() and any(
+    grad = tracked and any(
         t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
     if out is not None:
         if grad:

@@ -160,3 +160,28 @@ def workspace(shapes, dtype):
 def test_workspace_does_not_grow_with_the_list(shapes, code):
     one = max(workspace([s], code) for s in set(shapes))
     assert one <= workspace(shapes, code) <= max(one, (2 << 30) + (16 << 20))
+
+
+@pytest.mark.parametrize("which", ["cos", "sin"])
+def test_qk_norm_rotary_refuses_tables_that_want_a_gradient(which):
+    table = torch.zeros(5, 8, requires_grad=True)
+    with pytest.raises(ValueError, match="no gradient"):
+        qk(**{which: table})
+    with pytest.raises(ValueError, match="no gradient"):  # computed from learned frequencies
+        qk(**{which: 2 * table})
+    with torch.no_grad(), pytest.raises(TypeError):  # the next check: not on the GPU
+        qk(**{which: table})
+
+
+@pytest.mark.parametrize("which", ["q", "k", "cos", "sin", "q_weight", "k_weight"])
+def test_qk_norm_rotary_refuses_forward_mode(which):
+    import torch.autograd.forward_ad as fw
+    shapes = dict(q=(2, 3, 4, 16), k=(2, 3, 2, 16), cos=(5, 8), sin=(5, 8), q_weight=(16,),
+                  k_weight=(16,))
+    t = {n: torch.ones(s) for n, s in shapes.items()}
+    with fw.dual_level():
+        with pytest.raises(TypeError):  # no tangent: the next check, not on the GPU
+            qk(**t)
+        t[which] = fw.make_dual(t[which], torch.ones(shapes[which]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            qk(**t)
