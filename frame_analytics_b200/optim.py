@@ -219,8 +219,12 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
         r = shape[0]
         c = n // r
         rows.append((gm.data_ptr(), wm.data_ptr(), mm.data_ptr(), r, c, c, c, step))
-    if len({p for row in rows for p in row[1:3]}) < 2 * len(rows):
+    written = {p for row in rows for p in row[1:3]}
+    if len(written) < 2 * len(rows):
         raise ValueError("a weight or a momentum is given twice")
+    # a gradient is read again after the momenta, and other weights, are written
+    if any(row[0] in written and row[0] != row[1] for row in rows):
+        raise ValueError("a gradient is also given as a momentum or as another weight")
     if not rows:
         return
     mats = b"".join([_MATRIX(*row) for row in rows])

@@ -786,3 +786,18 @@ def test_muon_refuses_a_checkpoint_of_another_shape():
     two.step()
     with pytest.raises(ValueError, match="shape"):
         one.load_state_dict(two.state_dict())
+
+
+def test_muon_refuses_gradients_that_it_would_overwrite():
+    a, b = (torch.randn(300, 280, device="cuda") for _ in range(2))
+    m, n = torch.zeros_like(a), torch.zeros_like(a)
+    before = [t.clone() for t in (a, b, m, n)]
+    for ws, gs, ms in (([a], [m], [m]), ([a, b], [n, m], [m, n]), ([a, b], [b, a], [m, n]),
+                       ([a, a], [b, b], [m, n]), ([a, b], [b, b], [m, m])):
+        with pytest.raises(ValueError):
+            fa.muon_step(ws, gs, ms, lr=0.1)
+    assert all(torch.equal(x, y) for x, y in zip((a, b, m, n), before))
+    # its own weight is read before it is written
+    want, _ = plain_muon(a, a, m, 0.1, 0.95, True, 0.0, "none")
+    fa.muon_step([a], [a], [m], lr=0.1, scale="none")
+    assert rel(a, want) < 2e-6 and torch.equal(m, before[0])
