@@ -115,6 +115,24 @@ def _check_out(name, o, x):
         raise ValueError(f"{name} has elements that share memory")
 
 
+def _same_place(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
+def _check_places(q_out, k_out, q, k) -> None:
+    """Outputs start apart from one another and from every input but their own,
+    which they then cover element for element.  (Overlaps that start elsewhere
+    are the caller's to avoid.)"""
+    po, pk = q_out.data_ptr(), k_out.data_ptr()
+    for name, bad in (("out[0] and out[1]", po == pk),
+                      ("out[0] and k", po == k.data_ptr()),
+                      ("out[1] and q", pk == q.data_ptr()),
+                      ("out[0] and q", po == q.data_ptr() and not _same_place(q_out, q)),
+                      ("out[1] and k", pk == k.data_ptr() and not _same_place(k_out, k))):
+        if bad:
+            raise ValueError(f"{name} share memory")
+
+
 def _reject_tangents(*tensors) -> None:
     if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError("qk_norm_rotary has no forward-mode derivative")
@@ -185,7 +203,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor]
 
     Returns contiguous (B, L, Hq, D) and (B, L, Hk, D).  ``out=(q_out, k_out)``
     writes there instead (any strides with unit stride in D: a slice of a cache,
-    or the inputs themselves); it takes no part in autograd."""
+    or the inputs themselves, and no other memory that the call reads or
+    writes); it takes no part in autograd."""
     key = (q.shape, q.dtype, k.shape, k.dtype, eps, *[
         None if t is None else (t.shape, t.dtype)
         for t in (cos, sin, positions, q_weight, k_weight)])
@@ -236,6 +255,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor]
                torch.empty(k.shape, dtype=k.dtype, device=k.device))
         _forward(q, k, out[0], out[1], *rest)
     else:
+        _check_places(out[0], out[1], q, k)
         _forward(q, k, out[0], out[1], *rest)
         torch.autograd.graph.increment_version(out)
     return out[0], out[1]

@@ -801,3 +801,23 @@ def test_muon_refuses_gradients_that_it_would_overwrite():
     want, _ = plain_muon(a, a, m, 0.1, 0.95, True, 0.0, "none")
     fa.muon_step([a], [a], [m], lr=0.1, scale="none")
     assert rel(a, want) < 2e-6 and torch.equal(m, before[0])
+
+
+def test_qk_out_refuses_shared_memory():
+    q = torch.randn(2, 6, 4, 64, device="cuda")
+    k = torch.randn(2, 6, 4, 64, device="cuda")
+    o, p = torch.empty_like(q), torch.empty_like(k)
+    turned = q.view(2, 4, 6, 64).transpose(1, 2)  # q's memory in another order
+    before = q.clone(), k.clone()
+    for a, b, out in ((q, k, (o, o)), (q, k, (k, p)), (q, k, (o, q)), (q, k, (k, q)),
+                      (q, q, (q, p)), (q, q, (o, q)), (q, k, (turned, p)), (k, q, (o, turned))):
+        with pytest.raises(ValueError, match="share memory"):
+            fa.qk_norm_rotary(a, b, out=out)
+    assert torch.equal(q, before[0]) and torch.equal(k, before[1])
+    want = fa.qk_norm_rotary(q, k)
+    packed = torch.cat((q, k), 2)
+    a, b = packed[:, :, :4], packed[:, :, 4:]
+    got = fa.qk_norm_rotary(a, b, out=(a, b))  # both in place, interleaved in one buffer
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    same = fa.qk_norm_rotary(q, q, out=(o, p))  # one input twice
+    assert torch.equal(same[0], want[0]) and torch.equal(same[1], want[0])
