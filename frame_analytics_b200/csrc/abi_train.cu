@@ -9,6 +9,7 @@ int qk_impl(const fa_heads* q, const fa_heads* k, const fa_heads* gq, const fa_h
             const fa_heads* oq, const fa_heads* ok, bool backward, const fa_qk_params* pr,
             void* ws, size_t ws_bytes, void* dqw, void* dkw, int device, cudaStream_t st);
 size_t ns_ws_bytes(const fa_matrix* m, int count, int dtype);
+bool ns_shape_ok(int rows, int cols);
 int ns_check(const fa_matrix* m, int count, int dtype, bool update);
 int ns_impl(const fa_matrix* m, int count, int dtype, const double* coef, int steps, bool update,
             double mu, int nesterov, double decay, void* ws, size_t ws_bytes, int device,
@@ -57,7 +58,7 @@ FA_B200_API int fa_b200_orthogonalize_workspace_bytes(const fa_matrix* matrices,
   if (!out_bytes || !matrices || count <= 0) return FA_E_ARG;
   if (dtype != FA_F16 && dtype != FA_BF16 && dtype != FA_F32) return FA_E_DTYPE;
   for (int i = 0; i < count; ++i)
-    if (matrices[i].rows <= 0 || matrices[i].cols <= 0) return FA_E_SHAPE;
+    if (!ns_shape_ok(matrices[i].rows, matrices[i].cols)) return FA_E_SHAPE;
   *out_bytes = ns_ws_bytes(matrices, count, dtype);
   return FA_OK;
 }

@@ -1427,15 +1427,19 @@ size_t ns_ws_bytes(const fa_matrix* m, int count, int dtype) {
   return most ? up256(kNsHead) + parts + most : kNsNoWs;
 }
 
+// The longer side keeps a tile, and so a wait for one, below 0.1 s.
+bool ns_shape_ok(int rows, int cols) {
+  return std::min(rows, cols) >= 1 && std::min(rows, cols) <= 32768 &&
+         std::max(rows, cols) <= (1 << 22);
+}
+
 // Everything about a call that can be refused before the device is touched.
 int ns_check(const fa_matrix* m, int count, int dtype, bool update) {
   if (!m || count <= 0) return FA_E_ARG;
   if (dtype != FA_F16 && dtype != FA_BF16 && dtype != FA_F32) return FA_E_DTYPE;
   for (int i = 0; i < count; ++i) {
     if (!m[i].src || !m[i].dst || (update && !m[i].momentum)) return FA_E_ARG;
-    if (m[i].rows <= 0 || m[i].cols <= 0) return FA_E_SHAPE;
-    if (std::min(m[i].rows, m[i].cols) > 32768 || std::max(m[i].rows, m[i].cols) > (1 << 22))
-      return FA_E_SHAPE;
+    if (!ns_shape_ok(m[i].rows, m[i].cols)) return FA_E_SHAPE;
     if (m[i].src_row_stride < m[i].cols || m[i].dst_row_stride < m[i].cols) return FA_E_SHAPE;
   }
   return FA_OK;

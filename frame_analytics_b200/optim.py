@@ -63,6 +63,15 @@ def _coefficients(coefficients, steps: int):
     return arr
 
 
+_MAX_SHORT, _MAX_LONG = 32768, 1 << 22
+
+
+def _check_size(name: str, rows: int, cols: int) -> None:
+    if min(rows, cols) > _MAX_SHORT or max(rows, cols) > _MAX_LONG:
+        raise ValueError(f"{name} of {rows} x {cols}: the shorter side is at most {_MAX_SHORT}, "
+                         f"the longer {_MAX_LONG}")
+
+
 def _run(fn, mats, count: int, like: torch.Tensor, *args) -> None:
     L = backend.lib()
     code = backend.DTYPE_CODE[like.dtype]
@@ -84,7 +93,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5,
     float16, bfloat16 or float32 in and out; the result is contiguous.  bfloat16
     runs one tensor-core product per matrix product (about 1e-3 relative before
     the output is rounded); float16 and float32 run three (about 1e-6), and
-    matrices up to 64 x 128 run in float32.  The shorter side is at most 32768.
+    matrices up to 64 x 128 run in float32.  The shorter side is at most 32768,
+    the longer 4194304.
     ``coefficients``: a triple (a, b, c), or one for each step.  A zero matrix
     gives zeros; one that holds an infinity or a NaN gives NaN.  The result
     takes no part in autograd."""
@@ -93,9 +103,11 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5,
     if x.dtype not in _DTYPES:
         raise TypeError(f"orthogonalize takes float16, bfloat16 or float32, got {x.dtype}")
     coef = _coefficients(coefficients, steps)
+    m, n = x.shape[-2:]
+    if x.numel():
+        _check_size("a matrix", m, n)
     backend.require_cuda(x)
     x = x.detach()
-    m, n = x.shape[-2:]
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if x.numel() == 0:
         return out
@@ -194,10 +206,12 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
         if m.shape != shape or m.dtype != torch.float32:
             raise ValueError(f"momentum {i} must be float32 of shape {tuple(shape)}, got "
                              f"{m.dtype} {tuple(m.shape)}")
+        n = w.numel()
+        if n:
+            _check_size(f"weight {i}", shape[0], n // shape[0])
         if not (w.get_device() == g.get_device() == m.get_device() == index) or index < 0:
             backend.require_cuda(w, g, m)
             raise ValueError("weights, gradients and momenta must be on one device")
-        n = w.numel()
         if n == 0:
             continue
         wm, gm, mm = w, g, m

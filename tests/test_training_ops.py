@@ -185,3 +185,19 @@ def test_qk_norm_rotary_refuses_forward_mode(which):
         t[which] = fw.make_dual(t[which], torch.ones(shapes[which]))
         with pytest.raises(RuntimeError, match="forward-mode"):
             qk(**t)
+
+
+@pytest.mark.parametrize("shape", [(32769, 32769), (2, 32769, 40000), (1, (1 << 22) + 1),
+                                   (1 << 33, 4)])
+def test_matrices_past_the_limits_are_refused_before_anything_is_allocated(shape):
+    x = torch.zeros(1).expand(shape)
+    with pytest.raises(ValueError, match="at most"):
+        fa.orthogonalize(x)
+    with pytest.raises(ValueError, match="at most"):
+        fa.muon_step([x], [x], [x], lr=0.1)
+    L = _cabi.load()
+    size = ctypes.c_size_t(0)
+    m = (fa_matrix * 1)((16, 16, None, 32769, 32769, 32769, 32769, 0.1))
+    assert L.fa_b200_orthogonalize_workspace_bytes(m, 1, 3, ctypes.byref(size)) == 2
+    m[0].rows, m[0].cols = 1, (1 << 22) + 1
+    assert L.fa_b200_orthogonalize_workspace_bytes(m, 1, 3, ctypes.byref(size)) == 2
