@@ -205,6 +205,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor]
     writes there instead (any strides with unit stride in D: a slice of a cache,
     or the inputs themselves, and no other memory that the call reads or
     writes); it takes no part in autograd."""
+    eps = float(eps)
     key = (q.shape, q.dtype, k.shape, k.dtype, eps, *[
         None if t is None else (t.shape, t.dtype)
         for t in (cos, sin, positions, q_weight, k_weight)])
@@ -239,7 +240,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor]
         cos, sin = cos.contiguous(), sin.contiguous()
     q_weight = None if q_weight is None else q_weight.contiguous()
     k_weight = None if k_weight is None else k_weight.contiguous()
-    rest = (cos, sin, q_weight, k_weight, float(eps), positions, bool(interleaved))
+    rest = (cos, sin, q_weight, k_weight, eps, positions, bool(interleaved))
     if q.shape[0] == 0 or q.shape[1] == 0:
         if out is not None:
             return out[0], out[1]
@@ -248,7 +249,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, cos: Optional[torch.Tensor]
         return ((q * 1.0 + zero).to(q.dtype).contiguous(),
                 (k * 1.0 + zero).to(k.dtype).contiguous())
     if grad:
-        return _QkNormRotary.apply(q, k, q_weight, k_weight, cos, sin, float(eps), positions,
+        return _QkNormRotary.apply(q, k, q_weight, k_weight, cos, sin, eps, positions,
                                    bool(interleaved))
     if out is None:
         out = (torch.empty(q.shape, dtype=q.dtype, device=q.device),

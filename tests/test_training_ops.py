@@ -201,3 +201,11 @@ def test_matrices_past_the_limits_are_refused_before_anything_is_allocated(shape
     assert L.fa_b200_orthogonalize_workspace_bytes(m, 1, 3, ctypes.byref(size)) == 2
     m[0].rows, m[0].cols = 1, (1 << 22) + 1
     assert L.fa_b200_orthogonalize_workspace_bytes(m, 1, 3, ctypes.byref(size)) == 2
+
+
+def test_qk_norm_rotary_looks_at_eps_in_every_call():
+    eps = torch.tensor(1e-6)
+    with pytest.raises(TypeError):  # not on the GPU
+        qk(eps=eps)
+    with pytest.raises(ValueError, match="eps"):
+        qk(eps=eps.fill_(-1.0))
