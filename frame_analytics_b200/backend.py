@@ -125,7 +125,8 @@ def _luma_arg(luma) -> Optional[ctypes.Array]:
 # (device, stream) therefore serves every call issued in order on that stream;
 # it only ever grows.  Calls that may overlap on the GPU without being ordered
 # on one stream (CUDA-graph replays of different owners, say) need separate
-# buffers: private_workspaces gives an owner its own table.
+# buffers: private_workspaces gives an owner its own table, and a call that is
+# being captured outside of one gets a buffer of the graph's.
 # --------------------------------------------------------------------------- #
 
 _ws: dict = {}
@@ -152,6 +153,10 @@ def _pool() -> dict:
 
 def workspace(t: torch.Tensor, nbytes: int) -> torch.Tensor:
     pool = _pool()
+    if pool is _ws and torch.cuda.is_current_stream_capturing():
+        # Zeroed by this graph's replays, and by no others; the table's own
+        # buffer may be replaced while the graph lives.
+        return torch.zeros(max(int(nbytes), 256), dtype=torch.uint8, device=t.device)
     key = (_dev(t), _stream(t))
     buf = pool.get(key)
     if buf is None or buf.numel() < nbytes:

@@ -821,3 +821,45 @@ def test_qk_out_refuses_shared_memory():
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     same = fa.qk_norm_rotary(q, q, out=(o, p))  # one input twice
     assert torch.equal(same[0], want[0]) and torch.equal(same[1], want[0])
+
+
+def test_graphs_of_a_training_pass_replay_in_any_order():
+    """A workspace made under capture is zeroed by that graph's replays alone:
+    it must not serve another graph, nor a graph the buffer of eager calls."""
+    from frame_analytics_b200 import backend
+    q, k, cos, sin, pos, ws, gs, _ = qk_case((2, 65, 4, 2, 64, 64, False, "dim"), torch.float32)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, *ws)]
+
+    def backward():
+        out = fa.qk_norm_rotary(leaves[0], leaves[1], cos, sin, q_weight=leaves[2],
+                                k_weight=leaves[3], positions=pos)
+        return torch.autograd.grad(out, leaves, gs)
+
+    want = backward()
+    stream = torch.cuda.Stream()
+    backend._ws.pop((0, stream.cuda_stream), None)  # as on a stream that has run nothing
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            got.append(backward())
+    kept = backend._ws.get((0, stream.cuda_stream))
+    if kept is not None:  # what memory that nothing has zeroed may hold
+        kept.fill_(0x55)
+    for i in (1, 0, 1):
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got[i], want):
+            assert torch.equal(a, b)
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        backward()  # the stream has a buffer now
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        again = backward()
+    backend._ws.pop((0, stream.cuda_stream)).fill_(0x55)  # and gives it up
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
