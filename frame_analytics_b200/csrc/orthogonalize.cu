@@ -89,10 +89,11 @@ struct NsMat {
   float* mom;                      // momentum, or null
   long long src_row, dst_row;
   float step;                      // W <- decay W - step O
-  int cols, s, l, tall;            // s, l: its shorter and its longer side
-  int group;
-  int vec;                         // rows are whole aligned 16-byte vectors
-  int vec_dst;                     // the result's rows are whole aligned vectors of four
+  short cols, s, l;                // of one that fits a block; s, l: shorter, longer side
+  bool tall;
+  unsigned char group;
+  bool vec;                        // rows are whole aligned 16-byte vectors
+  bool vec_dst;                    // the result's rows are whole aligned vectors of four
 };
 
 struct NsStep {
@@ -1130,13 +1131,13 @@ __global__ void __launch_bounds__(256) ns_small_kernel(const __grid_constant__ N
   float* const B = A + kSmallS * kLdA;
   __shared__ double sm[32];
   const NsMat& m = a.m[blockIdx.x];
-  const int s = m.s, l = m.l, n = s * l;
+  const int cols = m.cols, tall = m.tall, s = m.s, l = m.l, n = s * l;
   for (int i = threadIdx.x; i < kSmallS * kLdX; i += 256) X[i] = 0.f;  // beyond s and l too
   __syncthreads();
   const T* src = reinterpret_cast<const T*>(m.src);
   double ss = 0;
   for (int i = threadIdx.x; i < n; i += 256) {
-    const int r = i / m.cols, c = i - r * m.cols;
+    const int r = i / cols, c = i - r * cols;
     float u = Ld<T>::f(src[r * m.src_row + c]);
     if (m.mom) {
       const float v = fmaf(a.mu, m.mom[i], u);
@@ -1144,7 +1145,7 @@ __global__ void __launch_bounds__(256) ns_small_kernel(const __grid_constant__ N
       u = a.nesterov ? fmaf(a.mu, v, u) : v;
     }
     ss += (double)u * u;
-    X[m.tall ? c * kLdX + r : r * kLdX + c] = u;
+    X[tall ? c * kLdX + r : r * kLdX + c] = u;
   }
   ss = block_sum(ss, sm);
   const bool finite = ss <= 1.7e308;
@@ -1222,8 +1223,8 @@ __global__ void __launch_bounds__(256) ns_small_kernel(const __grid_constant__ N
   }
   T* dst = reinterpret_cast<T*>(m.dst);
   for (int i = threadIdx.x; i < n; i += 256) {
-    const int r = i / m.cols, c = i - r * m.cols;
-    const float v = X[m.tall ? c * kLdX + r : r * kLdX + c];
+    const int r = i / cols, c = i - r * cols;
+    const float v = X[tall ? c * kLdX + r : r * kLdX + c];
     T* w = dst + r * m.dst_row + c;
     *w = St<T>::v(m.mom ? fmaf(a.decay, Ld<T>::f(*w), -m.step * v) : v);
   }
@@ -1313,6 +1314,13 @@ static void group_shape(NsGroup* g, int rows, int cols, int batch, int first) {
   g->pa = pitch64(g->s);
 }
 
+// At least a matrix's part of its group_layout.
+static size_t matrix_bytes(int rows, int cols, bool split) {
+  const int s = std::min(rows, cols), pa = pitch64(s);
+  return 4 * up256((size_t)2 * rows * pitch64(cols)) + (split ? 4 : 2) * up256((size_t)2 * s * pa) +
+         2 * up256((size_t)4 * pa);
+}
+
 // The next matrices that share a launch sequence: at most kMats, of at most
 // kGroups shapes, and of at most kMostBytes of workspace (but at least one).
 // Members of one shape are numbered together.  Matrices that fit one block are
@@ -1343,9 +1351,7 @@ static bool take_batch(const fa_matrix* m, int* next, int count, bool split, Bat
   o->groups = 0;
   for (; n < kMats && i < count; ++i) {
     if (fits_block(m[i])) continue;
-    NsGroup one{};
-    group_shape(&one, m[i].rows, m[i].cols, 1, 0);
-    bytes += group_layout(&one, split, nullptr);  // of n in one group: not more
+    bytes += matrix_bytes(m[i].rows, m[i].cols, split);
     if (n > 0 && bytes > kMostBytes) break;
     int g = 0;
     while (g < o->groups && (o->rows[g] != m[i].rows || o->cols[g] != m[i].cols)) ++g;
@@ -1590,11 +1596,13 @@ static void ns_fill(NsMat* o, const fa_matrix& f, int group, bool update, int dt
   o->src_row = f.src_row_stride;
   o->dst_row = f.dst_row_stride;
   o->step = (float)f.step;
-  o->cols = f.cols;
-  o->s = std::min(f.rows, f.cols);
-  o->l = std::max(f.rows, f.cols);
-  o->tall = f.rows > f.cols;
-  o->group = group;
+  if (fits_block(f)) {
+    o->cols = (short)f.cols;
+    o->s = (short)std::min(f.rows, f.cols);
+    o->l = (short)std::max(f.rows, f.cols);
+    o->tall = f.rows > f.cols;
+  }
+  o->group = (unsigned char)group;
   const int item = dtype == FA_F32 ? 4 : 2;
   o->vec = f.cols % 8 == 0 && reinterpret_cast<uintptr_t>(f.src) % 16 == 0 &&
            (f.rows == 1 || f.src_row_stride * item % 16 == 0) &&

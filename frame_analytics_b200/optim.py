@@ -207,8 +207,10 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
             raise ValueError(f"momentum {i} must be float32 of shape {tuple(shape)}, got "
                              f"{m.dtype} {tuple(m.shape)}")
         n = w.numel()
-        if n:
+        step = scales.get(shape)
+        if step is None and n:
             _check_size(f"weight {i}", shape[0], n // shape[0])
+            step = scales[shape] = lr * _scale(scale, shape[0], n // shape[0])
         if not (w.get_device() == g.get_device() == m.get_device() == index) or index < 0:
             backend.require_cuda(w, g, m)
             raise ValueError("weights, gradients and momenta must be on one device")
@@ -227,9 +229,6 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
             if gm is None:
                 gm = _rows_layout(torch.empty_like(w_).copy_(g.detach()))
                 keep.append(gm)
-        step = scales.get(shape)
-        if step is None:
-            step = scales[shape] = lr * _scale(scale, shape[0], n // shape[0])
         r = shape[0]
         c = n // r
         rows.append((gm.data_ptr(), wm.data_ptr(), mm.data_ptr(), r, c, c, c, step))
@@ -237,7 +236,8 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     if len(written) < 2 * len(rows):
         raise ValueError("a weight or a momentum is given twice")
     # a gradient is read again after the momenta, and other weights, are written
-    if any(row[0] in written and row[0] != row[1] for row in rows):
+    if not written.isdisjoint([row[0] for row in rows]) and any(
+            row[0] in written and row[0] != row[1] for row in rows):
         raise ValueError("a gradient is also given as a momentum or as another weight")
     if not rows:
         return
