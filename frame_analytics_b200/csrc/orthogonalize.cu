@@ -10,16 +10,18 @@
 //   M <- mu M + G,  U = G + mu M (Nesterov) or M,
 //   W <- (1 - lr wd) W - lr scale O(U).
 //
-// Three launches serve a whole list of matrices: momentum and norms, packing,
-// and one persistent kernel for all products of all steps.
+// Three launches serve up to 128 matrices of up to 8 shapes: momentum and norms,
+// packing, and one persistent kernel for all products of all steps.  Matrices
+// that fit one block have a kernel of their own.
 //
-// Measured on one B200, a call: 4096 x 8192 bfloat16 2.5 ms (0.98 PFLOP/s of
-// the products it cannot do without), 12 x 768 x 768 bfloat16 0.27 ms (0.41),
-// 2304 x 768 float32 0.27 ms (0.085, three times that in products run).  Large
-// matrices are bound by the products (0.45 us for 256 x 256 x 64 on a pair of
-// blocks), middle ones by operand bytes out of the second-level cache and the
+// Measured on one B200, a call: 4096 x 8192 bfloat16 2.7 ms (0.88 PFLOP/s of
+// the products it cannot do without, at the 1.56 GHz that the power limit leaves),
+// 12 x 768 x 768 bfloat16 0.27 ms (0.40), 2304 x 768 float32 0.26 ms (0.086,
+// three times that in products run).  Large matrices are bound by the products
+// (0.45 us for 256 x 256 x 64 on a pair of blocks) and the ends of the phases,
+// middle ones by operand bytes out of the second-level cache and the
 // ends of the phases, small ones by the latency of 15 dependent products (at
-// least 4 us each; matrices up to 64 x 128 have a kernel of their own).
+// least 4 us each).
 //
 // Number formats.  The products run on the tensor cores with float16 operands
 // and float32 accumulators; float16 has three more bits than bfloat16 at the
@@ -1394,7 +1396,9 @@ static int tile_count(const NsGroup& g, bool sym, int bm, int bn) {
 // tile's operands in and reading them out of shared memory take the rest, so
 // what counts is bytes a tile.  float32 tiles hold their sums in registers and
 // two accumulators, which leaves room for 128 columns; a pair gained nothing
-// there (2048 x 2048: 794 against 781 us).
+// there (2048 x 2048: 794 against 781 us).  With pairs and without, bfloat16, in
+// turn on one card: 4096 x 8192 2.70 and 2.99 ms, 4096 x 4096 1.61 and 1.76 ms,
+// 5 x 2100 x 1500 0.66 and 0.77 ms, 20 x 1030 x 1100 1.04 and 0.98 ms.
 struct TileTime { int bn; bool pair; double us, tail; };
 static const TileTime kTimes[2][4] = {
     {{64, false, 0.41, 3.0}, {128, false, 0.50, 6.0}, {256, false, 0.69, 12.0}, {256, true, 0.47, 15.0}},

@@ -177,8 +177,14 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
     weights' shapes) are updated; ``grads`` have the weights' dtype.  ``scale``
     s: ``"aspect"`` sqrt(max(1, rows / cols)), ``"rms"`` 0.2 sqrt(max(rows,
     cols)), ``"none"`` 1.  Contiguous tensors and channels-last kernels are used
-    where they lie, others through copies.  All matrices run through one sequence of launches,
-    whatever their shapes."""
+    where they lie, others through copies.
+
+    One sequence of launches serves up to 128 matrices of up to 8 shapes, and 2
+    GiB of workspace; longer lists take several.  Matrices up to 64 x 128 have
+    launches of 128 of their own.  The momentum is float32 whatever the weights;
+    the products are orthogonalize's for the weights' dtype, so larger bfloat16
+    weights take an update that is about 1e-3 (relative) off, beside their own
+    rounding."""
     weights, grads, momenta = list(weights), list(grads), list(momenta)
     if not len(weights) == len(grads) == len(momenta):
         raise ValueError(f"{len(weights)} weights, {len(grads)} gradients and {len(momenta)} momenta")

@@ -615,7 +615,8 @@ FA_B200_API int fa_b200_orthogonalize(const fa_matrix* matrices, int count, int 
                                       size_t workspace_bytes, int device, void* stream);
 
 /* The optimiser step: momentum <- mu momentum + src; U = src + mu momentum
- * (nesterov) or momentum; dst <- decay dst - step O(U).  Same workspace. */
+ * (nesterov) or momentum; dst <- decay dst - step O(U).  Same workspace.  No
+ * buffers overlap, but a matrix's src may be its own dst. */
 FA_B200_API int fa_b200_muon_step(const fa_matrix* matrices, int count, int dtype,
                                   const double* coefficients, int steps, double mu,
                                   int nesterov, double decay, void* workspace,
