@@ -11,12 +11,16 @@ biases and the position-free rest go to AdamW.
 from __future__ import annotations
 
 import argparse
+import sys
+from pathlib import Path
 
 import torch
 import torch.nn.functional as F
 from torch import nn
 
-import frame_analytics_b200 as fa
+sys.path.insert(0, str(Path(__file__).resolve().parents[1]))  # the package, from its checkout
+
+import frame_analytics_b200 as fa  # noqa: E402
 
 
 def angle_tables(rows: int, cols: int, rotary: int, device):

@@ -209,3 +209,16 @@ def test_qk_norm_rotary_looks_at_eps_in_every_call():
         qk(eps=eps)
     with pytest.raises(ValueError, match="eps"):
         qk(eps=eps.fill_(-1.0))
+
+
+def test_the_example_starts_from_anywhere(tmp_path):
+    import os
+    import subprocess
+    import sys
+
+    from conftest import REPO
+    env = {k: v for k, v in os.environ.items() if k != "PYTHONPATH"}
+    run = subprocess.run([sys.executable, str(REPO / "examples" / "train_restoration.py"), "--help"],
+                         cwd=tmp_path, env=env, capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr
+    assert "--steps" in run.stdout
