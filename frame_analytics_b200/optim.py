@@ -239,7 +239,8 @@ def muon_step(weights: Sequence[torch.Tensor], grads: Sequence[torch.Tensor],
         c = n // r
         rows.append((gm.data_ptr(), wm.data_ptr(), mm.data_ptr(), r, c, c, c, step))
     written = {p for row in rows for p in row[1:3]}
-    if len(written) < 2 * len(rows):
+    written.update([t.data_ptr() for t, _ in back])
+    if len(written) < 2 * len(rows) + len(back):
         raise ValueError("a weight or a momentum is given twice")
     # a gradient is read again after the momenta, and other weights, are written
     if not written.isdisjoint([row[0] for row in rows]) and any(

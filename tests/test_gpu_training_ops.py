@@ -863,3 +863,13 @@ def test_graphs_of_a_training_pass_replay_in_any_order():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+def test_muon_refuses_strided_tensors_given_twice():
+    a, b = (torch.randn(9, 8, device="cuda").t() for _ in range(2))
+    g, m, n = (torch.zeros(8, 9, device="cuda") for _ in range(3))
+    before = a.clone()
+    for ws, ms in (([a, a], [m, n]), ([a, b], [b, m]), ([g, n], [a, a]), ([a, g], [m, a])):
+        with pytest.raises(ValueError, match="twice"):
+            fa.muon_step(ws, [torch.ones_like(w) for w in ws], ms, lr=0.1)
+    assert torch.equal(a, before) and bool((m == 0).all())
