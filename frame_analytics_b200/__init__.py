@@ -6,7 +6,9 @@ A drop-in for the metric path of frame_analytics: ``psnr``, ``mse``, ``l1``,
 computed by hand-written CUDA kernels behind a C ABI (``include/fa_b200.h``).
 
 Around the losses, for networks trained against them: ``qk_norm_rotary``
-(attention operands), ``orthogonalize``, ``muon_step`` and ``Muon`` (weight updates).
+(attention operands), ``layer_norm``, ``gelu8``, ``linear8``, ``pack8`` and ``unpack8``
+(a block's operators with activations kept in 8 bits), ``orthogonalize``,
+``muon_step`` and ``Muon`` (weight updates).
 
 >>> import torch, frame_analytics_b200 as fa
 >>> a = torch.randint(0, 256, (8, 3, 1080, 1920), dtype=torch.uint8, device="cuda")
@@ -35,6 +37,7 @@ from .functional import (  # noqa: F401
 from . import planes  # noqa: F401
 from .ssimulacra2 import SSIMULACRA2, ssimulacra2  # noqa: F401
 from .attention import qk_norm_rotary  # noqa: F401
+from .block import Packed8, gelu8, layer_norm, linear8, pack8, unpack8  # noqa: F401
 from .optim import Muon, muon_step, orthogonalize  # noqa: F401
 from .modules import (GMSD, L1, MSE, MSSSIM, PSNR, SSIM, Charbonnier, Huber,  # noqa: F401
                       StreamingMetrics)
@@ -48,6 +51,7 @@ __all__ = [
     "MSE", "PSNR", "SSIM", "MSSSIM", "GMSD", "L1", "Charbonnier", "Huber",
     "ssimulacra2", "SSIMULACRA2", "backend_status",
     "qk_norm_rotary", "orthogonalize", "muon_step", "Muon",
+    "layer_norm", "gelu8", "linear8", "pack8", "unpack8", "Packed8",
 ]
 
 

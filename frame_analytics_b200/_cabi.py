@@ -106,6 +106,28 @@ class fa_matrix(ctypes.Structure):
     ]
 
 
+class fa_norm(ctypes.Structure):
+    """Mirror of ``struct fa_norm`` in include/fa_b200.h."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("rows", ctypes.c_int64),
+        ("width", ctypes.c_int32),
+        ("pad_", ctypes.c_int32),
+        ("eps", ctypes.c_double),
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("residual", ctypes.c_void_p),
+        ("residual_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("codes", ctypes.c_void_p),
+        ("ranges", ctypes.c_void_p),
+    ]
+
+
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
@@ -188,6 +210,16 @@ PROTOTYPES = {
     "fa_b200_orthogonalize": [_vp, _i, _i, _vp, _i, _vp, _sz, _i, _vp],
     "fa_b200_muon_step": [_vp, _i, _i, _vp, _i, _d, _i, _d, _vp, _sz, _i, _vp],
     "fa_b200_orthogonalize_wait_limit": [ctypes.c_ulonglong],
+    "fa_b200_pack8": [_vp, _i64, _i, _i64, _i, _vp, _vp, _i, _vp],
+    "fa_b200_unpack8": [_vp, _vp, _i, _i64, _i, _vp, _i64, _i, _vp],
+    "fa_b200_gelu8": [_vp, _i64, _i, _i64, _i, _i, _vp, _vp, _vp, _i, _vp],
+    "fa_b200_gelu8_backward": [_vp, _i64, _vp, _vp, _i, _i64, _i, _i, _vp, _i, _vp],
+    "fa_b200_layer_norm": [_vp, _vp, _vp, _i, _vp],
+    "fa_b200_layer_norm_backward_workspace_bytes": [_i64, _i, _i, _vp],
+    "fa_b200_layer_norm_backward": [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _i, _vp],
+    "fa_b200_linear8_weight_grad_workspace_bytes": [_i64, _i, _i, _i, _i, _vp],
+    "fa_b200_linear8_weight_grad": [_vp, _i64, _vp, _vp, _i, _i64, _i, _i, _vp, _vp, _vp, _sz,
+                                    _i, _vp],
     "fa_b200_ssim_gmsd": [_pview, _pview, _vp, _i, _d, _d, _d, _d, _d, _d, _vp, _sz,
                           _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp],
 }

@@ -1,0 +1,413 @@
+"""A transformer block's norm, activation and products with what they keep for the
+backward pass in 8 bits (no counterpart in the reference; ``csrc/keep8.cu``,
+``csrc/layer_norm.cu``, ``csrc/wgrad8.cu``).
+
+A network that restores whole frames keeps the input of every norm, activation
+and product until its gradient comes back; these inputs, not the weights, fill
+the memory.  ``pack8`` holds them at 1.06 bytes a value, and ``layer_norm``,
+``gelu8`` and ``linear8`` read that form in their backward passes without
+unpacking it first.
+"""
+
+from __future__ import annotations
+
+import math
+import struct
+from typing import NamedTuple, Optional, Tuple, Union
+
+import torch
+import torch.nn.functional as F
+from torch.autograd import forward_ad
+
+from . import backend
+from .functional import _reject_double_backward
+
+__all__ = ["Packed8", "pack8", "unpack8", "layer_norm", "gelu8", "linear8"]
+
+_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+_GROUP = 64
+_MAX_WIDTH = 1 << 24
+# struct fa_norm of include/fa_b200.h as bytes
+_NORM = struct.Struct("@2iq2idPqPq5P").pack
+
+
+class Packed8(NamedTuple):
+    """A tensor in 8 bits, made by :func:`pack8`.
+
+    ``codes``: uint8 (..., 64 G), G groups of 64 along the last dimension, zeros
+    past its end.  ``ranges``: each group's lowest value and step, int32 (..., G)
+    for 16-bit tensors (the lowest value in the low half, the step as bfloat16 in
+    the high half), float32 (..., G, 2) for float32.  ``shape`` and ``dtype`` are
+    the tensor's own."""
+
+    codes: torch.Tensor
+    ranges: torch.Tensor
+    shape: torch.Size
+    dtype: torch.dtype
+
+
+def _check_values(name: str, x: torch.Tensor, most: int) -> None:
+    if not torch.is_tensor(x):
+        raise TypeError(f"{name} must be a tensor, got {type(x).__name__}")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be float16, bfloat16 or float32, got {x.dtype}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= most:
+        raise ValueError(f"{name} must have a last dimension of 1..{most}, got shape "
+                         f"{tuple(x.shape)}")
+
+
+def _on_one_device(x: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    index = x.get_device()
+    for t in (x, *others):
+        if t is not None and (t.get_device() != index or index < 0):
+            backend.require_cuda(*[u for u in (x, *others) if u is not None])
+            raise ValueError("all tensors must be on one device")
+
+
+def _reject_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{name} has no forward-mode derivative")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """As a matrix of rows with unit stride; a copy where that takes one."""
+    width = t.shape[-1]
+    if t.stride(-1) != 1 and width > 1:
+        t = t.contiguous()
+    return t.reshape(-1, width)
+
+
+def _packed_like(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    lead, groups = x.shape[:-1], -(-x.shape[-1] // _GROUP)
+    codes = torch.empty((*lead, groups * _GROUP), dtype=torch.uint8, device=x.device)
+    if x.dtype == torch.float32:
+        return codes, torch.empty((*lead, groups, 2), dtype=torch.float32, device=x.device)
+    return codes, torch.empty((*lead, groups), dtype=torch.int32, device=x.device)
+
+
+# --------------------------------------------------------------------------- #
+# packing
+# --------------------------------------------------------------------------- #
+
+def _pack(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    codes, ranges = _packed_like(x)
+    if x.numel():
+        r = _rows(x)
+        backend._call(r, backend.lib().fa_b200_pack8, r.data_ptr(), r.stride(0),
+                      backend.DTYPE_CODE[x.dtype], r.shape[0], r.shape[1], codes.data_ptr(),
+                      ranges.data_ptr(), backend._dev(r), backend._stream(r))
+    return codes, ranges
+
+
+def pack8(x: torch.Tensor) -> Packed8:
+    """A tensor (float16, bfloat16 or float32, any strides) in 8 bits.
+
+    Groups of 64 values of the last dimension (the last group may be short) hold
+    their lowest value ``lo``, a step ``s`` (the smallest power of two, from
+    2^-126 up, with ``max - lo <= 255 s``) and codes ``rint((x - lo) / s)`` of 8
+    bits.  A value comes back as ``code s + lo``, at most ``(max - lo) / 255`` off
+    (before it is rounded to the dtype).  A group that holds an infinity or a NaN,
+    or whose spread is past float32's range, comes back as NaNs.  Takes no part
+    in autograd."""
+    _check_values("x", x, 2 ** 31 - 1)
+    backend.require_cuda(x)
+    return Packed8(*_pack(x.detach()), x.shape, x.dtype)
+
+
+def _check_packed(p: Packed8) -> None:
+    if not isinstance(p, Packed8):
+        raise TypeError(f"unpack8 takes what pack8 returns, got {type(p).__name__}")
+    if p.dtype not in _DTYPES or len(p.shape) < 1 or p.shape[-1] < 1:
+        raise ValueError(f"no packed tensor of shape {tuple(p.shape)} and {p.dtype}")
+    lead, groups = tuple(p.shape[:-1]), -(-p.shape[-1] // _GROUP)
+    wide = p.dtype == torch.float32
+    for name, t, shape, dtype in (
+            ("codes", p.codes, (*lead, groups * _GROUP), torch.uint8),
+            ("ranges", p.ranges, (*lead, groups, 2) if wide else (*lead, groups),
+             torch.float32 if wide else torch.int32)):
+        if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {dtype} of shape {shape}, got {t.dtype} "
+                             f"{tuple(t.shape)}")
+
+
+def unpack8(p: Packed8) -> torch.Tensor:
+    """The values that a packed tensor stands for, contiguous, in its dtype."""
+    _check_packed(p)
+    codes, ranges = p.codes.detach(), p.ranges.detach()
+    _on_one_device(codes, ranges)
+    out = torch.empty(tuple(p.shape), dtype=p.dtype, device=codes.device)
+    if out.numel():
+        # a buffer that was moved may start anywhere
+        codes = codes if codes.data_ptr() % 16 == 0 else codes.clone()
+        ranges = ranges if ranges.data_ptr() % 8 == 0 else ranges.clone()
+        width = p.shape[-1]
+        backend._call(out, backend.lib().fa_b200_unpack8, codes.data_ptr(), ranges.data_ptr(),
+                      backend.DTYPE_CODE[p.dtype], out.numel() // width, width, out.data_ptr(),
+                      width, backend._dev(out), backend._stream(out))
+    return out
+
+
+# --------------------------------------------------------------------------- #
+# layer norm
+# --------------------------------------------------------------------------- #
+
+def _norm_params(x, residual, weight, bias, eps, stats, codes, ranges, like) -> bytes:
+    """`x` and `residual`: rows; `like`: a tensor of the rows' shape and dtype."""
+    w = weight if weight is not None else bias
+    width = like.shape[-1]
+    code = backend.DTYPE_CODE[like.dtype]
+    return _NORM(code, code if w is None else backend.DTYPE_CODE[w.dtype],
+                 like.numel() // width, width, 0, eps,
+                 0 if x is None else x.data_ptr(), width if x is None else x.stride(0),
+                 0 if residual is None else residual.data_ptr(),
+                 0 if residual is None else residual.stride(0),
+                 0 if weight is None else weight.data_ptr(),
+                 0 if bias is None else bias.data_ptr(),
+                 0 if stats is None else stats.data_ptr(),
+                 0 if codes is None else codes.data_ptr(),
+                 0 if ranges is None else ranges.data_ptr())
+
+
+def _norm_forward(x, residual, weight, bias, eps, stats, codes, ranges):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    total = None if residual is None else torch.empty_like(y)
+    xr, rr = _rows(x), None if residual is None else _rows(residual)
+    p = _norm_params(xr, rr, weight, bias, eps, stats, codes, ranges, y)
+    backend._call(y, backend.lib().fa_b200_layer_norm, p, y.data_ptr(), backend._ptr(total),
+                  backend._dev(y), backend._stream(y))
+    return y, total
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, bias, eps, keep8):
+        ctx.set_materialize_grads(False)
+        stats = torch.empty((x.numel() // x.shape[-1], 2), dtype=torch.float32, device=x.device)
+        codes, ranges = _packed_like(x) if keep8 else (None, None)
+        y, total = _norm_forward(x, residual, weight, bias, eps, stats, codes, ranges)
+        kept = None if keep8 else (x if residual is None else total)
+        ctx.save_for_backward(kept, codes, ranges, stats, weight, bias)
+        ctx.eps = eps
+        return y if residual is None else (y, total)
+
+    @staticmethod
+    def backward(ctx, gy, gsum=None):
+        _reject_double_backward()
+        need = ctx.needs_input_grad
+        if gy is None:  # the norm itself took no part
+            return (gsum if need[0] else None, gsum if need[1] else None, None, None, None, None)
+        kept, codes, ranges, stats, weight, bias = ctx.saved_tensors
+        width = gy.shape[-1]
+        dx = torch.empty(gy.shape, dtype=gy.dtype, device=gy.device)
+        dw = torch.empty_like(weight) if weight is not None and need[2] else None
+        db = torch.empty_like(bias) if bias is not None and need[3] else None
+        g = _rows(gy)
+        s = None if gsum is None else _rows(gsum)
+        L = backend.lib()
+        ws, size = None, 0
+        if dw is not None or db is not None:
+            size = backend._cached_ws("norm", L.fa_b200_layer_norm_backward_workspace_bytes,
+                                      g.shape[0], width, backend._dev(g))
+            ws = torch.empty(size, dtype=torch.uint8, device=g.device)
+        p = _norm_params(None if kept is None else _rows(kept), None, weight, bias, ctx.eps, stats,
+                         codes, ranges, dx)
+        backend._call(g, L.fa_b200_layer_norm_backward, p, g.data_ptr(), g.stride(0),
+                      backend._ptr(s), 0 if s is None else s.stride(0), dx.data_ptr(),
+                      backend._ptr(dw), backend._ptr(db), backend._ptr(ws), size, backend._dev(g),
+                      backend._stream(g))
+        return dx if need[0] else None, dx if need[1] else None, dw, db, None, None
+
+
+def _check_affine(name: str, w: Optional[torch.Tensor], x: torch.Tensor) -> None:
+    if w is None:
+        return
+    if w.dtype not in (x.dtype, torch.float32):
+        raise TypeError(f"{name} must be {x.dtype} or float32, got {w.dtype}")
+    if tuple(w.shape) != (x.shape[-1],):
+        raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(w.shape)}")
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, *,
+               residual: Optional[torch.Tensor] = None, eps: float = 1e-5, keep8: bool = False
+               ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Layer norm over the last dimension, ``(x - mean) / sqrt(variance + eps) *
+    weight + bias``; differentiable once, in reverse mode.
+
+    With ``residual`` (``x``'s shape and dtype) the norm is that of ``s = x +
+    residual``, rounded to the dtype, and the call returns ``(y, s)``: the block's
+    residual sum costs no pass of its own, forward or backward.
+
+    ``x`` (..., N): float16, bfloat16 or float32, any strides; N at most 2^24.
+    ``weight`` and ``bias``, either or both: (N,), one dtype, ``x``'s or float32.
+    Results are contiguous.  Mean, variance and the weights' gradients are
+    summed in float32, in an order that does not change from run to run.
+
+    ``keep8``: keep ``x`` (or ``s``) for the backward pass as :func:`pack8` holds
+    it, with the exact mean and deviation, instead of itself."""
+    _check_values("x", x, _MAX_WIDTH)
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError(f"residual must be {x.dtype} of shape {tuple(x.shape)}, got "
+                         f"{residual.dtype} {tuple(residual.shape)}")
+    _check_affine("weight", weight, x)
+    _check_affine("bias", bias, x)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("weight and bias must have one dtype")
+    eps = float(eps)
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    _reject_tangents("layer_norm", x, residual, weight, bias)
+    _on_one_device(x, residual, weight, bias)
+    if weight is not None:
+        weight = weight.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    if x.numel() == 0:
+        # connected to the graph, so that a backward gives zero gradients
+        y = (x if residual is None else x + residual) * 1.0
+        for w in (weight, bias):
+            y = y if w is None else y + (w.sum() * 0).to(y.dtype)
+        return y if residual is None else (y, x + residual)
+    if torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (x, residual, weight, bias)):
+        return _LayerNorm.apply(x, residual, weight, bias, eps, bool(keep8))
+    y, total = _norm_forward(x, residual, weight, bias, eps, None, None, None)
+    return y if residual is None else (y, total)
+
+
+# --------------------------------------------------------------------------- #
+# activation
+# --------------------------------------------------------------------------- #
+
+def _gelu_forward(x, tanh_form, codes, ranges):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    r = _rows(x)
+    backend._call(r, backend.lib().fa_b200_gelu8, r.data_ptr(), r.stride(0),
+                  backend.DTYPE_CODE[x.dtype], r.shape[0], r.shape[1], tanh_form, y.data_ptr(),
+                  backend._ptr(codes), backend._ptr(ranges), backend._dev(r), backend._stream(r))
+    return y
+
+
+class _Gelu8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, tanh_form):
+        codes, ranges = _packed_like(x)
+        y = _gelu_forward(x, tanh_form, codes, ranges)
+        ctx.save_for_backward(codes, ranges)
+        ctx.tanh_form = tanh_form
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        _reject_double_backward()
+        codes, ranges = ctx.saved_tensors
+        dx = torch.empty(gy.shape, dtype=gy.dtype, device=gy.device)
+        g = _rows(gy)
+        backend._call(g, backend.lib().fa_b200_gelu8_backward, g.data_ptr(), g.stride(0),
+                      codes.data_ptr(), ranges.data_ptr(), backend.DTYPE_CODE[gy.dtype],
+                      g.shape[0], g.shape[1], ctx.tanh_form, dx.data_ptr(), backend._dev(g),
+                      backend._stream(g))
+        return dx, None
+
+
+def gelu8(x: torch.Tensor, *, approximate: str = "none") -> torch.Tensor:
+    """``x Phi(x)``, or with ``approximate="tanh"`` ``x (1 + tanh(sqrt(2 / pi) (x +
+    0.044715 x^3))) / 2``; the backward pass takes the slope at the values that
+    :func:`pack8` keeps of ``x``, so ``x`` itself need not be kept.  Differentiable
+    once, in reverse mode.
+
+    ``x``: float16, bfloat16 or float32, any strides; the result is contiguous.
+    The value is that of ``x`` itself."""
+    _check_values("x", x, 2 ** 31 - 1)
+    if approximate not in ("none", "tanh"):
+        raise ValueError(f"approximate must be 'none' or 'tanh', got {approximate!r}")
+    _reject_tangents("gelu8", x)
+    backend.require_cuda(x)
+    if x.numel() == 0:
+        return x * 1.0
+    tanh_form = int(approximate == "tanh")
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Gelu8.apply(x, tanh_form)
+    return _gelu_forward(x, tanh_form, None, None)
+
+
+# --------------------------------------------------------------------------- #
+# products
+# --------------------------------------------------------------------------- #
+
+def _weight_grad(g, codes, ranges, inputs: int, need_weight: bool, need_bias: bool):
+    """``g``: rows of the gradient."""
+    rows, outputs = g.shape
+    code = backend.DTYPE_CODE[g.dtype]
+    dw = torch.empty((outputs, inputs), dtype=g.dtype, device=g.device) if need_weight else None
+    db = torch.empty(outputs, dtype=g.dtype, device=g.device) if need_bias else None
+    L = backend.lib()
+    size = backend._cached_ws("wgrad8", L.fa_b200_linear8_weight_grad_workspace_bytes, rows,
+                              inputs, outputs, code, backend._dev(g))
+    ws = torch.empty(size, dtype=torch.uint8, device=g.device)
+    backend._call(g, L.fa_b200_linear8_weight_grad, g.data_ptr(), g.stride(0),
+                  backend._ptr(codes), backend._ptr(ranges), code, rows, inputs, outputs,
+                  backend._ptr(dw), backend._ptr(db), ws.data_ptr(), size, backend._dev(g),
+                  backend._stream(g))
+    return dw, db
+
+
+class _Linear8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        y = F.linear(x, weight, bias)
+        codes, ranges = _pack(x) if ctx.needs_input_grad[1] else (None, None)
+        ctx.save_for_backward(codes, ranges, weight)
+        return y
+
+    @staticmethod
+    def backward(ctx, gy):
+        _reject_double_backward()
+        codes, ranges, weight = ctx.saved_tensors
+        need, inputs = ctx.needs_input_grad, weight.shape[1]
+        g = _rows(gy)
+        dx = dw = db = None
+        if need[0]:
+            with torch.autocast("cuda", enabled=False):
+                dx = torch.matmul(g, weight).view(*gy.shape[:-1], inputs)
+        if need[1] or need[2]:
+            dw, db = _weight_grad(g, codes, ranges, inputs, need[1], need[2])
+        return dx, dw, db
+
+
+def linear8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None
+            ) -> torch.Tensor:
+    """``x W^T + bias`` that keeps ``x`` for the backward pass as :func:`pack8`
+    holds it: the weight's gradient ``dy^T x`` is a product of this package's own
+    that takes ``x`` from the 8-bit form inside (float16 and bfloat16 on the
+    tensor cores); the bias's gradient comes with it.  The value and the gradient
+    of ``x`` are torch's products of the operands themselves.  Differentiable
+    once, in reverse mode.
+
+    ``x`` (..., K), ``weight`` (M, K), ``bias`` (M,): one dtype, float16, bfloat16
+    or float32 (under autocast its dtype), any strides; K and M at most 4194303.
+    ``x`` is packed only where the weight wants a gradient."""
+    if torch.is_autocast_enabled("cuda"):
+        to = torch.get_autocast_dtype("cuda")
+        if to in _DTYPES:
+            x, weight, bias = (t.to(to) if torch.is_tensor(t) and t.dtype in _DTYPES else t
+                               for t in (x, weight, bias))
+    _check_values("x", x, (1 << 22) - 1)
+    if not torch.is_tensor(weight) or weight.dim() != 2 or weight.shape[1] != x.shape[-1] \
+            or weight.dtype != x.dtype:
+        raise ValueError(f"weight must be {x.dtype} of shape (M, {x.shape[-1]}), got "
+                         f"{getattr(weight, 'dtype', type(weight))} "
+                         f"{tuple(getattr(weight, 'shape', ()))}")
+    outputs = weight.shape[0]
+    if not 1 <= outputs < 1 << 22:
+        raise ValueError(f"the weight must have 1..{(1 << 22) - 1} rows, got {outputs}")
+    if bias is not None and (tuple(bias.shape) != (outputs,) or bias.dtype != x.dtype):
+        raise ValueError(f"bias must be {x.dtype} of shape ({outputs},), got {bias.dtype} "
+                         f"{tuple(bias.shape)}")
+    _reject_tangents("linear8", x, weight, bias)
+    _on_one_device(x, weight, bias)
+    if x.numel() == 0 or not torch.is_grad_enabled() or not (
+            weight.requires_grad or x.requires_grad or bias is not None and bias.requires_grad):
+        return F.linear(x, weight, bias)
+    return _Linear8.apply(x, weight, bias)

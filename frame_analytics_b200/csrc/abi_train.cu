@@ -1,5 +1,6 @@
 // extern "C" boundary of the training-step operators: the same conventions as
-// abi.cu (host-side checks, the caller's buffers, device and stream).
+// abi.cu (host-side checks, the caller's buffers, device and stream).  The 8-bit
+// operators check their arguments before they look for the device.
 #include "common.cuh"
 
 namespace fab {
@@ -15,6 +16,24 @@ int ns_impl(const fa_matrix* m, int count, int dtype, const double* coef, int st
             double mu, int nesterov, double decay, void* ws, size_t ws_bytes, int device,
             cudaStream_t st);
 int ns_wait_limit(unsigned long long limit_ns);
+int pack8_impl(const void* x, long long x_row, void* codes, void* ranges, int dtype,
+               long long rows, int width, int device, cudaStream_t st);
+int unpack8_impl(const void* codes, const void* ranges, void* y, long long y_row, int dtype,
+                 long long rows, int width, int device, cudaStream_t st);
+int gelu8_impl(const void* x, long long x_row, void* y, void* codes, void* ranges, int tanh_form,
+               int dtype, long long rows, int width, int device, cudaStream_t st);
+int gelu8_backward_impl(const void* g, long long g_row, const void* codes, const void* ranges,
+                        void* dx, int tanh_form, int dtype, long long rows, int width, int device,
+                        cudaStream_t st);
+size_t norm_ws_bytes(long long rows, int width, int device);
+int norm_impl(const fa_norm* p, void* y, void* sum, int device, cudaStream_t st);
+int norm_backward_impl(const fa_norm* p, const void* dy, long long dy_row, const void* ds,
+                       long long ds_row, void* dx, void* dw, void* db, void* ws, size_t ws_bytes,
+                       int device, cudaStream_t st);
+size_t wgrad8_ws_bytes(long long rows, int inputs, int outputs, int dtype, int device);
+int wgrad8_impl(const void* dy, long long dy_row, const void* codes, const void* ranges, int dtype,
+                long long rows, int inputs, int outputs, void* dw, void* db, void* ws,
+                size_t ws_bytes, int device, cudaStream_t st);
 
 }  // namespace fab
 
@@ -86,6 +105,80 @@ FA_B200_API int fa_b200_muon_step(const fa_matrix* matrices, int count, int dtyp
 
 FA_B200_API int fa_b200_orthogonalize_wait_limit(unsigned long long limit_ns) {
   return ns_wait_limit(limit_ns);
+}
+
+FA_B200_API int fa_b200_pack8(const void* x, int64_t x_stride, int dtype, int64_t rows, int width,
+                              void* codes, void* ranges, int device, void* stream) {
+  FAB_PENDING();
+  return pack8_impl(x, x_stride, codes, ranges, dtype, rows, width, device,
+                    static_cast<cudaStream_t>(stream));
+}
+
+FA_B200_API int fa_b200_unpack8(const void* codes, const void* ranges, int dtype, int64_t rows,
+                                int width, void* out, int64_t out_stride, int device,
+                                void* stream) {
+  FAB_PENDING();
+  return unpack8_impl(codes, ranges, out, out_stride, dtype, rows, width, device,
+                      static_cast<cudaStream_t>(stream));
+}
+
+FA_B200_API int fa_b200_gelu8(const void* x, int64_t x_stride, int dtype, int64_t rows, int width,
+                              int tanh_form, void* y, void* codes, void* ranges, int device,
+                              void* stream) {
+  FAB_PENDING();
+  return gelu8_impl(x, x_stride, y, codes, ranges, tanh_form, dtype, rows, width, device,
+                    static_cast<cudaStream_t>(stream));
+}
+
+FA_B200_API int fa_b200_gelu8_backward(const void* dy, int64_t dy_stride, const void* codes,
+                                       const void* ranges, int dtype, int64_t rows, int width,
+                                       int tanh_form, void* dx, int device, void* stream) {
+  FAB_PENDING();
+  return gelu8_backward_impl(dy, dy_stride, codes, ranges, dx, tanh_form, dtype, rows, width,
+                             device, static_cast<cudaStream_t>(stream));
+}
+
+FA_B200_API int fa_b200_layer_norm(const fa_norm* params, void* y, void* sum, int device,
+                                   void* stream) {
+  FAB_PENDING();
+  return norm_impl(params, y, sum, device, static_cast<cudaStream_t>(stream));
+}
+
+FA_B200_API int fa_b200_layer_norm_backward_workspace_bytes(int64_t rows, int width, int device,
+                                                            size_t* out_bytes) {
+  if (!out_bytes) return FA_E_ARG;
+  if (rows <= 0 || width <= 0 || width > (1 << 24)) return FA_E_SHAPE;
+  *out_bytes = norm_ws_bytes(rows, width, device);
+  return FA_OK;
+}
+
+FA_B200_API int fa_b200_layer_norm_backward(const fa_norm* params, const void* dy,
+                                            int64_t dy_stride, const void* ds, int64_t ds_stride,
+                                            void* dx, void* dweight, void* dbias, void* workspace,
+                                            size_t workspace_bytes, int device, void* stream) {
+  FAB_PENDING();
+  return norm_backward_impl(params, dy, dy_stride, ds, ds_stride, dx, dweight, dbias, workspace,
+                            workspace_bytes, device, static_cast<cudaStream_t>(stream));
+}
+
+FA_B200_API int fa_b200_linear8_weight_grad_workspace_bytes(int64_t rows, int inputs, int outputs,
+                                                            int dtype, int device,
+                                                            size_t* out_bytes) {
+  if (!out_bytes) return FA_E_ARG;
+  if (dtype != FA_F16 && dtype != FA_BF16 && dtype != FA_F32) return FA_E_DTYPE;
+  if (rows <= 0 || inputs <= 0 || outputs <= 0) return FA_E_SHAPE;
+  *out_bytes = wgrad8_ws_bytes(rows, inputs, outputs, dtype, device);
+  return FA_OK;
+}
+
+FA_B200_API int fa_b200_linear8_weight_grad(const void* dy, int64_t dy_stride, const void* codes,
+                                            const void* ranges, int dtype, int64_t rows,
+                                            int inputs, int outputs, void* dweight, void* dbias,
+                                            void* workspace, size_t workspace_bytes, int device,
+                                            void* stream) {
+  FAB_PENDING();
+  return wgrad8_impl(dy, dy_stride, codes, ranges, dtype, rows, inputs, outputs, dweight, dbias,
+                     workspace, workspace_bytes, device, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -627,6 +627,81 @@ FA_B200_API int fa_b200_muon_step(const fa_matrix* matrices, int count, int dtyp
  * the most (FA_E_ARG).  A launch may last longer than the limit of its waits. */
 FA_B200_API int fa_b200_orthogonalize_wait_limit(unsigned long long limit_ns);
 
+/* Activations in 8 bits.  Rows of `width` values of dtype FA_F16, FA_BF16 or
+ * FA_F32 (unit stride; row strides in elements) in groups of 64 along the row,
+ * the last possibly short, G = ceil(width / 64) a row.  A group is its lowest
+ * value lo, a power of two s (the smallest from 2^-126 up with max - min <= 255 s)
+ * and a code of 8 bits a value, which stands for code * s + lo rounded to the
+ * dtype; a group whose spread is not finite stands for NaNs.
+ *   codes:  uint8 [rows][64 G], 16-byte aligned, zeros past the width;
+ *   ranges: [rows][G], 8-byte aligned: for 16-bit dtypes a word with lo in the low
+ *           half and s as bfloat16 in the high half, for FA_F32 the floats lo, s.
+ * The buffers of a call do not overlap, unless an entry says so. */
+FA_B200_API int fa_b200_pack8(const void* x, int64_t x_stride, int dtype, int64_t rows, int width,
+                              void* codes, void* ranges, int device, void* stream);
+FA_B200_API int fa_b200_unpack8(const void* codes, const void* ranges, int dtype, int64_t rows,
+                                int width, void* out, int64_t out_stride, int device,
+                                void* stream);
+
+/* gelu: y = x Phi(x), or with tanh_form x (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) / 2.
+ * y is contiguous.  With codes and ranges x is packed too (null: not).  The
+ * gradient dx = dy gelu'(x) takes x from its packed copy; dx is contiguous. */
+FA_B200_API int fa_b200_gelu8(const void* x, int64_t x_stride, int dtype, int64_t rows, int width,
+                              int tanh_form, void* y, void* codes, void* ranges, int device,
+                              void* stream);
+FA_B200_API int fa_b200_gelu8_backward(const void* dy, int64_t dy_stride, const void* codes,
+                                       const void* ranges, int dtype, int64_t rows, int width,
+                                       int tanh_form, void* dx, int device, void* stream);
+
+/* Layer norm over rows of `width`:  s = x + residual rounded to dtype,
+ * y = (s - mean) / sqrt(variance + eps) * weight + bias.  residual, weight and
+ * bias may be null; the latter two have weight_dtype (dtype or FA_F32).  stats:
+ * float32 [rows][2], mean and 1 / deviation of every row.  Strides in elements;
+ * width at most 2^24. */
+typedef struct fa_norm {
+  int32_t dtype, weight_dtype;
+  int64_t rows;
+  int32_t width, pad_;
+  double eps;
+  const void* x;
+  int64_t x_stride;
+  const void* residual;
+  int64_t residual_stride;
+  const void* weight;
+  const void* bias;
+  float* stats;
+  void* codes;
+  void* ranges;
+} fa_norm;
+
+/* y, and sum (s; may be null), are contiguous.  stats and codes/ranges (s packed)
+ * are written where they are not null. */
+FA_B200_API int fa_b200_layer_norm(const fa_norm* params, void* y, void* sum, int device,
+                                   void* stream);
+
+/* Gradient: x is s, or codes/ranges its packed copy (then x is not read); stats as
+ * written forward.  dx = gradient of s, with ds (the gradient of the sum output, or
+ * null) added; dweight and dbias in weight_dtype, null to skip.  Workspace: 16-byte
+ * aligned, needs no zeroing, only for dweight or dbias. */
+FA_B200_API int fa_b200_layer_norm_backward_workspace_bytes(int64_t rows, int width, int device,
+                                                            size_t* out_bytes);
+FA_B200_API int fa_b200_layer_norm_backward(const fa_norm* params, const void* dy,
+                                            int64_t dy_stride, const void* ds, int64_t ds_stride,
+                                            void* dx, void* dweight, void* dbias, void* workspace,
+                                            size_t workspace_bytes, int device, void* stream);
+
+/* Weight gradient of y = x W^T + b from the packed copy of x [rows][inputs]:
+ * dweight [outputs][inputs] = dy^T x (null: not computed), dbias [outputs] = column
+ * sums of dy (null: not computed).  Workspace: 256-byte aligned, needs no zeroing. */
+FA_B200_API int fa_b200_linear8_weight_grad_workspace_bytes(int64_t rows, int inputs, int outputs,
+                                                            int dtype, int device,
+                                                            size_t* out_bytes);
+FA_B200_API int fa_b200_linear8_weight_grad(const void* dy, int64_t dy_stride, const void* codes,
+                                            const void* ranges, int dtype, int64_t rows,
+                                            int inputs, int outputs, void* dweight, void* dbias,
+                                            void* workspace, size_t workspace_bytes, int device,
+                                            void* stream);
+
 /* No counterpart in the reference: test hook of the bounded device-side
  * waits.  Launches one thread that waits `limit_ns` (at most 1 s) for an
  * mbarrier phase that nothing completes and then records FA_E_TIMEOUT the

@@ -1,0 +1,804 @@
+"""The 8-bit block operators on the GPU, against plain float64 formulas.
+
+Tolerances: u is half a step of the output's type relative to a value (2^-24,
+2^-11, 2^-8 for float32, float16, bfloat16); each output is rounded once.  Behind
+it stand float32 sums: a thread adds at most n / 32 + 64 terms of a row of n one
+after the other, then a few levels of a tree, so a row's mean, variance and dot
+products are off by at most (n / 32 + 80) 2^-24 of the sum of their terms'
+magnitudes.  Packed values are compared bit for bit.
+"""
+
+from __future__ import annotations
+
+import math
+import subprocess
+import sys
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+import frame_analytics_b200 as fa
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+E = 2.0 ** -24
+TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134}
+
+
+def rand(*shape, seed=0, scale=1.0, dtype=torch.float32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (scale * torch.randn(*shape, generator=g, device="cuda")).to(dtype)
+
+
+def within(got, want, tol, dtype):
+    err = (got.double() - want).abs()
+    tol = tol + TINY[dtype]
+    assert bool((err <= tol).all()), (err / tol).max().item()
+
+
+# --------------------------------------------------------------------------- #
+# packing
+# --------------------------------------------------------------------------- #
+
+def plain_pack(x):
+    """(values in x's dtype, codes) from the definition, group by group, float64."""
+    dtype, width = x.dtype, x.shape[-1]
+    rows = x.reshape(-1, width)
+    values, codes = torch.empty_like(rows), torch.zeros(
+        rows.shape[0], -(-width // 64) * 64, dtype=torch.uint8, device=x.device)
+    most = torch.finfo(dtype).max
+    for c in range(0, width, 64):
+        v = rows[:, c:c + 64].double()
+        lo, hi = v.amin(1, keepdim=True), v.amax(1, keepdim=True)
+        d = (hi - lo).float()
+        fine = d.isfinite()
+        d = torch.where(fine, d, torch.zeros_like(d)).double()
+        e = torch.full_like(d, -126)
+        for _ in range(300):  # the smallest e with d <= 255 2^e
+            e = torch.where(d > 255 * torch.exp2(e), e + 1, e)
+        s = torch.exp2(e)
+        q = ((v - lo).float().double() / s).round()
+        top = (d / s).round()
+        over = ((top * s + lo).to(dtype).double().abs() > most)
+        q = torch.where(over, torch.minimum(q, top - 1), q)
+        values[:, c:c + 64] = torch.where(fine, (q * s + lo).to(dtype).double(), math.nan).to(dtype)
+        codes[:, c:c + v.shape[1]] = torch.where(fine, q, torch.zeros_like(q)).to(torch.uint8)
+    return values.view(x.shape), codes.view(*x.shape[:-1], -1)
+
+
+def same_bits(a, b):
+    return a.shape == b.shape and a.dtype == b.dtype and torch.equal(
+        a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8)) or (
+        torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)))
+
+
+KINDS = {
+    "normal": lambda x: x,
+    "offset": lambda x: x + 1000,
+    "wide": lambda x: x * torch.exp2(torch.arange(x.shape[-1], device=x.device) % 40 - 20.0),
+    "one-sided": lambda x: x.relu(),
+    "constant": lambda x: torch.full_like(x, 0.37),
+    "zero": lambda x: torch.zeros_like(x),
+    "whole": lambda x: (x * 90).round(),
+    "halves": lambda x: (x * 200).round() / 2,      # ties between codes
+    "tiny": lambda x: x * 2.0 ** -136,
+}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 7), (2, 5, 64), (4, 65), (3, 200), (5, 128),
+                                   (33, 1000), (1000,), (130, 8)])
+def test_pack_bit_for_bit(shape, kind, dtype):
+    x = KINDS[kind](rand(*shape, seed=1)).to(dtype)
+    want, codes = plain_pack(x)
+    p = fa.pack8(x)
+    assert p.shape == x.shape and p.dtype == dtype
+    assert torch.equal(p.codes, codes)
+    assert same_bits(fa.unpack8(p), want + 0.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pack_is_within_its_bound(dtype):
+    x = rand(64, 640, seed=2, scale=3.0, dtype=dtype)
+    back = fa.unpack8(fa.pack8(x))
+    v = x.double().view(64, 10, 64)
+    d = v.amax(-1, keepdim=True) - v.amin(-1, keepdim=True)
+    err = (back.double().view_as(v) - v).abs()
+    # s / 2 < d / 255, and the value's own rounding
+    assert bool((err <= d / 255 + U[dtype] * (v.abs() + d / 255)).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pack_of_the_largest_and_of_what_is_not_finite(dtype):
+    most = torch.finfo(dtype).max
+    x = rand(12, 192, seed=3).to(dtype)
+    x[0, 3] = math.inf
+    x[1, 70] = -math.inf
+    x[2, 191] = math.nan
+    x[3, 5], x[3, 6] = math.inf, -math.inf
+    x[4] = most
+    x[5] = -most
+    x[6, 0] = most
+    x[7, 9], x[7, 10] = most, -most           # a spread past float32 for two of the types
+    x[8, 100] = -most
+    x[9, 0], x[9, 1] = most, most / 2
+    x[10] = math.nan
+    x[11] = math.inf
+    want, _ = plain_pack(x)
+    got = fa.unpack8(fa.pack8(x))
+    assert same_bits(got, want)
+    assert bool(got[0, :64].isnan().all()) and bool(got[0, 64:].isfinite().all())
+    assert bool((got[4] == most).all()) and bool(got[6].isfinite().all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("view", [
+    lambda x: x.mT, lambda x: x[:, 1:], lambda x: x[::3], lambda x: x[:, :100],
+    lambda x: x[:, ::2], lambda x: x[0].expand(9, -1), lambda x: x[:, :1].expand(-1, 70),
+    lambda x: x.view(4, 10, 136).transpose(0, 1), lambda x: x[3:, 8:72],
+])
+def test_pack_of_views(view, dtype):
+    x = view(rand(40, 136, seed=4, dtype=dtype))
+    want, codes = plain_pack(x.contiguous())
+    p = fa.pack8(x)
+    assert torch.equal(p.codes, codes) and same_bits(fa.unpack8(p), want)
+
+
+def test_unpack_of_what_was_moved():
+    x = rand(6, 200, seed=5, dtype=torch.bfloat16)
+    p = fa.pack8(x)
+    want = fa.unpack8(p)
+    host = p._replace(codes=p.codes.cpu(), ranges=p.ranges.cpu())
+    back = host._replace(codes=host.codes.cuda(), ranges=host.ranges.cuda())
+    assert torch.equal(fa.unpack8(back), want)
+    at = torch.empty(p.codes.numel() + 5, dtype=torch.uint8, device="cuda")[5:].view(p.codes.shape)
+    rt = torch.empty(p.ranges.numel() + 1, dtype=torch.int32, device="cuda")[1:].view(p.ranges.shape)
+    odd = p._replace(codes=at.copy_(p.codes), ranges=rt.copy_(p.ranges))  # odd addresses
+    assert torch.equal(fa.unpack8(odd), want)
+    with pytest.raises(TypeError):
+        fa.unpack8(p._replace(codes=host.codes))
+
+
+@pytest.mark.parametrize("width", [2112, 2111])
+def test_pack_past_2_31_values(width):
+    rows = (1 << 31) // width + 77
+    x = torch.zeros(rows, width, dtype=torch.bfloat16, device="cuda")
+    x[-50:] = rand(50, width, seed=6).bfloat16()
+    x[:50] = rand(50, width, seed=7).bfloat16()
+    p = fa.pack8(x)
+    back = fa.unpack8(p)
+    for part in (slice(0, 60), slice(rows - 60, rows)):
+        want, codes = plain_pack(x[part])
+        assert torch.equal(p.codes[part], codes) and torch.equal(back[part], want)
+    assert not bool(back[60:-60].any())
+
+
+# --------------------------------------------------------------------------- #
+# layer norm
+# --------------------------------------------------------------------------- #
+
+# leading shape, width, residual, affine, float32 weights
+NORMS = [
+    ((1,), 1, False, "none", False),
+    ((2,), 3, True, "both", False),
+    ((1,), 1024, True, "both", False),
+    ((4, 5), 64, False, "both", False),
+    ((37,), 577, False, "both", True),
+    ((130,), 200, True, "weight", False),
+    ((3, 3), 192, True, "both", True),
+    ((300,), 256, False, "bias", False),
+    ((65,), 512, True, "both", False),
+    ((21,), 1000, True, "none", False),
+    ((19,), 1025, False, "both", False),
+    ((9,), 2048, True, "both", True),
+    ((5,), 2056, False, "both", False),
+    ((7,), 4096, True, "both", False),
+    ((3,), 8192, False, "both", False),
+    ((2,), 8200, True, "both", False),
+    ((3,), 12001, False, "both", False),
+    ((2,), 40000, True, "both", True),
+    ((2000,), 72, True, "both", False),
+]
+
+
+def norm_case(case, dtype, seed=0):
+    lead, n, residual, affine, wide = case
+    wt = torch.float32 if wide else dtype
+    x = (rand(*lead, n, seed=seed) * 2 + 0.5).to(dtype)
+    res = rand(*lead, n, seed=seed + 1, dtype=dtype) if residual else None
+    w = (1 + 0.3 * rand(n, seed=seed + 2)).to(wt) if affine in ("both", "weight") else None
+    b = (0.3 * rand(n, seed=seed + 3)).to(wt) if affine in ("both", "bias") else None
+    gy = rand(*lead, n, seed=seed + 4, dtype=dtype)
+    gs = rand(*lead, n, seed=seed + 5, dtype=dtype) if residual else None
+    return x, res, w, b, gy, gs
+
+
+def norm_sum(x, res):
+    return x if res is None else (x.double() + res.double()).to(x.dtype)
+
+
+def norm_terms(s, eps):
+    """float64 mean, 1 / deviation, and the relative error of either float32 sum."""
+    s = s.double()
+    n = s.shape[-1]
+    m = s.mean(-1, keepdim=True)
+    r = 1 / ((s - m).square().mean(-1, keepdim=True) + eps).sqrt()
+    depth = n / 32 + 80
+    em = E * depth * s.abs().mean(-1, keepdim=True)   # of the mean
+    return m, r, em, E * depth
+
+
+def check_norm(y, s, w, b, eps, dtype):
+    m, r, em, rel = norm_terms(s, eps)
+    w = 1.0 if w is None else w.double()
+    b = torch.zeros((), device="cuda", dtype=torch.float64) if b is None else b.double()
+    part = (s.double() - m) * r * w
+    want = part + b
+    # the mean's error moves the value and, squared, the variance
+    tol = U[dtype] * want.abs() + (rel + 8 * E) * part.abs() + (em + E * s.double().abs()) * r * abs(w) \
+        + E * b.abs()
+    within(y, want, tol * 1.01 + part.abs() * (em * r) ** 2, dtype)
+
+
+def check_norm_grad(got, s, kept, w, b, gy, gs, eps, dtype):
+    """`kept`: what the backward pass has of s."""
+    m, r, em, rel = norm_terms(s, eps)
+    n = s.shape[-1]
+    xh = (kept.double() - m) * r
+    exh = (rel + 8 * E + (em * r) ** 2) * xh.abs() + (em + E * kept.double().abs()) * r
+    dy = gy.double()
+    wd = torch.ones(n, device="cuda", dtype=torch.float64) if w is None else w.double()
+    g = dy * wd
+    c1, c2 = g.mean(-1, keepdim=True), (g * xh).mean(-1, keepdim=True)
+    a1, a2 = g.abs().mean(-1, keepdim=True), (g * xh).abs().mean(-1, keepdim=True)
+    e2 = rel * a2 + (g.abs() * exh).mean(-1, keepdim=True)
+    dx = r * (g - c1 - xh * c2)
+    tol = r * (rel * a1 + xh.abs() * e2 + exh * c2.abs()) \
+        + (rel + 16 * E) * r * (g.abs() + a1 + xh.abs() * a2)
+    if gs is not None:
+        dx = dx + gs.double()
+        tol = tol + 2 * E * gs.double().abs()
+    within(got[0], dx, (1 + 2 * U[dtype]) * tol + U[dtype] * dx.abs(), dtype)
+    i = 1
+    if gs is not None:
+        assert torch.equal(got[1], got[0])
+        i = 2
+    # sums over rows: a warp adds its rows one after the other, then parts in order
+    rows = s.numel() // n
+    over = tuple(range(s.dim() - 1))
+    for p, term, err in ((w, dy * xh, dy.abs() * exh), (b, dy, torch.zeros_like(dy))):
+        if p is None:
+            continue
+        want = term.sum(over)
+        tol = E * (min(rows, 400) + 40) * term.abs().sum(over) + err.sum(over)
+        within(got[i], want, (1 + 2 * U[p.dtype]) * tol + U[p.dtype] * want.abs(), p.dtype)
+        assert got[i].dtype == p.dtype and got[i].shape == p.shape
+        i += 1
+    assert i == len(got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", NORMS)
+def test_norm_forward(case, dtype):
+    x, res, w, b, _, _ = norm_case(case, dtype)
+    got = fa.layer_norm(x, w, b, residual=res, eps=1e-5)
+    s = norm_sum(x, res)
+    if res is not None:
+        got, total = got
+        assert torch.equal(total, s) and total.is_contiguous()
+    assert got.shape == x.shape and got.dtype == dtype and got.is_contiguous()
+    check_norm(got, s, w, b, 1e-5, dtype)
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", NORMS)
+def test_norm_backward(case, dtype, keep8):
+    x, res, w, b, gy, gs = norm_case(case, dtype, seed=10)
+    leaves = [t.detach().requires_grad_(True) for t in (x, res, w, b) if t is not None]
+    it = iter(leaves)
+    xl, rl, wl, bl = (None if t is None else next(it) for t in (x, res, w, b))
+    out = fa.layer_norm(xl, wl, bl, residual=rl, eps=1e-5, keep8=keep8)
+    out = (out,) if res is None else out
+    s = norm_sum(x, res)
+    check_norm(out[0].detach(), s, w, b, 1e-5, dtype)
+    got = torch.autograd.grad(out, leaves, (gy,) if res is None else (gy, gs))
+    kept = fa.unpack8(fa.pack8(s)) if keep8 else s
+    check_norm_grad(got, s, kept, w, b, gy, gs, 1e-5, dtype)
+
+
+def test_norm_gradient_against_differences():
+    x, res, w, b, gy, gs = norm_case(((3,), 11, True, "both", False), torch.float32, seed=20)
+    leaves = [t.detach().clone().requires_grad_(True) for t in (x, res, w, b)]
+    out = fa.layer_norm(leaves[0], leaves[2], leaves[3], residual=leaves[1], eps=1e-2)
+    grads = torch.autograd.grad(out, leaves, (gy, gs))
+
+    def value(ts):
+        s = ts[0] + ts[1]
+        y = F.layer_norm(s, (11,), ts[2], ts[3], 1e-2)
+        return float((y * gy).sum() + (s * gs).sum())
+
+    wide = [t.detach().double() for t in leaves]
+    h = 1e-4
+    for i in range(4):
+        flat = wide[i].flatten()
+        for j in range(0, flat.numel(), 3):
+            vals = []
+            for sign in (1, -1):
+                moved = flat.clone()
+                moved[j] += sign * h
+                vals.append(value([*wide[:i], moved.view(wide[i].shape), *wide[i + 1:]]))
+            fd = (vals[0] - vals[1]) / (2 * h)
+            assert abs(fd - float(grads[i].flatten()[j])) < 2e-5 * (1 + abs(fd))
+
+
+@pytest.mark.parametrize("width", [200, 1024, 8200])
+def test_norm_of_an_offset_row_keeps_its_precision(width):
+    x = rand(5, width, seed=21) + 1000.0
+    check_norm(fa.layer_norm(x), x, None, None, 1e-5, torch.float32)
+    leaf = x.clone().requires_grad_(True)
+    gy = rand(5, width, seed=22)
+    w = torch.ones(width, device="cuda", requires_grad=True)
+    got = torch.autograd.grad(fa.layer_norm(leaf, w, keep8=True), (leaf, w), gy)
+    check_norm_grad(got, x, fa.unpack8(fa.pack8(x)), w.detach(), None, gy, None, 1e-5, torch.float32)
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+@pytest.mark.parametrize("width", [72, 1000, 9000])
+def test_norm_rows_with_an_infinity_or_a_nan_stay_alone(width, keep8):
+    x = rand(40, width, seed=23, dtype=torch.bfloat16)
+    x[3, 5], x[17, 0] = math.inf, math.nan
+    x[20] = 7.0                                  # no spread at all
+    leaf = x.clone().requires_grad_(True)
+    y = fa.layer_norm(leaf, keep8=keep8)
+    dx, = torch.autograd.grad(y, leaf, rand(40, width, seed=24, dtype=torch.bfloat16))
+    bad = torch.zeros(40, dtype=torch.bool, device="cuda")
+    bad[[3, 17]] = True
+    for t in (y, dx):
+        assert bool(t[bad].isnan().any(-1).all()) and bool(t[~bad].isfinite().all())
+    assert not bool(y[20].any())
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+@pytest.mark.parametrize("view", [
+    lambda t: t.mT, lambda t: t[:, 1:], lambda t: t[::3], lambda t: t[:, 8:136], lambda t: t[:, ::2],
+    lambda t: t.view(4, 34, 136).transpose(0, 1),
+])
+def test_norm_of_views_and_of_expanded_gradients(view, keep8):
+    x, res = rand(136, 136, seed=25), rand(136, 136, seed=26)
+    a, b = view(x), view(res)
+    w = 1 + 0.1 * rand(a.shape[-1] * 2, seed=27)[::2]
+    leaves = [t.detach().requires_grad_(True) for t in (a, b, w)]
+    y, s = fa.layer_norm(leaves[0], leaves[2], residual=leaves[1], keep8=keep8)
+    want_s = a + b
+    assert torch.equal(s, want_s)
+    got = torch.autograd.grad((y.sum() + (3 * s).sum()), leaves)
+    one = torch.ones_like(want_s)
+    kept = fa.unpack8(fa.pack8(want_s)) if keep8 else want_s
+    check_norm_grad(got, want_s, kept, w, None, one, 3 * one, 1e-5, torch.float32)
+
+
+def test_norm_gradients_of_one_output_alone_and_of_an_operand_twice():
+    x, res, w, b, gy, gs = norm_case(NORMS[8], torch.float32, seed=30)
+    leaves = [t.detach().requires_grad_(True) for t in (x, res, w)]
+    y, s = fa.layer_norm(leaves[0], leaves[2], residual=leaves[1])
+    only = torch.autograd.grad(s, leaves[:2], gs, retain_graph=True)
+    assert torch.equal(only[0], gs) and torch.equal(only[1], gs)
+    got = torch.autograd.grad(y, leaves, gy)
+    check_norm_grad((got[0], got[2]), norm_sum(x, res), norm_sum(x, res), w, None, gy, None, 1e-5,
+                    torch.float32)
+    y, s = fa.layer_norm(leaves[0], leaves[2], residual=leaves[0])
+    twice, = torch.autograd.grad(y, leaves[0], gy)
+    one = (2 * x).detach().requires_grad_(True)
+    ref, = torch.autograd.grad(fa.layer_norm(one, w), one, gy)
+    assert torch.equal(twice, 2 * ref)
+    # accumulated into the leaves, in the same buffers
+    a, c = (t.detach().clone().requires_grad_(True) for t in (x, res))
+    for _ in range(2):
+        y, s = fa.layer_norm(a, w, residual=c)
+        torch.autograd.backward((y, s), (gy, gs))
+    assert a.grad.data_ptr() != c.grad.data_ptr() and torch.equal(a.grad, c.grad)
+
+
+def test_norm_keeps_what_it_says():
+    x = rand(4096, 1024, seed=31, dtype=torch.bfloat16).requires_grad_(True)
+    held = []
+    for keep8 in (False, True):
+        before = torch.cuda.memory_allocated()
+        with torch.autograd.graph.saved_tensors_hooks(
+                lambda t: (held.append(t.numel() * t.element_size()), t)[1], lambda t: t):
+            y = fa.layer_norm(x, keep8=keep8)
+        del y
+        assert torch.cuda.memory_allocated() <= before
+    assert sum(held) == 2 * x.numel() + 8 * 4096 + x.numel() * 17 // 16 + 8 * 4096
+    y = fa.layer_norm(x * 1, keep8=True)
+    y.sum().backward()
+    base = (x.detach() * 1).requires_grad_(True)
+    inner = base * 1
+    y = fa.layer_norm(inner, keep8=False)
+    inner.data.add_(0)  # not seen
+    with torch.no_grad():
+        inner.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+
+
+# --------------------------------------------------------------------------- #
+# activation
+# --------------------------------------------------------------------------- #
+
+def plain_gelu(x, approximate):
+    return F.gelu(x, approximate=approximate)
+
+
+def check_gelu(y, x, approximate, dtype):
+    want = plain_gelu(x.double(), approximate)
+    # Phi (or the tanh form's factor) to 8 2^-24 absolute
+    within(y, want, U[dtype] * want.abs() * (1 + 2 * U[dtype]) + 8 * E * x.double().abs(), dtype)
+
+
+def check_gelu_grad(dx, kept, gy, approximate, dtype):
+    k = kept.double().requires_grad_(True)
+    slope, = torch.autograd.grad(plain_gelu(k, approximate).sum(), k)
+    want = slope * gy.double()
+    within(dx, want, U[dtype] * want.abs() * (1 + 2 * U[dtype])
+           + 16 * E * (1 + kept.double().abs()) * gy.double().abs(), dtype)
+
+
+@pytest.mark.parametrize("approximate", ["none", "tanh"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1,), (3, 7), (2, 5, 64), (33, 1000), (40, 1001), (500, 256)])
+def test_gelu(shape, dtype, approximate):
+    x = (3 * rand(*shape, seed=40)).to(dtype)
+    gy = rand(*shape, seed=41, dtype=dtype)
+    leaf = x.clone().requires_grad_(True)
+    y = fa.gelu8(leaf, approximate=approximate)
+    assert y.shape == x.shape and y.dtype == dtype
+    check_gelu(y.detach(), x, approximate, dtype)
+    assert torch.equal(fa.gelu8(x, approximate=approximate), y.detach())
+    dx, = torch.autograd.grad(y, leaf, gy)
+    check_gelu_grad(dx, fa.unpack8(fa.pack8(x)), gy, approximate, dtype)
+
+
+@pytest.mark.parametrize("approximate", ["none", "tanh"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gelu_over_its_range(dtype, approximate):
+    x = torch.linspace(-14, 14, 28 * 512 + 1, device="cuda").to(dtype)
+    x = torch.cat((x, torch.tensor([0.0, -0.0, 60.0, -60.0, 1e-5, -1e-5, 3e4, -3e4],
+                                   device="cuda").to(dtype)))
+    check_gelu(fa.gelu8(x, approximate=approximate), x, approximate, dtype)
+    # each value a group of its own is kept exactly
+    col = x[:, None].clone().requires_grad_(True)
+    gy = torch.ones_like(col)
+    dx, = torch.autograd.grad(fa.gelu8(col, approximate=approximate), col, gy)
+    check_gelu_grad(dx, col.detach(), gy, approximate, dtype)
+
+
+def test_gelu_of_what_is_not_finite():
+    x = torch.tensor([math.inf, math.nan, 1.0], device="cuda")
+    y = fa.gelu8(x)
+    assert y[0] == math.inf and bool(y[1].isnan()) and bool(y[2].isfinite())
+
+
+@pytest.mark.parametrize("view", [lambda t: t.mT, lambda t: t[:, 1:], lambda t: t[::2, 8:]])
+def test_gelu_of_views_and_of_expanded_gradients(view):
+    x = view(rand(136, 136, seed=42))
+    leaf = x.detach().requires_grad_(True)
+    y = fa.gelu8(leaf)
+    check_gelu(y.detach(), x, "none", torch.float32)
+    dx, = torch.autograd.grad(y.sum(), leaf)
+    check_gelu_grad(dx, fa.unpack8(fa.pack8(x)), torch.ones_like(x), "none", torch.float32)
+    gy = view(rand(136, 136, seed=43))
+    dx, = torch.autograd.grad(fa.gelu8(leaf), leaf, gy)
+    check_gelu_grad(dx, fa.unpack8(fa.pack8(x)), gy, "none", torch.float32)
+
+
+# --------------------------------------------------------------------------- #
+# products
+# --------------------------------------------------------------------------- #
+
+# rows, inputs, outputs, bias
+LINEARS = [
+    (1, 1, 1, True),
+    (1, 64, 32, True),
+    (2, 8, 8, False),
+    (5, 7, 3, True),
+    (17, 64, 64, True),
+    (63, 65, 130, True),
+    (64, 128, 128, False),
+    (65, 136, 264, True),
+    (200, 192, 768, False),
+    (333, 517, 333, True),
+    (1000, 256, 256, True),
+    (1037, 1000, 72, True),
+    (129, 40, 1030, True),
+    (4000, 64, 128, True),
+    (700, 520, 520, True),
+    (20000, 16, 24, True),
+]
+
+
+def linear_case(case, dtype, seed=0):
+    t, k, m, bias = case
+    x = (rand(t, k, seed=seed) * torch.exp(0.5 * rand(k, seed=seed + 1)) + 0.2).to(dtype)
+    w = rand(m, k, seed=seed + 2, scale=k ** -0.5, dtype=dtype)
+    b = rand(m, seed=seed + 3, dtype=dtype) if bias else None
+    return x, w, b, rand(t, m, seed=seed + 4, dtype=dtype)
+
+
+def check_weight_grad(dw, db, x, gy, dtype):
+    kept = fa.unpack8(fa.pack8(x)).double().reshape(-1, x.shape[-1])
+    g = gy.double().reshape(-1, gy.shape[-1])
+    t = g.shape[0]
+    # roundings (or truncations, on the tensor cores) of a sum of t terms: each at
+    # most 2^-23 of a partial sum, which is the sum of magnitudes at the very most
+    # and its square root's share of it for signs that vary
+    for got, want, size in ((dw, g.T @ kept, g.T.abs() @ kept.abs()),
+                            (db, g.sum(0), g.abs().sum(0))):
+        if got is not None:
+            tol = U[dtype] * want.abs() + (8 + 4 * math.sqrt(t)) * E * size
+            within(got, want, (1 + 2 * U[dtype]) * tol, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", LINEARS)
+def test_linear(case, dtype):
+    x, w, b, gy = linear_case(case, dtype)
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b) if t is not None]
+    y = fa.linear8(leaves[0], leaves[1], leaves[2] if b is not None else None)
+    assert torch.equal(y.detach(), F.linear(x, w, b))
+    got = torch.autograd.grad(y, leaves, gy)
+    assert torch.equal(got[0], gy @ w)
+    assert got[1].shape == w.shape and got[1].is_contiguous()
+    check_weight_grad(got[1], got[2] if b is not None else None, x, gy, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_of_views(dtype):
+    big = rand(2, 50, 300, seed=50, dtype=dtype)
+    grad = rand(2, 50, 400, seed=51, dtype=dtype)
+    w = rand(300, 160, seed=52, dtype=dtype)
+    for x, gy, wt in ((big[..., 4:164], grad[..., 8:168], w[:160]),
+                      (big[..., 1:161], grad[..., 3:163], w[:160]),
+                      (big[:, ::2, :160], grad[:, ::2, :160], w[::2][:160 // 2]),
+                      (big.transpose(0, 1)[..., :160], grad.transpose(0, 1)[..., :300], w),
+                      (big[0, :, :160].mT.reshape(160, 50).mT, grad[0, :, :300], w)):
+        m = min(wt.shape[0], gy.shape[-1])
+        wt, gy = wt[:m], gy[..., :m]
+        leaves = [x.detach().requires_grad_(True), wt.detach().requires_grad_(True)]
+        y = fa.linear8(*leaves)
+        # (which of its products torch takes for views depends on more than the operands)
+        size = F.linear(x.double().abs(), wt.double().abs())
+        want = F.linear(x.double(), wt.double())
+        within(y.detach(), want, U[dtype] * want.abs() + (8 + 4 * math.sqrt(x.shape[-1])) * E * size,
+               dtype)
+        dx, dw = torch.autograd.grad(y, leaves, gy)
+        assert dx.shape == x.shape
+        check_weight_grad(dw, None, x, gy, dtype)
+
+
+def test_linear_with_an_expanded_gradient_and_parts_that_need_none():
+    x, w, b, _ = linear_case(LINEARS[8][:3] + (True,), torch.bfloat16)
+    for need in ((True, False, False), (False, True, False), (False, False, True),
+                 (True, True, False), (False, True, True)):
+        leaves = [t.detach().clone().requires_grad_(n) for t, n in zip((x, w, b), need)]
+        y = fa.linear8(*leaves)
+        y.sum().backward()
+        one = torch.ones_like(y)
+        if need[0]:
+            assert torch.equal(leaves[0].grad, one @ w)
+        check_weight_grad(leaves[1].grad, leaves[2].grad, x, one, torch.bfloat16)
+        assert [t.grad is not None for t in leaves] == list(need)
+
+
+def test_linear_keeps_what_it_says():
+    x = rand(1024, 512, seed=53, dtype=torch.float16).requires_grad_(True)
+    w = rand(128, 512, seed=54, dtype=torch.float16)
+    for need, want in ((True, 1024 * 512 * 17 // 16), (False, 0)):
+        sizes = []
+        weight = w.clone().requires_grad_(need)
+        with torch.autograd.graph.saved_tensors_hooks(
+                lambda t: (sizes.append(t.numel() * t.element_size()), t)[1], lambda t: t):
+            fa.linear8(x, weight)
+        assert sum(sizes) == want + 128 * 512 * 2
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_linear_under_autocast(dtype):
+    x, w, b, gy = linear_case(LINEARS[10], torch.float32)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    with torch.autocast("cuda", dtype=dtype):
+        y = fa.linear8(*leaves)
+        want = F.linear(x, w, b)
+    assert y.dtype == dtype and torch.equal(y.detach(), want)
+    got = torch.autograd.grad(y, leaves, gy.to(dtype))
+    assert all(g.dtype == torch.float32 for g in got)
+    check_weight_grad(got[1].to(dtype), got[2].to(dtype), x.to(dtype), gy.to(dtype), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_rows_that_are_not_finite_reach_their_own_columns_alone(dtype):
+    x, w, _, gy = linear_case((100, 200, 64, False), dtype)
+    x[7, 70], x[9, 199] = math.inf, math.nan
+    leaf = w.clone().requires_grad_(True)
+    dw, = torch.autograd.grad(fa.linear8(x, leaf), leaf, gy)
+    bad = torch.zeros(200, dtype=torch.bool, device="cuda")
+    bad[64:128], bad[192:] = True, True          # the groups of the two
+    assert bool(dw[:, bad].isnan().all()) and bool(dw[:, ~bad].isfinite().all())
+
+
+# --------------------------------------------------------------------------- #
+# together
+# --------------------------------------------------------------------------- #
+
+def block(x, p):
+    """Norm, product, activation, product, residual sum and norm."""
+    y = fa.layer_norm(x, p[0], p[1], keep8=True)
+    y = fa.linear8(fa.gelu8(fa.linear8(y, p[2], p[3])), p[4], p[5])
+    return fa.layer_norm(y, p[6], p[7], residual=x, keep8=True)
+
+
+def block_params(width, dtype, seed=60):
+    return [1 + 0.1 * rand(width, seed=seed), 0.1 * rand(width, seed=seed + 1),
+            rand(4 * width, width, seed=seed + 2, scale=width ** -0.5),
+            0.1 * rand(4 * width, seed=seed + 3),
+            rand(width, 4 * width, seed=seed + 4, scale=0.5 * width ** -0.5),
+            0.1 * rand(width, seed=seed + 5),
+            1 + 0.1 * rand(width, seed=seed + 6), 0.1 * rand(width, seed=seed + 7)]
+
+
+class Kept64(torch.autograd.Function):
+    """float64 operators with float32 copies of their inputs, packed."""
+
+    @staticmethod
+    def forward(ctx, fn, x, *params):
+        ctx.fn, ctx.n = fn, len(params)
+        ctx.save_for_backward(x, *params)
+        return fn(x, x, *params)
+
+    @staticmethod
+    def backward(ctx, g):
+        x, *params = ctx.saved_tensors
+        kept = fa.unpack8(fa.pack8(x.float())).double()
+        with torch.enable_grad():
+            leaves = [t.detach().requires_grad_(True) for t in (kept, *params)]
+            return (None, *torch.autograd.grad(ctx.fn(x, leaves[0], *leaves[1:]), leaves, g))
+
+
+def norm64(x, kept, w, b):
+    m = x.mean(-1, keepdim=True)
+    r = 1 / ((x - m).square().mean(-1, keepdim=True) + 1e-5).sqrt()
+    # value and weight slope at `kept`; the input's slope is the norm's formula there
+    xh = (kept - m) * r
+
+    class Slope(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, k, h):
+            return h
+
+        @staticmethod
+        def backward(ctx, g):
+            h = xh.detach()
+            return r * (g - g.mean(-1, keepdim=True) - h * (g * h).mean(-1, keepdim=True)), None
+    return Slope.apply(kept, xh.detach()) * w + b
+
+
+def block64(x, p):
+    y = Kept64.apply(norm64, x, p[0], p[1])
+    y = Kept64.apply(lambda x, k, w, b: F.linear(k, w, b), y, p[2], p[3])
+    y = Kept64.apply(lambda x, k: F.gelu(k), y)
+    y = Kept64.apply(lambda x, k, w, b: F.linear(k, w, b), y, p[4], p[5])
+    s = x + y
+    return Kept64.apply(norm64, s, p[6], p[7]), s
+
+
+def test_a_block_of_them_against_float64():
+    x = rand(300, 96, seed=61)
+    p = block_params(96, torch.float32)
+    gy, gs = rand(300, 96, seed=62), rand(300, 96, seed=63)
+    leaves = [t.clone().requires_grad_(True) for t in (x, *p)]
+    out = block(leaves[0], leaves[1:])
+    got = torch.autograd.grad(out, leaves, (gy, gs))
+    wide = [t.detach().double().requires_grad_(True) for t in leaves]
+    ref = block64(wide[0], wide[1:])
+    want = torch.autograd.grad(ref, wide, (gy.double(), gs.double()))
+    for a, b in zip((*out, *got), (*ref, *want)):
+        # float32 products of up to 400 terms and a few of them in a row; where a
+        # rounding moves an intermediate over the border of two codes, one term of
+        # such a sum moves by 1 / 255 of its range (in under 1 in 10^4)
+        rel = float((a.double() - b).norm() / b.norm())
+        assert rel < 1e-4, rel
+    # and against the gradient without packing: 1/255 of the range of 64 values is at
+    # most 2 % of their deviation, and averages
+    plain = [t.detach().double().requires_grad_(True) for t in leaves]
+    y = F.layer_norm(plain[0], (96,), plain[1], plain[2])
+    y = F.linear(F.gelu(F.linear(y, plain[3], plain[4])), plain[5], plain[6])
+    s = plain[0] + y
+    exact = torch.autograd.grad((F.layer_norm(s, (96,), plain[7], plain[8]), s), plain,
+                                (gy.double(), gs.double()))
+    for a, b in zip(got, exact):
+        assert float((a.double() - b).norm() / b.norm()) < 0.02
+
+
+def train_step(x, p, gy, gs):
+    leaves = [t.requires_grad_(True) for t in (x, *p)]
+    out = block(leaves[0], leaves[1:])
+    return (*[t.detach() for t in out], *torch.autograd.grad(out, leaves, (gy, gs)))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_block_is_the_same_bits_every_time_and_on_another_stream(dtype):
+    x, gy, gs = (rand(700, 192, seed=64 + i, dtype=dtype) for i in range(3))
+    p = [t.to(dtype) for t in block_params(192, dtype)]
+    want = train_step(x, p, gy, gs)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(2):
+        with torch.cuda.stream(side):
+            got = train_step(*[t.detach() if torch.is_tensor(t) else [u.detach() for u in t]
+                               for t in (x, p, gy, gs)])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_graphs_of_blocks_replay_in_any_order():
+    inputs = [[rand(257, 96, seed=70 + 5 * k + i, dtype=torch.bfloat16) for i in range(3)]
+              for k in range(2)]
+    p = [t.bfloat16() for t in block_params(96, torch.bfloat16)]
+
+    def step(k):
+        x, gy, gs = inputs[k]
+        return train_step(x.detach(), [t.detach() for t in p], gy, gs)
+
+    want = [step(k) for k in range(2)]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for k in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(step(k))
+    for k in (1, 0, 1):
+        graphs[k].replay()
+        torch.cuda.synchronize()
+        step(1 - k)
+        assert all(torch.equal(a, b) for a, b in zip(got[k], want[k]))
+    for t in inputs[0]:
+        t.mul_(0.5)
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got[0], step(0)))
+
+
+def test_second_derivatives_are_refused():
+    x = rand(4, 64, seed=80).requires_grad_(True)
+    w = rand(8, 64, seed=81).requires_grad_(True)
+    for y in (fa.layer_norm(x), fa.layer_norm(x, keep8=True), fa.gelu8(x), fa.linear8(x, w)):
+        with pytest.raises(RuntimeError, match="[Dd]ouble|once|second|create_graph"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+@pytest.mark.parametrize("shape", [(0, 64), (3, 0, 8)])
+def test_no_rows(shape):
+    x = torch.empty(shape, device="cuda", requires_grad=True)
+    n = shape[-1]
+    w, b = (torch.ones(n, device="cuda", requires_grad=True) for _ in range(2))
+    y, s = fa.layer_norm(x, w, b, residual=x)
+    m = torch.ones(5, n, device="cuda", requires_grad=True)
+    total = y.sum() + s.sum() + fa.gelu8(x).sum() + fa.linear8(x, m).sum()
+    total.backward()
+    assert x.grad.shape == shape and not any(bool(t.grad.any()) for t in (w, b, m))
+    p = fa.pack8(x)
+    assert fa.unpack8(p).shape == shape
+
+
+def test_another_device_is_refused_and_the_current_one_is_kept():
+    x = rand(4, 64, seed=82)
+    with pytest.raises(TypeError):
+        fa.layer_norm(x, torch.ones(64))
+    with pytest.raises(TypeError):
+        fa.linear8(x, torch.ones(4, 64))
+    assert torch.cuda.current_device() == 0
