@@ -23,7 +23,7 @@ LIB = LIBDIR / "libfa_b200.so"
 SOURCES = ["abi.cu", "pixel.cu", "ssim_fwd.cu", "ssim_bwd.cu", "gmsd.cu", "pool.cu", "grad_scale.cu",
            "ssim_compat.cu", "f64.cu",
            "ssimulacra2.cu", "qk_rotary.cu", "orthogonalize.cu", "keep8.cu",
-           "layer_norm.cu", "wgrad8.cu", "abi_train.cu"]
+           "layer_norm.cu", "linear8.cu", "abi_train.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -1,6 +1,6 @@
 """A transformer block's norm, activation and products with what they keep for the
 backward pass in 8 bits (no counterpart in the reference; ``csrc/keep8.cu``,
-``csrc/layer_norm.cu``, ``csrc/wgrad8.cu``).
+``csrc/layer_norm.cu``, ``csrc/linear8.cu``).
 
 A network that restores whole frames keeps the input of every norm, activation
 and product until its gradient comes back; these inputs, not the weights, fill
@@ -27,6 +27,7 @@ __all__ = ["Packed8", "pack8", "unpack8", "layer_norm", "gelu8", "linear8"]
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
 _GROUP = 64
 _MAX_WIDTH = 1 << 24
+_MAX_SIDE, _MAX_ROWS = (1 << 22) - 64, 1 << 27  # of a product
 # struct fa_norm of include/fa_b200.h as bytes
 _NORM = struct.Struct("@2iq2idPqPq5P").pack
 
@@ -386,22 +387,25 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] 
     once, in reverse mode.
 
     ``x`` (..., K), ``weight`` (M, K), ``bias`` (M,): one dtype, float16, bfloat16
-    or float32 (under autocast its dtype), any strides; K and M at most 4194303.
+    or float32 (under autocast its dtype), any strides; K and M at most 4194240, and
+    2^27 rows.
     ``x`` is packed only where the weight wants a gradient."""
     if torch.is_autocast_enabled("cuda"):
         to = torch.get_autocast_dtype("cuda")
         if to in _DTYPES:
             x, weight, bias = (t.to(to) if torch.is_tensor(t) and t.dtype in _DTYPES else t
                                for t in (x, weight, bias))
-    _check_values("x", x, (1 << 22) - 1)
+    _check_values("x", x, _MAX_SIDE)
+    if x.numel() // x.shape[-1] > _MAX_ROWS:
+        raise ValueError(f"x of shape {tuple(x.shape)} has more than {_MAX_ROWS} rows")
     if not torch.is_tensor(weight) or weight.dim() != 2 or weight.shape[1] != x.shape[-1] \
             or weight.dtype != x.dtype:
         raise ValueError(f"weight must be {x.dtype} of shape (M, {x.shape[-1]}), got "
                          f"{getattr(weight, 'dtype', type(weight))} "
                          f"{tuple(getattr(weight, 'shape', ()))}")
     outputs = weight.shape[0]
-    if not 1 <= outputs < 1 << 22:
-        raise ValueError(f"the weight must have 1..{(1 << 22) - 1} rows, got {outputs}")
+    if not 1 <= outputs <= _MAX_SIDE:
+        raise ValueError(f"the weight must have 1..{_MAX_SIDE} rows, got {outputs}")
     if bias is not None and (tuple(bias.shape) != (outputs,) or bias.dtype != x.dtype):
         raise ValueError(f"bias must be {x.dtype} of shape ({outputs},), got {bias.dtype} "
                          f"{tuple(bias.shape)}")

@@ -692,7 +692,8 @@ FA_B200_API int fa_b200_layer_norm_backward(const fa_norm* params, const void* d
 
 /* Weight gradient of y = x W^T + b from the packed copy of x [rows][inputs]:
  * dweight [outputs][inputs] = dy^T x (null: not computed), dbias [outputs] = column
- * sums of dy (null: not computed).  Workspace: 256-byte aligned, needs no zeroing. */
+ * sums of dy (null: not computed).  At most 2^27 rows, 4194240 inputs and outputs.
+ * Workspace: 256-byte aligned, needs no zeroing. */
 FA_B200_API int fa_b200_linear8_weight_grad_workspace_bytes(int64_t rows, int inputs, int outputs,
                                                             int dtype, int device,
                                                             size_t* out_bytes);

@@ -34,8 +34,10 @@ def test_rows_past_the_limits_are_refused():
         fa.pack8(one.expand(1 << 31))
     with pytest.raises(ValueError, match="last dimension"):
         fa.linear8(one.expand(2, 1 << 22), one.expand(3, 1 << 22))
-    with pytest.raises(ValueError, match="rows"):
-        fa.linear8(one.expand(2, 4), one.expand(1 << 22, 4))
+    for x, w in ((one.expand(2, 4), one.expand(1 << 22, 4)),
+                 (one.expand((1 << 27) + 1, 4), one.expand(2, 4))):
+        with pytest.raises(ValueError, match="rows"):
+            fa.linear8(x, w)
 
 
 @pytest.mark.parametrize("kw,exc", [
