@@ -118,18 +118,16 @@ struct ProductArgs {
 
 template <bool PACKED>
 struct Product {
-  // Operand stages, and stages of codes, which run further ahead.  Even numbers: the
-  // two teams of writers take turns, and each then sees every phase of its stages.
-  static constexpr int kStages = PACKED ? 4 : 6;
-  static constexpr int kStage = 2 * kHalf;
-  static constexpr int kRaws = PACKED ? 8 : 0;
+  // Stages of the operands, and of the codes, which the writers read ahead of them.
+  static constexpr int kStages = PACKED ? 5 : 6, kC = PACKED ? 4 : 0;
   static constexpr int kWriters = PACKED ? 8 : 0;   // warps that unpack
   static constexpr int kEpi = PACKED ? 4 : 8;       // warps of the epilogue
   static constexpr int kThreads = 128 + 32 * (kWriters + kEpi);
-  static constexpr int kTurnAt = kStages * kStage;  // offsets in shared memory
-  static constexpr int kRawAt = kTurnAt + kEpi * kTurn;
-  static constexpr int kRangesAt = kRawAt + kRaws * kRaw;
-  static constexpr int kSmem = kRangesAt + kRaws * kRanges + 1024;
+  static constexpr int kBAt = kStages * kHalf;      // offsets in shared memory
+  static constexpr int kTurnAt = 2 * kBAt;
+  static constexpr int kCodesAt = kTurnAt + kEpi * kTurn;
+  static constexpr int kRangesAt = kCodesAt + kC * kRaw;
+  static constexpr int kSmem = kRangesAt + kC * kRanges + 1024;
 };
 
 struct Work {
@@ -151,20 +149,75 @@ __device__ __forceinline__ bool work_of(const ProductArgs& a, int item, Work* w)
   return true;
 }
 
+// Bounded waits that sleep.  Sixteen warps wait here at a time, and each poll of a
+// barrier holds up the others' (a poll of a phase that was complete took 260 cycles
+// when the waiting warps polled in a loop), so a poll may suspend its warp until the
+// phase completes, or up to 2 ms.  The error word, in host memory, is looked at once in
+// 16 such polls.
+__device__ __forceinline__ bool mbar_sleep(unsigned a, unsigned parity) {
+  unsigned done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(a), "r"(parity), "r"(2000000u)
+      : "memory");
+  return done != 0;
+}
+// Whether a phase is complete, without waiting.
+__device__ __forceinline__ bool mbar_peek(unsigned long long* bar, unsigned parity) {
+  unsigned done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+static __device__ __noinline__ void stage_wait_slow(unsigned a, unsigned parity, unsigned* err) {
+  const unsigned long long t0 = globaltimer_ns();
+  unsigned long long next = 1000000ull;
+  for (unsigned i = 1;; ++i) {
+    if (mbar_sleep(a, parity)) return;
+    const unsigned long long t = globaltimer_ns() - t0;
+    if ((i & 15u) != 0u || t < next) continue;
+    next = t + 1000000ull;
+    if (t > kWaitLimitNs || (err && *reinterpret_cast<volatile unsigned*>(err) != 0u)) {
+      if (err) {
+        *reinterpret_cast<volatile unsigned*>(err) = (unsigned)FA_E_TIMEOUT;
+        __threadfence_system();
+      }
+      return;
+    }
+  }
+}
+__device__ __forceinline__ void stage_wait(unsigned long long* bar, unsigned parity,
+                                           unsigned* err) {
+  const unsigned a = smem_u32(bar);
+  if (!mbar_sleep(a, parity)) stage_wait_slow(a, parity, err);
+}
+
 // A phase that the other block of the pair may complete.
 __device__ __forceinline__ void wait_pair(unsigned long long* bar, unsigned parity, unsigned* err) {
-  mbar_wait(bar, parity, err);
+  stage_wait(bar, parity, err);
   asm volatile("fence.acq_rel.cluster;\n" ::: "memory");
 }
 
 // A warp has written its share of a stage, here or in the other block of the pair.
 // What it wrote is in its own block's shared memory and fence.proxy.async has handed
 // it to the tensor cores; nothing else has to be ordered, and a release to the whole
-// cluster here, a memory barrier of about 1500 cycles, bounded the kernel (254
-// against 126 us for 16320 rows, 1024 x 4096).
+// cluster here, a memory barrier of over a thousand cycles a stage, bounded the kernel
+// (258 against 160 us for 16320 rows, 1024 x 4096).
 __device__ __forceinline__ void arrive_written(unsigned long long* bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(in_leader(smem_u32(bar)))
                : "memory");
+}
+
+// One lane polls, the others wait at the warp's barrier.
+__device__ __forceinline__ void warp_wait(unsigned long long* bar, unsigned parity, unsigned* err) {
+  if ((threadIdx.x & 31) == 0) stage_wait(bar, parity, err);
+  __syncwarp();
 }
 
 // 16 codes to 16 operand values, two to a word.  The low bytes of 2^23 + q and of
@@ -276,11 +329,11 @@ template <typename T, bool PACKED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kThreads, 1)
     product_kernel(const __grid_constant__ ProductArgs a) {
   typedef Product<PACKED> P;
-  constexpr int S = P::kStages, R = P::kRaws ? P::kRaws : 1;
+  constexpr int S = P::kStages, SC = PACKED ? P::kC : 1;
   extern __shared__ char smem_raw[];
   const unsigned smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   char* const smem = smem_raw + (smem0 - smem_u32(smem_raw));
-  __shared__ unsigned long long full[S], empty[S], ready[S], raw[R], raw_empty[R], tm_full[2],
+  __shared__ unsigned long long full[S], empty[S], c_full[SC], c_empty[SC], tm_full[2],
       tm_empty[2], drain;
   __shared__ unsigned tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x & 1;
@@ -288,13 +341,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
-      mbar_init(&full[i], 1);
+      // the copies' bytes, and a team of four writers in either block
+      mbar_init(&full[i], 1 + (PACKED ? P::kWriters : 0));
       mbar_init(&empty[i], 1);
-      mbar_init(&ready[i], PACKED ? P::kWriters : 1);  // a team of either block
     }
-    for (int i = 0; i < P::kRaws; ++i) {
-      mbar_init(&raw[i], 1 + 32);  // the codes' copy, and a warp's copies of ranges
-      mbar_init(&raw_empty[i], P::kWriters / 2);
+    for (int i = 0; i < SC; ++i) {
+      mbar_init(&c_full[i], 1 + 32);  // the codes' copy, and a warp's copies of ranges
+      mbar_init(&c_empty[i], PACKED ? P::kWriters / 2 : 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tm_full[i], 1);
@@ -324,26 +377,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
         const int ia = t.i0 + rank * 128, jb = t.j0 + rank * 128;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
           const int s = n % S;
-          if (n >= (unsigned)S) mbar_wait(&empty[s], (n / S - 1) & 1, a.err);
+          if (n >= (unsigned)S) stage_wait(&empty[s], (n / S - 1) & 1, a.err);
           // both blocks' copies count on the first block's barrier
           const unsigned bar = in_leader(smem_u32(&full[s]));
-          const unsigned base = smem0 + s * P::kStage;
           if (rank == 0) mbar_expect_tx(&full[s], 2 * (PACKED ? 1 : 2) * kHalf);
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            tma_box<true>(base + i * kBox, &a.a, a.a_mn ? ia + 64 * i : kb * kDepth,
+            tma_box<true>(smem0 + s * kHalf + i * kBox, &a.a, a.a_mn ? ia + 64 * i : kb * kDepth,
                           a.a_mn ? kb * kDepth : ia + 64 * i, 0, bar);
           if constexpr (!PACKED) {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              tma_box<true>(base + kHalf + i * kBox, &a.b, a.b_mn ? jb + 64 * i : kb * kDepth,
-                            a.b_mn ? kb * kDepth : jb + 64 * i, 0, bar);
+              tma_box<true>(smem0 + P::kBAt + s * kHalf + i * kBox, &a.b,
+                            a.b_mn ? jb + 64 * i : kb * kDepth, a.b_mn ? kb * kDepth : jb + 64 * i,
+                            0, bar);
           }
         }
       }
       // copies still in flight land before the block ends
       for (unsigned i = n > (unsigned)S ? n - S : 0; rank == 0 && i < n; ++i)
-        mbar_wait(&full[i % S], (i / S) & 1, a.err);
+        stage_wait(&full[i % S], (i / S) & 1, a.err);
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
@@ -359,23 +412,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
         const int buf = tile & 1;
         if (tile >= 2) wait_pair(&tm_empty[buf], (tile / 2 - 1) & 1, a.err);
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        bool ready = false;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
           const int s = n % S;
-          mbar_wait(&full[s], (n / S) & 1, a.err);
-          if (PACKED) mbar_wait(&ready[s], (n / S) & 1, a.err);
+          if (!ready) stage_wait(&full[s], (n / S) & 1, a.err);
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-          const unsigned base = smem0 + s * P::kStage;
-          const unsigned long long p = operand(base), q = operand(base + kHalf);
+          const unsigned long long p = operand(smem0 + s * kHalf),
+                                   q = operand(smem0 + P::kBAt + s * kHalf);
 #pragma unroll
-          for (int k = 0; k < kDepth / 16; ++k)
+          for (int k = 0; k < kDepth / 16; ++k) {
             mma_f16<true>(tmem + buf * 256, p + k * as, q + k * bs, idesc, kb > t.kb0 || k > 0);
+            // the next stage is asked for while this one's products run: few are queued,
+            // and a poll takes longer than the last of them
+            if (k == 1) ready = kb + 1 < t.kb1 && mbar_peek(&full[(n + 1) % S], ((n + 1) / S) & 1);
+          }
           mma_commit<true>(&empty[s]);
         }
         mma_commit<true>(&tm_full[buf]);
       }
       // products still in flight end before tensor memory is given back
       mma_commit<true>(&drain);
-      mbar_wait(&drain, 0, a.err);
+      stage_wait(&drain, 0, a.err);
     }
   } else if (PACKED && warp == 3) {
     // codes of a stage, and their ranges: 4 words a lane, zeros (operands of zero)
@@ -384,11 +441,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
     for (int item = first; work_of(a, item, &t); item += step) {
       const int jb = t.j0 + rank * 128, g = jb / kGroup8 + (lane & 1);
       for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
-        const int s = n % R;
-        if (n >= (unsigned)R) mbar_wait(&raw_empty[s], (n / R - 1) & 1, a.err);
+        const int s = n % SC;
+        if (n >= (unsigned)SC) warp_wait(&c_empty[s], (n / SC - 1) & 1, a.err);
         if (lane == 0) {
-          mbar_expect_tx(&raw[s], kRaw);
-          tma_box<false>(smem0 + P::kRawAt + s * kRaw, &a.b, jb, kb * kDepth, 0, smem_u32(&raw[s]));
+          mbar_expect_tx(&c_full[s], kRaw);
+          tma_box<false>(smem0 + P::kCodesAt + s * kRaw, &a.b, jb, kb * kDepth, 0,
+                         smem_u32(&c_full[s]));
         }
         const unsigned to = smem0 + P::kRangesAt + s * kRanges + lane * 4;
 #pragma unroll
@@ -400,13 +458,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
                        : "memory");
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(
-                         smem_u32(&raw[s]))
+                         smem_u32(&c_full[s]))
                      : "memory");
       }
     }
     asm volatile("cp.async.wait_all;\n" ::: "memory");
-    for (unsigned i = n > (unsigned)R ? n - R : 0; i < n; ++i)
-      mbar_wait(&raw[i % R], (i / R) & 1, a.err);
+    for (unsigned i = n > (unsigned)SC ? n - SC : 0; i < n; ++i)
+      warp_wait(&c_full[i % SC], (i / SC) & 1, a.err);
   } else if (PACKED && warp >= 4 && warp < 4 + P::kWriters) {
     // Two teams of four warps take the stages in turn, so that one team's loads and
     // barriers run beside the other's arithmetic.  A thread has 16 columns of four of
@@ -417,9 +475,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
     for (int item = first; work_of(a, item, &t); item += step) {
       for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
         if ((int)(n & 1) != team) continue;
-        const int s = n % S, c = n % R;
-        mbar_wait(&raw[c], (n / R) & 1, a.err);
-        const char* const codes = smem + P::kRawAt + c * kRaw + seg * 16;
+        const int s = n % S, c = n % SC;
+        warp_wait(&c_full[c], (n / SC) & 1, a.err);
+        const char* const codes = smem + P::kCodesAt + c * kRaw + seg * 16;
         const unsigned* const ranges =
             reinterpret_cast<const unsigned*>(smem + P::kRangesAt + c * kRanges) + odd;
         uint4 q[4];
@@ -429,8 +487,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
           q[h] = *reinterpret_cast<const uint4*>(codes + (row + 16 * h) * 128);
           bits[h] = ranges[(row + 16 * h) * 2];
         }
-        if (n >= (unsigned)S) mbar_wait(&empty[s], (n / S - 1) & 1, a.err);
-        char* const stage = smem + s * P::kStage + kHalf + odd * kBox;
+        if (n >= (unsigned)S) warp_wait(&empty[s], (n / S - 1) & 1, a.err);
+        // Only now: the codes of stage n + 5 then follow this stage's phase, so that the
+        // other team, whose that stage is, cannot take an older phase for it.
+        __syncwarp();
+        if (lane == 0) arrive_leader<false>(&c_empty[c]);
+        char* const stage = smem + P::kBAt + s * kHalf + odd * kBox;
 #pragma unroll
         for (int h = 0; h < 4; ++h) {
           const int r = row + 16 * h;
@@ -444,10 +506,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) {
-          arrive_written(&ready[s]);
-          arrive_leader<false>(&raw_empty[c]);
-        }
+        if (lane == 0) arrive_written(&full[s]);
       }
     }
   } else if (warp >= 4 + P::kWriters) {
@@ -457,7 +516,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
     unsigned tile = 0;
     for (int item = first; work_of(a, item, &t); item += step, ++tile) {
       const int buf = tile & 1;
-      wait_pair(&tm_full[buf], (tile / 2) & 1, a.err);
+      if (lane == 0) wait_pair(&tm_full[buf], (tile / 2) & 1, a.err);
+      __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       const int i = t.i0 + rank * 128 + 32 * w;
 #pragma unroll 1
@@ -491,7 +551,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
   cluster_sync();  // neither block's memory is in use any more
   // The first block has issued its last commit, which arrives at the second
   // block's barriers too: that block stays until it has.
-  if (rank == 1 && threadIdx.x == 32) mbar_wait(&drain, 0, a.err);
+  if (rank == 1 && threadIdx.x == 32) stage_wait(&drain, 0, a.err);
   if (warp == 2) {
     asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
