@@ -21,81 +21,162 @@ struct Rows8 {
   unsigned char* codes;
   void* ranges;
   long long units;      // rows x per_row
-  long long per_row;    // units of a row
+  long long per_row;    // units of a row; 0 where the rows join to one long one
+  unsigned inv;         // 1 / per_row, see rows8
+  int shift;
   int width;
-  int tanh_form;
 };
 
 enum { OP_PACK, OP_UNPACK, OP_GELU, OP_GELU_PACK, OP_GELU_GRAD };
 
-__device__ __forceinline__ float gelu_value(float x, int tanh_form) {
-  if (tanh_form) {
-    const float u = 0.7978845608028654f * (x + 0.044715f * x * x * x);
-    return 0.5f * x * (1.f + tanhf(u));
-  }
-  return x * normcdff(x);
+// exp(-x^2 / 2) and the upper tail of the normal distribution at |x|, to 1e-7:
+// Abramowitz and Stegun's 7.1.26 (Hastings), erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2),
+// t = 1 / (1 + p z), with the halves folded in.  A third of normcdff's instructions,
+// which bound the 16-bit kernels; what is then rounded to 16 bits does not see 1e-7.
+__device__ __forceinline__ float normal_tail(float x, float* bell) {
+  const float e = exp2f(x * x * -0.7213475204444817f);
+  const float t = __fdividef(1.f, fmaf(fabsf(x), 0.3275911f * 0.7071067811865476f, 1.f));
+  float p = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+  p = fmaf(p, t, 0.5f * 1.421413741f);
+  p = fmaf(p, t, 0.5f * -0.284496736f);
+  p = fmaf(p, t, 0.5f * 0.254829592f);
+  *bell = e;
+  return p * t * e;
 }
-__device__ __forceinline__ float gelu_slope(float x, int tanh_form) {
-  if (tanh_form) {
-    const float u = 0.7978845608028654f * (x + 0.044715f * x * x * x);
-    const float t = tanhf(u);
-    return 0.5f * (1.f + t) + 0.5f * x * (1.f - t * t) * 0.7978845608028654f *
-                                  (1.f + 3.f * 0.044715f * x * x);
-  }
-  return normcdff(x) + x * (0.3989422804014327f * expf(-0.5f * x * x));
+// (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)); `sq` is x^2, held where x^3 would overflow.
+__device__ __forceinline__ float tanh_factor(float x, float sq) {
+  const float u2 = x * fmaf(sq, 2.f * 0.7978845608028654f * 0.044715f, 2.f * 0.7978845608028654f);
+  return 1.f / (1.f + expf(-u2));
 }
 
-template <typename T, int OP, bool VEC>
+// `FAST`: for results of 16 bits.
+template <bool TANH, bool FAST>
+__device__ __forceinline__ float gelu_value(float x) {
+  if constexpr (TANH) {
+    const float sq = fminf(x * x, 1e12f);
+    if constexpr (FAST) {
+      const float u2 = x * fmaf(sq, -2.3022082f * 0.044715f, -2.3022082f);  // -2 sqrt(2/pi) log2(e)
+      return __fdividef(x, 1.f + exp2f(u2));
+    }
+    return x * tanh_factor(x, sq);
+  } else if constexpr (FAST) {
+    float bell;
+    const float q = normal_tail(x, &bell);
+    return x * (x >= 0.f ? 1.f - q : q);
+  } else {
+    return x * normcdff(x);
+  }
+}
+template <bool TANH, bool FAST>
+__device__ __forceinline__ float gelu_slope(float x) {
+  if constexpr (TANH) {
+    const float sq = fminf(x * x, 1e12f);
+    float f;
+    if constexpr (FAST)
+      f = __fdividef(1.f, 1.f + exp2f(x * fmaf(sq, -2.3022082f * 0.044715f, -2.3022082f)));
+    else
+      f = tanh_factor(x, sq);
+    // f + x f (1 - f) 2 u'
+    return fmaf(x * f * (1.f - f),
+                fmaf(sq, 6.f * 0.7978845608028654f * 0.044715f, 2.f * 0.7978845608028654f), f);
+  } else if constexpr (FAST) {
+    float bell;
+    const float q = normal_tail(x, &bell);
+    return fmaf(x * 0.3989422804014327f, bell, x >= 0.f ? 1.f - q : q);
+  } else {
+    return normcdff(x) + x * (0.3989422804014327f * expf(-0.5f * x * x));
+  }
+}
+
+// Bound by bytes: a thread has kUnits units at a time, whose loads are all under way
+// before the first is used, and a row's place takes one multiplication (`inv`).
+constexpr int kUnits = 4;
+
+template <typename T, int OP, bool VEC, bool TANH>
 __global__ void __launch_bounds__(256) rows8_kernel(const Rows8 a) {
   typedef typename RangeBits<T>::type Bits;
+  constexpr bool FAST = sizeof(T) == 2;
   // whole warps stay together: a row is a multiple of 8 units, a warp's 32 may span rows
-  for (long long u0 = (long long)blockIdx.x * 256; u0 < a.units; u0 += (long long)gridDim.x * 256) {
-    const long long u = u0 + threadIdx.x;
-    const bool in = u < a.units;
-    const long long row = in ? u / a.per_row : 0;
-    const long long unit = in ? u - row * a.per_row : 0;
-    const long long c = unit * 8;
-    const int n = in ? (int)max(0ll, min(8ll, a.width - c)) : 0;
-    uint2* const code = reinterpret_cast<uint2*>(a.codes) + u;
-    Bits* const bits = reinterpret_cast<Bits*>(a.ranges) + u / 8;
-    const T* const xp = reinterpret_cast<const T*>(a.x) + row * a.x_row + c;
-    T* const yp = reinterpret_cast<T*>(a.y) + row * a.y_row + c;
-    float x[8];
-    if constexpr (OP == OP_PACK || OP == OP_GELU || OP == OP_GELU_PACK) {
-      load8<T, VEC>(xp, n, x);
-      if constexpr (OP != OP_GELU) {
-        Range8 r;
-        const uint2 q = encode8<T>(x, n, &r);
-        if (in) {
-          *code = q;
-          if ((u & 7) == 0) *bits = range_bits(r, T());
+  const long long step = (long long)gridDim.x * (256 * kUnits);
+  for (long long u0 = (long long)blockIdx.x * (256 * kUnits); u0 < a.units; u0 += step) {
+    Raw8<T> raw[kUnits];
+    uint2 code[kUnits];
+    Bits bits[kUnits];
+    int n[kUnits];
+    long long at[kUnits];       // of this unit in y (and x where they are laid out alike)
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      const long long u = u0 + k * 256 + threadIdx.x;
+      n[k] = 0;
+      at[k] = 0;
+      if (u < a.units) {
+        long long row, c;
+        if (a.per_row == 0) {   // one long row
+          row = 0;
+          c = u * 8;
+          n[k] = 8;
+        } else {
+          row = a.units <= 0x7fffffffll
+                    ? (long long)(__umulhi((unsigned)u, a.inv) >> a.shift)
+                    : u / a.per_row;
+          c = (u - row * a.per_row) * 8;
+          n[k] = (int)max(0ll, min(8ll, a.width - c));
         }
+        at[k] = row * a.y_row + c;
+        if constexpr (OP != OP_UNPACK)
+          raw[k] = raw8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n[k]);
+        if constexpr (OP == OP_UNPACK || OP == OP_GELU_GRAD) {
+          code[k] = __ldg(reinterpret_cast<const uint2*>(a.codes) + u);
+          bits[k] = __ldg(reinterpret_cast<const Bits*>(a.ranges) + u / 8);
+        }
+      } else if constexpr (OP != OP_UNPACK) {
+        raw[k] = raw8<T, VEC>(nullptr, 0);
       }
-      if constexpr (OP != OP_PACK) {
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = gelu_value(x[i], a.tanh_form);
-        store8<T, VEC>(yp, n, x);
-      }
-    } else if (in) {
-      decode8<T>(*code, range_of(*bits, T()), x);
-      if constexpr (OP == OP_GELU_GRAD) {
-        float g[8];
-        load8<T, VEC>(xp, n, g);
+    for (int k = 0; k < kUnits; ++k) {
+      const long long u = u0 + k * 256 + threadIdx.x;
+      const bool in = u < a.units;
+      T* const yp = reinterpret_cast<T*>(a.y) + at[k];
+      float x[8];
+      if constexpr (OP == OP_PACK || OP == OP_GELU || OP == OP_GELU_PACK) {
+        widen8(raw[k], x);
+        if constexpr (OP != OP_GELU) {
+          Range8 r;
+          const uint2 q = encode8<T>(x, n[k], &r);
+          if (in) {
+            reinterpret_cast<uint2*>(a.codes)[u] = q;
+            if ((u & 7) == 0) reinterpret_cast<Bits*>(a.ranges)[u / 8] = range_bits(r, T());
+          }
+        }
+        if constexpr (OP != OP_PACK) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = g[i] * gelu_slope(x[i], a.tanh_form);
+          for (int i = 0; i < 8; ++i) x[i] = gelu_value<TANH, FAST>(x[i]);
+          if (in) store8<T, VEC>(yp, n[k], x);
+        }
+      } else if (in) {
+        decode8<T>(code[k], range_of(bits[k], T()), x);
+        if constexpr (OP == OP_GELU_GRAD) {
+          float g[8];
+          widen8(raw[k], g);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = g[i] * gelu_slope<TANH, FAST>(x[i]);
+        }
+        store8<T, VEC>(yp, n[k], x);
       }
-      store8<T, VEC>(yp, n, x);
     }
   }
 }
 
-template <typename T, int OP>
+template <typename T, int OP, bool TANH>
 static int rows8_run(const Rows8& a, bool vec, int device, cudaStream_t st) {
-  const long long blocks = std::min((a.units + 255) / 256, (long long)sm_count(device) * 32);
+  // fewer and longer-lived blocks than units: 8 a multiprocessor run at once
+  const long long blocks =
+      std::min((a.units + 256 * kUnits - 1) / (256 * kUnits), (long long)sm_count(device) * 64);
   if (vec)
-    rows8_kernel<T, OP, true><<<(unsigned)blocks, 256, 0, st>>>(a);
+    rows8_kernel<T, OP, true, TANH><<<(unsigned)blocks, 256, 0, st>>>(a);
   else
-    rows8_kernel<T, OP, false><<<(unsigned)blocks, 256, 0, st>>>(a);
+    rows8_kernel<T, OP, false, TANH><<<(unsigned)blocks, 256, 0, st>>>(a);
   FAB_LAUNCH_CHECK();
   return FA_OK;
 }
@@ -124,16 +205,29 @@ static int rows8(int op, const void* x, long long x_row, void* y, long long y_ro
   if (rows > (1ll << 62) / a.per_row) return FA_E_SHAPE;
   a.units = rows * a.per_row;
   a.width = width;
-  a.tanh_form = tanh_form;
+  // u / per_row for u < 2^31: with 2^s >= per_row, (u ceil(2^(31 + s) / per_row)) >> (31 + s)
+  a.shift = 0;
+  while ((1ll << a.shift) < a.per_row) ++a.shift;
+  a.inv = (unsigned)(((1ull << (31 + a.shift)) + a.per_row - 1) / a.per_row);
+  a.shift -= 1;                 // the high word is 32 of the 31 + s
   const bool vec = (!x || whole8(x, x_row, rows, width, item)) &&
                    (!y || whole8(y, y_row, rows, width, item));
+  if (width % kGroup8 == 0 && (!x || rows == 1 || x_row == width) &&
+      (!y || rows == 1 || y_row == width))
+    a.per_row = 0;
   FAB_DEVICE_SCOPE(device);
   FAB_FOR_TYPE(dtype, T, switch (op) {
-    case OP_PACK: return rows8_run<T, OP_PACK>(a, vec, device, st);
-    case OP_UNPACK: return rows8_run<T, OP_UNPACK>(a, vec, device, st);
-    case OP_GELU: return rows8_run<T, OP_GELU>(a, vec, device, st);
-    case OP_GELU_PACK: return rows8_run<T, OP_GELU_PACK>(a, vec, device, st);
-    default: return rows8_run<T, OP_GELU_GRAD>(a, vec, device, st);
+    case OP_PACK: return rows8_run<T, OP_PACK, false>(a, vec, device, st);
+    case OP_UNPACK: return rows8_run<T, OP_UNPACK, false>(a, vec, device, st);
+    case OP_GELU:
+      return tanh_form ? rows8_run<T, OP_GELU, true>(a, vec, device, st)
+                       : rows8_run<T, OP_GELU, false>(a, vec, device, st);
+    case OP_GELU_PACK:
+      return tanh_form ? rows8_run<T, OP_GELU_PACK, true>(a, vec, device, st)
+                       : rows8_run<T, OP_GELU_PACK, false>(a, vec, device, st);
+    default:
+      return tanh_form ? rows8_run<T, OP_GELU_GRAD, true>(a, vec, device, st)
+                       : rows8_run<T, OP_GELU_GRAD, false>(a, vec, device, st);
   });
 }
 

@@ -188,6 +188,60 @@ __device__ __forceinline__ void store8(T* p, int n, const float (&x)[8]) {
   }
 }
 
+// 8 values as they lie in memory: loaded early, widened where they are used.
+template <typename T> struct Raw8 {
+  uint4 v;
+};
+template <> struct Raw8<float> {
+  float4 a, b;
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw8<T> raw8(const T* p, int n) {
+  Raw8<T> r;
+  if constexpr (sizeof(T) == 4) {
+    r.a = r.b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if constexpr (VEC) {
+      if (n) {
+        r.a = __ldg(reinterpret_cast<const float4*>(p));
+        r.b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+      }
+    } else {
+      float x[8];
+      load8<T, false>(p, n, x);
+      r.a = make_float4(x[0], x[1], x[2], x[3]);
+      r.b = make_float4(x[4], x[5], x[6], x[7]);
+    }
+  } else {
+    r.v = make_uint4(0u, 0u, 0u, 0u);
+    if constexpr (VEC) {
+      if (n) r.v = __ldg(reinterpret_cast<const uint4*>(p));
+    } else {
+      unsigned w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = 2 * i < n ? (unsigned)ldro(p + 2 * i).bits : 0u;
+        if (2 * i + 1 < n) w[i] |= (unsigned)ldro(p + 2 * i + 1).bits << 16;
+      }
+      r.v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  return r;
+}
+__device__ __forceinline__ void widen8(const Raw8<float>& r, float (&x)[8]) {
+  x[0] = r.a.x; x[1] = r.a.y; x[2] = r.a.z; x[3] = r.a.w;
+  x[4] = r.b.x; x[5] = r.b.y; x[6] = r.b.z; x[7] = r.b.w;
+}
+template <typename T>
+__device__ __forceinline__ void widen8(const Raw8<T>& r, float (&x)[8]) {
+  const unsigned w[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    T v;
+    v.bits = (unsigned short)(w[i / 2] >> (16 * (i & 1)));
+    x[i] = Ld<T>::f(v);
+  }
+}
+
 // Whether rows at p are whole aligned vectors of 8.
 static inline bool whole8(const void* p, long long row_stride, long long rows, int width,
                           int item) {

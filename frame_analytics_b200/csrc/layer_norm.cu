@@ -22,6 +22,7 @@ struct NormArgs {
   long long x_row, res_row;
   const void *w, *b;            // or null
   int w32;                      // weights are float32
+  int w_vec;                    // and start at whole vectors
   void *y, *sum;                // forward: outputs, sum or null; backward: y is dx
   const void *dy, *ds;          // upstream gradients, ds or null
   long long dy_row, ds_row;
@@ -38,15 +39,18 @@ struct NormArgs {
 };
 
 // n weights from column c; `none` where there are none.
-template <typename T>
-__device__ __forceinline__ void weights8(const void* w, int w32, int c, int n, float none,
+template <typename T, bool VEC>
+__device__ __forceinline__ void weights8(const NormArgs& a, const void* w, int c, int n, float none,
                                          float (&x)[8]) {
+  if (!w) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = none;
-    if (w && i < n)
-      x[i] = w32 ? __ldg(reinterpret_cast<const float*>(w) + c + i)
-                 : Ld<T>::f(ldro(reinterpret_cast<const T*>(w) + c + i));
+    for (int i = 0; i < 8; ++i) x[i] = none;
+  } else if (a.w32) {
+    const float* p = reinterpret_cast<const float*>(w) + c;
+    if (VEC && a.w_vec) load8<float, true>(p, n, x); else load8<float, false>(p, n, x);
+  } else {
+    const T* p = reinterpret_cast<const T*>(w) + c;
+    if (VEC && a.w_vec) load8<T, true>(p, n, x); else load8<T, false>(p, n, x);
   }
 }
 
@@ -72,6 +76,189 @@ __device__ __forceinline__ void kept8(const NormArgs& a, long long row, int c, i
   const uint2 q = __ldg(reinterpret_cast<const uint2*>(a.codes + row * a.groups * kGroup8 + c));
   decode8<T>(q, range_of(__ldg(reinterpret_cast<const typename RangeBits<T>::type*>(a.ranges) + g),
                          T()), x);
+}
+
+// Rows that fit the registers of up to 32 warps: E units of 8 columns a lane, `wpr`
+// warps a row, every byte read and written once.
+template <typename T, bool VEC, int E, int NT>
+__global__ void __launch_bounds__(NT) norm_kernel(const NormArgs a, int wpr) {
+  __shared__ float sm[2][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int at = warp % wpr, first = warp - at;          // this warp in its row, the row's first
+  const long long row = (long long)blockIdx.x * (blockDim.x / 32 / wpr) + warp / wpr;
+  const bool in = row < a.rows;
+  const int units = a.groups * 8;
+  float x[E][8];
+  {
+    Raw8<T> r[E], q[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = ((e * wpr + at) * 32 + lane) * 8, n = in ? max(0, min(8, a.width - c)) : 0;
+      r[e] = raw8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n);
+      if (a.res) q[e] = raw8<T, VEC>(reinterpret_cast<const T*>(a.res) + row * a.res_row + c, n);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      widen8(r[e], x[e]);
+      if (a.res) {
+        float y[8];
+        widen8(q[e], y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[e][i] = round_to<T>(x[e][i] + y[i]);
+      }
+    }
+  }
+  const auto row_sum = [&](float t, int k) {
+    t = warp_sum(t);
+    if (wpr == 1) return t;
+    if (lane == 0) sm[k][warp] = t;
+    __syncthreads();
+    t = 0.f;
+    for (int w = 0; w < wpr; ++w) t += sm[k][first + w];
+    return t;
+  };
+  float t = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += x[e][i];
+  const float m = row_sum(t, 0) / (float)a.width;
+  t = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int n = a.width - ((e * wpr + at) * 32 + lane) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < n) t = fmaf(x[e][i] - m, x[e][i] - m, t);
+  }
+  const float r = 1.f / sqrtf(row_sum(t, 1) / (float)a.width + a.eps);
+  if (!in) return;
+  if (a.stats && at == 0 && lane == 0) a.stats[row] = make_float2(m, r);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int u = (e * wpr + at) * 32 + lane, c = u * 8, n = max(0, min(8, a.width - c));
+    if (a.sum) store8<T, VEC>(reinterpret_cast<T*>(a.sum) + row * a.width + c, n, x[e]);
+    if (a.codes) {
+      Range8 range;
+      const uint2 q = encode8<T>(x[e], n, &range);
+      if (u < units) {
+        reinterpret_cast<uint2*>(a.codes)[row * units + u] = q;
+        if ((u & 7) == 0)
+          reinterpret_cast<typename RangeBits<T>::type*>(a.ranges)[row * a.groups + u / 8] =
+              range_bits(range, T());
+      }
+    }
+    float w[8], b[8];
+    weights8<T, VEC>(a, a.w, c, n, 1.f, w);
+    weights8<T, VEC>(a, a.b, c, n, 0.f, b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[e][i] = fmaf((x[e][i] - m) * r, w[i], b[i]);
+    store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, x[e]);
+  }
+}
+
+// The backward pass of such rows: blocks stay and take rows in turn; a lane keeps the
+// weight gradients of its columns in registers, the block adds its rows' at the end
+// and writes one part.  x, dy and ds stay in registers as they lie in memory.
+template <typename T, bool VEC, int E, bool CODES, int NT>
+__global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs a, int wpr) {
+  __shared__ float2 sm[2][NT / 32];
+  __shared__ float join[NT / 32][32 * 9];
+  typedef typename RangeBits<T>::type Bits;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int at = warp % wpr, first = warp - at, rpb = NT / 32 / wpr;
+  float dw[E][8] = {}, db[E][8] = {};
+  int turn = 0;
+  for (long long row0 = (long long)blockIdx.x * rpb; row0 < a.rows;
+       row0 += (long long)gridDim.x * rpb, turn ^= 1) {
+    const long long row = row0 + warp / wpr;
+    const bool in = row < a.rows;
+    Raw8<T> xr[E], gr[E], sr[E];
+    uint2 code[E];
+    Bits bits[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int u = (e * wpr + at) * 32 + lane, c = u * 8, n = in ? max(0, min(8, a.width - c)) : 0;
+      if constexpr (CODES) {
+        code[e] = make_uint2(0u, 0u);
+        bits[e] = Bits();
+        if (n) {
+          code[e] = __ldg(reinterpret_cast<const uint2*>(a.codes) + row * a.groups * 8 + u);
+          bits[e] = __ldg(reinterpret_cast<const Bits*>(a.ranges) + row * a.groups + u / 8);
+        }
+      } else {
+        xr[e] = raw8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n);
+      }
+      gr[e] = raw8<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.dy_row + c, n);
+      if (a.ds) sr[e] = raw8<T, VEC>(reinterpret_cast<const T*>(a.ds) + row * a.ds_row + c, n);
+    }
+    const float2 st = in ? __ldg(a.stats + row) : make_float2(0.f, 0.f);
+    float c1 = 0.f, c2 = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = ((e * wpr + at) * 32 + lane) * 8, n = in ? max(0, min(8, a.width - c)) : 0;
+      float x[8], g[8], w[8];
+      if constexpr (CODES) decode8<T>(code[e], range_of(bits[e], T()), x); else widen8(xr[e], x);
+      widen8(gr[e], g);
+      weights8<T, VEC>(a, a.w, c, n, 1.f, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float h = i < n ? (x[i] - st.x) * st.y : 0.f, gw = g[i] * w[i];
+        dw[e][i] = fmaf(g[i], h, dw[e][i]);
+        db[e][i] += g[i];
+        c1 += gw;
+        c2 = fmaf(gw, h, c2);
+      }
+    }
+    c1 = warp_sum(c1);
+    c2 = warp_sum(c2);
+    if (wpr > 1) {
+      if (lane == 0) sm[turn][warp] = make_float2(c1, c2);
+      __syncthreads();          // one a row: the next row's sums have the other half
+      c1 = c2 = 0.f;
+      for (int w = 0; w < wpr; ++w) {
+        c1 += sm[turn][first + w].x;
+        c2 += sm[turn][first + w].y;
+      }
+    }
+    c1 /= (float)a.width;
+    c2 /= (float)a.width;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = ((e * wpr + at) * 32 + lane) * 8, n = in ? max(0, min(8, a.width - c)) : 0;
+      float x[8], g[8], w[8];
+      if constexpr (CODES) decode8<T>(code[e], range_of(bits[e], T()), x); else widen8(xr[e], x);
+      widen8(gr[e], g);
+      weights8<T, VEC>(a, a.w, c, n, 1.f, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        x[i] = st.y * (g[i] * w[i] - c1 - (x[i] - st.x) * st.y * c2);
+      if (a.ds) {
+        widen8(sr[e], g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] += g[i];
+      }
+      if (in) store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, x);
+    }
+  }
+  if (!a.dw && !a.db) return;
+  // warps that hold the same columns, in the order of their rows
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (!(k ? a.db : a.dw)) continue;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) join[warp][lane * 9 + i] = k ? db[e][i] : dw[e][i];
+      __syncthreads();
+      for (int j = threadIdx.x; j < wpr * 256; j += NT) {
+        const int w = j / 256, l = j % 256, col = (e * wpr + w) * 256 + l;
+        float t = 0.f;
+        for (int q = 0; q < rpb; ++q) t += join[q * wpr + w][l / 8 * 9 + l % 8];
+        if (col < a.width) a.part[((long long)blockIdx.x * 2 + k) * a.width + col] = t;
+      }
+    }
 }
 
 // A block to a row, which it reads again for each of its sums (from the
@@ -115,8 +302,8 @@ __global__ void __launch_bounds__(256) norm_rows_kernel(const NormArgs a) {
                 range_bits(range, T());
         }
       }
-      weights8<T>(a.w, a.w32, c, n, 1.f, w);
-      weights8<T>(a.b, a.w32, c, n, 0.f, b);
+      weights8<T, VEC>(a, a.w, c, n, 1.f, w);
+      weights8<T, VEC>(a, a.b, c, n, 0.f, b);
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = fmaf((x[i] - m) * r, w[i], b[i]);
       store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, x);
@@ -135,7 +322,7 @@ __global__ void __launch_bounds__(256) norm_grad_rows_kernel(const NormArgs a) {
       const int c = u * 8, n = max(0, min(8, a.width - c));
       kept8<T, VEC>(a, row, c, n, x);
       load8<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.dy_row + c, n, g);
-      weights8<T>(a.w, a.w32, c, n, 1.f, w);
+      weights8<T, VEC>(a, a.w, c, n, 1.f, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         if (i < n) {
@@ -149,7 +336,7 @@ __global__ void __launch_bounds__(256) norm_grad_rows_kernel(const NormArgs a) {
       const int c = u * 8, n = max(0, min(8, a.width - c));
       kept8<T, VEC>(a, row, c, n, x);
       load8<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.dy_row + c, n, g);
-      weights8<T>(a.w, a.w32, c, n, 1.f, w);
+      weights8<T, VEC>(a, a.w, c, n, 1.f, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
         x[i] = st.y * (g[i] * w[i] - c1 - (x[i] - st.x) * st.y * c2);
@@ -173,6 +360,7 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const NormArgs a) {
   const bool hats = a.x || a.codes;
   float dw[8] = {}, db[8] = {};
   const long long step = (long long)gridDim.y * 8;
+#pragma unroll 4
   for (long long row = blockIdx.y * 8ll + warp; row < a.rows; row += step) {
     float g[8], x[8];
     load8<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.dy_row + c, n, g);
@@ -204,21 +392,22 @@ __global__ void __launch_bounds__(256) column_sums_kernel(const NormArgs a) {
 
 // The parts' sums in their order, rounded to the weights' type.
 template <typename T>
-__global__ void __launch_bounds__(256) column_join_kernel(const NormArgs a) {
-  __shared__ float sm[8][33];
+__global__ void __launch_bounds__(1024) column_join_kernel(const NormArgs a) {
+  __shared__ float sm[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
   void* const out = blockIdx.y ? a.db : a.dw;
   if (!out) return;
   float t = 0.f;
   if (col < a.width)
-    for (int i = warp; i < a.splits; i += 8)
+#pragma unroll 8
+    for (int i = warp; i < a.splits; i += 32)
       t += a.part[((long long)i * 2 + blockIdx.y) * a.width + col];
   sm[warp][lane] = t;
   __syncthreads();
   if (warp || col >= a.width) return;
   t = 0.f;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) t += sm[w][lane];
+  for (int w = 0; w < 32; ++w) t += sm[w][lane];
   if (a.w32)
     reinterpret_cast<float*>(out)[col] = t;
   else
@@ -237,8 +426,39 @@ static int column_splits(long long rows, int width, int device) {
   return (int)std::min(most, (long long)std::max(1, sm_count(device) * 6 / strips));
 }
 
+// Warps that share a row and units of 8 columns a lane; 0 where a row does not fit.
+struct RowShape {
+  int wpr, e;
+};
+static RowShape forward_shape(int width) {
+  const long long units = groups8(width) * 8;
+  if (units <= 32) return {1, 1};
+  if (units <= 64) return {1, 2};
+  const long long wpr = (units + 127) / 128;
+  return wpr <= 32 ? RowShape{(int)wpr, 4} : RowShape{0, 0};
+}
+static RowShape backward_shape(int width) {
+  const long long units = groups8(width) * 8;
+  if (units <= 32) return {1, 1};
+  int wpr = 1;
+  while (wpr < 16 && units > 64ll * wpr) wpr *= 2;
+  return units <= 64ll * wpr ? RowShape{wpr, 2} : RowShape{0, 0};
+}
+// Blocks of the backward pass: 512 threads a multiprocessor, each with rows to take.
+static int backward_blocks(long long rows, int rpb, int threads, int device) {
+  return (int)std::min((rows + rpb - 1) / rpb, (long long)(512 / threads) * sm_count(device));
+}
+
 size_t norm_ws_bytes(long long rows, int width, int device) {
-  return (size_t)column_splits(rows, width, device) * 2 * (size_t)width * sizeof(float);
+  const int parts = std::max(column_splits(rows, width, device), 2 * sm_count(device));
+  return (size_t)parts * 2 * (size_t)width * sizeof(float);
+}
+
+template <typename T>
+static int column_join(const NormArgs& a, cudaStream_t st) {
+  column_join_kernel<T><<<dim3((unsigned)((a.width + 31) / 32), 2), 1024, 0, st>>>(a);
+  FAB_LAUNCH_CHECK();
+  return FA_OK;
 }
 
 template <typename T>
@@ -250,11 +470,8 @@ static int column_sums(NormArgs& a, bool vec, int device, cudaStream_t st) {
   else
     column_sums_kernel<T, false><<<grid, 256, 0, st>>>(a);
   FAB_LAUNCH_CHECK();
-  column_join_kernel<T><<<dim3((unsigned)((a.width + 31) / 32), 2), 256, 0, st>>>(a);
-  FAB_LAUNCH_CHECK();
-  return FA_OK;
+  return column_join<T>(a, st);
 }
-
 // Column sums of g alone (a bias's gradient), in the gradient's type.
 int bias_grad_impl(const void* g, long long g_row, void* db, int dtype, long long rows, int width,
                    void* ws, size_t ws_bytes, int device, cudaStream_t st) {
@@ -294,6 +511,7 @@ static NormArgs norm_args(const fa_norm& p) {
   a.w = p.weight;
   a.b = p.bias;
   a.w32 = p.weight_dtype == FA_F32;
+  a.w_vec = reinterpret_cast<size_t>(p.weight) % 16 == 0 && reinterpret_cast<size_t>(p.bias) % 16 == 0;
   a.stats = reinterpret_cast<float2*>(p.stats);
   a.codes = static_cast<unsigned char*>(p.codes);
   a.ranges = p.ranges;
@@ -304,8 +522,33 @@ static NormArgs norm_args(const fa_norm& p) {
   return a;
 }
 
+template <typename T, int E>
+static void norm_launch(const NormArgs& a, int wpr, bool vec, cudaStream_t st) {
+  const int rpb = wpr == 1 ? 4 : 1;
+  const unsigned grid = (unsigned)((a.rows + rpb - 1) / rpb);
+  const unsigned threads = 32 * wpr * rpb;
+  if (E == 4 && threads > 512) {
+    if (vec)
+      norm_kernel<T, true, 4, 1024><<<grid, threads, 0, st>>>(a, wpr);
+    else
+      norm_kernel<T, false, 4, 1024><<<grid, threads, 0, st>>>(a, wpr);
+  } else if (vec) {
+    norm_kernel<T, true, E, 512><<<grid, threads, 0, st>>>(a, wpr);
+  } else {
+    norm_kernel<T, false, E, 512><<<grid, threads, 0, st>>>(a, wpr);
+  }
+}
+
 template <typename T>
 static int norm_run(const NormArgs& a, bool vec, int device, cudaStream_t st) {
+  const RowShape shape = forward_shape(a.width);
+  if (shape.wpr && a.rows < 1ll << 31) {
+    if (shape.e == 1) norm_launch<T, 1>(a, shape.wpr, vec, st);
+    else if (shape.e == 2) norm_launch<T, 2>(a, shape.wpr, vec, st);
+    else norm_launch<T, 4>(a, shape.wpr, vec, st);
+    FAB_LAUNCH_CHECK();
+    return FA_OK;
+  }
   const unsigned grid = (unsigned)std::min(a.rows, (long long)sm_count(device) * 8);
   if (vec)
     norm_rows_kernel<T, true><<<grid, 256, 0, st>>>(a);
@@ -337,8 +580,28 @@ int norm_impl(const fa_norm* p, void* y, void* sum, int device, cudaStream_t st)
   FAB_FOR_TYPE(p->dtype, T, return norm_run<T>(a, vec, device, st));
 }
 
+template <typename T, int E, int NT>
+static int norm_grad_launch(NormArgs& a, int wpr, bool vec, int device, cudaStream_t st) {
+  a.splits = backward_blocks(a.rows, NT / 32 / wpr, NT, device);
+  const unsigned grid = (unsigned)a.splits;
+  if (a.codes && vec)
+    norm_grad_kernel<T, true, E, true, NT><<<grid, NT, 0, st>>>(a, wpr);
+  else if (a.codes)
+    norm_grad_kernel<T, false, E, true, NT><<<grid, NT, 0, st>>>(a, wpr);
+  else if (vec)
+    norm_grad_kernel<T, true, E, false, NT><<<grid, NT, 0, st>>>(a, wpr);
+  else
+    norm_grad_kernel<T, false, E, false, NT><<<grid, NT, 0, st>>>(a, wpr);
+  FAB_LAUNCH_CHECK();
+  return a.dw || a.db ? column_join<T>(a, st) : FA_OK;
+}
+
 template <typename T>
 static int norm_grad_run(NormArgs& a, bool vec, int device, cudaStream_t st) {
+  const RowShape shape = backward_shape(a.width);
+  if (shape.e == 1) return norm_grad_launch<T, 1, 256>(a, shape.wpr, vec, device, st);
+  if (shape.wpr > 8) return norm_grad_launch<T, 2, 512>(a, shape.wpr, vec, device, st);
+  if (shape.wpr) return norm_grad_launch<T, 2, 256>(a, shape.wpr, vec, device, st);
   const unsigned grid = (unsigned)std::min(a.rows, (long long)sm_count(device) * 8);
   if (vec)
     norm_grad_rows_kernel<T, true><<<grid, 256, 0, st>>>(a);
