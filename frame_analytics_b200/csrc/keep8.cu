@@ -96,6 +96,8 @@ template <typename T, int OP, bool VEC, bool TANH>
 __global__ void __launch_bounds__(256) rows8_kernel(const Rows8 a) {
   typedef typename RangeBits<T>::type Bits;
   constexpr bool FAST = sizeof(T) == 2;
+  __shared__ __align__(16) Turn8<T> turns[VEC ? 1 : 8];
+  Turn8<T>* const turn = turns + (VEC ? 0 : threadIdx.x / 32);
   // whole warps stay together: a row is a multiple of 8 units, a warp's 32 may span rows
   const long long step = (long long)gridDim.x * (256 * kUnits);
   for (long long u0 = (long long)blockIdx.x * (256 * kUnits); u0 < a.units; u0 += step) {
@@ -103,12 +105,16 @@ __global__ void __launch_bounds__(256) rows8_kernel(const Rows8 a) {
     uint2 code[kUnits];
     Bits bits[kUnits];
     int n[kUnits];
-    long long at[kUnits];       // of this unit in y (and x where they are laid out alike)
+    long long at[kUnits];       // of this unit in y
+    const T* from[kUnits];
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
       const long long u = u0 + k * 256 + threadIdx.x;
       n[k] = 0;
       at[k] = 0;
+      from[k] = reinterpret_cast<const T*>(a.x);
+      code[k] = make_uint2(0u, 0u);
+      bits[k] = Bits();
       if (u < a.units) {
         long long row, c;
         if (a.per_row == 0) {   // one long row
@@ -123,15 +129,13 @@ __global__ void __launch_bounds__(256) rows8_kernel(const Rows8 a) {
           n[k] = (int)max(0ll, min(8ll, a.width - c));
         }
         at[k] = row * a.y_row + c;
-        if constexpr (OP != OP_UNPACK)
-          raw[k] = raw8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n[k]);
+        from[k] = reinterpret_cast<const T*>(a.x) + row * a.x_row + c;
         if constexpr (OP == OP_UNPACK || OP == OP_GELU_GRAD) {
           code[k] = __ldg(reinterpret_cast<const uint2*>(a.codes) + u);
           bits[k] = __ldg(reinterpret_cast<const Bits*>(a.ranges) + u / 8);
         }
-      } else if constexpr (OP != OP_UNPACK) {
-        raw[k] = raw8<T, VEC>(nullptr, 0);
       }
+      if constexpr (OP != OP_UNPACK) raw[k] = fetch8<T, VEC>(from[k], n[k], turn);
     }
 #pragma unroll
     for (int k = 0; k < kUnits; ++k) {
@@ -143,7 +147,9 @@ __global__ void __launch_bounds__(256) rows8_kernel(const Rows8 a) {
         widen8(raw[k], x);
         if constexpr (OP != OP_GELU) {
           Range8 r;
-          const uint2 q = encode8<T>(x, n[k], &r);
+          float lo, hi;
+          extent8<VEC>(raw[k], n[k], &lo, &hi);
+          const uint2 q = encode8<T, VEC>(x, n[k], lo, hi, &r);
           if (in) {
             reinterpret_cast<uint2*>(a.codes)[u] = q;
             if ((u & 7) == 0) reinterpret_cast<Bits*>(a.ranges)[u / 8] = range_bits(r, T());
@@ -152,9 +158,9 @@ __global__ void __launch_bounds__(256) rows8_kernel(const Rows8 a) {
         if constexpr (OP != OP_PACK) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = gelu_value<TANH, FAST>(x[i]);
-          if (in) store8<T, VEC>(yp, n[k], x);
+          put8<T, VEC>(yp, n[k], x, turn);
         }
-      } else if (in) {
+      } else {
         decode8<T>(code[k], range_of(bits[k], T()), x);
         if constexpr (OP == OP_GELU_GRAD) {
           float g[8];
@@ -162,7 +168,7 @@ __global__ void __launch_bounds__(256) rows8_kernel(const Rows8 a) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = g[i] * gelu_slope<TANH, FAST>(x[i]);
         }
-        store8<T, VEC>(yp, n[k], x);
+        put8<T, VEC>(yp, n[k], x, turn);
       }
     }
   }

@@ -82,25 +82,34 @@ __device__ __forceinline__ Range8 range_of(unsigned b, T) {
   return {Ld<T>::f(lo), __uint_as_float(b & 0xffff0000u)};
 }
 
-// Range and codes of a group spread over 8 neighbouring lanes, 8 values a lane of
-// which the first n exist.  Every lane of the warp takes part.
-template <typename T>
-__device__ __forceinline__ uint2 encode8(const float (&x)[8], int n, Range8* r) {
-  float a = __uint_as_float(0x7f800000u), b = __uint_as_float(0xff800000u);
+// Lowest and highest of the first n of 8 values; VEC: n is 8 or 0.  A NaN among them
+// is both.
+template <bool VEC>
+__device__ __forceinline__ void extent8(const float (&x)[8], int n, float* lo, float* hi) {
+  *lo = __uint_as_float(0x7f800000u);
+  *hi = __uint_as_float(0xff800000u);
+  if (VEC && n == 0) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (i < n) {
-      a = min_nan(a, x[i]);
-      b = max_nan(b, x[i]);
+    if (VEC || i < n) {
+      *lo = min_nan(*lo, x[i]);
+      *hi = max_nan(*hi, x[i]);
     }
+}
+
+// Range and codes of a group spread over 8 neighbouring lanes, 8 values a lane of
+// which the first n exist and span [lo, hi].  Every lane of the warp takes part.
+template <typename T, bool VEC>
+__device__ __forceinline__ uint2 encode8(const float (&x)[8], int n, float lo, float hi,
+                                         Range8* r) {
 #pragma unroll
   for (int o = 1; o < 8; o <<= 1) {
-    a = min_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
-    b = max_nan(b, __shfl_xor_sync(0xffffffffu, b, o));
+    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
-  const float d = b - a;
+  const float d = hi - lo;
   const unsigned u = __float_as_uint(d);
-  r->lo = a;
+  r->lo = lo;
   if (!(d < __uint_as_float(0x7f800000u))) {
     r->s = __uint_as_float(0x7fc00000u);
     return make_uint2(0u, 0u);
@@ -109,16 +118,24 @@ __device__ __forceinline__ uint2 encode8(const float (&x)[8], int n, Range8* r) 
   const int e = max((int)(u >> 23) - 7 + (int)((u & 0x7fffffu) > 0x7f0000u), 1);
   r->s = __uint_as_float((unsigned)e << 23);
   const float inv = __uint_as_float((unsigned)(254 - e) << 23);
-  float top = kMagic8 + 255.f;
-  const float high = fmaf(d, inv, kMagic8);
-  if (fmaf(high - kMagic8, r->s, a) >= Over<T>::v()) top = high - 1.f;
-  unsigned q[8];
+  float q[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    q[i] = i < n ? __float_as_uint(fminf(fmaf(x[i] - a, inv, kMagic8), top)) : 0u;
+  for (int i = 0; i < 8; ++i) q[i] = fmaf(x[i] - lo, inv, kMagic8);
+  const float high = fmaf(d, inv, kMagic8);
+  if (fmaf(high - kMagic8, r->s, lo) >= Over<T>::v()) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = fminf(q[i], high - 1.f);
+  }
+  if (!VEC || n == 0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i >= n) q[i] = kMagic8;
+  }
   uint2 c;
-  c.x = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
-  c.y = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+#define FAB_LOW2(I) __byte_perm(__float_as_uint(q[I]), __float_as_uint(q[I + 1]), 0x0040)
+  c.x = __byte_perm(FAB_LOW2(0), FAB_LOW2(2), 0x5410);
+  c.y = __byte_perm(FAB_LOW2(4), FAB_LOW2(6), 0x5410);
+#undef FAB_LOW2
   return c;
 }
 
@@ -239,6 +256,132 @@ __device__ __forceinline__ void widen8(const Raw8<T>& r, float (&x)[8]) {
     T v;
     v.bits = (unsigned short)(w[i / 2] >> (16 * (i & 1)));
     x[i] = Ld<T>::f(v);
+  }
+}
+
+// The extent of 8 values as they lie: two 16-bit values an instruction.
+template <bool VEC>
+__device__ __forceinline__ void extent8(const Raw8<float>& r, int n, float* lo, float* hi) {
+  float x[8];
+  widen8(r, x);
+  extent8<VEC>(x, n, lo, hi);
+}
+template <bool VEC, typename T>
+__device__ __forceinline__ void extent8(const Raw8<T>& r, int n, float* lo, float* hi) {
+  if (!VEC && n != 8) {
+    float x[8];
+    widen8(r, x);
+    extent8<false>(x, n, lo, hi);
+    return;
+  }
+  *lo = __uint_as_float(0x7f800000u);
+  *hi = __uint_as_float(0xff800000u);
+  if (n == 0) return;
+  unsigned a = r.v.x, b = r.v.x;
+#define FAB_EXTENT(W)                                                                    \
+  if constexpr (std::is_same<T, bf16_t>::value) {                                        \
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(W));                        \
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(b), "r"(W));                        \
+  } else {                                                                               \
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(a), "r"(W));                         \
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(b) : "r"(b), "r"(W));                         \
+  }
+  FAB_EXTENT(r.v.y)
+  FAB_EXTENT(r.v.z)
+  FAB_EXTENT(r.v.w)
+#undef FAB_EXTENT
+  T l, h;
+  l.bits = (unsigned short)a;
+  h.bits = (unsigned short)(a >> 16);
+  *lo = min_nan(Ld<T>::f(l), Ld<T>::f(h));
+  l.bits = (unsigned short)b;
+  h.bits = (unsigned short)(b >> 16);
+  *hi = max_nan(Ld<T>::f(l), Ld<T>::f(h));
+}
+
+// 8 values rounded to T, as they lie.
+__device__ __forceinline__ Raw8<float> narrow8(const float (&x)[8], float) {
+  Raw8<float> r;
+  r.a = make_float4(x[0], x[1], x[2], x[3]);
+  r.b = make_float4(x[4], x[5], x[6], x[7]);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ Raw8<T> narrow8(const float (&x)[8], T) {
+  unsigned w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = (unsigned)St<T>::v(x[2 * i]).bits | ((unsigned)St<T>::v(x[2 * i + 1]).bits << 16);
+  Raw8<T> r;
+  r.v = make_uint4(w[0], w[1], w[2], w[3]);
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void put8(T* p, const Raw8<T>& r) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = r.a;
+    reinterpret_cast<float4*>(p)[1] = r.b;
+  } else {
+    *reinterpret_cast<uint4*>(p) = r.v;
+  }
+}
+
+// Rows that are not whole aligned vectors: a warp's 256 values go through shared
+// memory, so that neighbouring lanes touch neighbouring addresses (a lane's 8 values
+// with 8 loads or stores of its own touch 16 sectors an instruction, 2 bytes of each).
+// `p` is the lane's place, of which the first n values exist.
+template <typename T>
+struct Turn8 {
+  T v[256];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> gather8(const T* p, int n, Turn8<T>* t) {
+  const int lane = threadIdx.x & 31;
+  const unsigned long long at = reinterpret_cast<unsigned long long>(p);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int s = i * 4 + (lane >> 3), j = lane & 7;
+    const T* const q = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, at, s)) + j;
+    T v = T();
+    if (j < __shfl_sync(0xffffffffu, n, s)) v = ldro(q);
+    t->v[i * 32 + lane] = v;
+  }
+  __syncwarp();
+  Raw8<T> r;
+  if constexpr (sizeof(T) == 4) {
+    r.a = reinterpret_cast<const float4*>(t->v + lane * 8)[0];
+    r.b = reinterpret_cast<const float4*>(t->v + lane * 8)[1];
+  } else {
+    r.v = *reinterpret_cast<const uint4*>(t->v + lane * 8);
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void scatter8(T* p, int n, const Raw8<T>& r, Turn8<T>* t) {
+  const int lane = threadIdx.x & 31;
+  const unsigned long long at = reinterpret_cast<unsigned long long>(p);
+  __syncwarp();
+  put8<T>(t->v + lane * 8, r);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int s = i * 4 + (lane >> 3), j = lane & 7;
+    T* const q = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, at, s)) + j;
+    if (j < __shfl_sync(0xffffffffu, n, s)) *q = t->v[i * 32 + lane];
+  }
+}
+// Either way of loading and storing; every lane of the warp takes part.
+template <typename T, bool VEC>
+__device__ __forceinline__ Raw8<T> fetch8(const T* p, int n, Turn8<T>* t) {
+  if constexpr (VEC) return raw8<T, true>(p, n); else return gather8<T>(p, n, t);
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void put8(T* p, int n, const float (&x)[8], Turn8<T>* t) {
+  if constexpr (VEC) {
+    if (n) put8<T>(p, narrow8(x, T()));
+  } else {
+    scatter8<T>(p, n, narrow8(x, T()), t);
   }
 }
 

@@ -83,28 +83,36 @@ __device__ __forceinline__ void kept8(const NormArgs& a, long long row, int c, i
 template <typename T, bool VEC, int E, int NT>
 __global__ void __launch_bounds__(NT) norm_kernel(const NormArgs a, int wpr) {
   __shared__ float sm[2][32];
+  __shared__ __align__(16) Turn8<T> turns[VEC ? 1 : NT / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Turn8<T>* const turn = turns + (VEC ? 0 : warp);
   const int at = warp % wpr, first = warp - at;          // this warp in its row, the row's first
   const long long row = (long long)blockIdx.x * (blockDim.x / 32 / wpr) + warp / wpr;
   const bool in = row < a.rows;
   const int units = a.groups * 8;
-  float x[E][8];
+  // s stays as it lies in memory and is widened for each of the three passes over it:
+  // half the registers of float32 values, so twice the rows under way
+  Raw8<T> s[E];
+  int n[E];
   {
-    Raw8<T> r[E], q[E];
+    Raw8<T> q[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = ((e * wpr + at) * 32 + lane) * 8, n = in ? max(0, min(8, a.width - c)) : 0;
-      r[e] = raw8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n);
-      if (a.res) q[e] = raw8<T, VEC>(reinterpret_cast<const T*>(a.res) + row * a.res_row + c, n);
+      const int c = ((e * wpr + at) * 32 + lane) * 8;
+      n[e] = in ? max(0, min(8, a.width - c)) : 0;
+      s[e] = fetch8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n[e], turn);
+      if (a.res)
+        q[e] = fetch8<T, VEC>(reinterpret_cast<const T*>(a.res) + row * a.res_row + c, n[e], turn);
     }
+    if (a.res) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      widen8(r[e], x[e]);
-      if (a.res) {
-        float y[8];
+      for (int e = 0; e < E; ++e) {
+        float x[8], y[8];
+        widen8(s[e], x);
         widen8(q[e], y);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[e][i] = round_to<T>(x[e][i] + y[i]);
+        for (int i = 0; i < 8; ++i) x[i] += y[i];
+        s[e] = narrow8(x, T());
       }
     }
   }
@@ -119,29 +127,37 @@ __global__ void __launch_bounds__(NT) norm_kernel(const NormArgs a, int wpr) {
   };
   float t = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
+  for (int e = 0; e < E; ++e) {
+    float x[8];
+    widen8(s[e], x);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t += x[e][i];
+    for (int i = 0; i < 8; ++i) t += x[i];
+  }
   const float m = row_sum(t, 0) / (float)a.width;
   t = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int n = a.width - ((e * wpr + at) * 32 + lane) * 8;
+    if (VEC && n[e] == 0) continue;
+    float x[8];
+    widen8(s[e], x);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < n) t = fmaf(x[e][i] - m, x[e][i] - m, t);
+      if (VEC || i < n[e]) t = fmaf(x[i] - m, x[i] - m, t);
   }
   const float r = 1.f / sqrtf(row_sum(t, 1) / (float)a.width + a.eps);
-  if (!in) return;
-  if (a.stats && at == 0 && lane == 0) a.stats[row] = make_float2(m, r);
+  if (a.stats && in && at == 0 && lane == 0) a.stats[row] = make_float2(m, r);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int u = (e * wpr + at) * 32 + lane, c = u * 8, n = max(0, min(8, a.width - c));
-    if (a.sum) store8<T, VEC>(reinterpret_cast<T*>(a.sum) + row * a.width + c, n, x[e]);
+    const int u = (e * wpr + at) * 32 + lane, c = u * 8;
+    float x[8];
+    widen8(s[e], x);
+    if (a.sum) put8<T, VEC>(reinterpret_cast<T*>(a.sum) + row * a.width + c, n[e], x, turn);
     if (a.codes) {
       Range8 range;
-      const uint2 q = encode8<T>(x[e], n, &range);
-      if (u < units) {
+      float lo, hi;
+      extent8<VEC>(s[e], n[e], &lo, &hi);
+      const uint2 q = encode8<T, VEC>(x, n[e], lo, hi, &range);
+      if (in && u < units) {
         reinterpret_cast<uint2*>(a.codes)[row * units + u] = q;
         if ((u & 7) == 0)
           reinterpret_cast<typename RangeBits<T>::type*>(a.ranges)[row * a.groups + u / 8] =
@@ -149,11 +165,11 @@ __global__ void __launch_bounds__(NT) norm_kernel(const NormArgs a, int wpr) {
       }
     }
     float w[8], b[8];
-    weights8<T, VEC>(a, a.w, c, n, 1.f, w);
-    weights8<T, VEC>(a, a.b, c, n, 0.f, b);
+    weights8<T, VEC>(a, a.w, c, n[e], 1.f, w);
+    weights8<T, VEC>(a, a.b, c, n[e], 0.f, b);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[e][i] = fmaf((x[e][i] - m) * r, w[i], b[i]);
-    store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, x[e]);
+    for (int i = 0; i < 8; ++i) x[i] = fmaf((x[i] - m) * r, w[i], b[i]);
+    put8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n[e], x, turn);
   }
 }
 
@@ -164,46 +180,62 @@ template <typename T, bool VEC, int E, bool CODES, int NT>
 __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs a, int wpr) {
   __shared__ float2 sm[2][NT / 32];
   __shared__ float join[NT / 32][32 * 9];
+  __shared__ __align__(16) Turn8<T> turns[VEC ? 1 : NT / 32];
   typedef typename RangeBits<T>::type Bits;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Turn8<T>* const turn = turns + (VEC ? 0 : warp);
   const int at = warp % wpr, first = warp - at, rpb = NT / 32 / wpr;
   float dw[E][8] = {}, db[E][8] = {};
-  int turn = 0;
-  for (long long row0 = (long long)blockIdx.x * rpb; row0 < a.rows;
-       row0 += (long long)gridDim.x * rpb, turn ^= 1) {
-    const long long row = row0 + warp / wpr;
-    const bool in = row < a.rows;
-    Raw8<T> xr[E], gr[E], sr[E];
+  // what a row's loads bring; the next row's are under way while this one's sums run
+  struct Row {
+    Raw8<T> x[E], g[E], s[E];
     uint2 code[E];
     Bits bits[E];
+    float2 st;
+  };
+  const auto load = [&](long long row, Row& o) {
+    const bool in = row < a.rows;
+    if (!in) row = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int u = (e * wpr + at) * 32 + lane, c = u * 8, n = in ? max(0, min(8, a.width - c)) : 0;
       if constexpr (CODES) {
-        code[e] = make_uint2(0u, 0u);
-        bits[e] = Bits();
+        o.code[e] = make_uint2(0u, 0u);
+        o.bits[e] = Bits();
         if (n) {
-          code[e] = __ldg(reinterpret_cast<const uint2*>(a.codes) + row * a.groups * 8 + u);
-          bits[e] = __ldg(reinterpret_cast<const Bits*>(a.ranges) + row * a.groups + u / 8);
+          o.code[e] = __ldg(reinterpret_cast<const uint2*>(a.codes) + row * a.groups * 8 + u);
+          o.bits[e] = __ldg(reinterpret_cast<const Bits*>(a.ranges) + row * a.groups + u / 8);
         }
       } else {
-        xr[e] = raw8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n);
+        o.x[e] = fetch8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n, turn);
       }
-      gr[e] = raw8<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.dy_row + c, n);
-      if (a.ds) sr[e] = raw8<T, VEC>(reinterpret_cast<const T*>(a.ds) + row * a.ds_row + c, n);
+      o.g[e] = fetch8<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.dy_row + c, n, turn);
+      if (a.ds) o.s[e] = fetch8<T, VEC>(reinterpret_cast<const T*>(a.ds) + row * a.ds_row + c, n, turn);
     }
-    const float2 st = in ? __ldg(a.stats + row) : make_float2(0.f, 0.f);
+    o.st = in ? __ldg(a.stats + row) : make_float2(0.f, 0.f);
+  };
+  const long long step = (long long)gridDim.x * rpb;
+  int half = 0;
+  Row now, next;
+  load((long long)blockIdx.x * rpb + warp / wpr, now);
+  for (long long row0 = (long long)blockIdx.x * rpb; row0 < a.rows; row0 += step, half ^= 1) {
+    const long long row = row0 + warp / wpr;
+    const bool in = row < a.rows;
+    load(row + step, next);
+    const float2 st = now.st;
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = ((e * wpr + at) * 32 + lane) * 8, n = in ? max(0, min(8, a.width - c)) : 0;
+      if (VEC && n == 0) continue;
       float x[8], g[8], w[8];
-      if constexpr (CODES) decode8<T>(code[e], range_of(bits[e], T()), x); else widen8(xr[e], x);
-      widen8(gr[e], g);
+      if constexpr (CODES) decode8<T>(now.code[e], range_of(now.bits[e], T()), x);
+      else widen8(now.x[e], x);
+      widen8(now.g[e], g);
       weights8<T, VEC>(a, a.w, c, n, 1.f, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float h = i < n ? (x[i] - st.x) * st.y : 0.f, gw = g[i] * w[i];
+        const float h = VEC || i < n ? (x[i] - st.x) * st.y : 0.f, gw = g[i] * w[i];
         dw[e][i] = fmaf(g[i], h, dw[e][i]);
         db[e][i] += g[i];
         c1 += gw;
@@ -213,12 +245,12 @@ __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs 
     c1 = warp_sum(c1);
     c2 = warp_sum(c2);
     if (wpr > 1) {
-      if (lane == 0) sm[turn][warp] = make_float2(c1, c2);
+      if (lane == 0) sm[half][warp] = make_float2(c1, c2);
       __syncthreads();          // one a row: the next row's sums have the other half
       c1 = c2 = 0.f;
       for (int w = 0; w < wpr; ++w) {
-        c1 += sm[turn][first + w].x;
-        c2 += sm[turn][first + w].y;
+        c1 += sm[half][first + w].x;
+        c2 += sm[half][first + w].y;
       }
     }
     c1 /= (float)a.width;
@@ -227,19 +259,21 @@ __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs 
     for (int e = 0; e < E; ++e) {
       const int c = ((e * wpr + at) * 32 + lane) * 8, n = in ? max(0, min(8, a.width - c)) : 0;
       float x[8], g[8], w[8];
-      if constexpr (CODES) decode8<T>(code[e], range_of(bits[e], T()), x); else widen8(xr[e], x);
-      widen8(gr[e], g);
+      if constexpr (CODES) decode8<T>(now.code[e], range_of(now.bits[e], T()), x);
+      else widen8(now.x[e], x);
+      widen8(now.g[e], g);
       weights8<T, VEC>(a, a.w, c, n, 1.f, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        x[i] = st.y * (g[i] * w[i] - c1 - (x[i] - st.x) * st.y * c2);
+        x[i] = st.y * (fmaf(g[i], w[i], -c1) - (x[i] - st.x) * st.y * c2);
       if (a.ds) {
-        widen8(sr[e], g);
+        widen8(now.s[e], g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] += g[i];
       }
-      if (in) store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, x);
+      put8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, x, turn);
     }
+    now = next;
   }
   if (!a.dw && !a.db) return;
   // warps that hold the same columns, in the order of their rows
@@ -294,7 +328,9 @@ __global__ void __launch_bounds__(256) norm_rows_kernel(const NormArgs a) {
         store8<T, VEC>(reinterpret_cast<T*>(a.sum) + row * a.width + c, n, x);
       if (a.codes) {
         Range8 range;
-        const uint2 q = encode8<T>(x, n, &range);
+        float lo, hi;
+        extent8<VEC>(x, n, &lo, &hi);
+        const uint2 q = encode8<T, VEC>(x, n, lo, hi, &range);
         if (u < units) {
           reinterpret_cast<uint2*>(a.codes)[row * units + u] = q;
           if ((u & 7) == 0)
@@ -437,12 +473,14 @@ static RowShape forward_shape(int width) {
   const long long wpr = (units + 127) / 128;
   return wpr <= 32 ? RowShape{(int)wpr, 4} : RowShape{0, 0};
 }
-static RowShape backward_shape(int width) {
+// float32 rows hold one unit a lane where that covers the row: two take more registers
+// than there are.
+static RowShape backward_shape(int width, int item) {
   const long long units = groups8(width) * 8;
-  if (units <= 32) return {1, 1};
-  int wpr = 1;
-  while (wpr < 16 && units > 64ll * wpr) wpr *= 2;
-  return units <= 64ll * wpr ? RowShape{wpr, 2} : RowShape{0, 0};
+  for (int e = 1; e <= 2; ++e)
+    for (int wpr = 1; wpr <= 16; wpr *= 2)
+      if (units <= 32ll * e * wpr && (e == 2 || item == 4 || wpr == 1)) return {wpr, e};
+  return {0, 0};
 }
 // Blocks of the backward pass: 512 threads a multiprocessor, each with rows to take.
 static int backward_blocks(long long rows, int rpb, int threads, int device) {
@@ -598,7 +636,10 @@ static int norm_grad_launch(NormArgs& a, int wpr, bool vec, int device, cudaStre
 
 template <typename T>
 static int norm_grad_run(NormArgs& a, bool vec, int device, cudaStream_t st) {
-  const RowShape shape = backward_shape(a.width);
+  const RowShape shape = backward_shape(a.width, sizeof(T));
+  if constexpr (sizeof(T) == 4)
+    if (shape.e == 1 && shape.wpr > 8)
+      return norm_grad_launch<T, 1, 512>(a, shape.wpr, vec, device, st);
   if (shape.e == 1) return norm_grad_launch<T, 1, 256>(a, shape.wpr, vec, device, st);
   if (shape.wpr > 8) return norm_grad_launch<T, 2, 512>(a, shape.wpr, vec, device, st);
   if (shape.wpr) return norm_grad_launch<T, 2, 256>(a, shape.wpr, vec, device, st);
