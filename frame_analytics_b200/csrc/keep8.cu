@@ -29,62 +29,89 @@ struct Rows8 {
 
 enum { OP_PACK, OP_UNPACK, OP_GELU, OP_GELU_PACK, OP_GELU_GRAD };
 
-// exp(-x^2 / 2) and the upper tail of the normal distribution at |x|, to 1e-7:
-// Abramowitz and Stegun's 7.1.26 (Hastings), erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2),
-// t = 1 / (1 + p z), with the halves folded in.  A third of normcdff's instructions,
-// which bound the 16-bit kernels; what is then rounded to 16 bits does not see 1e-7.
-__device__ __forceinline__ float normal_tail(float x, float* bell) {
-  const float e = exp2f(x * x * -0.7213475204444817f);
-  const float t = __fdividef(1.f, fmaf(fabsf(x), 0.3275911f * 0.7071067811865476f, 1.f));
-  float p = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
-  p = fmaf(p, t, 0.5f * 1.421413741f);
-  p = fmaf(p, t, 0.5f * -0.284496736f);
-  p = fmaf(p, t, 0.5f * 0.254829592f);
-  *bell = e;
-  return p * t * e;
+__device__ __forceinline__ float2 exp2_fast(float2 v) {
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(v.x));
+  asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(v.y));
+  return v;
 }
-// (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)); `sq` is x^2, held where x^3 would overflow.
-__device__ __forceinline__ float tanh_factor(float x, float sq) {
-  const float u2 = x * fmaf(sq, 2.f * 0.7978845608028654f * 0.044715f, 2.f * 0.7978845608028654f);
-  return 1.f / (1.f + expf(-u2));
+__device__ __forceinline__ float2 over(float2 v) {  // 1 / v
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(v.x));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(v.y));
+  return v;
+}
+constexpr float kTanhIn = 0.7978845608028654f;   // sqrt(2 / pi)
+constexpr float kCube = 0.044715f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kBell = 0.3989422804014327f;     // 1 / sqrt(2 pi)
+
+// Results of 16 bits.  The upper tail of the normal distribution is, to 1e-7,
+// Abramowitz and Stegun's 7.1.26 (Hastings): erfc(z) = (a1 t + ... + a5 t^5) exp(-z^2),
+// t = 1 / (1 + p z).  Returned: t (a1 + ... + a5 t^4) / 2, with z = a / sqrt(2), a >= 0.
+// normcdff and expf take three times the instructions, which bound these kernels.
+__device__ __forceinline__ float2 tail_factor(float2 a) {
+  const float2 t = over(__ffma2_rn(a, both(0.3275911f * 0.7071067811865476f), both(1.f)));
+  float2 p = __ffma2_rn(t, both(0.5f * 1.061405429f), both(0.5f * -1.453152027f));
+  p = __ffma2_rn(p, t, both(0.5f * 1.421413741f));
+  p = __ffma2_rn(p, t, both(0.5f * -0.284496736f));
+  p = __ffma2_rn(p, t, both(0.5f * 0.254829592f));
+  return __fmul2_rn(p, t);
 }
 
-// `FAST`: for results of 16 bits.
+// (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)); `sq` is x^2, held where x^3 would overflow.
+__device__ __forceinline__ float tanh_factor(float x, float sq) {
+  return 1.f / (1.f + expf(-x * fmaf(sq, 2.f * kTanhIn * kCube, 2.f * kTanhIn)));
+}
+__device__ __forceinline__ float2 tanh_factor_fast(float2 x, float2 sq) {
+  const float2 u = __ffma2_rn(sq, both(-2.f * kTanhIn * kLog2e * kCube), both(-2.f * kTanhIn * kLog2e));
+  return over(__fadd2_rn(both(1.f), exp2_fast(__fmul2_rn(x, u))));
+}
+__device__ __forceinline__ float2 square(float2 x) {
+  const float2 s = __fmul2_rn(x, x);
+  return make_float2(fminf(s.x, 1e12f), fminf(s.y, 1e12f));
+}
+
+// `FAST`: for results of 16 bits.  Below -64 the value is zero; an infinity or a NaN
+// passes as such.
 template <bool TANH, bool FAST>
-__device__ __forceinline__ float gelu_value(float x) {
+__device__ __forceinline__ float2 gelu_value(float2 x) {
   if constexpr (TANH) {
-    const float sq = fminf(x * x, 1e12f);
-    if constexpr (FAST) {
-      const float u2 = x * fmaf(sq, -2.3022082f * 0.044715f, -2.3022082f);  // -2 sqrt(2/pi) log2(e)
-      return __fdividef(x, 1.f + exp2f(u2));
-    }
-    return x * tanh_factor(x, sq);
+    const float2 sq = square(x);
+    const float2 m = make_float2(max_nan(x.x, -64.f), max_nan(x.y, -64.f));
+    if constexpr (FAST) return __fmul2_rn(m, tanh_factor_fast(x, sq));
+    return make_float2(m.x * tanh_factor(x.x, sq.x), m.y * tanh_factor(x.y, sq.y));
   } else if constexpr (FAST) {
-    float bell;
-    const float q = normal_tail(x, &bell);
-    return x * (x >= 0.f ? 1.f - q : q);
+    // x Phi(x) = max(x, 0) - a Q(a), a = |x|, Q the upper tail
+    const float2 a = make_float2(min_nan(fabsf(x.x), 64.f), min_nan(fabsf(x.y), 64.f));
+    const float2 c = __fmul2_rn(a, both(-0.5f * kLog2e));
+    const float2 q = __fmul2_rn(tail_factor(a), exp2_fast(__fmul2_rn(c, a)));
+    return make_float2(fmaf(-a.x, q.x, max_nan(x.x, 0.f)), fmaf(-a.y, q.y, max_nan(x.y, 0.f)));
   } else {
-    return x * normcdff(x);
+    return make_float2(max_nan(x.x, -64.f) * normcdff(x.x), max_nan(x.y, -64.f) * normcdff(x.y));
   }
 }
 template <bool TANH, bool FAST>
-__device__ __forceinline__ float gelu_slope(float x) {
+__device__ __forceinline__ float2 gelu_slope(float2 x) {
   if constexpr (TANH) {
-    const float sq = fminf(x * x, 1e12f);
-    float f;
-    if constexpr (FAST)
-      f = __fdividef(1.f, 1.f + exp2f(x * fmaf(sq, -2.3022082f * 0.044715f, -2.3022082f)));
-    else
-      f = tanh_factor(x, sq);
+    const float2 sq = square(x);
+    float2 f;
+    if constexpr (FAST) f = tanh_factor_fast(x, sq);
+    else f = make_float2(tanh_factor(x.x, sq.x), tanh_factor(x.y, sq.y));
     // f + x f (1 - f) 2 u'
-    return fmaf(x * f * (1.f - f),
-                fmaf(sq, 6.f * 0.7978845608028654f * 0.044715f, 2.f * 0.7978845608028654f), f);
+    const float2 g = __ffma2_rn(f, make_float2(-f.x, -f.y), f);
+    const float2 u = __ffma2_rn(sq, both(6.f * kTanhIn * kCube), both(2.f * kTanhIn));
+    return __ffma2_rn(__fmul2_rn(x, g), u, f);
   } else if constexpr (FAST) {
-    float bell;
-    const float q = normal_tail(x, &bell);
-    return fmaf(x * 0.3989422804014327f, bell, x >= 0.f ? 1.f - q : q);
+    // with a = |x|: 1/2 + sign(x) (1/2 - Q(a) + a phi(a)), Q = bell factor(a)
+    const float2 a = make_float2(fabsf(x.x), fabsf(x.y));
+    const float2 e = exp2_fast(__fmul2_rn(__fmul2_rn(x, both(-0.5f * kLog2e)), x));
+    const float2 k = __ffma2_rn(a, both(kBell), __fmul2_rn(tail_factor(a), both(-1.f)));
+    const float2 v = __ffma2_rn(k, e, both(0.5f));
+    return __fadd2_rn(both(0.5f),
+                      make_float2(__uint_as_float(__float_as_uint(v.x) ^ (__float_as_uint(x.x) & 0x80000000u)),
+                                  __uint_as_float(__float_as_uint(v.y) ^ (__float_as_uint(x.y) & 0x80000000u))));
   } else {
-    return normcdff(x) + x * (0.3989422804014327f * expf(-0.5f * x * x));
+    return make_float2(normcdff(x.x) + x.x * (kBell * expf(-0.5f * x.x * x.x)),
+                       normcdff(x.y) + x.y * (kBell * expf(-0.5f * x.y * x.y)));
   }
 }
 
@@ -142,9 +169,8 @@ __global__ void __launch_bounds__(256) rows8_kernel(const Rows8 a) {
       const long long u = u0 + k * 256 + threadIdx.x;
       const bool in = u < a.units;
       T* const yp = reinterpret_cast<T*>(a.y) + at[k];
-      float x[8];
       if constexpr (OP == OP_PACK || OP == OP_GELU || OP == OP_GELU_PACK) {
-        widen8(raw[k], x);
+        F8 x = widen8(raw[k]);
         if constexpr (OP != OP_GELU) {
           Range8 r;
           float lo, hi;
@@ -157,18 +183,18 @@ __global__ void __launch_bounds__(256) rows8_kernel(const Rows8 a) {
         }
         if constexpr (OP != OP_PACK) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = gelu_value<TANH, FAST>(x[i]);
-          put8<T, VEC>(yp, n[k], x, turn);
+          for (int i = 0; i < 4; ++i) x.v[i] = gelu_value<TANH, FAST>(x.v[i]);
+          store8<T, VEC>(yp, n[k], x, turn);
         }
       } else {
-        decode8<T>(code[k], range_of(bits[k], T()), x);
+        F8 x = decode8<T>(code[k], range_of(bits[k], T()));
         if constexpr (OP == OP_GELU_GRAD) {
-          float g[8];
-          widen8(raw[k], g);
+          const F8 g = widen8(raw[k]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = g[i] * gelu_slope<TANH, FAST>(x[i]);
+          for (int i = 0; i < 4; ++i)
+            x.v[i] = __fmul2_rn(g.v[i], gelu_slope<TANH, FAST>(x.v[i]));
         }
-        put8<T, VEC>(yp, n[k], x, turn);
+        store8<T, VEC>(yp, n[k], x, turn);
       }
     }
   }

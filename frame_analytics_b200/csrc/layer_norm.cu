@@ -40,42 +40,71 @@ struct NormArgs {
 
 // n weights from column c; `none` where there are none.
 template <typename T, bool VEC>
-__device__ __forceinline__ void weights8(const NormArgs& a, const void* w, int c, int n, float none,
-                                         float (&x)[8]) {
+__device__ __forceinline__ F8 weights8(const NormArgs& a, const void* w, int c, int n, float none) {
+  F8 x;
   if (!w) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = none;
+    for (int i = 0; i < 4; ++i) x.v[i] = both(none);
   } else if (a.w32) {
     const float* p = reinterpret_cast<const float*>(w) + c;
-    if (VEC && a.w_vec) load8<float, true>(p, n, x); else load8<float, false>(p, n, x);
+    x = VEC && a.w_vec && n == 8 ? widen8(get8<float>(p)) : few8<float>(p, n);
   } else {
     const T* p = reinterpret_cast<const T*>(w) + c;
-    if (VEC && a.w_vec) load8<T, true>(p, n, x); else load8<T, false>(p, n, x);
+    x = VEC && a.w_vec && n == 8 ? widen8(get8<T>(p)) : few8<T>(p, n);
   }
+  return x;
 }
-
-// s of 8 columns, from the sum that this thread wrote earlier or from the inputs.
-template <typename T, bool VEC>
-__device__ __forceinline__ void input8(const NormArgs& a, long long row, int c, int n,
-                                       float (&x)[8]) {
-  load8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n, x);
-  if (a.res) {
-    float r[8];
-    load8<T, VEC>(reinterpret_cast<const T*>(a.res) + row * a.res_row + c, n, r);
+// (x - m) r
+__device__ __forceinline__ void normalise8(F8& x, float m, float r) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = round_to<T>(x[i] + r[i]);
-  }
+  for (int i = 0; i < 4; ++i) x.v[i] = __fmul2_rn(__fadd2_rn(x.v[i], both(-m)), both(r));
 }
 
+// s of 8 columns, from the inputs.
+template <typename T, bool VEC>
+__device__ __forceinline__ F8 input8(const NormArgs& a, long long row, int c, int n, Turn8<T>* t) {
+  F8 x = widen8(fetch8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n, t));
+  if (a.res) {
+    const F8 y =
+        widen8(fetch8<T, VEC>(reinterpret_cast<const T*>(a.res) + row * a.res_row + c, n, t));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.v[i] = __fadd2_rn(x.v[i], y.v[i]);
+    round8(x, T());
+  }
+  return x;
+}
 // s of 8 columns in the backward pass: kept, or from its codes.
 template <typename T, bool VEC>
-__device__ __forceinline__ void kept8(const NormArgs& a, long long row, int c, int n,
-                                      float (&x)[8]) {
-  if (!a.codes) return load8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n, x);
-  const long long g = row * a.groups + c / kGroup8;
-  const uint2 q = __ldg(reinterpret_cast<const uint2*>(a.codes + row * a.groups * kGroup8 + c));
-  decode8<T>(q, range_of(__ldg(reinterpret_cast<const typename RangeBits<T>::type*>(a.ranges) + g),
-                         T()), x);
+__device__ __forceinline__ F8 kept8(const NormArgs& a, long long row, int c, int n, Turn8<T>* t) {
+  if (!a.codes)
+    return widen8(fetch8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n, t));
+  uint2 q = make_uint2(0u, 0u);
+  typename RangeBits<T>::type bits = {};
+  if (n) {
+    q = __ldg(reinterpret_cast<const uint2*>(a.codes + row * a.groups * kGroup8 + c));
+    bits = __ldg(reinterpret_cast<const typename RangeBits<T>::type*>(a.ranges) + row * a.groups +
+                 c / kGroup8);
+  }
+  return decode8<T>(q, range_of(bits, T()));
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ F8 grad8(const void* g, long long g_row, long long row, int c, int n,
+                                    Turn8<T>* t) {
+  return widen8(fetch8<T, VEC>(reinterpret_cast<const T*>(g) + row * g_row + c, n, t));
+}
+// Codes and range of 8 columns of s.
+template <typename T, bool VEC, typename X>
+__device__ __forceinline__ void keep8(const NormArgs& a, long long row, int u, int n, bool in,
+                                      const F8& x, const X& as_extent) {
+  Range8 r;
+  float lo, hi;
+  extent8<VEC>(as_extent, n, &lo, &hi);
+  const uint2 q = encode8<T, VEC>(x, n, lo, hi, &r);
+  if (!in) return;
+  reinterpret_cast<uint2*>(a.codes)[row * a.groups * 8 + u] = q;
+  if ((u & 7) == 0)
+    reinterpret_cast<typename RangeBits<T>::type*>(a.ranges)[row * a.groups + u / 8] =
+        range_bits(r, T());
 }
 
 // Rows that fit the registers of up to 32 warps: E units of 8 columns a lane, `wpr`
@@ -107,11 +136,10 @@ __global__ void __launch_bounds__(NT) norm_kernel(const NormArgs a, int wpr) {
     if (a.res) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        float x[8], y[8];
-        widen8(s[e], x);
-        widen8(q[e], y);
+        F8 x = widen8(s[e]);
+        const F8 y = widen8(q[e]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += y[i];
+        for (int i = 0; i < 4; ++i) x.v[i] = __fadd2_rn(x.v[i], y.v[i]);
         s[e] = narrow8(x, T());
       }
     }
@@ -127,55 +155,39 @@ __global__ void __launch_bounds__(NT) norm_kernel(const NormArgs a, int wpr) {
   };
   float t = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    float x[8];
-    widen8(s[e], x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t += x[i];
-  }
+  for (int e = 0; e < E; ++e) t += sum8(widen8(s[e]));
   const float m = row_sum(t, 0) / (float)a.width;
-  t = 0.f;
+  float2 v = both(0.f);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     if (VEC && n[e] == 0) continue;
-    float x[8];
-    widen8(s[e], x);
+    F8 x = widen8(s[e]);
+    if (!VEC) fill_from(x, n[e], m);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (VEC || i < n[e]) t = fmaf(x[i] - m, x[i] - m, t);
+    for (int i = 0; i < 4; ++i) {
+      const float2 d = __fadd2_rn(x.v[i], both(-m));
+      v = __ffma2_rn(d, d, v);
+    }
   }
-  const float r = 1.f / sqrtf(row_sum(t, 1) / (float)a.width + a.eps);
+  const float r = 1.f / sqrtf(row_sum(v.x + v.y, 1) / (float)a.width + a.eps);
   if (a.stats && in && at == 0 && lane == 0) a.stats[row] = make_float2(m, r);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     const int u = (e * wpr + at) * 32 + lane, c = u * 8;
-    float x[8];
-    widen8(s[e], x);
-    if (a.sum) put8<T, VEC>(reinterpret_cast<T*>(a.sum) + row * a.width + c, n[e], x, turn);
-    if (a.codes) {
-      Range8 range;
-      float lo, hi;
-      extent8<VEC>(s[e], n[e], &lo, &hi);
-      const uint2 q = encode8<T, VEC>(x, n[e], lo, hi, &range);
-      if (in && u < units) {
-        reinterpret_cast<uint2*>(a.codes)[row * units + u] = q;
-        if ((u & 7) == 0)
-          reinterpret_cast<typename RangeBits<T>::type*>(a.ranges)[row * a.groups + u / 8] =
-              range_bits(range, T());
-      }
-    }
-    float w[8], b[8];
-    weights8<T, VEC>(a, a.w, c, n[e], 1.f, w);
-    weights8<T, VEC>(a, a.b, c, n[e], 0.f, b);
+    F8 x = widen8(s[e]);
+    if (a.sum) store8<T, VEC>(reinterpret_cast<T*>(a.sum) + row * a.width + c, n[e], x, turn);
+    if (a.codes) keep8<T, VEC>(a, row, u, n[e], in && u < units, x, s[e]);
+    const F8 w = weights8<T, VEC>(a, a.w, c, n[e], 1.f), b = weights8<T, VEC>(a, a.b, c, n[e], 0.f);
+    normalise8(x, m, r);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = fmaf((x[i] - m) * r, w[i], b[i]);
-    put8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n[e], x, turn);
+    for (int i = 0; i < 4; ++i) x.v[i] = __ffma2_rn(x.v[i], w.v[i], b.v[i]);
+    store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n[e], x, turn);
   }
 }
 
 // The backward pass of such rows: blocks stay and take rows in turn; a lane keeps the
 // weight gradients of its columns in registers, the block adds its rows' at the end
-// and writes one part.  x, dy and ds stay in registers as they lie in memory.
+// and writes one part.  The next row's loads are under way while a row's sums run.
 template <typename T, bool VEC, int E, bool CODES, int NT>
 __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs a, int wpr) {
   __shared__ float2 sm[2][NT / 32];
@@ -185,9 +197,17 @@ __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Turn8<T>* const turn = turns + (VEC ? 0 : warp);
   const int at = warp % wpr, first = warp - at, rpb = NT / 32 / wpr;
-  float dw[E][8] = {}, db[E][8] = {};
-  // what a row's loads bring; the next row's are under way while this one's sums run
-  struct Row {
+  F8 dw[E], db[E];
+  Raw8<T> w[E];                 // weights of the operands' type stay; others are read anew
+  const bool w_kept = VEC && a.w && a.w_vec && (sizeof(T) == 4 || !a.w32);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dw[e].v[i] = db[e].v[i] = both(0.f);
+    const int c = ((e * wpr + at) * 32 + lane) * 8;
+    w[e] = w_kept && c < a.width ? get8<T>(reinterpret_cast<const T*>(a.w) + c) : zero8<T>();
+  }
+  struct Row {                  // as it lies in memory
     Raw8<T> x[E], g[E], s[E];
     uint2 code[E];
     Bits bits[E];
@@ -216,64 +236,71 @@ __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs 
   };
   const long long step = (long long)gridDim.x * rpb;
   int half = 0;
-  Row now, next;
+  Row now;
   load((long long)blockIdx.x * rpb + warp / wpr, now);
   for (long long row0 = (long long)blockIdx.x * rpb; row0 < a.rows; row0 += step, half ^= 1) {
     const long long row = row0 + warp / wpr;
     const bool in = row < a.rows;
-    load(row + step, next);
-    const float2 st = now.st;
-    float c1 = 0.f, c2 = 0.f;
+    const float r = now.st.y;
+    F8 h[E], g[E];
+    float2 c1 = both(0.f), c2 = both(0.f);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = ((e * wpr + at) * 32 + lane) * 8, n = in ? max(0, min(8, a.width - c)) : 0;
+      if constexpr (CODES) h[e] = decode8<T>(now.code[e], range_of(now.bits[e], T()));
+      else h[e] = widen8(now.x[e]);
+      g[e] = widen8(now.g[e]);
       if (VEC && n == 0) continue;
-      float x[8], g[8], w[8];
-      if constexpr (CODES) decode8<T>(now.code[e], range_of(now.bits[e], T()), x);
-      else widen8(now.x[e], x);
-      widen8(now.g[e], g);
-      weights8<T, VEC>(a, a.w, c, n, 1.f, w);
+      normalise8(h[e], now.st.x, r);
+      if (!VEC) fill_from(h[e], n, 0.f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float h = VEC || i < n ? (x[i] - st.x) * st.y : 0.f, gw = g[i] * w[i];
-        dw[e][i] = fmaf(g[i], h, dw[e][i]);
-        db[e][i] += g[i];
-        c1 += gw;
-        c2 = fmaf(gw, h, c2);
+      for (int i = 0; i < 4; ++i) {
+        dw[e].v[i] = __ffma2_rn(g[e].v[i], h[e].v[i], dw[e].v[i]);
+        db[e].v[i] = __fadd2_rn(db[e].v[i], g[e].v[i]);
+      }
+      if (a.w) {
+        const F8 f = w_kept ? widen8(w[e]) : weights8<T, VEC>(a, a.w, c, n, 1.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[e].v[i] = __fmul2_rn(g[e].v[i], f.v[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c1 = __fadd2_rn(c1, g[e].v[i]);
+        c2 = __ffma2_rn(g[e].v[i], h[e].v[i], c2);
       }
     }
-    c1 = warp_sum(c1);
-    c2 = warp_sum(c2);
+    Raw8<T> s[E];
+    if (a.ds) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[e] = now.s[e];
+    }
+    load(row + step, now);
+    float s1 = warp_sum(c1.x + c1.y), s2 = warp_sum(c2.x + c2.y);
     if (wpr > 1) {
-      if (lane == 0) sm[half][warp] = make_float2(c1, c2);
+      if (lane == 0) sm[half][warp] = make_float2(s1, s2);
       __syncthreads();          // one a row: the next row's sums have the other half
-      c1 = c2 = 0.f;
-      for (int w = 0; w < wpr; ++w) {
-        c1 += sm[half][first + w].x;
-        c2 += sm[half][first + w].y;
+      s1 = s2 = 0.f;
+      for (int i = 0; i < wpr; ++i) {
+        s1 += sm[half][first + i].x;
+        s2 += sm[half][first + i].y;
       }
     }
-    c1 /= (float)a.width;
-    c2 /= (float)a.width;
+    // dx = r (g - s1 / N - h s2 / N)
+    s1 = -s1 / (float)a.width;
+    s2 = -s2 / (float)a.width;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = ((e * wpr + at) * 32 + lane) * 8, n = in ? max(0, min(8, a.width - c)) : 0;
-      float x[8], g[8], w[8];
-      if constexpr (CODES) decode8<T>(now.code[e], range_of(now.bits[e], T()), x);
-      else widen8(now.x[e], x);
-      widen8(now.g[e], g);
-      weights8<T, VEC>(a, a.w, c, n, 1.f, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        x[i] = st.y * (fmaf(g[i], w[i], -c1) - (x[i] - st.x) * st.y * c2);
+      for (int i = 0; i < 4; ++i)
+        g[e].v[i] = __fmul2_rn(__ffma2_rn(h[e].v[i], both(s2), __fadd2_rn(g[e].v[i], both(s1))), both(r));
       if (a.ds) {
-        widen8(now.s[e], g);
+        const F8 d = widen8(s[e]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += g[i];
+        for (int i = 0; i < 4; ++i) g[e].v[i] = __fadd2_rn(g[e].v[i], d.v[i]);
       }
-      put8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, x, turn);
+      store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, g[e], turn);
     }
-    now = next;
   }
   if (!a.dw && !a.db) return;
   // warps that hold the same columns, in the order of their rows
@@ -284,12 +311,12 @@ __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs 
       if (!(k ? a.db : a.dw)) continue;
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) join[warp][lane * 9 + i] = k ? db[e][i] : dw[e][i];
+      for (int i = 0; i < 8; ++i) join[warp][lane * 9 + i] = k ? db[e].at(i) : dw[e].at(i);
       __syncthreads();
       for (int j = threadIdx.x; j < wpr * 256; j += NT) {
-        const int w = j / 256, l = j % 256, col = (e * wpr + w) * 256 + l;
+        const int w0 = j / 256, l = j % 256, col = (e * wpr + w0) * 256 + l;
         float t = 0.f;
-        for (int q = 0; q < rpb; ++q) t += join[q * wpr + w][l / 8 * 9 + l % 8];
+        for (int q = 0; q < rpb; ++q) t += join[q * wpr + w0][l / 8 * 9 + l % 8];
         if (col < a.width) a.part[((long long)blockIdx.x * 2 + k) * a.width + col] = t;
       }
     }
@@ -300,49 +327,39 @@ __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) norm_rows_kernel(const NormArgs a) {
   __shared__ float sm[32];
+  __shared__ __align__(16) Turn8<T> turns[VEC ? 1 : 8];
+  Turn8<T>* const turn = turns + (VEC ? 0 : threadIdx.x / 32);
   const int units = a.groups * 8;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    float t = 0.f, x[8];
-    for (int u = threadIdx.x; u < units; u += 256) {
-      const int c = u * 8, n = max(0, min(8, a.width - c));
-      input8<T, VEC>(a, row, c, n, x);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) t += x[i];
+    float t = 0.f;
+    for (int u0 = 0; u0 < units; u0 += 256) {
+      const int c = (u0 + threadIdx.x) * 8, n = max(0, min(8, a.width - c));
+      t += sum8(input8<T, VEC>(a, row, c, n, turn));
     }
     const float m = block_sum(t, sm) / (float)a.width;
-    t = 0.f;
-    for (int u = threadIdx.x; u < units; u += 256) {
-      const int c = u * 8, n = max(0, min(8, a.width - c));
-      input8<T, VEC>(a, row, c, n, x);
+    float2 v = both(0.f);
+    for (int u0 = 0; u0 < units; u0 += 256) {
+      const int c = (u0 + threadIdx.x) * 8, n = max(0, min(8, a.width - c));
+      F8 x = input8<T, VEC>(a, row, c, n, turn);
+      fill_from(x, n, m);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) t += (x[i] - m) * (x[i] - m);
+      for (int i = 0; i < 4; ++i) {
+        const float2 d = __fadd2_rn(x.v[i], both(-m));
+        v = __ffma2_rn(d, d, v);
+      }
     }
-    const float r = 1.f / sqrtf(block_sum(t, sm) / (float)a.width + a.eps);
+    const float r = 1.f / sqrtf(block_sum(v.x + v.y, sm) / (float)a.width + a.eps);
     if (a.stats && threadIdx.x == 0) a.stats[row] = make_float2(m, r);
     for (int u0 = 0; u0 < units; u0 += 256) {
       const int u = u0 + threadIdx.x, c = u * 8, n = max(0, min(8, a.width - c));
-      float w[8], b[8];
-      input8<T, VEC>(a, row, c, n, x);
-      if (a.sum)
-        store8<T, VEC>(reinterpret_cast<T*>(a.sum) + row * a.width + c, n, x);
-      if (a.codes) {
-        Range8 range;
-        float lo, hi;
-        extent8<VEC>(x, n, &lo, &hi);
-        const uint2 q = encode8<T, VEC>(x, n, lo, hi, &range);
-        if (u < units) {
-          reinterpret_cast<uint2*>(a.codes)[row * units + u] = q;
-          if ((u & 7) == 0)
-            reinterpret_cast<typename RangeBits<T>::type*>(a.ranges)[row * a.groups + u / 8] =
-                range_bits(range, T());
-        }
-      }
-      weights8<T, VEC>(a, a.w, c, n, 1.f, w);
-      weights8<T, VEC>(a, a.b, c, n, 0.f, b);
+      F8 x = input8<T, VEC>(a, row, c, n, turn);
+      if (a.sum) store8<T, VEC>(reinterpret_cast<T*>(a.sum) + row * a.width + c, n, x, turn);
+      if (a.codes) keep8<T, VEC>(a, row, u, n, u < units, x, x);
+      const F8 w = weights8<T, VEC>(a, a.w, c, n, 1.f), b = weights8<T, VEC>(a, a.b, c, n, 0.f);
+      normalise8(x, m, r);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = fmaf((x[i] - m) * r, w[i], b[i]);
-      store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, x);
+      for (int i = 0; i < 4; ++i) x.v[i] = __ffma2_rn(x.v[i], w.v[i], b.v[i]);
+      store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, x, turn);
     }
   }
 }
@@ -350,74 +367,96 @@ __global__ void __launch_bounds__(256) norm_rows_kernel(const NormArgs a) {
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) norm_grad_rows_kernel(const NormArgs a) {
   __shared__ float sm[32];
+  __shared__ __align__(16) Turn8<T> turns[VEC ? 1 : 8];
+  Turn8<T>* const turn = turns + (VEC ? 0 : threadIdx.x / 32);
   const int units = a.groups * 8;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float2 st = a.stats[row];
-    float c1 = 0.f, c2 = 0.f, x[8], g[8], w[8];
-    for (int u = threadIdx.x; u < units; u += 256) {
-      const int c = u * 8, n = max(0, min(8, a.width - c));
-      kept8<T, VEC>(a, row, c, n, x);
-      load8<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.dy_row + c, n, g);
-      weights8<T, VEC>(a, a.w, c, n, 1.f, w);
+    float c1 = 0.f, c2 = 0.f;
+    for (int u0 = 0; u0 < units; u0 += 256) {
+      const int c = (u0 + threadIdx.x) * 8, n = max(0, min(8, a.width - c));
+      F8 h = kept8<T, VEC>(a, row, c, n, turn);
+      F8 g = grad8<T, VEC>(a.dy, a.dy_row, row, c, n, turn);
+      const F8 w = weights8<T, VEC>(a, a.w, c, n, 1.f);
+      normalise8(h, st.x, st.y);
+      fill_from(h, n, 0.f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) {
-          c1 += g[i] * w[i];
-          c2 += g[i] * w[i] * ((x[i] - st.x) * st.y);
-        }
-    }
-    c1 = block_sum(c1, sm) / (float)a.width;
-    c2 = block_sum(c2, sm) / (float)a.width;
-    for (int u = threadIdx.x; u < units; u += 256) {
-      const int c = u * 8, n = max(0, min(8, a.width - c));
-      kept8<T, VEC>(a, row, c, n, x);
-      load8<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.dy_row + c, n, g);
-      weights8<T, VEC>(a, a.w, c, n, 1.f, w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        x[i] = st.y * (g[i] * w[i] - c1 - (x[i] - st.x) * st.y * c2);
-      if (a.ds) {
-        load8<T, VEC>(reinterpret_cast<const T*>(a.ds) + row * a.ds_row + c, n, g);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += g[i];
+      for (int i = 0; i < 4; ++i) {
+        g.v[i] = __fmul2_rn(g.v[i], w.v[i]);
+        h.v[i] = __fmul2_rn(g.v[i], h.v[i]);
       }
-      store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, x);
+      c1 += sum8(g);
+      c2 += sum8(h);
+    }
+    c1 = -block_sum(c1, sm) / (float)a.width;
+    c2 = -block_sum(c2, sm) / (float)a.width;
+    for (int u0 = 0; u0 < units; u0 += 256) {
+      const int c = (u0 + threadIdx.x) * 8, n = max(0, min(8, a.width - c));
+      F8 h = kept8<T, VEC>(a, row, c, n, turn);
+      F8 g = grad8<T, VEC>(a.dy, a.dy_row, row, c, n, turn);
+      const F8 w = weights8<T, VEC>(a, a.w, c, n, 1.f);
+      normalise8(h, st.x, st.y);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        g.v[i] = __fmul2_rn(__ffma2_rn(h.v[i], both(c2), __ffma2_rn(g.v[i], w.v[i], both(c1))),
+                            both(st.y));
+      if (a.ds) {
+        const F8 d = grad8<T, VEC>(a.ds, a.ds_row, row, c, n, turn);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g.v[i] = __fadd2_rn(g.v[i], d.v[i]);
+      }
+      store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, g, turn);
     }
   }
 }
 
 // Column sums dw, db of one part of the rows: a block has 256 columns, a warp
-// every eighth row.  Without codes and x, db alone.
-template <typename T, bool VEC>
+// every eighth row, four at a time.  Without HATS db alone.
+template <typename T, bool VEC, bool HATS>
 __global__ void __launch_bounds__(256) column_sums_kernel(const NormArgs a) {
   __shared__ float sm[8][32 * 9];
+  __shared__ __align__(16) Turn8<T> turns[VEC ? 1 : 8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Turn8<T>* const turn = turns + (VEC ? 0 : warp);
   const int c = (blockIdx.x * 32 + lane) * 8, n = max(0, min(8, a.width - c));
-  const bool hats = a.x || a.codes;
-  float dw[8] = {}, db[8] = {};
-  const long long step = (long long)gridDim.y * 8;
-#pragma unroll 4
-  for (long long row = blockIdx.y * 8ll + warp; row < a.rows; row += step) {
-    float g[8], x[8];
-    load8<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.dy_row + c, n, g);
-    if (hats && n) {
-      const float2 st = __ldg(a.stats + row);
-      kept8<T, VEC>(a, row, c, n, x);
+  F8 dw, db;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < n) dw[i] += g[i] * ((x[i] - st.x) * st.y);
+  for (int i = 0; i < 4; ++i) dw.v[i] = db.v[i] = both(0.f);
+  const long long step = (long long)gridDim.y * 8;
+  for (long long row0 = blockIdx.y * 8ll + warp; row0 < a.rows; row0 += 4 * step) {
+    Raw8<T> g[4];
+    F8 h[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const long long row = row0 + q * step;
+      const bool in = row < a.rows;
+      g[q] = fetch8<T, VEC>(reinterpret_cast<const T*>(a.dy) + (in ? row : 0) * a.dy_row + c,
+                            in ? n : 0, turn);
+      if constexpr (HATS) {
+        h[q] = kept8<T, VEC>(a, in ? row : 0, c, in ? n : 0, turn);
+        const float2 st = in ? __ldg(a.stats + row) : make_float2(0.f, 0.f);
+        normalise8(h[q], st.x, st.y);
+        fill_from(h[q], n, 0.f);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) db[i] += g[i];
+    for (int q = 0; q < 4; ++q) {
+      const F8 x = widen8(g[q]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (HATS) dw.v[i] = __ffma2_rn(x.v[i], h[q].v[i], dw.v[i]);
+        db.v[i] = __fadd2_rn(db.v[i], x.v[i]);
+      }
+    }
   }
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+  for (int k = HATS ? 0 : 1; k < 2; ++k) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sm[warp][lane * 9 + i] = k ? db[i] : dw[i];
+    for (int i = 0; i < 8; ++i) sm[warp][lane * 9 + i] = k ? db.at(i) : dw.at(i);
     __syncthreads();
     const int col = blockIdx.x * 256 + threadIdx.x;
-    if (col < a.width && (k || hats)) {
+    if (col < a.width) {
       float t = 0.f;
 #pragma unroll
       for (int w = 0; w < 8; ++w) t += sm[w][threadIdx.x / 8 * 9 + threadIdx.x % 8];
@@ -454,12 +493,12 @@ __global__ void __launch_bounds__(1024) column_join_kernel(const NormArgs a) {
 // host
 // ---------------------------------------------------------------------------
 
-// Parts of the rows in the column sums: enough blocks for every multiprocessor,
+// Parts of the rows in the column sums: four blocks a multiprocessor run at once,
 // at least 8 rows to a warp.
 static int column_splits(long long rows, int width, int device) {
   const int strips = (width + 255) / 256;
   const long long most = std::max(1ll, (rows + 63) / 64);
-  return (int)std::min(most, (long long)std::max(1, sm_count(device) * 6 / strips));
+  return (int)std::min(most, (long long)std::max(1, sm_count(device) * 4 / strips));
 }
 
 // Warps that share a row and units of 8 columns a lane; 0 where a row does not fit.
@@ -503,10 +542,15 @@ template <typename T>
 static int column_sums(NormArgs& a, bool vec, int device, cudaStream_t st) {
   a.splits = column_splits(a.rows, a.width, device);
   const dim3 grid((unsigned)((a.width + 255) / 256), (unsigned)a.splits);
-  if (vec)
-    column_sums_kernel<T, true><<<grid, 256, 0, st>>>(a);
+  const bool hats = a.x || a.codes;
+  if (hats && vec)
+    column_sums_kernel<T, true, true><<<grid, 256, 0, st>>>(a);
+  else if (hats)
+    column_sums_kernel<T, false, true><<<grid, 256, 0, st>>>(a);
+  else if (vec)
+    column_sums_kernel<T, true, false><<<grid, 256, 0, st>>>(a);
   else
-    column_sums_kernel<T, false><<<grid, 256, 0, st>>>(a);
+    column_sums_kernel<T, false, false><<<grid, 256, 0, st>>>(a);
   FAB_LAUNCH_CHECK();
   return column_join<T>(a, st);
 }

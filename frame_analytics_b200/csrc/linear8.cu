@@ -53,15 +53,16 @@ __global__ void __launch_bounds__(256) wgrad_lanes_kernel(const WgradArgs a) {
     }
     if (threadIdx.x < kWgRows * 8) {
       const int t = threadIdx.x / 8, u = threadIdx.x % 8;
-      float x[8] = {};
+      uint2 q = make_uint2(0u, 0u);
+      typename RangeBits<T>::type bits = {};
       if (t0 + t < a.rows) {
         const long long g = (t0 + t) * a.groups + k0 / kGroup8;
-        decode8<T>(__ldg(reinterpret_cast<const uint2*>(a.codes) + g * 8 + u),
-                   range_of(__ldg(reinterpret_cast<const typename RangeBits<T>::type*>(a.ranges) + g),
-                            T()), x);
+        q = __ldg(reinterpret_cast<const uint2*>(a.codes) + g * 8 + u);
+        bits = __ldg(reinterpret_cast<const typename RangeBits<T>::type*>(a.ranges) + g);
       }
+      const F8 x = decode8<T>(q, range_of(bits, T()));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sb[t][u * 8 + i] = x[i];
+      for (int i = 0; i < 8; ++i) sb[t][u * 8 + i] = x.at(i);
     }
     __syncthreads();
 #pragma unroll
@@ -266,7 +267,7 @@ __device__ __forceinline__ void operands16(uint4 c, unsigned bits, uint4* out) {
 
 template <typename T>
 __device__ __forceinline__ unsigned pair_bits(float a, float b) {
-  return (unsigned)St<T>::v(a).bits | ((unsigned)St<T>::v(b).bits << 16);
+  return narrow2(make_float2(a, b), T());
 }
 
 // A warp's 32 rows x 64 columns of the result, at (i, j), a row a lane; `turn` is
@@ -280,10 +281,9 @@ __device__ __forceinline__ void put_result(const ProductArgs& a, int i, int j, f
     if (a.bias_vec && j + 64 <= a.n) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) {
-        float x[8];
-        load8<T, true>(b + 8 * q, 8, x);
+        const F8 x = widen8(get8<T>(b + 8 * q));
 #pragma unroll
-        for (int c = 0; c < 8; ++c) v[8 * q + c] += x[c];
+        for (int c = 0; c < 8; ++c) v[8 * q + c] += x.at(c);
       }
     } else {
 #pragma unroll
