@@ -74,6 +74,8 @@ def _reject_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """As a matrix of rows with unit stride; a copy where that takes one."""
     width = t.shape[-1]
+    if t.dim() == 2 and (t.stride(1) == 1 or width == 1):
+        return t
     if t.stride(-1) != 1 and width > 1:
         t = t.contiguous()
     return t.reshape(-1, width)
@@ -87,17 +89,39 @@ def _packed_like(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return codes, torch.empty((*lead, groups), dtype=torch.int32, device=x.device)
 
 
+def _kept_like(x: torch.Tensor, rows: int, stats: bool) -> Tuple[torch.Tensor, int, int]:
+    """One buffer for the codes, two floats a row (``stats``) and the ranges, in this
+    order; the offsets of the latter two.  An allocation costs as much host time as a
+    launch."""
+    groups = -(-x.shape[-1] // _GROUP)
+    at = rows * groups * _GROUP
+    ranges = at + (8 * rows if stats else 0)
+    size = ranges + rows * groups * (8 if x.dtype == torch.float32 else 4)
+    return torch.empty(size, dtype=torch.uint8, device=x.device), at, ranges
+
+
+def _empty(like: torch.Tensor) -> torch.Tensor:
+    """Contiguous, of the same shape."""
+    if like.is_contiguous():
+        return torch.empty_like(like)
+    return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+
+
 # --------------------------------------------------------------------------- #
 # packing
 # --------------------------------------------------------------------------- #
 
+def _pack_into(x: torch.Tensor, codes: int, ranges: int) -> None:
+    r = _rows(x)
+    backend._call(r, backend.lib().fa_b200_pack8, r.data_ptr(), r.stride(0),
+                  backend.DTYPE_CODE[x.dtype], r.shape[0], r.shape[1], codes, ranges,
+                  backend._dev(r), backend._stream(r))
+
+
 def _pack(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     codes, ranges = _packed_like(x)
     if x.numel():
-        r = _rows(x)
-        backend._call(r, backend.lib().fa_b200_pack8, r.data_ptr(), r.stride(0),
-                      backend.DTYPE_CODE[x.dtype], r.shape[0], r.shape[1], codes.data_ptr(),
-                      ranges.data_ptr(), backend._dev(r), backend._stream(r))
+        _pack_into(x, codes.data_ptr(), ranges.data_ptr())
     return codes, ranges
 
 
@@ -153,28 +177,23 @@ def unpack8(p: Packed8) -> torch.Tensor:
 # layer norm
 # --------------------------------------------------------------------------- #
 
-def _norm_params(x, residual, weight, bias, eps, stats, codes, ranges, like) -> bytes:
-    """`x` and `residual`: rows; `like`: a tensor of the rows' shape and dtype."""
+def _norm_params(x, residual, weight, bias, eps, stats, codes, ranges, rows, width, dtype) -> bytes:
+    """`x` and `residual`: rows; `stats`, `codes` and `ranges`: addresses."""
     w = weight if weight is not None else bias
-    width = like.shape[-1]
-    code = backend.DTYPE_CODE[like.dtype]
-    return _NORM(code, code if w is None else backend.DTYPE_CODE[w.dtype],
-                 like.numel() // width, width, 0, eps,
+    code = backend.DTYPE_CODE[dtype]
+    return _NORM(code, code if w is None else backend.DTYPE_CODE[w.dtype], rows, width, 0, eps,
                  0 if x is None else x.data_ptr(), width if x is None else x.stride(0),
                  0 if residual is None else residual.data_ptr(),
                  0 if residual is None else residual.stride(0),
                  0 if weight is None else weight.data_ptr(),
-                 0 if bias is None else bias.data_ptr(),
-                 0 if stats is None else stats.data_ptr(),
-                 0 if codes is None else codes.data_ptr(),
-                 0 if ranges is None else ranges.data_ptr())
+                 0 if bias is None else bias.data_ptr(), stats, codes, ranges)
 
 
 def _norm_forward(x, residual, weight, bias, eps, stats, codes, ranges):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _empty(x)
     total = None if residual is None else torch.empty_like(y)
     xr, rr = _rows(x), None if residual is None else _rows(residual)
-    p = _norm_params(xr, rr, weight, bias, eps, stats, codes, ranges, y)
+    p = _norm_params(xr, rr, weight, bias, eps, stats, codes, ranges, *xr.shape, x.dtype)
     backend._call(y, backend.lib().fa_b200_layer_norm, p, y.data_ptr(), backend._ptr(total),
                   backend._dev(y), backend._stream(y))
     return y, total
@@ -184,11 +203,18 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, eps, keep8):
         ctx.set_materialize_grads(False)
-        stats = torch.empty((x.numel() // x.shape[-1], 2), dtype=torch.float32, device=x.device)
-        codes, ranges = _packed_like(x) if keep8 else (None, None)
-        y, total = _norm_forward(x, residual, weight, bias, eps, stats, codes, ranges)
-        kept = None if keep8 else (x if residual is None else total)
-        ctx.save_for_backward(kept, codes, ranges, stats, weight, bias)
+        rows = x.numel() // x.shape[-1]
+        if keep8:
+            kept, stats, ranges = _kept_like(x, rows, True)
+            at = kept.data_ptr()
+            y, total = _norm_forward(x, residual, weight, bias, eps, at + stats, at, at + ranges)
+            ctx.save_for_backward(kept, None, weight, bias)
+            ctx.at = (stats, ranges)
+        else:
+            stats = torch.empty(2 * rows, dtype=torch.float32, device=x.device)
+            y, total = _norm_forward(x, residual, weight, bias, eps, stats.data_ptr(), 0, 0)
+            ctx.save_for_backward(stats, x if residual is None else total, weight, bias)
+            ctx.at = None
         ctx.eps = eps
         return y if residual is None else (y, total)
 
@@ -198,23 +224,27 @@ class _LayerNorm(torch.autograd.Function):
         need = ctx.needs_input_grad
         if gy is None:  # the norm itself took no part
             return (gsum if need[0] else None, gsum if need[1] else None, None, None, None, None)
-        kept, codes, ranges, stats, weight, bias = ctx.saved_tensors
-        width = gy.shape[-1]
-        dx = torch.empty(gy.shape, dtype=gy.dtype, device=gy.device)
+        kept, s, weight, bias = ctx.saved_tensors
+        dx = _empty(gy)
         dw = torch.empty_like(weight) if weight is not None and need[2] else None
         db = torch.empty_like(bias) if bias is not None and need[3] else None
-        g = _rows(gy)
-        s = None if gsum is None else _rows(gsum)
+        g, gs = _rows(gy), None if gsum is None else _rows(gsum)
+        rows, width = g.shape
         L = backend.lib()
         ws, size = None, 0
         if dw is not None or db is not None:
             size = backend._cached_ws("norm", L.fa_b200_layer_norm_backward_workspace_bytes,
-                                      g.shape[0], width, backend._dev(g))
+                                      rows, width, backend._dev(g))
             ws = torch.empty(size, dtype=torch.uint8, device=g.device)
-        p = _norm_params(None if kept is None else _rows(kept), None, weight, bias, ctx.eps, stats,
-                         codes, ranges, dx)
+        at = kept.data_ptr()
+        if ctx.at is None:
+            s = _rows(s)
+            p = _norm_params(s, None, weight, bias, ctx.eps, at, 0, 0, rows, width, g.dtype)
+        else:
+            p = _norm_params(None, None, weight, bias, ctx.eps, at + ctx.at[0], at, at + ctx.at[1],
+                             rows, width, g.dtype)
         backend._call(g, L.fa_b200_layer_norm_backward, p, g.data_ptr(), g.stride(0),
-                      backend._ptr(s), 0 if s is None else s.stride(0), dx.data_ptr(),
+                      backend._ptr(gs), 0 if gs is None else gs.stride(0), dx.data_ptr(),
                       backend._ptr(dw), backend._ptr(db), backend._ptr(ws), size, backend._dev(g),
                       backend._stream(g))
         return dx if need[0] else None, dx if need[1] else None, dw, db, None, None
@@ -273,7 +303,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     if torch.is_grad_enabled() and any(
             t is not None and t.requires_grad for t in (x, residual, weight, bias)):
         return _LayerNorm.apply(x, residual, weight, bias, eps, bool(keep8))
-    y, total = _norm_forward(x, residual, weight, bias, eps, None, None, None)
+    y, total = _norm_forward(x, residual, weight, bias, eps, 0, 0, 0)
     return y if residual is None else (y, total)
 
 
@@ -282,33 +312,34 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
 # --------------------------------------------------------------------------- #
 
 def _gelu_forward(x, tanh_form, codes, ranges):
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _empty(x)
     r = _rows(x)
     backend._call(r, backend.lib().fa_b200_gelu8, r.data_ptr(), r.stride(0),
                   backend.DTYPE_CODE[x.dtype], r.shape[0], r.shape[1], tanh_form, y.data_ptr(),
-                  backend._ptr(codes), backend._ptr(ranges), backend._dev(r), backend._stream(r))
+                  codes, ranges, backend._dev(r), backend._stream(r))
     return y
 
 
 class _Gelu8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, tanh_form):
-        codes, ranges = _packed_like(x)
-        y = _gelu_forward(x, tanh_form, codes, ranges)
-        ctx.save_for_backward(codes, ranges)
-        ctx.tanh_form = tanh_form
+        kept, ranges, _ = _kept_like(x, x.numel() // x.shape[-1], False)
+        at = kept.data_ptr()
+        y = _gelu_forward(x, tanh_form, at, at + ranges)
+        ctx.save_for_backward(kept)
+        ctx.ranges, ctx.tanh_form = ranges, tanh_form
         return y
 
     @staticmethod
     def backward(ctx, gy):
         _reject_double_backward()
-        codes, ranges = ctx.saved_tensors
-        dx = torch.empty(gy.shape, dtype=gy.dtype, device=gy.device)
+        kept, = ctx.saved_tensors
+        at = kept.data_ptr()
+        dx = _empty(gy)
         g = _rows(gy)
-        backend._call(g, backend.lib().fa_b200_gelu8_backward, g.data_ptr(), g.stride(0),
-                      codes.data_ptr(), ranges.data_ptr(), backend.DTYPE_CODE[gy.dtype],
-                      g.shape[0], g.shape[1], ctx.tanh_form, dx.data_ptr(), backend._dev(g),
-                      backend._stream(g))
+        backend._call(g, backend.lib().fa_b200_gelu8_backward, g.data_ptr(), g.stride(0), at,
+                      at + ctx.ranges, backend.DTYPE_CODE[gy.dtype], g.shape[0], g.shape[1],
+                      ctx.tanh_form, dx.data_ptr(), backend._dev(g), backend._stream(g))
         return dx, None
 
 
@@ -338,7 +369,7 @@ def gelu8(x: torch.Tensor, *, approximate: str = "none") -> torch.Tensor:
 # --------------------------------------------------------------------------- #
 
 def _weight_grad(g, codes, ranges, inputs: int, need_weight: bool, need_bias: bool):
-    """``g``: rows of the gradient."""
+    """``g``: rows of the gradient; ``codes`` and ``ranges``: addresses."""
     rows, outputs = g.shape
     code = backend.DTYPE_CODE[g.dtype]
     dw = torch.empty((outputs, inputs), dtype=g.dtype, device=g.device) if need_weight else None
@@ -347,10 +378,9 @@ def _weight_grad(g, codes, ranges, inputs: int, need_weight: bool, need_bias: bo
     size = backend._cached_ws("wgrad8", L.fa_b200_linear8_weight_grad_workspace_bytes, rows,
                               inputs, outputs, code, backend._dev(g))
     ws = torch.empty(size, dtype=torch.uint8, device=g.device)
-    backend._call(g, L.fa_b200_linear8_weight_grad, g.data_ptr(), g.stride(0),
-                  backend._ptr(codes), backend._ptr(ranges), code, rows, inputs, outputs,
-                  backend._ptr(dw), backend._ptr(db), ws.data_ptr(), size, backend._dev(g),
-                  backend._stream(g))
+    backend._call(g, L.fa_b200_linear8_weight_grad, g.data_ptr(), g.stride(0), codes, ranges, code,
+                  rows, inputs, outputs, backend._ptr(dw), backend._ptr(db), ws.data_ptr(), size,
+                  backend._dev(g), backend._stream(g))
     return dw, db
 
 
@@ -358,22 +388,32 @@ class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         y = F.linear(x, weight, bias)
-        codes, ranges = _pack(x) if ctx.needs_input_grad[1] else (None, None)
-        ctx.save_for_backward(codes, ranges, weight)
+        kept, ctx.ranges = None, 0
+        if ctx.needs_input_grad[1]:
+            kept, ctx.ranges, _ = _kept_like(x, x.numel() // x.shape[-1], False)
+            at = kept.data_ptr()
+            _pack_into(x, at, at + ctx.ranges)
+        ctx.save_for_backward(kept, weight)
         return y
 
     @staticmethod
     def backward(ctx, gy):
         _reject_double_backward()
-        codes, ranges, weight = ctx.saved_tensors
+        kept, weight = ctx.saved_tensors
         need, inputs = ctx.needs_input_grad, weight.shape[1]
         g = _rows(gy)
         dx = dw = db = None
         if need[0]:
-            with torch.autocast("cuda", enabled=False):
-                dx = torch.matmul(g, weight).view(*gy.shape[:-1], inputs)
+            if torch.is_autocast_enabled("cuda"):
+                with torch.autocast("cuda", enabled=False):
+                    dx = torch.matmul(g, weight)
+            else:
+                dx = torch.matmul(g, weight)
+            if gy.dim() != 2:
+                dx = dx.view(*gy.shape[:-1], inputs)
         if need[1] or need[2]:
-            dw, db = _weight_grad(g, codes, ranges, inputs, need[1], need[2])
+            at = 0 if kept is None else kept.data_ptr()
+            dw, db = _weight_grad(g, at, at + ctx.ranges, inputs, need[1], need[2])
         return dx, dw, db
 
 
