@@ -2,14 +2,17 @@
 //   dW[m, k] = sum over rows t of dy[t, m] x^[t, k],   db[m] = sum over t of dy[t, m],
 // where x^ are the values that the codes stand for.
 //
-// 16-bit types: tensor-core products of 256 x 256 tiles over pairs of blocks
-// (tcgen05, cta_group::2), persistent, accumulators double-buffered in tensor
-// memory.  dy arrives by TMA as it lies (its rows are the sum's axis: MN-major),
-// the codes by TMA as bytes; eight warps turn a stage's codes into operand values
-// in shared memory, in the layout that TMA would have written, while the tensor
-// cores work on the stages before it.  Every value q s + lo is rounded once, as
-// unpacking rounds it.  Where the tiles are fewer than the pairs of blocks, the
-// rows are cut into parts whose float32 sums are joined in order.
+// 16-bit types: tensor-core products of 256 inputs x 256 outputs over pairs of blocks
+// (tcgen05, cta_group::2), persistent.  dy arrives by TMA as it lies (its rows are the
+// sum's axis: MN-major) and is the products' second operand in shared memory.  The
+// codes arrive by TMA as bytes; eight warps turn them, transposed on the way out of
+// shared memory, into the first operand in TENSOR MEMORY (a lane an input, two rows t a
+// word), while the tensor cores work on the stages before.  So the unpacked values
+// never pass through shared memory, whose bytes bound these products: with them there
+// a stage of 64 rows took 1000 cycles against 670 with both operands from TMA.  Every
+// value q s + lo is rounded once, as unpacking rounds it.  Where the tiles are fewer
+// than the pairs of blocks, the rows are cut into parts whose float32 sums are joined
+// in order.
 #include <algorithm>
 #include <atomic>
 
@@ -93,42 +96,33 @@ __global__ void __launch_bounds__(256) wgrad_lanes_kernel(const WgradArgs a) {
 // 16-bit products on the tensor cores
 // ---------------------------------------------------------------------------
 
-constexpr int kTile = 256;      // rows and columns of a pair's tile
-constexpr int kDepth = 64;      // of the sum's axis, a stage
-constexpr int kHalf = 2 * kBox; // bytes of one block's 128 x 64 of an operand
+constexpr int kTile = 256;      // inputs and outputs of a pair's tile
+constexpr int kDepth = 64;      // rows t a stage
+constexpr int kHalf = 2 * kBox; // bytes of one block's 128 outputs of a stage
 constexpr int kRaw = kDepth * 128;  // bytes of a stage's codes
 constexpr int kRanges = kDepth * 8; // and of their ranges, two groups a row
-constexpr int kTurn = 4096;     // a warp's 32 x 64 of the result
+// Stages of operands and of codes, which run ahead of them.  Even numbers: the two
+// teams of writers take turns, and each then sees every phase of its stages.
+constexpr int kStages = 8, kCodeStages = 8;
+constexpr int kWriters = 8;     // warps that unpack, and write the sums out
+constexpr int kWgThreads = 128 + 32 * kWriters;
+constexpr int kCodesAt = kStages * kHalf;           // offsets in shared memory
+constexpr int kRangesAt = kCodesAt + kCodeStages * kRaw;
+constexpr int kWgSmem = kRangesAt + kCodeStages * kRanges + 1024;
+constexpr int kOperandAt = 256; // columns of tensor memory: the sums', then 32 a stage
 constexpr int kPartFloats = 128 * 256;  // of one block's part of a tile
 
-// D[m][n] = sum over k of A[m][k] B[n][k].
+// dW[n][m] = sum over t of x^[t][m] dy[t][n].
 struct ProductArgs {
-  CUtensorMap a, b, d;          // b: of the codes where they are packed
-  int m, n, kb;                 // kb: stages of the whole sum
-  int a_mn, b_mn;               // the operand lies with k as its rows
+  CUtensorMap codes, dy;
+  int m, n, kb;                 // inputs, outputs, stages of the whole sum
   int tiles_m, tiles_n, parts;
   const unsigned* ranges;
   long long rows;
   int groups;
-  void* out;                    // [m][n]
-  const void* bias;             // [n] or null
-  int tma_out, bias_vec;
+  void* out;
   float* part;
   unsigned* err;
-};
-
-template <bool PACKED>
-struct Product {
-  // Stages of the operands, and of the codes, which the writers read ahead of them.
-  static constexpr int kStages = PACKED ? 5 : 6, kC = PACKED ? 4 : 0;
-  static constexpr int kWriters = PACKED ? 8 : 0;   // warps that unpack
-  static constexpr int kEpi = PACKED ? 4 : 8;       // warps of the epilogue
-  static constexpr int kThreads = 128 + 32 * (kWriters + kEpi);
-  static constexpr int kBAt = kStages * kHalf;      // offsets in shared memory
-  static constexpr int kTurnAt = 2 * kBAt;
-  static constexpr int kCodesAt = kTurnAt + kEpi * kTurn;
-  static constexpr int kRangesAt = kCodesAt + kC * kRaw;
-  static constexpr int kSmem = kRangesAt + kC * kRanges + 1024;
 };
 
 struct Work {
@@ -221,138 +215,109 @@ __device__ __forceinline__ void warp_wait(unsigned long long* bar, unsigned pari
   __syncwarp();
 }
 
-// 16 codes to 16 operand values, two to a word.  The low bytes of 2^23 + q and of
-// 1024 + q are q, and q has 8 bits: bfloat16 holds it exactly, as the high half of
-// a float32.
+// Steps and lowest values of four rows t, two to a word.
+struct Range4 {
+  unsigned s[2], lo[2];
+};
 template <typename T>
-__device__ __forceinline__ void operands16(uint4 c, unsigned bits, uint4* out) {
-  const unsigned in[4] = {c.x, c.y, c.z, c.w};
-  unsigned o[8];
-  const Range8 r = range_of(bits, T());
-  if constexpr (std::is_same<T, bf16_t>::value) {
-    const unsigned lo2 = __byte_perm(bits, 0u, 0x1010), s2 = __byte_perm(bits, 0u, 0x3232);
+__device__ __forceinline__ Range4 range4(uint4 b) {
+  Range4 r;
+  r.lo[0] = __byte_perm(b.x, b.y, 0x5410);
+  r.lo[1] = __byte_perm(b.z, b.w, 0x5410);
+  r.s[0] = __byte_perm(b.x, b.y, 0x7632);
+  r.s[1] = __byte_perm(b.z, b.w, 0x7632);
+  if constexpr (std::is_same<T, f16_t>::value) {  // from bfloat16
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned w = in[i / 2], k = (i & 1) * 2;
-      const float q0 = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | k)) - kMagic8;
-      const float q1 = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | (k + 1))) - kMagic8;
-      const unsigned q = __byte_perm(__float_as_uint(q0), __float_as_uint(q1), 0x7632);
-      asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(o[i]) : "r"(q), "r"(s2), "r"(lo2));
-    }
-  } else if (r.s >= 5.9604644775390625e-8f) {  // 2^-24: float16 holds s
-    const unsigned lo2 = __byte_perm(bits, 0u, 0x1010);
-    const unsigned sh = __half_as_ushort(__float2half_rn(r.s)), s2 = sh | (sh << 16);
-    const unsigned less = 0xe400e400u;  // -1024
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      unsigned q = __byte_perm(in[i / 2], 0x64646464u, i & 1 ? 0x4342 : 0x4140);
-      asm("add.rn.f16x2 %0, %1, %2;" : "=r"(q) : "r"(q), "r"(less));
-      asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(o[i]) : "r"(q), "r"(s2), "r"(lo2));
-    }
-  } else {  // spreads below 2^-16, and groups that are not finite
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      unsigned h[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float q = (float)((in[i / 2] >> (16 * (i & 1) + 8 * j)) & 255u);
-        h[j] = St<T>::v(fmaf(q, r.s, r.lo)).bits;
-      }
-      o[i] = h[0] | (h[1] << 16);
-    }
+    for (int i = 0; i < 2; ++i) r.s[i] = narrow2(widen2(r.s[i], bf16_t()), f16_t());
   }
-  out[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  out[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  return r;
+}
+// Whether float16 holds every step: not of spreads below 2^-16, of rows behind the last
+// (zero), or of groups that are not finite (NaN).
+__device__ __forceinline__ bool held_in_half(uint4 b) {
+  const float s[4] = {range_of(b.x, f16_t()).s, range_of(b.y, f16_t()).s,
+                      range_of(b.z, f16_t()).s, range_of(b.w, f16_t()).s};
+  bool held = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) held = held && s[i] >= 5.9604644775390625e-8f;  // 2^-24
+  return held;
+}
+// Codes k and k + 1 of a word to two operand values.  The low bytes of 2^23 + q and of
+// 1024 + q are q, and q has 8 bits: bfloat16 holds it exactly, as the high half of a
+// float32.
+__device__ __forceinline__ unsigned operand2(unsigned w, int k, unsigned s, unsigned lo, bf16_t) {
+  const float2 q = __fadd2_rn(
+      make_float2(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | k)),
+                  __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 | (k + 1)))),
+      both(-kMagic8));
+  unsigned o = __byte_perm(__float_as_uint(q.x), __float_as_uint(q.y), 0x7632);
+  asm("fma.rn.bf16x2 %0, %0, %1, %2;" : "+r"(o) : "r"(s), "r"(lo));
+  return o;
+}
+__device__ __forceinline__ unsigned operand2(unsigned w, int k, unsigned s, unsigned lo, f16_t) {
+  unsigned o = __byte_perm(w, 0x64646464u, k ? 0x4342 : 0x4140);
+  asm("add.rn.f16x2 %0, %0, %1;" : "+r"(o) : "r"(0xe400e400u));  // -1024
+  asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(o) : "r"(s), "r"(lo));
+  return o;
+}
+// The same from the ranges themselves, where float16 does not hold a step.
+__device__ __forceinline__ unsigned operand2_wide(unsigned w, int k, unsigned b0, unsigned b1) {
+  const Range8 r0 = range_of(b0, f16_t()), r1 = range_of(b1, f16_t());
+  const float q0 = (float)((w >> (8 * k)) & 255u), q1 = (float)((w >> (8 * k + 8)) & 255u);
+  return narrow2(make_float2(fmaf(q0, r0.s, r0.lo), fmaf(q1, r1.s, r1.lo)), f16_t());
+}
+
+// 16 x 16 bytes transposed, twice: a lane gets, for rows t = 4 (lane % 4) ... + 3 of
+// either, the codes of inputs lane / 4 (o[0], o[2]) and lane / 4 + 8 (o[1], o[3]).
+__device__ __forceinline__ void codes16x2(unsigned addr, unsigned (&o)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];\n"
+               : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
+               : "r"(addr)
+               : "memory");
+}
+// 16 lanes x 32 columns of tensor memory, in the same arrangement.
+__device__ __forceinline__ void tmem_store16(unsigned addr, const unsigned (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15, %16};\n" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+// D (256 x 256 over the pair) += A (tensor memory) B (shared memory)
+__device__ __forceinline__ void mma_from_tmem(unsigned d, unsigned a, unsigned long long b,
+                                              unsigned idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((unsigned)add)
+      : "memory");
 }
 
 template <typename T>
-__device__ __forceinline__ unsigned pair_bits(float a, float b) {
-  return narrow2(make_float2(a, b), T());
-}
-
-// A warp's 32 rows x 64 columns of the result, at (i, j), a row a lane; `turn` is
-// 4 KB of shared memory of its own, rows of 128 bytes in the 128-byte swizzle.
-template <typename T>
-__device__ __forceinline__ void put_result(const ProductArgs& a, int i, int j, float (&v)[64],
-                                           char* turn) {
-  const int lane = threadIdx.x & 31;
-  if (a.bias) {
-    const T* b = reinterpret_cast<const T*>(a.bias) + j;
-    if (a.bias_vec && j + 64 <= a.n) {
-#pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const F8 x = widen8(get8<T>(b + 8 * q));
-#pragma unroll
-        for (int c = 0; c < 8; ++c) v[8 * q + c] += x.at(c);
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < 64; ++c)
-        if (j + c < a.n) v[c] += Ld<T>::f(ldro(b + c));
-    }
-  }
-  // the buffer's last store has been read out of it
-  asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
-  __syncwarp();
-#pragma unroll
-  for (int q = 0; q < 8; ++q)
-    *reinterpret_cast<uint4*>(turn + lane * 128 + (q ^ (lane & 7)) * 16) =
-        make_uint4(pair_bits<T>(v[8 * q], v[8 * q + 1]), pair_bits<T>(v[8 * q + 2], v[8 * q + 3]),
-                   pair_bits<T>(v[8 * q + 4], v[8 * q + 5]), pair_bits<T>(v[8 * q + 6], v[8 * q + 7]));
-  if (a.tma_out) {
-    fence_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      asm volatile(
-          "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n"
-          "cp.async.bulk.commit_group;\n" ::"l"(reinterpret_cast<unsigned long long>(&a.d)),
-          "r"(j), "r"(i), "r"(0), "r"(smem_u32(turn))
-          : "memory");
-    }
-  } else {
-    __syncwarp();
-    T* const out = reinterpret_cast<T*>(a.out);
-    for (int r = 0; r < min(32, a.m - i); ++r) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int c = lane + 32 * h;
-        if (j + c < a.n)
-          out[(long long)(i + r) * a.n + j + c] = *reinterpret_cast<const T*>(
-              turn + r * 128 + ((c / 8) ^ (r & 7)) * 16 + c % 8 * 2);
-      }
-    }
-    __syncwarp();
-  }
-}
-
-template <typename T, bool PACKED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kThreads, 1)
-    product_kernel(const __grid_constant__ ProductArgs a) {
-  typedef Product<PACKED> P;
-  constexpr int S = P::kStages, SC = PACKED ? P::kC : 1;
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
+    wgrad_kernel(const __grid_constant__ ProductArgs a) {
+  constexpr int S = kStages, SC = kCodeStages;
   extern __shared__ char smem_raw[];
   const unsigned smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   char* const smem = smem_raw + (smem0 - smem_u32(smem_raw));
-  __shared__ unsigned long long full[S], empty[S], c_full[SC], c_empty[SC], tm_full[2],
-      tm_empty[2], drain;
+  __shared__ unsigned long long full[S], empty[S], c_full[SC], c_empty[SC], tm_full, tm_empty,
+      drain;
   __shared__ unsigned tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x & 1;
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S; ++i) {
-      // the copies' bytes, and a team of four writers in either block
-      mbar_init(&full[i], 1 + (PACKED ? P::kWriters : 0));
+      mbar_init(&full[i], 1 + kWriters);  // the copies' bytes, a team of writers in either block
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < SC; ++i) {
-      mbar_init(&c_full[i], 1 + 32);  // the codes' copy, and a warp's copies of ranges
-      mbar_init(&c_empty[i], PACKED ? P::kWriters / 2 : 1);
+      mbar_init(&c_full[i], 1 + 32);      // the codes' copy, and a warp's copies of ranges
+      mbar_init(&c_empty[i], kWriters / 2);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&tm_full[i], 1);
-      mbar_init(&tm_empty[i], 2 * P::kEpi);
-    }
+    mbar_init(&tm_full, 1);
+    mbar_init(&tm_empty, 2 * kWriters);
     mbar_init(&drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     fence_async_smem();
@@ -374,24 +339,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
     if (lane == 0) {
       unsigned n = 0;
       for (int item = first; work_of(a, item, &t); item += step) {
-        const int ia = t.i0 + rank * 128, jb = t.j0 + rank * 128;
+        const int jb = t.j0 + rank * 128;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
           const int s = n % S;
           if (n >= (unsigned)S) stage_wait(&empty[s], (n / S - 1) & 1, a.err);
           // both blocks' copies count on the first block's barrier
           const unsigned bar = in_leader(smem_u32(&full[s]));
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * (PACKED ? 1 : 2) * kHalf);
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * kHalf);
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            tma_box<true>(smem0 + s * kHalf + i * kBox, &a.a, a.a_mn ? ia + 64 * i : kb * kDepth,
-                          a.a_mn ? kb * kDepth : ia + 64 * i, 0, bar);
-          if constexpr (!PACKED) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-              tma_box<true>(smem0 + P::kBAt + s * kHalf + i * kBox, &a.b,
-                            a.b_mn ? jb + 64 * i : kb * kDepth, a.b_mn ? kb * kDepth : jb + 64 * i,
-                            0, bar);
-          }
+            tma_box<true>(smem0 + s * kHalf + i * kBox, &a.dy, jb + 64 * i, kb * kDepth, 0, bar);
         }
       }
       // copies still in flight land before the block ends
@@ -400,60 +357,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      // float32 sums; both operands float16 or both bfloat16; 256 x 256 over the pair
+      // float32 sums; both operands float16 or both bfloat16; 256 x 256 over the pair;
+      // the second operand with t as its rows
       const unsigned kind = std::is_same<T, bf16_t>::value ? (1u << 7) | (1u << 10) : 0u;
-      const unsigned idesc = (1u << 4) | kind | ((unsigned)a.a_mn << 15) |
-                             ((unsigned)a.b_mn << 16) | ((unsigned)(kTile / 8) << 17) |
+      const unsigned idesc = (1u << 4) | kind | (1u << 16) | ((unsigned)(kTile / 8) << 17) |
                              ((unsigned)(kTile / 16) << 24);
-      // 16 of k further: 2 groups of 8 rows, or 32 bytes along a row
-      const unsigned as = (a.a_mn ? 2048u : 32u) >> 4, bs = (a.b_mn ? 2048u : 32u) >> 4;
       unsigned n = 0, tile = 0;
       for (int item = first; work_of(a, item, &t); item += step, ++tile) {
-        const int buf = tile & 1;
-        if (tile >= 2) wait_pair(&tm_empty[buf], (tile / 2 - 1) & 1, a.err);
+        if (tile >= 1) wait_pair(&tm_empty, (tile - 1) & 1, a.err);
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         bool ready = false;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
           const int s = n % S;
           if (!ready) stage_wait(&full[s], (n / S) & 1, a.err);
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-          const unsigned long long p = operand(smem0 + s * kHalf),
-                                   q = operand(smem0 + P::kBAt + s * kHalf);
+          const unsigned p = tmem + kOperandAt + s * 32;
+          const unsigned long long q = operand(smem0 + s * kHalf);
 #pragma unroll
           for (int k = 0; k < kDepth / 16; ++k) {
-            mma_f16<true>(tmem + buf * 256, p + k * as, q + k * bs, idesc, kb > t.kb0 || k > 0);
+            mma_from_tmem(tmem, p + 8 * k, q + k * (2048u >> 4), idesc, kb > t.kb0 || k > 0);
             // the next stage is asked for while this one's products run: few are queued,
             // and a poll takes longer than the last of them
             if (k == 1) ready = kb + 1 < t.kb1 && mbar_peek(&full[(n + 1) % S], ((n + 1) / S) & 1);
           }
           mma_commit<true>(&empty[s]);
         }
-        mma_commit<true>(&tm_full[buf]);
+        mma_commit<true>(&tm_full);
       }
       // products still in flight end before tensor memory is given back
       mma_commit<true>(&drain);
       stage_wait(&drain, 0, a.err);
     }
-  } else if (PACKED && warp == 3) {
-    // codes of a stage, and their ranges: 4 words a lane, zeros (operands of zero)
-    // behind the last row
+  } else if (warp == 3) {
+    // codes of a stage, and their ranges, a group's 64 rows after another's: 4 words a
+    // lane, zeros (operands of zero) behind the last row
     unsigned n = 0;
     for (int item = first; work_of(a, item, &t); item += step) {
-      const int jb = t.j0 + rank * 128, g = jb / kGroup8 + (lane & 1);
+      const int ia = t.i0 + rank * 128, g = ia / kGroup8 + (lane & 1);
       for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
         const int s = n % SC;
         if (n >= (unsigned)SC) warp_wait(&c_empty[s], (n / SC - 1) & 1, a.err);
         if (lane == 0) {
           mbar_expect_tx(&c_full[s], kRaw);
-          tma_box<false>(smem0 + P::kCodesAt + s * kRaw, &a.b, jb, kb * kDepth, 0,
+          tma_box<false>(smem0 + kCodesAt + s * kRaw, &a.codes, ia, kb * kDepth, 0,
                          smem_u32(&c_full[s]));
         }
-        const unsigned to = smem0 + P::kRangesAt + s * kRanges + lane * 4;
+        const unsigned to =
+            smem0 + kRangesAt + s * kRanges + ((lane & 1) * kDepth + (lane >> 1)) * 4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const long long r = (long long)kb * kDepth + 16 * i + (lane >> 1);
           const bool in = g < a.groups && r < a.rows;
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(to + 128 * i),
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(to + 64 * i),
                        "l"(a.ranges + (in ? r * a.groups + g : 0)), "r"(in ? 4 : 0)
                        : "memory");
         }
@@ -465,86 +420,96 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
     asm volatile("cp.async.wait_all;\n" ::: "memory");
     for (unsigned i = n > (unsigned)SC ? n - SC : 0; i < n; ++i)
       warp_wait(&c_full[i % SC], (i / SC) & 1, a.err);
-  } else if (PACKED && warp >= 4 && warp < 4 + P::kWriters) {
+  } else if (warp >= 4) {
     // Two teams of four warps take the stages in turn, so that one team's loads and
-    // barriers run beside the other's arithmetic.  A thread has 16 columns of four of
-    // a stage's 64 rows.
-    const int team = (warp - 4) >> 2, id = threadIdx.x & 127, row = id >> 3, seg = id & 7;
-    const int odd = seg >> 2, u = (seg & 3) * 2;
-    unsigned n = 0;
-    for (int item = first; work_of(a, item, &t); item += step) {
+    // barriers run beside the other's arithmetic.  A warp has 32 inputs, the lanes of
+    // tensor memory that it may touch, and all 64 rows of a stage.
+    const int team = (warp - 4) >> 2, w = warp & 3;
+    unsigned n = 0, tile = 0;
+    for (int item = first; work_of(a, item, &t); item += step, ++tile) {
       for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
         if ((int)(n & 1) != team) continue;
         const int s = n % S, c = n % SC;
         warp_wait(&c_full[c], (n / SC) & 1, a.err);
-        const char* const codes = smem + P::kCodesAt + c * kRaw + seg * 16;
-        const unsigned* const ranges =
-            reinterpret_cast<const unsigned*>(smem + P::kRangesAt + c * kRanges) + odd;
-        uint4 q[4];
-        unsigned bits[4];
+        const uint4* const ranges =
+            reinterpret_cast<const uint4*>(smem + kRangesAt + c * kRanges) + (w >> 1) * (kDepth / 4) +
+            (lane & 3);
+        Range4 r[4];
+        bool held = true;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          q[h] = *reinterpret_cast<const uint4*>(codes + (row + 16 * h) * 128);
-          bits[h] = ranges[(row + 16 * h) * 2];
+        for (int b = 0; b < 4; ++b) {  // 16 rows each, four of them this lane's
+          const uint4 bits = ranges[4 * b];
+          r[b] = range4<T>(bits);
+          if constexpr (std::is_same<T, f16_t>::value) held = held && held_in_half(bits);
         }
-        if (n >= (unsigned)S) warp_wait(&empty[s], (n / S - 1) & 1, a.err);
-        // Only now: the codes of stage n + 5 then follow this stage's phase, so that the
-        // other team, whose that stage is, cannot take an older phase for it.
-        __syncwarp();
-        if (lane == 0) arrive_leader<false>(&c_empty[c]);
-        char* const stage = smem + P::kBAt + s * kHalf + odd * kBox;
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          const int r = row + 16 * h;
-          uint4 o[2];
-          operands16<T>(q[h], bits[h], o);
-          // blocks of 64 columns; 128-byte rows whose 16-byte units are xor-ed with the
-          // row; the two halves of a row's columns take turns at the banks
-          char* const to = stage + r * 128;
-          *reinterpret_cast<uint4*>(to + (((u + odd) ^ (r & 7)) << 4)) = odd ? o[1] : o[0];
-          *reinterpret_cast<uint4*>(to + (((u + 1 - odd) ^ (r & 7)) << 4)) = odd ? o[0] : o[1];
+        for (int half = 0; half < 2; ++half) {
+          unsigned v[16];
+#pragma unroll
+          for (int bb = 0; bb < 2; ++bb) {
+            // rows of 128 bytes whose 16-byte units are xor-ed with the row
+            const int row = 32 * bb + lane;
+            unsigned q[4];
+            codes16x2(smem0 + kCodesAt + c * kRaw + row * 128 + (((2 * w + half) ^ (row & 7)) << 4), q);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {  // block of 16 rows, input, pair of rows
+              const int b = i >> 2, in = (i >> 1) & 1, k = i & 1;
+              const Range4& g = r[2 * bb + b];
+              v[8 * bb + i] = operand2(q[2 * b + in], 2 * k, g.s[k], g.lo[k], T());
+            }
+            if constexpr (std::is_same<T, f16_t>::value) {
+              if (!held) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const int b = i >> 2, in = (i >> 1) & 1, k = i & 1;
+                  const uint4 bits = ranges[4 * (2 * bb + b)];
+                  v[8 * bb + i] = operand2_wide(q[2 * b + in], 2 * k, k ? bits.z : bits.x,
+                                                k ? bits.w : bits.y);
+                }
+              }
+            }
+          }
+          if (half == 0) {
+            if (n >= (unsigned)S) warp_wait(&empty[s], (n / S - 1) & 1, a.err);
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          }
+          tmem_store16(tmem + kOperandAt + s * 32 + ((unsigned)(32 * w + 16 * half) << 16), v);
         }
-        fence_async_smem();
+        asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
         __syncwarp();
-        if (lane == 0) arrive_written(&full[s]);
+        if (lane == 0) {
+          arrive_written(&full[s]);
+          arrive_leader<false>(&c_empty[c]);
+        }
       }
-    }
-  } else if (warp >= 4 + P::kWriters) {
-    const int w = warp & 3, h = (warp - 4 - P::kWriters) >> 2;
-    constexpr int kCols = kTile * 4 / P::kEpi;  // columns of a warp
-    char* const turn = smem + P::kTurnAt + (warp - 4 - P::kWriters) * kTurn;
-    unsigned tile = 0;
-    for (int item = first; work_of(a, item, &t); item += step, ++tile) {
-      const int buf = tile & 1;
-      if (lane == 0) wait_pair(&tm_full[buf], (tile / 2) & 1, a.err);
+      // the tile's sums: a lane an input, this team's half of the outputs
+      if (lane == 0) wait_pair(&tm_full, tile & 1, a.err);
       __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-      const int i = t.i0 + rank * 128 + 32 * w;
+      const int i = t.i0 + rank * 128 + 32 * w + lane;
 #pragma unroll 1
-      for (int c = h * kCols; c < (h + 1) * kCols; c += 64) {
-        float v[64];
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-          tmem_load32(tmem + buf * 256 + c + 32 * q + ((unsigned)(32 * w) << 16),
-                      *reinterpret_cast<float(*)[32]>(v + 32 * q));
-        if (c + 64 == (h + 1) * kCols) {
+      for (int c = team * 128; c < team * 128 + 128; c += 32) {
+        float v[32];
+        tmem_load32(tmem + c + ((unsigned)(32 * w) << 16), v);
+        if (c + 32 == team * 128 + 128) {
           __syncwarp();
           asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-          if (lane == 0) arrive_leader<true>(&tm_empty[buf]);
+          if (lane == 0) arrive_leader<true>(&tm_empty);
         }
-        if (PACKED && a.parts > 1) {
-          // [item][block][columns / 4][128 rows] of four columns each
-          float4* const to = reinterpret_cast<float4*>(
-              a.part + ((long long)t.item * 2 + rank) * kPartFloats) + c / 4 * 128 + 32 * w + lane;
+        if (a.parts > 1) {  // [item][block][outputs][128 inputs]
+          float* const to =
+              a.part + ((long long)t.item * 2 + rank) * kPartFloats + c * 128 + 32 * w + lane;
 #pragma unroll
-          for (int q = 0; q < 16; ++q)
-            to[q * 128] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        } else if (i < a.m && t.j0 + c < a.n) {
-          put_result<T>(a, i, t.j0 + c, v, turn);
+          for (int q = 0; q < 32; ++q) to[q * 128] = v[q];
+        } else if (i < a.m) {
+          T* const to = reinterpret_cast<T*>(a.out) + (long long)(t.j0 + c) * a.m + i;
+#pragma unroll
+          for (int q = 0; q < 32; ++q)
+            if (t.j0 + c + q < a.n) to[(long long)q * a.m] = St<T>::v(v[q]);
         }
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
@@ -558,7 +523,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Product<PACKED>::kTh
   }
 }
 
-// The parts of a tile added in order: a thread has 16 columns of a row.
+// The parts of a tile added in order: a block has 16 outputs of 128 inputs.
 template <typename T>
 __global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__ ProductArgs a) {
   const int tiles = a.tiles_m * a.tiles_n;
@@ -569,29 +534,15 @@ __global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__
   if (i >= a.m || j >= a.n) return;
   float v[16] = {};
   for (int p = 0; p < a.parts; ++p) {
-    const float4* const from = reinterpret_cast<const float4*>(
-        a.part + ((long long)(p * tiles + tile) * 2 + rank) * kPartFloats) + c / 4 * 128 + threadIdx.x;
+    const float* const from =
+        a.part + ((long long)(p * tiles + tile) * 2 + rank) * kPartFloats + c * 128 + threadIdx.x;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float4 f = from[q * 128];
-      v[4 * q] += f.x;
-      v[4 * q + 1] += f.y;
-      v[4 * q + 2] += f.z;
-      v[4 * q + 3] += f.w;
-    }
+    for (int q = 0; q < 16; ++q) v[q] += from[q * 128];
   }
-  T* const out = reinterpret_cast<T*>(a.out) + (long long)i * a.n + j;
-  if (a.tma_out && j + 16 <= a.n) {
+  T* const out = reinterpret_cast<T*>(a.out) + (long long)j * a.m + i;
 #pragma unroll
-    for (int q = 0; q < 2; ++q)
-      reinterpret_cast<uint4*>(out)[q] =
-          make_uint4(pair_bits<T>(v[8 * q], v[8 * q + 1]), pair_bits<T>(v[8 * q + 2], v[8 * q + 3]),
-                     pair_bits<T>(v[8 * q + 4], v[8 * q + 5]), pair_bits<T>(v[8 * q + 6], v[8 * q + 7]));
-  } else {
-#pragma unroll
-    for (int q = 0; q < 16; ++q)
-      if (j + q < a.n) out[q] = St<T>::v(v[q]);
-  }
+  for (int q = 0; q < 16; ++q)
+    if (j + q < a.n) out[(long long)q * a.m] = St<T>::v(v[q]);
 }
 
 // Rows at a pitch of whole 16 bytes, for TMA.
@@ -618,19 +569,19 @@ constexpr int kMaxSide = (1 << 22) - 64;  // 65535 tiles of 64
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// [rows][pitch bytes] of 16-bit values, boxes of 64 x `high` in the 128-byte
-// swizzle; or of bytes, boxes of 128 x 64 as they lie.  Outside arrives as zeros.
+// [rows][pitch bytes] of 16-bit values in boxes of 64 x 64, or of bytes in boxes of
+// 128 x 64, in the 128-byte swizzle.  Outside arrives as zeros.
 static bool box_map(CUtensorMap* map, const void* p, long long rows, long long cols,
-                    long long pitch, bool bytes, int high) {
+                    long long pitch, bool bytes) {
   EncodeTiledFn fn = encode_tiled();
   if (!fn) return false;
   const cuuint64_t dim[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1};
   const cuuint64_t stride[2] = {(cuuint64_t)pitch, (cuuint64_t)(pitch * rows)};
-  const cuuint32_t box[3] = {bytes ? 128u : 64u, (cuuint32_t)high, 1}, one[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {bytes ? 128u : 64u, (cuuint32_t)kDepth, 1}, one[3] = {1, 1, 1};
   return fn(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3,
             const_cast<void*>(p), dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            bytes ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 static int tiles_of(long long n) { return (int)((n + kTile - 1) / kTile); }
@@ -662,17 +613,17 @@ static int resident_pairs(int device) {
   const ScopedDevice scope(device < MAXD ? device : -1);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(sm_count(device) / 2 * 2));
-  cfg.blockDim = dim3(Product<true>::kThreads);
-  cfg.dynamicSmemBytes = Product<true>::kSmem;
+  cfg.blockDim = dim3(kWgThreads);
+  cfg.dynamicSmemBytes = kWgSmem;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = 2;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  if (cudaFuncSetAttribute(product_kernel<bf16_t, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           Product<true>::kSmem) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, product_kernel<bf16_t, true>, &cfg) != cudaSuccess || n < 1) {
+  if (cudaFuncSetAttribute(wgrad_kernel<bf16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           kWgSmem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, wgrad_kernel<bf16_t>, &cfg) != cudaSuccess || n < 1) {
     cudaGetLastError();
     n = std::max(1, sm_count(device) / 2);
   }
@@ -705,17 +656,6 @@ size_t wgrad8_ws_bytes(long long rows, int inputs, int outputs, int dtype, int d
   return wgrad_plan(rows, inputs, outputs, dtype, device).bytes;
 }
 
-template <typename T, bool PACKED>
-static int product_run(const ProductArgs& a, int pairs, cudaStream_t st) {
-  constexpr int smem = Product<PACKED>::kSmem;
-  FAB_TRY(cudaFuncSetAttribute(product_kernel<T, PACKED>,
-                               cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  const int items = a.tiles_m * a.tiles_n * a.parts;
-  product_kernel<T, PACKED><<<2 * std::min(items, pairs), Product<PACKED>::kThreads, smem, st>>>(a);
-  FAB_LAUNCH_CHECK();
-  return FA_OK;
-}
-
 template <typename T>
 static int wgrad_run(const void* dy, long long dy_row, const void* codes, const void* ranges,
                      long long rows, int inputs, int outputs, void* dw, char* ws,
@@ -733,17 +673,14 @@ static int wgrad_run(const void* dy, long long dy_row, const void* codes, const 
   if (rows == 1) dy_row = plan.pitch;
   ProductArgs a = {};
   const long long groups = groups8(inputs);
-  if (!box_map(&a.a, dy, rows, outputs, dy_row * 2, false, 64) ||
-      !box_map(&a.b, codes, rows, groups * kGroup8, groups * kGroup8, true, kDepth))
+  if (!box_map(&a.dy, dy, rows, outputs, dy_row * 2, false) ||
+      !box_map(&a.codes, codes, rows, groups * kGroup8, groups * kGroup8, true))
     return FA_E_INTERNAL;
-  a.tma_out = inputs % 8 == 0 && reinterpret_cast<size_t>(dw) % 16 == 0;
-  if (a.tma_out && !box_map(&a.d, dw, outputs, inputs, inputs * 2ll, false, 32)) return FA_E_INTERNAL;
-  a.m = outputs;
-  a.n = inputs;
+  a.m = inputs;
+  a.n = outputs;
   a.kb = (int)((rows + kDepth - 1) / kDepth);
-  a.a_mn = a.b_mn = 1;
-  a.tiles_m = tiles_of(outputs);
-  a.tiles_n = tiles_of(inputs);
+  a.tiles_m = tiles_of(inputs);
+  a.tiles_n = tiles_of(outputs);
   a.parts = plan.parts;
   a.ranges = static_cast<const unsigned*>(ranges);
   a.rows = rows;
@@ -751,7 +688,10 @@ static int wgrad_run(const void* dy, long long dy_row, const void* codes, const 
   a.out = dw;
   a.part = reinterpret_cast<float*>(ws + plan.part);
   a.err = wait_error_word();
-  if (const int rc = product_run<T, true>(a, plan.pairs, st)) return rc;
+  FAB_TRY(cudaFuncSetAttribute(wgrad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmem));
+  const int items = a.tiles_m * a.tiles_n * a.parts;
+  wgrad_kernel<T><<<2 * std::min(items, plan.pairs), kWgThreads, kWgSmem, st>>>(a);
+  FAB_LAUNCH_CHECK();
   if (a.parts > 1) {
     join_parts_kernel<T><<<(unsigned)(a.tiles_m * a.tiles_n * 32), 128, 0, st>>>(a);
     FAB_LAUNCH_CHECK();
