@@ -388,28 +388,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
       mma_commit<true>(&drain);
       stage_wait(&drain, 0, a.err);
     }
-  } else if (warp == 3) {
-    // codes of a stage, and their ranges, a group's 64 rows after another's: 4 words a
-    // lane, zeros (operands of zero) behind the last row
-    unsigned n = 0;
-    for (int item = first; work_of(a, item, &t); item += step) {
-      const int ia = t.i0 + rank * 128, g = ia / kGroup8 + (lane & 1);
-      for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
-        const int s = n % SC;
-        if (n >= (unsigned)SC) warp_wait(&c_empty[s], (n / SC - 1) & 1, a.err);
-        if (lane == 0) {
+  } else if (warp == 2) {
+    if (lane == 0) {  // codes
+      unsigned n = 0;
+      for (int item = first; work_of(a, item, &t); item += step)
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
+          const int s = n % SC;
+          if (n >= (unsigned)SC) stage_wait(&c_empty[s], (n / SC - 1) & 1, a.err);
           mbar_expect_tx(&c_full[s], kRaw);
-          tma_box<false>(smem0 + kCodesAt + s * kRaw, &a.codes, ia, kb * kDepth, 0,
+          tma_box<false>(smem0 + kCodesAt + s * kRaw, &a.codes, t.i0 + rank * 128, kb * kDepth, 0,
                          smem_u32(&c_full[s]));
         }
+      for (unsigned i = n > (unsigned)SC ? n - SC : 0; i < n; ++i)
+        stage_wait(&c_full[i % SC], (i / SC) & 1, a.err);
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // ranges, a group's 64 rows after another's: 4 words a lane, zeros (operands of
+    // zero) behind the last row
+    unsigned n = 0;
+    for (int item = first; work_of(a, item, &t); item += step) {
+      const int g = (t.i0 + rank * 128) / kGroup8 + (lane & 1);
+      const bool in = g < a.groups;
+      long long r = (long long)t.kb0 * kDepth + (lane >> 1);
+      const unsigned* from = a.ranges + (in ? r * a.groups + g : 0);
+      const long long apart = in ? 16ll * a.groups : 0;
+      for (int kb = t.kb0; kb < t.kb1; ++kb, ++n, r += kDepth, from += 4 * apart) {
+        const int s = n % SC;
+        if (n >= (unsigned)SC) warp_wait(&c_empty[s], (n / SC - 1) & 1, a.err);
         const unsigned to =
             smem0 + kRangesAt + s * kRanges + ((lane & 1) * kDepth + (lane >> 1)) * 4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const long long r = (long long)kb * kDepth + 16 * i + (lane >> 1);
-          const bool in = g < a.groups && r < a.rows;
+          const bool here = in && r + 16 * i < a.rows;
           asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(to + 64 * i),
-                       "l"(a.ranges + (in ? r * a.groups + g : 0)), "r"(in ? 4 : 0)
+                       "l"(here ? from + i * apart : a.ranges), "r"(here ? 4 : 0)
                        : "memory");
         }
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(
@@ -418,8 +431,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
       }
     }
     asm volatile("cp.async.wait_all;\n" ::: "memory");
-    for (unsigned i = n > (unsigned)SC ? n - SC : 0; i < n; ++i)
-      warp_wait(&c_full[i % SC], (i / SC) & 1, a.err);
   } else if (warp >= 4) {
     // Two teams of four warps take the stages in turn, so that one team's loads and
     // barriers run beside the other's arithmetic.  A warp has 32 inputs, the lanes of
@@ -586,14 +597,14 @@ static bool box_map(CUtensorMap* map, const void* p, long long rows, long long c
 
 static int tiles_of(long long n) { return (int)((n + kTile - 1) / kTile); }
 
-// Parts of the sum's axis: the number whose waves take the least time, at 0.4 us a
-// stage of a pair, 3 us a tile's end, and the parts' trip through memory.
+// Parts of the sum's axis: the number whose waves take the least time, at 0.42 us a
+// stage of a pair, 6 us a tile's end, and the parts' trip through memory.
 static int parts_of(int tiles, int kb, int pairs) {
   int best = 1;
   double least = 0;
   for (int p = 1; p <= 32 && p <= kb; ++p) {
     const double waves = (double)((tiles * (long long)p + pairs - 1) / pairs);
-    double us = waves * (0.4 * ((kb + p - 1) / p) + 3.0);
+    double us = waves * (0.42 * ((kb + p - 1) / p) + 6.0);
     if (p > 1) us += 4.0 + tiles * (double)p * 2 * kPartFloats * 4 * 2 / 4e6;
     if (p == 1 || us < least) {
       least = us;
