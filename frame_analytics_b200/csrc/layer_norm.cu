@@ -31,7 +31,7 @@ struct NormArgs {
   void* ranges;
   long long rows;
   int width, groups;
-  float eps;
+  float eps, inv_width;
   // weight gradients
   float* part;                  // [splits][2][width] partial sums
   void *dw, *db;                // or null
@@ -107,33 +107,76 @@ __device__ __forceinline__ void keep8(const NormArgs& a, long long row, int u, i
         range_bits(r, T());
 }
 
-// Rows that fit the registers of up to 32 warps: E units of 8 columns a lane, `wpr`
-// warps a row, every byte read and written once.
+// 1 / sqrt(v): the fast root and a Newton step.
+__device__ __forceinline__ float inv_sqrt(float v) {
+  const float r = rsqrtf(v);
+  // of an infinite variance (0) or a variance and eps of 0 (infinity) there is no step
+  return r > 0.f && r < __uint_as_float(0x7f800000u) ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
+}
+
+// A sum over the row's length: the reciprocal, corrected once, so that an even row's mean
+// is its value.
+__device__ __forceinline__ float mean_of(float t, const NormArgs& a) {
+  const float q = t * a.inv_width;
+  return fmaf(fmaf(-q, (float)a.width, t), a.inv_width, q);
+}
+
+// Two sums over the warp with the shuffles of little more than one: the halves of the
+// warp take one each.  Lane 0 has the first, lane 16 the second.
+__device__ __forceinline__ float warp_sum2(float a, float b) {
+  const bool low = (threadIdx.x & 16) == 0;
+  const float give = low ? b : a;
+  float t = (low ? a : b) + __shfl_xor_sync(0xffffffffu, give, 16);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  return t;
+}
+
+// Both passes below keep a row in the registers of `wpr` warps, E units of 256 columns
+// a warp, and read and write every byte once.  What a row costs apart from its values
+// (addresses, the joining of sums) bounds them as much as bytes do.
 template <typename T, bool VEC, int E, int NT>
-__global__ void __launch_bounds__(NT) norm_kernel(const NormArgs a, int wpr) {
-  __shared__ float sm[2][32];
+__global__ void __launch_bounds__(NT, 1024 / NT) norm_kernel(const NormArgs a, int wpr) {
+  __shared__ float sm[4][32];
   __shared__ __align__(16) Turn8<T> turns[VEC ? 1 : NT / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Turn8<T>* const turn = turns + (VEC ? 0 : warp);
   const int at = warp % wpr, first = warp - at;          // this warp in its row, the row's first
-  const long long row = (long long)blockIdx.x * (blockDim.x / 32 / wpr) + warp / wpr;
-  const bool in = row < a.rows;
-  const int units = a.groups * 8;
-  // s stays as it lies in memory and is widened for each of the three passes over it:
-  // half the registers of float32 values, so twice the rows under way
-  Raw8<T> s[E];
+  const int rpb = blockDim.x / 32 / wpr;
+  const int c0 = (at * E * 32 + lane) * 8;
   int n[E];
-  {
-    Raw8<T> q[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int c = ((e * wpr + at) * 32 + lane) * 8;
-      n[e] = in ? max(0, min(8, a.width - c)) : 0;
-      s[e] = fetch8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n[e], turn);
-      if (a.res)
-        q[e] = fetch8<T, VEC>(reinterpret_cast<const T*>(a.res) + row * a.res_row + c, n[e], turn);
-    }
+  for (int e = 0; e < E; ++e) n[e] = max(0, min(8, a.width - c0 - 256 * e));
+  const long long start = (long long)blockIdx.x * rpb + warp / wpr;
+  const long long step = (long long)gridDim.x * rpb;
+  const T* xp = reinterpret_cast<const T*>(a.x) + start * a.x_row + c0;
+  const T* rp = reinterpret_cast<const T*>(a.res) + (a.res ? start * a.res_row + c0 : 0);
+  T* yp = reinterpret_cast<T*>(a.y) + start * a.width + c0;
+  const long long to_sum = a.sum ? reinterpret_cast<T*>(a.sum) - reinterpret_cast<T*>(a.y) : 0;
+  int half = 0;
+  const auto row_sum = [&](float t, int k) {
+    t = warp_sum(t);
+    if (wpr == 1) return t;
+    if (lane == 0) sm[k][warp] = t;
+    __syncthreads();            // the next row's sums have the other buffers
+    t = 0.f;
+    for (int w = 0; w < wpr; ++w) t += sm[k][first + w];
+    return t;
+  };
+  long long row = start;
+  for (long long row0 = (long long)blockIdx.x * rpb; row0 < a.rows;
+       row0 += step, row += step, half ^= 2) {
+    const bool in = row < a.rows;
+    // s stays as it lies in memory and is widened for each of the three passes over it:
+    // half the registers of float32 values, so twice the rows under way
+    Raw8<T> s[E];
     if (a.res) {
+      Raw8<T> q[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        s[e] = fetch8<T, VEC>(xp + 256 * e, in ? n[e] : 0, turn);
+        q[e] = fetch8<T, VEC>(rp + 256 * e, in ? n[e] : 0, turn);
+      }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         F8 x = widen8(s[e]);
@@ -142,52 +185,57 @@ __global__ void __launch_bounds__(NT) norm_kernel(const NormArgs a, int wpr) {
         for (int i = 0; i < 4; ++i) x.v[i] = __fadd2_rn(x.v[i], y.v[i]);
         s[e] = narrow8(x, T());
       }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) s[e] = fetch8<T, VEC>(xp + 256 * e, in ? n[e] : 0, turn);
     }
-  }
-  const auto row_sum = [&](float t, int k) {
-    t = warp_sum(t);
-    if (wpr == 1) return t;
-    if (lane == 0) sm[k][warp] = t;
-    __syncthreads();
-    t = 0.f;
-    for (int w = 0; w < wpr; ++w) t += sm[k][first + w];
-    return t;
-  };
-  float t = 0.f;
+    float2 t = both(0.f);
 #pragma unroll
-  for (int e = 0; e < E; ++e) t += sum8(widen8(s[e]));
-  const float m = row_sum(t, 0) / (float)a.width;
-  float2 v = both(0.f);
+    for (int e = 0; e < E; ++e) {
+      const F8 x = widen8(s[e]);
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    if (VEC && n[e] == 0) continue;
-    F8 x = widen8(s[e]);
-    if (!VEC) fill_from(x, n[e], m);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 d = __fadd2_rn(x.v[i], both(-m));
-      v = __ffma2_rn(d, d, v);
+      for (int i = 0; i < 4; ++i) t = __fadd2_rn(t, x.v[i]);
     }
-  }
-  const float r = 1.f / sqrtf(row_sum(v.x + v.y, 1) / (float)a.width + a.eps);
-  if (a.stats && in && at == 0 && lane == 0) a.stats[row] = make_float2(m, r);
+    const float m = mean_of(row_sum(t.x + t.y, half), a);
+    float2 v = both(0.f);
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int u = (e * wpr + at) * 32 + lane, c = u * 8;
-    F8 x = widen8(s[e]);
-    if (a.sum) store8<T, VEC>(reinterpret_cast<T*>(a.sum) + row * a.width + c, n[e], x, turn);
-    if (a.codes) keep8<T, VEC>(a, row, u, n[e], in && u < units, x, s[e]);
-    const F8 w = weights8<T, VEC>(a, a.w, c, n[e], 1.f), b = weights8<T, VEC>(a, a.b, c, n[e], 0.f);
-    normalise8(x, m, r);
+    for (int e = 0; e < E; ++e) {
+      if (VEC && n[e] == 0) continue;
+      F8 x = widen8(s[e]);
+      if (!VEC) fill_from(x, n[e], m);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x.v[i] = __ffma2_rn(x.v[i], w.v[i], b.v[i]);
-    store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n[e], x, turn);
+      for (int i = 0; i < 4; ++i) {
+        const float2 d = __fadd2_rn(x.v[i], both(-m));
+        v = __ffma2_rn(d, d, v);
+      }
+    }
+    const float r = inv_sqrt(fmaf(row_sum(v.x + v.y, half + 1), a.inv_width, a.eps));
+    if (a.stats && in && at == 0 && lane == 0) a.stats[row] = make_float2(m, r);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int k = in ? n[e] : 0;
+      F8 x = widen8(s[e]);
+      if (a.sum) store8<T, VEC>(yp + to_sum + 256 * e, k, x, turn);
+      if (a.codes)
+        keep8<T, VEC>(a, row, c0 / 8 + 32 * e, k, in && c0 / 8 + 32 * e < a.groups * 8, x, s[e]);
+      normalise8(x, m, r);
+      if (a.w || a.b) {
+        const F8 w = weights8<T, VEC>(a, a.w, c0 + 256 * e, n[e], 1.f),
+                 b = weights8<T, VEC>(a, a.b, c0 + 256 * e, n[e], 0.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.v[i] = __ffma2_rn(x.v[i], w.v[i], b.v[i]);
+      }
+      store8<T, VEC>(yp + 256 * e, k, x, turn);
+    }
+    xp += step * a.x_row;
+    rp += step * a.res_row;
+    yp += step * a.width;
   }
 }
 
-// The backward pass of such rows: blocks stay and take rows in turn; a lane keeps the
-// weight gradients of its columns in registers, the block adds its rows' at the end
-// and writes one part.  The next row's loads are under way while a row's sums run.
+// Backward: a lane keeps the weight gradients of its columns in registers, the block
+// adds its rows' at the end and writes one part.  The next row's loads are under way
+// while a row's sums run.
 template <typename T, bool VEC, int E, bool CODES, int NT>
 __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs a, int wpr) {
   __shared__ float2 sm[2][NT / 32];
@@ -197,69 +245,88 @@ __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Turn8<T>* const turn = turns + (VEC ? 0 : warp);
   const int at = warp % wpr, first = warp - at, rpb = NT / 32 / wpr;
+  const int c0 = (at * E * 32 + lane) * 8;
   F8 dw[E], db[E];
   Raw8<T> w[E];                 // weights of the operands' type stay; others are read anew
+  int n[E];
   const bool w_kept = VEC && a.w && a.w_vec && (sizeof(T) == 4 || !a.w32);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) dw[e].v[i] = db[e].v[i] = both(0.f);
-    const int c = ((e * wpr + at) * 32 + lane) * 8;
-    w[e] = w_kept && c < a.width ? get8<T>(reinterpret_cast<const T*>(a.w) + c) : zero8<T>();
+    n[e] = max(0, min(8, a.width - c0 - 256 * e));
+    w[e] = w_kept && n[e] ? get8<T>(reinterpret_cast<const T*>(a.w) + c0 + 256 * e) : zero8<T>();
   }
+  const long long start = (long long)blockIdx.x * rpb + warp / wpr;
+  const long long step = (long long)gridDim.x * rpb;
+  const T* gp = reinterpret_cast<const T*>(a.dy) + start * a.dy_row + c0;
+  const T* sp = reinterpret_cast<const T*>(a.ds) + (a.ds ? start * a.ds_row + c0 : 0);
+  const T* xp = reinterpret_cast<const T*>(a.x) + (CODES ? 0 : start * a.x_row + c0);
+  const uint2* cp = reinterpret_cast<const uint2*>(a.codes) + (start * a.groups * 8 + c0 / 8);
+  const Bits* bp = reinterpret_cast<const Bits*>(a.ranges) + (start * a.groups + c0 / kGroup8);
+  T* yp = reinterpret_cast<T*>(a.y) + start * a.width + c0;
   struct Row {                  // as it lies in memory
     Raw8<T> x[E], g[E], s[E];
     uint2 code[E];
     Bits bits[E];
     float2 st;
   };
-  const auto load = [&](long long row, Row& o) {
+  const auto load = [&](long long row, Row& o) {  // and on to the next
     const bool in = row < a.rows;
-    if (!in) row = 0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int u = (e * wpr + at) * 32 + lane, c = u * 8, n = in ? max(0, min(8, a.width - c)) : 0;
+      const int k = in ? n[e] : 0;
       if constexpr (CODES) {
-        o.code[e] = make_uint2(0u, 0u);
-        o.bits[e] = Bits();
-        if (n) {
-          o.code[e] = __ldg(reinterpret_cast<const uint2*>(a.codes) + row * a.groups * 8 + u);
-          o.bits[e] = __ldg(reinterpret_cast<const Bits*>(a.ranges) + row * a.groups + u / 8);
+        if (!VEC || k) {
+          o.code[e] = k ? __ldg(cp + 32 * e) : make_uint2(0u, 0u);
+          o.bits[e] = k ? __ldg(bp + 4 * e) : Bits();
         }
       } else {
-        o.x[e] = fetch8<T, VEC>(reinterpret_cast<const T*>(a.x) + row * a.x_row + c, n, turn);
+        o.x[e] = fetch8<T, VEC>(xp + 256 * e, k, turn);
       }
-      o.g[e] = fetch8<T, VEC>(reinterpret_cast<const T*>(a.dy) + row * a.dy_row + c, n, turn);
-      if (a.ds) o.s[e] = fetch8<T, VEC>(reinterpret_cast<const T*>(a.ds) + row * a.ds_row + c, n, turn);
+      o.g[e] = fetch8<T, VEC>(gp + 256 * e, k, turn);
+      if (a.ds) o.s[e] = fetch8<T, VEC>(sp + 256 * e, k, turn);
     }
-    o.st = in ? __ldg(a.stats + row) : make_float2(0.f, 0.f);
+    if (in) o.st = __ldg(a.stats + row);
+    if constexpr (CODES) {
+      cp += step * a.groups * 8;
+      bp += step * a.groups;
+    } else {
+      xp += step * a.x_row;
+    }
+    gp += step * a.dy_row;
+    sp += step * a.ds_row;
   };
-  const long long step = (long long)gridDim.x * rpb;
   int half = 0;
   Row now;
-  load((long long)blockIdx.x * rpb + warp / wpr, now);
+  now.st = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    now.code[e] = make_uint2(0u, 0u);
+    now.bits[e] = Bits();
+  }
+  long long row = start;
+  load(row, now);
   for (long long row0 = (long long)blockIdx.x * rpb; row0 < a.rows; row0 += step, half ^= 1) {
-    const long long row = row0 + warp / wpr;
     const bool in = row < a.rows;
-    const float r = now.st.y;
+    const float m = now.st.x, r = now.st.y;
     F8 h[E], g[E];
     float2 c1 = both(0.f), c2 = both(0.f);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = ((e * wpr + at) * 32 + lane) * 8, n = in ? max(0, min(8, a.width - c)) : 0;
+      if (VEC && (!in || !n[e])) continue;
       if constexpr (CODES) h[e] = decode8<T>(now.code[e], range_of(now.bits[e], T()));
       else h[e] = widen8(now.x[e]);
       g[e] = widen8(now.g[e]);
-      if (VEC && n == 0) continue;
-      normalise8(h[e], now.st.x, r);
-      if (!VEC) fill_from(h[e], n, 0.f);
+      normalise8(h[e], m, r);
+      if (!VEC) fill_from(h[e], in ? n[e] : 0, 0.f);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         dw[e].v[i] = __ffma2_rn(g[e].v[i], h[e].v[i], dw[e].v[i]);
         db[e].v[i] = __fadd2_rn(db[e].v[i], g[e].v[i]);
       }
       if (a.w) {
-        const F8 f = w_kept ? widen8(w[e]) : weights8<T, VEC>(a, a.w, c, n, 1.f);
+        const F8 f = w_kept ? widen8(w[e]) : weights8<T, VEC>(a, a.w, c0 + 256 * e, n[e], 1.f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) g[e].v[i] = __fmul2_rn(g[e].v[i], f.v[i]);
       }
@@ -274,33 +341,40 @@ __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs 
 #pragma unroll
       for (int e = 0; e < E; ++e) s[e] = now.s[e];
     }
-    load(row + step, now);
-    float s1 = warp_sum(c1.x + c1.y), s2 = warp_sum(c2.x + c2.y);
+    row += step;
+    load(row, now);
+    const float both_sums = warp_sum2(c1.x + c1.y, c2.x + c2.y);
+    float s1, s2;
     if (wpr > 1) {
-      if (lane == 0) sm[half][warp] = make_float2(s1, s2);
+      if ((lane & 15) == 0) reinterpret_cast<float*>(&sm[half][warp])[lane >> 4] = both_sums;
       __syncthreads();          // one a row: the next row's sums have the other half
       s1 = s2 = 0.f;
       for (int i = 0; i < wpr; ++i) {
         s1 += sm[half][first + i].x;
         s2 += sm[half][first + i].y;
       }
+    } else {
+      s1 = __shfl_sync(0xffffffffu, both_sums, 0);
+      s2 = __shfl_sync(0xffffffffu, both_sums, 16);
     }
     // dx = r (g - s1 / N - h s2 / N)
-    s1 = -s1 / (float)a.width;
-    s2 = -s2 / (float)a.width;
+    s1 *= -a.inv_width * r;
+    s2 *= -a.inv_width * r;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int c = ((e * wpr + at) * 32 + lane) * 8, n = in ? max(0, min(8, a.width - c)) : 0;
+      const int k = in ? n[e] : 0;
+      if (VEC && !k) continue;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        g[e].v[i] = __fmul2_rn(__ffma2_rn(h[e].v[i], both(s2), __fadd2_rn(g[e].v[i], both(s1))), both(r));
+        g[e].v[i] = __ffma2_rn(h[e].v[i], both(s2), __ffma2_rn(g[e].v[i], both(r), both(s1)));
       if (a.ds) {
         const F8 d = widen8(s[e]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) g[e].v[i] = __fadd2_rn(g[e].v[i], d.v[i]);
       }
-      store8<T, VEC>(reinterpret_cast<T*>(a.y) + row * a.width + c, n, g[e], turn);
+      store8<T, VEC>(yp + 256 * e, k, g[e], turn);
     }
+    yp += step * a.width;
   }
   if (!a.dw && !a.db) return;
   // warps that hold the same columns, in the order of their rows
@@ -314,7 +388,7 @@ __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs 
       for (int i = 0; i < 8; ++i) join[warp][lane * 9 + i] = k ? db[e].at(i) : dw[e].at(i);
       __syncthreads();
       for (int j = threadIdx.x; j < wpr * 256; j += NT) {
-        const int w0 = j / 256, l = j % 256, col = (e * wpr + w0) * 256 + l;
+        const int w0 = j / 256, l = j % 256, col = (w0 * E + e) * 256 + l;
         float t = 0.f;
         for (int q = 0; q < rpb; ++q) t += join[q * wpr + w0][l / 8 * 9 + l % 8];
         if (col < a.width) a.part[((long long)blockIdx.x * 2 + k) * a.width + col] = t;
@@ -601,33 +675,37 @@ static NormArgs norm_args(const fa_norm& p) {
   a.width = p.width;
   a.groups = (int)groups8(p.width);
   a.eps = (float)p.eps;
+  a.inv_width = 1.f / (float)p.width;
   return a;
 }
 
 template <typename T, int E>
-static void norm_launch(const NormArgs& a, int wpr, bool vec, cudaStream_t st) {
+static void norm_launch(const NormArgs& a, int wpr, bool vec, int device, cudaStream_t st) {
   const int rpb = wpr == 1 ? 4 : 1;
-  const unsigned grid = (unsigned)((a.rows + rpb - 1) / rpb);
   const unsigned threads = 32 * wpr * rpb;
-  if (E == 4 && threads > 512) {
+  // Forward, a block has one row of its own: blocks that stayed and took rows in turn,
+  // two a multiprocessor's worth of warps, took 342 us where these take 272 (65280 x
+  // 4096 bfloat16), since all of a block's warps load, sum and store at the same time.
+  const unsigned grid = (unsigned)std::min((a.rows + rpb - 1) / rpb, 0x7fffffffll);
+  if (threads > 256) {
     if (vec)
-      norm_kernel<T, true, 4, 1024><<<grid, threads, 0, st>>>(a, wpr);
+      norm_kernel<T, true, E, 1024><<<grid, threads, 0, st>>>(a, wpr);
     else
-      norm_kernel<T, false, 4, 1024><<<grid, threads, 0, st>>>(a, wpr);
+      norm_kernel<T, false, E, 1024><<<grid, threads, 0, st>>>(a, wpr);
   } else if (vec) {
-    norm_kernel<T, true, E, 512><<<grid, threads, 0, st>>>(a, wpr);
+    norm_kernel<T, true, E, 256><<<grid, threads, 0, st>>>(a, wpr);
   } else {
-    norm_kernel<T, false, E, 512><<<grid, threads, 0, st>>>(a, wpr);
+    norm_kernel<T, false, E, 256><<<grid, threads, 0, st>>>(a, wpr);
   }
 }
 
 template <typename T>
 static int norm_run(const NormArgs& a, bool vec, int device, cudaStream_t st) {
   const RowShape shape = forward_shape(a.width);
-  if (shape.wpr && a.rows < 1ll << 31) {
-    if (shape.e == 1) norm_launch<T, 1>(a, shape.wpr, vec, st);
-    else if (shape.e == 2) norm_launch<T, 2>(a, shape.wpr, vec, st);
-    else norm_launch<T, 4>(a, shape.wpr, vec, st);
+  if (shape.wpr) {
+    if (shape.e == 1) norm_launch<T, 1>(a, shape.wpr, vec, device, st);
+    else if (shape.e == 2) norm_launch<T, 2>(a, shape.wpr, vec, device, st);
+    else norm_launch<T, 4>(a, shape.wpr, vec, device, st);
     FAB_LAUNCH_CHECK();
     return FA_OK;
   }
