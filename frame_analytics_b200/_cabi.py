@@ -128,6 +128,23 @@ class fa_norm(ctypes.Structure):
     ]
 
 
+class fa_linear8(ctypes.Structure):
+    """Mirror of ``struct fa_linear8`` in include/fa_b200.h."""
+
+    _fields_ = [
+        *[(name, ctypes.c_int32) for name in ("dtype", "inputs", "outputs", "pad_")],
+        ("rows", ctypes.c_int64),
+        ("x", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64),
+        ("dy", ctypes.c_void_p),
+        ("dy_stride", ctypes.c_int64),
+        ("weight", ctypes.c_void_p),
+        ("weight_stride", ctypes.c_int64),
+        *[(name, ctypes.c_void_p) for name in
+          ("bias", "codes", "ranges", "y", "dx", "dweight", "dbias")],
+    ]
+
+
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
@@ -217,9 +234,9 @@ PROTOTYPES = {
     "fa_b200_layer_norm": [_vp, _vp, _vp, _i, _vp],
     "fa_b200_layer_norm_backward_workspace_bytes": [_i64, _i, _i, _vp],
     "fa_b200_layer_norm_backward": [_vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _sz, _i, _vp],
-    "fa_b200_linear8_weight_grad_workspace_bytes": [_i64, _i, _i, _i, _i, _vp],
-    "fa_b200_linear8_weight_grad": [_vp, _i64, _vp, _vp, _i, _i64, _i, _i, _vp, _vp, _vp, _sz,
-                                    _i, _vp],
+    "fa_b200_linear8_workspace_bytes": [_vp, _i, _vp],
+    "fa_b200_linear8": [_vp, _vp, _sz, _i, _vp],
+    "fa_b200_linear8_backward": [_vp, _vp, _sz, _i, _vp],
     "fa_b200_ssim_gmsd": [_pview, _pview, _vp, _i, _d, _d, _d, _d, _d, _d, _vp, _sz,
                           _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp],
 }

@@ -30,6 +30,8 @@ _MAX_WIDTH = 1 << 24
 _MAX_SIDE, _MAX_ROWS = (1 << 22) - 64, 1 << 27  # of a product
 # struct fa_norm of include/fa_b200.h as bytes
 _NORM = struct.Struct("@2iq2idPqPq5P").pack
+# struct fa_linear8
+_LINEAR = struct.Struct("@4iqPqPqPq7P").pack
 
 
 class Packed8(NamedTuple):
@@ -368,31 +370,59 @@ def gelu8(x: torch.Tensor, *, approximate: str = "none") -> torch.Tensor:
 # products
 # --------------------------------------------------------------------------- #
 
-def _weight_grad(g, codes, ranges, inputs: int, need_weight: bool, need_bias: bool):
-    """``g``: rows of the gradient; ``codes`` and ``ranges``: addresses."""
-    rows, outputs = g.shape
-    code = backend.DTYPE_CODE[g.dtype]
-    dw = torch.empty((outputs, inputs), dtype=g.dtype, device=g.device) if need_weight else None
-    db = torch.empty(outputs, dtype=g.dtype, device=g.device) if need_bias else None
-    L = backend.lib()
-    size = backend._cached_ws("wgrad8", L.fa_b200_linear8_weight_grad_workspace_bytes, rows,
-                              inputs, outputs, code, backend._dev(g))
-    ws = torch.empty(size, dtype=torch.uint8, device=g.device)
-    backend._call(g, L.fa_b200_linear8_weight_grad, g.data_ptr(), g.stride(0), codes, ranges, code,
-                  rows, inputs, outputs, backend._ptr(dw), backend._ptr(db), ws.data_ptr(), size,
-                  backend._dev(g), backend._stream(g))
-    return dw, db
+_linear_ws: dict = {}
+
+
+def _linear_call(fn, t: torch.Tensor, rows: int, inputs: int, outputs: int, x, dy, weight, bias,
+                 codes: int, ranges: int, y, dx, dw, db) -> None:
+    """One of the two entries on `t`'s device; `x` and `dy` are rows, all but the
+    addresses `codes` and `ranges` tensors or None."""
+    at = [0 if v is None else v.data_ptr() for v in (x, dy, weight, bias, y, dx, dw, db)]
+    p = _LINEAR(backend.DTYPE_CODE[t.dtype], inputs, outputs, 0, rows,
+                at[0], 0 if x is None else x.stride(0), at[1], 0 if dy is None else dy.stride(0),
+                at[2], 0 if weight is None else weight.stride(0), at[3], codes, ranges, *at[4:])
+    device = backend._dev(t)
+    # what the size depends on: the sizes, which results, and which operands are copied
+    key = (p[:24], device, *[bool(v) for v in at[4:]], at[0] % 16, at[1] % 16, at[2] % 16,
+           *[v is not None and v.stride(0) for v in (x, dy, weight)])
+    size = _linear_ws.get(key)
+    if size is None:
+        size = backend._ws_query(backend.lib().fa_b200_linear8_workspace_bytes, p, device)
+        if len(_linear_ws) > 4096:
+            _linear_ws.clear()
+        _linear_ws[key] = size
+    ws = torch.empty(size, dtype=torch.uint8, device=t.device) if size else None
+    backend._call(t, fn, p, backend._ptr(ws), size, device, backend._stream(t))
+
+
+def _linear_forward(x, weight, bias, kept, ranges: int) -> torch.Tensor:
+    """The product, and x packed into `kept` where that is given."""
+    r = _rows(x)
+    rows, inputs = r.shape
+    outputs = weight.shape[0]
+    fn = backend.lib().fa_b200_linear8
+    at = 0 if kept is None else kept.data_ptr()
+    if x.dtype == torch.float32:
+        if kept is not None:
+            _pack_into(r, at, at + ranges)
+        return F.linear(x, weight, bias)
+    if weight.stride(1) != 1 and inputs > 1:
+        weight = weight.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    y = torch.empty((*x.shape[:-1], outputs), dtype=x.dtype, device=x.device)
+    _linear_call(fn, r, rows, inputs, outputs, r, None, weight, bias, at,
+                 at + ranges if at else 0, y, None, None, None)
+    return y
 
 
 class _Linear8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
-        y = F.linear(x, weight, bias)
         kept, ctx.ranges = None, 0
         if ctx.needs_input_grad[1]:
             kept, ctx.ranges, _ = _kept_like(x, x.numel() // x.shape[-1], False)
-            at = kept.data_ptr()
-            _pack_into(x, at, at + ctx.ranges)
+        y = _linear_forward(x, weight, bias, kept, ctx.ranges)
         ctx.save_for_backward(kept, weight)
         return y
 
@@ -400,36 +430,44 @@ class _Linear8(torch.autograd.Function):
     def backward(ctx, gy):
         _reject_double_backward()
         kept, weight = ctx.saved_tensors
-        need, inputs = ctx.needs_input_grad, weight.shape[1]
+        need, (outputs, inputs) = ctx.needs_input_grad, weight.shape
         g = _rows(gy)
         dx = dw = db = None
+        own = gy.dtype != torch.float32
         if need[0]:
-            if torch.is_autocast_enabled("cuda"):
-                with torch.autocast("cuda", enabled=False):
-                    dx = torch.matmul(g, weight)
+            if own:
+                dx = torch.empty((*gy.shape[:-1], inputs), dtype=gy.dtype, device=gy.device)
+                if weight.stride(1) != 1 and inputs > 1:
+                    weight = weight.contiguous()
             else:
-                dx = torch.matmul(g, weight)
-            if gy.dim() != 2:
-                dx = dx.view(*gy.shape[:-1], inputs)
-        if need[1] or need[2]:
-            at = 0 if kept is None else kept.data_ptr()
-            dw, db = _weight_grad(g, at, at + ctx.ranges, inputs, need[1], need[2])
+                with torch.autocast("cuda", enabled=False):
+                    dx = torch.matmul(g, weight).view(*gy.shape[:-1], inputs)
+        if need[1]:
+            dw = torch.empty((outputs, inputs), dtype=gy.dtype, device=gy.device)
+        if need[2]:
+            db = torch.empty(outputs, dtype=gy.dtype, device=gy.device)
+        if need[1] or need[2] or own:
+            at = 0 if kept is None or not need[1] else kept.data_ptr()
+            _linear_call(backend.lib().fa_b200_linear8_backward, g, g.shape[0], inputs, outputs,
+                         None, g, weight if own and need[0] else None, None, at,
+                         at + ctx.ranges if at else 0, None, dx if own else None, dw, db)
         return dx, dw, db
 
 
 def linear8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None
             ) -> torch.Tensor:
     """``x W^T + bias`` that keeps ``x`` for the backward pass as :func:`pack8`
-    holds it: the weight's gradient ``dy^T x`` is a product of this package's own
-    that takes ``x`` from the 8-bit form inside (float16 and bfloat16 on the
-    tensor cores); the bias's gradient comes with it.  The value and the gradient
-    of ``x`` are torch's products of the operands themselves.  Differentiable
-    once, in reverse mode.
+    holds it: the weight's gradient ``dy^T x`` takes ``x`` from the 8-bit form.
+    Differentiable once, in reverse mode.
 
     ``x`` (..., K), ``weight`` (M, K), ``bias`` (M,): one dtype, float16, bfloat16
     or float32 (under autocast its dtype), any strides; K and M at most 4194240, and
-    2^27 rows.
-    ``x`` is packed only where the weight wants a gradient."""
+    2^27 rows.  ``x`` is packed only where the weight wants a gradient.
+
+    float16 and bfloat16 run on the tensor cores with float32 sums that are rounded
+    once, however an axis is split.  In float32 the value and the gradient of ``x``
+    are torch's products, and the weight's gradient is summed in float32 without
+    tensor cores."""
     if torch.is_autocast_enabled("cuda"):
         to = torch.get_autocast_dtype("cuda")
         if to in _DTYPES:
@@ -451,7 +489,9 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] 
                          f"{tuple(bias.shape)}")
     _reject_tangents("linear8", x, weight, bias)
     _on_one_device(x, weight, bias)
-    if x.numel() == 0 or not torch.is_grad_enabled() or not (
-            weight.requires_grad or x.requires_grad or bias is not None and bias.requires_grad):
+    if x.numel() == 0:
         return F.linear(x, weight, bias)
-    return _Linear8.apply(x, weight, bias)
+    if torch.is_grad_enabled() and (
+            weight.requires_grad or x.requires_grad or bias is not None and bias.requires_grad):
+        return _Linear8.apply(x, weight, bias)
+    return _linear_forward(x, weight, bias, None, 0)

@@ -30,10 +30,10 @@ int norm_impl(const fa_norm* p, void* y, void* sum, int device, cudaStream_t st)
 int norm_backward_impl(const fa_norm* p, const void* dy, long long dy_row, const void* ds,
                        long long ds_row, void* dx, void* dw, void* db, void* ws, size_t ws_bytes,
                        int device, cudaStream_t st);
-size_t wgrad8_ws_bytes(long long rows, int inputs, int outputs, int dtype, int device);
-int wgrad8_impl(const void* dy, long long dy_row, const void* codes, const void* ranges, int dtype,
-                long long rows, int inputs, int outputs, void* dw, void* db, void* ws,
-                size_t ws_bytes, int device, cudaStream_t st);
+int linear8_ws_bytes(const fa_linear8* l, int device, size_t* out);
+int linear8_impl(const fa_linear8* l, void* ws, size_t bytes, int device, cudaStream_t st);
+int linear8_backward_impl(const fa_linear8* l, void* ws, size_t bytes, int device,
+                          cudaStream_t st);
 
 }  // namespace fab
 
@@ -161,24 +161,24 @@ FA_B200_API int fa_b200_layer_norm_backward(const fa_norm* params, const void* d
                             workspace_bytes, device, static_cast<cudaStream_t>(stream));
 }
 
-FA_B200_API int fa_b200_linear8_weight_grad_workspace_bytes(int64_t rows, int inputs, int outputs,
-                                                            int dtype, int device,
-                                                            size_t* out_bytes) {
+FA_B200_API int fa_b200_linear8_workspace_bytes(const fa_linear8* params, int device,
+                                                size_t* out_bytes) {
   if (!out_bytes) return FA_E_ARG;
-  if (dtype != FA_F16 && dtype != FA_BF16 && dtype != FA_F32) return FA_E_DTYPE;
-  if (rows <= 0 || inputs <= 0 || outputs <= 0) return FA_E_SHAPE;
-  *out_bytes = wgrad8_ws_bytes(rows, inputs, outputs, dtype, device);
-  return FA_OK;
+  return linear8_ws_bytes(params, device, out_bytes);
 }
 
-FA_B200_API int fa_b200_linear8_weight_grad(const void* dy, int64_t dy_stride, const void* codes,
-                                            const void* ranges, int dtype, int64_t rows,
-                                            int inputs, int outputs, void* dweight, void* dbias,
-                                            void* workspace, size_t workspace_bytes, int device,
-                                            void* stream) {
+FA_B200_API int fa_b200_linear8(const fa_linear8* params, void* workspace, size_t workspace_bytes,
+                                int device, void* stream) {
   FAB_PENDING();
-  return wgrad8_impl(dy, dy_stride, codes, ranges, dtype, rows, inputs, outputs, dweight, dbias,
-                     workspace, workspace_bytes, device, static_cast<cudaStream_t>(stream));
+  return linear8_impl(params, workspace, workspace_bytes, device,
+                      static_cast<cudaStream_t>(stream));
+}
+
+FA_B200_API int fa_b200_linear8_backward(const fa_linear8* params, void* workspace,
+                                         size_t workspace_bytes, int device, void* stream) {
+  FAB_PENDING();
+  return linear8_backward_impl(params, workspace, workspace_bytes, device,
+                               static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

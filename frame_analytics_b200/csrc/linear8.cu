@@ -1,8 +1,10 @@
-// Weight gradient of a product y = x W^T from the packed copy of x (keep8.cuh):
+// A product that keeps its operand packed (keep8.cuh):
+//   y = x W^T + b,   dx = dy W,
 //   dW[m, k] = sum over rows t of dy[t, m] x^[t, k],   db[m] = sum over t of dy[t, m],
-// where x^ are the values that the codes stand for.
+// where x^ are the values that the codes stand for.  All sums are float32 and rounded
+// once, also where an axis is cut into parts.
 //
-// 16-bit types: tensor-core products of 256 inputs x 256 outputs over pairs of blocks
+// dW in 16-bit types: tensor-core products of 256 inputs x 256 outputs over pairs of blocks
 // (tcgen05, cta_group::2), persistent.  dy arrives by TMA as it lies (its rows are the
 // sum's axis: MN-major) and is the products' second operand in shared memory.  The
 // codes arrive by TMA as bytes; eight warps turn them, transposed on the way out of
@@ -24,6 +26,8 @@ namespace fab {
 int bias_grad_impl(const void* g, long long g_row, void* db, int dtype, long long rows, int width,
                    void* ws, size_t ws_bytes, int device, cudaStream_t st);
 size_t norm_ws_bytes(long long rows, int width, int device);
+int pack8_impl(const void* x, long long x_row, void* codes, void* ranges, int dtype,
+               long long rows, int width, int device, cudaStream_t st);
 
 struct WgradArgs {
   const void* dy;
@@ -130,7 +134,8 @@ struct Work {
 };
 // Items are numbered part by part; inside a part eight rows of tiles are walked
 // column by column, so the tiles at work share operand panels in the L2 cache.
-__device__ __forceinline__ bool work_of(const ProductArgs& a, int item, Work* w) {
+template <typename Args>
+__device__ __forceinline__ bool work_of(const Args& a, int item, Work* w) {
   const int tiles = a.tiles_m * a.tiles_n;
   if (item >= tiles * a.parts) return false;
   const int part = item / tiles, tile = item - part * tiles;
@@ -556,6 +561,254 @@ __global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__
     if (j + q < a.n) out[(long long)q * a.m] = St<T>::v(v[q]);
 }
 
+// ---------------------------------------------------------------------------
+// y = x W^T + bias and dx = dy W, 16-bit types
+// ---------------------------------------------------------------------------
+
+// D[m][n] = sum over k of A[m][k] B[n][k] (+ bias[n]): A with k along its rows, B so or
+// with k as its rows (b_mn).  The same tiles of a pair of blocks; both operands by TMA,
+// two accumulators in turn, eight warps that write the one while the other is summed.
+constexpr int kPlainStages = 6;
+constexpr int kPlainThreads = 128 + 32 * kWriters;
+constexpr int kTurn = 2048;     // bytes of 32 x 32 of the result; two a warp
+constexpr int kTurnAt = kPlainStages * 2 * kHalf;
+constexpr int kPlainSmem = kTurnAt + kWriters * 2 * kTurn + 1024;
+
+struct PlainArgs {
+  CUtensorMap a, b, d;
+  int m, n, kb;                 // kb: stages of the whole sum
+  int b_mn;
+  int tiles_m, tiles_n, parts;
+  void* out;                    // [m][n]
+  const void* bias;             // [n] or null
+  int tma_out, bias_vec;
+  float* part;
+  unsigned* err;
+};
+
+// A warp's 32 rows x 32 columns of the result at (i, j), a row a lane.
+template <typename T>
+__device__ __forceinline__ void add_bias(const PlainArgs& a, int j, float (&v)[32]) {
+  if (!a.bias) return;
+  const T* b = reinterpret_cast<const T*>(a.bias) + j;
+  if (a.bias_vec && j + 32 <= a.n) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const F8 x = widen8(get8<T>(b + 8 * q));
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[8 * q + c] += x.at(c);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 32; ++c)
+      if (j + c < a.n) v[c] += Ld<T>::f(ldro(b + c));
+  }
+}
+// `turn` is 2 KB of shared memory of the warp's own: rows of 64 bytes in the 64-byte
+// swizzle, whose copy to memory is under way when this returns.
+template <typename T>
+__device__ __forceinline__ void put_result(const PlainArgs& a, int i, int j, const float (&v)[32],
+                                           char* turn) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<uint4*>(turn + lane * 64 + ((q ^ (lane >> 1)) & 3) * 16) = make_uint4(
+        narrow2(make_float2(v[8 * q], v[8 * q + 1]), T()),
+        narrow2(make_float2(v[8 * q + 2], v[8 * q + 3]), T()),
+        narrow2(make_float2(v[8 * q + 4], v[8 * q + 5]), T()),
+        narrow2(make_float2(v[8 * q + 6], v[8 * q + 7]), T()));
+  if (a.tma_out) {
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0)
+      asm volatile(
+          "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n"
+          "cp.async.bulk.commit_group;\n" ::"l"(reinterpret_cast<unsigned long long>(&a.d)),
+          "r"(j), "r"(i), "r"(0), "r"(smem_u32(turn))
+          : "memory");
+  } else {
+    __syncwarp();
+    T* const out = reinterpret_cast<T*>(a.out) + (long long)i * a.n + j + lane;
+    if (j + lane < a.n)
+      for (int r = 0; r < min(32, a.m - i); ++r)
+        out[(long long)r * a.n] = *reinterpret_cast<const T*>(
+            turn + r * 64 + (((lane >> 3) ^ (r >> 1)) & 3) * 16 + (lane & 7) * 2);
+    __syncwarp();
+  }
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
+    product_kernel(const __grid_constant__ PlainArgs a) {
+  constexpr int S = kPlainStages;
+  extern __shared__ char smem_raw[];
+  const unsigned smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  char* const smem = smem_raw + (smem0 - smem_u32(smem_raw));
+  __shared__ unsigned long long full[S], empty[S], tm_full[2], tm_empty[2], drain;
+  __shared__ unsigned tmem_base;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.x & 1;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tm_full[i], 1);
+      mbar_init(&tm_empty[i], 2 * kWriters);
+    }
+    mbar_init(&drain, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    fence_async_smem();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(
+                     smem_u32(&tmem_base))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  cluster_sync();
+  asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+  const unsigned tmem = tmem_base;
+  Work t;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      unsigned n = 0;
+      for (int item = first; work_of(a, item, &t); item += step) {
+        const int ia = t.i0 + rank * 128, jb = t.j0 + rank * 128;
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
+          const int s = n % S;
+          if (n >= (unsigned)S) stage_wait(&empty[s], (n / S - 1) & 1, a.err);
+          // both blocks' copies count on the first block's barrier
+          const unsigned bar = in_leader(smem_u32(&full[s])), to = smem0 + s * 2 * kHalf;
+          if (rank == 0) mbar_expect_tx(&full[s], 4 * kHalf);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            tma_box<true>(to + i * kBox, &a.a, kb * kDepth, ia + 64 * i, 0, bar);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            tma_box<true>(to + kHalf + i * kBox, &a.b, a.b_mn ? jb + 64 * i : kb * kDepth,
+                          a.b_mn ? kb * kDepth : jb + 64 * i, 0, bar);
+        }
+      }
+      // copies still in flight land before the block ends
+      for (unsigned i = n > (unsigned)S ? n - S : 0; rank == 0 && i < n; ++i)
+        stage_wait(&full[i % S], (i / S) & 1, a.err);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      // float32 sums; both operands float16 or both bfloat16; 256 x 256 over the pair
+      const unsigned kind = std::is_same<T, bf16_t>::value ? (1u << 7) | (1u << 10) : 0u;
+      const unsigned idesc = (1u << 4) | kind | ((unsigned)a.b_mn << 16) |
+                             ((unsigned)(kTile / 8) << 17) | ((unsigned)(kTile / 16) << 24);
+      // 16 of k further: 32 bytes along a row, or 2 groups of 8 rows
+      const unsigned bs = (a.b_mn ? 2048u : 32u) >> 4;
+      unsigned n = 0, tile = 0;
+      for (int item = first; work_of(a, item, &t); item += step, ++tile) {
+        const unsigned d = tmem + (tile & 1) * 256;
+        if (tile >= 2) wait_pair(&tm_empty[tile & 1], (tile / 2 - 1) & 1, a.err);
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        bool ready = false;
+        for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
+          const int s = n % S;
+          if (!ready) stage_wait(&full[s], (n / S) & 1, a.err);
+          asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+          const unsigned long long p = operand(smem0 + s * 2 * kHalf),
+                                   q = operand(smem0 + s * 2 * kHalf + kHalf);
+#pragma unroll
+          for (int k = 0; k < kDepth / 16; ++k) {
+            mma_f16<true>(d, p + k * (32u >> 4), q + k * bs, idesc, kb > t.kb0 || k > 0);
+            if (k == 1) ready = kb + 1 < t.kb1 && mbar_peek(&full[(n + 1) % S], ((n + 1) / S) & 1);
+          }
+          mma_commit<true>(&empty[s]);
+        }
+        mma_commit<true>(&tm_full[tile & 1]);
+      }
+      // products still in flight end before tensor memory is given back
+      mma_commit<true>(&drain);
+      stage_wait(&drain, 0, a.err);
+    }
+  } else if (warp >= 4) {
+    const int w = warp & 3, h = (warp - 4) >> 2;
+    char* const turn = smem + kTurnAt + (warp - 4) * 2 * kTurn;
+    unsigned tile = 0;
+    int other = 0;
+    for (int item = first; work_of(a, item, &t); item += step, ++tile) {
+      const int buf = tile & 1;
+      if (lane == 0) wait_pair(&tm_full[buf], (tile / 2) & 1, a.err);
+      __syncwarp();
+      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+      const int i = t.i0 + rank * 128 + 32 * w;
+#pragma unroll 1
+      for (int c = h * 128; c < h * 128 + 128; c += 32) {
+        float v[32];
+        tmem_load32(tmem + buf * 256 + c + ((unsigned)(32 * w) << 16), v);
+        if (c + 32 == h * 128 + 128) {
+          __syncwarp();
+          asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+          if (lane == 0) arrive_leader<true>(&tm_empty[buf]);
+        }
+        if (a.parts > 1) {  // [item][block][columns / 4][128 rows] of four columns each
+          float4* const to = reinterpret_cast<float4*>(
+              a.part + ((long long)t.item * 2 + rank) * kPartFloats) + c / 4 * 128 + 32 * w + lane;
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            to[q * 128] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        } else if (i < a.m && t.j0 + c < a.n) {
+          add_bias<T>(a, t.j0 + c, v);
+          // the copy before the last has been read out of this half
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");
+          __syncwarp();
+          put_result<T>(a, i, t.j0 + c, v, turn + other * kTurn);
+          other ^= 1;
+        }
+      }
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+  __syncthreads();
+  cluster_sync();  // neither block's memory is in use any more
+  if (rank == 1 && threadIdx.x == 32) stage_wait(&drain, 0, a.err);  // as in wgrad_kernel
+  if (warp == 2) {
+    asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
+  }
+}
+
+// The parts of a tile added in order: a thread has 16 columns of a row.
+template <typename T>
+__global__ void __launch_bounds__(128) join_rows_kernel(const __grid_constant__ PlainArgs a) {
+  const int tiles = a.tiles_m * a.tiles_n;
+  const int tile = blockIdx.x >> 5, rank = (blockIdx.x >> 4) & 1, c = (blockIdx.x & 15) * 16;
+  Work t;
+  work_of(a, tile, &t);
+  const int i = t.i0 + rank * 128 + threadIdx.x, j = t.j0 + c;
+  if (i >= a.m || j >= a.n) return;
+  float v[16] = {};
+  for (int p = 0; p < a.parts; ++p) {
+    const float4* const from = reinterpret_cast<const float4*>(
+        a.part + ((long long)(p * tiles + tile) * 2 + rank) * kPartFloats) + c / 4 * 128 + threadIdx.x;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 f = from[q * 128];
+      v[4 * q] += f.x;
+      v[4 * q + 1] += f.y;
+      v[4 * q + 2] += f.z;
+      v[4 * q + 3] += f.w;
+    }
+  }
+  const T* const b = reinterpret_cast<const T*>(a.bias);
+  T* const out = reinterpret_cast<T*>(a.out) + (long long)i * a.n + j;
+#pragma unroll
+  for (int q = 0; q < 16; ++q)
+    if (j + q < a.n) out[q] = St<T>::v(b ? v[q] + Ld<T>::f(ldro(b + j + q)) : v[q]);
+}
+
 // Rows at a pitch of whole 16 bytes, for TMA.
 template <typename T>
 __global__ void __launch_bounds__(256) pitch_kernel(const T* x, long long x_row, T* y, int pitch,
@@ -580,19 +833,23 @@ constexpr int kMaxSide = (1 << 22) - 64;  // 65535 tiles of 64
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// [rows][pitch bytes] of 16-bit values in boxes of 64 x 64, or of bytes in boxes of
-// 128 x 64, in the 128-byte swizzle.  Outside arrives as zeros.
+// [rows][pitch bytes] of 16-bit values in boxes of 64 x 64 in the 128-byte swizzle.
+// Outside arrives as zeros.  BYTES: boxes of 128 bytes; RESULT: of 32 x 32 in the
+// 64-byte swizzle.
+enum BoxKind { BOX, BYTES, RESULT };
 static bool box_map(CUtensorMap* map, const void* p, long long rows, long long cols,
-                    long long pitch, bool bytes) {
+                    long long pitch, BoxKind kind) {
   EncodeTiledFn fn = encode_tiled();
   if (!fn) return false;
   const cuuint64_t dim[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1};
   const cuuint64_t stride[2] = {(cuuint64_t)pitch, (cuuint64_t)(pitch * rows)};
-  const cuuint32_t box[3] = {bytes ? 128u : 64u, (cuuint32_t)kDepth, 1}, one[3] = {1, 1, 1};
-  return fn(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3,
+  const cuuint32_t one[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {kind == BOX ? 64u : kind == BYTES ? 128u : 32u,
+                             kind == RESULT ? 32u : 64u, 1};
+  return fn(map, kind == BYTES ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3,
             const_cast<void*>(p), dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            kind == RESULT ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 static int tiles_of(long long n) { return (int)((n + kTile - 1) / kTile); }
@@ -642,62 +899,156 @@ static int resident_pairs(int device) {
   return n;
 }
 
-// What one call of the weight gradient takes from its workspace.
-struct WgradPlan {
-  int pitch;                    // of the copy of dy, in values (0: no copy)
-  int parts, pairs;
-  size_t copy, part, bytes;     // offsets and size
+// A matrix of 16-bit values as an operand: TMA reads rows at a pitch of whole 16 bytes
+// that do not overlap; others are copied to such rows first.
+struct Operand {
+  const void* p;
+  long long rows, stride;
+  int cols;
+  size_t copy;                  // its place in the workspace
+  bool copied;
 };
-static WgradPlan wgrad_plan(long long rows, int inputs, int outputs, int dtype, int device) {
-  WgradPlan p = {};
-  p.bytes = up256(norm_ws_bytes(rows, outputs, device));
-  if (dtype == FA_F32) return p;
-  p.copy = p.bytes;
-  p.pitch = (outputs + 7) / 8 * 8;
-  p.bytes += up256((size_t)rows * p.pitch * 2);
-  const int tiles = tiles_of(inputs) * tiles_of(outputs);
-  p.pairs = resident_pairs(device);
-  p.parts = parts_of(tiles, (int)((rows + kDepth - 1) / kDepth), p.pairs);
-  p.part = p.bytes;
-  if (p.parts > 1) p.bytes += (size_t)tiles * p.parts * 2 * kPartFloats * sizeof(float);
+static int pitch_of(int cols) { return (cols + 7) / 8 * 8; }
+static Operand operand_of(const void* p, long long rows, int cols, long long stride, size_t* used) {
+  Operand o = {p, rows, rows == 1 ? pitch_of(cols) : stride, cols, *used, false};
+  o.copied = p && (reinterpret_cast<size_t>(p) % 16 ||
+                   (rows > 1 && (stride % 8 || stride < cols)));
+  if (o.copied) *used += up256((size_t)rows * pitch_of(cols) * 2);
+  return o;
+}
+template <typename T>
+static int ready_operand(Operand* o, char* ws, long long stride, int device, cudaStream_t st) {
+  if (!o->copied) return FA_OK;
+  const int pitch = pitch_of(o->cols);
+  T* const copy = reinterpret_cast<T*>(ws + o->copy);
+  const long long blocks =
+      std::min((o->rows * pitch + 255) / 256, (long long)sm_count(device) * 16);
+  pitch_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(static_cast<const T*>(o->p), stride, copy,
+                                                    pitch, o->rows, o->cols);
+  FAB_LAUNCH_CHECK();
+  o->p = copy;
+  o->stride = pitch;
+  o->copied = false;
+  return FA_OK;
+}
+
+// What a call takes from its workspace: sums of columns, operands' copies, and the parts
+// of one product after the other.
+struct LinearPlan {
+  Operand x, dy, w;
+  int y_parts, dx_parts, dw_parts, pairs;
+  size_t part, bytes;
+};
+static int stages_of(long long n) { return (int)((n + kDepth - 1) / kDepth); }
+static LinearPlan linear_plan(const fa_linear8& l, int device) {
+  LinearPlan p = {};
+  size_t used = l.dbias ? up256(norm_ws_bytes(l.rows, l.outputs, device)) : 0, part = 0;
+  if (l.dtype != FA_F32) {
+    if (l.y) p.x = operand_of(l.x, l.rows, l.inputs, l.x_stride, &used);
+    if (l.dx || l.dweight) p.dy = operand_of(l.dy, l.rows, l.outputs, l.dy_stride, &used);
+    if (l.y || l.dx) p.w = operand_of(l.weight, l.outputs, l.inputs, l.weight_stride, &used);
+    p.pairs = resident_pairs(device);
+    const int in = tiles_of(l.inputs), out = tiles_of(l.outputs);
+    const long long rows = tiles_of(l.rows);
+    const auto parts = [&](bool wanted, long long tiles, int kb) {
+      if (!wanted || tiles > p.pairs) return 1;
+      const int n = parts_of((int)tiles, kb, p.pairs);
+      if (n > 1) part = std::max(part, (size_t)tiles * n * 2 * kPartFloats * sizeof(float));
+      return n;
+    };
+    p.y_parts = parts(l.y, rows * out, stages_of(l.inputs));
+    p.dx_parts = parts(l.dx, rows * in, stages_of(l.outputs));
+    p.dw_parts = parts(l.dweight, (long long)in * out, stages_of(l.rows));
+  }
+  p.part = used;
+  p.bytes = used + part;
   return p;
 }
 
-size_t wgrad8_ws_bytes(long long rows, int inputs, int outputs, int dtype, int device) {
-  return wgrad_plan(rows, inputs, outputs, dtype, device).bytes;
+static int linear_check(const fa_linear8* l) {
+  if (!l) return FA_E_ARG;
+  if (!train_dtype(l->dtype)) return FA_E_DTYPE;
+  if (l->rows <= 0 || l->inputs <= 0 || l->outputs <= 0 || l->rows > kMaxRows ||
+      l->inputs > kMaxSide || l->outputs > kMaxSide)
+    return FA_E_SHAPE;
+  if (l->dtype == FA_F32 && (l->y || l->dx)) return FA_E_DTYPE;
+  const int item = item_size(l->dtype);
+  for (const void* q : {l->x, l->dy, l->weight, l->bias, (const void*)l->y, (const void*)l->dx,
+                        (const void*)l->dweight, (const void*)l->dbias})
+    if (reinterpret_cast<size_t>(q) % item) return FA_E_ARG;
+  if (!l->codes != !l->ranges || reinterpret_cast<size_t>(l->codes) % 16 ||
+      reinterpret_cast<size_t>(l->ranges) % 8)
+    return FA_E_ARG;
+  if ((l->y && (!l->x || !l->weight)) || (l->dx && (!l->dy || !l->weight)) ||
+      (l->dweight && (!l->dy || !l->codes)) || (l->dbias && !l->dy))
+    return FA_E_ARG;
+  return FA_OK;
+}
+
+int linear8_ws_bytes(const fa_linear8* l, int device, size_t* out) {
+  if (const int rc = linear_check(l)) return rc;
+  *out = linear_plan(*l, device).bytes;
+  return FA_OK;
+}
+
+static int workspace_check(const LinearPlan& p, const void* ws, size_t bytes) {
+  return p.bytes && (!ws || reinterpret_cast<size_t>(ws) % 256 || bytes < p.bytes) ? FA_E_ARG : FA_OK;
+}
+
+// D (rows x cols) = A (rows x depth) B: B with depth along its rows, or as its rows.
+template <typename T>
+static int product_run(const Operand& x, const Operand& w, int depth, bool w_mn, const void* bias,
+                       void* out, long long rows, int cols, int parts, char* part,
+                       const LinearPlan& plan, cudaStream_t st) {
+  PlainArgs a = {};
+  a.tma_out = cols % 8 == 0 && reinterpret_cast<size_t>(out) % 16 == 0;
+  if (!box_map(&a.a, x.p, rows, depth, x.stride * 2, BOX) ||
+      !box_map(&a.b, w.p, w.rows, w.cols, w.stride * 2, BOX) ||
+      (a.tma_out && !box_map(&a.d, out, rows, cols, cols * 2ll, RESULT)))
+    return FA_E_INTERNAL;
+  a.m = (int)rows;
+  a.n = cols;
+  a.kb = stages_of(depth);
+  a.b_mn = w_mn;
+  a.tiles_m = tiles_of(rows);
+  a.tiles_n = tiles_of(cols);
+  a.parts = parts;
+  a.out = out;
+  a.bias = bias;
+  a.bias_vec = reinterpret_cast<size_t>(bias) % 16 == 0;
+  a.part = reinterpret_cast<float*>(part);
+  a.err = wait_error_word();
+  FAB_TRY(cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kPlainSmem));
+  const int items = a.tiles_m * a.tiles_n * parts;
+  product_kernel<T><<<2 * std::min(items, plan.pairs), kPlainThreads, kPlainSmem, st>>>(a);
+  FAB_LAUNCH_CHECK();
+  if (parts > 1) {
+    join_rows_kernel<T><<<(unsigned)(a.tiles_m * a.tiles_n * 32), 128, 0, st>>>(a);
+    FAB_LAUNCH_CHECK();
+  }
+  return FA_OK;
 }
 
 template <typename T>
-static int wgrad_run(const void* dy, long long dy_row, const void* codes, const void* ranges,
-                     long long rows, int inputs, int outputs, void* dw, char* ws,
-                     const WgradPlan& plan, int device, cudaStream_t st) {
-  // TMA reads rows at a pitch of whole 16 bytes that do not overlap
-  if (reinterpret_cast<size_t>(dy) % 16 || (rows > 1 && (dy_row % 8 || dy_row < outputs))) {
-    T* const copy = reinterpret_cast<T*>(ws + plan.copy);
-    const long long blocks = std::min((rows * plan.pitch + 255) / 256, (long long)sm_count(device) * 16);
-    pitch_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(static_cast<const T*>(dy), dy_row, copy,
-                                                      plan.pitch, rows, outputs);
-    FAB_LAUNCH_CHECK();
-    dy = copy;
-    dy_row = plan.pitch;
-  }
-  if (rows == 1) dy_row = plan.pitch;
+static int wgrad_run(const fa_linear8& l, const Operand& dy, char* part, const LinearPlan& plan,
+                     cudaStream_t st) {
   ProductArgs a = {};
-  const long long groups = groups8(inputs);
-  if (!box_map(&a.dy, dy, rows, outputs, dy_row * 2, false) ||
-      !box_map(&a.codes, codes, rows, groups * kGroup8, groups * kGroup8, true))
+  const long long groups = groups8(l.inputs);
+  if (!box_map(&a.dy, dy.p, l.rows, l.outputs, dy.stride * 2, BOX) ||
+      !box_map(&a.codes, l.codes, l.rows, groups * kGroup8, groups * kGroup8, BYTES))
     return FA_E_INTERNAL;
-  a.m = inputs;
-  a.n = outputs;
-  a.kb = (int)((rows + kDepth - 1) / kDepth);
-  a.tiles_m = tiles_of(inputs);
-  a.tiles_n = tiles_of(outputs);
-  a.parts = plan.parts;
-  a.ranges = static_cast<const unsigned*>(ranges);
-  a.rows = rows;
+  a.m = l.inputs;
+  a.n = l.outputs;
+  a.kb = stages_of(l.rows);
+  a.tiles_m = tiles_of(l.inputs);
+  a.tiles_n = tiles_of(l.outputs);
+  a.parts = plan.dw_parts;
+  a.ranges = static_cast<const unsigned*>(l.ranges);
+  a.rows = l.rows;
   a.groups = (int)groups;
-  a.out = dw;
-  a.part = reinterpret_cast<float*>(ws + plan.part);
+  a.out = l.dweight;
+  a.part = reinterpret_cast<float*>(part);
   a.err = wait_error_word();
   FAB_TRY(cudaFuncSetAttribute(wgrad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmem));
   const int items = a.tiles_m * a.tiles_n * a.parts;
@@ -710,44 +1061,65 @@ static int wgrad_run(const void* dy, long long dy_row, const void* codes, const 
   return FA_OK;
 }
 
-int wgrad8_impl(const void* dy, long long dy_row, const void* codes, const void* ranges, int dtype,
-                long long rows, int inputs, int outputs, void* dw, void* db, void* ws,
-                size_t ws_bytes, int device, cudaStream_t st) {
-  if (!train_dtype(dtype)) return FA_E_DTYPE;
-  if (rows <= 0 || inputs <= 0 || outputs <= 0 || rows > kMaxRows || inputs > kMaxSide ||
-      outputs > kMaxSide)
-    return FA_E_SHAPE;
-  const int item = item_size(dtype);
-  if (!dy || (dw && (!codes || !ranges)) || reinterpret_cast<size_t>(dy) % item ||
-      reinterpret_cast<size_t>(dw) % item || reinterpret_cast<size_t>(db) % item ||
-      reinterpret_cast<size_t>(codes) % 16 || reinterpret_cast<size_t>(ranges) % 8 || !ws ||
-      reinterpret_cast<size_t>(ws) % 256)
-    return FA_E_ARG;
-  const WgradPlan plan = wgrad_plan(rows, inputs, outputs, dtype, device);
-  if (ws_bytes < plan.bytes) return FA_E_ARG;
-  FAB_DEVICE_SCOPE(device);
-  if (db)
-    if (const int rc = bias_grad_impl(dy, dy_row, db, dtype, rows, outputs, ws, ws_bytes, device, st))
+template <typename T>
+static int linear_forward(const fa_linear8& l, LinearPlan& p, char* ws, int device, cudaStream_t st) {
+  if (const int rc = ready_operand<T>(&p.x, ws, l.x_stride, device, st)) return rc;
+  if (const int rc = ready_operand<T>(&p.w, ws, l.weight_stride, device, st)) return rc;
+  return product_run<T>(p.x, p.w, l.inputs, false, l.bias, l.y, l.rows, l.outputs, p.y_parts,
+                        ws + p.part, p, st);
+}
+
+template <typename T>
+static int linear_backward(const fa_linear8& l, LinearPlan& p, char* ws, int device, cudaStream_t st) {
+  if (const int rc = ready_operand<T>(&p.dy, ws, l.dy_stride, device, st)) return rc;
+  if (const int rc = ready_operand<T>(&p.w, ws, l.weight_stride, device, st)) return rc;
+  if (l.dx)
+    if (const int rc = product_run<T>(p.dy, p.w, l.outputs, true, nullptr, l.dx, l.rows, l.inputs,
+                                      p.dx_parts, ws + p.part, p, st))
       return rc;
-  if (!dw) return FA_OK;
-  if (dtype == FA_F16)
-    return wgrad_run<f16_t>(dy, dy_row, codes, ranges, rows, inputs, outputs, dw,
-                            static_cast<char*>(ws), plan, device, st);
-  if (dtype == FA_BF16)
-    return wgrad_run<bf16_t>(dy, dy_row, codes, ranges, rows, inputs, outputs, dw,
-                             static_cast<char*>(ws), plan, device, st);
+  return l.dweight ? wgrad_run<T>(l, p.dy, ws + p.part, p, st) : FA_OK;
+}
+
+int linear8_impl(const fa_linear8* l, void* ws, size_t bytes, int device, cudaStream_t st) {
+  if (const int rc = linear_check(l)) return rc;
+  if (l->dx || l->dweight || l->dbias || (!l->y && !l->codes) || !l->x) return FA_E_ARG;
+  LinearPlan p = linear_plan(*l, device);
+  if (const int rc = workspace_check(p, ws, bytes)) return rc;
+  FAB_DEVICE_SCOPE(device);
+  if (l->codes)
+    if (const int rc = pack8_impl(l->x, l->x_stride, l->codes, l->ranges, l->dtype, l->rows,
+                                  l->inputs, device, st))
+      return rc;
+  if (!l->y) return FA_OK;
+  if (l->dtype == FA_F16) return linear_forward<f16_t>(*l, p, static_cast<char*>(ws), device, st);
+  return linear_forward<bf16_t>(*l, p, static_cast<char*>(ws), device, st);
+}
+
+int linear8_backward_impl(const fa_linear8* l, void* ws, size_t bytes, int device, cudaStream_t st) {
+  if (const int rc = linear_check(l)) return rc;
+  if (l->y || (!l->dx && !l->dweight && !l->dbias)) return FA_E_ARG;
+  LinearPlan p = linear_plan(*l, device);
+  if (const int rc = workspace_check(p, ws, bytes)) return rc;
+  FAB_DEVICE_SCOPE(device);
+  if (l->dbias)
+    if (const int rc = bias_grad_impl(l->dy, l->dy_stride, l->dbias, l->dtype, l->rows, l->outputs,
+                                      ws, bytes, device, st))
+      return rc;
+  if (l->dtype == FA_F16) return linear_backward<f16_t>(*l, p, static_cast<char*>(ws), device, st);
+  if (l->dtype == FA_BF16) return linear_backward<bf16_t>(*l, p, static_cast<char*>(ws), device, st);
+  if (!l->dweight) return FA_OK;
   WgradArgs a;
-  a.dy = dy;
-  a.dy_row = dy_row;
-  a.codes = static_cast<const unsigned char*>(codes);
-  a.ranges = ranges;
-  a.rows = rows;
-  a.inputs = inputs;
-  a.outputs = outputs;
-  a.groups = (int)groups8(inputs);
-  a.dw = dw;
-  const dim3 grid((unsigned)((inputs + kWgTile - 1) / kWgTile),
-                  (unsigned)((outputs + kWgTile - 1) / kWgTile));
+  a.dy = l->dy;
+  a.dy_row = l->dy_stride;
+  a.codes = static_cast<const unsigned char*>(l->codes);
+  a.ranges = l->ranges;
+  a.rows = l->rows;
+  a.inputs = l->inputs;
+  a.outputs = l->outputs;
+  a.groups = (int)groups8(l->inputs);
+  a.dw = l->dweight;
+  const dim3 grid((unsigned)((l->inputs + kWgTile - 1) / kWgTile),
+                  (unsigned)((l->outputs + kWgTile - 1) / kWgTile));
   wgrad_lanes_kernel<float><<<grid, 256, 0, st>>>(a);
   FAB_LAUNCH_CHECK();
   return FA_OK;

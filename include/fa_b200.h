@@ -690,18 +690,40 @@ FA_B200_API int fa_b200_layer_norm_backward(const fa_norm* params, const void* d
                                             void* dx, void* dweight, void* dbias, void* workspace,
                                             size_t workspace_bytes, int device, void* stream);
 
-/* Weight gradient of y = x W^T + b from the packed copy of x [rows][inputs]:
- * dweight [outputs][inputs] = dy^T x (null: not computed), dbias [outputs] = column
- * sums of dy (null: not computed).  At most 2^27 rows, 4194240 inputs and outputs.
- * Workspace: 256-byte aligned, needs no zeroing. */
-FA_B200_API int fa_b200_linear8_weight_grad_workspace_bytes(int64_t rows, int inputs, int outputs,
-                                                            int dtype, int device,
-                                                            size_t* out_bytes);
-FA_B200_API int fa_b200_linear8_weight_grad(const void* dy, int64_t dy_stride, const void* codes,
-                                            const void* ranges, int dtype, int64_t rows,
-                                            int inputs, int outputs, void* dweight, void* dbias,
-                                            void* workspace, size_t workspace_bytes, int device,
-                                            void* stream);
+/* y = x W^T + bias, with x kept packed for the backward pass:
+ *   x [rows][inputs], weight [outputs][inputs], y and dy [rows][outputs],
+ *   dx = dy W,  dweight [outputs][inputs] = dy^T x^ (x^ the packed copy's values),
+ *   dbias = column sums of dy.
+ * Strides in elements between rows of unit stride; results are contiguous.  Sums are
+ * float32.  At most 2^27 rows, 4194240 inputs and outputs.  Forward: x, and y (with
+ * weight, and bias or null) or codes/ranges, or both.  Backward: dy, and any of dx
+ * (with weight), dweight (with codes/ranges) and dbias; the others null.  FA_F32 has
+ * no y and no dx.  Workspace (size from the query, for the same structure): 256-byte
+ * aligned, needs no zeroing; null where the size is 0. */
+typedef struct fa_linear8 {
+  int32_t dtype, inputs, outputs, pad_;
+  int64_t rows;
+  const void* x;
+  int64_t x_stride;
+  const void* dy;
+  int64_t dy_stride;
+  const void* weight;
+  int64_t weight_stride;
+  const void* bias;
+  void* codes;
+  void* ranges;
+  void* y;
+  void* dx;
+  void* dweight;
+  void* dbias;
+} fa_linear8;
+
+FA_B200_API int fa_b200_linear8_workspace_bytes(const fa_linear8* params, int device,
+                                                size_t* out_bytes);
+FA_B200_API int fa_b200_linear8(const fa_linear8* params, void* workspace, size_t workspace_bytes,
+                                int device, void* stream);
+FA_B200_API int fa_b200_linear8_backward(const fa_linear8* params, void* workspace,
+                                         size_t workspace_bytes, int device, void* stream);
 
 /* No counterpart in the reference: test hook of the bounded device-side
  * waits.  Launches one thread that waits `limit_ns` (at most 1 s) for an

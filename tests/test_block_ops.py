@@ -129,6 +129,8 @@ def test_forward_mode_is_refused(name):
 def test_structure_matches_the_header():
     assert ctypes.sizeof(_cabi.fa_norm) == 16 + 8 + 8 + 4 * 8 + 5 * 8
     assert len(block._NORM(3, 3, 1, 1, 0, 0.0, *[0] * 9)) == ctypes.sizeof(_cabi.fa_norm)
+    assert ctypes.sizeof(_cabi.fa_linear8) == 16 + 8 + 3 * 16 + 7 * 8
+    assert len(block._LINEAR(*[0] * 18)) == ctypes.sizeof(_cabi.fa_linear8)
 
 
 def test_c_entries_refuse_before_any_launch():
@@ -172,14 +174,28 @@ def test_c_entries_refuse_before_any_launch():
     assert L.fa_b200_layer_norm_backward_workspace_bytes(0, 8, 0, ctypes.byref(size)) == 2
     assert L.fa_b200_layer_norm_backward_workspace_bytes(3, 8, 0, None) == 5
 
-    q = L.fa_b200_linear8_weight_grad_workspace_bytes
-    assert q(3, 8, 8, F16, 0, ctypes.byref(size)) == 0 and size.value > 0
-    assert q(3, 8, 8, 4, 0, ctypes.byref(size)) == 1 and q(3, 0, 8, F16, 0, ctypes.byref(size)) == 2
-
-    def wgrad(dy=512, codes=512, ranges=512, dtype=F16, rows=3, k=8, m=8, dw=512, db=512, ws=512,
-              room=1 << 30):
-        return L.fa_b200_linear8_weight_grad(dy, 8, codes, ranges, dtype, rows, k, m, dw, db, ws,
-                                             room, 0, None)
-    assert wgrad(dtype=4) == 1 and wgrad(rows=0) == 2 and wgrad(k=1 << 23) == 2
-    assert wgrad(dy=None) == 5 and wgrad(codes=None) == 5 and wgrad(ranges=None) == 5
-    assert wgrad(ws=None) == 5 and wgrad(room=0) == 5 and wgrad(dy=513) == 5 and wgrad(codes=520) == 5
+    def linear(**kw):
+        f = dict(dtype=F16, inputs=8, outputs=8, rows=3, x=512, x_stride=8, weight=512,
+                 weight_stride=8, y=512)
+        f.update(kw)
+        return ctypes.byref(_cabi.fa_linear8(**f))
+    back = dict(x=None, y=None, dy=512, dy_stride=8, dx=512)
+    q = L.fa_b200_linear8_workspace_bytes
+    assert q(linear(), 0, ctypes.byref(size)) == 0 and q(linear(), 0, None) == 5
+    assert q(None, 0, ctypes.byref(size)) == 5
+    # an operand that TMA does not read is copied
+    assert q(linear(inputs=7, x_stride=7, weight_stride=7), 0, ctypes.byref(size)) == 0
+    assert size.value >= 2 * 256
+    room = 1 << 30
+    for kw, want in (({"dtype": 4}, 1), ({"dtype": F32}, 1), ({"rows": 0}, 2), ({"inputs": 0}, 2),
+                     ({"outputs": 1 << 23}, 2), ({"rows": (1 << 27) + 1}, 2), ({"x": None}, 5),
+                     ({"weight": None}, 5), ({"x": 513}, 5), ({"y": None}, 5), ({"codes": 512}, 5),
+                     ({"codes": 520, "ranges": 512}, 5), ({"dx": 512, "dy": 512}, 5)):
+        assert L.fa_b200_linear8(linear(**kw), 512, room, 0, None) == want, kw
+    for kw, want in (({"dtype": F32}, 1), ({"dy": None}, 5), ({"weight": None}, 5), ({"dx": None}, 5),
+                     ({"y": 512, "x": 512}, 5), ({"dweight": 512}, 5), ({"dy": 511}, 5)):
+        assert L.fa_b200_linear8_backward(linear(**{**back, **kw}), 512, room, 0, None) == want, kw
+    copied = linear(**{**back, "outputs": 7, "dy_stride": 7})
+    assert L.fa_b200_linear8_backward(copied, None, 0, 0, None) == 5
+    assert L.fa_b200_linear8_backward(copied, 512, 16, 0, None) == 5
+    assert L.fa_b200_linear8_backward(copied, 520, room, 0, None) == 5

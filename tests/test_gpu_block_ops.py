@@ -519,6 +519,10 @@ LINEARS = [
     (4000, 64, 128, True),
     (700, 520, 520, True),
     (20000, 16, 24, True),
+    (3, 5000, 264, True),      # few tiles, a long sum
+    (300, 64, 3000, True),
+    (2500, 300, 20, False),
+    (1030, 1100, 2056, True),
 ]
 
 
@@ -528,6 +532,16 @@ def linear_case(case, dtype, seed=0):
     w = rand(m, k, seed=seed + 2, scale=k ** -0.5, dtype=dtype)
     b = rand(m, seed=seed + 3, dtype=dtype) if bias else None
     return x, w, b, rand(t, m, seed=seed + 4, dtype=dtype)
+
+
+def check_product(got, a, b, bias, dtype):
+    """got = a b^T + bias: float32 sums of k terms, rounded once."""
+    a, b = a.double(), b.double()
+    want = a @ b.mT
+    tol = (8 + 4 * math.sqrt(a.shape[-1])) * E * (a.abs() @ b.abs().mT)
+    if bias is not None:
+        want, tol = want + bias.double(), tol + 2 * E * bias.double().abs()
+    within(got, want, (1 + 2 * U[dtype]) * tol + U[dtype] * want.abs(), dtype)
 
 
 def check_weight_grad(dw, db, x, gy, dtype):
@@ -550,9 +564,10 @@ def test_linear(case, dtype):
     x, w, b, gy = linear_case(case, dtype)
     leaves = [t.detach().requires_grad_(True) for t in (x, w, b) if t is not None]
     y = fa.linear8(leaves[0], leaves[1], leaves[2] if b is not None else None)
-    assert torch.equal(y.detach(), F.linear(x, w, b))
+    assert torch.equal(y.detach(), fa.linear8(x, w, b))
+    check_product(y.detach(), x, w, b, dtype)
     got = torch.autograd.grad(y, leaves, gy)
-    assert torch.equal(got[0], gy @ w)
+    check_product(got[0], gy, w.mT, None, dtype)
     assert got[1].shape == w.shape and got[1].is_contiguous()
     check_weight_grad(got[1], got[2] if b is not None else None, x, gy, dtype)
 
@@ -571,13 +586,9 @@ def test_linear_of_views(dtype):
         wt, gy = wt[:m], gy[..., :m]
         leaves = [x.detach().requires_grad_(True), wt.detach().requires_grad_(True)]
         y = fa.linear8(*leaves)
-        # (which of its products torch takes for views depends on more than the operands)
-        size = F.linear(x.double().abs(), wt.double().abs())
-        want = F.linear(x.double(), wt.double())
-        within(y.detach(), want, U[dtype] * want.abs() + (8 + 4 * math.sqrt(x.shape[-1])) * E * size,
-               dtype)
+        check_product(y.detach(), x, wt, None, dtype)
         dx, dw = torch.autograd.grad(y, leaves, gy)
-        assert dx.shape == x.shape
+        check_product(dx, gy, wt.mT, None, dtype)
         check_weight_grad(dw, None, x, gy, dtype)
 
 
@@ -590,7 +601,7 @@ def test_linear_with_an_expanded_gradient_and_parts_that_need_none():
         y.sum().backward()
         one = torch.ones_like(y)
         if need[0]:
-            assert torch.equal(leaves[0].grad, one @ w)
+            check_product(leaves[0].grad, one, w.mT, None, torch.bfloat16)
         check_weight_grad(leaves[1].grad, leaves[2].grad, x, one, torch.bfloat16)
         assert [t.grad is not None for t in leaves] == list(need)
 
@@ -613,8 +624,8 @@ def test_linear_under_autocast(dtype):
     leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
     with torch.autocast("cuda", dtype=dtype):
         y = fa.linear8(*leaves)
-        want = F.linear(x, w, b)
-    assert y.dtype == dtype and torch.equal(y.detach(), want)
+    assert y.dtype == dtype
+    check_product(y.detach(), x.to(dtype), w.to(dtype), b.to(dtype), dtype)
     got = torch.autograd.grad(y, leaves, gy.to(dtype))
     assert all(g.dtype == torch.float32 for g in got)
     check_weight_grad(got[1].to(dtype), got[2].to(dtype), x.to(dtype), gy.to(dtype), dtype)
