@@ -198,12 +198,6 @@ __device__ __forceinline__ void stage_wait(unsigned long long* bar, unsigned par
   if (!mbar_sleep(a, parity)) stage_wait_slow(a, parity, err);
 }
 
-// A phase that the other block of the pair may complete.
-__device__ __forceinline__ void wait_pair(unsigned long long* bar, unsigned parity, unsigned* err) {
-  stage_wait(bar, parity, err);
-  asm volatile("fence.acq_rel.cluster;\n" ::: "memory");
-}
-
 // A warp has written its share of a stage, here or in the other block of the pair.
 // What it wrote is in its own block's shared memory and fence.proxy.async has handed
 // it to the tensor cores; nothing else has to be ordered, and a release to the whole
@@ -369,7 +363,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
                              ((unsigned)(kTile / 16) << 24);
       unsigned n = 0, tile = 0;
       for (int item = first; work_of(a, item, &t); item += step, ++tile) {
-        if (tile >= 1) wait_pair(&tm_empty, (tile - 1) & 1, a.err);
+        if (tile >= 1) stage_wait(&tm_empty, (tile - 1) & 1, a.err);
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         bool ready = false;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
@@ -500,7 +494,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
         }
       }
       // the tile's sums: a lane an input, this team's half of the outputs
-      if (lane == 0) wait_pair(&tm_full, tile & 1, a.err);
+      if (lane == 0) stage_wait(&tm_full, tile & 1, a.err);
       __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       const int i = t.i0 + rank * 128 + 32 * w + lane;
@@ -710,7 +704,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
       unsigned n = 0, tile = 0;
       for (int item = first; work_of(a, item, &t); item += step, ++tile) {
         const unsigned d = tmem + (tile & 1) * 256;
-        if (tile >= 2) wait_pair(&tm_empty[tile & 1], (tile / 2 - 1) & 1, a.err);
+        if (tile >= 2) stage_wait(&tm_empty[tile & 1], (tile / 2 - 1) & 1, a.err);
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         bool ready = false;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
@@ -739,7 +733,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
     int other = 0;
     for (int item = first; work_of(a, item, &t); item += step, ++tile) {
       const int buf = tile & 1;
-      if (lane == 0) wait_pair(&tm_full[buf], (tile / 2) & 1, a.err);
+      if (lane == 0) stage_wait(&tm_full[buf], (tile / 2) & 1, a.err);
       __syncwarp();
       asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
       const int i = t.i0 + rank * 128 + 32 * w;
