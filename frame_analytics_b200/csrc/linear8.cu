@@ -29,71 +29,115 @@ size_t norm_ws_bytes(long long rows, int width, int device);
 int pack8_impl(const void* x, long long x_row, void* codes, void* ranges, int dtype,
                long long rows, int width, int device, cudaStream_t st);
 
+// ---------------------------------------------------------------------------
+// dW in float32
+// ---------------------------------------------------------------------------
+
+// 128 outputs x 128 inputs a block, 8 x 8 a thread, in float32 on the ordinary lanes
+// (two products an instruction): the tensor cores would round the operands.  16 rows t
+// a stage; the next stage's dy and codes are on their way while this one's products
+// run.  Few tiles: the rows are cut into parts, whose sums are joined in order.
+constexpr int kWgTile = 128, kWgRows = 16;
+
 struct WgradArgs {
-  const void* dy;
+  const float* dy;
   long long dy_row;
   const unsigned char* codes;
-  const void* ranges;
-  long long rows;
-  int inputs, outputs, groups;
-  void* dw;                     // [outputs][inputs]
+  const float2* ranges;
+  long long rows, per_part;     // rows of a part, whole stages
+  int inputs, outputs, groups, parts;
+  float* dw;                    // [parts][outputs][inputs]
+  int dy_vec;                   // rows of dy are whole aligned vectors of four
 };
 
-constexpr int kWgTile = 64;     // rows and columns of a block's part of dW
-constexpr int kWgRows = 16;     // rows t at a time
-
-// One block to a 64 x 64 tile in float32 on the ordinary lanes.
-template <typename T>
 __global__ void __launch_bounds__(256) wgrad_lanes_kernel(const WgradArgs a) {
-  __shared__ float sa[kWgRows][kWgTile + 4], sb[kWgRows][kWgTile + 4];
-  const int m0 = blockIdx.y * kWgTile, k0 = blockIdx.x * kWgTile;
+  __shared__ __align__(16) float sa[2][kWgRows][kWgTile], sb[2][kWgRows][kWgTile];
+  const int m0 = blockIdx.x * kWgTile, k0 = blockIdx.y * kWgTile;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (long long t0 = 0; t0 < a.rows; t0 += kWgRows) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < kWgRows * kWgTile; i += 256) {
-      const int t = i / kWgTile, m = i % kWgTile;
-      float v = 0.f;
-      if (t0 + t < a.rows && m0 + m < a.outputs)
-        v = Ld<T>::f(ldro(reinterpret_cast<const T*>(a.dy) + (t0 + t) * a.dy_row + m0 + m));
-      sa[t][m] = v;
-    }
-    if (threadIdx.x < kWgRows * 8) {
-      const int t = threadIdx.x / 8, u = threadIdx.x % 8;
-      uint2 q = make_uint2(0u, 0u);
-      typename RangeBits<T>::type bits = {};
-      if (t0 + t < a.rows) {
-        const long long g = (t0 + t) * a.groups + k0 / kGroup8;
-        q = __ldg(reinterpret_cast<const uint2*>(a.codes) + g * 8 + u);
-        bits = __ldg(reinterpret_cast<const typename RangeBits<T>::type*>(a.ranges) + g);
+  const long long t0 = blockIdx.z * a.per_part, t1 = min(a.rows, t0 + a.per_part);
+  // this thread's share of a stage: 2 x 4 of dy's columns, 8 codes
+  const int ra = threadIdx.x >> 5, ca = (threadIdx.x & 31) * 4;   // rows ra, ra + 8
+  const int rb = threadIdx.x >> 4, ub = threadIdx.x & 15;         // row rb, unit ub
+  const int g = k0 / kGroup8 + (ub >> 3);
+  float4 na[2];
+  uint2 nq;
+  float2 nr;
+  const auto fetch = [&](long long t) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long long r = t + ra + 8 * h;
+      na[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < t1) {
+        const float* p = a.dy + r * a.dy_row + m0 + ca;
+        if (a.dy_vec && m0 + ca + 4 <= a.outputs) {
+          na[h] = __ldg(reinterpret_cast<const float4*>(p));
+        } else {
+          if (m0 + ca < a.outputs) na[h].x = __ldg(p);
+          if (m0 + ca + 1 < a.outputs) na[h].y = __ldg(p + 1);
+          if (m0 + ca + 2 < a.outputs) na[h].z = __ldg(p + 2);
+          if (m0 + ca + 3 < a.outputs) na[h].w = __ldg(p + 3);
+        }
       }
-      const F8 x = decode8<T>(q, range_of(bits, T()));
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sb[t][u * 8 + i] = x.at(i);
     }
+    nq = make_uint2(0u, 0u);
+    nr = make_float2(0.f, 0.f);
+    if (t + rb < t1 && g < a.groups) {
+      const long long at = (t + rb) * a.groups + g;
+      nq = __ldg(reinterpret_cast<const uint2*>(a.codes) + at * 8 + (ub & 7));
+      nr = __ldg(a.ranges + at);
+    }
+  };
+  const auto put = [&](int half) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) *reinterpret_cast<float4*>(&sa[half][ra + 8 * h][ca]) = na[h];
+    put8<float>(&sb[half][rb][ub * 8], narrow8(decode8<float>(nq, range_of(nr, 0.f)), 0.f));
+  };
+  float2 acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = both(0.f);
+  fetch(t0);
+  put(0);
+  int half = 0;
+  for (long long t = t0; t < t1; t += kWgRows, half ^= 1) {
     __syncthreads();
+    fetch(t + kWgRows);
 #pragma unroll
-    for (int t = 0; t < kWgRows; ++t) {
-      float p[4], q[4];
+    for (int r = 0; r < kWgRows; ++r) {
+      // outputs ty * 4 + 0..3 and 64 on, inputs tx * 4 + 0..3 and 64 on
+      const float4 p0 = *reinterpret_cast<const float4*>(&sa[half][r][ty * 4]),
+                   p1 = *reinterpret_cast<const float4*>(&sa[half][r][64 + ty * 4]),
+                   q0 = *reinterpret_cast<const float4*>(&sb[half][r][tx * 4]),
+                   q1 = *reinterpret_cast<const float4*>(&sb[half][r][64 + tx * 4]);
+      const float p[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+      const float2 q[4] = {{q0.x, q0.y}, {q0.z, q0.w}, {q1.x, q1.y}, {q1.z, q1.w}};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = sa[t][ty * 4 + i];
-        q[i] = sb[t][tx * 4 + i];
-      }
+      for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 4; ++j) acc[i][j] = __ffma2_rn(both(p[i]), q[j], acc[i][j]);
+    }
+    if (t + kWgRows < t1) put(half ^ 1);
+  }
+  float* const out = a.dw + (long long)blockIdx.z * a.outputs * a.inputs;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(p[i], q[j], acc[i][j]);
+  for (int i = 0; i < 8; ++i) {
+    const int m = m0 + (i >> 2) * 64 + ty * 4 + (i & 3);
+    if (m >= a.outputs) continue;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int k = k0 + (j >> 2) * 64 + tx * 4 + (j & 3);
+      if (k < a.inputs) out[(long long)m * a.inputs + k] = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
     }
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int m = m0 + ty * 4 + i, k = k0 + tx * 4 + j;
-      if (m < a.outputs && k < a.inputs)
-        reinterpret_cast<T*>(a.dw)[(long long)m * a.inputs + k] = St<T>::v(acc[i][j]);
-    }
+}
+__global__ void __launch_bounds__(256) join_lanes_kernel(const float* part, float* dw, int parts,
+                                                         long long size) {
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < size; i += gridDim.x * 256ll) {
+    float t = 0.f;
+    for (int p = 0; p < parts; ++p) t += part[p * size + i];
+    dw[i] = t;
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -823,7 +867,7 @@ __global__ void __launch_bounds__(256) pitch_kernel(const T* x, long long x_row,
 
 // A tile's sum over 2^27 rows takes under a second, and a wait for it two at most.
 constexpr long long kMaxRows = 1ll << 27;
-constexpr int kMaxSide = (1 << 22) - 64;  // 65535 tiles of 64
+constexpr int kMaxSide = (1 << 22) - 64;
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -954,6 +998,13 @@ static LinearPlan linear_plan(const fa_linear8& l, int device) {
     p.dx_parts = parts(l.dx, rows * in, stages_of(l.outputs));
     p.dw_parts = parts(l.dweight, (long long)in * out, stages_of(l.rows));
   }
+  if (l.dtype == FA_F32 && l.dweight) {
+    // parts that fill the multiprocessors twice, of 256 rows or more
+    const long long tiles = (long long)((l.inputs + kWgTile - 1) / kWgTile) *
+                            ((l.outputs + kWgTile - 1) / kWgTile);
+    p.dw_parts = (int)std::max(1ll, std::min((long long)(l.rows + 255) / 256, 2ll * sm_count(device) / tiles));
+    if (p.dw_parts > 1) part = sizeof(float) * (size_t)p.dw_parts * l.inputs * l.outputs;
+  }
   p.part = used;
   p.bytes = used + part;
   return p;
@@ -1012,6 +1063,7 @@ static int product_run(const Operand& x, const Operand& w, int depth, bool w_mn,
   a.bias_vec = reinterpret_cast<size_t>(bias) % 16 == 0;
   a.part = reinterpret_cast<float*>(part);
   a.err = wait_error_word();
+  if (!a.err) return FA_E_INTERNAL;  // a wait that gave up could not be reported
   FAB_TRY(cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                kPlainSmem));
   const int items = a.tiles_m * a.tiles_n * parts;
@@ -1044,6 +1096,7 @@ static int wgrad_run(const fa_linear8& l, const Operand& dy, char* part, const L
   a.out = l.dweight;
   a.part = reinterpret_cast<float*>(part);
   a.err = wait_error_word();
+  if (!a.err) return FA_E_INTERNAL;  // a wait that gave up could not be reported
   FAB_TRY(cudaFuncSetAttribute(wgrad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmem));
   const int items = a.tiles_m * a.tiles_n * a.parts;
   wgrad_kernel<T><<<2 * std::min(items, plan.pairs), kWgThreads, kWgSmem, st>>>(a);
@@ -1074,6 +1127,35 @@ static int linear_backward(const fa_linear8& l, LinearPlan& p, char* ws, int dev
   return l.dweight ? wgrad_run<T>(l, p.dy, ws + p.part, p, st) : FA_OK;
 }
 
+static int wgrad_lanes(const fa_linear8& l, const LinearPlan& p, char* ws, int device,
+                       cudaStream_t st) {
+  WgradArgs a = {};
+  a.dy = static_cast<const float*>(l.dy);
+  a.dy_row = l.dy_stride;
+  a.dy_vec = reinterpret_cast<size_t>(l.dy) % 16 == 0 && (l.rows == 1 || l.dy_stride % 4 == 0);
+  a.codes = static_cast<const unsigned char*>(l.codes);
+  a.ranges = static_cast<const float2*>(l.ranges);
+  a.rows = l.rows;
+  a.inputs = l.inputs;
+  a.outputs = l.outputs;
+  a.groups = (int)groups8(l.inputs);
+  const long long stages = (l.rows + kWgRows - 1) / kWgRows;
+  a.per_part = (stages + p.dw_parts - 1) / p.dw_parts * kWgRows;
+  a.parts = (int)((l.rows + a.per_part - 1) / a.per_part);
+  a.dw = a.parts > 1 ? reinterpret_cast<float*>(ws + p.part) : static_cast<float*>(l.dweight);
+  const dim3 grid((unsigned)((l.outputs + kWgTile - 1) / kWgTile),
+                  (unsigned)((l.inputs + kWgTile - 1) / kWgTile), (unsigned)a.parts);
+  wgrad_lanes_kernel<<<grid, 256, 0, st>>>(a);
+  FAB_LAUNCH_CHECK();
+  if (a.parts > 1) {
+    const long long size = (long long)l.outputs * l.inputs;
+    join_lanes_kernel<<<(unsigned)std::min((size + 255) / 256, 8ll * sm_count(device)), 256, 0, st>>>(
+        a.dw, static_cast<float*>(l.dweight), a.parts, size);
+    FAB_LAUNCH_CHECK();
+  }
+  return FA_OK;
+}
+
 int linear8_impl(const fa_linear8* l, void* ws, size_t bytes, int device, cudaStream_t st) {
   if (const int rc = linear_check(l)) return rc;
   if (l->dx || l->dweight || l->dbias || (!l->y && !l->codes) || !l->x) return FA_E_ARG;
@@ -1101,22 +1183,7 @@ int linear8_backward_impl(const fa_linear8* l, void* ws, size_t bytes, int devic
       return rc;
   if (l->dtype == FA_F16) return linear_backward<f16_t>(*l, p, static_cast<char*>(ws), device, st);
   if (l->dtype == FA_BF16) return linear_backward<bf16_t>(*l, p, static_cast<char*>(ws), device, st);
-  if (!l->dweight) return FA_OK;
-  WgradArgs a;
-  a.dy = l->dy;
-  a.dy_row = l->dy_stride;
-  a.codes = static_cast<const unsigned char*>(l->codes);
-  a.ranges = l->ranges;
-  a.rows = l->rows;
-  a.inputs = l->inputs;
-  a.outputs = l->outputs;
-  a.groups = (int)groups8(l->inputs);
-  a.dw = l->dweight;
-  const dim3 grid((unsigned)((l->inputs + kWgTile - 1) / kWgTile),
-                  (unsigned)((l->outputs + kWgTile - 1) / kWgTile));
-  wgrad_lanes_kernel<float><<<grid, 256, 0, st>>>(a);
-  FAB_LAUNCH_CHECK();
-  return FA_OK;
+  return l->dweight ? wgrad_lanes(*l, p, static_cast<char*>(ws), device, st) : FA_OK;
 }
 
 }  // namespace fab
