@@ -3,7 +3,9 @@
 Noisy frames are cut into patches; each block normalises and rotates its queries
 and keys (``fa.qk_norm_rotary``), the loss is ``1 - SSIM`` plus a Charbonnier
 term, and the weight matrices take orthogonalised updates (``fa.Muon``); norms,
-biases and the position-free rest go to AdamW.
+biases and the position-free rest go to AdamW.  With ``--keep8`` the blocks' norms,
+activations and products keep their inputs for the backward pass in 8 bits
+(``fa.layer_norm``, ``fa.gelu8``, ``fa.linear8``).
 
     python examples/train_restoration.py --steps 100
 """
@@ -36,9 +38,9 @@ def angle_tables(rows: int, cols: int, rotary: int, device):
 
 
 class Block(nn.Module):
-    def __init__(self, width: int, heads: int):
+    def __init__(self, width: int, heads: int, keep8: bool = False):
         super().__init__()
-        self.heads, self.dim = heads, width // heads
+        self.heads, self.dim, self.keep8 = heads, width // heads, keep8
         self.norm1, self.norm2 = nn.LayerNorm(width), nn.LayerNorm(width)
         self.qkv = nn.Linear(width, 3 * width, bias=False)
         self.proj = nn.Linear(width, width, bias=False)
@@ -47,23 +49,35 @@ class Block(nn.Module):
         self.q_weight = nn.Parameter(torch.ones(self.dim))
         self.k_weight = nn.Parameter(torch.ones(self.dim))
 
+    def norm(self, norm, x, residual=None):
+        return fa.layer_norm(x, norm.weight, norm.bias, residual=residual, eps=norm.eps, keep8=True)
+
     def forward(self, x, cos, sin):
         b, n, w = x.shape
-        packed = self.qkv(self.norm1(x)).view(b, n, 3 * self.heads, self.dim)
+        if self.keep8:
+            packed = fa.linear8(self.norm(self.norm1, x), self.qkv.weight)
+        else:
+            packed = self.qkv(self.norm1(x))
+        packed = packed.view(b, n, 3 * self.heads, self.dim)
         q, k, v = packed.split(self.heads, dim=2)
         q, k = fa.qk_norm_rotary(q, k, cos, sin, q_weight=self.q_weight, k_weight=self.k_weight)
         y = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2),
                                            v.transpose(1, 2))
-        x = x + self.proj(y.transpose(1, 2).reshape(b, n, w))
+        y = y.transpose(1, 2).reshape(b, n, w)
+        if self.keep8:
+            y, x = self.norm(self.norm2, fa.linear8(y, self.proj.weight), residual=x)
+            return x + fa.linear8(fa.gelu8(fa.linear8(y, self.up.weight)), self.down.weight)
+        x = x + self.proj(y)
         return x + self.down(F.gelu(self.up(self.norm2(x))))
 
 
 class Restorer(nn.Module):
-    def __init__(self, patch: int = 8, width: int = 192, heads: int = 6, depth: int = 2):
+    def __init__(self, patch: int = 8, width: int = 192, heads: int = 6, depth: int = 2,
+                 keep8: bool = False):
         super().__init__()
         self.patch, self.rotary = patch, width // heads
         self.embed = nn.Conv2d(3, width, patch, patch)
-        self.blocks = nn.ModuleList(Block(width, heads) for _ in range(depth))
+        self.blocks = nn.ModuleList(Block(width, heads, keep8) for _ in range(depth))
         self.head = nn.Linear(width, 3 * patch * patch)
         nn.init.zeros_(self.head.weight)
         nn.init.zeros_(self.head.bias)
@@ -86,11 +100,12 @@ def batch(n: int, size: int, generator, device):
     return clean, (clean + noise).clamp(0, 1)
 
 
-def train(steps: int = 100, size: int = 96, frames: int = 8, device="cuda", report=None):
+def train(steps: int = 100, size: int = 96, frames: int = 8, device="cuda", report=None,
+          keep8: bool = False):
     """Returns the loss of every step."""
     torch.manual_seed(0)
     g = torch.Generator(device=device).manual_seed(1)
-    net = Restorer().to(device)
+    net = Restorer(keep8=keep8).to(device)
     matrices = [p for name, p in net.named_parameters() if p.dim() >= 2 and "head" not in name]
     chosen = {id(p) for p in matrices}
     others = [p for p in net.parameters() if id(p) not in chosen]
@@ -117,5 +132,6 @@ if __name__ == "__main__":
     ap.add_argument("--steps", type=int, default=100)
     ap.add_argument("--size", type=int, default=96)
     ap.add_argument("--frames", type=int, default=8)
+    ap.add_argument("--keep8", action="store_true", help="keep activations in 8 bits")
     args = ap.parse_args()
-    train(args.steps, args.size, args.frames, report=10)
+    train(args.steps, args.size, args.frames, report=10, keep8=args.keep8)

@@ -50,7 +50,7 @@ struct WgradArgs {
   int dy_vec;                   // rows of dy are whole aligned vectors of four
 };
 
-__global__ void __launch_bounds__(256) wgrad_lanes_kernel(const WgradArgs a) {
+__global__ void __launch_bounds__(256, 2) wgrad_lanes_kernel(const WgradArgs a) {
   __shared__ __align__(16) float sa[2][kWgRows][kWgTile], sb[2][kWgRows][kWgTile];
   const int m0 = blockIdx.x * kWgTile, k0 = blockIdx.y * kWgTile;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
