@@ -402,15 +402,11 @@ def _linear_forward(x, weight, bias, kept, ranges: int) -> torch.Tensor:
     outputs = weight.shape[0]
     fn = backend.lib().fa_b200_linear8
     at = 0 if kept is None else kept.data_ptr()
-    if x.dtype == torch.float32:
-        if kept is not None:
-            _pack_into(r, at, at + ranges)
-        return F.linear(x, weight, bias)
     if weight.stride(1) != 1 and inputs > 1:
         weight = weight.contiguous()
     if bias is not None:
         bias = bias.contiguous()
-    y = torch.empty((*x.shape[:-1], outputs), dtype=x.dtype, device=x.device)
+    y = x.new_empty((*x.shape[:-1], outputs))
     _linear_call(fn, r, rows, inputs, outputs, r, None, weight, bias, at,
                  at + ranges if at else 0, y, None, None, None)
     return y
@@ -432,25 +428,17 @@ class _Linear8(torch.autograd.Function):
         kept, weight = ctx.saved_tensors
         need, (outputs, inputs) = ctx.needs_input_grad, weight.shape
         g = _rows(gy)
-        dx = dw = db = None
-        own = gy.dtype != torch.float32
+        dx = dw = db = w = None
+        at = 0
         if need[0]:
-            if own:
-                dx = torch.empty((*gy.shape[:-1], inputs), dtype=gy.dtype, device=gy.device)
-                if weight.stride(1) != 1 and inputs > 1:
-                    weight = weight.contiguous()
-            else:
-                with torch.autocast("cuda", enabled=False):
-                    dx = torch.matmul(g, weight).view(*gy.shape[:-1], inputs)
+            dx = g.new_empty((*gy.shape[:-1], inputs))
+            w = weight if weight.stride(1) == 1 or inputs == 1 else weight.contiguous()
         if need[1]:
-            dw = torch.empty((outputs, inputs), dtype=gy.dtype, device=gy.device)
+            dw, at = g.new_empty((outputs, inputs)), kept.data_ptr()
         if need[2]:
-            db = torch.empty(outputs, dtype=gy.dtype, device=gy.device)
-        if need[1] or need[2] or own:
-            at = 0 if kept is None or not need[1] else kept.data_ptr()
-            _linear_call(backend.lib().fa_b200_linear8_backward, g, g.shape[0], inputs, outputs,
-                         None, g, weight if own and need[0] else None, None, at,
-                         at + ctx.ranges if at else 0, None, dx if own else None, dw, db)
+            db = g.new_empty(outputs)
+        _linear_call(backend.lib().fa_b200_linear8_backward, g, g.shape[0], inputs, outputs, None,
+                     g, w, None, at, at + ctx.ranges if at else 0, None, dx, dw, db)
         return dx, dw, db
 
 
@@ -464,10 +452,9 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] 
     or float32 (under autocast its dtype), any strides; K and M at most 4194240, and
     2^27 rows.  ``x`` is packed only where the weight wants a gradient.
 
-    float16 and bfloat16 run on the tensor cores with float32 sums that are rounded
-    once, however an axis is split.  In float32 the value and the gradient of ``x``
-    are torch's products, and the weight's gradient is summed in float32 without
-    tensor cores."""
+    All products are this package's own, with float32 sums that are rounded once,
+    however an axis is split: float16 and bfloat16 on the tensor cores, float32 in
+    float32 (torch's settings for reduced precision do not matter)."""
     if torch.is_autocast_enabled("cuda"):
         to = torch.get_autocast_dtype("cuda")
         if to in _DTYPES:

@@ -30,82 +30,118 @@ int pack8_impl(const void* x, long long x_row, void* codes, void* ranges, int dt
                long long rows, int width, int device, cudaStream_t st);
 
 // ---------------------------------------------------------------------------
-// dW in float32
+// float32
 // ---------------------------------------------------------------------------
 
-// 128 outputs x 128 inputs a block, 8 x 8 a thread, in float32 on the ordinary lanes
-// (two products an instruction): the tensor cores would round the operands.  16 rows t
-// a stage; the next stage's dy and codes are on their way while this one's products
-// run.  Few tiles: the rows are cut into parts, whose sums are joined in order.
-constexpr int kWgTile = 128, kWgRows = 16;
+// All three products in float32, on the ordinary lanes (two products an instruction):
+// the tensor cores would round the operands.  D[m][n] = sum over k of A B, 128 x 128 a
+// block, 8 x 8 a thread, 16 of k a stage; the next stage is on its way while this one's
+// products run.  Few tiles: k is cut into parts, whose sums are joined in order.
+// Bound by the products: 16320 rows, 1024 x 1024, dW 0.75 ms, 46 TFLOP/s.
+constexpr int kLaneTile = 128, kLaneDepth = 16;
 
-struct WgradArgs {
-  const float* dy;
-  long long dy_row;
+struct LaneArgs {
+  const float *a, *b;           // or codes
+  long long a_row, b_row;
   const unsigned char* codes;
   const float2* ranges;
-  long long rows, per_part;     // rows of a part, whole stages
-  int inputs, outputs, groups, parts;
-  float* dw;                    // [parts][outputs][inputs]
-  int dy_vec;                   // rows of dy are whole aligned vectors of four
+  long long k, per_part;        // whole stages a part
+  int m, n, groups, parts;
+  const float* bias;            // [n] or null
+  float* d;                     // [parts][m][n]
+  int a_vec, b_vec;             // rows are whole aligned vectors of four
 };
 
-__global__ void __launch_bounds__(256, 2) wgrad_lanes_kernel(const WgradArgs a) {
-  __shared__ __align__(16) float sa[2][kWgRows][kWgTile], sb[2][kWgRows][kWgTile];
-  const int m0 = blockIdx.x * kWgTile, k0 = blockIdx.y * kWgTile;
+// How an operand lies: its tile's axis as rows with k along them, k as rows, or packed
+// rows k.
+enum LaneOperand { ALONG_K, ROWS_K, CODES_K };
+
+// 4 values of a row from column c, those past the n-th zero.
+__device__ __forceinline__ float4 four(const float* p, long long c, long long n, int vec) {
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (vec && c + 4 <= n) return __ldg(reinterpret_cast<const float4*>(p + c));
+  if (c < n) v.x = __ldg(p + c);
+  if (c + 1 < n) v.y = __ldg(p + c + 1);
+  if (c + 2 < n) v.z = __ldg(p + c + 2);
+  if (c + 3 < n) v.w = __ldg(p + c + 3);
+  return v;
+}
+
+template <LaneOperand A, LaneOperand B>
+__global__ void __launch_bounds__(256, 2) lanes_kernel(const LaneArgs a) {
+  constexpr int P = kLaneTile + 4;  // pitch: transposed stores meet two at a bank, not eight
+  __shared__ __align__(16) float sa[2][kLaneDepth][P], sb[2][kLaneDepth][P];
+  const int m0 = blockIdx.x * kLaneTile, n0 = blockIdx.y * kLaneTile;
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const long long t0 = blockIdx.z * a.per_part, t1 = min(a.rows, t0 + a.per_part);
-  // this thread's share of a stage: 2 x 4 of dy's columns, 8 codes
-  const int ra = threadIdx.x >> 5, ca = (threadIdx.x & 31) * 4;   // rows ra, ra + 8
-  const int rb = threadIdx.x >> 4, ub = threadIdx.x & 15;         // row rb, unit ub
-  const int g = k0 / kGroup8 + (ub >> 3);
-  float4 na[2];
+  const long long k0 = blockIdx.z * a.per_part, k1 = min(a.k, k0 + a.per_part);
+  // this thread's share of a stage: two vectors of four, or 8 codes
+  const int rk = threadIdx.x >> 5, ck = (threadIdx.x & 31) * 4;   // k rows rk, rk + 8
+  const int rt = threadIdx.x >> 2, ct = (threadIdx.x & 3) * 4;    // tile rows rt, rt + 64
+  const int rc = threadIdx.x >> 4, uc = threadIdx.x & 15;         // codes: k row, unit
+  float4 na[2], nb[2];
   uint2 nq;
   float2 nr;
-  const auto fetch = [&](long long t) {
+  const auto share = [&](LaneOperand how, const float* p, long long row, int i0, int size, int vec,
+                         long long k, float4 (&to)[2]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const long long r = t + ra + 8 * h;
-      na[h] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < t1) {
-        const float* p = a.dy + r * a.dy_row + m0 + ca;
-        if (a.dy_vec && m0 + ca + 4 <= a.outputs) {
-          na[h] = __ldg(reinterpret_cast<const float4*>(p));
-        } else {
-          if (m0 + ca < a.outputs) na[h].x = __ldg(p);
-          if (m0 + ca + 1 < a.outputs) na[h].y = __ldg(p + 1);
-          if (m0 + ca + 2 < a.outputs) na[h].z = __ldg(p + 2);
-          if (m0 + ca + 3 < a.outputs) na[h].w = __ldg(p + 3);
-        }
+      to[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (how == ROWS_K) {
+        if (k + rk + 8 * h < k1) to[h] = four(p + (k + rk + 8 * h) * row, i0 + ck, size, vec);
+      } else if (i0 + rt + 64 * h < size) {
+        to[h] = four(p + (i0 + rt + 64 * h) * row, k + ct, k1, vec);
       }
     }
-    nq = make_uint2(0u, 0u);
-    nr = make_float2(0.f, 0.f);
-    if (t + rb < t1 && g < a.groups) {
-      const long long at = (t + rb) * a.groups + g;
-      nq = __ldg(reinterpret_cast<const uint2*>(a.codes) + at * 8 + (ub & 7));
-      nr = __ldg(a.ranges + at);
+  };
+  const auto fetch = [&](long long k) {
+    share(A, a.a, a.a_row, m0, a.m, a.a_vec, k, na);
+    if constexpr (B != CODES_K) {
+      share(B, a.b, a.b_row, n0, a.n, a.b_vec, k, nb);
+    } else {
+      const int g = n0 / kGroup8 + (uc >> 3);
+      nq = make_uint2(0u, 0u);
+      nr = make_float2(0.f, 0.f);
+      if (k + rc < k1 && g < a.groups) {
+        const long long at = (k + rc) * a.groups + g;
+        nq = __ldg(reinterpret_cast<const uint2*>(a.codes) + at * 8 + (uc & 7));
+        nr = __ldg(a.ranges + at);
+      }
+    }
+  };
+  const auto lay = [&](LaneOperand how, float (*to)[P], const float4 (&v)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (how == ROWS_K) {
+        *reinterpret_cast<float4*>(&to[rk + 8 * h][ck]) = v[h];
+      } else {
+        to[ct][rt + 64 * h] = v[h].x;
+        to[ct + 1][rt + 64 * h] = v[h].y;
+        to[ct + 2][rt + 64 * h] = v[h].z;
+        to[ct + 3][rt + 64 * h] = v[h].w;
+      }
     }
   };
   const auto put = [&](int half) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) *reinterpret_cast<float4*>(&sa[half][ra + 8 * h][ca]) = na[h];
-    put8<float>(&sb[half][rb][ub * 8], narrow8(decode8<float>(nq, range_of(nr, 0.f)), 0.f));
+    lay(A, sa[half], na);
+    if constexpr (B != CODES_K)
+      lay(B, sb[half], nb);
+    else
+      put8<float>(&sb[half][rc][uc * 8], narrow8(decode8<float>(nq, range_of(nr, 0.f)), 0.f));
   };
   float2 acc[8][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = both(0.f);
-  fetch(t0);
+  fetch(k0);
   put(0);
   int half = 0;
-  for (long long t = t0; t < t1; t += kWgRows, half ^= 1) {
+  for (long long k = k0; k < k1; k += kLaneDepth, half ^= 1) {
     __syncthreads();
-    fetch(t + kWgRows);
+    fetch(k + kLaneDepth);
 #pragma unroll
-    for (int r = 0; r < kWgRows; ++r) {
-      // outputs ty * 4 + 0..3 and 64 on, inputs tx * 4 + 0..3 and 64 on
+    for (int r = 0; r < kLaneDepth; ++r) {
+      // rows ty * 4 + 0..3 and 64 on, columns tx * 4 + 0..3 and 64 on
       const float4 p0 = *reinterpret_cast<const float4*>(&sa[half][r][ty * 4]),
                    p1 = *reinterpret_cast<const float4*>(&sa[half][r][64 + ty * 4]),
                    q0 = *reinterpret_cast<const float4*>(&sb[half][r][tx * 4]),
@@ -117,26 +153,28 @@ __global__ void __launch_bounds__(256, 2) wgrad_lanes_kernel(const WgradArgs a) 
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = __ffma2_rn(both(p[i]), q[j], acc[i][j]);
     }
-    if (t + kWgRows < t1) put(half ^ 1);
+    if (k + kLaneDepth < k1) put(half ^ 1);
   }
-  float* const out = a.dw + (long long)blockIdx.z * a.outputs * a.inputs;
+  float* const out = a.d + (long long)blockIdx.z * a.m * a.n;
+  const float* const bias = a.parts == 1 ? a.bias : nullptr;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int m = m0 + (i >> 2) * 64 + ty * 4 + (i & 3);
-    if (m >= a.outputs) continue;
+    if (m >= a.m) continue;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int k = k0 + (j >> 2) * 64 + tx * 4 + (j & 3);
-      if (k < a.inputs) out[(long long)m * a.inputs + k] = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
+      const int n = n0 + (j >> 2) * 64 + tx * 4 + (j & 3);
+      const float v = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
+      if (n < a.n) out[(long long)m * a.n + n] = bias ? v + __ldg(bias + n) : v;
     }
   }
 }
-__global__ void __launch_bounds__(256) join_lanes_kernel(const float* part, float* dw, int parts,
-                                                         long long size) {
+__global__ void __launch_bounds__(256) join_lanes_kernel(const float* part, float* d, int parts,
+                                                         long long size, const float* bias, int n) {
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < size; i += gridDim.x * 256ll) {
     float t = 0.f;
     for (int p = 0; p < parts; ++p) t += part[p * size + i];
-    dw[i] = t;
+    d[i] = bias ? t + __ldg(bias + i % n) : t;
   }
 }
 
@@ -867,7 +905,7 @@ __global__ void __launch_bounds__(256) pitch_kernel(const T* x, long long x_row,
 
 // A tile's sum over 2^27 rows takes under a second, and a wait for it two at most.
 constexpr long long kMaxRows = 1ll << 27;
-constexpr int kMaxSide = (1 << 22) - 64;
+constexpr int kMaxSide = (1 << 22) - 64;  // 32768 tiles of 128
 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -998,12 +1036,18 @@ static LinearPlan linear_plan(const fa_linear8& l, int device) {
     p.dx_parts = parts(l.dx, rows * in, stages_of(l.outputs));
     p.dw_parts = parts(l.dweight, (long long)in * out, stages_of(l.rows));
   }
-  if (l.dtype == FA_F32 && l.dweight) {
-    // parts that fill the multiprocessors twice, of 256 rows or more
-    const long long tiles = (long long)((l.inputs + kWgTile - 1) / kWgTile) *
-                            ((l.outputs + kWgTile - 1) / kWgTile);
-    p.dw_parts = (int)std::max(1ll, std::min((long long)(l.rows + 255) / 256, 2ll * sm_count(device) / tiles));
-    if (p.dw_parts > 1) part = sizeof(float) * (size_t)p.dw_parts * l.inputs * l.outputs;
+  if (l.dtype == FA_F32) {
+    // parts that fill the multiprocessors twice, of 256 and more of k
+    const auto parts = [&](bool wanted, long long m, long long n, long long k) {
+      const long long tiles = ((m + kLaneTile - 1) / kLaneTile) * ((n + kLaneTile - 1) / kLaneTile);
+      if (!wanted) return 1;
+      const int c = (int)std::max(1ll, std::min((k + 255) / 256, 2ll * sm_count(device) / tiles));
+      if (c > 1) part = std::max(part, (size_t)(sizeof(float) * c * m * n));
+      return c;
+    };
+    p.y_parts = parts(l.y, l.rows, l.outputs, l.inputs);
+    p.dx_parts = parts(l.dx, l.rows, l.inputs, l.outputs);
+    p.dw_parts = parts(l.dweight, l.outputs, l.inputs, l.rows);
   }
   p.part = used;
   p.bytes = used + part;
@@ -1016,7 +1060,6 @@ static int linear_check(const fa_linear8* l) {
   if (l->rows <= 0 || l->inputs <= 0 || l->outputs <= 0 || l->rows > kMaxRows ||
       l->inputs > kMaxSide || l->outputs > kMaxSide)
     return FA_E_SHAPE;
-  if (l->dtype == FA_F32 && (l->y || l->dx)) return FA_E_DTYPE;
   const int item = item_size(l->dtype);
   for (const void* q : {l->x, l->dy, l->weight, l->bias, (const void*)l->y, (const void*)l->dx,
                         (const void*)l->dweight, (const void*)l->dbias})
@@ -1127,33 +1170,71 @@ static int linear_backward(const fa_linear8& l, LinearPlan& p, char* ws, int dev
   return l.dweight ? wgrad_run<T>(l, p.dy, ws + p.part, p, st) : FA_OK;
 }
 
-static int wgrad_lanes(const fa_linear8& l, const LinearPlan& p, char* ws, int device,
-                       cudaStream_t st) {
-  WgradArgs a = {};
-  a.dy = static_cast<const float*>(l.dy);
-  a.dy_row = l.dy_stride;
-  a.dy_vec = reinterpret_cast<size_t>(l.dy) % 16 == 0 && (l.rows == 1 || l.dy_stride % 4 == 0);
-  a.codes = static_cast<const unsigned char*>(l.codes);
-  a.ranges = static_cast<const float2*>(l.ranges);
-  a.rows = l.rows;
-  a.inputs = l.inputs;
-  a.outputs = l.outputs;
-  a.groups = (int)groups8(l.inputs);
-  const long long stages = (l.rows + kWgRows - 1) / kWgRows;
-  a.per_part = (stages + p.dw_parts - 1) / p.dw_parts * kWgRows;
-  a.parts = (int)((l.rows + a.per_part - 1) / a.per_part);
-  a.dw = a.parts > 1 ? reinterpret_cast<float*>(ws + p.part) : static_cast<float*>(l.dweight);
-  const dim3 grid((unsigned)((l.outputs + kWgTile - 1) / kWgTile),
-                  (unsigned)((l.inputs + kWgTile - 1) / kWgTile), (unsigned)a.parts);
-  wgrad_lanes_kernel<<<grid, 256, 0, st>>>(a);
+template <LaneOperand A, LaneOperand B>
+static int lanes_run(LaneArgs a, int parts, float* out, float* part, int device, cudaStream_t st) {
+  const long long stages = (a.k + kLaneDepth - 1) / kLaneDepth;
+  a.per_part = (stages + parts - 1) / parts * kLaneDepth;
+  a.parts = (int)((a.k + a.per_part - 1) / a.per_part);
+  a.d = a.parts > 1 ? part : out;
+  const dim3 grid((unsigned)((a.m + kLaneTile - 1) / kLaneTile),
+                  (unsigned)((a.n + kLaneTile - 1) / kLaneTile), (unsigned)a.parts);
+  lanes_kernel<A, B><<<grid, 256, 0, st>>>(a);
   FAB_LAUNCH_CHECK();
   if (a.parts > 1) {
-    const long long size = (long long)l.outputs * l.inputs;
+    const long long size = (long long)a.m * a.n;
     join_lanes_kernel<<<(unsigned)std::min((size + 255) / 256, 8ll * sm_count(device)), 256, 0, st>>>(
-        a.dw, static_cast<float*>(l.dweight), a.parts, size);
+        part, out, a.parts, size, a.bias, a.n);
     FAB_LAUNCH_CHECK();
   }
   return FA_OK;
+}
+static int whole4(const void* p, long long row, long long rows) {
+  return reinterpret_cast<size_t>(p) % 16 == 0 && (rows == 1 || row % 4 == 0);
+}
+
+static int lanes_forward(const fa_linear8& l, const LinearPlan& p, char* ws, int device,
+                         cudaStream_t st) {
+  LaneArgs a = {};
+  a.a = static_cast<const float*>(l.x);
+  a.a_row = l.x_stride;
+  a.a_vec = whole4(l.x, l.x_stride, l.rows);
+  a.b = static_cast<const float*>(l.weight);
+  a.b_row = l.weight_stride;
+  a.b_vec = whole4(l.weight, l.weight_stride, l.outputs);
+  a.k = l.inputs;
+  a.m = (int)l.rows;
+  a.n = l.outputs;
+  a.bias = static_cast<const float*>(l.bias);
+  return lanes_run<ALONG_K, ALONG_K>(a, p.y_parts, static_cast<float*>(l.y),
+                                     reinterpret_cast<float*>(ws + p.part), device, st);
+}
+
+static int lanes_backward(const fa_linear8& l, const LinearPlan& p, char* ws, int device,
+                          cudaStream_t st) {
+  LaneArgs a = {};
+  a.a = static_cast<const float*>(l.dy);
+  a.a_row = l.dy_stride;
+  a.a_vec = whole4(l.dy, l.dy_stride, l.rows);
+  if (l.dx) {
+    a.b = static_cast<const float*>(l.weight);
+    a.b_row = l.weight_stride;
+    a.b_vec = whole4(l.weight, l.weight_stride, l.outputs);
+    a.k = l.outputs;
+    a.m = (int)l.rows;
+    a.n = l.inputs;
+    if (const int rc = lanes_run<ALONG_K, ROWS_K>(a, p.dx_parts, static_cast<float*>(l.dx),
+                                                  reinterpret_cast<float*>(ws + p.part), device, st))
+      return rc;
+  }
+  if (!l.dweight) return FA_OK;
+  a.codes = static_cast<const unsigned char*>(l.codes);
+  a.ranges = static_cast<const float2*>(l.ranges);
+  a.groups = (int)groups8(l.inputs);
+  a.k = l.rows;
+  a.m = l.outputs;
+  a.n = l.inputs;
+  return lanes_run<ROWS_K, CODES_K>(a, p.dw_parts, static_cast<float*>(l.dweight),
+                                    reinterpret_cast<float*>(ws + p.part), device, st);
 }
 
 int linear8_impl(const fa_linear8* l, void* ws, size_t bytes, int device, cudaStream_t st) {
@@ -1167,6 +1248,7 @@ int linear8_impl(const fa_linear8* l, void* ws, size_t bytes, int device, cudaSt
                                   l->inputs, device, st))
       return rc;
   if (!l->y) return FA_OK;
+  if (l->dtype == FA_F32) return lanes_forward(*l, p, static_cast<char*>(ws), device, st);
   if (l->dtype == FA_F16) return linear_forward<f16_t>(*l, p, static_cast<char*>(ws), device, st);
   return linear_forward<bf16_t>(*l, p, static_cast<char*>(ws), device, st);
 }
@@ -1183,7 +1265,7 @@ int linear8_backward_impl(const fa_linear8* l, void* ws, size_t bytes, int devic
       return rc;
   if (l->dtype == FA_F16) return linear_backward<f16_t>(*l, p, static_cast<char*>(ws), device, st);
   if (l->dtype == FA_BF16) return linear_backward<bf16_t>(*l, p, static_cast<char*>(ws), device, st);
-  return l->dweight ? wgrad_lanes(*l, p, static_cast<char*>(ws), device, st) : FA_OK;
+  return lanes_backward(*l, p, static_cast<char*>(ws), device, st);
 }
 
 }  // namespace fab

@@ -187,12 +187,12 @@ def test_c_entries_refuse_before_any_launch():
     assert q(linear(inputs=7, x_stride=7, weight_stride=7), 0, ctypes.byref(size)) == 0
     assert size.value >= 2 * 256
     room = 1 << 30
-    for kw, want in (({"dtype": 4}, 1), ({"dtype": F32}, 1), ({"rows": 0}, 2), ({"inputs": 0}, 2),
+    for kw, want in (({"dtype": 4}, 1), ({"rows": 0}, 2), ({"inputs": 0}, 2),
                      ({"outputs": 1 << 23}, 2), ({"rows": (1 << 27) + 1}, 2), ({"x": None}, 5),
                      ({"weight": None}, 5), ({"x": 513}, 5), ({"y": None}, 5), ({"codes": 512}, 5),
                      ({"codes": 520, "ranges": 512}, 5), ({"dx": 512, "dy": 512}, 5)):
         assert L.fa_b200_linear8(linear(**kw), 512, room, 0, None) == want, kw
-    for kw, want in (({"dtype": F32}, 1), ({"dy": None}, 5), ({"weight": None}, 5), ({"dx": None}, 5),
+    for kw, want in (({"dy": None}, 5), ({"weight": None}, 5), ({"dx": None}, 5),
                      ({"y": 512, "x": 512}, 5), ({"dweight": 512}, 5), ({"dy": 511}, 5)):
         assert L.fa_b200_linear8_backward(linear(**{**back, **kw}), 512, room, 0, None) == want, kw
     copied = linear(**{**back, "outputs": 7, "dy_stride": 7})
