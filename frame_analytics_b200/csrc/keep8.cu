@@ -115,88 +115,101 @@ __device__ __forceinline__ float2 gelu_slope(float2 x) {
   }
 }
 
-// Bound by bytes: a thread has kUnits units at a time, whose loads are all under way
-// before the first is used, and a row's place takes one multiplication (`inv`).
+// A thread has kUnits units at a time, whose loads are all under way before the first
+// is used.  WHOLE: rows that join to one long one, and all of the block's units in it:
+// addresses are one base each, which leaves the kernels to their bytes (65280 x 4096
+// bfloat16: see the figures at rows8).  Otherwise a row's place takes one
+// multiplication (`inv`).
 constexpr int kUnits = 4;
+
+template <typename T, int OP, bool VEC, bool TANH, bool WHOLE>
+__device__ __forceinline__ void rows8_units(const Rows8& a, long long u0, Turn8<T>* turn) {
+  typedef typename RangeBits<T>::type Bits;
+  constexpr bool FAST = sizeof(T) == 2;
+  constexpr bool READS = OP == OP_UNPACK || OP == OP_GELU_GRAD;   // codes
+  const long long u1 = u0 + threadIdx.x;
+  uint2* const codes = reinterpret_cast<uint2*>(a.codes) + u1;
+  Bits* const ranges = reinterpret_cast<Bits*>(a.ranges) + u1 / 8;
+  const T* const x0 = reinterpret_cast<const T*>(a.x) + (WHOLE ? u1 * 8 : 0);
+  T* const y0 = reinterpret_cast<T*>(a.y) + (WHOLE ? u1 * 8 : 0);
+  Raw8<T> raw[kUnits];
+  uint2 code[kUnits];
+  Bits bits[kUnits];
+  int n[kUnits];
+  long long at[kUnits];         // of this unit in y
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+    const long long u = u1 + k * 256;
+    const bool in = WHOLE || u < a.units;
+    const T* from = x0 + k * 2048;
+    n[k] = 8;
+    at[k] = k * 2048;
+    if constexpr (!WHOLE) {
+      n[k] = 0;
+      at[k] = 0;
+      from = x0;
+      if (in) {
+        long long row = 0, c = u * 8;
+        n[k] = 8;
+        if (a.per_row) {
+          row = a.units <= 0x7fffffffll ? (long long)(__umulhi((unsigned)u, a.inv) >> a.shift)
+                                        : u / a.per_row;
+          c = (u - row * a.per_row) * 8;
+          n[k] = (int)max(0ll, min(8ll, a.width - c));
+        }
+        at[k] = row * a.y_row + c;
+        from = x0 + row * a.x_row + c;
+      }
+    }
+    if constexpr (READS) {
+      code[k] = in ? __ldg(codes + k * 256) : make_uint2(0u, 0u);
+      bits[k] = in ? __ldg(ranges + k * 32) : Bits();
+    }
+    if constexpr (OP != OP_UNPACK) raw[k] = fetch8<T, VEC>(from, n[k], turn);
+  }
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+    const bool in = WHOLE || u1 + k * 256 < a.units;
+    F8 x;
+    if constexpr (READS) {
+      x = decode8<T>(code[k], range_of(bits[k], T()));
+    } else {
+      x = widen8(raw[k]);
+    }
+    if constexpr (OP == OP_PACK || OP == OP_GELU_PACK) {
+      Range8 r;
+      float lo, hi;
+      extent8<VEC>(raw[k], n[k], &lo, &hi);
+      const uint2 q = encode8<T, VEC>(x, n[k], lo, hi, &r);
+      if (in) {
+        codes[k * 256] = q;
+        if ((threadIdx.x & 7) == 0) ranges[k * 32] = range_bits(r, T());
+      }
+    }
+    if constexpr (OP == OP_GELU || OP == OP_GELU_PACK) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.v[i] = gelu_value<TANH, FAST>(x.v[i]);
+    }
+    if constexpr (OP == OP_GELU_GRAD) {
+      const F8 g = widen8(raw[k]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.v[i] = __fmul2_rn(g.v[i], gelu_slope<TANH, FAST>(x.v[i]));
+    }
+    if constexpr (OP != OP_PACK) store8<T, VEC>(y0 + at[k], n[k], x, turn);
+  }
+}
 
 template <typename T, int OP, bool VEC, bool TANH>
 __global__ void __launch_bounds__(256) rows8_kernel(const Rows8 a) {
-  typedef typename RangeBits<T>::type Bits;
-  constexpr bool FAST = sizeof(T) == 2;
   __shared__ __align__(16) Turn8<T> turns[VEC ? 1 : 8];
   Turn8<T>* const turn = turns + (VEC ? 0 : threadIdx.x / 32);
   // whole warps stay together: a row is a multiple of 8 units, a warp's 32 may span rows
   const long long step = (long long)gridDim.x * (256 * kUnits);
   for (long long u0 = (long long)blockIdx.x * (256 * kUnits); u0 < a.units; u0 += step) {
-    Raw8<T> raw[kUnits];
-    uint2 code[kUnits];
-    Bits bits[kUnits];
-    int n[kUnits];
-    long long at[kUnits];       // of this unit in y
-    const T* from[kUnits];
-#pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-      const long long u = u0 + k * 256 + threadIdx.x;
-      n[k] = 0;
-      at[k] = 0;
-      from[k] = reinterpret_cast<const T*>(a.x);
-      code[k] = make_uint2(0u, 0u);
-      bits[k] = Bits();
-      if (u < a.units) {
-        long long row, c;
-        if (a.per_row == 0) {   // one long row
-          row = 0;
-          c = u * 8;
-          n[k] = 8;
-        } else {
-          row = a.units <= 0x7fffffffll
-                    ? (long long)(__umulhi((unsigned)u, a.inv) >> a.shift)
-                    : u / a.per_row;
-          c = (u - row * a.per_row) * 8;
-          n[k] = (int)max(0ll, min(8ll, a.width - c));
-        }
-        at[k] = row * a.y_row + c;
-        from[k] = reinterpret_cast<const T*>(a.x) + row * a.x_row + c;
-        if constexpr (OP == OP_UNPACK || OP == OP_GELU_GRAD) {
-          code[k] = __ldg(reinterpret_cast<const uint2*>(a.codes) + u);
-          bits[k] = __ldg(reinterpret_cast<const Bits*>(a.ranges) + u / 8);
-        }
-      }
-      if constexpr (OP != OP_UNPACK) raw[k] = fetch8<T, VEC>(from[k], n[k], turn);
-    }
-#pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-      const long long u = u0 + k * 256 + threadIdx.x;
-      const bool in = u < a.units;
-      T* const yp = reinterpret_cast<T*>(a.y) + at[k];
-      if constexpr (OP == OP_PACK || OP == OP_GELU || OP == OP_GELU_PACK) {
-        F8 x = widen8(raw[k]);
-        if constexpr (OP != OP_GELU) {
-          Range8 r;
-          float lo, hi;
-          extent8<VEC>(raw[k], n[k], &lo, &hi);
-          const uint2 q = encode8<T, VEC>(x, n[k], lo, hi, &r);
-          if (in) {
-            reinterpret_cast<uint2*>(a.codes)[u] = q;
-            if ((u & 7) == 0) reinterpret_cast<Bits*>(a.ranges)[u / 8] = range_bits(r, T());
-          }
-        }
-        if constexpr (OP != OP_PACK) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x.v[i] = gelu_value<TANH, FAST>(x.v[i]);
-          store8<T, VEC>(yp, n[k], x, turn);
-        }
-      } else {
-        F8 x = decode8<T>(code[k], range_of(bits[k], T()));
-        if constexpr (OP == OP_GELU_GRAD) {
-          const F8 g = widen8(raw[k]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            x.v[i] = __fmul2_rn(g.v[i], gelu_slope<TANH, FAST>(x.v[i]));
-        }
-        store8<T, VEC>(yp, n[k], x, turn);
-      }
-    }
+    if (VEC && a.per_row == 0 && u0 + 256 * kUnits <= a.units)
+      rows8_units<T, OP, VEC, TANH, VEC>(a, u0, turn);
+    else
+      rows8_units<T, OP, VEC, TANH, false>(a, u0, turn);
   }
 }
 
