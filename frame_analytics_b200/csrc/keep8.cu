@@ -200,7 +200,7 @@ __device__ __forceinline__ void rows8_units(const Rows8& a, long long u0, Turn8<
 }
 
 template <typename T, int OP, bool VEC, bool TANH>
-__global__ void __launch_bounds__(256) rows8_kernel(const Rows8 a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) rows8_kernel(const Rows8 a) {
   __shared__ __align__(16) Turn8<T> turns[VEC ? 1 : 8];
   Turn8<T>* const turn = turns + (VEC ? 0 : threadIdx.x / 32);
   // whole warps stay together: a row is a multiple of 8 units, a warp's 32 may span rows
