@@ -135,109 +135,144 @@ __device__ __forceinline__ float warp_sum2(float a, float b) {
 // Both passes below keep a row in the registers of `wpr` warps, E units of 256 columns
 // a warp, and read and write every byte once.  What a row costs apart from its values
 // (addresses, the joining of sums) bounds them as much as bytes do.
-template <typename T, bool VEC, int E, int NT>
-__global__ void __launch_bounds__(NT, 1024 / NT) norm_kernel(const NormArgs a, int wpr) {
-  __shared__ float sm[4][32];
+//
+// How rows lie: in any way; in whole aligned vectors; or so that every lane's units are
+// whole and weights of the operands' type lie so too, which leaves the loops without
+// conditions and with one address an operand.
+enum RowKind { ODD, VECTORS, FULL };
+
+template <typename T, RowKind KIND, int E, int NT>
+__global__ void __launch_bounds__(NT, NT > 512 ? 1 : 768 / NT) norm_kernel(const NormArgs a, int wpr) {
+  constexpr bool VEC = KIND != ODD;
+  typedef typename RangeBits<T>::type Bits;
+  __shared__ float sm[2][32];
   __shared__ __align__(16) Turn8<T> turns[VEC ? 1 : NT / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Turn8<T>* const turn = turns + (VEC ? 0 : warp);
   const int at = warp % wpr, first = warp - at;          // this warp in its row, the row's first
-  const int rpb = blockDim.x / 32 / wpr;
   const int c0 = (at * E * 32 + lane) * 8;
+  const long long row = (long long)blockIdx.x * (blockDim.x / 32 / wpr) + warp / wpr;
+  const bool in = row < a.rows;
+  if (KIND == FULL && !in) return;                       // a row of one warp: no barrier waits
   int n[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) n[e] = max(0, min(8, a.width - c0 - 256 * e));
-  const long long start = (long long)blockIdx.x * rpb + warp / wpr;
-  const long long step = (long long)gridDim.x * rpb;
-  const T* xp = reinterpret_cast<const T*>(a.x) + start * a.x_row + c0;
-  const T* rp = reinterpret_cast<const T*>(a.res) + (a.res ? start * a.res_row + c0 : 0);
-  T* yp = reinterpret_cast<T*>(a.y) + start * a.width + c0;
-  const long long to_sum = a.sum ? reinterpret_cast<T*>(a.sum) - reinterpret_cast<T*>(a.y) : 0;
-  int half = 0;
+  for (int e = 0; e < E; ++e)
+    n[e] = KIND == FULL ? 8 : in ? max(0, min(8, a.width - c0 - 256 * e)) : 0;
+  const T* const xp = reinterpret_cast<const T*>(a.x) + row * a.x_row + c0;
+  T* const yp = reinterpret_cast<T*>(a.y) + row * a.width + c0;
+  // s stays as it lies in memory and is widened for each of the three passes over it:
+  // half the registers of float32 values, so twice the rows under way
+  Raw8<T> s[E];
+  if (a.res) {
+    const T* const rp = reinterpret_cast<const T*>(a.res) + row * a.res_row + c0;
+    Raw8<T> q[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      s[e] = fetch8<T, VEC>(xp + 256 * e, n[e], turn);
+      q[e] = fetch8<T, VEC>(rp + 256 * e, n[e], turn);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      F8 x = widen8(s[e]);
+      const F8 y = widen8(q[e]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.v[i] = __fadd2_rn(x.v[i], y.v[i]);
+      s[e] = narrow8(x, T());
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[e] = fetch8<T, VEC>(xp + 256 * e, n[e], turn);
+  }
   const auto row_sum = [&](float t, int k) {
     t = warp_sum(t);
     if (wpr == 1) return t;
     if (lane == 0) sm[k][warp] = t;
-    __syncthreads();            // the next row's sums have the other buffers
+    __syncthreads();
     t = 0.f;
     for (int w = 0; w < wpr; ++w) t += sm[k][first + w];
     return t;
   };
-  long long row = start;
-  for (long long row0 = (long long)blockIdx.x * rpb; row0 < a.rows;
-       row0 += step, row += step, half ^= 2) {
-    const bool in = row < a.rows;
-    // s stays as it lies in memory and is widened for each of the three passes over it:
-    // half the registers of float32 values, so twice the rows under way
-    Raw8<T> s[E];
-    if (a.res) {
-      Raw8<T> q[E];
+  float2 t = both(0.f);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        s[e] = fetch8<T, VEC>(xp + 256 * e, in ? n[e] : 0, turn);
-        q[e] = fetch8<T, VEC>(rp + 256 * e, in ? n[e] : 0, turn);
-      }
+  for (int e = 0; e < E; ++e) {
+    const F8 x = widen8(s[e]);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        F8 x = widen8(s[e]);
-        const F8 y = widen8(q[e]);
+    for (int i = 0; i < 4; ++i) t = __fadd2_rn(t, x.v[i]);
+  }
+  const float m = mean_of(row_sum(t.x + t.y, 0), a);
+  float2 v = both(0.f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x.v[i] = __fadd2_rn(x.v[i], y.v[i]);
-        s[e] = narrow8(x, T());
-      }
-    } else {
+  for (int e = 0; e < E; ++e) {
+    if (KIND == VECTORS && n[e] == 0) continue;
+    F8 x = widen8(s[e]);
+    if (!VEC) fill_from(x, n[e], m);
 #pragma unroll
-      for (int e = 0; e < E; ++e) s[e] = fetch8<T, VEC>(xp + 256 * e, in ? n[e] : 0, turn);
+    for (int i = 0; i < 4; ++i) {
+      const float2 d = __fadd2_rn(x.v[i], both(-m));
+      v = __ffma2_rn(d, d, v);
     }
-    float2 t = both(0.f);
+  }
+  const float r = inv_sqrt(fmaf(row_sum(v.x + v.y, 1), a.inv_width, a.eps));
+  if (a.stats && in && at == 0 && lane == 0) a.stats[row] = make_float2(m, r);
+  if (a.sum) {
+    T* const sp = reinterpret_cast<T*>(a.sum) + row * a.width + c0;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const F8 x = widen8(s[e]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) t = __fadd2_rn(t, x.v[i]);
-    }
-    const float m = mean_of(row_sum(t.x + t.y, half), a);
-    float2 v = both(0.f);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (VEC && n[e] == 0) continue;
-      F8 x = widen8(s[e]);
-      if (!VEC) fill_from(x, n[e], m);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 d = __fadd2_rn(x.v[i], both(-m));
-        v = __ffma2_rn(d, d, v);
+      if constexpr (VEC) {
+        if (n[e]) put8<T>(sp + 256 * e, s[e]);
+      } else {
+        scatter8<T>(sp + 256 * e, n[e], s[e], turn);
       }
     }
-    const float r = inv_sqrt(fmaf(row_sum(v.x + v.y, half + 1), a.inv_width, a.eps));
-    if (a.stats && in && at == 0 && lane == 0) a.stats[row] = make_float2(m, r);
+  }
+  if (a.codes) {
+    uint2* const cp = reinterpret_cast<uint2*>(a.codes) + (row * a.groups * 8 + c0 / 8);
+    Bits* const bp = reinterpret_cast<Bits*>(a.ranges) + (row * a.groups + c0 / kGroup8);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int k = in ? n[e] : 0;
-      F8 x = widen8(s[e]);
-      if (a.sum) store8<T, VEC>(yp + to_sum + 256 * e, k, x, turn);
-      if (a.codes)
-        keep8<T, VEC>(a, row, c0 / 8 + 32 * e, k, in && c0 / 8 + 32 * e < a.groups * 8, x, s[e]);
-      normalise8(x, m, r);
-      if (a.w || a.b) {
-        const F8 w = weights8<T, VEC>(a, a.w, c0 + 256 * e, n[e], 1.f),
-                 b = weights8<T, VEC>(a, a.b, c0 + 256 * e, n[e], 0.f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x.v[i] = __ffma2_rn(x.v[i], w.v[i], b.v[i]);
+      Range8 range;
+      float lo, hi;
+      extent8<VEC>(s[e], n[e], &lo, &hi);
+      const uint2 q = encode8<T, VEC>(widen8(s[e]), n[e], lo, hi, &range);
+      if (KIND == FULL || (in && c0 / 8 + 32 * e < a.groups * 8)) {
+        cp[32 * e] = q;
+        if ((lane & 7) == 0) bp[4 * e] = range_bits(range, T());
       }
-      store8<T, VEC>(yp + 256 * e, k, x, turn);
     }
-    xp += step * a.x_row;
-    rp += step * a.res_row;
-    yp += step * a.width;
+  }
+  const T* const wp = reinterpret_cast<const T*>(a.w) + c0;
+  const T* const bp = reinterpret_cast<const T*>(a.b) + c0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    F8 x = widen8(s[e]);
+    normalise8(x, m, r);
+    if constexpr (KIND == FULL) {
+      if (a.w) {
+        const F8 w = widen8(get8<T>(wp + 256 * e));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.v[i] = __fmul2_rn(x.v[i], w.v[i]);
+      }
+      if (a.b) {
+        const F8 b = widen8(get8<T>(bp + 256 * e));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x.v[i] = __fadd2_rn(x.v[i], b.v[i]);
+      }
+    } else if (a.w || a.b) {
+      const F8 w = weights8<T, VEC>(a, a.w, c0 + 256 * e, n[e], 1.f),
+               b = weights8<T, VEC>(a, a.b, c0 + 256 * e, n[e], 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x.v[i] = __fadd2_rn(__fmul2_rn(x.v[i], w.v[i]), b.v[i]);
+    }
+    store8<T, VEC>(yp + 256 * e, n[e], x, turn);
   }
 }
 
 // Backward: a lane keeps the weight gradients of its columns in registers, the block
 // adds its rows' at the end and writes one part.  The next row's loads are under way
 // while a row's sums run.
-template <typename T, bool VEC, int E, bool CODES, int NT>
+template <typename T, RowKind KIND, int E, bool CODES, int NT>
 __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs a, int wpr) {
+  constexpr bool VEC = KIND != ODD;
   __shared__ float2 sm[2][NT / 32];
   __shared__ float join[NT / 32][32 * 9];
   __shared__ __align__(16) Turn8<T> turns[VEC ? 1 : NT / 32];
@@ -249,12 +284,12 @@ __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs 
   F8 dw[E], db[E];
   Raw8<T> w[E];                 // weights of the operands' type stay; others are read anew
   int n[E];
-  const bool w_kept = VEC && a.w && a.w_vec && (sizeof(T) == 4 || !a.w32);
+  const bool w_kept = VEC && a.w && (KIND == FULL || (a.w_vec && (sizeof(T) == 4 || !a.w32)));
 #pragma unroll
   for (int e = 0; e < E; ++e) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) dw[e].v[i] = db[e].v[i] = both(0.f);
-    n[e] = max(0, min(8, a.width - c0 - 256 * e));
+    n[e] = KIND == FULL ? 8 : max(0, min(8, a.width - c0 - 256 * e));
     w[e] = w_kept && n[e] ? get8<T>(reinterpret_cast<const T*>(a.w) + c0 + 256 * e) : zero8<T>();
   }
   const long long start = (long long)blockIdx.x * rpb + warp / wpr;
@@ -314,7 +349,7 @@ __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs 
     float2 c1 = both(0.f), c2 = both(0.f);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if (VEC && (!in || !n[e])) continue;
+      if (VEC && (!in || (KIND != FULL && !n[e]))) continue;
       if constexpr (CODES) h[e] = decode8<T>(now.code[e], range_of(now.bits[e], T()));
       else h[e] = widen8(now.x[e]);
       g[e] = widen8(now.g[e]);
@@ -326,7 +361,8 @@ __global__ void __launch_bounds__(NT, 512 / NT) norm_grad_kernel(const NormArgs 
         db[e].v[i] = __fadd2_rn(db[e].v[i], g[e].v[i]);
       }
       if (a.w) {
-        const F8 f = w_kept ? widen8(w[e]) : weights8<T, VEC>(a, a.w, c0 + 256 * e, n[e], 1.f);
+        const F8 f = KIND == FULL || w_kept ? widen8(w[e])
+                                            : weights8<T, VEC>(a, a.w, c0 + 256 * e, n[e], 1.f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) g[e].v[i] = __fmul2_rn(g[e].v[i], f.v[i]);
       }
@@ -679,33 +715,41 @@ static NormArgs norm_args(const fa_norm& p) {
   return a;
 }
 
-template <typename T, int E>
-static void norm_launch(const NormArgs& a, int wpr, bool vec, int device, cudaStream_t st) {
+// Rows of whole units on every lane, with weights of the operands' type that lie so.
+static RowKind kind_of(const NormArgs& a, bool vec, int item, RowShape shape) {
+  if (!vec) return ODD;
+  const bool weights = (!a.w && !a.b) || (a.w_vec && (item == 4 || !a.w32));
+  return weights && a.width == 256 * shape.wpr * shape.e ? FULL : VECTORS;
+}
+
+// Forward, a block has one row of its own: blocks that stayed and took rows in turn, two
+// a multiprocessor's worth of warps, took 342 us where these take 272 (65280 x 4096
+// bfloat16), since all of a block's warps load, sum and store at the same time.
+template <typename T, RowKind KIND, int E>
+static void norm_launch(const NormArgs& a, int wpr, cudaStream_t st) {
   const int rpb = wpr == 1 ? 4 : 1;
   const unsigned threads = 32 * wpr * rpb;
-  // Forward, a block has one row of its own: blocks that stayed and took rows in turn,
-  // two a multiprocessor's worth of warps, took 342 us where these take 272 (65280 x
-  // 4096 bfloat16), since all of a block's warps load, sum and store at the same time.
-  const unsigned grid = (unsigned)std::min((a.rows + rpb - 1) / rpb, 0x7fffffffll);
-  if (threads > 256) {
-    if (vec)
-      norm_kernel<T, true, E, 1024><<<grid, threads, 0, st>>>(a, wpr);
-    else
-      norm_kernel<T, false, E, 1024><<<grid, threads, 0, st>>>(a, wpr);
-  } else if (vec) {
-    norm_kernel<T, true, E, 256><<<grid, threads, 0, st>>>(a, wpr);
-  } else {
-    norm_kernel<T, false, E, 256><<<grid, threads, 0, st>>>(a, wpr);
-  }
+  const unsigned grid = (unsigned)((a.rows + rpb - 1) / rpb);
+  if (threads > 256)
+    norm_kernel<T, KIND, E, 1024><<<grid, threads, 0, st>>>(a, wpr);
+  else
+    norm_kernel<T, KIND, E, 256><<<grid, threads, 0, st>>>(a, wpr);
+}
+template <typename T, int E>
+static void norm_launch(const NormArgs& a, int wpr, bool vec, cudaStream_t st) {
+  const RowKind kind = kind_of(a, vec, sizeof(T), RowShape{wpr, E});
+  if (kind == FULL) norm_launch<T, FULL, E>(a, wpr, st);
+  else if (kind == VECTORS) norm_launch<T, VECTORS, E>(a, wpr, st);
+  else norm_launch<T, ODD, E>(a, wpr, st);
 }
 
 template <typename T>
 static int norm_run(const NormArgs& a, bool vec, int device, cudaStream_t st) {
   const RowShape shape = forward_shape(a.width);
-  if (shape.wpr) {
-    if (shape.e == 1) norm_launch<T, 1>(a, shape.wpr, vec, device, st);
-    else if (shape.e == 2) norm_launch<T, 2>(a, shape.wpr, vec, device, st);
-    else norm_launch<T, 4>(a, shape.wpr, vec, device, st);
+  if (shape.wpr && a.rows < 1ll << 31) {
+    if (shape.e == 1) norm_launch<T, 1>(a, shape.wpr, vec, st);
+    else if (shape.e == 2) norm_launch<T, 2>(a, shape.wpr, vec, st);
+    else norm_launch<T, 4>(a, shape.wpr, vec, st);
     FAB_LAUNCH_CHECK();
     return FA_OK;
   }
@@ -740,18 +784,24 @@ int norm_impl(const fa_norm* p, void* y, void* sum, int device, cudaStream_t st)
   FAB_FOR_TYPE(p->dtype, T, return norm_run<T>(a, vec, device, st));
 }
 
+template <typename T, int E, int NT, bool CODES>
+static void norm_grad_launch(const NormArgs& a, int wpr, RowKind kind, cudaStream_t st) {
+  const unsigned grid = (unsigned)a.splits;
+  if (kind == FULL)
+    norm_grad_kernel<T, FULL, E, CODES, NT><<<grid, NT, 0, st>>>(a, wpr);
+  else if (kind == VECTORS)
+    norm_grad_kernel<T, VECTORS, E, CODES, NT><<<grid, NT, 0, st>>>(a, wpr);
+  else
+    norm_grad_kernel<T, ODD, E, CODES, NT><<<grid, NT, 0, st>>>(a, wpr);
+}
 template <typename T, int E, int NT>
 static int norm_grad_launch(NormArgs& a, int wpr, bool vec, int device, cudaStream_t st) {
   a.splits = backward_blocks(a.rows, NT / 32 / wpr, NT, device);
-  const unsigned grid = (unsigned)a.splits;
-  if (a.codes && vec)
-    norm_grad_kernel<T, true, E, true, NT><<<grid, NT, 0, st>>>(a, wpr);
-  else if (a.codes)
-    norm_grad_kernel<T, false, E, true, NT><<<grid, NT, 0, st>>>(a, wpr);
-  else if (vec)
-    norm_grad_kernel<T, true, E, false, NT><<<grid, NT, 0, st>>>(a, wpr);
+  const RowKind kind = kind_of(a, vec, sizeof(T), RowShape{wpr, E});
+  if (a.codes)
+    norm_grad_launch<T, E, NT, true>(a, wpr, kind, st);
   else
-    norm_grad_kernel<T, false, E, false, NT><<<grid, NT, 0, st>>>(a, wpr);
+    norm_grad_launch<T, E, NT, false>(a, wpr, kind, st);
   FAB_LAUNCH_CHECK();
   return a.dw || a.db ? column_join<T>(a, st) : FA_OK;
 }
