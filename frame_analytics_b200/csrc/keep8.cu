@@ -5,7 +5,11 @@
 //   or      x (1 + tanh u) / 2,     u = sqrt(2/pi) (x + 0.044715 x^3)
 //
 // Each kernel reads its operands once and writes its outputs once; 8 lanes hold
-// a group of 64, so a group's range costs three shuffles.
+// a group of 64, so a group's range costs three shuffles.  Measured on one B200, 65280 x
+// 4096 bfloat16: packing 128 us and unpacking 130 us (0.98 and 0.96 of the copy rate),
+// gelu with packing 221 us and its gradient 222 us (0.93), the tanh form 212 us (0.98).
+// float32 gelu is bound by normcdff and expf (0.5 of the copy rate), rows that are not
+// whole vectors by their loads and stores of single values (0.35 to 0.55).
 #include <algorithm>
 
 #include "keep8.cuh"
@@ -118,8 +122,8 @@ __device__ __forceinline__ float2 gelu_slope(float2 x) {
 // A thread has kUnits units at a time, whose loads are all under way before the first
 // is used.  WHOLE: rows that join to one long one, and all of the block's units in it:
 // addresses are one base each, which leaves the kernels to their bytes (65280 x 4096
-// bfloat16: see the figures at rows8).  Otherwise a row's place takes one
-// multiplication (`inv`).
+// bfloat16: packing 143 -> 128 us, gelu 264 -> 221 us).  Otherwise a row's place takes
+// one multiplication (`inv`).
 constexpr int kUnits = 4;
 
 template <typename T, int OP, bool VEC, bool TANH, bool WHOLE>

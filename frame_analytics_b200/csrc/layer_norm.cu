@@ -11,6 +11,13 @@
 // The variance is summed about the mean (not as a difference of squares, which a
 // common offset would cancel); all sums are float32.  dw and db are summed in a
 // fixed order without atomics, so they are the same bits on every run.
+//
+// Measured on one B200, 65280 x 4096 bfloat16: forward 217 us (0.75 of the copy rate),
+// with the residual sum 317 us (1.0), with packing too 381 us (0.97); backward 377 us
+// (0.65), with the sum's gradient 407 us (0.80), from packed input 412 us (0.70).  The
+// forward pass is bound by bytes where there are more than a read and a write of each
+// value; the backward pass by the latency of joining a row's two sums, with 16 warps a
+// multiprocessor that its registers allow.
 #include <algorithm>
 
 #include "keep8.cuh"

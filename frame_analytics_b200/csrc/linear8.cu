@@ -14,7 +14,14 @@
 // a stage of 64 rows took 1000 cycles against 670 with both operands from TMA.  Every
 // value q s + lo is rounded once, as unpacking rounds it.  Where the tiles are fewer
 // than the pairs of blocks, the rows are cut into parts whose float32 sums are joined
-// in order.
+// in order.  y and dx: the same tiles, both operands by TMA.  float32: on the ordinary
+// lanes.
+//
+// Measured on one B200 at 16320 rows, 1024 inputs, 4096 outputs, bfloat16: y 115 us, dx
+// 113 us, dW 115 us (1.19 PFLOP/s each; torch's products 98, 92 and 90 us), packing 11
+// us, db 26 us.  y and dx are bound by operand bytes out of the second-level cache (11.3
+// TB/s; the tensor pipe 72 % active at 8192 x 4096 x 4096, 194 us), dW by the products
+// themselves (685 cycles for 256 x 256 x 64) and by 64 tiles for 74 pairs of blocks.
 #include <algorithm>
 #include <atomic>
 
@@ -197,6 +204,12 @@ constexpr int kRangesAt = kCodesAt + kCodeStages * kRaw;
 constexpr int kWgSmem = kRangesAt + kCodeStages * kRanges + 1024;
 constexpr int kOperandAt = 256; // columns of tensor memory: the sums', then 32 a stage
 constexpr int kPartFloats = 128 * 256;  // of one block's part of a tile
+// The tensor cores add to a sum with truncation, up to 2^-24 of it for each 16 terms and
+// always towards zero.  A sum of more than 32768 terms is therefore taken in chunks of
+// so many, each at most 6e-5 of it short on average (a quarter of float16's half step),
+// and the chunks are added with rounding: the rows of dW are cut into parts of a chunk
+// at most (chunks inside the kernel cost its writers 6 %), y and dx add their chunks.
+constexpr int kChunk = 512;     // stages
 
 // dW[n][m] = sum over t of x^[t][m] dy[t][n].
 struct ProductArgs {
@@ -784,26 +797,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
       // 16 of k further: 32 bytes along a row, or 2 groups of 8 rows
       const unsigned bs = (a.b_mn ? 2048u : 32u) >> 4;
       unsigned n = 0, tile = 0;
-      for (int item = first; work_of(a, item, &t); item += step, ++tile) {
-        const unsigned d = tmem + (tile & 1) * 256;
-        if (tile >= 2) stage_wait(&tm_empty[tile & 1], (tile / 2 - 1) & 1, a.err);
-        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        bool ready = false;
-        for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
-          const int s = n % S;
-          if (!ready) stage_wait(&full[s], (n / S) & 1, a.err);
+      for (int item = first; work_of(a, item, &t); item += step)
+        for (int c0 = t.kb0; c0 < t.kb1; c0 += kChunk, ++tile) {
+          const int c1 = min(t.kb1, c0 + kChunk);
+          const unsigned d = tmem + (tile & 1) * 256;
+          if (tile >= 2) stage_wait(&tm_empty[tile & 1], (tile / 2 - 1) & 1, a.err);
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-          const unsigned long long p = operand(smem0 + s * 2 * kHalf),
-                                   q = operand(smem0 + s * 2 * kHalf + kHalf);
+          bool ready = false;
+          for (int kb = c0; kb < c1; ++kb, ++n) {
+            const int s = n % S;
+            if (!ready) stage_wait(&full[s], (n / S) & 1, a.err);
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            const unsigned long long p = operand(smem0 + s * 2 * kHalf),
+                                     q = operand(smem0 + s * 2 * kHalf + kHalf);
 #pragma unroll
-          for (int k = 0; k < kDepth / 16; ++k) {
-            mma_f16<true>(d, p + k * (32u >> 4), q + k * bs, idesc, kb > t.kb0 || k > 0);
-            if (k == 1) ready = kb + 1 < t.kb1 && mbar_peek(&full[(n + 1) % S], ((n + 1) / S) & 1);
+            for (int k = 0; k < kDepth / 16; ++k) {
+              mma_f16<true>(d, p + k * (32u >> 4), q + k * bs, idesc, kb > c0 || k > 0);
+              if (k == 1) ready = kb + 1 < c1 && mbar_peek(&full[(n + 1) % S], ((n + 1) / S) & 1);
+            }
+            mma_commit<true>(&empty[s]);
           }
-          mma_commit<true>(&empty[s]);
+          mma_commit<true>(&tm_full[tile & 1]);
         }
-        mma_commit<true>(&tm_full[tile & 1]);
-      }
       // products still in flight end before tensor memory is given back
       mma_commit<true>(&drain);
       stage_wait(&drain, 0, a.err);
@@ -813,37 +828,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
     char* const turn = smem + kTurnAt + (warp - 4) * 2 * kTurn;
     unsigned tile = 0;
     int other = 0;
-    for (int item = first; work_of(a, item, &t); item += step, ++tile) {
-      const int buf = tile & 1;
-      if (lane == 0) stage_wait(&tm_full[buf], (tile / 2) & 1, a.err);
-      __syncwarp();
-      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-      const int i = t.i0 + rank * 128 + 32 * w;
+    for (int item = first; work_of(a, item, &t); item += step)
+      for (int c0 = t.kb0; c0 < t.kb1; c0 += kChunk, ++tile) {
+        const int buf = tile & 1, c1 = min(t.kb1, c0 + kChunk);
+        if (lane == 0) stage_wait(&tm_full[buf], (tile / 2) & 1, a.err);
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const int i = t.i0 + rank * 128 + 32 * w;
 #pragma unroll 1
-      for (int c = h * 128; c < h * 128 + 128; c += 32) {
-        float v[32];
-        tmem_load32(tmem + buf * 256 + c + ((unsigned)(32 * w) << 16), v);
-        if (c + 32 == h * 128 + 128) {
-          __syncwarp();
-          asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-          if (lane == 0) arrive_leader<true>(&tm_empty[buf]);
-        }
-        if (a.parts > 1) {  // [item][block][columns / 4][128 rows] of four columns each
+        for (int c = h * 128; c < h * 128 + 128; c += 32) {
+          float v[32];
+          tmem_load32(tmem + buf * 256 + c + ((unsigned)(32 * w) << 16), v);
+          if (c + 32 == h * 128 + 128) {
+            __syncwarp();
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+            if (lane == 0) arrive_leader<true>(&tm_empty[buf]);
+          }
+          // [item][block][columns / 4][128 rows] of four columns each
           float4* const to = reinterpret_cast<float4*>(
               a.part + ((long long)t.item * 2 + rank) * kPartFloats) + c / 4 * 128 + 32 * w + lane;
+          if (c0 > t.kb0) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            to[q * 128] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        } else if (i < a.m && t.j0 + c < a.n) {
-          add_bias<T>(a, t.j0 + c, v);
-          // the copy before the last has been read out of this half
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");
-          __syncwarp();
-          put_result<T>(a, i, t.j0 + c, v, turn + other * kTurn);
-          other ^= 1;
+            for (int q = 0; q < 8; ++q) {
+              const float4 f = to[q * 128];
+              v[4 * q] += f.x;
+              v[4 * q + 1] += f.y;
+              v[4 * q + 2] += f.z;
+              v[4 * q + 3] += f.w;
+            }
+          }
+          if (a.parts > 1 || c1 < t.kb1) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              to[q * 128] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+          } else if (i < a.m && t.j0 + c < a.n) {
+            add_bias<T>(a, t.j0 + c, v);
+            // the copy before the last has been read out of this half
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");
+            __syncwarp();
+            put_result<T>(a, i, t.j0 + c, v, turn + other * kTurn);
+            other ^= 1;
+          }
         }
       }
-    }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
@@ -885,17 +912,26 @@ __global__ void __launch_bounds__(128) join_rows_kernel(const __grid_constant__ 
     if (j + q < a.n) out[q] = St<T>::v(b ? v[q] + Ld<T>::f(ldro(b + j + q)) : v[q]);
 }
 
-// Rows at a pitch of whole 16 bytes, for TMA.
+// Rows at a pitch of whole 16 bytes, for TMA: a warp a row, 8 of a lane's columns at a
+// time, zeros in the pitch's last columns.
 template <typename T>
 __global__ void __launch_bounds__(256) pitch_kernel(const T* x, long long x_row, T* y, int pitch,
                                                     long long rows, int width) {
-  const long long n = rows * pitch;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-    const long long r = i / pitch;
-    const int c = (int)(i - r * pitch);
-    T v = T();
-    if (c < width) v = ldro(x + r * x_row + c);
-    y[i] = v;
+  const int lane = threadIdx.x & 31;
+  for (long long r = blockIdx.x * 8ll + threadIdx.x / 32; r < rows; r += gridDim.x * 8ll) {
+    const T* const from = x + r * x_row;
+    T* const to = y + r * pitch;
+    for (int c0 = lane; c0 < pitch; c0 += 256) {
+      T v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = T();
+        if (c0 + 32 * i < width) v[i] = ldro(from + c0 + 32 * i);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (c0 + 32 * i < pitch) to[c0 + 32 * i] = v[i];
+    }
   }
 }
 
@@ -903,7 +939,6 @@ __global__ void __launch_bounds__(256) pitch_kernel(const T* x, long long x_row,
 // host
 // ---------------------------------------------------------------------------
 
-// A tile's sum over 2^27 rows takes under a second, and a wait for it two at most.
 constexpr long long kMaxRows = 1ll << 27;
 constexpr int kMaxSide = (1 << 22) - 64;  // 32768 tiles of 128
 
@@ -932,14 +967,14 @@ static int tiles_of(long long n) { return (int)((n + kTile - 1) / kTile); }
 
 // Parts of the sum's axis: the number whose waves take the least time, at 0.42 us a
 // stage of a pair, 6 us a tile's end, and the parts' trip through memory.
-static int parts_of(int tiles, int kb, int pairs) {
-  int best = 1;
+static int parts_of(long long tiles, int kb, int pairs, int least_parts) {
+  int best = least_parts;
   double least = 0;
-  for (int p = 1; p <= 32 && p <= kb; ++p) {
-    const double waves = (double)((tiles * (long long)p + pairs - 1) / pairs);
+  for (int p = least_parts; p < least_parts + 32 && p <= kb; ++p) {
+    const double waves = (double)((tiles * p + pairs - 1) / pairs);
     double us = waves * (0.42 * ((kb + p - 1) / p) + 6.0);
     if (p > 1) us += 4.0 + tiles * (double)p * 2 * kPartFloats * 4 * 2 / 4e6;
-    if (p == 1 || us < least) {
+    if (p == least_parts || us < least) {
       least = us;
       best = p;
     }
@@ -997,8 +1032,7 @@ static int ready_operand(Operand* o, char* ws, long long stride, int device, cud
   if (!o->copied) return FA_OK;
   const int pitch = pitch_of(o->cols);
   T* const copy = reinterpret_cast<T*>(ws + o->copy);
-  const long long blocks =
-      std::min((o->rows * pitch + 255) / 256, (long long)sm_count(device) * 16);
+  const long long blocks = std::min((o->rows + 7) / 8, (long long)sm_count(device) * 16);
   pitch_kernel<T><<<(unsigned)blocks, 256, 0, st>>>(static_cast<const T*>(o->p), stride, copy,
                                                     pitch, o->rows, o->cols);
   FAB_LAUNCH_CHECK();
@@ -1026,15 +1060,22 @@ static LinearPlan linear_plan(const fa_linear8& l, int device) {
     p.pairs = resident_pairs(device);
     const int in = tiles_of(l.inputs), out = tiles_of(l.outputs);
     const long long rows = tiles_of(l.rows);
+    const auto room = [&](long long tiles, int n) {
+      part = std::max(part, (size_t)tiles * n * 2 * kPartFloats * sizeof(float));
+    };
     const auto parts = [&](bool wanted, long long tiles, int kb) {
-      if (!wanted || tiles > p.pairs) return 1;
-      const int n = parts_of((int)tiles, kb, p.pairs);
-      if (n > 1) part = std::max(part, (size_t)tiles * n * 2 * kPartFloats * sizeof(float));
+      const int n = !wanted || tiles > p.pairs ? 1 : parts_of(tiles, kb, p.pairs, 1);
+      if (wanted && (n > 1 || kb > kChunk)) room(tiles, n);
       return n;
     };
     p.y_parts = parts(l.y, rows * out, stages_of(l.inputs));
     p.dx_parts = parts(l.dx, rows * in, stages_of(l.outputs));
-    p.dw_parts = parts(l.dweight, (long long)in * out, stages_of(l.rows));
+    if (l.dweight) {
+      const long long tiles = (long long)in * out;
+      const int kb = stages_of(l.rows), chunks = (kb + kChunk - 1) / kChunk;
+      p.dw_parts = tiles > p.pairs ? chunks : parts_of(tiles, kb, p.pairs, chunks);
+      if (p.dw_parts > 1) room(tiles, p.dw_parts);
+    }
   }
   if (l.dtype == FA_F32) {
     // parts that fill the multiprocessors twice, of 256 and more of k

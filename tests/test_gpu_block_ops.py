@@ -952,3 +952,30 @@ def test_the_example_runs_with_kept_activations_and_its_gradients_are_close():
         # each kept value is off by at most 1/255 of the range of 64: under 2 % of its
         # deviation, and the same operators exactly otherwise
         assert float((a.double() - b.double()).norm()) <= 0.05 * float(b.double().norm())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_sums_of_many_terms_of_one_sign(dtype):
+    """Longer than one chunk of a tensor-core sum, whose additions truncate."""
+    x = rand(1_100_000, 16, seed=120).abs().to(dtype)
+    gy = (2.0 ** -10 * rand(1_100_000, 24, seed=121).abs()).to(dtype)
+    w = rand(24, 16, seed=122, dtype=dtype).requires_grad_(True)
+    b = rand(24, seed=123, dtype=dtype).requires_grad_(True)
+    dw, db = torch.autograd.grad(fa.linear8(x, w, b), (w, b), gy)
+    kept = fa.unpack8(fa.pack8(x)).double()
+    for got, want in ((dw, gy.double().T @ kept), (db, gy.double().sum(0))):
+        # chunks of 32768 terms: 2048 additions, each at most 2^-24 of the sum short;
+        # column sums: a few thousand rounded additions
+        tol = (U[dtype] + 2048 * E) * want.abs()
+        within(got, want, (1 + 2 * U[dtype]) * tol, dtype)
+
+
+def test_products_over_more_inputs_than_a_chunk():
+    x = rand(5000, 33000, seed=124, dtype=torch.bfloat16)
+    w = rand(1000, 33000, seed=125, dtype=torch.bfloat16)
+    y = fa.linear8(x, w)
+    check_product(y[::7], x[::7], w, None, torch.bfloat16)
+    leaf = x[:200].clone().requires_grad_(True)
+    gy = rand(200, 1000, seed=126, dtype=torch.bfloat16)
+    dx, = torch.autograd.grad(fa.linear8(leaf, w), leaf, gy)
+    check_product(dx, gy, w.mT, None, torch.bfloat16)
