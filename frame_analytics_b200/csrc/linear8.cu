@@ -227,16 +227,16 @@ struct ProductArgs {
 struct Work {
   int i0, j0, kb0, kb1, item;
 };
-// Items are numbered part by part; inside a part eight rows of tiles are walked
+// ROWS of a tile.  Items are numbered part by part; inside a part eight rows of tiles are walked
 // column by column, so the tiles at work share operand panels in the L2 cache.
-template <typename Args>
+template <int ROWS = kTile, typename Args>
 __device__ __forceinline__ bool work_of(const Args& a, int item, Work* w) {
   const int tiles = a.tiles_m * a.tiles_n;
   if (item >= tiles * a.parts) return false;
   const int part = item / tiles, tile = item - part * tiles;
   const int band = tile / (8 * a.tiles_n), in = tile - band * 8 * a.tiles_n;
   const int high = min(8, a.tiles_m - band * 8);
-  w->i0 = (band * 8 + in % high) * kTile;
+  w->i0 = (band * 8 + in % high) * ROWS;
   w->j0 = in / high * kTile;
   w->kb0 = (int)((long long)a.kb * part / a.parts);
   w->kb1 = (int)((long long)a.kb * (part + 1) / a.parts);
@@ -655,12 +655,14 @@ __global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__
 // ---------------------------------------------------------------------------
 
 // D[m][n] = sum over k of A[m][k] B[n][k] (+ bias[n]): A with k along its rows, B so or
-// with k as its rows (b_mn).  The same tiles of a pair of blocks; both operands by TMA,
-// two accumulators in turn, eight warps that write the one while the other is summed.
-constexpr int kPlainStages = 6;
+// with k as its rows (b_mn).  Both operands by TMA, eight warps that write the result.  A
+// pair of blocks has 256 x 256 of it, with two accumulators in turn, so that one is
+// written while the other is summed; or (TALL) 512 x 256, which takes three quarters of
+// the operand bytes a product, but all of tensor memory, so that writing shows.  Operand
+// bytes out of the second-level cache bound these products.
 constexpr int kPlainThreads = 128 + 32 * kWriters;
 constexpr int kTurn = 2048;     // bytes of 32 x 32 of the result; two a warp
-constexpr int kTurnAt = kPlainStages * 2 * kHalf;
+constexpr int kTurnAt = 12 * kHalf;  // 6 stages of 2 x 128 rows of operands, or 4 of 3
 constexpr int kPlainSmem = kTurnAt + kWriters * 2 * kTurn + 1024;
 
 struct PlainArgs {
@@ -726,10 +728,11 @@ __device__ __forceinline__ void put_result(const PlainArgs& a, int i, int j, con
   }
 }
 
-template <typename T>
+template <typename T, bool TALL>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
     product_kernel(const __grid_constant__ PlainArgs a) {
-  constexpr int S = kPlainStages;
+  constexpr int R = TALL ? 2 : 1;              // blocks of 128 rows of A in either block
+  constexpr int S = TALL ? 4 : 6, kStage = (R + 1) * kHalf, ROWS = R * kTile;
   extern __shared__ char smem_raw[];
   const unsigned smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
   char* const smem = smem_raw + (smem0 - smem_u32(smem_raw));
@@ -767,20 +770,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
   if (warp == 0) {
     if (lane == 0) {
       unsigned n = 0;
-      for (int item = first; work_of(a, item, &t); item += step) {
+      for (int item = first; work_of<ROWS>(a, item, &t); item += step) {
         const int ia = t.i0 + rank * 128, jb = t.j0 + rank * 128;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
           const int s = n % S;
           if (n >= (unsigned)S) stage_wait(&empty[s], (n / S - 1) & 1, a.err);
           // both blocks' copies count on the first block's barrier
-          const unsigned bar = in_leader(smem_u32(&full[s])), to = smem0 + s * 2 * kHalf;
-          if (rank == 0) mbar_expect_tx(&full[s], 4 * kHalf);
+          const unsigned bar = in_leader(smem_u32(&full[s])), to = smem0 + s * kStage;
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * kStage);
+#pragma unroll
+          for (int i = 0; i < 2 * R; ++i)
+            tma_box<true>(to + i * kBox, &a.a, kb * kDepth, ia + (i >> 1) * 256 + (i & 1) * 64, 0,
+                          bar);
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            tma_box<true>(to + i * kBox, &a.a, kb * kDepth, ia + 64 * i, 0, bar);
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            tma_box<true>(to + kHalf + i * kBox, &a.b, a.b_mn ? jb + 64 * i : kb * kDepth,
+            tma_box<true>(to + R * kHalf + i * kBox, &a.b, a.b_mn ? jb + 64 * i : kb * kDepth,
                           a.b_mn ? kb * kDepth : jb + 64 * i, 0, bar);
         }
       }
@@ -797,27 +801,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
       // 16 of k further: 32 bytes along a row, or 2 groups of 8 rows
       const unsigned bs = (a.b_mn ? 2048u : 32u) >> 4;
       unsigned n = 0, tile = 0;
-      for (int item = first; work_of(a, item, &t); item += step)
+      for (int item = first; work_of<ROWS>(a, item, &t); item += step)
         for (int c0 = t.kb0; c0 < t.kb1; c0 += kChunk, ++tile) {
           const int c1 = min(t.kb1, c0 + kChunk);
-          const unsigned d = tmem + (tile & 1) * 256;
-          if (tile >= 2) stage_wait(&tm_empty[tile & 1], (tile / 2 - 1) & 1, a.err);
+          const unsigned d = TALL ? tmem : tmem + (tile & 1) * 256;
+          if (TALL && tile >= 1) stage_wait(&tm_empty[0], (tile - 1) & 1, a.err);
+          if (!TALL && tile >= 2) stage_wait(&tm_empty[tile & 1], (tile / 2 - 1) & 1, a.err);
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
           bool ready = false;
           for (int kb = c0; kb < c1; ++kb, ++n) {
             const int s = n % S;
             if (!ready) stage_wait(&full[s], (n / S) & 1, a.err);
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-            const unsigned long long p = operand(smem0 + s * 2 * kHalf),
-                                     q = operand(smem0 + s * 2 * kHalf + kHalf);
+            const unsigned long long p = operand(smem0 + s * kStage),
+                                     q = operand(smem0 + s * kStage + R * kHalf);
 #pragma unroll
             for (int k = 0; k < kDepth / 16; ++k) {
-              mma_f16<true>(d, p + k * (32u >> 4), q + k * bs, idesc, kb > c0 || k > 0);
+#pragma unroll
+              for (int r = 0; r < R; ++r)
+                mma_f16<true>(d + r * 256, p + r * (kHalf >> 4) + k * (32u >> 4), q + k * bs, idesc,
+                              kb > c0 || k > 0);
               if (k == 1) ready = kb + 1 < c1 && mbar_peek(&full[(n + 1) % S], ((n + 1) / S) & 1);
             }
             mma_commit<true>(&empty[s]);
           }
-          mma_commit<true>(&tm_full[tile & 1]);
+          mma_commit<true>(&tm_full[TALL ? 0 : tile & 1]);
         }
       // products still in flight end before tensor memory is given back
       mma_commit<true>(&drain);
@@ -828,40 +836,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
     char* const turn = smem + kTurnAt + (warp - 4) * 2 * kTurn;
     unsigned tile = 0;
     int other = 0;
-    for (int item = first; work_of(a, item, &t); item += step)
+    for (int item = first; work_of<ROWS>(a, item, &t); item += step)
       for (int c0 = t.kb0; c0 < t.kb1; c0 += kChunk, ++tile) {
-        const int buf = tile & 1, c1 = min(t.kb1, c0 + kChunk);
-        if (lane == 0) stage_wait(&tm_full[buf], (tile / 2) & 1, a.err);
+        const int buf = TALL ? 0 : tile & 1, c1 = min(t.kb1, c0 + kChunk);
+        if (lane == 0) stage_wait(&tm_full[buf], (TALL ? tile : tile / 2) & 1, a.err);
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        const int i = t.i0 + rank * 128 + 32 * w;
 #pragma unroll 1
-        for (int c = h * 128; c < h * 128 + 128; c += 32) {
+        for (int g = 0; g < 4 * R; ++g) {
+          const int c = h * 128 + (g & 3) * 32, i = t.i0 + (g >> 2) * 256 + rank * 128 + 32 * w;
           float v[32];
-          tmem_load32(tmem + buf * 256 + c + ((unsigned)(32 * w) << 16), v);
-          if (c + 32 == h * 128 + 128) {
+          tmem_load32(tmem + (buf + (g >> 2)) * 256 + c + ((unsigned)(32 * w) << 16), v);
+          if (g + 1 == 4 * R) {
             __syncwarp();
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             if (lane == 0) arrive_leader<true>(&tm_empty[buf]);
           }
-          // [item][block][columns / 4][128 rows] of four columns each
-          float4* const to = reinterpret_cast<float4*>(
-              a.part + ((long long)t.item * 2 + rank) * kPartFloats) + c / 4 * 128 + 32 * w + lane;
-          if (c0 > t.kb0) {
+          if constexpr (!TALL) {
+            // [item][block][columns / 4][128 rows] of four columns each
+            float4* const to = reinterpret_cast<float4*>(
+                a.part + ((long long)t.item * 2 + rank) * kPartFloats) + c / 4 * 128 + 32 * w + lane;
+            if (c0 > t.kb0) {
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-              const float4 f = to[q * 128];
-              v[4 * q] += f.x;
-              v[4 * q + 1] += f.y;
-              v[4 * q + 2] += f.z;
-              v[4 * q + 3] += f.w;
+              for (int q = 0; q < 8; ++q) {
+                const float4 f = to[q * 128];
+                v[4 * q] += f.x;
+                v[4 * q + 1] += f.y;
+                v[4 * q + 2] += f.z;
+                v[4 * q + 3] += f.w;
+              }
+            }
+            if (a.parts > 1 || c1 < t.kb1) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                to[q * 128] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+              continue;
             }
           }
-          if (a.parts > 1 || c1 < t.kb1) {
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              to[q * 128] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-          } else if (i < a.m && t.j0 + c < a.n) {
+          if (i < a.m && t.j0 + c < a.n) {
             add_bias<T>(a, t.j0 + c, v);
             // the copy before the last has been read out of this half
             if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");
@@ -1125,6 +1137,16 @@ static int workspace_check(const LinearPlan& p, const void* ws, size_t bytes) {
 }
 
 // D (rows x cols) = A (rows x depth) B: B with depth along its rows, or as its rows.
+// Whether the taller tiles take less time: waves of tiles, at 0.40 us a stage and 2 us a
+// tile's end against 0.69 and 6.  Measured, bfloat16: 18944 rows, 4096 -> 1024, 2 waves
+// of tall tiles 105 us, 4 of low ones 115; 18944 rows, 512 -> 2048, 4 waves 54 us, 8 49.
+static bool tall_pays(long long rows, int cols, int kb, int pairs) {
+  if (kb > kChunk) return false;
+  const long long wide = tiles_of(cols);
+  const auto waves = [&](long long row_tiles) { return (row_tiles * wide + pairs - 1) / pairs; };
+  return waves((rows + 511) / 512) * (0.69 * kb + 6.0) < waves((rows + 255) / 256) * (0.40 * kb + 2.0);
+}
+
 template <typename T>
 static int product_run(const Operand& x, const Operand& w, int depth, bool w_mn, const void* bias,
                        void* out, long long rows, int cols, int parts, char* part,
@@ -1148,10 +1170,19 @@ static int product_run(const Operand& x, const Operand& w, int depth, bool w_mn,
   a.part = reinterpret_cast<float*>(part);
   a.err = wait_error_word();
   if (!a.err) return FA_E_INTERNAL;  // a wait that gave up could not be reported
-  FAB_TRY(cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               kPlainSmem));
+  if (parts == 1 && tall_pays(rows, cols, a.kb, plan.pairs)) {
+    a.tiles_m = (int)((rows + 511) / 512);
+    FAB_TRY(cudaFuncSetAttribute(product_kernel<T, true>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kPlainSmem));
+    product_kernel<T, true><<<2 * std::min(a.tiles_m * a.tiles_n, plan.pairs), kPlainThreads,
+                              kPlainSmem, st>>>(a);
+    FAB_LAUNCH_CHECK();
+    return FA_OK;
+  }
+  FAB_TRY(cudaFuncSetAttribute(product_kernel<T, false>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, kPlainSmem));
   const int items = a.tiles_m * a.tiles_n * parts;
-  product_kernel<T><<<2 * std::min(items, plan.pairs), kPlainThreads, kPlainSmem, st>>>(a);
+  product_kernel<T, false><<<2 * std::min(items, plan.pairs), kPlainThreads, kPlainSmem, st>>>(a);
   FAB_LAUNCH_CHECK();
   if (parts > 1) {
     join_rows_kernel<T><<<(unsigned)(a.tiles_m * a.tiles_n * 32), 128, 0, st>>>(a);

@@ -523,6 +523,8 @@ LINEARS = [
     (300, 64, 3000, True),
     (2500, 300, 20, False),
     (1030, 1100, 2056, True),
+    (9990, 1304, 700, True),   # tall tiles: two waves of low ones
+    (9990, 700, 1304, False),  # the same for dx
 ]
 
 
