@@ -17,10 +17,10 @@
 // in order.  y and dx: the same tiles, both operands by TMA.  float32: on the ordinary
 // lanes.
 //
-// Measured on one B200 at 16320 rows, 1024 inputs, 4096 outputs, bfloat16: y 115 us, dx
-// 113 us, dW 115 us (1.19 PFLOP/s each; torch's products 98, 92 and 90 us), packing 11
+// Measured on one B200 at 16320 rows, 1024 inputs, 4096 outputs, bfloat16: y 113 us, dx
+// 98 us, dW 114 us (1.2 to 1.4 PFLOP/s; torch's products 99, 94 and 90 us), packing 11
 // us, db 26 us.  y and dx are bound by operand bytes out of the second-level cache (11.3
-// TB/s; the tensor pipe 72 % active at 8192 x 4096 x 4096, 194 us), dW by the products
+// TB/s; the tensor pipe 72 % active at 8192 x 4096 x 4096, 189 us), dW by the products
 // themselves (685 cycles for 256 x 256 x 64) and by 64 tiles for 74 pairs of blocks.
 #include <algorithm>
 #include <atomic>
@@ -661,9 +661,9 @@ __global__ void __launch_bounds__(128) join_parts_kernel(const __grid_constant__
 // the operand bytes a product, but all of tensor memory, so that writing shows.  Operand
 // bytes out of the second-level cache bound these products.
 constexpr int kPlainThreads = 128 + 32 * kWriters;
-constexpr int kTurn = 2048;     // bytes of 32 x 32 of the result; two a warp
+constexpr int kTurn = 4096;     // bytes of a warp's 32 x 64 of the result
 constexpr int kTurnAt = 12 * kHalf;  // 6 stages of 2 x 128 rows of operands, or 4 of 3
-constexpr int kPlainSmem = kTurnAt + kWriters * 2 * kTurn + 1024;
+constexpr int kPlainSmem = kTurnAt + kWriters * kTurn + 1024;
 
 struct PlainArgs {
   CUtensorMap a, b, d;
@@ -677,37 +677,48 @@ struct PlainArgs {
   unsigned* err;
 };
 
-// A warp's 32 rows x 32 columns of the result at (i, j), a row a lane.
+// The biases of a warp's 128 columns from j, four a lane, fetched while the tile's sum is
+// still running; and added to the 64 values of the columns' half `g`.
 template <typename T>
-__device__ __forceinline__ void add_bias(const PlainArgs& a, int j, float (&v)[32]) {
-  if (!a.bias) return;
-  const T* b = reinterpret_cast<const T*>(a.bias) + j;
-  if (a.bias_vec && j + 32 <= a.n) {
+__device__ __forceinline__ uint2 fetch_bias(const PlainArgs& a, int j) {
+  j += 4 * (threadIdx.x & 31);
+  const T* const b = reinterpret_cast<const T*>(a.bias) + j;
+  if (a.bias_vec && j + 4 <= a.n) return __ldg(reinterpret_cast<const uint2*>(b));
+  float v[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const F8 x = widen8(get8<T>(b + 8 * q));
+  for (int i = 0; i < 4; ++i) v[i] = j + i < a.n ? Ld<T>::f(ldro(b + i)) : 0.f;
+  return make_uint2(narrow2(make_float2(v[0], v[1]), T()), narrow2(make_float2(v[2], v[3]), T()));
+}
+template <typename T>
+__device__ __forceinline__ void add_bias(uint2 bias, int g, float (&v)[64]) {
 #pragma unroll
-      for (int c = 0; c < 8; ++c) v[8 * q + c] += x.at(c);
-    }
-  } else {
-#pragma unroll
-    for (int c = 0; c < 32; ++c)
-      if (j + c < a.n) v[c] += Ld<T>::f(ldro(b + c));
+  for (int q = 0; q < 16; ++q) {
+    const float2 x = widen2(__shfl_sync(0xffffffffu, bias.x, 16 * g + q), T()),
+                 y = widen2(__shfl_sync(0xffffffffu, bias.y, 16 * g + q), T());
+    v[4 * q] += x.x;
+    v[4 * q + 1] += x.y;
+    v[4 * q + 2] += y.x;
+    v[4 * q + 3] += y.y;
   }
 }
-// `turn` is 2 KB of shared memory of the warp's own: rows of 64 bytes in the 64-byte
-// swizzle, whose copy to memory is under way when this returns.
+// A warp's 32 rows x 64 columns of the result at (i, j), a row a lane.  `turn` is 4 KB of
+// shared memory of the warp's own: rows of 128 bytes in the 128-byte swizzle, whose copy
+// to memory is under way when this returns.  (Rows of 64 bytes, two buffers in turn: 47
+// against 45 us for 18944 rows, 512 -> 2048 bfloat16.)
 template <typename T>
-__device__ __forceinline__ void put_result(const PlainArgs& a, int i, int j, const float (&v)[32],
+__device__ __forceinline__ void put_result(const PlainArgs& a, int i, int j, const float (&v)[64],
                                            char* turn) {
   const int lane = threadIdx.x & 31;
+  unsigned o[32];
 #pragma unroll
-  for (int q = 0; q < 4; ++q)
-    *reinterpret_cast<uint4*>(turn + lane * 64 + ((q ^ (lane >> 1)) & 3) * 16) = make_uint4(
-        narrow2(make_float2(v[8 * q], v[8 * q + 1]), T()),
-        narrow2(make_float2(v[8 * q + 2], v[8 * q + 3]), T()),
-        narrow2(make_float2(v[8 * q + 4], v[8 * q + 5]), T()),
-        narrow2(make_float2(v[8 * q + 6], v[8 * q + 7]), T()));
+  for (int q = 0; q < 32; ++q) o[q] = narrow2(make_float2(v[2 * q], v[2 * q + 1]), T());
+  // the buffer's last copy has been read out of it
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 8; ++q)
+    *reinterpret_cast<uint4*>(turn + lane * 128 + ((q ^ lane) & 7) * 16) =
+        make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
   if (a.tma_out) {
     fence_async_smem();
     __syncwarp();
@@ -720,10 +731,13 @@ __device__ __forceinline__ void put_result(const PlainArgs& a, int i, int j, con
   } else {
     __syncwarp();
     T* const out = reinterpret_cast<T*>(a.out) + (long long)i * a.n + j + lane;
-    if (j + lane < a.n)
-      for (int r = 0; r < min(32, a.m - i); ++r)
-        out[(long long)r * a.n] = *reinterpret_cast<const T*>(
-            turn + r * 64 + (((lane >> 3) ^ (r >> 1)) & 3) * 16 + (lane & 7) * 2);
+    for (int r = 0; r < min(32, a.m - i); ++r) {
+#pragma unroll
+      for (int c = 0; c < 64; c += 32)
+        if (j + lane + c < a.n)
+          out[(long long)r * a.n + c] = *reinterpret_cast<const T*>(
+              turn + r * 128 + ((((lane + c) >> 3) ^ r) & 7) * 16 + (lane & 7) * 2);
+    }
     __syncwarp();
   }
 }
@@ -833,21 +847,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
     }
   } else if (warp >= 4) {
     const int w = warp & 3, h = (warp - 4) >> 2;
-    char* const turn = smem + kTurnAt + (warp - 4) * 2 * kTurn;
+    char* const turn = smem + kTurnAt + (warp - 4) * kTurn;
     unsigned tile = 0;
-    int other = 0;
     for (int item = first; work_of<ROWS>(a, item, &t); item += step)
       for (int c0 = t.kb0; c0 < t.kb1; c0 += kChunk, ++tile) {
         const int buf = TALL ? 0 : tile & 1, c1 = min(t.kb1, c0 + kChunk);
+        const uint2 bias = a.bias ? fetch_bias<T>(a, t.j0 + h * 128) : make_uint2(0u, 0u);
         if (lane == 0) stage_wait(&tm_full[buf], (TALL ? tile : tile / 2) & 1, a.err);
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
 #pragma unroll 1
-        for (int g = 0; g < 4 * R; ++g) {
-          const int c = h * 128 + (g & 3) * 32, i = t.i0 + (g >> 2) * 256 + rank * 128 + 32 * w;
-          float v[32];
-          tmem_load32(tmem + (buf + (g >> 2)) * 256 + c + ((unsigned)(32 * w) << 16), v);
-          if (g + 1 == 4 * R) {
+        for (int g = 0; g < 2 * R; ++g) {
+          const int c = h * 128 + (g & 1) * 64, i = t.i0 + (g >> 1) * 256 + rank * 128 + 32 * w;
+          float v[64];
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            tmem_load32(tmem + (buf + (g >> 1)) * 256 + c + 32 * q + ((unsigned)(32 * w) << 16),
+                        *reinterpret_cast<float(*)[32]>(v + 32 * q));
+          if (g + 1 == 2 * R) {
             __syncwarp();
             asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
             if (lane == 0) arrive_leader<true>(&tm_empty[buf]);
@@ -858,7 +875,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
                 a.part + ((long long)t.item * 2 + rank) * kPartFloats) + c / 4 * 128 + 32 * w + lane;
             if (c0 > t.kb0) {
 #pragma unroll
-              for (int q = 0; q < 8; ++q) {
+              for (int q = 0; q < 16; ++q) {
                 const float4 f = to[q * 128];
                 v[4 * q] += f.x;
                 v[4 * q + 1] += f.y;
@@ -868,18 +885,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
             }
             if (a.parts > 1 || c1 < t.kb1) {
 #pragma unroll
-              for (int q = 0; q < 8; ++q)
+              for (int q = 0; q < 16; ++q)
                 to[q * 128] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
               continue;
             }
           }
           if (i < a.m && t.j0 + c < a.n) {
-            add_bias<T>(a, t.j0 + c, v);
-            // the copy before the last has been read out of this half
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;\n" ::: "memory");
-            __syncwarp();
-            put_result<T>(a, i, t.j0 + c, v, turn + other * kTurn);
-            other ^= 1;
+            if (a.bias) add_bias<T>(bias, g & 1, v);
+            put_result<T>(a, i, t.j0 + c, v, turn);
           }
         }
       }
@@ -957,8 +970,7 @@ constexpr int kMaxSide = (1 << 22) - 64;  // 32768 tiles of 128
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // [rows][pitch bytes] of 16-bit values in boxes of 64 x 64 in the 128-byte swizzle.
-// Outside arrives as zeros.  BYTES: boxes of 128 bytes; RESULT: of 32 x 32 in the
-// 64-byte swizzle.
+// Outside arrives as zeros.  BYTES: boxes of 128 bytes; RESULT: 32 rows high.
 enum BoxKind { BOX, BYTES, RESULT };
 static bool box_map(CUtensorMap* map, const void* p, long long rows, long long cols,
                     long long pitch, BoxKind kind) {
@@ -967,12 +979,11 @@ static bool box_map(CUtensorMap* map, const void* p, long long rows, long long c
   const cuuint64_t dim[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1};
   const cuuint64_t stride[2] = {(cuuint64_t)pitch, (cuuint64_t)(pitch * rows)};
   const cuuint32_t one[3] = {1, 1, 1};
-  const cuuint32_t box[3] = {kind == BOX ? 64u : kind == BYTES ? 128u : 32u,
-                             kind == RESULT ? 32u : 64u, 1};
+  const cuuint32_t box[3] = {kind == BYTES ? 128u : 64u, kind == RESULT ? 32u : 64u, 1};
   return fn(map, kind == BYTES ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3,
             const_cast<void*>(p), dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            kind == RESULT ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 static int tiles_of(long long n) { return (int)((n + kTile - 1) / kTile); }
