@@ -54,12 +54,6 @@ template <> struct Over<bf16_t> {
   static __device__ __forceinline__ float v() { return __uint_as_float(0x7f7f8000u); }
 };
 
-// A value rounded to T, as float32.
-template <typename T>
-__device__ __forceinline__ float round_to(float f) {
-  return Ld<T>::f(St<T>::v(f));
-}
-
 // The range of one group.
 struct Range8 {
   float lo, s;
@@ -215,13 +209,17 @@ template <typename T>
 struct Turn8 {
   T v[256];
 };
-// Whether the warp's values follow one another from lane 0's place; then how many.
+// Whether the warp's values follow one another from lane 0's place; then how many.  Lanes
+// whose values are fewer than 8 come last: rows padded to whole groups lie 8 values a lane
+// too, but with gaps between them.
 template <typename T>
 __device__ __forceinline__ bool one_run(const T* p, int n, const T** first, int* count) {
   const unsigned long long at = reinterpret_cast<unsigned long long>(p);
   *first = reinterpret_cast<const T*>(__shfl_sync(0xffffffffu, at, 0));
   *count = __reduce_add_sync(0xffffffffu, n);
-  return __all_sync(0xffffffffu, n == 0 || p == *first + (threadIdx.x & 31) * 8);
+  const unsigned any = __ballot_sync(0xffffffffu, n > 0), all = __ballot_sync(0xffffffffu, n == 8);
+  return (any & (any + 1u)) == 0u && ((any ^ all) & (any >> 1)) == 0u &&
+         __all_sync(0xffffffffu, n == 0 || p == *first + (threadIdx.x & 31) * 8);
 }
 template <typename T>
 __device__ __forceinline__ Raw8<T> gather8(const T* p, int n, Turn8<T>* t) {

@@ -981,3 +981,25 @@ def test_products_over_more_inputs_than_a_chunk():
     gy = rand(200, 1000, seed=126, dtype=torch.bfloat16)
     dx, = torch.autograd.grad(fa.linear8(leaf, w), leaf, gy)
     check_product(dx, gy, w.mT, None, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width,pitch", [(939, 960), (57, 64), (1, 64), (65, 128), (63, 64), (8, 64),
+                                         (200, 256), (939, 968), (57, 60)])
+def test_rows_padded_to_a_pitch(width, pitch, dtype):
+    """Rows at a pitch of whole groups: neighbouring lanes' places then lie 8 values apart
+    across the gaps, too."""
+    x = rand(41, pitch, seed=140, dtype=dtype)[:, :width]
+    g = rand(41, pitch, seed=141, dtype=dtype)[:, :width]
+    got, want = fa.pack8(x), fa.pack8(x.contiguous())
+    assert torch.equal(got.codes, want.codes) and torch.equal(got.ranges, want.ranges)
+    assert torch.equal(fa.gelu8(x), fa.gelu8(x.contiguous()))
+    w = rand(24, width, seed=142, dtype=dtype)
+    results = []
+    for a, b in ((x, g), (x.contiguous(), g.contiguous())):
+        leaf, wl = a.detach().requires_grad_(True), w.clone().requires_grad_(True)
+        dx, = torch.autograd.grad(fa.gelu8(leaf), leaf, b)
+        dn, = torch.autograd.grad(fa.layer_norm(leaf, keep8=True), leaf, b)
+        dw, = torch.autograd.grad(fa.linear8(leaf, wl), wl, b[:, :1].expand(41, 24))
+        results.append((dx, dn, dw))
+    assert all(torch.equal(p, q) for p, q in zip(*results))
