@@ -255,6 +255,8 @@ class _LayerNorm(torch.autograd.Function):
 def _check_affine(name: str, w: Optional[torch.Tensor], x: torch.Tensor) -> None:
     if w is None:
         return
+    if not torch.is_tensor(w):
+        raise TypeError(f"{name} must be a tensor or None, got {type(w).__name__}")
     if w.dtype not in (x.dtype, torch.float32):
         raise TypeError(f"{name} must be {x.dtype} or float32, got {w.dtype}")
     if tuple(w.shape) != (x.shape[-1],):
@@ -280,6 +282,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     ``keep8``: keep ``x`` (or ``s``) for the backward pass as :func:`pack8` holds
     it, with the exact mean and deviation, instead of itself."""
     _check_values("x", x, _MAX_WIDTH)
+    if residual is not None and not torch.is_tensor(residual):
+        raise TypeError(f"residual must be a tensor or None, got {type(residual).__name__}")
     if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
         raise ValueError(f"residual must be {x.dtype} of shape {tuple(x.shape)}, got "
                          f"{residual.dtype} {tuple(residual.shape)}")
@@ -471,6 +475,8 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] 
     outputs = weight.shape[0]
     if not 1 <= outputs <= _MAX_SIDE:
         raise ValueError(f"the weight must have 1..{_MAX_SIDE} rows, got {outputs}")
+    if bias is not None and not torch.is_tensor(bias):
+        raise TypeError(f"bias must be a tensor or None, got {type(bias).__name__}")
     if bias is not None and (tuple(bias.shape) != (outputs,) or bias.dtype != x.dtype):
         raise ValueError(f"bias must be {x.dtype} of shape ({outputs},), got {bias.dtype} "
                          f"{tuple(bias.shape)}")

@@ -643,8 +643,11 @@ static int backward_blocks(long long rows, int rpb, int threads, int device) {
   return (int)std::min((rows + rpb - 1) / rpb, (long long)(512 / threads) * sm_count(device));
 }
 
+// Room for the column sums' parts, or for a part a block where rows fit a block's registers.
 size_t norm_ws_bytes(long long rows, int width, int device) {
-  const int parts = std::max(column_splits(rows, width, device), 2 * sm_count(device));
+  long long parts = column_splits(rows, width, device);
+  if (backward_shape(width, 2).wpr)
+    parts = std::max(parts, std::min(rows, 2ll * sm_count(device)));
   return (size_t)parts * 2 * (size_t)width * sizeof(float);
 }
 
@@ -730,8 +733,9 @@ static RowKind kind_of(const NormArgs& a, bool vec, int item, RowShape shape) {
 }
 
 // Forward, a block has one row of its own: blocks that stayed and took rows in turn, two
-// a multiprocessor's worth of warps, took 342 us where these take 272 (65280 x 4096
-// bfloat16), since all of a block's warps load, sum and store at the same time.
+// a multiprocessor's worth of warps, took 342 us where these took 272 (65280 x 4096
+// bfloat16, both on the path of VECTORS; FULL takes 217), since all of a block's warps
+// load, sum and store at the same time.
 template <typename T, RowKind KIND, int E>
 static void norm_launch(const NormArgs& a, int wpr, cudaStream_t st) {
   const int rpb = wpr == 1 ? 4 : 1;

@@ -49,6 +49,8 @@ def test_rows_past_the_limits_are_refused():
     ({"x": torch.zeros(3, 8).half(), "weight": torch.ones(8), "bias": torch.ones(8).half()},
      ValueError),
     ({"bias": torch.ones(9)}, ValueError),
+    ({"bias": [0.0] * 8}, TypeError),
+    ({"residual": 1.0}, TypeError),
     ({"residual": torch.zeros(8)}, ValueError),                  # no broadcast
     ({"residual": torch.zeros(3, 8).half()}, ValueError),
     ({"eps": -1e-5}, ValueError),
@@ -76,6 +78,7 @@ def test_gelu8_refuses_other_forms():
     ({"weight": torch.zeros(0, 8)}, ValueError),
     ({"weight": None}, ValueError),
     ({"bias": torch.zeros(4)}, ValueError),
+    ({"bias": 0.0}, TypeError),
     ({"bias": torch.zeros(5).half()}, ValueError),
 ])
 def test_linear8_refuses(kw, exc):

@@ -983,6 +983,34 @@ def test_products_over_more_inputs_than_a_chunk():
     check_product(dx, gy, w.mT, None, torch.bfloat16)
 
 
+def test_wide_rows_take_a_workspace_of_their_own_size():
+    """Parts of the column sums as there are rows for, not as there are multiprocessors."""
+    x = rand(3, 1 << 22, seed=130, dtype=torch.bfloat16).requires_grad_(True)
+    w = rand(1 << 22, seed=131).requires_grad_(True)
+    y = fa.layer_norm(x, w)
+    gy = torch.ones_like(y)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    _, dw = torch.autograd.grad(y, (x, w), gy)
+    assert torch.cuda.max_memory_allocated() - before <= 8 * x.numel() * x.element_size()
+    mean, var = x.detach().double().mean(1, True), x.detach().double().var(1, False, keepdim=True)
+    want = ((x.detach().double() - mean) / (var + 1e-5).sqrt()).sum(0)
+    # mean and variance of 2^22 float32 terms, 2^14 in a lane's row: 2^14 steps each, of
+    # which the values, below 8, take all, and then three additions of them
+    assert float((dw.double() - want).abs().max()) <= 3 * 8 * 2.0 ** 14 * E + 8 * 4 * E
+
+    inputs = rand(3, 8, seed=132, dtype=torch.bfloat16)
+    weight = rand(1 << 21, 8, seed=133, dtype=torch.bfloat16)
+    bias = torch.zeros(1 << 21, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    y = fa.linear8(inputs, weight, bias)
+    gy = torch.ones_like(y)
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    db, = torch.autograd.grad(y, bias, gy)
+    assert torch.cuda.max_memory_allocated() - before <= 8 * y.numel() * y.element_size()
+    assert torch.equal(db, torch.full_like(db, 3.0))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("width,pitch", [(939, 960), (57, 64), (1, 64), (65, 128), (63, 64), (8, 64),
                                          (200, 256), (939, 968), (57, 60)])
