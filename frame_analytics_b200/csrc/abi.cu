@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <new>
 #include <utility>
 #include <array>
 #include <atomic>
@@ -117,6 +118,53 @@ static bool view_ok(const fa_view* v) {
   return v && v->data && v->w > 0 && v->h > 0 && v->c > 0 && v->n > 0;
 }
 
+
+static std::atomic<Side*> g_side[64];
+
+static void side_free(Side* s) {
+  if (!s) return;
+  if (s->begin) cudaEventDestroy(s->begin);
+  if (s->end) cudaEventDestroy(s->end);
+  if (s->stream) cudaStreamDestroy(s->stream);
+  delete s;
+}
+
+Side* side_fork(int device, cudaStream_t st) {
+  if (device < 0 && cudaGetDevice(&device) != cudaSuccess) device = 64;
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  if (device >= 64 || cudaStreamIsCapturing(st, &cap) != cudaSuccess ||
+      cap != cudaStreamCaptureStatusNone) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  Side* s = g_side[device].exchange(nullptr);
+  if (!s) {
+    s = new (std::nothrow) Side;
+    if (!s) return nullptr;
+    if (cudaStreamCreateWithFlags(&s->stream, cudaStreamNonBlocking) != cudaSuccess ||
+        cudaEventCreateWithFlags(&s->begin, cudaEventDisableTiming) != cudaSuccess ||
+        cudaEventCreateWithFlags(&s->end, cudaEventDisableTiming) != cudaSuccess) {
+      cudaGetLastError();
+      side_free(s);
+      return nullptr;
+    }
+  }
+  if (cudaEventRecord(s->begin, st) != cudaSuccess ||
+      cudaStreamWaitEvent(s->stream, s->begin, 0) != cudaSuccess) {
+    cudaGetLastError();
+    side_free(s);
+    return nullptr;
+  }
+  return s;
+}
+
+int side_join(Side* s, int device, cudaStream_t st) {
+  if (device < 0 && cudaGetDevice(&device) != cudaSuccess) device = 0;
+  int rc = status_of(cudaEventRecord(s->end, s->stream));
+  if (!rc) rc = status_of(cudaStreamWaitEvent(st, s->end, 0));
+  side_free(g_side[device].exchange(s));
+  return rc;
+}
 
 // The bounded waits' error word.  Pinned, mapped host memory: the kernels
 // store to it without a copy back, and the host reads it without a

@@ -170,6 +170,18 @@ unsigned int* wait_error_word();
 // call, else FA_OK.  Never allocates.
 int take_wait_error();
 
+// A stream beside a call's own, for work that the call's other kernels leave room for.
+// It serves one call at a time; one is kept for each device.
+struct Side {
+  cudaStream_t stream = nullptr;
+  cudaEvent_t begin = nullptr, end = nullptr;
+};
+// A stream that follows `st`; null where one is not to be had, or where `st` is
+// being captured (a kept stream would join the capture).
+Side* side_fork(int device, cudaStream_t st);
+// What was launched on `s` since, as seen by `st`.
+int side_join(Side* s, int device, cudaStream_t st);
+
 // Host-side request for the squared-difference outputs of the fused SSIM
 // forward (SSIM + MSE/PSNR from one read of the frame pair).
 struct SqOut {

@@ -44,7 +44,7 @@ int pack8_impl(const void* x, long long x_row, void* codes, void* ranges, int dt
 // the tensor cores would round the operands.  D[m][n] = sum over k of A B, 128 x 128 a
 // block, 8 x 8 a thread, 16 of k a stage; the next stage is on its way while this one's
 // products run.  Few tiles: k is cut into parts, whose sums are joined in order.
-// Bound by the products: 16320 rows, 1024 x 1024, dW 0.75 ms, 46 TFLOP/s.
+// Bound by the products: 16320 rows, 1024 x 1024, dW 0.80 ms, 43 TFLOP/s.
 constexpr int kLaneTile = 128, kLaneDepth = 16;
 
 struct LaneArgs {
@@ -1242,15 +1242,37 @@ static int linear_forward(const fa_linear8& l, LinearPlan& p, char* ws, int devi
                         ws + p.part, p, st);
 }
 
+static int bias_run(const fa_linear8& l, void* ws, size_t bytes, int device, cudaStream_t st) {
+  return bias_grad_impl(l.dy, l.dy_stride, l.dbias, l.dtype, l.rows, l.outputs, ws, bytes, device, st);
+}
+// Whether the bias's gradient runs beside dW: where dW's tiles leave multiprocessors idle,
+// and dy is large enough to be worth a second stream's host time.  All gradients, bfloat16,
+// beside and after one another: 16320 rows, 1024 -> 4096, 219 and 252 us; 65280 rows,
+// 256 -> 256, 70 and 84 us; 510 rows, 1024 -> 4096, 45 and 53 us.
+static bool bias_beside(const fa_linear8& l, const LinearPlan& p) {
+  const long long items = (long long)tiles_of(l.inputs) * tiles_of(l.outputs) * p.dw_parts;
+  return items <= p.pairs - 6 && l.rows * l.outputs >= 1 << 20;
+}
+
 template <typename T>
-static int linear_backward(const fa_linear8& l, LinearPlan& p, char* ws, int device, cudaStream_t st) {
+static int linear_backward(const fa_linear8& l, LinearPlan& p, char* ws, size_t bytes, bool beside,
+                           int device, cudaStream_t st) {
   if (const int rc = ready_operand<T>(&p.dy, ws, l.dy_stride, device, st)) return rc;
   if (const int rc = ready_operand<T>(&p.w, ws, l.weight_stride, device, st)) return rc;
   if (l.dx)
     if (const int rc = product_run<T>(p.dy, p.w, l.outputs, true, nullptr, l.dx, l.rows, l.inputs,
                                       p.dx_parts, ws + p.part, p, st))
       return rc;
-  return l.dweight ? wgrad_run<T>(l, p.dy, ws + p.part, p, st) : FA_OK;
+  if (!l.dweight) return FA_OK;
+  if (!beside) return wgrad_run<T>(l, p.dy, ws + p.part, p, st);
+  Side* const side = side_fork(device, st);
+  int rc = wgrad_run<T>(l, p.dy, ws + p.part, p, st);
+  if (!rc) rc = bias_run(l, ws, bytes, device, side ? side->stream : st);
+  if (side) {
+    const int joined = side_join(side, device, st);
+    if (!rc) rc = joined;
+  }
+  return rc;
 }
 
 template <LaneOperand A, LaneOperand B>
@@ -1342,13 +1364,13 @@ int linear8_backward_impl(const fa_linear8* l, void* ws, size_t bytes, int devic
   LinearPlan p = linear_plan(*l, device);
   if (const int rc = workspace_check(p, ws, bytes)) return rc;
   FAB_DEVICE_SCOPE(device);
-  if (l->dbias)
-    if (const int rc = bias_grad_impl(l->dy, l->dy_stride, l->dbias, l->dtype, l->rows, l->outputs,
-                                      ws, bytes, device, st))
-      return rc;
-  if (l->dtype == FA_F16) return linear_backward<f16_t>(*l, p, static_cast<char*>(ws), device, st);
-  if (l->dtype == FA_BF16) return linear_backward<bf16_t>(*l, p, static_cast<char*>(ws), device, st);
-  return lanes_backward(*l, p, static_cast<char*>(ws), device, st);
+  char* const work = static_cast<char*>(ws);
+  const bool beside = l->dbias && l->dweight && l->dtype != FA_F32 && bias_beside(*l, p);
+  if (l->dbias && !beside)
+    if (const int rc = bias_run(*l, ws, bytes, device, st)) return rc;
+  if (l->dtype == FA_F16) return linear_backward<f16_t>(*l, p, work, bytes, beside, device, st);
+  if (l->dtype == FA_BF16) return linear_backward<bf16_t>(*l, p, work, bytes, beside, device, st);
+  return lanes_backward(*l, p, work, device, st);
 }
 
 }  // namespace fab

@@ -1524,63 +1524,6 @@ static int ns_run(NsArgs& a, int device, cudaStream_t st) {
   return ns_products<SPLIT, false, T>(a, sms, st);
 }
 
-// Where a list holds both kinds, its one-block matrices run on a stream of their
-// own beside the tiled ones: 3 x 64 x 64 with 6 x 64 x 576 and 4 x 180 x 180,
-// bfloat16, take 105 us so, and 157 us one kind after the other.  A stream serves
-// one call at a time; one is kept for each device.
-struct Side {
-  cudaStream_t stream = nullptr;
-  cudaEvent_t begin = nullptr, end = nullptr;
-};
-static std::atomic<Side*> g_side[64];
-
-static void side_free(Side* s) {
-  if (!s) return;
-  if (s->begin) cudaEventDestroy(s->begin);
-  if (s->end) cudaEventDestroy(s->end);
-  if (s->stream) cudaStreamDestroy(s->stream);
-  delete s;
-}
-
-// A stream that follows `st`; null where one is not to be had, or where `st` is
-// being captured (a kept stream would join the capture).
-static Side* side_fork(int device, cudaStream_t st) {
-  if (device < 0 && cudaGetDevice(&device) != cudaSuccess) device = 64;
-  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  if (device >= 64 || cudaStreamIsCapturing(st, &cap) != cudaSuccess ||
-      cap != cudaStreamCaptureStatusNone) {
-    cudaGetLastError();
-    return nullptr;
-  }
-  Side* s = g_side[device].exchange(nullptr);
-  if (!s) {
-    s = new (std::nothrow) Side;
-    if (!s) return nullptr;
-    if (cudaStreamCreateWithFlags(&s->stream, cudaStreamNonBlocking) != cudaSuccess ||
-        cudaEventCreateWithFlags(&s->begin, cudaEventDisableTiming) != cudaSuccess ||
-        cudaEventCreateWithFlags(&s->end, cudaEventDisableTiming) != cudaSuccess) {
-      cudaGetLastError();
-      side_free(s);
-      return nullptr;
-    }
-  }
-  if (cudaEventRecord(s->begin, st) != cudaSuccess ||
-      cudaStreamWaitEvent(s->stream, s->begin, 0) != cudaSuccess) {
-    cudaGetLastError();
-    side_free(s);
-    return nullptr;
-  }
-  return s;
-}
-
-static int side_join(Side* s, int device, cudaStream_t st) {
-  if (device < 0 && cudaGetDevice(&device) != cudaSuccess) device = 0;
-  int rc = status_of(cudaEventRecord(s->end, s->stream));
-  if (!rc) rc = status_of(cudaStreamWaitEvent(st, s->end, 0));
-  side_free(g_side[device].exchange(s));
-  return rc;
-}
-
 // The matrices that fit one block, each.
 static int ns_blocks(NsArgs& a, const fa_matrix* mats, int count, int dtype, bool update,
                      cudaStream_t st) {
@@ -1652,6 +1595,9 @@ int ns_impl(const fa_matrix* mats, int count, int dtype, const double* coef, int
   a.joins = a.failed + 1;
   a.parts = reinterpret_cast<float*>(static_cast<char*>(ws) + up256(kNsHead));
   // tiled matrices need a workspace: both kinds are in the list
+  // Where a list holds both kinds, its one-block matrices run on a stream of their own
+  // beside the tiled ones: 3 x 64 x 64 with 6 x 64 x 576 and 4 x 180 x 180, bfloat16,
+  // take 105 us so, and 157 us one kind after the other.
   Side* side = need > kNsNoWs && small ? side_fork(device, st) : nullptr;
   int rc = ns_blocks(a, mats, count, dtype, update, side ? side->stream : st);
   if (!rc) rc = ns_tiles(a, mats, count, dtype, update, static_cast<char*>(ws), device, st);

@@ -1031,3 +1031,30 @@ def test_rows_padded_to_a_pitch(width, pitch, dtype):
         dw, = torch.autograd.grad(fa.linear8(leaf, wl), wl, b[:, :1].expand(41, 24))
         results.append((dx, dn, dw))
     assert all(torch.equal(p, q) for p, q in zip(*results))
+
+
+@pytest.mark.parametrize("rows,inputs,outputs", [(510, 1024, 4096), (9001, 200, 264), (4080, 256, 1000)])
+def test_a_bias_gradient_beside_the_weights_is_the_same_bits(rows, inputs, outputs):
+    """The two run at the same time where there is room; alone, and in a graph, they do not."""
+    x, g = (rand(rows, n, seed=150, dtype=torch.bfloat16) for n in (inputs, outputs))
+    w = rand(outputs, inputs, seed=151, dtype=torch.bfloat16).requires_grad_(True)
+    b = rand(outputs, seed=152, dtype=torch.bfloat16).requires_grad_(True)
+    alone = [torch.autograd.grad(fa.linear8(x, w, b), t, g)[0] for t in (w, b)]
+    for _ in range(10):
+        dw, db = torch.autograd.grad(fa.linear8(x, w, b), (w, b), g)
+        # the results' memory is free for others when the call returns
+        y = fa.linear8(x, w.detach(), b.detach())
+        assert torch.equal(dw, alone[0]) and torch.equal(db, alone[1])
+        del dw, db, y
+    # the sum of at most 9001 rows is off by t (a row's additions pass through no more than
+    # 4096 roundings), and its rounding to the dtype by U of what it then is: U (|sum| + t)
+    want, t = g.double().sum(0), 4096 * E * g.double().abs().sum(0)
+    within(alone[1], want, t + U[torch.bfloat16] * (want.abs() + t), torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        dw, db = torch.autograd.grad(fa.linear8(x, w, b), (w, b), g)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(dw, alone[0]) and torch.equal(db, alone[1])
