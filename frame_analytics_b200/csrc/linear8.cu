@@ -46,6 +46,7 @@ int pack8_impl(const void* x, long long x_row, void* codes, void* ranges, int dt
 // products run.  Few tiles: k is cut into parts, whose sums are joined in order.
 // Bound by the products: 16320 rows, 1024 x 1024, dW 0.80 ms, 43 TFLOP/s.
 constexpr int kLaneTile = 128, kLaneDepth = 16;
+constexpr long long kLongest = 32768;  // terms of a part
 
 struct LaneArgs {
   const float *a, *b;           // or codes
@@ -1101,11 +1102,13 @@ static LinearPlan linear_plan(const fa_linear8& l, int device) {
     }
   }
   if (l.dtype == FA_F32) {
-    // parts that fill the multiprocessors twice, of 256 and more of k
+    // parts that fill the multiprocessors twice, of 256 and more of k; none longer than
+    // 32768, so that the roundings of a long sum do not add up
     const auto parts = [&](bool wanted, long long m, long long n, long long k) {
       const long long tiles = ((m + kLaneTile - 1) / kLaneTile) * ((n + kLaneTile - 1) / kLaneTile);
       if (!wanted) return 1;
-      const int c = (int)std::max(1ll, std::min((k + 255) / 256, 2ll * sm_count(device) / tiles));
+      const int c = (int)std::max((k + kLongest - 1) / kLongest,
+                                  std::min((k + 255) / 256, 2ll * sm_count(device) / tiles));
       if (c > 1) part = std::max(part, (size_t)(sizeof(float) * c * m * n));
       return c;
     };

@@ -1058,3 +1058,18 @@ def test_a_bias_gradient_beside_the_weights_is_the_same_bits(rows, inputs, outpu
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(dw, alone[0]) and torch.equal(db, alone[1])
+
+
+def test_float32_sums_of_many_terms_of_one_sign():
+    """More tiles than run at once: the rows' parts are there for the sum's sake alone."""
+    rows = 200_001
+    x = (1.0 + rand(rows, 1, seed=160).abs()).expand(rows, 2560).contiguous()
+    g = (1.0 + rand(rows, 1, seed=161).abs()).expand(rows, 2048).contiguous()
+    w = rand(2048, 2560, seed=162).requires_grad_(True)
+    dw, = torch.autograd.grad(fa.linear8(x, w), w, g)
+    kept = fa.unpack8(fa.pack8(x[:, :1].contiguous())).double()
+    want = (g[:, :1].double() * kept).sum()
+    # parts of at most 32768 terms, each addition off by E of the part's sum at most: on
+    # average half of it, as the sum grows evenly; 7 additions of parts, one a product's
+    tol = (0.51 * 32768 + 32 + 7) * E * float(want)
+    assert float((dw.double() - want).abs().max()) <= tol
