@@ -975,16 +975,11 @@ static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 enum BoxKind { BOX, BYTES, RESULT };
 static bool box_map(CUtensorMap* map, const void* p, long long rows, long long cols,
                     long long pitch, BoxKind kind) {
-  EncodeTiledFn fn = encode_tiled();
-  if (!fn) return false;
-  const cuuint64_t dim[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 1};
-  const cuuint64_t stride[2] = {(cuuint64_t)pitch, (cuuint64_t)(pitch * rows)};
-  const cuuint32_t one[3] = {1, 1, 1};
-  const cuuint32_t box[3] = {kind == BYTES ? 128u : 64u, kind == RESULT ? 32u : 64u, 1};
-  return fn(map, kind == BYTES ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 3,
-            const_cast<void*>(p), dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_map(map,
+                    kind == BYTES ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, p,
+                    {(cuuint64_t)cols, (cuuint64_t)rows, 1},
+                    {(cuuint64_t)pitch, (cuuint64_t)(pitch * rows)},
+                    {kind == BYTES ? 128u : 64u, kind == RESULT ? 32u : 64u, 1});
 }
 
 static int tiles_of(long long n) { return (int)((n + kTile - 1) / kTile); }

@@ -1141,14 +1141,9 @@ __global__ void __launch_bounds__(256) ns_small_kernel(const __grid_constant__ N
 // [batch][rows][pitch] float16 with `cols` live columns; boxes of 64 x 64.
 // Elements outside arrive as zeros.
 static bool half_map(CUtensorMap* map, __half* p, int batch, int rows, int cols, int pitch) {
-  EncodeTiledFn fn = encode_tiled();
-  if (!fn) return false;
-  const cuuint64_t dim[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch};
-  const cuuint64_t stride[2] = {(cuuint64_t)pitch * 2, (cuuint64_t)pitch * 2 * rows};
-  const cuuint32_t box[3] = {64, 64, 1}, one[3] = {1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p, dim, stride, box, one,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, p,
+                    {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)batch},
+                    {(cuuint64_t)pitch * 2, (cuuint64_t)pitch * 2 * rows}, {64, 64, 1});
 }
 
 static constexpr size_t kNsHead = sizeof(double) * kMats * kNormBlocks + 4 * (3 * kMats + 1 + 2 * kSplitTiles);

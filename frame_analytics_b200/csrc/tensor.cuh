@@ -122,5 +122,23 @@ static EncodeTiledFn encode_tiled() {
   }();
   return fn;
 }
+// A tensor map in three dimensions, in the 128-byte swizzle; outside arrives as zeros.
+static bool encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* p,
+                       const cuuint64_t (&dim)[3], const cuuint64_t (&stride)[2],
+                       const cuuint32_t (&box)[3]) {
+  const EncodeTiledFn fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint32_t one[3] = {1, 1, 1};
+  const auto encode = [&] {
+    return fn(map, type, 3, const_cast<void*>(p), dim, stride, box, one,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (encode()) return true;
+  // The driver's call wants a context, which a thread that has launched nothing yet does
+  // not have (autograd's, in the first backward pass); setting its device gives it one.
+  int device;
+  return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && encode();
+}
 
 }  // namespace fab

@@ -1073,3 +1073,38 @@ def test_float32_sums_of_many_terms_of_one_sign():
     # average half of it, as the sum grows evenly; 7 additions of parts, one a product's
     tol = (0.51 * 32768 + 32 + 7) * E * float(want)
     assert float((dw.double() - want).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("what", ["value", "gradient"])
+def test_a_thread_may_make_its_first_call_here(what):
+    """A thread that has launched nothing has no context of its own yet."""
+    import textwrap
+    from conftest import REPO
+    code = textwrap.dedent(f"""
+        import sys, threading, torch
+        sys.path.insert(0, {str(REPO)!r})
+        import frame_analytics_b200 as fa
+        x, gy = (torch.randn(256, 128, device="cuda").bfloat16() for _ in range(2))
+        w = torch.randn(128, 128, device="cuda").bfloat16().requires_grad_({what == "gradient"})
+        q = fa.orthogonalize(x)
+        got = []
+        if {what == "gradient"}:             # autograd's own thread
+            grad, = torch.autograd.grad(fa.linear8(x, w), w, gy)
+            got.append(torch.equal(grad, torch.autograd.grad(fa.linear8(x, w), w, gy)[0]))
+        else:
+            y = fa.linear8(x, w)
+            spare = [torch.empty_like(y) for _ in range(4)]
+            del spare                        # the allocator has what the threads take
+            calls = ((lambda: fa.linear8(x, w), y), (lambda: fa.orthogonalize(x), q))
+            def run(call, want):
+                a = call()
+                got.append(torch.equal(a, want))
+            for call in calls:
+                t = threading.Thread(target=run, args=call)
+                t.start()
+                t.join()
+        assert len(got) == (1 if {what == "gradient"} else 2) and all(got), got
+        print("same")
+    """)
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and "same" in out.stdout, out.stderr
