@@ -250,32 +250,46 @@ __device__ __forceinline__ bool work_of(const Args& a, int item, Work* w) {
 // when the waiting warps polled in a loop), so a poll may suspend its warp until the
 // phase completes, or up to 2 ms.  The error word, in host memory, is looked at once in
 // 16 such polls.
+// PAIR: threads of the pair's other block arrive at the barrier, too, so that what is
+// acquired is the whole cluster's.
+template <bool PAIR>
 __device__ __forceinline__ bool mbar_sleep(unsigned a, unsigned parity) {
   unsigned done;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
-      " selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(done)
-      : "r"(a), "r"(parity), "r"(2000000u)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(a), "r"(parity), "r"(2000000u)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(done)
+        : "r"(a), "r"(parity), "r"(2000000u)
+        : "memory");
   return done != 0;
 }
 // Whether a phase is complete, without waiting.
 __device__ __forceinline__ bool mbar_peek(unsigned long long* bar, unsigned parity) {
   unsigned done;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "{\n .reg .pred p;\n"
+      " mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
       " selp.u32 %0, 1, 0, p;\n}\n"
       : "=r"(done)
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
   return done != 0;
 }
+template <bool PAIR>
 static __device__ __noinline__ void stage_wait_slow(unsigned a, unsigned parity, unsigned* err) {
   const unsigned long long t0 = globaltimer_ns();
   unsigned long long next = 1000000ull;
   for (unsigned i = 1;; ++i) {
-    if (mbar_sleep(a, parity)) return;
+    if (mbar_sleep<PAIR>(a, parity)) return;
     const unsigned long long t = globaltimer_ns() - t0;
     if ((i & 15u) != 0u || t < next) continue;
     next = t + 1000000ull;
@@ -288,19 +302,23 @@ static __device__ __noinline__ void stage_wait_slow(unsigned a, unsigned parity,
     }
   }
 }
+template <bool PAIR = false>
 __device__ __forceinline__ void stage_wait(unsigned long long* bar, unsigned parity,
                                            unsigned* err) {
   const unsigned a = smem_u32(bar);
-  if (!mbar_sleep(a, parity)) stage_wait_slow(a, parity, err);
+  if (!mbar_sleep<PAIR>(a, parity)) stage_wait_slow<PAIR>(a, parity, err);
 }
 
-// A warp has written its share of a stage, here or in the other block of the pair.
-// What it wrote is in its own block's shared memory and fence.proxy.async has handed
-// it to the tensor cores; nothing else has to be ordered, and a release to the whole
-// cluster here, a memory barrier of over a thousand cycles a stage, bounded the kernel
-// (258 against 160 us for 16320 rows, 1024 x 4096).
+// A warp has written its share of a stage into its own block's tensor memory, and the
+// first block's thread that waits for it issues a product that reads both blocks'.  What
+// orders the two is tcgen05's own chain: the stores' wait, the fence before the arrival,
+// the fence behind the wait; between them the arrival and the wait have to be of the
+// cluster's scope, as the blocks are two, but nothing else is handed over, so the arrival
+// releases nothing (dW of 16320 rows, 1024 x 4096 bfloat16, 115 us; 226 with a release,
+// which waits for all of the warp's memory operations).
 __device__ __forceinline__ void arrive_written(unsigned long long* bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(in_leader(smem_u32(bar)))
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(
+                   in_leader(smem_u32(bar)))
                : "memory");
 }
 
@@ -459,12 +477,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
                              ((unsigned)(kTile / 16) << 24);
       unsigned n = 0, tile = 0;
       for (int item = first; work_of(a, item, &t); item += step, ++tile) {
-        if (tile >= 1) stage_wait(&tm_empty, (tile - 1) & 1, a.err);
+        if (tile >= 1) stage_wait<true>(&tm_empty, (tile - 1) & 1, a.err);
         asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
         bool ready = false;
         for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
           const int s = n % S;
-          if (!ready) stage_wait(&full[s], (n / S) & 1, a.err);
+          if (!ready) stage_wait<true>(&full[s], (n / S) & 1, a.err);
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
           const unsigned p = tmem + kOperandAt + s * 32;
           const unsigned long long q = operand(smem0 + s * kHalf);
@@ -820,13 +838,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
         for (int c0 = t.kb0; c0 < t.kb1; c0 += kChunk, ++tile) {
           const int c1 = min(t.kb1, c0 + kChunk);
           const unsigned d = TALL ? tmem : tmem + (tile & 1) * 256;
-          if (TALL && tile >= 1) stage_wait(&tm_empty[0], (tile - 1) & 1, a.err);
-          if (!TALL && tile >= 2) stage_wait(&tm_empty[tile & 1], (tile / 2 - 1) & 1, a.err);
+          if (TALL && tile >= 1) stage_wait<true>(&tm_empty[0], (tile - 1) & 1, a.err);
+          if (!TALL && tile >= 2) stage_wait<true>(&tm_empty[tile & 1], (tile / 2 - 1) & 1, a.err);
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
           bool ready = false;
           for (int kb = c0; kb < c1; ++kb, ++n) {
             const int s = n % S;
-            if (!ready) stage_wait(&full[s], (n / S) & 1, a.err);
+            if (!ready) stage_wait<true>(&full[s], (n / S) & 1, a.err);
             asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
             const unsigned long long p = operand(smem0 + s * kStage),
                                      q = operand(smem0 + s * kStage + R * kHalf);

@@ -3,6 +3,8 @@
 from __future__ import annotations
 
 import ctypes
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -202,3 +204,17 @@ def test_c_entries_refuse_before_any_launch():
     assert L.fa_b200_linear8_backward(copied, None, 0, 0, None) == 5
     assert L.fa_b200_linear8_backward(copied, 512, 16, 0, None) == 5
     assert L.fa_b200_linear8_backward(copied, 520, room, 0, None) == 5
+
+
+def test_arrivals_in_the_other_block_are_of_the_cluster():
+    """An arrival without a scope orders nothing outside its own block, and neither does
+    a wait: the products' pairs are two blocks."""
+    csrc = Path(block.__file__).parent / "csrc"
+    text = (csrc / "linear8.cu").read_text() + (csrc / "tensor.cuh").read_text()
+    remote = re.findall(r"mbarrier\.arrive[\w.:]*shared::cluster[\w.:]*", text)
+    assert remote and all(".cluster.shared::cluster" in a for a in remote), remote
+    # the barriers with such arrivals: the stages that are written, the sums that are read
+    product = (csrc / "linear8.cu").read_text()
+    waits = re.findall(r"stage_wait(<\w+>)?\((&full\[s\], \(n / S\)|&tm_empty)", product)
+    assert len(waits) == 5 and all(kind == "<true>" for kind, _ in waits), waits
+    assert product.count("wait.parity.acquire.cluster.shared::cta") == 2

@@ -1108,3 +1108,21 @@ def test_a_thread_may_make_its_first_call_here(what):
     """)
     out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and "same" in out.stdout, out.stderr
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,inputs,outputs", [(200, 256, 256), (1600, 512, 256), (700, 1100, 520)])
+def test_a_weight_gradient_sees_every_stage_as_written(rows, inputs, outputs, dtype):
+    """Both blocks of a pair write the stages that one of them multiplies.  Calls on other
+    values in between, so that a stage read too early would hold something else."""
+    cases = [linear_case((rows, inputs, outputs, False), dtype, seed=170 + 7 * i) for i in range(2)]
+    leaves = [w.detach().requires_grad_(True) for _, w, _, _ in cases]
+
+    def grad(i):
+        return torch.autograd.grad(fa.linear8(cases[i][0], leaves[i]), leaves[i], cases[i][3])[0]
+
+    want = [grad(i) for i in range(2)]
+    for dw, (x, _, _, gy) in zip(want, cases):
+        check_weight_grad(dw, None, x, gy, dtype)
+    for k in range(60):
+        assert torch.equal(grad(k % 2), want[k % 2])
