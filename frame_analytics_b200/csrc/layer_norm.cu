@@ -8,12 +8,17 @@
 // where h comes from s, or from what its packed copy (keep8.cuh) stands for; m
 // and r are those of s either way, kept in float32.
 //
-// The variance is summed about the mean (not as a difference of squares, which a
-// common offset would cancel); all sums are float32.  dw and db are summed in a
+// The variance is summed about a first mean (not as a difference of squares, which a
+// common offset would cancel), and the same pass sums the values' distances from it: a
+// float32 sum of n values is up to n 2^-24 of their size off, which against eps is not
+// little for a row of one value (0.15 instead of 0 at 4096 columns around 1000), while
+// the sum of the distances carries no common part any more.  With d = s - m0:
+//   m = m0 + mean d,  variance = mean d^2 - (mean d)^2.
+// All sums are float32.  dw and db are summed in a
 // fixed order without atomics, so they are the same bits on every run.
 //
-// Measured on one B200, 65280 x 4096 bfloat16: forward 217 us (0.75 of the copy rate),
-// with the residual sum 317 us (1.0), with packing too 381 us (0.97); backward 377 us
+// Measured on one B200, 65280 x 4096 bfloat16: forward 211 us (0.77 of the copy rate),
+// with the residual sum 313 us (1.0), with packing too 358 us (1.0); backward 377 us
 // (0.65), with the sum's gradient 407 us (0.80), from packed input 412 us (0.70).  The
 // forward pass is bound by bytes where there are more than a read and a write of each
 // value; the backward pass by the latency of joining a row's two sums, with 16 warps a
@@ -121,11 +126,13 @@ __device__ __forceinline__ float inv_sqrt(float v) {
   return r > 0.f && r < __uint_as_float(0x7f800000u) ? r * fmaf(-0.5f * v * r, r, 1.5f) : r;
 }
 
-// A sum over the row's length: the reciprocal, corrected once, so that an even row's mean
-// is its value.
-__device__ __forceinline__ float mean_of(float t, const NormArgs& a) {
-  const float q = t * a.inv_width;
-  return fmaf(fmaf(-q, (float)a.width, t), a.inv_width, q);
+// Mean and 1 / deviation from a first mean m0 and the sums of the distances from it and
+// of their squares.
+__device__ __forceinline__ float2 moments(float m0, float d, float d2, float inv_width, float eps) {
+  const float mean = d * inv_width;
+  const float v = fmaf(d2, inv_width, -mean * mean);
+  // rounding may leave a row of one value less than nothing
+  return make_float2(m0 + mean, inv_sqrt((v < 0.f ? 0.f : v) + eps));
 }
 
 // Two sums over the warp with the shuffles of little more than one: the halves of the
@@ -152,7 +159,8 @@ template <typename T, RowKind KIND, int E, int NT>
 __global__ void __launch_bounds__(NT, NT > 512 ? 1 : 768 / NT) norm_kernel(const NormArgs a, int wpr) {
   constexpr bool VEC = KIND != ODD;
   typedef typename RangeBits<T>::type Bits;
-  __shared__ float sm[2][32];
+  __shared__ float sm[32];
+  __shared__ float2 sm2[32];
   __shared__ __align__(16) Turn8<T> turns[VEC ? 1 : NT / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   Turn8<T>* const turn = turns + (VEC ? 0 : warp);
@@ -190,15 +198,6 @@ __global__ void __launch_bounds__(NT, NT > 512 ? 1 : 768 / NT) norm_kernel(const
 #pragma unroll
     for (int e = 0; e < E; ++e) s[e] = fetch8<T, VEC>(xp + 256 * e, n[e], turn);
   }
-  const auto row_sum = [&](float t, int k) {
-    t = warp_sum(t);
-    if (wpr == 1) return t;
-    if (lane == 0) sm[k][warp] = t;
-    __syncthreads();
-    t = 0.f;
-    for (int w = 0; w < wpr; ++w) t += sm[k][first + w];
-    return t;
-  };
   float2 t = both(0.f);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
@@ -206,20 +205,40 @@ __global__ void __launch_bounds__(NT, NT > 512 ? 1 : 768 / NT) norm_kernel(const
 #pragma unroll
     for (int i = 0; i < 4; ++i) t = __fadd2_rn(t, x.v[i]);
   }
-  const float m = mean_of(row_sum(t.x + t.y, 0), a);
-  float2 v = both(0.f);
+  float total = warp_sum(t.x + t.y);
+  if (wpr > 1) {
+    if (lane == 0) sm[warp] = total;
+    __syncthreads();
+    total = 0.f;
+    for (int w = 0; w < wpr; ++w) total += sm[first + w];
+  }
+  const float m0 = total * a.inv_width;
+  float2 t1 = both(0.f), t2 = both(0.f);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     if (KIND == VECTORS && n[e] == 0) continue;
     F8 x = widen8(s[e]);
-    if (!VEC) fill_from(x, n[e], m);
+    if (!VEC) fill_from(x, n[e], m0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 d = __fadd2_rn(x.v[i], both(-m));
-      v = __ffma2_rn(d, d, v);
+      const float2 d = __fadd2_rn(x.v[i], both(-m0));
+      t1 = __fadd2_rn(t1, d);
+      t2 = __ffma2_rn(d, d, t2);
     }
   }
-  const float r = inv_sqrt(fmaf(row_sum(v.x + v.y, 1), a.inv_width, a.eps));
+  const float both_sums = warp_sum2(t1.x + t1.y, t2.x + t2.y);
+  float2 sums;
+  if (wpr > 1) {
+    if ((lane & 15) == 0) reinterpret_cast<float*>(sm2 + warp)[lane >> 4] = both_sums;
+    __syncthreads();
+    sums = both(0.f);
+    for (int w = 0; w < wpr; ++w) sums = __fadd2_rn(sums, sm2[first + w]);
+  } else {
+    sums.x = __shfl_sync(0xffffffffu, both_sums, 0);
+    sums.y = __shfl_sync(0xffffffffu, both_sums, 16);
+  }
+  const float2 moment = moments(m0, sums.x, sums.y, a.inv_width, a.eps);
+  const float m = moment.x, r = moment.y;
   if (a.stats && in && at == 0 && lane == 0) a.stats[row] = make_float2(m, r);
   if (a.sum) {
     T* const sp = reinterpret_cast<T*>(a.sum) + row * a.width + c0;
@@ -453,19 +472,22 @@ __global__ void __launch_bounds__(256) norm_rows_kernel(const NormArgs a) {
       const int c = (u0 + threadIdx.x) * 8, n = max(0, min(8, a.width - c));
       t += sum8(input8<T, VEC>(a, row, c, n, turn));
     }
-    const float m = block_sum(t, sm) / (float)a.width;
-    float2 v = both(0.f);
+    const float m0 = block_sum(t, sm) * a.inv_width;
+    float2 t1 = both(0.f), t2 = both(0.f);
     for (int u0 = 0; u0 < units; u0 += 256) {
       const int c = (u0 + threadIdx.x) * 8, n = max(0, min(8, a.width - c));
       F8 x = input8<T, VEC>(a, row, c, n, turn);
-      fill_from(x, n, m);
+      fill_from(x, n, m0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 d = __fadd2_rn(x.v[i], both(-m));
-        v = __ffma2_rn(d, d, v);
+        const float2 d = __fadd2_rn(x.v[i], both(-m0));
+        t1 = __fadd2_rn(t1, d);
+        t2 = __ffma2_rn(d, d, t2);
       }
     }
-    const float r = 1.f / sqrtf(block_sum(v.x + v.y, sm) / (float)a.width + a.eps);
+    const float s1 = block_sum(t1.x + t1.y, sm), s2 = block_sum(t2.x + t2.y, sm);
+    const float2 moment = moments(m0, s1, s2, a.inv_width, a.eps);
+    const float m = moment.x, r = moment.y;
     if (a.stats && threadIdx.x == 0) a.stats[row] = make_float2(m, r);
     for (int u0 = 0; u0 < units; u0 += 256) {
       const int u = u0 + threadIdx.x, c = u * 8, n = max(0, min(8, a.width - c));
@@ -734,7 +756,7 @@ static RowKind kind_of(const NormArgs& a, bool vec, int item, RowShape shape) {
 
 // Forward, a block has one row of its own: blocks that stayed and took rows in turn, two
 // a multiprocessor's worth of warps, took 342 us where these took 272 (65280 x 4096
-// bfloat16, both on the path of VECTORS; FULL takes 217), since all of a block's warps
+// bfloat16, both on the path of VECTORS; FULL takes 211), since all of a block's warps
 // load, sum and store at the same time.
 template <typename T, RowKind KIND, int E>
 static void norm_launch(const NormArgs& a, int wpr, cudaStream_t st) {

@@ -1126,3 +1126,38 @@ def test_a_weight_gradient_sees_every_stage_as_written(rows, inputs, outputs, dt
         check_weight_grad(dw, None, x, gy, dtype)
     for k in range(60):
         assert torch.equal(grad(k % 2), want[k % 2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("width", [1, 24, 192, 577, 1024, 4096, 8192, 20480, 32760, 40000])
+def test_norm_of_rows_of_one_value_is_nothing(width, dtype):
+    """Whatever the value: its mean is itself, which a plain float32 sum misses."""
+    values = torch.cat((torch.tensor([0.37, 1234.567, -998.2, 3.3e4], device="cuda"),
+                        1000 + 30 * rand(36, seed=180)))[:, None].to(dtype)
+    x = values.expand(40, width).contiguous()
+    w, b = 1 + rand(width, seed=181).abs(), rand(width, seed=182)
+    for keep8 in (False, True):
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        y = fa.layer_norm(*leaves, keep8=keep8)
+        assert torch.equal(y.detach(), b.to(dtype).expand(40, width))
+        gy = torch.ones_like(y)
+        dw, db = torch.autograd.grad(y, leaves[1:], gy)
+        # each distance is nothing, and 40 is a float32 number
+        assert not bool(dw.any()) and bool((db == 40).all())
+
+
+@pytest.mark.parametrize("width", [192, 577, 1024, 4096, 40000])
+def test_norm_of_a_row_whose_spread_is_small_against_its_offset(width):
+    x = 1000 + 0.01 * rand(64, width, seed=183)
+    m = x.double().mean(1, keepdim=True)
+    r = 1 / ((x.double() - m).square().mean(1, keepdim=True) + 1e-5).sqrt()
+    want = (x.double() - m) * r
+    # The mean that is taken off is rounded to float32 once, E |m|, behind a first one m0
+    # that is at most e0 = (n / 32 + 80) E |m| off and a mean of distances from m0, which
+    # is as far off relative to them (|d| <= |s - m| + e0); the mean of d^2, the variance
+    # and at most e0^2, likewise, and half of that is 1 / deviation's.
+    rel = (width / 32 + 80) * E
+    e0 = rel * m.abs()
+    em = E * m.abs() + rel * ((x.double() - m).abs().mean(1, keepdim=True) + e0)
+    tol = (em + 2 * E * (x.double() - m).abs()) * r + want.abs() * (rel * (1 + 2 * (e0 * r) ** 2) + 8 * E)
+    within(fa.layer_norm(x), want, tol + E * want.abs(), torch.float32)
