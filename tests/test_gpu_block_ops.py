@@ -1161,3 +1161,40 @@ def test_norm_of_a_row_whose_spread_is_small_against_its_offset(width):
     em = E * m.abs() + rel * ((x.double() - m).abs().mean(1, keepdim=True) + e0)
     tol = (em + 2 * E * (x.double() - m).abs()) * r + want.abs() * (rel * (1 + 2 * (e0 * r) ** 2) + 8 * E)
     within(fa.layer_norm(x), want, tol + E * want.abs(), torch.float32)
+
+
+@pytest.mark.parametrize("approximate", ["none", "tanh"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gelu_far_out_relative_to_its_value(dtype, approximate):
+    """Down to -13, where values and slopes are 1e-37 (tanh form: nothing).
+
+    Both are at most (32 + 2 x^2) E of their terms off: 20 E of the tail's factor (1.1e-6)
+    and its rounding, 4 E of an approximate exponential, the roundings of an exponent of
+    x^2 / 2 (three, of a value that the exponential takes absolutely) and of the few
+    operations around; the tanh form with its own exponent 2 u, four roundings, in place of
+    x^2 / 2.  float32's library functions are closer than that."""
+    x = torch.linspace(-13, 13, 26 * 512 + 1, device="cuda").to(dtype)[:, None]
+    leaf = x.clone().requires_grad_(True)       # each value a group of its own: kept exactly
+    y = fa.gelu8(leaf, approximate=approximate)
+    dx, = torch.autograd.grad(y, leaf, torch.ones_like(x))
+    d = x.double()
+    if approximate == "tanh":
+        c = (2 / math.pi) ** 0.5
+        two_u, up = 2 * c * (d + 0.044715 * d ** 3), 2 * c * (1 + 3 * 0.044715 * d * d)
+        f = torch.sigmoid(two_u)
+        value, first, second = d * f, f, d * f * torch.sigmoid(-two_u) * up
+        rel = (32 + 4 * two_u.abs()) * E
+        # above zero f (1 - f) is within E, a rounding of f
+        extra = torch.where(d > 0, 2 * E * d * up, 0.0)
+    else:
+        first = torch.special.erfc(-d / 2 ** 0.5) / 2
+        value, second = d * first, d * torch.exp(-d * d / 2) / (2 * math.pi) ** 0.5
+        rel, extra, up = (32 + 2 * d * d) * E, torch.zeros_like(d), d.abs()
+    # A factor f (or an exponential) below 2^-126 may be flushed, which moves f by that,
+    # the value x f by |x| of it, and the slope f + x f (1 - f) up by 1 + |x| up of it
+    # (the other form's x exp(-x^2 / 2): by |x|)
+    low = 2.0 ** -126
+    for got, want, size, by in ((y.detach(), value, value.abs(), 1 + d.abs()),
+                                (dx, first + second, first + second.abs(), 1 + d.abs() * (1 + up))):
+        tol = rel * size + (0 if got is not dx else extra) + low * by
+        within(got, want, U[dtype] * want.abs() + (1 + 2 * U[dtype]) * tol, dtype)
