@@ -43,10 +43,12 @@ int pack8_impl(const void* x, long long x_row, void* codes, void* ranges, int dt
 // All three products in float32, on the ordinary lanes (two products an instruction):
 // the tensor cores would round the operands.  D[m][n] = sum over k of A B, 128 x 128 a
 // block, 8 x 8 a thread, 16 of k a stage; the next stage is on its way while this one's
-// products run.  Few tiles: k is cut into parts, whose sums are joined in order.
+// products run.  Few tiles: k is cut into parts, whose sums are joined in order.  After
+// every 32768 terms the sum goes to its place in the result, so that a long one's roundings
+// do not add up.
 // Bound by the products: 16320 rows, 1024 x 1024, dW 0.80 ms, 43 TFLOP/s.
 constexpr int kLaneTile = 128, kLaneDepth = 16;
-constexpr long long kLongest = 32768;  // terms of a part
+constexpr long long kLongest = 32768;  // terms of a sum
 
 struct LaneArgs {
   const float *a, *b;           // or codes
@@ -75,7 +77,8 @@ __device__ __forceinline__ float4 four(const float* p, long long c, long long n,
   return v;
 }
 
-template <LaneOperand A, LaneOperand B>
+// LONG: some part is longer than 32768.
+template <LaneOperand A, LaneOperand B, bool LONG>
 __global__ void __launch_bounds__(256, 2) lanes_kernel(const LaneArgs a) {
   constexpr int P = kLaneTile + 4;  // pitch: transposed stores meet two at a bank, not eight
   __shared__ __align__(16) float sa[2][kLaneDepth][P], sb[2][kLaneDepth][P];
@@ -137,45 +140,53 @@ __global__ void __launch_bounds__(256, 2) lanes_kernel(const LaneArgs a) {
       put8<float>(&sb[half][rc][uc * 8], narrow8(decode8<float>(nq, range_of(nr, 0.f)), 0.f));
   };
   float2 acc[8][4];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = both(0.f);
   fetch(k0);
   put(0);
   int half = 0;
-  for (long long k = k0; k < k1; k += kLaneDepth, half ^= 1) {
-    __syncthreads();
-    fetch(k + kLaneDepth);
+  long long k = k0;
+  do {
+    const long long c0 = k, c1 = LONG ? min(k1, c0 + kLongest) : k1;
 #pragma unroll
-    for (int r = 0; r < kLaneDepth; ++r) {
-      // rows ty * 4 + 0..3 and 64 on, columns tx * 4 + 0..3 and 64 on
-      const float4 p0 = *reinterpret_cast<const float4*>(&sa[half][r][ty * 4]),
-                   p1 = *reinterpret_cast<const float4*>(&sa[half][r][64 + ty * 4]),
-                   q0 = *reinterpret_cast<const float4*>(&sb[half][r][tx * 4]),
-                   q1 = *reinterpret_cast<const float4*>(&sb[half][r][64 + tx * 4]);
-      const float p[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
-      const float2 q[4] = {{q0.x, q0.y}, {q0.z, q0.w}, {q1.x, q1.y}, {q1.z, q1.w}};
+    for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int j = 0; j < 4; ++j) acc[i][j] = both(0.f);
+    for (; k < c1; k += kLaneDepth, half ^= 1) {
+      __syncthreads();
+      fetch(k + kLaneDepth);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __ffma2_rn(both(p[i]), q[j], acc[i][j]);
+      for (int r = 0; r < kLaneDepth; ++r) {
+        // rows ty * 4 + 0..3 and 64 on, columns tx * 4 + 0..3 and 64 on
+        const float4 p0 = *reinterpret_cast<const float4*>(&sa[half][r][ty * 4]),
+                     p1 = *reinterpret_cast<const float4*>(&sa[half][r][64 + ty * 4]),
+                     q0 = *reinterpret_cast<const float4*>(&sb[half][r][tx * 4]),
+                     q1 = *reinterpret_cast<const float4*>(&sb[half][r][64 + tx * 4]);
+        const float p[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
+        const float2 q[4] = {{q0.x, q0.y}, {q0.z, q0.w}, {q1.x, q1.y}, {q1.z, q1.w}};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = __ffma2_rn(both(p[i]), q[j], acc[i][j]);
+      }
+      if (k + kLaneDepth < k1) put(half ^ 1);
     }
-    if (k + kLaneDepth < k1) put(half ^ 1);
-  }
-  float* const out = a.d + (long long)blockIdx.z * a.m * a.n;
-  const float* const bias = a.parts == 1 ? a.bias : nullptr;
+    // what is there is the sum before
+    float* const out = a.d + (long long)blockIdx.z * a.m * a.n;
+    const float* const bias = a.parts == 1 && c1 == k1 ? a.bias : nullptr;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int m = m0 + (i >> 2) * 64 + ty * 4 + (i & 3);
-    if (m >= a.m) continue;
+    for (int i = 0; i < 8; ++i) {
+      const int m = m0 + (i >> 2) * 64 + ty * 4 + (i & 3);
+      if (m >= a.m) continue;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int n = n0 + (j >> 2) * 64 + tx * 4 + (j & 3);
-      const float v = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
-      if (n < a.n) out[(long long)m * a.n + n] = bias ? v + __ldg(bias + n) : v;
+      for (int j = 0; j < 8; ++j) {
+        const int n = n0 + (j >> 2) * 64 + tx * 4 + (j & 3);
+        float v = j & 1 ? acc[i][j / 2].y : acc[i][j / 2].x;
+        if (n < a.n) {
+          if (LONG && c0 > k0) v += out[(long long)m * a.n + n];
+          out[(long long)m * a.n + n] = bias ? v + __ldg(bias + n) : v;
+        }
+      }
     }
-  }
+  } while (LONG && k < k1);
 }
 __global__ void __launch_bounds__(256) join_lanes_kernel(const float* part, float* d, int parts,
                                                          long long size, const float* bias, int n) {
@@ -208,8 +219,8 @@ constexpr int kPartFloats = 128 * 256;  // of one block's part of a tile
 // The tensor cores add to a sum with truncation, up to 2^-24 of it for each 16 terms and
 // always towards zero.  A sum of more than 32768 terms is therefore taken in chunks of
 // so many, each at most 6e-5 of it short on average (a quarter of float16's half step),
-// and the chunks are added with rounding: the rows of dW are cut into parts of a chunk
-// at most (chunks inside the kernel cost its writers 6 %), y and dx add their chunks.
+// and the chunks are added with rounding, in a slab of float32 that a pair of blocks keeps
+// for all of its tiles (or a part its own): the workspace does not grow with the sum.
 constexpr int kChunk = 512;     // stages
 
 // dW[n][m] = sum over t of x^[t][m] dy[t][n].
@@ -221,7 +232,7 @@ struct ProductArgs {
   long long rows;
   int groups;
   void* out;
-  float* part;
+  float* part;                  // a slab of 256 x 256 a part, or (one part) a pair of blocks
   unsigned* err;
 };
 
@@ -407,7 +418,9 @@ __device__ __forceinline__ void mma_from_tmem(unsigned d, unsigned a, unsigned l
       : "memory");
 }
 
-template <typename T>
+// CHUNKS: some part is longer than a chunk (the writers' sums then end a part's stages
+// more than once, which costs 5 % where it is not needed).
+template <typename T, bool CHUNKS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
     wgrad_kernel(const __grid_constant__ ProductArgs a) {
   constexpr int S = kStages, SC = kCodeStages;
@@ -476,27 +489,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
       const unsigned idesc = (1u << 4) | kind | (1u << 16) | ((unsigned)(kTile / 8) << 17) |
                              ((unsigned)(kTile / 16) << 24);
       unsigned n = 0, tile = 0;
-      for (int item = first; work_of(a, item, &t); item += step, ++tile) {
-        if (tile >= 1) stage_wait<true>(&tm_empty, (tile - 1) & 1, a.err);
-        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-        bool ready = false;
-        for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
-          const int s = n % S;
-          if (!ready) stage_wait<true>(&full[s], (n / S) & 1, a.err);
+      for (int item = first; work_of(a, item, &t); item += step)
+        for (int c0 = t.kb0, c1; c0 < t.kb1; c0 = c1, ++tile) {
+          c1 = CHUNKS ? min(t.kb1, c0 + kChunk) : t.kb1;
+          if (tile >= 1) stage_wait<true>(&tm_empty, (tile - 1) & 1, a.err);
           asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-          const unsigned p = tmem + kOperandAt + s * 32;
-          const unsigned long long q = operand(smem0 + s * kHalf);
+          bool ready = false;
+          for (int kb = c0; kb < c1; ++kb, ++n) {
+            const int s = n % S;
+            if (!ready) stage_wait<true>(&full[s], (n / S) & 1, a.err);
+            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            const unsigned p = tmem + kOperandAt + s * 32;
+            const unsigned long long q = operand(smem0 + s * kHalf);
 #pragma unroll
-          for (int k = 0; k < kDepth / 16; ++k) {
-            mma_from_tmem(tmem, p + 8 * k, q + k * (2048u >> 4), idesc, kb > t.kb0 || k > 0);
-            // the next stage is asked for while this one's products run: few are queued,
-            // and a poll takes longer than the last of them
-            if (k == 1) ready = kb + 1 < t.kb1 && mbar_peek(&full[(n + 1) % S], ((n + 1) / S) & 1);
+            for (int k = 0; k < kDepth / 16; ++k) {
+              mma_from_tmem(tmem, p + 8 * k, q + k * (2048u >> 4), idesc, kb > c0 || k > 0);
+              // the next stage is asked for while this one's products run: few are queued,
+              // and a poll takes longer than the last of them
+              if (k == 1) ready = kb + 1 < c1 && mbar_peek(&full[(n + 1) % S], ((n + 1) / S) & 1);
+            }
+            mma_commit<true>(&empty[s]);
           }
-          mma_commit<true>(&empty[s]);
+          mma_commit<true>(&tm_full);
         }
-        mma_commit<true>(&tm_full);
-      }
       // products still in flight end before tensor memory is given back
       mma_commit<true>(&drain);
       stage_wait(&drain, 0, a.err);
@@ -550,90 +565,99 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kWgThreads, 1)
     // tensor memory that it may touch, and all 64 rows of a stage.
     const int team = (warp - 4) >> 2, w = warp & 3;
     unsigned n = 0, tile = 0;
-    for (int item = first; work_of(a, item, &t); item += step, ++tile) {
-      for (int kb = t.kb0; kb < t.kb1; ++kb, ++n) {
-        if ((int)(n & 1) != team) continue;
-        const int s = n % S, c = n % SC;
-        warp_wait(&c_full[c], (n / SC) & 1, a.err);
-        const uint4* const ranges =
-            reinterpret_cast<const uint4*>(smem + kRangesAt + c * kRanges) + (w >> 1) * (kDepth / 4) +
-            (lane & 3);
-        Range4 r[4];
-        bool held = true;
+    for (int item = first; work_of(a, item, &t); item += step)
+      for (int c0 = t.kb0, c1; c0 < t.kb1; c0 = c1, ++tile) {
+        c1 = CHUNKS ? min(t.kb1, c0 + kChunk) : t.kb1;
+        for (int kb = c0; kb < c1; ++kb, ++n) {
+          if ((int)(n & 1) != team) continue;
+          const int s = n % S, c = n % SC;
+          warp_wait(&c_full[c], (n / SC) & 1, a.err);
+          const uint4* const ranges =
+              reinterpret_cast<const uint4*>(smem + kRangesAt + c * kRanges) +
+              (w >> 1) * (kDepth / 4) + (lane & 3);
+          Range4 r[4];
+          bool held = true;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {  // 16 rows each, four of them this lane's
-          const uint4 bits = ranges[4 * b];
-          r[b] = range4<T>(bits);
-          if constexpr (std::is_same<T, f16_t>::value) held = held && held_in_half(bits);
-        }
+          for (int b = 0; b < 4; ++b) {  // 16 rows each, four of them this lane's
+            const uint4 bits = ranges[4 * b];
+            r[b] = range4<T>(bits);
+            if constexpr (std::is_same<T, f16_t>::value) held = held && held_in_half(bits);
+          }
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          unsigned v[16];
+          for (int half = 0; half < 2; ++half) {
+            unsigned v[16];
 #pragma unroll
-          for (int bb = 0; bb < 2; ++bb) {
-            // rows of 128 bytes whose 16-byte units are xor-ed with the row
-            const int row = 32 * bb + lane;
-            unsigned q[4];
-            codes16x2(smem0 + kCodesAt + c * kRaw + row * 128 + (((2 * w + half) ^ (row & 7)) << 4), q);
+            for (int bb = 0; bb < 2; ++bb) {
+              // rows of 128 bytes whose 16-byte units are xor-ed with the row
+              const int row = 32 * bb + lane;
+              unsigned q[4];
+              codes16x2(smem0 + kCodesAt + c * kRaw + row * 128 +
+                            (((2 * w + half) ^ (row & 7)) << 4),
+                        q);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {  // block of 16 rows, input, pair of rows
-              const int b = i >> 2, in = (i >> 1) & 1, k = i & 1;
-              const Range4& g = r[2 * bb + b];
-              v[8 * bb + i] = operand2(q[2 * b + in], 2 * k, g.s[k], g.lo[k], T());
-            }
-            if constexpr (std::is_same<T, f16_t>::value) {
-              if (!held) {
+              for (int i = 0; i < 8; ++i) {  // block of 16 rows, input, pair of rows
+                const int b = i >> 2, in = (i >> 1) & 1, k = i & 1;
+                const Range4& g = r[2 * bb + b];
+                v[8 * bb + i] = operand2(q[2 * b + in], 2 * k, g.s[k], g.lo[k], T());
+              }
+              if constexpr (std::is_same<T, f16_t>::value) {
+                if (!held) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  const int b = i >> 2, in = (i >> 1) & 1, k = i & 1;
-                  const uint4 bits = ranges[4 * (2 * bb + b)];
-                  v[8 * bb + i] = operand2_wide(q[2 * b + in], 2 * k, k ? bits.z : bits.x,
-                                                k ? bits.w : bits.y);
+                  for (int i = 0; i < 8; ++i) {
+                    const int b = i >> 2, in = (i >> 1) & 1, k = i & 1;
+                    const uint4 bits = ranges[4 * (2 * bb + b)];
+                    v[8 * bb + i] = operand2_wide(q[2 * b + in], 2 * k, k ? bits.z : bits.x,
+                                                  k ? bits.w : bits.y);
+                  }
                 }
               }
             }
+            if (half == 0) {
+              if (n >= (unsigned)S) warp_wait(&empty[s], (n / S - 1) & 1, a.err);
+              asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+            }
+            tmem_store16(tmem + kOperandAt + s * 32 + ((unsigned)(32 * w + 16 * half) << 16), v);
           }
-          if (half == 0) {
-            if (n >= (unsigned)S) warp_wait(&empty[s], (n / S - 1) & 1, a.err);
-            asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-          }
-          tmem_store16(tmem + kOperandAt + s * 32 + ((unsigned)(32 * w + 16 * half) << 16), v);
-        }
-        asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
-        asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-          arrive_written(&full[s]);
-          arrive_leader<false>(&c_empty[c]);
-        }
-      }
-      // the tile's sums: a lane an input, this team's half of the outputs
-      if (lane == 0) stage_wait(&tm_full, tile & 1, a.err);
-      __syncwarp();
-      asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
-      const int i = t.i0 + rank * 128 + 32 * w + lane;
-#pragma unroll 1
-      for (int c = team * 128; c < team * 128 + 128; c += 32) {
-        float v[32];
-        tmem_load32(tmem + c + ((unsigned)(32 * w) << 16), v);
-        if (c + 32 == team * 128 + 128) {
-          __syncwarp();
+          asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory");
           asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
-          if (lane == 0) arrive_leader<true>(&tm_empty);
+          __syncwarp();
+          if (lane == 0) {
+            arrive_written(&full[s]);
+            arrive_leader<false>(&c_empty[c]);
+          }
         }
-        if (a.parts > 1) {  // [item][block][outputs][128 inputs]
-          float* const to =
-              a.part + ((long long)t.item * 2 + rank) * kPartFloats + c * 128 + 32 * w + lane;
+        // the tile's sums: a lane an input, this team's half of the outputs
+        if (lane == 0) stage_wait(&tm_full, tile & 1, a.err);
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory");
+        const int i = t.i0 + rank * 128 + 32 * w + lane;
+#pragma unroll 1
+        for (int c = team * 128; c < team * 128 + 128; c += 32) {
+          float v[32];
+          tmem_load32(tmem + c + ((unsigned)(32 * w) << 16), v);
+          if (c + 32 == team * 128 + 128) {
+            __syncwarp();
+            asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
+            if (lane == 0) arrive_leader<true>(&tm_empty);
+          }
+          // [slab][block][outputs][128 inputs]
+          const long long slab = a.parts > 1 ? t.item : first;
+          float* const to = a.part + (slab * 2 + rank) * kPartFloats + c * 128 + 32 * w + lane;
+          if (CHUNKS && c0 > t.kb0) {
 #pragma unroll
-          for (int q = 0; q < 32; ++q) to[q * 128] = v[q];
-        } else if (i < a.m) {
-          T* const to = reinterpret_cast<T*>(a.out) + (long long)(t.j0 + c) * a.m + i;
+            for (int q = 0; q < 32; ++q) v[q] += to[q * 128];
+          }
+          if (a.parts > 1 || (CHUNKS && c1 < t.kb1)) {
 #pragma unroll
-          for (int q = 0; q < 32; ++q)
-            if (t.j0 + c + q < a.n) to[(long long)q * a.m] = St<T>::v(v[q]);
+            for (int q = 0; q < 32; ++q) to[q * 128] = v[q];
+          } else if (i < a.m) {
+            T* const to = reinterpret_cast<T*>(a.out) + (long long)(t.j0 + c) * a.m + i;
+#pragma unroll
+            for (int q = 0; q < 32; ++q)
+              if (t.j0 + c + q < a.n) to[(long long)q * a.m] = St<T>::v(v[q]);
+          }
         }
       }
-    }
   }
   asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory");
   __syncthreads();
@@ -692,7 +716,7 @@ struct PlainArgs {
   void* out;                    // [m][n]
   const void* bias;             // [n] or null
   int tma_out, bias_vec;
-  float* part;
+  float* part;                  // as in ProductArgs
   unsigned* err;
 };
 
@@ -889,9 +913,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
             if (lane == 0) arrive_leader<true>(&tm_empty[buf]);
           }
           if constexpr (!TALL) {
-            // [item][block][columns / 4][128 rows] of four columns each
-            float4* const to = reinterpret_cast<float4*>(
-                a.part + ((long long)t.item * 2 + rank) * kPartFloats) + c / 4 * 128 + 32 * w + lane;
+            // [slab][block][columns / 4][128 rows] of four columns each
+            const long long slab = a.parts > 1 ? t.item : first;
+            float4* const to = reinterpret_cast<float4*>(a.part + (slab * 2 + rank) * kPartFloats) +
+                               c / 4 * 128 + 32 * w + lane;
             if (c0 > t.kb0) {
 #pragma unroll
               for (int q = 0; q < 16; ++q) {
@@ -1003,15 +1028,17 @@ static bool box_map(CUtensorMap* map, const void* p, long long rows, long long c
 static int tiles_of(long long n) { return (int)((n + kTile - 1) / kTile); }
 
 // Parts of the sum's axis: the number whose waves take the least time, at 0.42 us a
-// stage of a pair, 6 us a tile's end, and the parts' trip through memory.
-static int parts_of(long long tiles, int kb, int pairs, int least_parts) {
-  int best = least_parts;
+// stage of a pair, 6 us a chunk's end, and the parts' trip through memory.  Every part of
+// every tile has a slab of its own, eight for a pair of blocks at most (155 MB).
+static int parts_of(long long tiles, int kb, int pairs) {
+  int best = 1;
   double least = 0;
-  for (int p = least_parts; p < least_parts + 32 && p <= kb; ++p) {
+  for (int p = 1; p <= 32 && p <= kb && (p == 1 || tiles * p <= 8ll * pairs); ++p) {
     const double waves = (double)((tiles * p + pairs - 1) / pairs);
-    double us = waves * (0.42 * ((kb + p - 1) / p) + 6.0);
+    const int stages = (kb + p - 1) / p;
+    double us = waves * (0.42 * stages + 6.0 * ((stages + kChunk - 1) / kChunk));
     if (p > 1) us += 4.0 + tiles * (double)p * 2 * kPartFloats * 4 * 2 / 4e6;
-    if (p == least_parts || us < least) {
+    if (p == 1 || us < least) {
       least = us;
       best = p;
     }
@@ -1037,9 +1064,9 @@ static int resident_pairs(int device) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  if (cudaFuncSetAttribute(wgrad_kernel<bf16_t>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  if (cudaFuncSetAttribute(wgrad_kernel<bf16_t, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            kWgSmem) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, wgrad_kernel<bf16_t>, &cfg) != cudaSuccess || n < 1) {
+      cudaOccupancyMaxActiveClusters(&n, wgrad_kernel<bf16_t, false>, &cfg) != cudaSuccess || n < 1) {
     cudaGetLastError();
     n = std::max(1, sm_count(device) / 2);
   }
@@ -1097,31 +1124,32 @@ static LinearPlan linear_plan(const fa_linear8& l, int device) {
     p.pairs = resident_pairs(device);
     const int in = tiles_of(l.inputs), out = tiles_of(l.outputs);
     const long long rows = tiles_of(l.rows);
-    const auto room = [&](long long tiles, int n) {
-      part = std::max(part, (size_t)tiles * n * 2 * kPartFloats * sizeof(float));
-    };
-    const auto parts = [&](bool wanted, long long tiles, int kb) {
-      const int n = !wanted || tiles > p.pairs ? 1 : parts_of(tiles, kb, p.pairs, 1);
-      if (wanted && (n > 1 || kb > kChunk)) room(tiles, n);
+    const auto parts = [&](bool wanted, long long tiles, int kb, bool even) {
+      if (!wanted) return 1;
+      const int n = tiles > p.pairs && !even ? 1 : parts_of(tiles, kb, p.pairs);
+      const long long slabs = n > 1 ? tiles * n : kb > kChunk ? std::min(tiles, (long long)p.pairs) : 0;
+      part = std::max(part, (size_t)slabs * 2 * kPartFloats * sizeof(float));
       return n;
     };
-    p.y_parts = parts(l.y, rows * out, stages_of(l.inputs));
-    p.dx_parts = parts(l.dx, rows * in, stages_of(l.outputs));
-    if (l.dweight) {
-      const long long tiles = (long long)in * out;
-      const int kb = stages_of(l.rows), chunks = (kb + kChunk - 1) / kChunk;
-      p.dw_parts = tiles > p.pairs ? chunks : parts_of(tiles, kb, p.pairs, chunks);
-      if (p.dw_parts > 1) room(tiles, p.dw_parts);
-    }
+    // a long sum over more tiles than pairs is cut for the sake of its last wave (65280 rows,
+    // 4096 x 4096: 2.0 ms in two parts, 2.4 in one)
+    p.y_parts = parts(l.y, rows * out, stages_of(l.inputs), false);
+    p.dx_parts = parts(l.dx, rows * in, stages_of(l.outputs), false);
+    p.dw_parts = parts(l.dweight, (long long)in * out, stages_of(l.rows), l.rows > kLongest);
   }
   if (l.dtype == FA_F32) {
-    // parts that fill the multiprocessors twice, of 256 and more of k; none longer than
-    // 32768, so that the roundings of a long sum do not add up
+    // parts that fill the multiprocessors twice, of 256 and more of k; of sums longer than
+    // 32768, also parts whose last wave is fuller, in 77 MB at most (65280 rows, 2560 x 2048:
+    // dW 18.0 ms in one part, 14.1 in three)
     const auto parts = [&](bool wanted, long long m, long long n, long long k) {
       const long long tiles = ((m + kLaneTile - 1) / kLaneTile) * ((n + kLaneTile - 1) / kLaneTile);
+      const long long room = 2ll * sm_count(device);
       if (!wanted) return 1;
-      const int c = (int)std::max((k + kLongest - 1) / kLongest,
-                                  std::min((k + 255) / 256, 2ll * sm_count(device) / tiles));
+      int c = (int)std::max(1ll, std::min((k + 255) / 256, room / tiles));
+      const auto waves = [&](int q) { return (double)((tiles * q + room - 1) / room) / q; };
+      if (k > kLongest && tiles > room)
+        for (int q = 2; tiles * q <= 4 * room; ++q)
+          if (waves(q) < waves(c)) c = q;
       if (c > 1) part = std::max(part, (size_t)(sizeof(float) * c * m * n));
       return c;
     };
@@ -1239,9 +1267,11 @@ static int wgrad_run(const fa_linear8& l, const Operand& dy, char* part, const L
   a.part = reinterpret_cast<float*>(part);
   a.err = wait_error_word();
   if (!a.err) return FA_E_INTERNAL;  // a wait that gave up could not be reported
-  FAB_TRY(cudaFuncSetAttribute(wgrad_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmem));
+  const auto kernel = (a.kb + a.parts - 1) / a.parts > kChunk ? wgrad_kernel<T, true>
+                                                              : wgrad_kernel<T, false>;
+  FAB_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWgSmem));
   const int items = a.tiles_m * a.tiles_n * a.parts;
-  wgrad_kernel<T><<<2 * std::min(items, plan.pairs), kWgThreads, kWgSmem, st>>>(a);
+  kernel<<<2 * std::min(items, plan.pairs), kWgThreads, kWgSmem, st>>>(a);
   FAB_LAUNCH_CHECK();
   if (a.parts > 1) {
     join_parts_kernel<T><<<(unsigned)(a.tiles_m * a.tiles_n * 32), 128, 0, st>>>(a);
@@ -1299,7 +1329,8 @@ static int lanes_run(LaneArgs a, int parts, float* out, float* part, int device,
   a.d = a.parts > 1 ? part : out;
   const dim3 grid((unsigned)((a.m + kLaneTile - 1) / kLaneTile),
                   (unsigned)((a.n + kLaneTile - 1) / kLaneTile), (unsigned)a.parts);
-  lanes_kernel<A, B><<<grid, 256, 0, st>>>(a);
+  if (a.per_part > kLongest) lanes_kernel<A, B, true><<<grid, 256, 0, st>>>(a);
+  else lanes_kernel<A, B, false><<<grid, 256, 0, st>>>(a);
   FAB_LAUNCH_CHECK();
   if (a.parts > 1) {
     const long long size = (long long)a.m * a.n;

@@ -218,3 +218,25 @@ def test_arrivals_in_the_other_block_are_of_the_cluster():
     waits = re.findall(r"stage_wait(<\w+>)?\((&full\[s\], \(n / S\)|&tm_empty)", product)
     assert len(waits) == 5 and all(kind == "<true>" for kind, _ in waits), waits
     assert product.count("wait.parity.acquire.cluster.shared::cta") == 2
+
+
+@pytest.mark.parametrize("dtype,most", [(1, 160 << 20), (2, 160 << 20), (3, 80 << 20)])
+def test_the_products_workspace_does_not_grow_with_their_sums(dtype, most):
+    """Sizes at which a float32 copy of the result for every 32768 terms takes gigabytes."""
+    L = _cabi.load()
+    size = ctypes.c_size_t(0)
+
+    def workspace(rows, inputs, outputs, **which):
+        p = _cabi.fa_linear8(dtype=dtype, inputs=inputs, outputs=outputs, rows=rows,
+                             x_stride=inputs, dy_stride=outputs, weight_stride=inputs,
+                             **{k: 1 << 20 for k in which})
+        assert L.fa_b200_linear8_workspace_bytes(ctypes.byref(p), 0, ctypes.byref(size)) == 0
+        return size.value
+
+    grad = dict(dy=1, codes=1, ranges=1, dweight=1)
+    for rows, inputs, outputs in ((131072, 4096, 128256), (1100000, 4096, 16384),
+                                  (1 << 27, 4096, 4096), (1 << 27, 16, 24), (70000, 1024, 4096),
+                                  (1 << 22, 512, 2048)):
+        assert workspace(rows, inputs, outputs, **grad) <= most
+    assert workspace(60000, 40000, 4096, x=1, weight=1, y=1) <= most
+    assert workspace(60000, 4096, 40000, dy=1, weight=1, dx=1) <= most

@@ -1198,3 +1198,59 @@ def test_gelu_far_out_relative_to_its_value(dtype, approximate):
                                 (dx, first + second, first + second.abs(), 1 + d.abs() * (1 + up))):
         tol = rel * size + (0 if got is not dx else extra) + low * by
         within(got, want, U[dtype] * want.abs() + (1 + 2 * U[dtype]) * tol, dtype)
+
+
+@pytest.mark.parametrize("dtype,rows,inputs,outputs", [
+    (torch.bfloat16, 131_073, 2304, 2304),     # more tiles than pairs of blocks, five chunks
+    (torch.float16, 100_000, 2304, 2304),
+    (torch.bfloat16, 300_001, 520, 260),       # fewer, cut into parts of a few chunks each
+    (torch.bfloat16, 1_000_003, 1024, 1024),
+    (torch.float32, 70_001, 2304, 2304),
+    (torch.float32, 150_001, 520, 260),
+])
+def test_weight_gradients_of_many_rows_take_little_memory(dtype, rows, inputs, outputs):
+    """Sums of many chunks, in a workspace that does not depend on how many."""
+    # each row is one of 64, so that what the sums come to is known in float64 at once
+    bx, bg = (rand(64, n, seed=190 + i, dtype=dtype) for i, n in enumerate((inputs, outputs)))
+    at = torch.arange(rows, device="cuda") % 64
+    at[: rows // 3] = at[: rows // 3].flip(0)
+    x, g = bx[at], bg[(at * 7 + 3) % 64]
+    w = rand(outputs, inputs, seed=192, dtype=dtype).requires_grad_(True)
+    y = fa.linear8(x, w)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    dw, = torch.autograd.grad(y, w, g)
+    scratch = torch.cuda.max_memory_allocated() - before - dw.numel() * dw.element_size()
+    # eight slabs a pair of blocks, and a copy of rows that are not whole 16 bytes
+    copy = rows * 264 * 2 if outputs == 260 and dtype != torch.float32 else 0
+    assert scratch <= 8 * 74 * 2 ** 18 + copy + (1 << 20), scratch
+    many = torch.bincount(at, minlength=64).double()[:, None]
+    kept = fa.unpack8(fa.pack8(bx)).double()
+    bg = bg[(torch.arange(64, device="cuda") * 7 + 3) % 64].double()
+    want, size = bg.T @ (kept * many), bg.T.abs() @ (kept.abs() * many)
+    # The rows repeat, so roundings repeat too and add up: of a sum of 32768 terms every
+    # addition (16 terms each on the tensor cores, which truncate: a whole step) may be off by
+    # E (2 E) of what the sum then is, at most `size`; then a rounding a chunk or a part.
+    steps = 32768 if dtype == torch.float32 else 2 * 2048
+    tol = U[dtype] * want.abs() + (steps + 32 + rows / 32768) * E * size
+    past = want.abs() > torch.finfo(dtype).max * (1 - 2 * U[dtype])   # rounded to infinity
+    within(dw[~past], want[~past], ((1 + 2 * U[dtype]) * tol)[~past], dtype)
+    assert bool((dw[past].sign() == want[past].sign()).all())
+    assert torch.equal(dw, torch.autograd.grad(fa.linear8(x, w), w, g)[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_products_of_many_tiles_over_more_inputs_than_a_chunk(dtype):
+    rows, inputs, outputs = 5200, 40_000, 1100
+    x, w = rand(rows, inputs, seed=195, dtype=dtype), rand(outputs, inputs, seed=196, dtype=dtype)
+    b = rand(outputs, seed=197, dtype=dtype)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    y = fa.linear8(x, w, b)
+    scratch = torch.cuda.max_memory_allocated() - before - y.numel() * y.element_size()
+    # a slab a pair of blocks; float32: three parts of the result
+    most = 74 * 2 ** 18 if dtype != torch.float32 else 12 * rows * outputs
+    assert scratch <= most + (1 << 20), scratch
+    check_product(y[::13], x[::13], w, b, dtype)
