@@ -263,6 +263,20 @@ def _check_affine(name: str, w: Optional[torch.Tensor], x: torch.Tensor) -> None
         raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(w.shape)}")
 
 
+def _autocast_norm(x, residual, weight, bias):
+    """Under autocast the norm's operands come in two types: products give its own, what
+    they are added to and the weights may be in another.  Such operands meet in float32."""
+    def ours(*tensors):
+        return all(t is None or torch.is_tensor(t) and t.dtype in _DTYPES for t in tensors)
+
+    if ours(x, residual) and residual is not None and x.dtype != residual.dtype:
+        x, residual = x.float(), residual.float()
+    types = {t.dtype for t in (weight, bias) if torch.is_tensor(t)}
+    if ours(x, weight, bias) and not types <= {x.dtype} and types != {torch.float32}:
+        weight, bias = (None if t is None else t.float() for t in (weight, bias))
+    return x, residual, weight, bias
+
+
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None, *,
                residual: Optional[torch.Tensor] = None, eps: float = 1e-5, keep8: bool = False
@@ -277,10 +291,14 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     ``x`` (..., N): float16, bfloat16 or float32, any strides; N at most 2^24.
     ``weight`` and ``bias``, either or both: (N,), one dtype, ``x``'s or float32.
     Results are contiguous.  Mean, variance and the weights' gradients are
-    summed in float32, in an order that does not change from run to run.
+    summed in float32, in an order that does not change from run to run.  Under
+    autocast ``x`` and ``residual`` of two dtypes are taken, and returned, as float32,
+    and so are weights that do not fit.
 
     ``keep8``: keep ``x`` (or ``s``) for the backward pass as :func:`pack8` holds
     it, with the exact mean and deviation, instead of itself."""
+    if torch.is_autocast_enabled("cuda"):
+        x, residual, weight, bias = _autocast_norm(x, residual, weight, bias)
     _check_values("x", x, _MAX_WIDTH)
     if residual is not None and not torch.is_tensor(residual):
         raise TypeError(f"residual must be a tensor or None, got {type(residual).__name__}")

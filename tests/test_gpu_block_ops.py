@@ -1254,3 +1254,51 @@ def test_products_of_many_tiles_over_more_inputs_than_a_chunk(dtype):
     most = 74 * 2 ** 18 if dtype != torch.float32 else 12 * rows * outputs
     assert scratch <= most + (1 << 20), scratch
     check_product(y[::13], x[::13], w, b, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_block_under_autocast(dtype):
+    """A float32 residual stream and weights around products in 16 bits."""
+    x, gy = rand(300, 96, seed=200), rand(300, 96, seed=201)
+    p = block_params(96, torch.float32, seed=202)
+    leaves = [t.clone().requires_grad_(True) for t in (x, *p)]
+    with torch.autocast("cuda", dtype=dtype):
+        y, s = block(leaves[0], leaves[1:])
+    assert y.dtype == s.dtype == torch.float32
+    got = torch.autograd.grad((y, s), leaves, (gy, gy))
+    assert all(g.dtype == torch.float32 and g.shape == t.shape for g, t in zip(got, leaves))
+    # the same with every change of type written out
+    again = [t.clone().requires_grad_(True) for t in (x, *p)]
+    q = again[1:]
+    h = fa.layer_norm(again[0], q[0], q[1], keep8=True).to(dtype)
+    h = fa.gelu8(fa.linear8(h, q[2].to(dtype), q[3].to(dtype)))
+    h = fa.linear8(h, q[4].to(dtype), q[5].to(dtype)).float()
+    want = fa.layer_norm(h, q[6], q[7], residual=again[0], keep8=True)
+    assert torch.equal(y, want[0]) and torch.equal(s, want[1])
+    for a, b in zip(got, torch.autograd.grad(want, again, (gy, gy))):
+        assert torch.equal(a, b)
+
+
+def test_norm_operands_of_two_types_meet_in_float32_under_autocast():
+    x, w, b = rand(9, 64, seed=203), 1 + rand(64, seed=204).abs(), rand(64, seed=205)
+    half, bf = torch.float16, torch.bfloat16
+    with torch.autocast("cuda", dtype=bf):
+        for a, r in ((bf, torch.float32), (torch.float32, half), (half, bf)):
+            y, s = fa.layer_norm(x.to(a), w, b, residual=x.to(r))
+            want, t = fa.layer_norm(x.to(a).float(), w, b, residual=x.to(r).float())
+            assert torch.equal(y, want) and torch.equal(s, t) and y.dtype == torch.float32
+        # what fits is left as it is
+        y, s = fa.layer_norm(x.to(bf), w, b, residual=x.to(bf))
+        assert y.dtype == s.dtype == bf
+        assert fa.layer_norm(x.to(bf), w.to(bf), b.to(bf)).dtype == bf
+        for wt, bt in ((half, half), (half, torch.float32), (bf, torch.float32), (half, None)):
+            bias = None if bt is None else b.to(bt)
+            y = fa.layer_norm(x.to(bf), w.to(wt), bias)
+            want = fa.layer_norm(x.to(bf), w.to(wt).float(), None if bias is None else bias.float())
+            assert torch.equal(y, want) and y.dtype == bf
+        with pytest.raises(ValueError, match="residual"):
+            fa.layer_norm(x, residual=x[:3].half())
+        with pytest.raises(TypeError, match="weight"):
+            fa.layer_norm(x, w.double())
+    with pytest.raises(ValueError, match="residual"):
+        fa.layer_norm(x, residual=x.half())
