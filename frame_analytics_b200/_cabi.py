@@ -237,6 +237,7 @@ PROTOTYPES = {
     "fa_b200_linear8_workspace_bytes": [_vp, _i, _vp],
     "fa_b200_linear8": [_vp, _vp, _sz, _i, _vp],
     "fa_b200_linear8_backward": [_vp, _vp, _sz, _i, _vp],
+    "fa_b200_linear8_wait_selftest": [ctypes.c_ulonglong, _i, _vp],
     "fa_b200_ssim_gmsd": [_pview, _pview, _vp, _i, _d, _d, _d, _d, _d, _d, _vp, _sz,
                           _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp],
 }

@@ -34,6 +34,7 @@ int linear8_ws_bytes(const fa_linear8* l, int device, size_t* out);
 int linear8_impl(const fa_linear8* l, void* ws, size_t bytes, int device, cudaStream_t st);
 int linear8_backward_impl(const fa_linear8* l, void* ws, size_t bytes, int device,
                           cudaStream_t st);
+int stage_wait_selftest(unsigned long long limit_ns, int device, cudaStream_t st);
 
 }  // namespace fab
 
@@ -179,6 +180,12 @@ FA_B200_API int fa_b200_linear8_backward(const fa_linear8* params, void* workspa
   FAB_PENDING();
   return linear8_backward_impl(params, workspace, workspace_bytes, device,
                                static_cast<cudaStream_t>(stream));
+}
+
+FA_B200_API int fa_b200_linear8_wait_selftest(unsigned long long limit_ns, int device,
+                                              void* stream) {
+  FAB_PENDING();
+  return stage_wait_selftest(limit_ns, device, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

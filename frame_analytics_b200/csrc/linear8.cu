@@ -260,7 +260,7 @@ __device__ __forceinline__ bool work_of(const Args& a, int item, Work* w) {
 // barrier holds up the others' (a poll of a phase that was complete took 260 cycles
 // when the waiting warps polled in a loop), so a poll may suspend its warp until the
 // phase completes, or up to 2 ms.  The error word, in host memory, is looked at once in
-// 16 such polls.
+// 16 such polls, and once in a millisecond.
 // PAIR: threads of the pair's other block arrive at the barrier, too, so that what is
 // acquired is the whole cluster's.
 template <bool PAIR>
@@ -296,7 +296,8 @@ __device__ __forceinline__ bool mbar_peek(unsigned long long* bar, unsigned pari
   return done != 0;
 }
 template <bool PAIR>
-static __device__ __noinline__ void stage_wait_slow(unsigned a, unsigned parity, unsigned* err) {
+static __device__ __noinline__ void stage_wait_slow(unsigned a, unsigned parity, unsigned* err,
+                                                    unsigned long long limit_ns) {
   const unsigned long long t0 = globaltimer_ns();
   unsigned long long next = 1000000ull;
   for (unsigned i = 1;; ++i) {
@@ -304,7 +305,7 @@ static __device__ __noinline__ void stage_wait_slow(unsigned a, unsigned parity,
     const unsigned long long t = globaltimer_ns() - t0;
     if ((i & 15u) != 0u || t < next) continue;
     next = t + 1000000ull;
-    if (t > kWaitLimitNs || (err && *reinterpret_cast<volatile unsigned*>(err) != 0u)) {
+    if (t > limit_ns || (err && *reinterpret_cast<volatile unsigned*>(err) != 0u)) {
       if (err) {
         *reinterpret_cast<volatile unsigned*>(err) = (unsigned)FA_E_TIMEOUT;
         __threadfence_system();
@@ -317,7 +318,7 @@ template <bool PAIR = false>
 __device__ __forceinline__ void stage_wait(unsigned long long* bar, unsigned parity,
                                            unsigned* err) {
   const unsigned a = smem_u32(bar);
-  if (!mbar_sleep<PAIR>(a, parity)) stage_wait_slow<PAIR>(a, parity, err);
+  if (!mbar_sleep<PAIR>(a, parity)) stage_wait_slow<PAIR>(a, parity, err, kWaitLimitNs);
 }
 
 // A warp has written its share of a stage into its own block's tensor memory, and the
@@ -785,6 +786,18 @@ __device__ __forceinline__ void put_result(const PlainArgs& a, int i, int j, con
   }
 }
 
+// A wait for a phase that nothing completes, with nothing in flight: the error word is all
+// that running out of time leaves.
+__global__ void stage_wait_selftest_kernel(unsigned* err, unsigned long long limit_ns) {
+  __shared__ __align__(8) unsigned long long bar;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    fence_async_smem();
+    stage_wait_slow<false>(smem_u32(&bar), 0u, err, limit_ns);
+    stage_wait_slow<true>(smem_u32(&bar), 0u, err, limit_ns);
+  }
+}
+
 template <typename T, bool TALL>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPlainThreads, 1)
     product_kernel(const __grid_constant__ PlainArgs a) {
@@ -1178,6 +1191,16 @@ static int linear_check(const fa_linear8* l) {
   if ((l->y && (!l->x || !l->weight)) || (l->dx && (!l->dy || !l->weight)) ||
       (l->dweight && (!l->dy || !l->codes)) || (l->dbias && !l->dy))
     return FA_E_ARG;
+  return FA_OK;
+}
+
+int stage_wait_selftest(unsigned long long limit_ns, int device, cudaStream_t st) {
+  if (limit_ns > 1000000000ull) return FA_E_ARG;
+  FAB_DEVICE_SCOPE(device);
+  unsigned* const w = wait_error_word();
+  if (!w) return FA_E_INTERNAL;
+  stage_wait_selftest_kernel<<<1, 32, 0, st>>>(w, limit_ns);
+  FAB_LAUNCH_CHECK();
   return FA_OK;
 }
 

@@ -723,6 +723,10 @@ FA_B200_API int fa_b200_linear8(const fa_linear8* params, void* workspace, size_
                                 int device, void* stream);
 FA_B200_API int fa_b200_linear8_backward(const fa_linear8* params, void* workspace,
                                          size_t workspace_bytes, int device, void* stream);
+/* fa_b200_wait_selftest for the waits of these products: two waits of `limit_ns` (at
+ * most 1 s, else FA_E_ARG) one after the other, of which the second gives up soon. */
+FA_B200_API int fa_b200_linear8_wait_selftest(unsigned long long limit_ns, int device,
+                                              void* stream);
 
 /* No counterpart in the reference: test hook of the bounded device-side
  * waits.  Launches one thread that waits `limit_ns` (at most 1 s) for an

@@ -240,3 +240,7 @@ def test_the_products_workspace_does_not_grow_with_their_sums(dtype, most):
         assert workspace(rows, inputs, outputs, **grad) <= most
     assert workspace(60000, 40000, 4096, x=1, weight=1, y=1) <= most
     assert workspace(60000, 4096, 40000, dy=1, weight=1, dx=1) <= most
+
+
+def test_the_wait_hook_is_bounded():
+    assert _cabi.load().fa_b200_linear8_wait_selftest(1_000_000_001, 0, None) == 5

@@ -1302,3 +1302,24 @@ def test_norm_operands_of_two_types_meet_in_float32_under_autocast():
             fa.layer_norm(x, w.double())
     with pytest.raises(ValueError, match="residual"):
         fa.layer_norm(x, residual=x.half())
+
+
+def test_a_wait_that_gives_up_is_reported_by_the_next_call():
+    """A product's own waits, which sleep: a phase that nothing completes, with nothing in
+    flight, for 50 ms.  A second wait behind it gives up without its own 50 ms."""
+    from frame_analytics_b200 import _cabi
+    L = _cabi.load()
+    x, w, b, _ = linear_case((300, 200, 264, True), torch.bfloat16, seed=210)
+    want = fa.linear8(x, w, b)
+    t = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    stream = torch.cuda.current_stream().cuda_stream
+    t[0].record()
+    assert L.fa_b200_linear8_wait_selftest(50_000_000, 0, stream) == 0
+    t[1].record()
+    torch.cuda.synchronize()
+    # the clock is looked at behind every sixteenth poll, of 2 ms at most, and so is the
+    # word that says that a wait has given up: 50 and twice 16 x 2, and not twice 50 and that
+    assert 50 <= t[0].elapsed_time(t[1]) < 50 + 2 * 32 + 10
+    with pytest.raises(_cabi.KernelError, match="timed out"):
+        fa.linear8(x, w, b)
+    assert torch.equal(fa.linear8(x, w, b), want)
