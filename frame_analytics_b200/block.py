@@ -76,6 +76,8 @@ def _reject_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """As a matrix of rows with unit stride; a copy where that takes one."""
     width = t.shape[-1]
+    if t.is_neg():  # an imaginary part, or its gradient: the sign is not in memory
+        t = t.resolve_neg()
     if t.dim() == 2 and (t.stride(1) == 1 or width == 1):
         return t
     if t.stride(-1) != 1 and width > 1:
@@ -315,9 +317,9 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     _reject_tangents("layer_norm", x, residual, weight, bias)
     _on_one_device(x, residual, weight, bias)
     if weight is not None:
-        weight = weight.contiguous()
+        weight = weight.resolve_neg().contiguous()
     if bias is not None:
-        bias = bias.contiguous()
+        bias = bias.resolve_neg().contiguous()
     if x.numel() == 0:
         # connected to the graph, so that a backward gives zero gradients
         y = (x if residual is None else x + residual) * 1.0
@@ -427,7 +429,7 @@ def _linear_forward(x, weight, bias, kept, ranges: int) -> torch.Tensor:
     if weight.stride(1) != 1 and inputs > 1:
         weight = weight.contiguous()
     if bias is not None:
-        bias = bias.contiguous()
+        bias = bias.resolve_neg().contiguous()
     y = x.new_empty((*x.shape[:-1], outputs))
     _linear_call(fn, r, rows, inputs, outputs, r, None, weight, bias, at,
                  at + ranges if at else 0, y, None, None, None)
@@ -500,6 +502,7 @@ def linear8(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] 
                          f"{tuple(bias.shape)}")
     _reject_tangents("linear8", x, weight, bias)
     _on_one_device(x, weight, bias)
+    weight = weight.resolve_neg()
     if x.numel() == 0:
         return F.linear(x, weight, bias)
     if torch.is_grad_enabled() and (

@@ -1323,3 +1323,36 @@ def test_a_wait_that_gives_up_is_reported_by_the_next_call():
     with pytest.raises(_cabi.KernelError, match="timed out"):
         fa.linear8(x, w, b)
     assert torch.equal(fa.linear8(x, w, b), want)
+
+
+@pytest.mark.parametrize("shape", [(9, 1), (2, 5, 1), (1,), (9, 66)])
+def test_imaginary_parts_keep_their_sign(shape):
+    """The imaginary part of a conjugate, and the gradient of one, are views whose sign is
+    not in memory; a column of them needs no copy for its strides."""
+    def imag(seed, *shape):
+        c = torch.complex(rand(*shape, seed=seed), rand(*shape, seed=seed + 1))
+        view = c.conj().imag
+        assert view.is_neg()
+        return view, -c.imag.contiguous()
+
+    n = shape[-1]
+    pairs = [imag(220 + 2 * i, *s) for i, s in enumerate((shape, shape, (n,), (n,), (3, n), (3,)))]
+    p, q = fa.pack8(pairs[0][0]), fa.pack8(pairs[0][1])
+    assert torch.equal(p.codes, q.codes) and torch.equal(p.ranges, q.ranges)
+    results = []
+    for k in range(2):
+        x, r, w, b, m, c = (pair[k].detach().requires_grad_(True) for pair in pairs)
+        gy = pairs[1][k]
+        y, s = fa.layer_norm(x, w, b, residual=r, keep8=True)
+        a = fa.gelu8(x)
+        z = fa.linear8(x, m, c)
+        column = fa.linear8(x, m[:1], c[:1])
+        results.append([t.detach() for t in (y, s, a, z, column)])
+        results[-1] += torch.autograd.grad((y, s), (x, r, w, b), (gy, gy))
+        results[-1] += torch.autograd.grad(a, x, gy)
+        results[-1] += torch.autograd.grad(z, (x, m, c), torch.ones_like(z))
+        results[-1] += torch.autograd.grad(column, (x, m, c), gy[..., :1])
+        with torch.no_grad():
+            results[-1] += [fa.layer_norm(x, w, b), fa.linear8(x, m, c)]
+    for got, want in zip(*results):
+        assert torch.equal(got, want)
