@@ -1356,3 +1356,50 @@ def test_imaginary_parts_keep_their_sign(shape):
             results[-1] += [fa.layer_norm(x, w, b), fa.linear8(x, m, c)]
     for got, want in zip(*results):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("width", [2112, 2111])
+def test_norm_and_gelu_past_2_31_values(width):
+    """Rows stand alone, so those at either end are the bits of a call on them."""
+    rows = (1 << 31) // width + 77
+    x = torch.full((rows, width), 0.5, dtype=torch.bfloat16, device="cuda")
+    g = torch.full((rows, width), 0.25, dtype=torch.bfloat16, device="cuda")
+    ends = [slice(0, 40), slice(rows - 40, rows)]
+    for i, part in enumerate(ends):
+        x[part], g[part] = (rand(40, width, seed=230 + 2 * i + k).bfloat16() for k in range(2))
+    w = (1 + 0.1 * rand(width, seed=235)).bfloat16()
+    for call in (lambda t: fa.layer_norm(t, w, residual=t, keep8=True)[0],
+                 lambda t: fa.layer_norm(t, w), fa.gelu8):
+        leaf = x.detach().requires_grad_(True)
+        y = call(leaf)
+        dx, = torch.autograd.grad(y, leaf, g)
+        for part in ends:
+            small = x[part].clone().requires_grad_(True)
+            want = call(small)
+            assert torch.equal(y[part], want)
+            assert torch.equal(dx[part], torch.autograd.grad(want, small, g[part])[0])
+        del y, dx
+
+
+@pytest.mark.parametrize("dtype,inputs", [(torch.bfloat16, 2112), (torch.bfloat16, 2111),
+                                          (torch.float32, 2111)])
+def test_products_past_2_31_values(dtype, inputs):
+    """Inputs and results of more than 2^31 values, in rows that are all nothing but at
+    their ends: the weight's gradient is that of the ends."""
+    rows, outputs = (1 << 31) // 2111 + 77, 2112
+    x = torch.zeros(rows, inputs, dtype=dtype, device="cuda")
+    g = torch.zeros(rows, outputs, dtype=dtype, device="cuda")
+    ends = [slice(0, 40), slice(rows - 40, rows)]
+    for i, part in enumerate(ends):
+        x[part], g[part] = (rand(40, n, seed=240 + 2 * i + k).to(dtype)
+                            for k, n in enumerate((inputs, outputs)))
+    w = rand(outputs, inputs, seed=245, scale=inputs ** -0.5).to(dtype).requires_grad_(True)
+    leaf = x.detach().requires_grad_(True)
+    y = fa.linear8(leaf, w)
+    dx, dw = torch.autograd.grad(y, (leaf, w), g)
+    for part in ends:
+        check_product(y[part].detach(), x[part], w.detach(), None, dtype)
+        check_product(dx[part], g[part], w.detach().mT, None, dtype)
+    assert not bool(y[40:80].any()) and not bool(dx[rows - 80:rows - 40].any())
+    both = [torch.cat([t[part] for part in ends]) for t in (x, g)]
+    check_weight_grad(dw, None, *both, dtype)
