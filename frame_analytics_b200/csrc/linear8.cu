@@ -17,8 +17,8 @@
 // in order.  y and dx: the same tiles, both operands by TMA.  float32: on the ordinary
 // lanes.
 //
-// Measured on one B200 at 16320 rows, 1024 inputs, 4096 outputs, bfloat16: y 113 us, dx
-// 98 us, dW 114 us (1.2 to 1.4 PFLOP/s; torch's products 99, 94 and 90 us), packing 11
+// Measured on one B200 at 16320 rows, 1024 inputs, 4096 outputs, bfloat16: y 109 us, dx
+// 98 us, dW 115 us (1.2 to 1.4 PFLOP/s; torch's products 99, 94 and 90 us), packing 11
 // us, db 26 us.  y and dx are bound by operand bytes out of the second-level cache (11.3
 // TB/s; the tensor pipe 72 % active at 8192 x 4096 x 4096, 189 us), dW by the products
 // themselves (685 cycles for 256 x 256 x 64) and by 64 tiles for 74 pairs of blocks.
@@ -46,7 +46,8 @@ int pack8_impl(const void* x, long long x_row, void* codes, void* ranges, int dt
 // products run.  Few tiles: k is cut into parts, whose sums are joined in order.  After
 // every 32768 terms the sum goes to its place in the result, so that a long one's roundings
 // do not add up.
-// Bound by the products: 16320 rows, 1024 x 1024, dW 0.80 ms, 43 TFLOP/s.
+// Bound by the products: 16320 rows, 1024 x 1024, y 0.68, dx 0.63, dW 0.84 ms, 41 to 54
+// TFLOP/s.
 constexpr int kLaneTile = 128, kLaneDepth = 16;
 constexpr long long kLongest = 32768;  // terms of a sum
 
@@ -1216,8 +1217,12 @@ static int workspace_check(const LinearPlan& p, const void* ws, size_t bytes) {
 
 // D (rows x cols) = A (rows x depth) B: B with depth along its rows, or as its rows.
 // Whether the taller tiles take less time: waves of tiles, at 0.40 us a stage and 2 us a
-// tile's end against 0.69 and 6.  Measured, bfloat16: 18944 rows, 4096 -> 1024, 2 waves
-// of tall tiles 105 us, 4 of low ones 115; 18944 rows, 512 -> 2048, 4 waves 54 us, 8 49.
+// tile's end against 0.69 and 6.  Low tiles have two accumulators, so between waves the
+// next tile's products run beside an end (18944 rows, bfloat16, sums of 512 to 8192 terms:
+// 0.40 us a stage in 2, 4 and 8 waves, and 14, 16 and 17 us besides, the launch among
+// them); a single wave, which parts_of is about, shows all of it.  Measured: 18944 rows,
+// 4096 -> 1024, 2 waves of tall tiles 102 us, 4 of low ones 117; 4096 -> 512, 1 and 2
+// waves, 59 and 66; 512 -> 2048, 4 waves of tall ones 54, 8 of low ones 49.
 static bool tall_pays(long long rows, int cols, int kb, int pairs) {
   if (kb > kChunk) return false;
   const long long wide = tiles_of(cols);

@@ -697,8 +697,10 @@ FA_B200_API int fa_b200_layer_norm_backward(const fa_norm* params, const void* d
  * Strides in elements between rows of unit stride; results are contiguous.  Sums are
  * float32.  At most 2^27 rows, 4194240 inputs and outputs.  Forward: x, and y (with
  * weight, and bias or null) or codes/ranges, or both.  Backward: dy, and any of dx
- * (with weight), dweight (with codes/ranges) and dbias; the others null.  Workspace (size from the query, for the same structure): 256-byte
- * aligned, needs no zeroing; null where the size is 0. */
+ * (with weight), dweight (with codes/ranges) and dbias; the others null.  Workspace
+ * (size from the query, for the same structure): 256-byte aligned, needs no zeroing;
+ * null where the size is 0; at most 155 MB and copies of the 16-bit operands whose rows
+ * are not whole aligned 16 bytes. */
 typedef struct fa_linear8 {
   int32_t dtype, inputs, outputs, pad_;
   int64_t rows;
