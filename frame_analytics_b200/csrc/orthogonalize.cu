@@ -267,11 +267,12 @@ __device__ __forceinline__ unsigned ld_acquire(const unsigned* p) {
 // word is across the bus and is only written.  No wait spans more than the few
 // tiles that it is for, the longest about 0.1 s (65536 blocks of K): a launch may
 // last longer than the limit.
+template <bool PAIR>
 __device__ __noinline__ bool wait_slow(unsigned bar, unsigned parity, const unsigned* flag,
                                        unsigned want, const NsArgs& a) {
   const unsigned long long t0 = globaltimer_ns();
   for (unsigned i = 1;; ++i) {
-    if (flag ? ld_acquire(flag) >= want : mbar_try(bar, parity)) return true;
+    if (flag ? ld_acquire(flag) >= want : mbar_try_pair<PAIR>(bar, parity)) return true;
     if ((i & 255u) == 0u) {
       const bool failed = *reinterpret_cast<volatile unsigned*>(a.failed) != 0u;
       if (failed || globaltimer_ns() - t0 > a.limit_ns) {
@@ -285,17 +286,19 @@ __device__ __noinline__ bool wait_slow(unsigned bar, unsigned parity, const unsi
     }
   }
 }
+// PAIR: threads of the pair's other block arrive there, too.
+template <bool PAIR = false>
 __device__ __forceinline__ bool wait_bar(unsigned long long* bar, unsigned parity,
                                          const NsArgs& a) {
   const unsigned b = smem_u32(bar);
 #pragma unroll 1
   for (int i = 0; i < 8; ++i)
-    if (mbar_try(b, parity)) return true;
-  return wait_slow(b, parity, nullptr, 0, a);
+    if (mbar_try_pair<PAIR>(b, parity)) return true;
+  return wait_slow<PAIR>(b, parity, nullptr, 0, a);
 }
 __device__ __forceinline__ bool wait_flag(const unsigned* flag, unsigned want, const NsArgs& a) {
   if (ld_acquire(flag) >= want) return true;
-  return wait_slow(0, 0, flag, want, a);
+  return wait_slow<false>(0, 0, flag, want, a);
 }
 
 // Where a tile is.  Tiles are numbered phase by phase (A, A^2, B X of step 0,
@@ -839,11 +842,11 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
                                ((unsigned)(t.bn / 8) << 17) | ((unsigned)((PAIR ? 2 : 1) * BM / 16) << 24);
         const int chunk = SPLIT ? kChunk : t.kb1 - t.kb0;
         const unsigned ps = (p_mn ? 2048u : 32u) >> 4, qs = (q_mn ? 2048u : 32u) >> 4;
-        if (SPLIT && tile >= 2 && !wait_bar(&sm_empty[tile & 1], (tile / 2 - 1) & 1, a)) break;
+        if (SPLIT && tile >= 2 && !wait_bar<PAIR>(&sm_empty[tile & 1], (tile / 2 - 1) & 1, a)) break;
         const unsigned dsmall = tmem + 256 + (tile & 1) * 128;
         for (int kb0 = t.kb0; ok && kb0 < t.kb1; kb0 += chunk, ++sums) {
           const int buf = sums & 1;
-          if (sums >= 2 && !wait_bar(&tm_empty[buf], (sums / 2 - 1) & 1, a)) {
+          if (sums >= 2 && !wait_bar<PAIR>(&tm_empty[buf], (sums / 2 - 1) & 1, a)) {
             ok = false;
             break;
           }
@@ -852,7 +855,7 @@ __global__ void __launch_bounds__(kThreads, 1) ns_product_kernel(const __grid_co
           const int kb1 = min(t.kb1, kb0 + chunk);
           for (int kb = kb0; kb < kb1; ++kb, ++n) {
             const int s = n % S;
-            if (!wait_bar(&full[s], (n / S) & 1, a)) {
+            if (!wait_bar<PAIR>(&full[s], (n / S) & 1, a)) {
               ok = false;
               break;
             }

@@ -82,6 +82,20 @@ __device__ __forceinline__ void arrive_leader(unsigned long long* bar) {
   else
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];\n" ::"r"(smem_u32(bar)) : "memory");
 }
+// mbar_try for a barrier at which threads of the pair's other block arrive, too: what is
+// acquired is then the whole cluster's.
+template <bool PAIR>
+__device__ __forceinline__ bool mbar_try_pair(unsigned a, unsigned parity) {
+  if constexpr (!PAIR) return mbar_try(a, parity);
+  unsigned done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(done)
+      : "r"(a), "r"(parity)
+      : "memory");
+  return done != 0;
+}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::
                    : "memory");

@@ -222,3 +222,15 @@ def test_the_example_starts_from_anywhere(tmp_path):
                          cwd=tmp_path, env=env, capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr
     assert "--steps" in run.stdout
+
+
+def test_waits_for_the_pairs_other_block_are_of_the_cluster():
+    """Barriers at which threads of the other block arrive, or its copies: the sums that
+    are read, and the stages."""
+    import re
+    from pathlib import Path
+    csrc = Path(fa.__file__).parent / "csrc"
+    waits = re.findall(r"wait_bar(<\w+>)?\((&full\[s\]|&tm_empty|&sm_empty)",
+                       (csrc / "orthogonalize.cu").read_text())
+    assert len(waits) == 3 and all(kind == "<PAIR>" for kind, _ in waits), waits
+    assert "try_wait.parity.acquire.cluster.shared::cta" in (csrc / "tensor.cuh").read_text()
