@@ -7,8 +7,8 @@ and product until its gradient comes back; these inputs, not the weights, fill
 the memory.  ``pack8`` holds them in 68 bytes (float32: 72) for every 64 values of
 a row, also where the last 64 are not all there: long rows take 1.06 (1.13) bytes a
 value, and only rows of up to 34, or 65 to 68, 16-bit (18 float32) values no less
-than they do themselves.  ``layer_norm``, ``gelu8`` and ``linear8`` read that form in their backward
-passes without unpacking it first.
+than they do themselves.  ``layer_norm``, ``gelu8`` and ``linear8`` read that form in
+their backward passes without unpacking it first.
 """
 
 from __future__ import annotations

@@ -7,10 +7,9 @@
 // Each kernel reads its operands once and writes its outputs once; 8 lanes hold
 // a group of 64, so a group's range costs three shuffles.  Measured on one B200, 65280 x
 // 4096 bfloat16: packing 128 us and unpacking 130 us (0.98 and 0.96 of the copy rate),
-// gelu with packing 229 us and its gradient 238 us (0.90 and 0.87), the tanh form 213 and 211 us
-// (0.97).
-// float32 gelu is bound by normcdff and expf (0.5 of the copy rate), rows that are not
-// whole vectors by their loads and stores of single values (0.35 to 0.55).
+// gelu with packing 229 us and its gradient 238 us (0.90 and 0.87), the tanh form 213 and
+// 211 us (0.97).  float32 gelu is bound by normcdff and expf (0.5 of the copy rate), rows
+// that are not whole vectors by their loads and stores of single values (0.35 to 0.55).
 #include <algorithm>
 
 #include "keep8.cuh"
