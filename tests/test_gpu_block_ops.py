@@ -1403,3 +1403,22 @@ def test_products_past_2_31_values(dtype, inputs):
     assert not bool(y[40:80].any()) and not bool(dx[rows - 80:rows - 40].any())
     both = [torch.cat([t[part] for part in ends]) for t in (x, g)]
     check_weight_grad(dw, None, *both, dtype)
+
+
+def test_float32_tanh_slopes_are_as_close_as_their_terms():
+    """f + x f (1 - f) 2 u' with f = 1 / (1 + e), e = exp(-2 u): e is off by 4 E of itself
+    (2 ulp) and the exponent's roundings, five of 2 u at most; f by two roundings and what
+    e's error moves it, f (1 - f) of that; the second term by as much twice and a dozen
+    roundings of its own.  A rounding of f itself, where f is near one and 1 - f is small,
+    is nothing to the second term."""
+    x = torch.linspace(-6, 13, 19 * 512 + 1, device="cuda")[:, None]
+    leaf = x.clone().requires_grad_(True)       # each value a group of its own: kept exactly
+    dx, = torch.autograd.grad(fa.gelu8(leaf, approximate="tanh"), leaf, torch.ones_like(x))
+    d = x.double()
+    c = (2 / math.pi) ** 0.5
+    two_u, up = 2 * c * (d + 0.044715 * d ** 3), 2 * c * (1 + 3 * 0.044715 * d * d)
+    f, rest = torch.sigmoid(two_u), torch.sigmoid(-two_u)
+    second = d * f * rest * up
+    of_e = (4 + 5 * two_u.abs()) * E
+    tol = 2 * E * f + f * rest * of_e + second.abs() * (2 * of_e + 12 * E)
+    within(dx, f + second, 1.01 * tol + E * (f + second).abs(), torch.float32)
